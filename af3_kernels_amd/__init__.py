@@ -14,6 +14,7 @@ GEMM is the right tool (the projection of the three-launch path where it is larg
 wider than 128 columns: hipBLASLt through torch); each function's docstring names its limits.
 """
 from . import _lib
+from .cross import cross_attention, relative_position_bias  # noqa: F401
 from .fused import GridSelfAttentionCpp, Linear, _attention_cpp, clear_weight_cache, gated_linear_unit_cpp, layernorm_pair_bias, self_attention_cpp  # noqa: F401
 from .ops import (  # noqa: F401
     convert,
@@ -34,4 +35,5 @@ __all__ = [
     "dot_product_attention_cpp", "dot_product_attention_fp8", "pad_and_align_tensor", "vnni_repack_tensor",
     "reset_debug_timers", "print_debug_timers", "print_debug_thread_imbalance", "convert", "quantize_fp8_e4m3",
     "selected_kernel", "set_exact_bias", "set_rows_kernel", "_attention_cpp", "self_attention_cpp", "GridSelfAttentionCpp", "layernorm_pair_bias", "gated_linear_unit_cpp", "Linear", "clear_weight_cache",
+    "cross_attention", "relative_position_bias",
 ]

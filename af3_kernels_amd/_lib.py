@@ -47,6 +47,40 @@ class GridAttentionParams(ctypes.Structure):
     ]
 
 
+class CrossAttentionParams(ctypes.Structure):
+    """Mirror of struct af3_cross_attention_params."""
+    _fields_ = [
+        ("q", vp), ("k", vp), ("v", vp), ("bias", vp), ("key_mask", vp), ("out", vp), ("stats", vp),
+        ("B", i64), ("H", i64), ("Hkv", i64), ("Lq", i64), ("Lk", i64), ("D", i64),
+        ("q_stride", i64 * 3), ("k_stride", i64 * 3), ("v_stride", i64 * 3), ("out_stride", i64 * 3),
+        ("bias_stride", i64 * 2), ("key_mask_stride_b", i64),
+        ("dtype", i32), ("softmax_scale", f32),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class CrossAttentionGrads(ctypes.Structure):
+    """Mirror of struct af3_cross_attention_grads."""
+    _fields_ = [
+        ("grad_out", vp), ("grad_out_stride", i64 * 3),
+        ("grad_q", vp), ("grad_k", vp), ("grad_v", vp), ("grad_bias", vp),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class PositionBiasParams(ctypes.Structure):
+    """Mirror of struct af3_position_bias_params."""
+    _fields_ = [
+        ("table", vp), ("out", vp), ("grad", vp), ("q_positions", vp), ("k_positions", vp), ("q_offset", i64),
+        ("table_stride", i64 * 2), ("grad_stride", i64 * 2),
+        ("buckets", i64), ("H", i64), ("Lq", i64), ("Lk", i64), ("max_distance", i64),
+        ("scheme", i32), ("bidirectional", i32), ("dtype", i32), ("reserved", i32),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+POSITION_SCHEMES = {"log": 0, "clip": 1}   # af3_position_scheme
+POSITION_BIAS_MAX_BUCKETS = 576            # AF3_POSITION_BIAS_MAX_BUCKETS
 QKV_SCRATCH_FLOATS = 768   # AF3_QKV_SCRATCH_FLOATS
 
 # name -> (restype, argtypes); every symbol include/af3_dpa.h declares
@@ -62,6 +96,13 @@ SYMBOLS = {
     "af3_gated_linear_unit": (ctypes.c_int, [vp, vp, vp, i64, i64, i64, i32, vp]),
     "af3_silu_mul": (ctypes.c_int, [vp, vp, i64, i64, i32, vp]),
     "af3_linear": (ctypes.c_int, [vp, vp, vp, i64, i64, i64, i32, vp]),
+    "af3_cross_attention_forward": (ctypes.c_int, [ctypes.POINTER(CrossAttentionParams), vp]),
+    "af3_cross_attention_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(CrossAttentionParams)]),
+    "af3_cross_attention_backward": (ctypes.c_int, [ctypes.POINTER(CrossAttentionParams), ctypes.POINTER(CrossAttentionGrads), vp]),
+    "af3_cross_attention_backward_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(CrossAttentionParams)]),
+    "af3_position_bias_forward": (ctypes.c_int, [ctypes.POINTER(PositionBiasParams), vp]),
+    "af3_position_bias_backward": (ctypes.c_int, [ctypes.POINTER(PositionBiasParams), vp]),
+    "af3_position_bias_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(PositionBiasParams)]),
     "af3_convert": (ctypes.c_int, [vp, i32, vp, i32, i64, vp]),
     "af3_amax": (ctypes.c_int, [vp, i32, i64, vp, vp]),
     "af3_quantize_fp8_e4m3": (ctypes.c_int, [vp, i32, vp, i64, i64, i64, i32, i64, i64, f32, vp, vp, vp, vp]),
@@ -90,7 +131,10 @@ def load():
                 "There is no CPU or PyTorch fallback for these ops.")
         lib = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in (SYMBOLS | INTERNAL_SYMBOLS).items():
-            fn = getattr(lib, name)
+            try:
+                fn = getattr(lib, name)
+            except AttributeError:
+                raise ImportError(f"{LIB_PATH} has no {name}, it was built from older sources: rebuild it with `python -m af3_kernels_amd.build`") from None
             fn.restype, fn.argtypes = res, args
         if lib.af3_abi_version() != ABI_VERSION:
             raise ImportError(f"{LIB_PATH} has ABI version {lib.af3_abi_version()}, this package expects {ABI_VERSION}: rebuild it")
@@ -122,7 +166,10 @@ def load_host():
     """The native host side where it is built already (its functions are then the module's own), else a stand-in that finds it later."""
     if not (os.path.exists(HOST_PATH) and os.path.exists(LIB_PATH)):
         return _Host()
-    load()
+    try:
+        load()
+    except ImportError:
+        return _Host()   # (a library of older sources: importing the package must still work, or it could not be rebuilt; calls say what is wrong)
     import torch  # noqa: F401 -- its libraries must be loaded first
     from . import _host
     return _host

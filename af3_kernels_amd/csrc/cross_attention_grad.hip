@@ -1,0 +1,606 @@
+// The gradients of cross_attention.hip's attention: from P = softmax(S), out = P.V and dO = the gradient of out,
+//     dV = P^T . dO,  dP = dO . V^T,  delta = rowsum(dO * out),  dS = P * (dP - delta),
+//     dQ = scale dS . K,  dK = scale dS^T . Q,  dbias = dS summed over the batch.
+// S and P are computed again from q, k and the two numbers per row that the forward pass left (maximum and 1 / sum: kept apart, since
+// a maximum of the lowest float plus the logarithm of a sum is that maximum again).  Three kernels, none with atomics: each element
+// of a result is summed by one workgroup, or by one per part of the long axis and a joining kernel, always in the same order.
+//   cross_dq_kernel    32 query rows per wavefront, keys in tiles (writes delta too)
+//   cross_dkv_kernel   32 keys per wavefront, query rows in tiles, over all query heads of the key head
+//   cross_dbias_kernel 64 query rows x 32 keys per wavefront, over the batch
+#include "cross_tiles.hpp"
+
+#include <math.h>
+
+namespace af3 {
+
+int validate_cross_attention(const af3_cross_attention_params* p);
+
+namespace cross {
+
+struct grad_args {
+	af3_cross_attention_params p;
+	af3_cross_attention_grads  g;
+	uint32_t tiles, splits;   // workgroups per (batch, key head), parts of the long axis
+	int64_t  part;            // dq: keys per part; dkv: tiles of query rows per part
+	float    factor;
+	int32_t  whole;
+	float*   delta;           // [B, H, Lq]
+	float*   partial;         // dq [splits][B H Lq][D]; dkv [splits][2][B Hkv Lk][D]
+};
+
+// the sum of the wavefronts' results of equal shape, wavefront w keeps the blocks of columns that are w modulo N; `mine`: N tables of 32 x (DP + 4)
+template <int DP, int N>
+__device__ __forceinline__ void add_up(float* tables, int w, int lane, f32x16 (&o)[DP / 32]) {
+	const int at = (lane & 31) * (DP + 4) + 16 * (lane >> 5);
+#pragma unroll
+	for(int db = 0; db < DP / 32; db++)
+#pragma unroll
+		for(int i = 0; i < 4; i++) *reinterpret_cast<f32x4*>(tables + w * 32 * (DP + 4) + at + 32 * db + 4 * i) = f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+	__syncthreads();
+#pragma unroll
+	for(int db = 0; db < DP / 32; db++) {
+		if(db % N != w) continue;
+		o[db] = f32x16{};
+#pragma unroll
+		for(int k = 0; k < N; k++)
+#pragma unroll
+			for(int i = 0; i < 4; i++) {
+				const f32x4 v = *reinterpret_cast<const f32x4*>(tables + k * 32 * (DP + 4) + at + 32 * db + 4 * i);
+#pragma unroll
+				for(int e = 0; e < 4; e++) o[db][4 * i + e] += v[e];
+			}
+	}
+}
+
+// ---- dQ ----
+template <typename T, int DP, int KW>
+struct dq_shape {
+	static constexpr int KT = KW == 4 ? 128 : 64, SUB = KT / (32 * KW), ROWS = 32 * (WAVES / KW);
+	static constexpr int TILE = KT * tile<T, DP>::STRIDE;
+	static constexpr int BUFFERS = 4 * TILE <= 81920 ? 2 : 1;
+	static constexpr int JOIN = KW > 1 ? WAVES * 32 * (DP + 4) * 4 : 0;
+	static constexpr int LDS = 2 * BUFFERS * TILE > JOIN ? 2 * BUFFERS * TILE : JOIN;
+};
+
+template <typename T, int DP, int KW, bool BIAS>
+__global__ void __launch_bounds__(THREADS) cross_dq_kernel(grad_args a) {
+	using S  = dq_shape<T, DP, KW>;
+	using TL = tile<T, DP>;
+	constexpr int E = kind<T>::E, KT = S::KT;
+	const af3_cross_attention_params& p = a.p;
+	extern __shared__ __align__(16) unsigned char smem[];
+	__shared__ live_keys<KT> live;
+
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+	const int kwave = wave % KW, rwave = wave / KW;
+	uint32_t  id = xcd_order(blockIdx.x, gridDim.x);
+	const uint32_t row_tile = id % a.tiles;
+	id /= a.tiles;
+	const uint32_t split = id % a.splits;
+	id /= a.splits;
+	const int64_t b = id / (uint32_t)p.Hkv, hk = id % (uint32_t)p.Hkv;
+	const int64_t G = p.H / p.Hkv, rows = G * p.Lq;
+	const int     D = (int)p.D;
+
+	const int64_t R  = (int64_t)row_tile * S::ROWS + 32 * rwave + (lane & 31);
+	const bool    ok = R < rows;
+	const int64_t g = ok ? R / p.Lq : 0, qi = ok ? R - g * p.Lq : 0, h = hk * G + g, row = (b * p.H + h) * p.Lq + qi;
+	u32x4 qf[TL::STEPS], gf[TL::STEPS];
+	load_operand<T, DP>(qf, static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1] + qi * p.q_stride[2], ok, D, lane);
+	load_operand<T, DP>(gf, static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1] + qi * a.g.grad_out_stride[2], ok, D, lane);
+	float delta = 0.f;
+	{
+		u32x4 of[TL::STEPS];
+		load_operand<T, DP>(of, static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2], ok, D, lane);
+#pragma unroll
+		for(int s = 0; s < TL::STEPS; s++)
+#pragma unroll
+			for(int e = 0; e < E; e++) delta = __builtin_fmaf(kind<T>::at(gf[s], e), kind<T>::at(of[s], e), delta);
+		delta += other_half(delta);
+	}
+	if(ok && half == 0 && kwave == 0 && split == 0) a.delta[row] = delta;
+	const float  m = ok ? p.stats[2 * row] : 0.f, inv = ok ? p.stats[2 * row + 1] : 0.f;
+	const T* const kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[1];
+	const T* const vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
+	const T* const bias = BIAS ? static_cast<const T*>(p.bias) + h * p.bias_stride[0] + qi * p.bias_stride[1] : nullptr;
+	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b : nullptr;
+
+	f32x16 dq[TL::BLOCKS];
+#pragma unroll
+	for(int db = 0; db < TL::BLOCKS; db++) dq[db] = f32x16{};
+
+	const int64_t last = (int64_t)(split + 1) * a.part < p.Lk ? (int64_t)(split + 1) * a.part : p.Lk;
+	passage<T, DP, KT> pk, pv;
+	int buffer = 0;
+	for(int64_t first = (int64_t)split * a.part; first < last; first += SEGMENT) {
+		const int64_t end = first + SEGMENT < last ? first + SEGMENT : last;
+		live.scan(mask, first, end);
+		int t = live.next(0);
+		if(t < 0) continue;
+		pk.load(kb, p.k_stride[2], first + (int64_t)t * KT, end, D, a.whole);
+		pv.load(vb, p.v_stride[2], first + (int64_t)t * KT, end, D, a.whole);
+		while(t >= 0) {
+			unsigned char* const ks = smem + buffer * 2 * S::TILE;
+			unsigned char* const vs = ks + S::TILE;
+			float bs[BIAS ? S::SUB : 1][16];
+			if constexpr(BIAS) {
+#pragma unroll
+				for(int s = 0; s < S::SUB; s++) load_row16(bs[s], bias, first + (int64_t)t * KT + 32 * (kwave * S::SUB + s) + 16 * half, p.Lk);
+			}
+			if constexpr(S::BUFFERS == 1) __syncthreads();
+			pk.store(ks, D, [&](int r) { return live.keeps(t * KT + r); });
+			pv.store(vs, D, [&](int r) { return live.keeps(t * KT + r); });
+			__syncthreads();
+			const int following = live.next(t + 1);
+			if(following >= 0) {
+				pk.load(kb, p.k_stride[2], first + (int64_t)following * KT, end, D, a.whole);
+				pv.load(vb, p.v_stride[2], first + (int64_t)following * KT, end, D, a.whole);
+			}
+#pragma unroll
+			for(int s = 0; s < S::SUB; s++) {
+				const int      block = kwave * S::SUB + s;
+				const uint32_t keep  = live.word(t * (KT / 32) + block);
+				if(keep == 0u) continue;
+				f32x16 acc{}, dp{};
+#pragma unroll
+				for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(ks, 32 * block, i, lane), qf[i], acc);
+#pragma unroll
+				for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(vs, 32 * block, i, lane), gf[i], dp);
+				float x[16];
+#pragma unroll
+				for(int r = 0; r < 16; r++) {
+					const float t0 = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, bs[s][r]) : acc[r];
+					x[r] = __builtin_amdgcn_exp2f((t0 - m) * a.factor) * inv * (dp[r] - delta);
+				}
+				if(keep != ~0u) {
+					const uint32_t mine = keep >> (16 * half);
+#pragma unroll
+					for(int r = 0; r < 16; r++) x[r] = (mine >> r) & 1u ? x[r] : 0.f;
+				}
+#pragma unroll
+				for(int j = 0; j < TL::JOINTS; j++) {
+					const u32x4 f = kind<T>::pack(x + E * j);
+#pragma unroll
+					for(int db = 0; db < TL::BLOCKS; db++) dq[db] = kind<T>::mma(TL::col_frag(ks, 32 * block, db, j, lane), f, dq[db]);
+				}
+			}
+			t = following;
+			if constexpr(S::BUFFERS == 2) buffer ^= 1;
+		}
+	}
+	if constexpr(KW > 1) {
+		__syncthreads();
+		add_up<DP, KW>(reinterpret_cast<float*>(smem) + rwave * KW * 32 * (DP + 4), kwave, lane, dq);
+	}
+	if(!ok) return;
+#pragma unroll
+	for(int db = 0; db < TL::BLOCKS; db++) {
+		if(db % KW != kwave) continue;
+		float v[16];
+#pragma unroll
+		for(int r = 0; r < 16; r++) v[r] = dq[db][r] * p.softmax_scale;
+		if(a.splits > 1) store_row16(a.partial + (split * (p.B * p.H * p.Lq) + row) * D, 32 * db + 16 * half, D, v);
+		else store_row16(static_cast<T*>(a.g.grad_q) + row * D, 32 * db + 16 * half, D, v);
+	}
+}
+
+// delta alone, for calls that want no gradient of q: one wavefront per row
+template <typename T>
+__global__ void __launch_bounds__(THREADS) cross_delta_kernel(grad_args a) {
+	const af3_cross_attention_params& p = a.p;
+	const int64_t row = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+	const int     lane = threadIdx.x & 63;
+	if(row >= p.B * p.H * p.Lq) return;
+	const int64_t qi = row % p.Lq, h = row / p.Lq % p.H, b = row / p.Lq / p.H;
+	const T* const g = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1] + qi * a.g.grad_out_stride[2];
+	const T* const o = static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2];
+	float sum = 0.f;
+	for(int64_t d = lane; d < p.D; d += 64) sum = __builtin_fmaf(kind<T>::value(g[d]), kind<T>::value(o[d]), sum);
+#pragma unroll
+	for(int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
+	if(lane == 0) a.delta[row] = sum;
+}
+
+// ---- dK, dV ----
+// RW: wavefronts that share 32 keys and each take 32 rows of a tile of query rows (1: every wavefront has its own keys and takes the whole tile)
+template <typename T, int DP, int RW>
+struct dkv_shape {
+	static constexpr int QT = RW == 4 ? 128 : sizeof(T) == 2 ? 64 : 32, SUB = QT / (32 * RW), KEYS = 32 * (WAVES / RW);
+	static constexpr int TILE = QT * tile<T, DP>::STRIDE, STATS = 3 * QT * 4, SET = 2 * TILE + STATS;
+	static constexpr int BUFFERS = 2 * SET <= 81920 ? 2 : 1;
+	static constexpr int JOIN = RW > 1 ? WAVES * 32 * (DP + 4) * 4 : 0;
+	static constexpr int LDS = BUFFERS * SET > JOIN ? BUFFERS * SET : JOIN;
+};
+
+template <typename T, int DP, int RW, bool BIAS>
+__global__ void __launch_bounds__(THREADS) cross_dkv_kernel(grad_args a) {
+	using S  = dkv_shape<T, DP, RW>;
+	using TL = tile<T, DP>;
+	constexpr int E = kind<T>::E, QT = S::QT;
+	const af3_cross_attention_params& p = a.p;
+	extern __shared__ __align__(16) unsigned char smem[];
+
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+	const int rwave = wave % RW, kwave = wave / RW;
+	uint32_t  id = xcd_order(blockIdx.x, gridDim.x);
+	const uint32_t key_tile = id % a.tiles;
+	id /= a.tiles;
+	const uint32_t split = id % a.splits;
+	id /= a.splits;
+	const int64_t b = id / (uint32_t)p.Hkv, hk = id % (uint32_t)p.Hkv;
+	const int64_t G = p.H / p.Hkv;
+	const int     D = (int)p.D;
+
+	const int64_t key = (int64_t)key_tile * S::KEYS + 32 * kwave + (lane & 31);
+	const bool    in = key < p.Lk;
+	const bool    dead = p.stats[2 * ((b * p.H + hk * G) * p.Lq)] == -INFINITY;   // no live key in the batch row: P is 1 / Lk for all keys, S none of its business
+	const bool    lives = in && (!p.key_mask || p.key_mask[b * p.key_mask_stride_b + key] != 0);
+	u32x4 kf[TL::STEPS], vf[TL::STEPS];
+	load_operand<T, DP>(kf, static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[1] + (in ? key : 0) * p.k_stride[2], in, D, lane);
+	load_operand<T, DP>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], in, D, lane);
+	const bool work = __any(lives || (dead && in));   // (of this wavefront)
+
+	f32x16 dk[TL::BLOCKS], dv[TL::BLOCKS];
+#pragma unroll
+	for(int db = 0; db < TL::BLOCKS; db++) dk[db] = f32x16{}, dv[db] = f32x16{};
+
+	const int64_t q_tiles = (p.Lq + QT - 1) / QT, n = G * q_tiles;
+	const int64_t last = (int64_t)(split + 1) * a.part < n ? (int64_t)(split + 1) * a.part : n;
+	passage<T, DP, QT> pq, pg;
+	float row_stat[3];
+	auto fetch = [&](int64_t it) {
+		const int64_t h = hk * G + it / q_tiles, q0 = it % q_tiles * QT;
+		pq.load(static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1], p.q_stride[2], q0, p.Lq, D, a.whole);
+		pg.load(static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1], a.g.grad_out_stride[2], q0, p.Lq, D, a.whole);
+		row_stat[0] = row_stat[1] = row_stat[2] = 0.f;
+		if((int)threadIdx.x < QT && q0 + threadIdx.x < p.Lq) {
+			const int64_t row = (b * p.H + h) * p.Lq + q0 + threadIdx.x;
+			row_stat[0] = p.stats[2 * row], row_stat[1] = p.stats[2 * row + 1], row_stat[2] = a.delta[row];
+		}
+	};
+	int     buffer = 0;
+	int64_t it = (int64_t)split * a.part;
+	// (a workgroup none of whose keys counts has nothing to read)
+	const bool any = __syncthreads_or(work);
+	if(!any) it = last;
+	if(it < last) fetch(it);
+	for(; it < last; it++) {
+		unsigned char* const qs = smem + buffer * S::SET;
+		unsigned char* const gs = qs + S::TILE;
+		float* const         st = reinterpret_cast<float*>(gs + S::TILE);
+		const int64_t        h = hk * G + it / q_tiles, q0 = it % q_tiles * QT;
+		if constexpr(S::BUFFERS == 1) __syncthreads();
+		const int64_t left = p.Lq - q0;
+		pq.store(qs, D, [&](int r) { return r < left; });
+		pg.store(gs, D, [&](int r) { return r < left; });
+		if((int)threadIdx.x < QT) st[threadIdx.x] = row_stat[0], st[QT + threadIdx.x] = row_stat[1], st[2 * QT + threadIdx.x] = row_stat[2];
+		__syncthreads();
+		if(it + 1 < last) fetch(it + 1);
+		if(work) {
+#pragma unroll
+			for(int s = 0; s < S::SUB; s++) {
+				const int row0 = 32 * (rwave * S::SUB + s);
+				if(q0 + row0 >= p.Lq) continue;
+				float x[16], y[16];
+				const float* const sm = st + row0 + 16 * half;
+				if(dead) {
+#pragma unroll
+					for(int r = 0; r < 16; r++) x[r] = sm[QT + r], y[r] = 0.f;
+				} else {
+					f32x16 acc{}, dp{};
+#pragma unroll
+					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, row0, i, lane), kf[i], acc);
+#pragma unroll
+					for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, row0, i, lane), vf[i], dp);
+					float bs[16];
+					if constexpr(BIAS) {
+						const T* const at = static_cast<const T*>(p.bias) + h * p.bias_stride[0] + (in ? key : 0);
+#pragma unroll
+						for(int r = 0; r < 16; r++) {
+							const int64_t q = q0 + row0 + 16 * half + r;
+							const float   v = kind<T>::value(at[(q < p.Lq ? q : 0) * p.bias_stride[1]]);
+							bs[r] = q < p.Lq ? v : 0.f;
+						}
+					}
+#pragma unroll
+					for(int r = 0; r < 16; r++) {
+						const float t0 = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, bs[r]) : acc[r];
+						x[r] = __builtin_amdgcn_exp2f((t0 - sm[r]) * a.factor) * sm[QT + r];
+						y[r] = x[r] * (dp[r] - sm[2 * QT + r]);
+					}
+				}
+#pragma unroll
+				for(int j = 0; j < TL::JOINTS; j++) {
+					const u32x4 pf = kind<T>::pack(x + E * j), df = kind<T>::pack(y + E * j);
+#pragma unroll
+					for(int db = 0; db < TL::BLOCKS; db++) {
+						dv[db] = kind<T>::mma(TL::col_frag(gs, row0, db, j, lane), pf, dv[db]);
+						dk[db] = kind<T>::mma(TL::col_frag(qs, row0, db, j, lane), df, dk[db]);
+					}
+				}
+			}
+		}
+		if constexpr(S::BUFFERS == 2) buffer ^= 1;
+	}
+	if constexpr(RW > 1) {
+		float* const tables = reinterpret_cast<float*>(smem) + kwave * RW * 32 * (DP + 4);
+		__syncthreads();
+		add_up<DP, RW>(tables, rwave, lane, dv);
+		__syncthreads();
+		add_up<DP, RW>(tables, rwave, lane, dk);
+	}
+	if(!in) return;
+	const int64_t at = (b * p.Hkv + hk) * p.Lk + key, n_keys = p.B * p.Hkv * p.Lk;
+	const bool    counts_v = lives || dead, counts_k = lives && !dead;
+#pragma unroll
+	for(int db = 0; db < TL::BLOCKS; db++) {
+		if(db % RW != rwave) continue;
+		float v[16], k[16];
+#pragma unroll
+		for(int r = 0; r < 16; r++) v[r] = counts_v ? dv[db][r] : 0.f, k[r] = counts_k ? dk[db][r] * p.softmax_scale : 0.f;
+		if(a.splits > 1) {
+			store_row16(a.partial + (2 * split * n_keys + at) * D, 32 * db + 16 * half, D, k);
+			store_row16(a.partial + ((2 * split + 1) * n_keys + at) * D, 32 * db + 16 * half, D, v);
+		} else {
+			if(a.g.grad_k) store_row16(static_cast<T*>(a.g.grad_k) + at * D, 32 * db + 16 * half, D, k);
+			if(a.g.grad_v) store_row16(static_cast<T*>(a.g.grad_v) + at * D, 32 * db + 16 * half, D, v);
+		}
+	}
+}
+
+// The parts' sums added in order: n elements per part, parts `step` elements apart.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) cross_sum_kernel(const float* partial, int64_t step, uint32_t splits, T* out, int64_t n) {
+	const int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4;
+	if(i >= n) return;
+	float v[4] = {0.f, 0.f, 0.f, 0.f};
+	if(i + 4 <= n) {
+		for(uint32_t s = 0; s < splits; s++) {
+			const f32x4 x = *reinterpret_cast<const f32x4_any*>(partial + s * step + i);
+#pragma unroll
+			for(int e = 0; e < 4; e++) v[e] += x[e];
+		}
+#pragma unroll
+		for(int e = 0; e < 4; e++) out[i + e] = kind<T>::bits(v[e]);
+	} else {
+		for(int e = 0; i + e < n; e++) {
+			float x = 0.f;
+			for(uint32_t s = 0; s < splits; s++) x += partial[s * step + i + e];
+			out[i + e] = kind<T>::bits(x);
+		}
+	}
+}
+
+// ---- dbias ----
+template <typename T, int DP>
+struct dbias_shape {
+	static constexpr int QT = sizeof(T) == 2 ? 64 : 32, SUB = QT / 32, KEYS = 128;
+	static constexpr int TILE = QT * tile<T, DP>::STRIDE, STATS = 3 * QT * 4, SET = 2 * TILE + STATS;
+	static constexpr int BUFFERS = 2 * SET <= 81920 ? 2 : 1, LDS = BUFFERS * SET;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS) cross_dbias_kernel(grad_args a) {
+	using S  = dbias_shape<T, DP>;
+	using TL = tile<T, DP>;
+	constexpr int QT = S::QT;
+	const af3_cross_attention_params& p = a.p;
+	extern __shared__ __align__(16) unsigned char smem[];
+
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+	const uint32_t key_tiles = (uint32_t)((p.Lk + S::KEYS - 1) / S::KEYS);
+	uint32_t       id = xcd_order(blockIdx.x, gridDim.x);
+	const uint32_t key_tile = id % key_tiles;
+	id /= key_tiles;
+	const int64_t  q0 = (int64_t)(id % a.tiles) * QT, h = id / a.tiles, hk = h / (p.H / p.Hkv);
+	const int      D = (int)p.D;
+	const int64_t  key = (int64_t)key_tile * S::KEYS + 32 * wave + (lane & 31);
+	const bool     in = key < p.Lk;
+
+	float sum[S::SUB][16], bs[S::SUB][16];
+#pragma unroll
+	for(int s = 0; s < S::SUB; s++)
+#pragma unroll
+		for(int r = 0; r < 16; r++) {
+			const int64_t q = q0 + 32 * s + 16 * half + r;
+			sum[s][r] = 0.f, bs[s][r] = 0.f;
+			if(in && q < p.Lq) bs[s][r] = kind<T>::value(static_cast<const T*>(p.bias)[h * p.bias_stride[0] + q * p.bias_stride[1] + key]);
+		}
+	passage<T, DP, QT> pq, pg;
+	float row_stat[3];
+	auto fetch = [&](int64_t b) {
+		pq.load(static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1], p.q_stride[2], q0, p.Lq, D, a.whole);
+		pg.load(static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1], a.g.grad_out_stride[2], q0, p.Lq, D, a.whole);
+		row_stat[0] = row_stat[1] = row_stat[2] = 0.f;
+		if((int)threadIdx.x < QT && q0 + threadIdx.x < p.Lq) {
+			const int64_t row = (b * p.H + h) * p.Lq + q0 + threadIdx.x;
+			row_stat[0] = p.stats[2 * row], row_stat[1] = p.stats[2 * row + 1], row_stat[2] = a.delta[row];
+		}
+	};
+	int buffer = 0;
+	fetch(0);
+	for(int64_t b = 0; b < p.B; b++) {
+		unsigned char* const qs = smem + buffer * S::SET;
+		unsigned char* const gs = qs + S::TILE;
+		float* const         st = reinterpret_cast<float*>(gs + S::TILE);
+		u32x4 kf[TL::STEPS], vf[TL::STEPS];
+		const bool lives = in && (!p.key_mask || p.key_mask[b * p.key_mask_stride_b + key] != 0);
+		load_operand<T, DP>(kf, static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[1] + (in ? key : 0) * p.k_stride[2], lives, D, lane);
+		load_operand<T, DP>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], lives, D, lane);
+		if constexpr(S::BUFFERS == 1) __syncthreads();
+		const int64_t left = p.Lq - q0;
+		pq.store(qs, D, [&](int r) { return r < left; });
+		pg.store(gs, D, [&](int r) { return r < left; });
+		if((int)threadIdx.x < QT) st[threadIdx.x] = row_stat[0], st[QT + threadIdx.x] = row_stat[1], st[2 * QT + threadIdx.x] = row_stat[2];
+		__syncthreads();
+		if(b + 1 < p.B) fetch(b + 1);
+		if(st[0] != -INFINITY && __any(lives)) {   // (-inf: a batch row without a live key)
+#pragma unroll
+			for(int s = 0; s < S::SUB; s++) {
+				f32x16 acc{}, dp{};
+#pragma unroll
+				for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, 32 * s, i, lane), kf[i], acc);
+#pragma unroll
+				for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, 32 * s, i, lane), vf[i], dp);
+				const float* const sm = st + 32 * s + 16 * half;
+#pragma unroll
+				for(int r = 0; r < 16; r++) {
+					const float pr = __builtin_amdgcn_exp2f((__builtin_fmaf(acc[r], p.softmax_scale, bs[s][r]) - sm[r]) * a.factor) * sm[QT + r];
+					const float ds = pr * (dp[r] - sm[2 * QT + r]);
+					sum[s][r] += lives ? ds : 0.f;
+				}
+			}
+		}
+		if constexpr(S::BUFFERS == 2) buffer ^= 1;
+	}
+	if(!in) return;
+	T* const out = static_cast<T*>(a.g.grad_bias) + h * p.Lq * p.Lk + key;
+#pragma unroll
+	for(int s = 0; s < S::SUB; s++)
+#pragma unroll
+		for(int r = 0; r < 16; r++) {
+			const int64_t q = q0 + 32 * s + 16 * half + r;
+			if(q < p.Lq) out[q * p.Lk] = kind<T>::bits(sum[s][r]);
+		}
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------
+struct cut {
+	bool     shared;   // wavefronts share 32 rows (dq) or keys (dkv)
+	uint32_t tiles, splits;
+	int64_t  part;
+};
+inline int64_t over(int64_t n, int64_t per) { return (n + per - 1) / per; }
+
+// `length` rows that results belong to (128 or 32 of them per workgroup), `steps(shared)` tiles of the other axis
+template <typename F>
+cut cut_for(int64_t length, int64_t groups, bool may_share, F steps) {
+	cut c;
+	c.shared = may_share && (length <= 32 || over(length, 128) * groups < 256);
+	c.tiles  = (uint32_t)over(length, c.shared ? 32 : 128);
+	const int64_t n = steps(c.shared), busy = groups * c.tiles;
+	int64_t       splits = busy >= 512 ? 1 : over(512, busy);
+	if(splits > (n + 1) / 2) splits = (n + 1) / 2;
+	if(splits < 1) splits = 1;
+	c.part   = over(n, splits);
+	c.splits = (uint32_t)over(n, c.part);
+	return c;
+}
+cut dq_cut(const af3_cross_attention_params& p) {
+	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, true, [&](bool shared) { return over(p.Lk, shared ? 128 : 64); });
+	c.part *= c.shared ? 128 : 64;
+	return c;
+}
+cut dkv_cut(const af3_cross_attention_params& p) {
+	// (fp32 beyond 64 columns: the tile of 128 rows leaves no registers for the sums)
+	return cut_for(p.Lk, p.B * p.Hkv, p.dtype == AF3_BF16 || p.D <= 64, [&](bool shared) { return p.H / p.Hkv * over(p.Lq, shared ? 128 : p.dtype == AF3_F32 ? 32 : 64); });
+}
+
+struct grad_space {
+	int64_t delta, dq, dkv, bytes;   // floats
+};
+grad_space grad_workspace(const af3_cross_attention_params& p) {
+	const cut  q = dq_cut(p), kv = dkv_cut(p);
+	grad_space w;
+	w.delta = over(p.B * p.H * p.Lq, 4) * 4;
+	w.dq    = q.splits > 1 ? over(q.splits * p.B * p.H * p.Lq * p.D, 4) * 4 : 0;
+	w.dkv   = kv.splits > 1 ? 2 * (int64_t)kv.splits * p.B * p.Hkv * p.Lk * p.D : 0;
+	w.bytes = (w.delta + (w.dq > w.dkv ? w.dq : w.dkv)) * 4;   // (one after the other on the stream)
+	return w;
+}
+
+template <typename K>
+int launch(K kernel, int lds, uint32_t grid, const grad_args& a, hipStream_t s) {
+	if(lds > 65536 - 8192 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+		(void)hipGetLastError();
+		return AF3_ERR_LAUNCH;
+	}
+	hipLaunchKernelGGL(kernel, dim3(grid), dim3(THREADS), lds, s, a);
+	return launch_status();
+}
+
+template <typename T>
+int sum_parts(const float* partial, int64_t step, uint32_t splits, void* out, int64_t n, hipStream_t s) {
+	hipLaunchKernelGGL(cross_sum_kernel<T>, dim3((uint32_t)over(n, 4 * THREADS)), dim3(THREADS), 0, s, partial, step, splits, static_cast<T*>(out), n);
+	return launch_status();
+}
+
+template <typename T, int DP>
+int backward(grad_args a, hipStream_t s) {
+	const af3_cross_attention_params& p = a.p;
+	const int64_t n_rows = p.B * p.H * p.Lq, n_keys = p.B * p.Hkv * p.Lk;
+	if(a.g.grad_q) {
+		const cut c = dq_cut(p);
+		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part;
+		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * c.tiles * c.splits;
+		int rc;
+		if(c.shared) rc = p.bias ? launch(cross_dq_kernel<T, DP, 4, true>, dq_shape<T, DP, 4>::LDS, grid, a, s) : launch(cross_dq_kernel<T, DP, 4, false>, dq_shape<T, DP, 4>::LDS, grid, a, s);
+		else rc = p.bias ? launch(cross_dq_kernel<T, DP, 1, true>, dq_shape<T, DP, 1>::LDS, grid, a, s) : launch(cross_dq_kernel<T, DP, 1, false>, dq_shape<T, DP, 1>::LDS, grid, a, s);
+		if(rc == AF3_OK && c.splits > 1) rc = sum_parts<T>(a.partial, n_rows * p.D, c.splits, a.g.grad_q, n_rows * p.D, s);
+		if(rc != AF3_OK) return rc;
+	} else {
+		hipLaunchKernelGGL(cross_delta_kernel<T>, dim3((uint32_t)over(n_rows, WAVES)), dim3(THREADS), 0, s, a);
+		if(const int rc = launch_status(); rc != AF3_OK) return rc;
+	}
+	if(a.g.grad_k || a.g.grad_v) {
+		const cut c = dkv_cut(p);
+		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part;
+		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * c.tiles * c.splits;
+		int rc = AF3_ERR_LAUNCH;
+		if constexpr(sizeof(T) == 2 || DP <= 64)
+			if(c.shared) rc = p.bias ? launch(cross_dkv_kernel<T, DP, 4, true>, dkv_shape<T, DP, 4>::LDS, grid, a, s) : launch(cross_dkv_kernel<T, DP, 4, false>, dkv_shape<T, DP, 4>::LDS, grid, a, s);
+		if(!c.shared) rc = p.bias ? launch(cross_dkv_kernel<T, DP, 1, true>, dkv_shape<T, DP, 1>::LDS, grid, a, s) : launch(cross_dkv_kernel<T, DP, 1, false>, dkv_shape<T, DP, 1>::LDS, grid, a, s);
+		if(rc == AF3_OK && c.splits > 1 && a.g.grad_k) rc = sum_parts<T>(a.partial, 2 * n_keys * p.D, c.splits, a.g.grad_k, n_keys * p.D, s);
+		if(rc == AF3_OK && c.splits > 1 && a.g.grad_v) rc = sum_parts<T>(a.partial + n_keys * p.D, 2 * n_keys * p.D, c.splits, a.g.grad_v, n_keys * p.D, s);
+		if(rc != AF3_OK) return rc;
+	}
+	if(a.g.grad_bias) {
+		using S = dbias_shape<T, DP>;
+		a.tiles = (uint32_t)over(p.Lq, S::QT);
+		return launch(cross_dbias_kernel<T, DP>, S::LDS, (uint32_t)(p.H * a.tiles * over(p.Lk, S::KEYS)), a, s);
+	}
+	return AF3_OK;
+}
+template <typename T>
+int backward_type(const grad_args& a, hipStream_t s) {
+	if(a.p.D <= 32) return backward<T, 32>(a, s);
+	if(a.p.D <= 64) return backward<T, 64>(a, s);
+	if(a.p.D <= 96) return backward<T, 96>(a, s);
+	return backward<T, 128>(a, s);
+}
+
+int validate_grads(const af3_cross_attention_params* p, const af3_cross_attention_grads* g) {
+	if(const int rc = validate_cross_attention(p); rc != AF3_OK) return rc;
+	if(!g || !g->grad_out || !p->stats || (!g->grad_q && !g->grad_k && !g->grad_v && !g->grad_bias)) return AF3_ERR_NULL_POINTER;
+	if(g->grad_bias && !p->bias) return AF3_ERR_NULL_POINTER;
+	for(int i = 0; i < 3; i++)
+		if(g->grad_out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
+	// (workgroup numbers of the kernels whose results are the keys' and the bias's)
+	if(p->B * p->Hkv * over(p->Lk, 32) > 0x3ffffff || p->H * over(p->Lq, 32) > 0x3ffffff || p->H * over(p->Lq, 32) * over(p->Lk, 128) > 0x3ffffff) return AF3_ERR_BAD_SHAPE;
+	return AF3_OK;
+}
+
+}  // namespace cross
+}  // namespace af3
+
+using namespace af3;
+
+extern "C" int64_t af3_cross_attention_backward_workspace_bytes(const af3_cross_attention_params* params) {
+	const int rc = validate_cross_attention(params);
+	return rc != AF3_OK ? rc : cross::grad_workspace(*params).bytes;
+}
+
+extern "C" int af3_cross_attention_backward(const af3_cross_attention_params* params, const af3_cross_attention_grads* grads, void* hip_stream) {
+	if(const int rc = cross::validate_grads(params, grads); rc != AF3_OK) return rc;
+	const cross::grad_space w = cross::grad_workspace(*params);
+	if(!grads->workspace || grads->workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(grads->workspace) & 15)) return AF3_ERR_BAD_ARGUMENT;
+	if(const int dc = current_device_status(); dc != AF3_OK) return dc;
+	cross::grad_args a;
+	a.p = *params, a.g = *grads, a.tiles = a.splits = 1, a.part = 0;
+	a.factor  = params->bias ? LOG2E : params->softmax_scale * LOG2E;
+	a.whole   = params->D * (params->dtype == AF3_F32 ? 4 : 2) % 16 == 0;
+	a.delta   = static_cast<float*>(grads->workspace);
+	a.partial = a.delta + w.delta;
+	const hipStream_t s = static_cast<hipStream_t>(hip_stream);
+	return params->dtype == AF3_F32 ? cross::backward_type<float>(a, s) : cross::backward_type<uint16_t>(a, s);
+}

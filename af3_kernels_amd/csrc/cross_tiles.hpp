@@ -1,0 +1,254 @@
+// What the kernels of attention to states of another length share (cross_attention.hip, cross_attention_grad.hip): tiles of rows in
+// LDS, and matrix fragments of them for bf16 and fp32 alike.
+//
+// Every fragment is 16 bytes per lane, E = 16 / sizeof(T) elements, and one step contracts 2E of them: bf16 one
+// v_mfma_f32_32x32x16_bf16, fp32 four v_mfma_f32_32x32x2_f32.  A contraction takes its elements in any order as long as both operands
+// do, and so do the 32 rows of a result as long as the reader knows them.  Both freedoms are used the same way everywhere: row i of
+// an A operand is tile row tile_row(i), chosen so that register r of a lane in half h of the wavefront holds result row 16 h + r.
+// A result's registers, packed, are then the B operand of the next product as they stand (contraction step j: rows 16 h + E j ...),
+// a lane's 16 values of a bias row lie side by side in memory, and so do the 16 it stores of a result row.
+#pragma once
+#include "mfma_helpers.hpp"
+
+namespace af3 {
+namespace cross {
+
+constexpr int THREADS = 256, WAVES = 4;
+constexpr float LOWEST = -3.402823466e38f;
+
+template <typename T>
+struct kind;
+template <>
+struct kind<uint16_t> {   // bf16 bits
+	static constexpr int E = 8;
+	static __device__ __forceinline__ f32x16 mma(const u32x4& a, const u32x4& b, f32x16 c) {
+		return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+	}
+	// registers E j .. E j + E - 1 of a result as step j of a B operand (rounded to bf16: the product that follows takes nothing wider)
+	static __device__ __forceinline__ u32x4 pack(const float* r) { return u32x4{pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]), pack_bf16x2(r[4], r[5]), pack_bf16x2(r[6], r[7])}; }
+	static __device__ __forceinline__ float at(const u32x4& v, int i) { return i & 1 ? __uint_as_float(v[i >> 1] & 0xffff0000u) : __uint_as_float(v[i >> 1] << 16); }
+	static __device__ __forceinline__ float value(uint16_t x) { return bf16_bits_to_f32(x); }
+	static __device__ __forceinline__ uint16_t bits(float f) { return (uint16_t)f32_to_bf16_bits(f); }
+};
+template <>
+struct kind<float> {
+	static constexpr int E = 4;
+	static __device__ __forceinline__ f32x16 mma(const u32x4& a, const u32x4& b, f32x16 c) {
+#pragma unroll
+		for(int i = 0; i < 4; i++) {
+			const uint32_t x = a[i], y = b[i];
+			c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x), __uint_as_float(y), c, 0, 0, 0);
+		}
+		return c;
+	}
+	static __device__ __forceinline__ u32x4 pack(const float* r) { return u32x4{__float_as_uint(r[0]), __float_as_uint(r[1]), __float_as_uint(r[2]), __float_as_uint(r[3])}; }
+	static __device__ __forceinline__ float at(const u32x4& v, int i) {
+		const uint32_t x = v[i];
+		return __uint_as_float(x);
+	}
+	static __device__ __forceinline__ float value(float x) { return x; }
+	static __device__ __forceinline__ float bits(float f) { return f; }
+};
+
+typedef __attribute__((ext_vector_type(4), aligned(4))) uint32_t u32x4_f32;
+template <typename T>
+__device__ __forceinline__ u32x4 load16(const T* p) {   // 16 bytes at any element's address
+	if constexpr(sizeof(T) == 2) return *reinterpret_cast<const u32x4_any*>(p);
+	else return *reinterpret_cast<const u32x4_f32*>(p);
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const u32x4& v) {
+	if constexpr(sizeof(T) == 2) *reinterpret_cast<u32x4_any*>(p) = v;
+	else *reinterpret_cast<u32x4_f32*>(p) = v;
+}
+// E elements of a row from element d on, zeros from D on
+template <typename T>
+__device__ __forceinline__ u32x4 load_guarded(const T* row, int d, int D) {
+	constexpr int E = kind<T>::E;
+	T             e[E];
+#pragma unroll
+	for(int i = 0; i < E; i++) {
+		e[i] = T(0);
+		if(d + i < D) e[i] = row[d + i];
+	}
+	return *reinterpret_cast<const u32x4*>(e);
+}
+
+__device__ __forceinline__ int   tile_row(int i) { return 16 * ((i >> 2) & 1) + (i & 3) + 4 * (i >> 3); }
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }   // (NaN stays)
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// A tile in LDS: rows of DP elements and 16 bytes more, which puts consecutive rows on other banks.
+template <typename T, int DP>
+struct tile {
+	static constexpr int STRIDE = DP * (int)sizeof(T) + 16, STEPS = DP * (int)sizeof(T) / 32, BLOCKS = DP / 32, CHUNKS = DP * (int)sizeof(T) / 16, JOINTS = 32 / (2 * kind<T>::E);
+	// contraction over the columns: A operand, step s, of the 32 rows from `row0` on
+	static __device__ __forceinline__ u32x4 row_frag(const unsigned char* lds, int row0, int s, int lane) {
+		return *reinterpret_cast<const u32x4*>(lds + (row0 + tile_row(lane & 31)) * STRIDE + 32 * s + 16 * (lane >> 5));
+	}
+	// contraction over the 32 rows from `row0` on: A operand, step j, of columns 32 db .. 32 db + 31
+	static __device__ __forceinline__ u32x4 col_frag(const unsigned char* lds, int row0, int db, int j, int lane) {
+		if constexpr(sizeof(T) == 2) {
+			// (ds_read_b64_tr_b16: lane i of a group of 16 supplies 4 columns of row i / 4 and receives 4 rows of the group's column i)
+			const int i = lane & 15, G = lane >> 4;
+			u32x4     f;
+#pragma unroll
+			for(int t = 0; t < 2; t++) {
+				const int   row = row0 + 16 * (G >> 1) + 8 * j + 4 * t + (i >> 2), col = 32 * db + 16 * (i & 1) + 4 * ((i >> 1) & 1) + 8 * (G & 1);
+				const u32x2 r   = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + row * STRIDE + col * 2)));
+				f[2 * t] = r[0], f[2 * t + 1] = r[1];
+			}
+			return f;
+		} else {
+			u32x4 f;
+#pragma unroll
+			for(int t = 0; t < 4; t++) f[t] = *reinterpret_cast<const uint32_t*>(lds + (row0 + 16 * (lane >> 5) + 4 * j + t) * STRIDE + (32 * db + tile_row(lane & 31)) * 4);
+			return f;
+		}
+	}
+};
+
+// ROWS rows on their way from memory into a tile, spread over the workgroup's threads.  Where D is a whole number of 16-byte pieces
+// (whole) every piece is one load at a place that exists, and pieces that lie past the rows or past D become zeros on the way into LDS.
+template <typename T, int DP, int ROWS>
+struct passage {
+	using TL = tile<T, DP>;
+	static constexpr int N = ROWS * TL::CHUNKS / THREADS;
+	static_assert(N * THREADS == ROWS * TL::CHUNKS);
+	u32x4 piece[N];
+	// rows row0 .. row0 + ROWS - 1 of a matrix, those below `rows` exist (one at least)
+	__device__ __forceinline__ void load(const T* base, int64_t stride, int64_t row0, int64_t rows, int D, bool whole) {
+		const T*  at   = base + row0 * stride;
+		const int left = rows - row0 < ROWS ? (int)(rows - row0) : ROWS;
+		if(whole) {
+#pragma unroll
+			for(int n = 0; n < N; n++) {
+				const int c = threadIdx.x + THREADS * n, row = c / TL::CHUNKS, d = (c % TL::CHUNKS) * kind<T>::E;
+				piece[n] = load16(at + (int64_t)(row < left ? row : 0) * stride + (d < D ? d : 0));
+			}
+		} else {
+#pragma unroll
+			for(int n = 0; n < N; n++) {
+				const int c = threadIdx.x + THREADS * n, row = c / TL::CHUNKS, d = (c % TL::CHUNKS) * kind<T>::E;
+				piece[n] = load_guarded(at + (int64_t)(row < left ? row : 0) * stride, d, D);
+			}
+		}
+	}
+	// keep(row): whether the tile is to hold that row (zeros otherwise)
+	template <typename F>
+	__device__ __forceinline__ void store(unsigned char* lds, int D, F keep) const {
+#pragma unroll
+		for(int n = 0; n < N; n++) {
+			const int  c = threadIdx.x + THREADS * n, row = c / TL::CHUNKS, col = c % TL::CHUNKS;
+			const bool in = keep(row) && col * kind<T>::E < D;
+			u32x4      v = piece[n];
+#pragma unroll
+			for(int i = 0; i < 4; i++) {
+				const uint32_t x = v[i];
+				v[i] = in ? x : 0u;
+			}
+			*reinterpret_cast<u32x4*>(lds + row * TL::STRIDE + 16 * col) = v;
+		}
+	}
+};
+
+// 32 rows of a matrix as a B operand, held in registers: lane holds column (= row of memory) `row`, zeros where `ok` is not
+template <typename T, int DP, int N>
+__device__ __forceinline__ void load_operand(u32x4 (&f)[N], const T* row, bool ok, int D, int lane) {
+	constexpr int E = kind<T>::E;
+	static_assert(N == tile<T, DP>::STEPS);
+#pragma unroll
+	for(int s = 0; s < N; s++) {
+		const int d = 2 * E * s + E * (lane >> 5);
+		f[s] = u32x4{0u, 0u, 0u, 0u};
+		if(ok && d + E <= D) f[s] = load16(row + d);
+		else if(ok && d < D) f[s] = load_guarded(row, d, D);
+	}
+}
+
+// 16 entries of a row from `first` on as floats, those from L on left at 0 (`row` is the row's first entry)
+template <typename T>
+__device__ __forceinline__ void load_row16(float (&out)[16], const T* row, int64_t first, int64_t L) {
+	constexpr int E = kind<T>::E;
+	if(first + 16 <= L) {
+#pragma unroll
+		for(int i = 0; i < 16 / E; i++) {
+			const u32x4 v = load16(row + first + E * i);
+#pragma unroll
+			for(int e = 0; e < E; e++) out[E * i + e] = kind<T>::at(v, e);
+		}
+	} else {
+#pragma unroll
+		for(int i = 0; i < 16; i++) {
+			out[i] = 0.f;
+			if(first + i < L) out[i] = kind<T>::value(row[first + i]);
+		}
+	}
+}
+// 16 results side by side, from element d on, those below D
+template <typename T>
+__device__ __forceinline__ void store_row16(T* row, int d, int D, const float (&v)[16]) {
+	constexpr int E = kind<T>::E;
+	if(d + 16 <= D) {
+#pragma unroll
+		for(int i = 0; i < 16 / E; i++) store16(row + d + E * i, kind<T>::pack(v + E * i));
+	} else {
+#pragma unroll
+		for(int i = 0; i < 16; i++)
+			if(d + i < D) row[d + i] = kind<T>::bits(v[i]);
+	}
+}
+
+// ---- which keys are live ----
+// A stretch of SEGMENT keys at a time: one bit per key in `bits`, one bit per tile of KT keys that has a live one in `tiles`.
+constexpr int SEGMENT = 16384;
+template <int KT>
+struct live_keys {
+	uint32_t bits[SEGMENT / 32];
+	uint32_t tiles[SEGMENT / KT / 32];
+	// keys first .. last - 1 (at most SEGMENT of them); a barrier stands before and behind it
+	__device__ __forceinline__ void scan(const uint8_t* mask, int64_t first, int64_t last) {
+		__syncthreads();
+		for(int i = threadIdx.x; i < SEGMENT / KT / 32; i += THREADS) tiles[i] = 0u;
+		__syncthreads();
+		const int n = (int)(last - first);
+		for(int k = 32 * threadIdx.x; k < n; k += 32 * THREADS) {
+			uint32_t w = 0u;
+			if(!mask) {
+				w = n - k >= 32 ? ~0u : (1u << (n - k)) - 1u;
+			} else if(n - k >= 32) {
+				const u32_bytes* m = reinterpret_cast<const u32_bytes*>(mask + first + k);
+#pragma unroll
+				for(int i = 0; i < 8; i++) w |= ((live_bytes(m[i]) * 0x01020408u) >> 24) << (4 * i);
+			} else {
+				for(int i = 0; i < n - k; i++) w |= (mask[first + k + i] != 0 ? 1u : 0u) << i;
+			}
+			bits[k >> 5] = w;
+			if(w) atomicOr(&tiles[(k / KT) >> 5], 1u << ((k / KT) & 31));
+		}
+		// (the words of a tile that begins below n and ends behind it)
+		for(int k = (n + 31) / 32 + threadIdx.x; k < (n + KT - 1) / KT * (KT / 32); k += THREADS) bits[k] = 0u;
+		__syncthreads();
+	}
+	// the first live tile from t on, -1: none
+	__device__ __forceinline__ int next(int t) const {
+		for(int w = t >> 5; w < SEGMENT / KT / 32; w++) {
+			uint32_t x = tiles[w];
+			if(w == t >> 5) x &= ~0u << (t & 31);
+			x = (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+			if(x) return 32 * w + __builtin_ctz(x);
+		}
+		return -1;
+	}
+	__device__ __forceinline__ uint32_t word(int i) const { return (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[i]); }
+	__device__ __forceinline__ bool keeps(int key) const { return (bits[key >> 5] >> (key & 31)) & 1u; }
+};
+
+// Workgroups that read the same keys and values on the same XCD (workgroup i runs on XCD i % 8): their numbers, side by side
+__device__ __forceinline__ uint32_t xcd_order(uint32_t i, uint32_t n) {
+	const uint32_t whole = n & ~7u;
+	return i < whole ? (i & 7u) * (whole >> 3) + (i >> 3) : i;
+}
+
+}  // namespace cross
+}  // namespace af3

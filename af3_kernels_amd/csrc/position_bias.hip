@@ -1,0 +1,329 @@
+// The learned relative position bias: out[h][q][k] = table[bucket(k_pos[k] - q_pos[q])][h], and the table's gradient, the sums of
+// out's gradient by bucket.  af3_position_bias_forward, af3_position_bias_backward.
+//
+// A bucket is found by its smallest distance: `border` holds those of one side in ascending order, worked out on the host in whole
+// numbers, so that no logarithm's rounding decides at a border.  From the last border on (`reach`) nothing changes any more: the
+// buckets (backward) or the head's values (forward) of the offsets -reach .. reach are a table in LDS, and 16 bytes of keys that all
+// lie beyond it are one value.  Both kernels are bound by memory: the forward pass writes, the backward pass reads H Lq Lk values.
+#include "cross_tiles.hpp"
+
+#include <math.h>
+#include <vector>
+
+namespace af3 {
+namespace position {
+
+using cross::kind;
+using cross::load16;
+using cross::store16;
+
+constexpr int MAX_BUCKETS = AF3_POSITION_BIAS_MAX_BUCKETS;
+constexpr int MAX_OFFSETS = 4097;   // of the table in LDS; with more, buckets are searched for one by one
+constexpr int THREADS = 256;
+
+struct args {
+	const void*    table;    // forward: the values; backward: not read
+	void*          out;      // forward: [H, Lq, Lk]; backward: the table's gradient
+	const void*    grad;     // backward: [H, Lq, Lk]
+	float*         partial;  // backward: [H][parts][buckets]
+	const int64_t *q_pos, *k_pos;
+	int64_t        q_offset;
+	int64_t        table_stride[2], grad_stride[2];
+	int64_t        H, Lq, Lk;
+	int32_t        buckets, borders, reach;
+	int32_t        first_behind, step_behind, first_ahead, step_ahead;   // bucket = first + step * (borders passed), keys behind (and at) the query and ahead of it
+	int32_t        columns_log2, rows;   // threads across the columns of a workgroup, rows of a workgroup
+	int32_t        border[MAX_BUCKETS];
+};
+
+__device__ __forceinline__ int passed(const int* border, int n, int d) {   // how many borders are <= d
+	int low = 0;
+	while(n > 0) {
+		const int half = n >> 1;
+		if(border[low + half] <= d) low += half + 1, n -= half + 1;
+		else n = half;
+	}
+	return low;
+}
+__device__ __forceinline__ int bucket_of(const args& a, const int* border, int rel) {
+	return rel <= 0 ? a.first_behind + a.step_behind * passed(border, a.borders, -rel) : a.first_ahead + a.step_ahead * passed(border, a.borders, rel);
+}
+__device__ __forceinline__ int limited(int64_t rel, int reach) { return rel < -reach ? -reach : rel > reach ? reach : (int)rel; }
+// the difference of two positions, limited where it passes 64 bits
+__device__ __forceinline__ int64_t apart(int64_t k, int64_t q) {
+	int64_t d;
+	if(__builtin_sub_overflow(k, q, &d)) d = k < q ? INT64_MIN : INT64_MAX;
+	return d;
+}
+
+// offsets (limited to +-reach) of the E keys of a column chunk from one query
+template <int E>
+struct keys_of_chunk {
+	int64_t k[E];
+	int64_t first;
+	bool    given;
+	__device__ __forceinline__ keys_of_chunk(const args& a, int64_t col) : first(col), given(a.k_pos != nullptr) {
+#pragma unroll
+		for(int e = 0; e < E; e++) k[e] = given ? a.k_pos[col + e < a.Lk ? col + e : a.Lk - 1] : col + e;
+	}
+	__device__ __forceinline__ void offsets(int64_t q, int reach, int (&rel)[E]) const {
+		if(given) {
+#pragma unroll
+			for(int e = 0; e < E; e++) rel[e] = limited(apart(k[e], q), reach);
+		} else {   // (counted positions: the first one's offset, then one more each)
+			const int64_t r0 = apart(first, q);
+			const int     low = -reach - E, from = r0 < low ? low : r0 > reach ? reach : (int)r0;
+#pragma unroll
+			for(int e = 0; e < E; e++) rel[e] = from + e < -reach ? -reach : from + e > reach ? reach : from + e;
+		}
+	}
+};
+
+template <typename T, bool LUT>
+__global__ void __launch_bounds__(THREADS) position_bias_kernel(args a) {
+	constexpr int E = kind<T>::E;
+	__shared__ T   values[LUT ? MAX_OFFSETS : MAX_BUCKETS];   // of the offsets, or of the buckets
+	__shared__ int border[MAX_BUCKETS];
+	const int64_t  h = blockIdx.z;
+	for(int i = threadIdx.x; i < a.borders; i += THREADS) border[i] = a.border[i];
+	__syncthreads();
+	const T* const table = static_cast<const T*>(a.table) + h * a.table_stride[1];
+	for(int i = threadIdx.x; i < (LUT ? 2 * a.reach + 1 : a.buckets); i += THREADS) values[i] = table[(LUT ? bucket_of(a, border, i - a.reach) : i) * a.table_stride[0]];
+	__syncthreads();
+
+	const int     columns = 1 << a.columns_log2, tx = threadIdx.x & (columns - 1), ty = threadIdx.x >> a.columns_log2;
+	const int64_t col = ((int64_t)blockIdx.x * columns + tx) * E;
+	if(col >= a.Lk) return;
+	const keys_of_chunk<E> keys(a, col);
+	const int64_t row0 = (int64_t)blockIdx.y * a.rows, last = row0 + a.rows < a.Lq ? row0 + a.rows : a.Lq;
+	T* const      out = static_cast<T*>(a.out) + h * a.Lq * a.Lk + col;
+	for(int64_t row = row0 + ty; row < last; row += THREADS >> a.columns_log2) {
+		int rel[E];
+		keys.offsets(a.q_pos ? a.q_pos[row] : row + a.q_offset, a.reach, rel);
+		T v[E];
+#pragma unroll
+		for(int e = 0; e < E; e++) v[e] = values[LUT ? rel[e] + a.reach : bucket_of(a, border, rel[e])];
+		T* const at = out + row * a.Lk;
+		if(col + E <= a.Lk) {
+			u32x4 packed;
+#pragma unroll
+			for(int i = 0; i < 4; i++) {
+				if constexpr(sizeof(T) == 2) packed[i] = (uint32_t)v[2 * i] | (uint32_t)v[2 * i + 1] << 16;
+				else packed[i] = __float_as_uint(v[i]);
+			}
+			store16(at, packed);
+		} else {
+#pragma unroll
+			for(int e = 0; e < E; e++)
+				if(col + e < a.Lk) at[e] = v[e];
+		}
+	}
+}
+
+// Sums by bucket.  Every thread has a column of the bins in LDS to itself (64 threads to a workgroup), so that nothing is added in an order that
+// changes; the sums of the threads, then of the workgroups (in 64 bits) follow in a fixed order.
+constexpr int COLUMNS = 64;
+template <typename T, bool LUT>
+__global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
+	constexpr int E = kind<T>::E;
+	extern __shared__ float bins[];   // [buckets][COLUMNS]
+	__shared__ uint16_t bucket[LUT ? MAX_OFFSETS : 1];
+	__shared__ int      border[MAX_BUCKETS];
+	const int64_t  h = blockIdx.z;
+	for(int i = threadIdx.x; i < a.borders; i += COLUMNS) border[i] = a.border[i];
+	for(int i = 0; i < a.buckets; i++) bins[i * COLUMNS + threadIdx.x] = 0.f;
+	__syncthreads();
+	if constexpr(LUT)
+		for(int i = threadIdx.x; i < 2 * a.reach + 1; i += COLUMNS) bucket[i] = (uint16_t)bucket_of(a, border, i - a.reach);
+	__syncthreads();
+
+	const int     columns = 1 << a.columns_log2, tx = threadIdx.x & (columns - 1), ty = threadIdx.x >> a.columns_log2;
+	const int64_t col = ((int64_t)blockIdx.x * columns + tx) * E;
+	if(col < a.Lk) {
+		const keys_of_chunk<E> keys(a, col);
+		const int64_t row0 = (int64_t)blockIdx.y * a.rows, last = row0 + a.rows < a.Lq ? row0 + a.rows : a.Lq;
+		const T* const grad = static_cast<const T*>(a.grad) + h * a.grad_stride[0] + col;
+		float* const   mine = bins + threadIdx.x;
+		int   current = 0;
+		float run     = 0.f;   // of bucket `current`, not yet in its bin
+		for(int64_t row = row0 + ty; row < last; row += COLUMNS >> a.columns_log2) {
+			float v[E];
+			const T* const at = grad + row * a.grad_stride[1];
+			if(col + E <= a.Lk) {
+				const u32x4 x = load16(at);
+#pragma unroll
+				for(int e = 0; e < E; e++) v[e] = kind<T>::at(x, e);
+			} else {
+#pragma unroll
+				for(int e = 0; e < E; e++) {
+					v[e] = 0.f;
+					if(col + e < a.Lk) v[e] = kind<T>::value(at[e]);
+				}
+			}
+			int rel[E];
+			keys.offsets(a.q_pos ? a.q_pos[row] : row + a.q_offset, a.reach, rel);
+#pragma unroll
+			for(int e = 0; e < E; e++) {
+				const int bk = LUT ? bucket[rel[e] + a.reach] : bucket_of(a, border, rel[e]);
+				if(bk != current) mine[current * COLUMNS] += run, run = 0.f, current = bk;
+				run += v[e];
+			}
+		}
+		mine[current * COLUMNS] += run;
+	}
+	__syncthreads();
+	const int64_t part = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, parts = (int64_t)gridDim.x * gridDim.y;
+	for(int i = 0; i < a.buckets; i++) {
+		float sum = bins[i * COLUMNS + threadIdx.x];
+#pragma unroll
+		for(int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
+		if(threadIdx.x == 0) a.partial[(h * parts + part) * a.buckets + i] = sum;
+	}
+}
+template <typename T>
+__global__ void __launch_bounds__(THREADS) position_bias_join_kernel(args a, int64_t parts) {   // one wavefront per head and bucket
+	const int64_t n = (int64_t)blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6);
+	const int     lane = threadIdx.x & 63;
+	if(n >= a.H * a.buckets) return;
+	const int64_t h = n / a.buckets, i = n % a.buckets;
+	double        sum = 0.0;
+	for(int64_t part = lane; part < parts; part += 64) sum += (double)a.partial[(h * parts + part) * a.buckets + i];
+#pragma unroll
+	for(int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
+	if(lane == 0) static_cast<T*>(a.out)[i * a.table_stride[0] + h * a.table_stride[1]] = kind<T>::bits((float)sum);
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------
+// a^n1 * b^n2 as digits of 32 bits, lowest first
+std::vector<uint32_t> product(uint32_t a, int n1, uint32_t b, int n2) {
+	std::vector<uint32_t> d(1, 1u);
+	for(int i = 0; i < n1 + n2; i++) {
+		const uint64_t f = i < n1 ? a : b;
+		uint64_t       carry = 0;
+		for(uint32_t& x : d) carry += x * f, x = (uint32_t)carry, carry >>= 32;
+		if(carry) d.push_back((uint32_t)carry);
+	}
+	return d;
+}
+bool not_less(const std::vector<uint32_t>& a, const std::vector<uint32_t>& b) {
+	if(a.size() != b.size()) return a.size() > b.size();
+	for(size_t i = a.size(); i-- > 0;)
+		if(a[i] != b[i]) return a[i] > b[i];
+	return true;
+}
+
+int prepare(const af3_position_bias_params* p, args& a) {
+	if(!p) return AF3_ERR_NULL_POINTER;
+	if(p->dtype != AF3_F32 && p->dtype != AF3_BF16) return AF3_ERR_BAD_DTYPE;
+	if(p->buckets <= 0 || p->buckets > MAX_BUCKETS || p->H <= 0 || p->H > 0xffff || p->Lq <= 0 || p->Lk <= 0 || p->Lq > 0x3fffffff || p->Lk > 0x3fffffff) return AF3_ERR_BAD_SHAPE;
+	if(p->table_stride[0] < 0 || p->table_stride[1] < 0) return AF3_ERR_BAD_STRIDE;
+	if(p->max_distance < 1 || p->max_distance > 0x3fffffff || p->q_offset > (int64_t)1 << 62 || p->q_offset < -((int64_t)1 << 62)) return AF3_ERR_BAD_ARGUMENT;
+	const bool both = p->bidirectional != 0;
+	a.buckets = (int)p->buckets;
+	if(p->scheme == AF3_POSITION_CLIP) {
+		if(p->buckets != p->max_distance * (both ? 2 : 1) + 1) return AF3_ERR_BAD_ARGUMENT;
+		a.borders = (int)p->max_distance;
+		for(int i = 0; i < a.borders; i++) a.border[i] = i + 1;
+		a.first_behind = both ? a.borders : 0, a.step_behind = 1, a.first_ahead = both ? a.borders : 0, a.step_ahead = both ? -1 : 0;
+	} else if(p->scheme == AF3_POSITION_LOG) {
+		if(both && p->buckets % 2 != 0) return AF3_ERR_BAD_ARGUMENT;
+		const int n = (int)(both ? p->buckets / 2 : p->buckets), near = n / 2, far = n - near;
+		if(near < 1 || p->max_distance <= near) return AF3_ERR_BAD_ARGUMENT;
+		a.borders = n - 1;
+		for(int i = 0; i < near; i++) a.border[i] = i + 1;
+		for(int i = 1; i < far; i++) {   // the smallest d with (d / near)^far >= (max_distance / near)^i
+			const long double y = near * powl((long double)p->max_distance / near, (long double)i / far), r = roundl(y);
+			int               d;
+			if(fabsl(y - r) > 1e-6L) d = (int)ceill(y);
+			else d = (int)r + (not_less(product((uint32_t)r, far, 1u, 0), product((uint32_t)p->max_distance, i, (uint32_t)near, far - i)) ? 0 : 1);
+			a.border[near + i - 1] = d;
+		}
+		a.first_behind = 0, a.step_behind = 1, a.first_ahead = both ? n : 0, a.step_ahead = both ? 1 : 0;
+	} else {
+		return AF3_ERR_BAD_ARGUMENT;
+	}
+	a.reach = a.borders > 0 ? a.border[a.borders - 1] : 1;
+	a.q_pos = p->q_positions, a.k_pos = p->k_positions, a.q_offset = p->q_offset;
+	a.table_stride[0] = p->table_stride[0], a.table_stride[1] = p->table_stride[1];
+	a.grad_stride[0] = p->grad_stride[0], a.grad_stride[1] = p->grad_stride[1];
+	a.H = p->H, a.Lq = p->Lq, a.Lk = p->Lk;
+	a.table = p->table, a.out = p->out, a.grad = p->grad, a.partial = nullptr;
+	return AF3_OK;
+}
+bool tabulated(const args& a) { return 2 * (int64_t)a.reach + 1 <= MAX_OFFSETS; }
+
+// columns and rows of a workgroup of n threads, and the grid: about `each` 16-byte pieces per thread
+dim3 shape(args& a, int E, int n, int64_t each) {
+	const int64_t chunks = (a.Lk + E - 1) / E;
+	a.columns_log2 = 0;
+	while((1 << a.columns_log2) < n && (1 << a.columns_log2) < chunks) a.columns_log2++;
+	const int64_t across = (chunks + (1 << a.columns_log2) - 1) >> a.columns_log2, deep = n >> a.columns_log2;
+	int64_t       rows = deep * each;
+	while((a.Lq + rows - 1) / rows > 0xffff) rows *= 2;
+	a.rows = (int32_t)(rows < a.Lq ? rows : a.Lq);
+	return dim3((uint32_t)across, (uint32_t)((a.Lq + a.rows - 1) / a.rows), (uint32_t)a.H);
+}
+dim3 sums_shape(args& a, int E) {
+	// about 2048 workgroups; each adds its bins up, which is worth a few hundred rows of reading
+	const int64_t pieces = a.H * a.Lq * ((a.Lk + E - 1) / E);
+	int64_t       each = pieces / (2048 * COLUMNS);
+	return shape(a, E, COLUMNS, each < 16 ? 16 : each > 4096 ? 4096 : each);
+}
+
+template <typename T>
+int forward(const args& a, dim3 grid, hipStream_t s) {
+	if(tabulated(a)) hipLaunchKernelGGL((position_bias_kernel<T, true>), grid, dim3(THREADS), 0, s, a);
+	else hipLaunchKernelGGL((position_bias_kernel<T, false>), grid, dim3(THREADS), 0, s, a);
+	return launch_status();
+}
+template <typename T, bool LUT>
+int sums(const args& a, dim3 grid, hipStream_t s) {
+	const int lds = a.buckets * COLUMNS * 4;
+	if(lds > 32768 && hipFuncSetAttribute(reinterpret_cast<const void*>(&position_bias_sums_kernel<T, LUT>), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+		(void)hipGetLastError();
+		return AF3_ERR_LAUNCH;
+	}
+	hipLaunchKernelGGL((position_bias_sums_kernel<T, LUT>), grid, dim3(COLUMNS), lds, s, a);
+	return launch_status();
+}
+template <typename T>
+int backward(const args& a, dim3 grid, hipStream_t s) {
+	if(const int rc = tabulated(a) ? sums<T, true>(a, grid, s) : sums<T, false>(a, grid, s); rc != AF3_OK) return rc;
+	hipLaunchKernelGGL(position_bias_join_kernel<T>, dim3((uint32_t)((a.H * a.buckets + 3) / 4)), dim3(THREADS), 0, s, a, (int64_t)grid.x * grid.y);
+	return launch_status();
+}
+
+}  // namespace position
+}  // namespace af3
+
+using namespace af3;
+
+extern "C" int af3_position_bias_forward(const af3_position_bias_params* params, void* hip_stream) {
+	position::args a;
+	if(const int rc = position::prepare(params, a); rc != AF3_OK) return rc;
+	if(!params->table || !params->out) return AF3_ERR_NULL_POINTER;
+	if(const int dc = current_device_status(); dc != AF3_OK) return dc;
+	const hipStream_t s = static_cast<hipStream_t>(hip_stream);
+	const dim3 grid = position::shape(a, params->dtype == AF3_F32 ? 4 : 8, position::THREADS, 16);
+	return params->dtype == AF3_F32 ? position::forward<float>(a, grid, s) : position::forward<uint16_t>(a, grid, s);
+}
+
+extern "C" int64_t af3_position_bias_workspace_bytes(const af3_position_bias_params* params) {
+	position::args a;
+	if(const int rc = position::prepare(params, a); rc != AF3_OK) return rc;
+	const dim3 grid = position::sums_shape(a, params->dtype == AF3_F32 ? 4 : 8);
+	return (int64_t)grid.x * grid.y * grid.z * a.buckets * 4;
+}
+
+extern "C" int af3_position_bias_backward(const af3_position_bias_params* params, void* hip_stream) {
+	position::args a;
+	if(const int rc = position::prepare(params, a); rc != AF3_OK) return rc;
+	if(!params->grad || !params->out || !params->workspace) return AF3_ERR_NULL_POINTER;
+	if(params->grad_stride[0] < 0 || params->grad_stride[1] < 0) return AF3_ERR_BAD_STRIDE;
+	const dim3 grid = position::sums_shape(a, params->dtype == AF3_F32 ? 4 : 8);
+	if(params->workspace_bytes < (int64_t)grid.x * grid.y * grid.z * a.buckets * 4 || (reinterpret_cast<uintptr_t>(params->workspace) & 15)) return AF3_ERR_BAD_ARGUMENT;
+	if(const int dc = current_device_status(); dc != AF3_OK) return dc;
+	a.partial = static_cast<float*>(params->workspace);
+	const hipStream_t s = static_cast<hipStream_t>(hip_stream);
+	return params->dtype == AF3_F32 ? position::backward<float>(a, grid, s) : position::backward<uint16_t>(a, grid, s);
+}

@@ -330,6 +330,101 @@ int af3_silu_mul(const void* y, void* out, int64_t M, int64_t N, int32_t dtype, 
 int af3_linear(const void* x, const void* weight, void* out, int64_t M, int64_t K, int64_t N, int32_t dtype, void* hip_stream);
 
 /*
+ * Attention of queries to states of another length, one query token or many:
+ *     out = softmax(q . k^T * softmax_scale + bias, key_mask) . v
+ * No reference counterpart (the reference's attention has q_len == k_len, src/csrc/dot_product_attention.cpp:50-52, and no gradient).
+ *   q, out    : [B, H, Lq, D]; k, v: [B, Hkv, Lk, D], H a multiple of Hkv: query heads h / (H / Hkv) share a key head.  Element strides
+ *               for the first three axes, innermost stride 1, any alignment of the element type.  Inputs may have strides of 0.
+ *   bias      : [H, Lq, Lk] shared by the batch, of `dtype`, element strides for H and the query axis (0 repeats), key axis stride 1; NULL: none.
+ *               -inf drops that key for that query.  The lowest finite value does as the formula says: a row of nothing else weights its
+ *               live keys alike.  NaN or +inf at a live key makes the query's row NaN.
+ *   key_mask  : bytes, non-zero = attend, [B, Lk] with batch stride key_mask_stride_b (0: one row for the batch); NULL: all.  Nothing that k, v and
+ *               bias hold for a dropped key reaches a result.  A batch row whose keys are all dropped yields the mean of its V rows.
+ *               A query whose live keys are all dropped by the bias yields zeros.
+ *   dtype     : AF3_BF16 (bf16 products, fp32 accumulation and softmax) or AF3_F32 (fp32 throughout), of q, k, v, bias, out.
+ *   stats     : optional, [B, H, Lq, 2] floats written for af3_cross_attention_backward (maximum in the softmax's units and 1 / sum).
+ *   workspace : af3_cross_attention_workspace_bytes() bytes, 16-byte aligned; NULL where that is 0.  Overwritten.
+ * B, H, Lq, Lk, D >= 1, D <= AF3_DPA_MAX_HEAD_DIM, Lq and Lk < 2^30, H * Lq < 2^31, B * H * ceil(Lq / 32) < 2^26.
+ */
+typedef struct af3_cross_attention_params {
+	const void*    q;
+	const void*    k;
+	const void*    v;
+	const void*    bias;
+	const uint8_t* key_mask;
+	void*          out;
+	float*         stats;
+	int64_t        B, H, Hkv, Lq, Lk, D;
+	int64_t        q_stride[3];
+	int64_t        k_stride[3];
+	int64_t        v_stride[3];
+	int64_t        out_stride[3];
+	int64_t        bias_stride[2];
+	int64_t        key_mask_stride_b;
+	int32_t        dtype;
+	float          softmax_scale;
+	void*          workspace;
+	int64_t        workspace_bytes;
+} af3_cross_attention_params;
+
+int     af3_cross_attention_forward(const af3_cross_attention_params* params, void* hip_stream);
+int64_t af3_cross_attention_workspace_bytes(const af3_cross_attention_params* params);   /* host only */
+
+/*
+ * Gradients of af3_cross_attention_forward.  `params` as in the forward call, with the `out` and `stats` that it wrote (its workspace is not
+ * used); grad_out [B, H, Lq, D] with strides, of `dtype`.  grad_q [B, H, Lq, D], grad_k, grad_v [B, Hkv, Lk, D] and grad_bias [H, Lq, Lk] (summed over
+ * the batch) are contiguous and written whole, zeros for dropped keys among it; NULL: not wanted.  No atomics: the same bits every time.
+ * workspace: af3_cross_attention_backward_workspace_bytes() bytes, 16-byte aligned, required.
+ */
+typedef struct af3_cross_attention_grads {
+	const void* grad_out;
+	int64_t     grad_out_stride[3];
+	void*       grad_q;
+	void*       grad_k;
+	void*       grad_v;
+	void*       grad_bias;
+	void*       workspace;
+	int64_t     workspace_bytes;
+} af3_cross_attention_grads;
+
+int     af3_cross_attention_backward(const af3_cross_attention_params* params, const af3_cross_attention_grads* grads, void* hip_stream);
+int64_t af3_cross_attention_backward_workspace_bytes(const af3_cross_attention_params* params);   /* host only */
+
+/*
+ * Learned relative position bias by buckets: out[h][q][k] = table[bucket(k_position - q_position)][h], contiguous [H, Lq, Lk] of `dtype`, the layout the
+ * attention entry points read; and its gradient, the sums by bucket of a gradient [H, Lq, Lk].  No reference counterpart.
+ * With d the distance, r = max_distance:
+ *   AF3_POSITION_LOG  : n = buckets (bidirectional: buckets / 2) per side; near = n / 2.  d < near: bucket d; from there
+ *                       near + floor((n - near) log(d / near) / log(r / near)), at most n - 1, exactly (no floating-point logarithm decides).
+ *                       Bidirectional: d = |k - q|, keys ahead of the query add n.  Otherwise d = max(q - k, 0).  near >= 1, r > near.
+ *   AF3_POSITION_CLIP : bidirectional: q - k limited to -r .. r, plus r (buckets == 2 r + 1); otherwise q - k limited to 0 .. r (buckets == r + 1).
+ * Positions are q_offset + 0, 1, 2, ... and 0, 1, 2, ..., or, where given, q_positions [Lq] and k_positions [Lk] (device memory, any 64-bit numbers).
+ * forward: table [buckets, H] with element strides, out.  backward: grad [H, Lq, Lk] with strides for H and q (key stride 1), out = the table's
+ * gradient [buckets, H] with table_stride, workspace of af3_position_bias_workspace_bytes() bytes, 16-byte aligned; sums in a fixed order.
+ * H <= 65535, Lq and Lk < 2^30, buckets <= AF3_POSITION_BIAS_MAX_BUCKETS, |q_offset| <= 2^62.
+ */
+#define AF3_POSITION_BIAS_MAX_BUCKETS 576
+typedef enum af3_position_scheme { AF3_POSITION_LOG = 0, AF3_POSITION_CLIP = 1 } af3_position_scheme;
+typedef struct af3_position_bias_params {
+	const void*    table;
+	void*          out;
+	const void*    grad;
+	const int64_t* q_positions;
+	const int64_t* k_positions;
+	int64_t        q_offset;
+	int64_t        table_stride[2];
+	int64_t        grad_stride[2];
+	int64_t        buckets, H, Lq, Lk, max_distance;
+	int32_t        scheme, bidirectional, dtype, reserved;
+	void*          workspace;
+	int64_t        workspace_bytes;
+} af3_position_bias_params;
+
+int     af3_position_bias_forward(const af3_position_bias_params* params, void* hip_stream);
+int     af3_position_bias_backward(const af3_position_bias_params* params, void* hip_stream);
+int64_t af3_position_bias_workspace_bytes(const af3_position_bias_params* params);   /* host only */
+
+/*
  * N-dimensional pad (ndim <= AF3_PAD_MAX_DIMS): copy src (shape src_shape, element strides
  * src_strides) into the low corner of a contiguous dst of shape dst_shape (>= src_shape in
  * every axis) and fill the rest with the 32-bit pattern `fill_bits` truncated to elem_size

@@ -1,0 +1,156 @@
+"""The C entry points of cross attention and of the relative position bias, as far as the host goes: layouts, refusals, workspaces.  No GPU."""
+import ctypes
+import math
+import os
+import subprocess
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+i64x2, i64x3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
+BASE = 1 << 40   # (addresses that nothing follows)
+
+
+def _cross(B=2, H=4, Hkv=2, Lq=50, Lk=70, D=32, **kw):
+    from af3_kernels_amd import _lib
+    p = _lib.CrossAttentionParams(q=BASE, k=2 * BASE, v=3 * BASE, out=4 * BASE, stats=5 * BASE, B=B, H=H, Hkv=Hkv, Lq=Lq, Lk=Lk, D=D,
+                                  q_stride=i64x3(H * Lq * D, Lq * D, D), k_stride=i64x3(Hkv * Lk * D, Lk * D, D), v_stride=i64x3(Hkv * Lk * D, Lk * D, D),
+                                  out_stride=i64x3(H * Lq * D, Lq * D, D), dtype=_lib.AF3_BF16, softmax_scale=0.25)
+    for name, value in kw.items():
+        setattr(p, name, value)
+    return p
+
+
+def _grads(**kw):
+    from af3_kernels_amd import _lib
+    g = _lib.CrossAttentionGrads(grad_out=6 * BASE, grad_out_stride=i64x3(6400, 1600, 32), grad_q=7 * BASE, grad_k=8 * BASE, grad_v=9 * BASE, workspace=10 * BASE, workspace_bytes=1 << 40)
+    for name, value in kw.items():
+        setattr(g, name, value)
+    return g
+
+
+def _position(buckets=32, H=4, Lq=10, Lk=20, scheme=0, bidirectional=1, max_distance=128, **kw):
+    from af3_kernels_amd import _lib
+    p = _lib.PositionBiasParams(table=BASE, out=2 * BASE, grad=3 * BASE, table_stride=i64x2(H, 1), grad_stride=i64x2(Lq * Lk, Lk), buckets=buckets, H=H, Lq=Lq, Lk=Lk,
+                                max_distance=max_distance, scheme=scheme, bidirectional=bidirectional, dtype=_lib.AF3_F32, workspace=4 * BASE, workspace_bytes=1 << 40)
+    for name, value in kw.items():
+        setattr(p, name, value)
+    return p
+
+
+def test_struct_mirrors_match_what_a_c_compiler_lays_out(tmp_path):
+    from af3_kernels_amd import _lib
+    mirrors = {"af3_cross_attention_params": _lib.CrossAttentionParams, "af3_cross_attention_grads": _lib.CrossAttentionGrads, "af3_position_bias_params": _lib.PositionBiasParams}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "af3_dpa.h"', "int main(void) {"]
+    for name, cls in mirrors.items():
+        lines.append(f'printf("{name} %zu\\n", sizeof({name}));')
+        lines += [f'printf("{name}.{f} %zu\\n", offsetof({name}, {f}));' for f, _ in cls._fields_]
+    lines.append('printf("buckets %d\\n", AF3_POSITION_BIAS_MAX_BUCKETS); return 0; }')
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines))
+    subprocess.run(["gcc", "-std=c99", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "layout")], check=True)
+    found = dict(l.rsplit(" ", 1) for l in subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.splitlines())
+    for name, cls in mirrors.items():
+        assert int(found[name]) == ctypes.sizeof(cls)
+        for f, _ in cls._fields_:
+            assert int(found[f"{name}.{f}"]) == getattr(cls, f).offset, (name, f)
+    assert int(found["buckets"]) == _lib.POSITION_BIAS_MAX_BUCKETS
+
+
+def test_cross_attention_validates_on_the_host():
+    from af3_kernels_amd import _lib
+    lib = _lib.load()
+    fwd = lambda p: lib.af3_cross_attention_forward(ctypes.byref(p), None)
+    assert lib.af3_cross_attention_forward(None, None) == -1
+    for name in ("q", "k", "v", "out"):
+        assert fwd(_cross(**{name: None})) == -1
+    assert fwd(_cross(dtype=_lib.AF3_FP8_E4M3)) == -2
+    for name in ("B", "H", "Hkv", "Lq", "Lk", "D"):
+        for value in (0, -1):
+            assert fwd(_cross(**{name: value})) in (-3, -5), name
+    assert fwd(_cross(H=4, Hkv=3)) == -3
+    assert fwd(_cross(Lk=1 << 30)) == -3
+    assert fwd(_cross(B=1 << 24)) == -3
+    assert fwd(_cross(Lq=1 << 29, H=64, Hkv=64)) == -3
+    assert fwd(_cross(D=129)) == -5
+    for name in ("q_stride", "k_stride", "v_stride", "out_stride"):
+        assert fwd(_cross(**{name: i64x3(-1, 32, 32)})) == -4
+    assert fwd(_cross(out_stride=i64x3(6400, 1600, 31))) == -4
+    assert fwd(_cross(bias=BASE, bias_stride=i64x2(-1, 1))) == -4
+    assert fwd(_cross(key_mask=BASE, key_mask_stride_b=-1)) == -4
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        assert fwd(_cross(softmax_scale=scale)) == -7
+    # one query over many keys needs room for the parts' results
+    long = _cross(B=1, H=2, Lq=1, Lk=40000)
+    need = lib.af3_cross_attention_workspace_bytes(ctypes.byref(long))
+    assert need > 0 and need % 4 == 0 and fwd(long) == -7
+    long.workspace, long.workspace_bytes = BASE, need - 1
+    assert fwd(long) == -7
+    long.workspace, long.workspace_bytes = BASE + 4, need
+    assert fwd(long) == -7
+    assert lib.af3_cross_attention_workspace_bytes(ctypes.byref(_cross(B=64, H=16, Hkv=16, Lq=512))) == 0
+    assert lib.af3_cross_attention_workspace_bytes(ctypes.byref(_cross(D=0))) == -3
+
+
+def test_cross_attention_backward_validates_on_the_host():
+    from af3_kernels_amd import _lib
+    lib = _lib.load()
+    bwd = lambda p, g: lib.af3_cross_attention_backward(ctypes.byref(p), ctypes.byref(g), None)
+    assert lib.af3_cross_attention_backward(ctypes.byref(_cross()), None, None) == -1
+    assert bwd(_cross(stats=None), _grads()) == -1
+    assert bwd(_cross(), _grads(grad_out=None)) == -1
+    assert bwd(_cross(), _grads(grad_q=None, grad_k=None, grad_v=None)) == -1
+    assert bwd(_cross(), _grads(grad_bias=BASE)) == -1          # the gradient of a bias that is not there
+    assert bwd(_cross(), _grads(grad_out_stride=i64x3(1, -1, 1))) == -4
+    assert bwd(_cross(Lq=0), _grads()) == -3
+    need = lib.af3_cross_attention_backward_workspace_bytes(ctypes.byref(_cross()))
+    assert need >= 2 * 4 * 50 * 4
+    assert bwd(_cross(), _grads(workspace_bytes=need - 1)) == -7
+    assert bwd(_cross(), _grads(workspace=None)) == -7
+    assert bwd(_cross(), _grads(workspace=BASE + 8)) == -7
+    assert bwd(_cross(H=1 << 15, Hkv=1, B=1, Lq=1 << 15, Lk=1 << 28, bias=BASE), _grads(grad_bias=BASE)) == -3
+
+
+def test_position_bias_validates_on_the_host():
+    from af3_kernels_amd import _lib
+    lib = _lib.load()
+    fwd, bwd = (lambda p, f=f: f(ctypes.byref(p), None) for f in (lib.af3_position_bias_forward, lib.af3_position_bias_backward))
+    for call in (fwd, bwd):
+        assert call(_position(dtype=_lib.AF3_FP8_E4M3)) == -2
+        for bad in ({"buckets": 0}, {"buckets": 577}, {"H": 0}, {"H": 1 << 16}, {"Lq": 0}, {"Lk": 1 << 30}):
+            assert call(_position(**bad)) == -3, bad
+        assert call(_position(table_stride=i64x2(-1, 1))) == -4
+        for bad in ({"max_distance": 0}, {"max_distance": 1 << 30}, {"max_distance": 8}, {"scheme": 2}, {"buckets": 31}, {"buckets": 2}, {"buckets": 1, "bidirectional": 0},
+                    {"scheme": 1, "max_distance": 32}, {"scheme": 1, "max_distance": 32, "buckets": 64}, {"q_offset": (1 << 62) + 1}, {"q_offset": -(1 << 62) - 1}):
+            assert call(_position(**bad)) == -7, bad
+        assert call(_position(out=None)) == -1
+    assert lib.af3_position_bias_forward(None, None) == -1 and lib.af3_position_bias_backward(None, None) == -1
+    assert fwd(_position(table=None)) == -1
+    assert bwd(_position(grad=None)) == -1 and bwd(_position(workspace=None)) == -1
+    assert bwd(_position(grad_stride=i64x2(-1, 1))) == -4
+    need = lib.af3_position_bias_workspace_bytes(ctypes.byref(_position()))
+    assert need > 0 and bwd(_position(workspace_bytes=need - 1)) == -7 and bwd(_position(workspace=BASE + 4)) == -7
+
+
+def test_wrappers_reject_cpu_tensors():
+    import af3_kernels_amd as af3
+    q = torch.zeros(1, 1, 2, 8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        af3.cross_attention(q, q, q)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        af3.relative_position_bias(torch.zeros(32, 1), 2, 2)
+
+
+def test_a_stale_library_says_so_and_does_not_keep_the_package_from_being_imported(tmp_path):
+    """A library built before a symbol was added: importing works (or `python -m af3_kernels_amd.build` could not), calls raise."""
+    import shutil
+    import sys
+    copy = tmp_path / "af3_kernels_amd"
+    shutil.copytree(os.path.join(ROOT, "af3_kernels_amd"), copy, ignore=shutil.ignore_patterns("csrc", "*.so", "__pycache__"))
+    (tmp_path / "old.c").write_text("int af3_abi_version(void) { return 4; }")
+    subprocess.run(["gcc", "-shared", "-fPIC", str(tmp_path / "old.c"), "-o", str(copy / "libaf3_dpa.so")], check=True)
+    (copy / "_host.so").write_bytes(b"")
+    code = "import af3_kernels_amd as a\ntry:\n    a._lib.load()\nexcept ImportError as e:\n    print('said:', 'rebuild' in str(e))"
+    r = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True)
+    assert r.returncode == 0 and "said: True" in r.stdout, r.stdout + r.stderr
