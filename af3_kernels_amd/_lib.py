@@ -50,7 +50,7 @@ class GridAttentionParams(ctypes.Structure):
 class CrossAttentionParams(ctypes.Structure):
     """Mirror of struct af3_cross_attention_params."""
     _fields_ = [
-        ("q", vp), ("k", vp), ("v", vp), ("bias", vp), ("key_mask", vp), ("out", vp), ("stats", vp),
+        ("q", vp), ("k", vp), ("v", vp), ("bias", vp), ("key_mask", vp), ("out", vp), ("stats", vp), ("out_residual", vp),
         ("B", i64), ("H", i64), ("Hkv", i64), ("Lq", i64), ("Lk", i64), ("D", i64),
         ("q_stride", i64 * 3), ("k_stride", i64 * 3), ("v_stride", i64 * 3), ("out_stride", i64 * 3),
         ("bias_stride", i64 * 2), ("key_mask_stride_b", i64),

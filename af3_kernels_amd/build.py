@@ -23,6 +23,9 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # the feature, which is harmless.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Wall", "-Wno-unused-function",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# Results of matrix instructions in ordinary vector registers: with the accumulators in the other file the cross-attention kernels copied each of them
+# out and back around every product (64 of 154 instructions of the forward pass's inner part).
+EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("cross_attention.hip", "cross_attention_grad.hip")}
 
 
 def _stale(target, deps):
@@ -36,7 +39,7 @@ def _compile(src, force):
     obj = os.path.join(OBJDIR, src + ".o")
     path = os.path.join(CSRC, src)
     if force or _stale(obj, [path] + HEADERS):
-        r = subprocess.run([HIPCC] + FLAGS + ["-c", path, "-o", obj], capture_output=True, text=True)
+        r = subprocess.run([HIPCC] + FLAGS + EXTRA_FLAGS.get(src, []) + ["-c", path, "-o", obj], capture_output=True, text=True)
         msgs = "\n".join(l for l in (r.stdout + r.stderr).splitlines() if "packed-fp32-ops" not in l and l.strip())
         if r.returncode != 0:
             raise RuntimeError(f"hipcc failed on {src}:\n{msgs}")

@@ -31,7 +31,7 @@ def _inner_contig(t):
 
 
 # ---- attention ----------------------------------------------------------------------------------------------------------
-def _fill(q, k, v, keep, bias, out, stats, scale) -> CrossAttentionParams:
+def _fill(q, k, v, keep, bias, out, stats, lost, scale) -> CrossAttentionParams:
     p = CrossAttentionParams()
     p.q, p.k, p.v, p.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     p.B, p.H, p.Lq, p.D = q.shape
@@ -43,17 +43,20 @@ def _fill(q, k, v, keep, bias, out, stats, scale) -> CrossAttentionParams:
         p.key_mask, p.key_mask_stride_b = keep.data_ptr(), 0 if keep.shape[0] == 1 else keep.stride(0)
     if stats is not None:
         p.stats = stats.data_ptr()
+    if lost is not None:
+        p.out_residual = lost.data_ptr()
     p.dtype, p.softmax_scale = _DTYPES[q.dtype], scale
     return p
 
 
 def _forward(q, k, v, keep, bias, scale, want_stats):
-    """(out, stats): stats [B, H, Lq, 2] where the gradient will be asked for."""
+    """(out, stats, lost): where the gradient will be asked for, stats [B, H, Lq, 2] and what out lost by its rounding to bfloat16."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if out.numel() == 0 or k.shape[2] == 0:
-        return out.zero_(), None
+        return out.zero_(), None, None
     stats = torch.empty(*q.shape[:3], 2, dtype=torch.float32, device=q.device) if want_stats else None
-    p = _fill(q, k, v, keep, bias, out, stats, scale)
+    lost = torch.empty_like(out) if want_stats and q.dtype == torch.bfloat16 else None
+    p = _fill(q, k, v, keep, bias, out, stats, lost, scale)
     lib = _lib.load()
     with ops._on_device(q.device):
         need = lib.af3_cross_attention_workspace_bytes(ctypes.byref(p))
@@ -61,17 +64,17 @@ def _forward(q, k, v, keep, bias, scale, want_stats):
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             p.workspace, p.workspace_bytes = ws.data_ptr(), need
         _lib.check(lib.af3_cross_attention_forward(ctypes.byref(p), ops._stream_ptr(q.device)), "af3_cross_attention_forward")
-    return out, stats
+    return out, stats, lost
 
 
-def _backward(grad, q, k, v, keep, bias, out, stats, scale, wants):
+def _backward(grad, q, k, v, keep, bias, out, stats, lost, scale, wants):
     """Gradients of q, k, v and bias, None for those not wanted."""
     shapes = (q.shape, k.shape, v.shape, None if bias is None else (q.shape[1], q.shape[2], k.shape[2]))
     if stats is None:
         return tuple(torch.zeros(s, dtype=q.dtype, device=q.device) if w else None for s, w in zip(shapes, wants))
     grads = tuple(torch.empty(s, dtype=q.dtype, device=q.device) if w else None for s, w in zip(shapes, wants))
     grad = _inner_contig(grad)
-    p = _fill(q, k, v, keep, bias, out, stats, scale)
+    p = _fill(q, k, v, keep, bias, out, stats, lost, scale)
     g = CrossAttentionGrads()
     g.grad_out, g.grad_out_stride = grad.data_ptr(), _i64x3(*grad.stride()[:3])
     g.grad_q, g.grad_k, g.grad_v, g.grad_bias = (0 if t is None else t.data_ptr() for t in grads)
@@ -87,17 +90,17 @@ def _backward(grad, q, k, v, keep, bias, out, stats, scale, wants):
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, keep, bias, scale):
-        out, stats = _forward(q, k, v, keep, bias, scale, True)
-        ctx.save_for_backward(q, k, v, keep, bias, out, stats)
+        out, stats, lost = _forward(q, k, v, keep, bias, scale, True)
+        ctx.save_for_backward(q, k, v, keep, bias, out, stats, lost)
         ctx.scale = scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, keep, bias, out, stats = ctx.saved_tensors
+        q, k, v, keep, bias, out, stats, lost = ctx.saved_tensors
         needs = ctx.needs_input_grad
-        dq, dk, dv, dbias = _backward(grad, q, k, v, keep, bias, out, stats, ctx.scale, (needs[0], needs[1], needs[2], needs[4]))
+        dq, dk, dv, dbias = _backward(grad, q, k, v, keep, bias, out, stats, lost, ctx.scale, (needs[0], needs[1], needs[2], needs[4]))
         return dq, dk, dv, None, dbias, None
 
 

@@ -22,6 +22,18 @@ struct forward_args {
 	float*   part_stat;            // ... [splits][B * Hkv * G * Lq][2] (maximum, sum); maximum -inf: no live key in the part
 };
 
+// what a result loses by its rounding to bf16, itself as bf16: the gradient's delta then has the result to 16 bits
+template <typename T>
+__device__ __forceinline__ void store_residual(const af3_cross_attention_params& p, int64_t row, int d, const float (&v)[16]) {
+	if constexpr(sizeof(T) == 2) {
+		if(!p.out_residual) return;
+		float r[16];
+#pragma unroll
+		for(int i = 0; i < 16; i++) r[i] = v[i] - kind<T>::value(kind<T>::bits(v[i]));
+		store_row16(static_cast<T*>(p.out_residual) + row, d, (int)p.D, r);
+	}
+}
+
 // KW: wavefronts that share 32 query rows and each take 32 keys of a tile (1: a wavefront takes all 64 keys of one)
 template <typename T, int DP, int KW>
 struct forward_shape {
@@ -144,31 +156,47 @@ __global__ void __launch_bounds__(THREADS) cross_forward_kernel(forward_args a) 
 	l += other_half(l);
 
 	const int64_t bh = b * p.Hkv + hk, n_rows = p.B * p.Hkv * rows;
-	if(!any) {   // no live key here: the mean of the values, or left to the joining kernel
+	if(!any) {
+		// No live key here.  Where the batch row has one elsewhere that is all; where it has none, its result is the mean of the values: this part's sum
+		// of them, which is the same for all rows.
 		if(a.splits > 1) {
-			if(ok && kwave == 0 && half == 0) a.part_stat[2 * (split * n_rows + bh * rows + R)] = -INFINITY;
-			return;
+			bool elsewhere = false;
+			for(int64_t key = threadIdx.x; key < p.Lk; key += THREADS) elsewhere = elsewhere || mask[key] != 0;   // (no mask: there is a live key)
+			if(__syncthreads_or(elsewhere)) {
+				if(ok && kwave == 0 && half == 0) a.part_stat[2 * (split * n_rows + bh * rows + R)] = -INFINITY, a.part_stat[2 * (split * n_rows + bh * rows + R) + 1] = 0.f;
+				return;
+			}
 		}
-		float* const sums = reinterpret_cast<float*>(smem);   // [THREADS / DP][DP]
+		const int64_t first = (int64_t)split * a.part;
+		float* const  sums = reinterpret_cast<float*>(smem);   // [THREADS / DP][DP]
 		constexpr int PARTS = THREADS / DP;
 		const int     d = threadIdx.x % DP, part = threadIdx.x / DP;
 		float         sum = 0.f;
-		if(part < PARTS && d < D)
-			for(int64_t key = part; key < p.Lk; key += PARTS) sum += kind<T>::value(vb[key * p.v_stride[2] + d]);
+		if(part < PARTS && d < D) {
+#pragma unroll 4
+			for(int64_t key = first + part; key < last; key += PARTS) sum += kind<T>::value(vb[key * p.v_stride[2] + d]);
+		}
 		if(part < PARTS) sums[part * DP + d] = sum;
 		__syncthreads();
 		if(!ok || kwave != 0) return;
+		const int64_t at = split * n_rows + bh * rows + R;
+		if(a.splits > 1 && half == 0) a.part_stat[2 * at] = -INFINITY, a.part_stat[2 * at + 1] = (float)(last - first);
 		T* const out = static_cast<T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2];
 		for(int db = 0; db < TL::BLOCKS; db++) {
 			float v[16];
 			for(int r = 0; r < 16; r++) {
 				v[r] = 0.f;
 				for(int i = 0; i < PARTS; i++) v[r] += sums[i * DP + 32 * db + 16 * half + r];
-				v[r] /= (float)p.Lk;
 			}
+			if(a.splits > 1) {
+				store_row16(a.part_out + at * D, 32 * db + 16 * half, D, v);
+				continue;
+			}
+			for(int r = 0; r < 16; r++) v[r] /= (float)p.Lk;
 			store_row16(out, 32 * db + 16 * half, D, v);
+			store_residual<T>(p, ((b * p.H + h) * p.Lq + qi) * D, 32 * db + 16 * half, v);
 		}
-		if(p.stats && half == 0) {
+		if(p.stats && half == 0 && a.splits == 1) {
 			float* const st = p.stats + 2 * ((b * p.H + h) * p.Lq + qi);
 			st[0] = -INFINITY, st[1] = 1.f / (float)p.Lk;
 		}
@@ -235,48 +263,62 @@ __global__ void __launch_bounds__(THREADS) cross_forward_kernel(forward_args a) 
 #pragma unroll
 		for(int r = 0; r < 16; r++) v[r] = o[db][r] * inv;
 		store_row16(out, 32 * db + 16 * half, D, v);
+		store_residual<T>(p, ((b * p.H + h) * p.Lq + qi) * D, 32 * db + 16 * half, v);
 	}
 }
 
-// The parts of the key axis joined: one wavefront per query row, columns over its lanes.
+// The parts of the key axis joined: one wavefront per query row, columns over its lanes.  The parts' maxima and sums come one to a lane (64 parts at
+// most), so that the parts' results, eight of them in flight, wait for nothing but each other.
+constexpr int MAX_PARTS = 64;
 template <typename T>
 __global__ void __launch_bounds__(THREADS) cross_join_kernel(forward_args a) {
 	const af3_cross_attention_params& p = a.p;
 	const int64_t G = p.H / p.Hkv, rows = G * p.Lq, n_rows = p.B * p.Hkv * rows;
-	const int     lane = threadIdx.x & 63, D = (int)p.D;
+	const int     lane = threadIdx.x & 63, D = (int)p.D, splits = (int)a.splits;
 	const int64_t at = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
 	if(at >= n_rows) return;
 	const int64_t R = at % rows, bh = at / rows, hk = bh % p.Hkv, b = bh / p.Hkv, g = R / p.Lq, qi = R - g * p.Lq, h = hk * G + g;
-	float top = -INFINITY;
-	for(uint32_t s = 0; s < a.splits; s++) top = maximum(top, a.part_stat[2 * (s * n_rows + at)]);
-	T* const     out = static_cast<T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2];
-	float* const st = p.stats ? p.stats + 2 * ((b * p.H + h) * p.Lq + qi) : nullptr;
-	if(top == -INFINITY) {   // no live key in the batch row: the mean of the values
-		const T* const v = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
-		for(int d = lane; d < D; d += 64) {
-			float sum = 0.f;
-			for(int64_t key = 0; key < p.Lk; key++) sum += kind<T>::value(v[key * p.v_stride[2] + d]);
-			out[d] = kind<T>::bits(sum / (float)p.Lk);
-		}
-		if(st && lane == 0) st[0] = -INFINITY, st[1] = 1.f / (float)p.Lk;
-		return;
-	}
-	float sum = 0.f, o[2] = {0.f, 0.f};
-	for(uint32_t s = 0; s < a.splits; s++) {
-		const int64_t i = s * n_rows + at;
-		const float   m = a.part_stat[2 * i];
-		if(m == -INFINITY) continue;   // (that part wrote nothing else)
-		const float by = __builtin_amdgcn_exp2f((m - top) * a.factor);
-		sum += a.part_stat[2 * i + 1] * by;
+	float m = -INFINITY, l = 0.f;
+	if(lane < splits) m = a.part_stat[2 * (lane * n_rows + at)], l = a.part_stat[2 * (lane * n_rows + at) + 1];
+	float top = m;
 #pragma unroll
-		for(int k = 0; k < 2; k++)
-			if(lane + 64 * k < D) o[k] += a.part_out[i * D + lane + 64 * k] * by;
+	for(int i = 32; i; i >>= 1) top = maximum(top, __shfl_xor(top, i));
+	// (-inf throughout: no live key in the batch row, and l keys of even weight in a part)
+	const bool dead = top == -INFINITY;
+	const float weight = dead ? 1.f : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.factor);
+	float sum = l * weight;
+#pragma unroll
+	for(int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
+	float o[2] = {0.f, 0.f};
+	for(int s0 = 0; s0 < splits; s0 += 8) {
+		float x[8][2];
+#pragma unroll
+		for(int s = 0; s < 8; s++)
+#pragma unroll
+			for(int k = 0; k < 2; k++) {
+				x[s][k] = 0.f;
+				if(s0 + s < splits && lane + 64 * k < D) x[s][k] = a.part_out[((s0 + s) * n_rows + at) * D + lane + 64 * k];
+			}
+#pragma unroll
+		for(int s = 0; s < 8; s++) {
+			const float w = __shfl(weight, (s0 + s) & 63);
+			const bool  none = !dead && __shfl(m, (s0 + s) & 63) == -INFINITY;   // (that part wrote nothing)
+#pragma unroll
+			for(int k = 0; k < 2; k++) o[k] += none || s0 + s >= splits ? 0.f : x[s][k] * w;
+		}
 	}
-	const float inv = sum == 0.f ? 0.f : 1.f / sum;
+	const float  inv = sum == 0.f ? 0.f : 1.f / sum;
+	T* const     out = static_cast<T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2];
+	const int64_t row = (b * p.H + h) * p.Lq + qi;
 #pragma unroll
 	for(int k = 0; k < 2; k++)
-		if(lane + 64 * k < D) out[lane + 64 * k] = kind<T>::bits(o[k] * inv);
-	if(st && lane == 0) st[0] = top, st[1] = inv;
+		if(lane + 64 * k < D) {
+			const float v = o[k] * inv;
+			out[lane + 64 * k] = kind<T>::bits(v);
+			if constexpr(sizeof(T) == 2)
+				if(p.out_residual) static_cast<T*>(p.out_residual)[row * D + lane + 64 * k] = kind<T>::bits(v - kind<T>::value(kind<T>::bits(v)));
+		}
+	if(p.stats && lane == 0) p.stats[2 * row] = dead ? -INFINITY : top, p.stats[2 * row + 1] = inv;
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
@@ -295,6 +337,7 @@ plan forward_plan(const af3_cross_attention_params& p) {
 	const int64_t kt = f.kw == 4 ? 128 : 64, key_tiles = (p.Lk + kt - 1) / kt, busy = groups * f.row_tiles;
 	int64_t       splits = busy >= 512 ? 1 : (512 + busy - 1) / busy;
 	if(splits > (key_tiles + 1) / 2) splits = (key_tiles + 1) / 2;   // (at least two tiles to a part)
+	if(splits > MAX_PARTS) splits = MAX_PARTS;
 	if(splits < 1) splits = 1;
 	const int64_t per = (key_tiles + splits - 1) / splits;
 	f.part   = per * kt;

@@ -25,7 +25,8 @@ struct grad_args {
 	float    factor;
 	int32_t  whole;
 	float*   delta;           // [B, H, Lq]
-	float*   partial;         // dq [splits][B H Lq][D]; dkv [splits][2][B Hkv Lk][D]
+	float*   partial;         // dq: [splits][B H Lq][D]; dkv: [splits][2][B Hkv Lk][D]
+	float *  dq_space, *dkv_space;
 };
 
 // the sum of the wavefronts' results of equal shape, wavefront w keeps the blocks of columns that are w modulo N; `mine`: N tables of 32 x (DP + 4)
@@ -50,6 +51,27 @@ __device__ __forceinline__ void add_up(float* tables, int w, int lane, f32x16 (&
 				for(int e = 0; e < 4; e++) o[db][4 * i + e] += v[e];
 			}
 	}
+}
+
+// delta of a lane's query row from the lane's half of the gradient of out; the other half-wave has the other half
+template <typename T, int DP, int N>
+__device__ __forceinline__ float row_delta(const grad_args& a, const u32x4 (&gf)[N], int64_t b, int64_t h, int64_t qi, bool ok, int lane) {
+	const af3_cross_attention_params& p = a.p;
+	float delta = 0.f;
+	u32x4 of[N];
+	auto  add = [&] {
+#pragma unroll
+		for(int s = 0; s < N; s++)
+#pragma unroll
+			for(int e = 0; e < kind<T>::E; e++) delta = __builtin_fmaf(kind<T>::at(gf[s], e), kind<T>::at(of[s], e), delta);
+	};
+	load_operand<T, DP>(of, static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2], ok, (int)p.D, lane);
+	add();
+	if(sizeof(T) == 2 && p.out_residual) {
+		load_operand<T, DP>(of, static_cast<const T*>(p.out_residual) + ((b * p.H + h) * p.Lq + qi) * p.D, ok, (int)p.D, lane);
+		add();
+	}
+	return delta + other_half(delta);
 }
 
 // ---- dQ ----
@@ -88,16 +110,7 @@ __global__ void __launch_bounds__(THREADS) cross_dq_kernel(grad_args a) {
 	u32x4 qf[TL::STEPS], gf[TL::STEPS];
 	load_operand<T, DP>(qf, static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1] + qi * p.q_stride[2], ok, D, lane);
 	load_operand<T, DP>(gf, static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1] + qi * a.g.grad_out_stride[2], ok, D, lane);
-	float delta = 0.f;
-	{
-		u32x4 of[TL::STEPS];
-		load_operand<T, DP>(of, static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2], ok, D, lane);
-#pragma unroll
-		for(int s = 0; s < TL::STEPS; s++)
-#pragma unroll
-			for(int e = 0; e < E; e++) delta = __builtin_fmaf(kind<T>::at(gf[s], e), kind<T>::at(of[s], e), delta);
-		delta += other_half(delta);
-	}
+	const float delta = row_delta<T, DP>(a, gf, b, h, qi, ok, lane);
 	if(ok && half == 0 && kwave == 0 && split == 0) a.delta[row] = delta;
 	const float  m = ok ? p.stats[2 * row] : 0.f, inv = ok ? p.stats[2 * row + 1] : 0.f;
 	const T* const kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[1];
@@ -184,21 +197,18 @@ __global__ void __launch_bounds__(THREADS) cross_dq_kernel(grad_args a) {
 	}
 }
 
-// delta alone, for calls that want no gradient of q: one wavefront per row
-template <typename T>
+// delta alone, for calls that want no gradient of q: 32 rows per wavefront, added up as cross_dq_kernel does
+template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS) cross_delta_kernel(grad_args a) {
 	const af3_cross_attention_params& p = a.p;
-	const int64_t row = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
 	const int     lane = threadIdx.x & 63;
-	if(row >= p.B * p.H * p.Lq) return;
-	const int64_t qi = row % p.Lq, h = row / p.Lq % p.H, b = row / p.Lq / p.H;
-	const T* const g = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1] + qi * a.g.grad_out_stride[2];
-	const T* const o = static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2];
-	float sum = 0.f;
-	for(int64_t d = lane; d < p.D; d += 64) sum = __builtin_fmaf(kind<T>::value(g[d]), kind<T>::value(o[d]), sum);
-#pragma unroll
-	for(int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
-	if(lane == 0) a.delta[row] = sum;
+	const int64_t row = ((int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6)) * 32 + (lane & 31);
+	const bool    ok = row < p.B * p.H * p.Lq;
+	const int64_t qi = ok ? row % p.Lq : 0, h = ok ? row / p.Lq % p.H : 0, b = ok ? row / p.Lq / p.H : 0;
+	u32x4 gf[tile<T, DP>::STEPS];
+	load_operand<T, DP>(gf, static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1] + qi * a.g.grad_out_stride[2], ok, (int)p.D, lane);
+	const float delta = row_delta<T, DP>(a, gf, b, h, qi, ok, lane);
+	if(ok && lane < 32) a.delta[row] = delta;
 }
 
 // ---- dK, dV ----
@@ -348,25 +358,34 @@ __global__ void __launch_bounds__(THREADS) cross_dkv_kernel(grad_args a) {
 	}
 }
 
-// The parts' sums added in order: n elements per part, parts `step` elements apart.
+// The parts' sums added in order, of up to three results at once (a result of one part was written where it belongs).
+struct parts {
+	const float* partial[3];
+	int64_t      step[3], n[3];   // elements from one part to the next, elements
+	uint32_t     splits[3], blocks[3];
+	void*        out[3];
+};
 template <typename T>
-__global__ void __launch_bounds__(THREADS) cross_sum_kernel(const float* partial, int64_t step, uint32_t splits, T* out, int64_t n) {
-	const int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4;
+__global__ void __launch_bounds__(THREADS) cross_sum_kernel(parts a) {
+	uint32_t block = blockIdx.x;
+	int      which = 0;
+	while(which < 2 && block >= a.blocks[which]) block -= a.blocks[which++];
+	const int64_t  i = ((int64_t)block * THREADS + threadIdx.x) * 4, n = a.n[which], step = a.step[which];
+	const uint32_t splits = a.splits[which];
+	const float*   at = a.partial[which] + i;
+	T* const       out = static_cast<T*>(a.out[which]) + i;
 	if(i >= n) return;
-	float v[4] = {0.f, 0.f, 0.f, 0.f};
 	if(i + 4 <= n) {
-		for(uint32_t s = 0; s < splits; s++) {
-			const f32x4 x = *reinterpret_cast<const f32x4_any*>(partial + s * step + i);
+		f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+		for(uint32_t s = 0; s < splits; s++, at += step) sum += *reinterpret_cast<const f32x4_any*>(at);
 #pragma unroll
-			for(int e = 0; e < 4; e++) v[e] += x[e];
-		}
-#pragma unroll
-		for(int e = 0; e < 4; e++) out[i + e] = kind<T>::bits(v[e]);
+		for(int e = 0; e < 4; e++) out[e] = kind<T>::bits(sum[e]);
 	} else {
 		for(int e = 0; i + e < n; e++) {
 			float x = 0.f;
-			for(uint32_t s = 0; s < splits; s++) x += partial[s * step + i + e];
-			out[i + e] = kind<T>::bits(x);
+			for(uint32_t s = 0; s < splits; s++) x += at[s * step + e];
+			out[e] = kind<T>::bits(x);
 		}
 	}
 }
@@ -505,7 +524,7 @@ grad_space grad_workspace(const af3_cross_attention_params& p) {
 	w.delta = over(p.B * p.H * p.Lq, 4) * 4;
 	w.dq    = q.splits > 1 ? over(q.splits * p.B * p.H * p.Lq * p.D, 4) * 4 : 0;
 	w.dkv   = kv.splits > 1 ? 2 * (int64_t)kv.splits * p.B * p.Hkv * p.Lk * p.D : 0;
-	w.bytes = (w.delta + (w.dq > w.dkv ? w.dq : w.dkv)) * 4;   // (one after the other on the stream)
+	w.bytes = (w.delta + w.dq + w.dkv) * 4;
 	return w;
 }
 
@@ -519,40 +538,49 @@ int launch(K kernel, int lds, uint32_t grid, const grad_args& a, hipStream_t s) 
 	return launch_status();
 }
 
-template <typename T>
-int sum_parts(const float* partial, int64_t step, uint32_t splits, void* out, int64_t n, hipStream_t s) {
-	hipLaunchKernelGGL(cross_sum_kernel<T>, dim3((uint32_t)over(n, 4 * THREADS)), dim3(THREADS), 0, s, partial, step, splits, static_cast<T*>(out), n);
-	return launch_status();
-}
-
 template <typename T, int DP>
 int backward(grad_args a, hipStream_t s) {
 	const af3_cross_attention_params& p = a.p;
 	const int64_t n_rows = p.B * p.H * p.Lq, n_keys = p.B * p.Hkv * p.Lk;
+	parts    sums{};
+	int      n_sums = 0;
+	uint32_t sum_blocks = 0;
+	auto add = [&](const float* partial, int64_t step, uint32_t splits, void* out, int64_t n) {
+		if(!out) return;
+		sums.partial[n_sums] = partial, sums.step[n_sums] = step, sums.n[n_sums] = n, sums.splits[n_sums] = splits, sums.out[n_sums] = out;
+		sum_blocks += sums.blocks[n_sums] = (uint32_t)over(n, 4 * THREADS);
+		n_sums++;
+	};
 	if(a.g.grad_q) {
 		const cut c = dq_cut(p);
-		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part;
+		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part, a.partial = a.dq_space;
 		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * c.tiles * c.splits;
 		int rc;
 		if(c.shared) rc = p.bias ? launch(cross_dq_kernel<T, DP, 4, true>, dq_shape<T, DP, 4>::LDS, grid, a, s) : launch(cross_dq_kernel<T, DP, 4, false>, dq_shape<T, DP, 4>::LDS, grid, a, s);
 		else rc = p.bias ? launch(cross_dq_kernel<T, DP, 1, true>, dq_shape<T, DP, 1>::LDS, grid, a, s) : launch(cross_dq_kernel<T, DP, 1, false>, dq_shape<T, DP, 1>::LDS, grid, a, s);
-		if(rc == AF3_OK && c.splits > 1) rc = sum_parts<T>(a.partial, n_rows * p.D, c.splits, a.g.grad_q, n_rows * p.D, s);
 		if(rc != AF3_OK) return rc;
+		if(c.splits > 1) add(a.partial, n_rows * p.D, c.splits, a.g.grad_q, n_rows * p.D);
 	} else {
-		hipLaunchKernelGGL(cross_delta_kernel<T>, dim3((uint32_t)over(n_rows, WAVES)), dim3(THREADS), 0, s, a);
+		hipLaunchKernelGGL((cross_delta_kernel<T, DP>), dim3((uint32_t)over(n_rows, 32 * WAVES)), dim3(THREADS), 0, s, a);
 		if(const int rc = launch_status(); rc != AF3_OK) return rc;
 	}
 	if(a.g.grad_k || a.g.grad_v) {
 		const cut c = dkv_cut(p);
-		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part;
+		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part, a.partial = a.dkv_space;
 		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * c.tiles * c.splits;
 		int rc = AF3_ERR_LAUNCH;
 		if constexpr(sizeof(T) == 2 || DP <= 64)
 			if(c.shared) rc = p.bias ? launch(cross_dkv_kernel<T, DP, 4, true>, dkv_shape<T, DP, 4>::LDS, grid, a, s) : launch(cross_dkv_kernel<T, DP, 4, false>, dkv_shape<T, DP, 4>::LDS, grid, a, s);
 		if(!c.shared) rc = p.bias ? launch(cross_dkv_kernel<T, DP, 1, true>, dkv_shape<T, DP, 1>::LDS, grid, a, s) : launch(cross_dkv_kernel<T, DP, 1, false>, dkv_shape<T, DP, 1>::LDS, grid, a, s);
-		if(rc == AF3_OK && c.splits > 1 && a.g.grad_k) rc = sum_parts<T>(a.partial, 2 * n_keys * p.D, c.splits, a.g.grad_k, n_keys * p.D, s);
-		if(rc == AF3_OK && c.splits > 1 && a.g.grad_v) rc = sum_parts<T>(a.partial + n_keys * p.D, 2 * n_keys * p.D, c.splits, a.g.grad_v, n_keys * p.D, s);
 		if(rc != AF3_OK) return rc;
+		if(c.splits > 1) {
+			add(a.partial, 2 * n_keys * p.D, c.splits, a.g.grad_k, n_keys * p.D);
+			add(a.partial + n_keys * p.D, 2 * n_keys * p.D, c.splits, a.g.grad_v, n_keys * p.D);
+		}
+	}
+	if(n_sums) {
+		hipLaunchKernelGGL(cross_sum_kernel<T>, dim3(sum_blocks), dim3(THREADS), 0, s, sums);
+		if(const int rc = launch_status(); rc != AF3_OK) return rc;
 	}
 	if(a.g.grad_bias) {
 		using S = dbias_shape<T, DP>;
@@ -600,7 +628,7 @@ extern "C" int af3_cross_attention_backward(const af3_cross_attention_params* pa
 	a.factor  = params->bias ? LOG2E : params->softmax_scale * LOG2E;
 	a.whole   = params->D * (params->dtype == AF3_F32 ? 4 : 2) % 16 == 0;
 	a.delta   = static_cast<float*>(grads->workspace);
-	a.partial = a.delta + w.delta;
+	a.partial = nullptr, a.dq_space = a.delta + w.delta, a.dkv_space = a.dq_space + w.dq;
 	const hipStream_t s = static_cast<hipStream_t>(hip_stream);
 	return params->dtype == AF3_F32 ? cross::backward_type<float>(a, s) : cross::backward_type<uint16_t>(a, s);
 }

@@ -343,6 +343,9 @@ int af3_linear(const void* x, const void* weight, void* out, int64_t M, int64_t 
  *               A query whose live keys are all dropped by the bias yields zeros.
  *   dtype     : AF3_BF16 (bf16 products, fp32 accumulation and softmax) or AF3_F32 (fp32 throughout), of q, k, v, bias, out.
  *   stats     : optional, [B, H, Lq, 2] floats written for af3_cross_attention_backward (maximum in the softmax's units and 1 / sum).
+ *   out_residual : optional, [B, H, Lq, D] contiguous, AF3_BF16 only: what out lost by its rounding, as bf16.  Given to af3_cross_attention_backward
+ *               too, the row sums of grad_out * out that it takes off every dS are those of out to 16 bits (with out alone they are off by up to
+ *               2^-8 in the same direction along a row, which does not average out of a gradient summed along rows, like a position bias's).
  *   workspace : af3_cross_attention_workspace_bytes() bytes, 16-byte aligned; NULL where that is 0.  Overwritten.
  * B, H, Lq, Lk, D >= 1, D <= AF3_DPA_MAX_HEAD_DIM, Lq and Lk < 2^30, H * Lq < 2^31, B * H * ceil(Lq / 32) < 2^26.
  */
@@ -354,6 +357,7 @@ typedef struct af3_cross_attention_params {
 	const uint8_t* key_mask;
 	void*          out;
 	float*         stats;
+	void*          out_residual;
 	int64_t        B, H, Hkv, Lq, Lk, D;
 	int64_t        q_stride[3];
 	int64_t        k_stride[3];
