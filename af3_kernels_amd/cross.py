@@ -15,6 +15,7 @@ import torch
 from . import _lib, ops
 from ._lib import CrossAttentionGrads, CrossAttentionParams, PositionBiasParams
 
+_host = ops._host
 _i64x2, _i64x3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
 _DTYPES = {torch.float32: _lib.AF3_F32, torch.bfloat16: _lib.AF3_BF16}
 
@@ -137,7 +138,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
     says: a row of nothing else weights its live keys alike.  Lk == 0 gives zeros.
 
     Gradients flow to q, k, v and bias (the same bits every time); not through a second derivative.  In a HIP graph: capture forward and backward
-    together, with leaves that no graph of eager calls still holds (their gradients' accumulation would wait for a stream outside the capture)."""
+    together, with leaves that no result of an earlier call on another stream still holds: their gradients would be accumulated on that stream, outside of
+    the capture, so such a call raises RuntimeError."""
+    out = _host.cross_attention(q, k, v, mask, bias, softmax_scale)
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_cross_attention_forward")
     _same_device(q, k, v, mask, bias)
     if q.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {q.dtype}: float32 or bfloat16")
@@ -154,6 +159,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
+        _host.check_capture(q, k, v, bias)
         return _CrossAttention.apply(q, k, v, keep, bias, scale)
     return _forward(q, k, v, keep, bias, scale, False)[0]
 
@@ -255,6 +261,9 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, scheme: 
     Positions are 0, 1, 2, ... for keys and q_offset, q_offset + 1, ... for queries (a decoder's token t: q_len=1, q_offset=t), or what q_positions [q_len]
     and k_positions [k_len] hold (int64 or int32, on the table's device; q_offset then does not count for queries).
     The gradient flows to the table: sums by bucket in a fixed order."""
+    out = _host.position_bias(table, q_len, k_len, _lib.POSITION_SCHEMES.get(scheme, -1), bidirectional, max_distance, q_positions, k_positions, q_offset)
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_position_bias_forward")
     _same_device(table, q_positions, k_positions)
     if table.dim() != 2:
         raise ValueError(f"table must be [buckets, H], got {tuple(table.shape)}")
@@ -267,5 +276,6 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, scheme: 
     q_positions, k_positions = _positions_of(q_positions, q_len, "q_positions"), _positions_of(k_positions, k_len, "k_positions")
     settings = (scheme, bool(bidirectional), max_distance, q_offset)
     if torch.is_grad_enabled() and table.requires_grad:
+        _host.check_capture(table)
         return _PositionBias.apply(table, q_len, k_len, settings, q_positions, k_positions)
     return _position_forward(table, q_len, k_len, settings, q_positions, k_positions)

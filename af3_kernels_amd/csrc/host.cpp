@@ -10,6 +10,7 @@
 #include <cmath>
 #include <mutex>
 #include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include <ATen/core/Tensor.h>
@@ -21,6 +22,9 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/af3_dpa.h"
@@ -625,6 +629,272 @@ PyObject* py_gated_linear_unit(PyObject*, PyObject* const* a, Py_ssize_t n) {
 	END_HANDLE_TH_ERRORS
 }
 
+// ---- attention to states of another length, relative position bias ------------------------------------------------------------
+// A graph that is captured may not wait for work outside of it.  The gradient of a leaf is accumulated on the stream that was current when the leaf
+// first came into a graph of operations that is still alive; inside a capture that must be the capturing stream, or the engine makes the two wait for each
+// other and ends the process.  Looked at while capturing only.
+void check_capture(at::ArrayRef<const Tensor*> inputs, int dev) {
+	hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+	const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev);
+	if(hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+	std::vector<torch::autograd::Node*>        open;
+	std::unordered_set<torch::autograd::Node*> seen;
+	std::vector<std::shared_ptr<torch::autograd::Node>> leaves;
+	auto look = [&](const std::shared_ptr<torch::autograd::Node>& node) {
+		if(node && seen.insert(node.get()).second) open.push_back(node.get());
+	};
+	for(const Tensor* t : inputs) {
+		if(!t || !t->defined() || !t->requires_grad()) continue;
+		if(t->grad_fn()) look(t->grad_fn());
+		else if(auto leaf = torch::autograd::impl::try_get_grad_accumulator(*t)) leaves.push_back(leaf), look(leaf);
+	}
+	while(!open.empty()) {
+		torch::autograd::Node* node = open.back();
+		open.pop_back();
+		if(dynamic_cast<torch::autograd::AccumulateGrad*>(node)) {
+			const auto own = node->stream();
+			TORCH_CHECK(!own || own->id() == stream.id(),
+						"a gradient is captured into a HIP graph while a graph of operations recorded on another stream still holds one of its leaves (an earlier result that was not "
+						"freed, for instance): the capture would wait for that stream. Free it first, or capture with leaves of their own");
+		}
+		for(const auto& e : node->next_edges()) look(e.function);
+	}
+}
+// The gradients as results that know no derivative of their own: asking for one raises.
+torch::autograd::variable_list once(torch::autograd::variable_list grads, const char* what) {
+	if(!at::GradMode::is_enabled()) return grads;
+	torch::autograd::variable_list in;
+	for(Tensor& g : grads) in.push_back(g.defined() ? g.detach().requires_grad_(true) : g);
+	auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative", (int64_t)in.size());
+	return error->apply(std::move(in));
+}
+void raise(int rc, const char* what) { TORCH_CHECK(rc == AF3_OK, what, ": ", af3_status_string(rc), " (af3_status ", rc, ")"); }
+
+struct cross_call {
+	Tensor         q, k, v, mask, bias;   // mask as bytes [1|B, Lk] or undefined, bias undefined: none
+	double         scale;
+	af3_cross_attention_params block() const {
+		af3_cross_attention_params p{};
+		p.q = q.const_data_ptr(), p.k = k.const_data_ptr(), p.v = v.const_data_ptr();
+		p.B = q.size(0), p.H = q.size(1), p.Lq = q.size(2), p.D = q.size(3), p.Hkv = k.size(1), p.Lk = k.size(2);
+		put_strides(p.q_stride, q), put_strides(p.k_stride, k), put_strides(p.v_stride, v);
+		if(bias.defined()) p.bias = bias.const_data_ptr(), p.bias_stride[0] = bias.stride(0), p.bias_stride[1] = bias.stride(1);
+		if(mask.defined()) p.key_mask = static_cast<const uint8_t*>(mask.const_data_ptr()), p.key_mask_stride_b = mask.dim() > 1 && mask.size(0) != 1 ? mask.stride(0) : 0;
+		p.dtype = dtype_code(q), p.softmax_scale = (float)scale;
+		return p;
+	}
+	int forward(Tensor& out, Tensor* stats, Tensor* lost) const {
+		const int dev = (int)q.get_device();
+		out = new_tensor(q.sizes(), q.scalar_type(), dev);
+		af3_cross_attention_params p = block();
+		p.out = out.data_ptr();
+		put_strides(p.out_stride, out);
+		if(stats) {
+			*stats  = new_tensor({p.B, p.H, p.Lq, 2}, at::kFloat, dev);
+			p.stats = static_cast<float*>(stats->data_ptr());
+			if(p.dtype == AF3_BF16) *lost = new_tensor(q.sizes(), q.scalar_type(), dev), p.out_residual = lost->data_ptr();
+		}
+		at::DataPtr   ws;
+		const int64_t bytes = af3_cross_attention_workspace_bytes(&p);
+		if(bytes < 0) return (int)bytes;
+		if(bytes > 0) ws = new_scratch(bytes), p.workspace = ws.get(), p.workspace_bytes = bytes;
+		return af3_cross_attention_forward(&p, current_stream(dev));
+	}
+};
+struct cross_function : torch::autograd::Function<cross_function> {
+	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& given_bias,
+					  const std::optional<Tensor>& given_mask, double scale) {
+		const Tensor bias = given_bias.value_or(Tensor()), mask = given_mask.value_or(Tensor());
+		Tensor       out, stats, lost;
+		raise(cross_call{q, k, v, mask, bias, scale}.forward(out, &stats, &lost), "af3_cross_attention_forward");
+		ctx->save_for_backward({q, k, v, bias, mask, out, stats, lost});
+		ctx->saved_data["scale"] = scale;
+		return out;
+	}
+	static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_out) {
+		const auto saved = ctx->get_saved_variables();
+		const cross_call call{saved[0], saved[1], saved[2], saved[4], saved[3], ctx->saved_data["scale"].toDouble()};
+		const int        dev = (int)call.q.get_device();
+		Tensor           g = grad_out[0];
+		torch::autograd::variable_list grads(6);
+		{
+			at::AutoGradMode none(false);
+			if(!inner_1(g)) g = g.contiguous();
+			af3_cross_attention_params p = call.block();
+			p.out = saved[5].data_ptr(), p.stats = static_cast<float*>(saved[6].data_ptr());
+			put_strides(p.out_stride, saved[5]);
+			if(saved[7].defined()) p.out_residual = saved[7].data_ptr();
+			af3_cross_attention_grads o{};
+			o.grad_out = g.const_data_ptr();
+			put_strides(o.grad_out_stride, g);
+			auto want = [&](int i, at::IntArrayRef sizes) -> void* {
+				if(!ctx->needs_input_grad((size_t)i)) return nullptr;
+				grads[i] = new_tensor(sizes, call.q.scalar_type(), dev);
+				return grads[i].data_ptr();
+			};
+			o.grad_q = want(0, call.q.sizes()), o.grad_k = want(1, call.k.sizes()), o.grad_v = want(2, call.v.sizes());
+			if(call.bias.defined()) o.grad_bias = want(3, call.bias.sizes());
+			const int64_t     bytes = af3_cross_attention_backward_workspace_bytes(&p);
+			raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_cross_attention_backward_workspace_bytes");
+			const at::DataPtr ws = new_scratch(bytes);
+			o.workspace = ws.get(), o.workspace_bytes = bytes;
+			raise(af3_cross_attention_backward(&p, &o, current_stream(dev)), "af3_cross_attention_backward");
+		}
+		return once(std::move(grads), "cross_attention");
+	}
+};
+std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+	if(!at::GradMode::is_enabled()) return false;
+	for(const Tensor* t : tensors)
+		if(t && t->defined() && t->requires_grad()) return true;
+	return false;
+}
+// cross_attention(q, k, v, mask, bias, scale or None)
+PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+	HANDLE_TH_ERRORS
+	if(n != 6) return none();
+	const Tensor *q = tensor_of(a[0]), *k = tensor_of(a[1]), *v = tensor_of(a[2]);
+	if(!q || !k || !v || q->dim() != 4 || k->dim() != 4 || k->sizes() != v->sizes() || q->numel() == 0 || k->numel() == 0) return none();
+	const int dev = device_of(q);
+	const auto type = q->scalar_type();
+	if(dev < 0 || dtype_code(*q) < 0 || k->scalar_type() != type || v->scalar_type() != type || !on_device(*k, dev) || !on_device(*v, dev) || !inner_1(*q) || !inner_1(*k) || !inner_1(*v)) return none();
+	const int64_t B = q->size(0), H = q->size(1), Lq = q->size(2), D = q->size(3), Lk = k->size(2);
+	if(k->size(0) != B || k->size(3) != D || H % k->size(1) != 0 || D > AF3_DPA_MAX_HEAD_DIM) return none();
+	cross_call c{*q, *k, *v, Tensor(), Tensor(), 0.0};
+	key_mask   m;
+	if(!mask_of(a[3], B, Lk, dev, m)) return none();
+	if(a[3] != Py_None) {
+		const Tensor& t = *tensor_of(a[3]);
+		c.mask = t.dim() == 4 ? t.as_strided({t.size(0), Lk}, {t.stride(0), 1}) : t;
+	}
+	if(a[4] != Py_None) {
+		const Tensor* t = tensor_of(a[4]);
+		if(!t || !on_device(*t, dev) || t->scalar_type() != type || t->dim() != 3 || t->size(0) != H || t->size(1) != Lq || t->size(2) != Lk || !inner_1(*t)) return none();
+		c.bias = *t;
+	}
+	c.scale = a[5] == Py_None ? std::pow((double)D, -0.5) : PyFloat_AsDouble(a[5]);
+	if(PyErr_Occurred()) {
+		PyErr_Clear();
+		return none();
+	}
+	if(!(c.scale > 0.0 && (float)c.scale > 0.f && (float)c.scale < INFINITY)) return none();
+	Tensor out;
+	int    rc = AF3_OK;
+	const bool graph = wants_grad({q, k, v, &c.bias});
+	{
+		without_gil g;
+		if(graph) check_capture({q, k, v, &c.bias}, dev), out = cross_function::apply(c.q, c.k, c.v, given(c.bias), given(c.mask), c.scale);
+		else rc = c.forward(out, nullptr, nullptr);
+	}
+	return answer(rc, std::move(out));
+	END_HANDLE_TH_ERRORS
+}
+
+struct position_call {
+	Tensor  table, q_positions, k_positions;
+	int64_t Lq, Lk, scheme, both, distance, offset;
+	af3_position_bias_params block(at::IntArrayRef table_sizes, at::IntArrayRef strides, at::ScalarType type) const {
+		af3_position_bias_params p{};
+		if(q_positions.defined()) p.q_positions = static_cast<const int64_t*>(q_positions.const_data_ptr());
+		if(k_positions.defined()) p.k_positions = static_cast<const int64_t*>(k_positions.const_data_ptr());
+		p.q_offset = offset, p.buckets = table_sizes[0], p.H = table_sizes[1], p.Lq = Lq, p.Lk = Lk, p.max_distance = distance;
+		p.table_stride[0] = strides[0], p.table_stride[1] = strides[1];
+		p.scheme = (int32_t)scheme, p.bidirectional = (int32_t)both, p.dtype = type == at::kBFloat16 ? AF3_BF16 : AF3_F32;
+		return p;
+	}
+	int forward(Tensor& out) const {
+		const int dev = (int)table.get_device();
+		af3_position_bias_params p = block(table.sizes(), table.strides(), table.scalar_type());
+		out = new_tensor({p.H, Lq, Lk}, table.scalar_type(), dev);
+		p.table = table.const_data_ptr(), p.out = out.data_ptr();
+		return af3_position_bias_forward(&p, current_stream(dev));
+	}
+};
+struct position_function : torch::autograd::Function<position_function> {
+	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& table, const std::optional<Tensor>& given_q, const std::optional<Tensor>& given_k,
+					  std::vector<int64_t> s) {
+		const Tensor q_positions = given_q.value_or(Tensor()), k_positions = given_k.value_or(Tensor());
+		Tensor       out;
+		raise(position_call{table, q_positions, k_positions, s[0], s[1], s[2], s[3], s[4], s[5]}.forward(out), "af3_position_bias_forward");
+		ctx->save_for_backward({q_positions, k_positions});
+		s.push_back(table.size(0)), s.push_back(table.size(1));
+		ctx->saved_data["settings"] = std::move(s);
+		return out;
+	}
+	static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_out) {
+		torch::autograd::variable_list grads(4);
+		{
+			at::AutoGradMode none(false);
+			const auto                 saved = ctx->get_saved_variables();
+			const std::vector<int64_t> s     = ctx->saved_data["settings"].toIntVector();
+			Tensor                     g     = grad_out[0];
+			const int                  dev   = (int)g.get_device();
+			if(!inner_1(g)) g = g.contiguous();
+			grads[0] = new_tensor({s[6], s[7]}, g.scalar_type(), dev);
+			const position_call call{Tensor(), saved[0], saved[1], s[0], s[1], s[2], s[3], s[4], s[5]};
+			af3_position_bias_params p = call.block(grads[0].sizes(), grads[0].strides(), g.scalar_type());
+			p.grad = g.const_data_ptr(), p.grad_stride[0] = g.stride(0), p.grad_stride[1] = g.stride(1), p.out = grads[0].data_ptr();
+			const int64_t bytes = af3_position_bias_workspace_bytes(&p);
+			raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_position_bias_workspace_bytes");
+			const at::DataPtr ws = new_scratch(bytes);
+			p.workspace = ws.get(), p.workspace_bytes = bytes;
+			raise(af3_position_bias_backward(&p, current_stream(dev)), "af3_position_bias_backward");
+		}
+		return once(std::move(grads), "relative_position_bias");
+	}
+};
+bool positions_of(PyObject* o, int64_t n, int dev, Tensor& t) {
+	if(o == Py_None) return true;
+	const Tensor* x = tensor_of(o);
+	if(!x || !on_device(*x, dev) || x->scalar_type() != at::kLong || x->dim() != 1 || x->size(0) != n || !x->is_contiguous()) return false;
+	t = *x;
+	return true;
+}
+// position_bias(table, q_len, k_len, scheme, bidirectional, max_distance, q_positions, k_positions, q_offset); scheme as its number
+PyObject* py_position_bias(PyObject*, PyObject* const* a, Py_ssize_t n) {
+	HANDLE_TH_ERRORS
+	if(n != 9) return none();
+	const Tensor* table = tensor_of(a[0]);
+	const int     dev   = device_of(table);
+	if(dev < 0 || table->dim() != 2 || dtype_code(*table) < 0 || table->numel() == 0) return none();
+	int64_t number[5];   // q_len, k_len, scheme, max_distance, q_offset
+	const int at[5] = {1, 2, 3, 5, 8};
+	for(int i = 0; i < 5; i++) {
+		if(!PyLong_CheckExact(a[at[i]])) return none();
+		number[i] = PyLong_AsLongLong(a[at[i]]);
+	}
+	if(PyErr_Occurred()) {
+		PyErr_Clear();
+		return none();
+	}
+	position_call c{*table, Tensor(), Tensor(), number[0], number[1], number[2], a[4] == Py_True, number[3], number[4]};
+	if((a[4] != Py_True && a[4] != Py_False) || c.Lq < 1 || c.Lk < 1 || !positions_of(a[6], c.Lq, dev, c.q_positions) || !positions_of(a[7], c.Lk, dev, c.k_positions)) return none();
+	const af3_position_bias_params p = c.block(table->sizes(), table->strides(), table->scalar_type());
+	if(af3_position_bias_workspace_bytes(&p) < 0) return none();   // (settings that do not go together: the Python side says what is wrong)
+	Tensor     out;
+	int        rc = AF3_OK;
+	const bool graph = wants_grad({table});
+	{
+		without_gil g;
+		if(graph) check_capture({table}, dev), out = position_function::apply(c.table, given(c.q_positions), given(c.k_positions), std::vector<int64_t>{c.Lq, c.Lk, c.scheme, c.both, c.distance, c.offset});
+		else rc = c.forward(out);
+	}
+	return answer(rc, std::move(out));
+	END_HANDLE_TH_ERRORS
+}
+// check_capture(tensor or None...): raises where a gradient of these cannot be captured
+PyObject* py_check_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
+	HANDLE_TH_ERRORS
+	std::vector<const Tensor*> tensors;
+	int                        dev = -1;
+	for(Py_ssize_t i = 0; i < n; i++)
+		if(const Tensor* t = tensor_of(a[i]); t && t->is_cuda()) tensors.push_back(t), dev = (int)t->get_device();
+	if(dev >= 0) check_capture(tensors, dev);
+	return none();
+	END_HANDLE_TH_ERRORS
+}
+
 #define AF3_FN(name, doc) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_##name)), METH_FASTCALL, doc}
 PyMethodDef methods[] = {
 	AF3_FN(attention, "attention(q, k, v, mask, bias, kernel_hint, exact_bias)"),
@@ -636,6 +906,9 @@ PyMethodDef methods[] = {
 	AF3_FN(linear, "linear(x, weight)"),
 	AF3_FN(layernorm_pair_bias, "layernorm_pair_bias(pair, ln_weight, ln_bias, eps, proj_weight)"),
 	AF3_FN(gated_linear_unit, "gated_linear_unit(x, weight, tag)"),
+	AF3_FN(cross_attention, "cross_attention(q, k, v, mask, bias, scale)"),
+	AF3_FN(position_bias, "position_bias(table, q_len, k_len, scheme, bidirectional, max_distance, q_positions, k_positions, q_offset)"),
+	AF3_FN(check_capture, "check_capture(tensor...): raises where their gradients cannot be captured into a graph"),
 	AF3_FN(remember, "remember(tag, value, source...): a matrix derived from weights"),
 	AF3_FN(recalls, "recalls(tag, source...): whether one is remembered for these"),
 	AF3_FN(forget_source, "forget_source(address): drops what was derived from this tensor"),

@@ -607,3 +607,86 @@ def test_the_bias_feeds_the_other_attention_calls(af3, oracle):
     want = oracle.dpa_formula(*(t.cpu().numpy() for t in (q, k, v)), m.cpu().numpy(), bias.cpu().numpy())
     for t in (a, b):
         assert abs(t.cpu().numpy() - want).max() <= 1e-4
+
+
+# ---- the two host sides, and what autograd may not do ------------------------------------------------------------------------------
+class _NoNativeHost:
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def test_calls_prepared_in_python_give_the_same_bits(af3, monkeypatch):
+    from af3_kernels_amd import cross
+    for dtype, sizes, bias in ((BF16, (2, 4, 2, 70, 150, 64), "given"), (F32, (3, 2, 2, 1, 400, 32), "none")):
+        t = make(*sizes, dtype, 81, "empty", bias)
+        table = torch.randn(32, 4, device="cuda", dtype=dtype).requires_grad_(True)
+        grad = torch.randn(4, 30, 50, device="cuda", dtype=dtype)
+        args = dict(q_positions=torch.arange(30, device="cuda") * 3, k_positions=torch.arange(50, device="cuda") * 2)
+
+        def everything():
+            b = af3.relative_position_bias(table, 30, 50, **args)
+            return [*run(af3, *t).values(), af3.cross_attention(*t[:5]), b, torch.autograd.grad(b, table, grad)[0]]
+        native = everything()
+        with monkeypatch.context() as m:
+            m.setattr(cross, "_host", _NoNativeHost())
+            python = everything()
+        assert all(torch.equal(a, b) for a, b in zip(native, python))
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_no_second_derivative(af3, monkeypatch, native):
+    from af3_kernels_amd import cross
+    if not native:
+        monkeypatch.setattr(cross, "_host", _NoNativeHost())
+    q = torch.randn(1, 2, 4, 16, device="cuda").requires_grad_(True)
+    g = torch.autograd.grad(af3.cross_attention(q, q, q).sum(), q, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="second derivative" if native else None):
+        g.sum().backward()
+    with pytest.raises(RuntimeError):       # (not a gradient that is silently zero either)
+        torch.autograd.grad(g.sum(), q)
+    table = torch.randn(32, 2, device="cuda").requires_grad_(True)
+    g = torch.autograd.grad(af3.relative_position_bias(table, 4, 4).sum(), table, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="second derivative" if native else None):
+        g.sum().backward()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), table)
+
+
+def test_inputs_changed_between_forward_and_backward_are_noticed(af3):
+    q, k, v, m, b, g = make(1, 2, 2, 10, 20, 16, F32, 82, "random", "given")
+    q.requires_grad_(True)
+    for t in (k, m):
+        out = af3.cross_attention(q, k, v, m, b)
+        t.zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, q, g)
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_a_capture_that_would_wait_for_another_stream_is_refused(af3, monkeypatch, native):
+    """The leaf's gradient is accumulated on the default stream while an eager result holds the leaf: captured, that would end the process."""
+    from af3_kernels_amd import cross
+
+    class Only:
+        check_capture = staticmethod(cross._host.check_capture)
+
+        def __getattr__(self, name):
+            return lambda *args: None
+    if not native:
+        monkeypatch.setattr(cross, "_host", Only())
+    q = torch.randn(1, 2, 4, 16, device="cuda").requires_grad_(True)
+    table = torch.randn(32, 2, device="cuda").requires_grad_(True)
+    eager = af3.cross_attention(q, q, q), af3.relative_position_bias(table, 4, 4)
+    refused = []
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: af3.cross_attention(q, q, q), lambda: af3.cross_attention(q * 2, q.detach(), q.detach()), lambda: af3.relative_position_bias(table, 4, 4)):
+            with pytest.raises(RuntimeError, match="captured") as e:
+                call()
+            refused.append(e)
+        plain = af3.cross_attention(q.detach(), q.detach(), q.detach())      # a call without a gradient is captured as ever
+    assert len(refused) == 3
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(plain, eager[0])
+    del eager
