@@ -63,7 +63,7 @@ class CrossAttentionGrads(ctypes.Structure):
     """Mirror of struct af3_cross_attention_grads."""
     _fields_ = [
         ("grad_out", vp), ("grad_out_stride", i64 * 3),
-        ("grad_q", vp), ("grad_k", vp), ("grad_v", vp), ("grad_bias", vp),
+        ("grad_q", vp), ("grad_k", vp), ("grad_v", vp), ("grad_bias", vp), ("grad_bias_residual", vp),
         ("workspace", vp), ("workspace_bytes", i64),
     ]
 

@@ -69,8 +69,9 @@ def _forward(q, k, v, keep, bias, scale, want_stats):
 
 
 def _backward(grad, q, k, v, keep, bias, out, stats, lost, scale, wants):
-    """Gradients of q, k, v and bias, None for those not wanted."""
-    shapes = (q.shape, k.shape, v.shape, None if bias is None else (q.shape[1], q.shape[2], k.shape[2]))
+    """Gradients of q, k, v and bias, None for those not wanted, and with wants[4] what the bias's lost by its rounding."""
+    bias_shape = None if bias is None else (q.shape[1], q.shape[2], k.shape[2])
+    shapes = (q.shape, k.shape, v.shape, bias_shape, bias_shape)
     if stats is None:
         return tuple(torch.zeros(s, dtype=q.dtype, device=q.device) if w else None for s, w in zip(shapes, wants))
     grads = tuple(torch.empty(s, dtype=q.dtype, device=q.device) if w else None for s, w in zip(shapes, wants))
@@ -78,7 +79,7 @@ def _backward(grad, q, k, v, keep, bias, out, stats, lost, scale, wants):
     p = _fill(q, k, v, keep, bias, out, stats, lost, scale)
     g = CrossAttentionGrads()
     g.grad_out, g.grad_out_stride = grad.data_ptr(), _i64x3(*grad.stride()[:3])
-    g.grad_q, g.grad_k, g.grad_v, g.grad_bias = (0 if t is None else t.data_ptr() for t in grads)
+    g.grad_q, g.grad_k, g.grad_v, g.grad_bias, g.grad_bias_residual = (0 if t is None else t.data_ptr() for t in grads)
     lib = _lib.load()
     with ops._on_device(q.device):
         need = lib.af3_cross_attention_backward_workspace_bytes(ctypes.byref(p))
@@ -89,20 +90,37 @@ def _backward(grad, q, k, v, keep, bias, out, stats, lost, scale, wants):
 
 
 class _CrossAttention(torch.autograd.Function):
+    """A bfloat16 bias straight out of relative_position_bias hands its table on (`table`, with that call's positions and settings): its gradient reaches the table
+    as bfloat16, and what that rounding lost reaches the table directly."""
+
     @staticmethod
-    def forward(ctx, q, k, v, keep, bias, scale):
+    def forward(ctx, q, k, v, keep, bias, scale, table, settings, q_positions, k_positions):
         out, stats, lost = _forward(q, k, v, keep, bias, scale, True)
-        ctx.save_for_backward(q, k, v, keep, bias, out, stats, lost)
-        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, keep, bias, out, stats, lost, q_positions, k_positions)
+        ctx.scale, ctx.settings, ctx.table_shape = scale, settings, None if table is None else table.shape
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, keep, bias, out, stats, lost = ctx.saved_tensors
+        q, k, v, keep, bias, out, stats, lost, q_positions, k_positions = ctx.saved_tensors
         needs = ctx.needs_input_grad
-        dq, dk, dv, dbias = _backward(grad, q, k, v, keep, bias, out, stats, lost, ctx.scale, (needs[0], needs[1], needs[2], needs[4]))
-        return dq, dk, dv, None, dbias, None
+        residual = needs[4] and needs[6] and stats is not None
+        dq, dk, dv, dbias, bias_lost = _backward(grad, q, k, v, keep, bias, out, stats, lost, ctx.scale, (needs[0], needs[1], needs[2], needs[4], residual))
+        dtable = _position_sums(bias_lost, ctx.table_shape, ctx.settings, q_positions, k_positions) if residual else None
+        return dq, dk, dv, None, dbias, None, dtable, None, None, None
+
+
+def _source(bias):
+    """(table, settings, q_positions, k_positions) of a bfloat16 bias that is relative_position_bias's result as it stands."""
+    node = bias.grad_fn if bias is not None and bias.dtype == torch.bfloat16 and bias.requires_grad else None
+    if isinstance(node, _PositionBias._backward_cls):
+        try:
+            q_positions, k_positions = node.saved_tensors
+        except RuntimeError:   # (that graph was freed: a backward pass through the bias will say so)
+            return None, None, None, None
+        return node.table, node.settings, q_positions, k_positions
+    return None, None, None, None
 
 
 def _check_cross(q, k, v, keep, bias):
@@ -160,7 +178,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
         raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         _host.check_capture(q, k, v, bias)
-        return _CrossAttention.apply(q, k, v, keep, bias, scale)
+        return _CrossAttention.apply(q, k, v, keep, bias, scale, *_source(bias))
     return _forward(q, k, v, keep, bias, scale, False)[0]
 
 
@@ -190,31 +208,36 @@ def _position_forward(table, q_len, k_len, settings, q_positions, k_positions):
     return out
 
 
+def _position_sums(grad, table_shape, settings, q_positions, k_positions):
+    """The table's gradient of a gradient [H, Lq, Lk] of the bias."""
+    out = torch.empty(table_shape, dtype=grad.dtype, device=grad.device)
+    if grad.numel() == 0:
+        return out.zero_()
+    grad = _inner_contig(grad)
+    p = _position_params(table_shape, out.stride(), grad.dtype, grad.shape[1], grad.shape[2], settings, q_positions, k_positions)
+    p.grad, p.grad_stride, p.out = grad.data_ptr(), _i64x2(grad.stride(0), grad.stride(1)), out.data_ptr()
+    lib = _lib.load()
+    with ops._on_device(grad.device):
+        need = lib.af3_position_bias_workspace_bytes(ctypes.byref(p))
+        _lib.check(min(need, 0), "af3_position_bias_workspace_bytes")
+        ws = torch.empty(need, dtype=torch.uint8, device=grad.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        _lib.check(lib.af3_position_bias_backward(ctypes.byref(p), ops._stream_ptr(grad.device)), "af3_position_bias_backward")
+    return out
+
+
 class _PositionBias(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, q_len, k_len, settings, q_positions, k_positions):
         ctx.save_for_backward(q_positions, k_positions)
-        ctx.shape, ctx.settings = table.shape, settings
+        ctx.table, ctx.settings = table, settings   # (not a saved tensor: the gradient does not need its values, which may change)
         return _position_forward(table, q_len, k_len, settings, q_positions, k_positions)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         q_positions, k_positions = ctx.saved_tensors
-        out = torch.empty(ctx.shape, dtype=grad.dtype, device=grad.device)
-        if grad.numel() == 0:
-            return out.zero_(), None, None, None, None, None
-        grad = _inner_contig(grad)
-        p = _position_params(ctx.shape, out.stride(), grad.dtype, grad.shape[1], grad.shape[2], ctx.settings, q_positions, k_positions)
-        p.grad, p.grad_stride, p.out = grad.data_ptr(), _i64x2(grad.stride(0), grad.stride(1)), out.data_ptr()
-        lib = _lib.load()
-        with ops._on_device(grad.device):
-            need = lib.af3_position_bias_workspace_bytes(ctypes.byref(p))
-            _lib.check(min(need, 0), "af3_position_bias_workspace_bytes")
-            ws = torch.empty(need, dtype=torch.uint8, device=grad.device)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), need
-            _lib.check(lib.af3_position_bias_backward(ctypes.byref(p), ops._stream_ptr(grad.device)), "af3_position_bias_backward")
-        return out, None, None, None, None, None
+        return _position_sums(grad, ctx.table.shape, ctx.settings, q_positions, k_positions), None, None, None, None, None
 
 
 def _check_settings(buckets, scheme, bidirectional, max_distance, q_offset):

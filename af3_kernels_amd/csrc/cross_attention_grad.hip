@@ -479,7 +479,11 @@ __global__ void __launch_bounds__(THREADS) cross_dbias_kernel(grad_args a) {
 #pragma unroll
 		for(int r = 0; r < 16; r++) {
 			const int64_t q = q0 + 32 * s + 16 * half + r;
-			if(q < p.Lq) out[q * p.Lk] = kind<T>::bits(sum[s][r]);
+			if(q < p.Lq) {
+				const T rounded = kind<T>::bits(sum[s][r]);
+				out[q * p.Lk] = rounded;
+				if(sizeof(T) == 2 && a.g.grad_bias_residual) static_cast<T*>(a.g.grad_bias_residual)[(h * p.Lq + q) * p.Lk + key] = kind<T>::bits(sum[s][r] - kind<T>::value(rounded));
+			}
 		}
 }
 
@@ -600,7 +604,7 @@ int backward_type(const grad_args& a, hipStream_t s) {
 int validate_grads(const af3_cross_attention_params* p, const af3_cross_attention_grads* g) {
 	if(const int rc = validate_cross_attention(p); rc != AF3_OK) return rc;
 	if(!g || !g->grad_out || !p->stats || (!g->grad_q && !g->grad_k && !g->grad_v && !g->grad_bias)) return AF3_ERR_NULL_POINTER;
-	if(g->grad_bias && !p->bias) return AF3_ERR_NULL_POINTER;
+	if((g->grad_bias && !p->bias) || (g->grad_bias_residual && !g->grad_bias)) return AF3_ERR_NULL_POINTER;
 	for(int i = 0; i < 3; i++)
 		if(g->grad_out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
 	// (workgroup numbers of the kernels whose results are the keys' and the bias's)

@@ -670,6 +670,64 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads, const 
 }
 void raise(int rc, const char* what) { TORCH_CHECK(rc == AF3_OK, what, ": ", af3_status_string(rc), " (af3_status ", rc, ")"); }
 
+struct position_call {
+	Tensor  table, q_positions, k_positions;
+	int64_t Lq, Lk, scheme, both, distance, offset;
+	af3_position_bias_params block(at::IntArrayRef table_sizes, at::IntArrayRef strides, at::ScalarType type) const {
+		af3_position_bias_params p{};
+		if(q_positions.defined()) p.q_positions = static_cast<const int64_t*>(q_positions.const_data_ptr());
+		if(k_positions.defined()) p.k_positions = static_cast<const int64_t*>(k_positions.const_data_ptr());
+		p.q_offset = offset, p.buckets = table_sizes[0], p.H = table_sizes[1], p.Lq = Lq, p.Lk = Lk, p.max_distance = distance;
+		p.table_stride[0] = strides[0], p.table_stride[1] = strides[1];
+		p.scheme = (int32_t)scheme, p.bidirectional = (int32_t)both, p.dtype = type == at::kBFloat16 ? AF3_BF16 : AF3_F32;
+		return p;
+	}
+	int forward(Tensor& out) const {
+		const int dev = (int)table.get_device();
+		af3_position_bias_params p = block(table.sizes(), table.strides(), table.scalar_type());
+		out = new_tensor({p.H, Lq, Lk}, table.scalar_type(), dev);
+		p.table = table.const_data_ptr(), p.out = out.data_ptr();
+		return af3_position_bias_forward(&p, current_stream(dev));
+	}
+};
+struct position_function : torch::autograd::Function<position_function> {
+	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& table, const std::optional<Tensor>& given_q, const std::optional<Tensor>& given_k,
+					  std::vector<int64_t> s) {
+		const Tensor q_positions = given_q.value_or(Tensor()), k_positions = given_k.value_or(Tensor());
+		Tensor       out;
+		raise(position_call{table, q_positions, k_positions, s[0], s[1], s[2], s[3], s[4], s[5]}.forward(out), "af3_position_bias_forward");
+		ctx->save_for_backward({q_positions, k_positions});
+		ctx->saved_data["table"] = table;   // (for apply_cross; not a saved variable: the gradient does not need its values, which may change)
+		s.push_back(table.size(0)), s.push_back(table.size(1));
+		ctx->saved_data["settings"] = std::move(s);
+		return out;
+	}
+	// the table's gradient [buckets, H] of a gradient g of the bias
+	static Tensor sums(Tensor g, const Tensor& q_positions, const Tensor& k_positions, const std::vector<int64_t>& s) {
+		const int dev = (int)g.get_device();
+		if(!inner_1(g)) g = g.contiguous();
+		Tensor out = new_tensor({s[6], s[7]}, g.scalar_type(), dev);
+		const position_call call{Tensor(), q_positions, k_positions, s[0], s[1], s[2], s[3], s[4], s[5]};
+		af3_position_bias_params p = call.block(out.sizes(), out.strides(), g.scalar_type());
+		p.grad = g.const_data_ptr(), p.grad_stride[0] = g.stride(0), p.grad_stride[1] = g.stride(1), p.out = out.data_ptr();
+		const int64_t bytes = af3_position_bias_workspace_bytes(&p);
+		raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_position_bias_workspace_bytes");
+		const at::DataPtr ws = new_scratch(bytes);
+		p.workspace = ws.get(), p.workspace_bytes = bytes;
+		raise(af3_position_bias_backward(&p, current_stream(dev)), "af3_position_bias_backward");
+		return out;
+	}
+	static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_out) {
+		torch::autograd::variable_list grads(4);
+		{
+			at::AutoGradMode none(false);
+			const auto saved = ctx->get_saved_variables();
+			grads[0] = sums(grad_out[0], saved[0], saved[1], ctx->saved_data["settings"].toIntVector());
+		}
+		return once(std::move(grads), "relative_position_bias");
+	}
+};
+
 struct cross_call {
 	Tensor         q, k, v, mask, bias;   // mask as bytes [1|B, Lk] or undefined, bias undefined: none
 	double         scale;
@@ -701,13 +759,22 @@ struct cross_call {
 		return af3_cross_attention_forward(&p, current_stream(dev));
 	}
 };
+// A bfloat16 bias that comes straight out of relative_position_bias hands its table on as an input (`table`, with that call's positions and settings): the
+// bias's gradient takes its usual way to the table, rounded to bfloat16 as a gradient of a bfloat16 tensor has to be, and what that rounding lost goes
+// to the table directly.  The sum of the two is the table's gradient; what a caller does with the bias's gradient on the way is none of the second part's business
+// (2^-8 of the first).
 struct cross_function : torch::autograd::Function<cross_function> {
-	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& given_bias,
-					  const std::optional<Tensor>& given_mask, double scale) {
+	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& given_bias, const std::optional<Tensor>& table,
+					  const std::optional<Tensor>& given_mask, double scale, torch::autograd::variable_list positions, std::vector<int64_t> settings) {
 		const Tensor bias = given_bias.value_or(Tensor()), mask = given_mask.value_or(Tensor());
 		Tensor       out, stats, lost;
 		raise(cross_call{q, k, v, mask, bias, scale}.forward(out, &stats, &lost), "af3_cross_attention_forward");
-		ctx->save_for_backward({q, k, v, bias, mask, out, stats, lost});
+		torch::autograd::variable_list saved{q, k, v, bias, mask, out, stats, lost};
+		if(table) {
+			saved.insert(saved.end(), positions.begin(), positions.end());
+			ctx->saved_data["settings"] = std::move(settings);
+		}
+		ctx->save_for_backward(std::move(saved));
 		ctx->saved_data["scale"] = scale;
 		return out;
 	}
@@ -716,7 +783,8 @@ struct cross_function : torch::autograd::Function<cross_function> {
 		const cross_call call{saved[0], saved[1], saved[2], saved[4], saved[3], ctx->saved_data["scale"].toDouble()};
 		const int        dev = (int)call.q.get_device();
 		Tensor           g = grad_out[0];
-		torch::autograd::variable_list grads(6);
+		torch::autograd::variable_list grads(9);
+		Tensor           bias_lost;
 		{
 			at::AutoGradMode none(false);
 			if(!inner_1(g)) g = g.contiguous();
@@ -734,11 +802,13 @@ struct cross_function : torch::autograd::Function<cross_function> {
 			};
 			o.grad_q = want(0, call.q.sizes()), o.grad_k = want(1, call.k.sizes()), o.grad_v = want(2, call.v.sizes());
 			if(call.bias.defined()) o.grad_bias = want(3, call.bias.sizes());
+			if(o.grad_bias && saved.size() > 8 && ctx->needs_input_grad(4)) bias_lost = new_tensor(call.bias.sizes(), call.q.scalar_type(), dev), o.grad_bias_residual = bias_lost.data_ptr();
 			const int64_t     bytes = af3_cross_attention_backward_workspace_bytes(&p);
 			raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_cross_attention_backward_workspace_bytes");
 			const at::DataPtr ws = new_scratch(bytes);
 			o.workspace = ws.get(), o.workspace_bytes = bytes;
 			raise(af3_cross_attention_backward(&p, &o, current_stream(dev)), "af3_cross_attention_backward");
+			if(bias_lost.defined()) grads[4] = position_function::sums(bias_lost, saved[8], saved[9], ctx->saved_data["settings"].toIntVector());
 		}
 		return once(std::move(grads), "cross_attention");
 	}
@@ -749,6 +819,20 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
 	for(const Tensor* t : tensors)
 		if(t && t->defined() && t->requires_grad()) return true;
 	return false;
+}
+Tensor apply_cross(const cross_call& c) {
+	std::optional<Tensor>          table;
+	torch::autograd::variable_list positions;
+	std::vector<int64_t>           settings;
+	if(c.bias.defined() && c.bias.scalar_type() == at::kBFloat16 && c.bias.requires_grad())
+		if(auto* node = dynamic_cast<torch::autograd::CppNode<position_function>*>(c.bias.grad_fn().get())) {
+			try {
+				positions = node->ctx_.get_saved_variables(), table = node->ctx_.saved_data["table"].toTensor(), settings = node->ctx_.saved_data["settings"].toIntVector();
+			} catch(const c10::Error&) {   // (that graph was freed: a backward pass through the bias will say so)
+				table.reset();
+			}
+		}
+	return cross_function::apply(c.q, c.k, c.v, given(c.bias), table, given(c.mask), c.scale, positions, settings);
 }
 // cross_attention(q, k, v, mask, bias, scale or None)
 PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -784,66 +868,13 @@ PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 	const bool graph = wants_grad({q, k, v, &c.bias});
 	{
 		without_gil g;
-		if(graph) check_capture({q, k, v, &c.bias}, dev), out = cross_function::apply(c.q, c.k, c.v, given(c.bias), given(c.mask), c.scale);
+		if(graph) check_capture({q, k, v, &c.bias}, dev), out = apply_cross(c);
 		else rc = c.forward(out, nullptr, nullptr);
 	}
 	return answer(rc, std::move(out));
 	END_HANDLE_TH_ERRORS
 }
 
-struct position_call {
-	Tensor  table, q_positions, k_positions;
-	int64_t Lq, Lk, scheme, both, distance, offset;
-	af3_position_bias_params block(at::IntArrayRef table_sizes, at::IntArrayRef strides, at::ScalarType type) const {
-		af3_position_bias_params p{};
-		if(q_positions.defined()) p.q_positions = static_cast<const int64_t*>(q_positions.const_data_ptr());
-		if(k_positions.defined()) p.k_positions = static_cast<const int64_t*>(k_positions.const_data_ptr());
-		p.q_offset = offset, p.buckets = table_sizes[0], p.H = table_sizes[1], p.Lq = Lq, p.Lk = Lk, p.max_distance = distance;
-		p.table_stride[0] = strides[0], p.table_stride[1] = strides[1];
-		p.scheme = (int32_t)scheme, p.bidirectional = (int32_t)both, p.dtype = type == at::kBFloat16 ? AF3_BF16 : AF3_F32;
-		return p;
-	}
-	int forward(Tensor& out) const {
-		const int dev = (int)table.get_device();
-		af3_position_bias_params p = block(table.sizes(), table.strides(), table.scalar_type());
-		out = new_tensor({p.H, Lq, Lk}, table.scalar_type(), dev);
-		p.table = table.const_data_ptr(), p.out = out.data_ptr();
-		return af3_position_bias_forward(&p, current_stream(dev));
-	}
-};
-struct position_function : torch::autograd::Function<position_function> {
-	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& table, const std::optional<Tensor>& given_q, const std::optional<Tensor>& given_k,
-					  std::vector<int64_t> s) {
-		const Tensor q_positions = given_q.value_or(Tensor()), k_positions = given_k.value_or(Tensor());
-		Tensor       out;
-		raise(position_call{table, q_positions, k_positions, s[0], s[1], s[2], s[3], s[4], s[5]}.forward(out), "af3_position_bias_forward");
-		ctx->save_for_backward({q_positions, k_positions});
-		s.push_back(table.size(0)), s.push_back(table.size(1));
-		ctx->saved_data["settings"] = std::move(s);
-		return out;
-	}
-	static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_out) {
-		torch::autograd::variable_list grads(4);
-		{
-			at::AutoGradMode none(false);
-			const auto                 saved = ctx->get_saved_variables();
-			const std::vector<int64_t> s     = ctx->saved_data["settings"].toIntVector();
-			Tensor                     g     = grad_out[0];
-			const int                  dev   = (int)g.get_device();
-			if(!inner_1(g)) g = g.contiguous();
-			grads[0] = new_tensor({s[6], s[7]}, g.scalar_type(), dev);
-			const position_call call{Tensor(), saved[0], saved[1], s[0], s[1], s[2], s[3], s[4], s[5]};
-			af3_position_bias_params p = call.block(grads[0].sizes(), grads[0].strides(), g.scalar_type());
-			p.grad = g.const_data_ptr(), p.grad_stride[0] = g.stride(0), p.grad_stride[1] = g.stride(1), p.out = grads[0].data_ptr();
-			const int64_t bytes = af3_position_bias_workspace_bytes(&p);
-			raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_position_bias_workspace_bytes");
-			const at::DataPtr ws = new_scratch(bytes);
-			p.workspace = ws.get(), p.workspace_bytes = bytes;
-			raise(af3_position_bias_backward(&p, current_stream(dev)), "af3_position_bias_backward");
-		}
-		return once(std::move(grads), "relative_position_bias");
-	}
-};
 bool positions_of(PyObject* o, int64_t n, int dev, Tensor& t) {
 	if(o == Py_None) return true;
 	const Tensor* x = tensor_of(o);

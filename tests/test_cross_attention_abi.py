@@ -102,6 +102,7 @@ def test_cross_attention_backward_validates_on_the_host():
     assert bwd(_cross(), _grads(grad_out=None)) == -1
     assert bwd(_cross(), _grads(grad_q=None, grad_k=None, grad_v=None)) == -1
     assert bwd(_cross(), _grads(grad_bias=BASE)) == -1          # the gradient of a bias that is not there
+    assert bwd(_cross(bias=BASE), _grads(grad_bias_residual=BASE)) == -1      # what the rounding of no gradient lost
     assert bwd(_cross(), _grads(grad_out_stride=i64x3(1, -1, 1))) == -4
     assert bwd(_cross(Lq=0), _grads()) == -3
     need = lib.af3_cross_attention_backward_workspace_bytes(ctypes.byref(_cross()))

@@ -599,6 +599,40 @@ def test_an_encoder_layer_and_a_decoder_step(af3, dtype):
         check(f"token {t}", step, (whole[0][:, :, t:t + 1], lambda up, uo: whole[1](up, uo)[:, :, t:t + 1]), dtype)
 
 
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_a_table_behind_bf16_attention_loses_nothing_to_the_biass_gradient(af3, monkeypatch, native):
+    """The rows of dS sum to zero, so that a bucket's sum is small beside its terms: rounding each of them to bf16 would be felt.  The bias's own gradient is
+    still that of a bf16 tensor, and a bias that was changed on the way takes the plain route."""
+    from af3_kernels_amd import cross
+    if not native:
+        monkeypatch.setattr(cross, "_host", _NoNativeHost())
+    B, H, L, D = 4, 4, 200, 64
+    q, k, v, m, _, g = make(B, H, H, L, L, D, BF16, 73, "ragged", "none")
+    table = torch.randn(32, H).to(BF16).cuda().requires_grad_(True)
+    bias = af3.relative_position_bias(table, L, L)
+    out = af3.cross_attention(q, k, v, m, bias)
+    dbias, dtable = torch.autograd.grad(out, (bias, table), g, retain_graph=True)
+    want = formula(q, k, v, m, bias, g, D ** -0.5)
+    check("dbias", dbias, want["dbias"], BF16)
+    leaf = bias.detach().requires_grad_(True)
+    assert torch.equal(dbias, torch.autograd.grad(af3.cross_attention(q, k, v, m, leaf), leaf, g)[0])
+    b = torch.tensor([[bucket(j - i, 32, "log", True, 128) for j in range(L)] for i in range(L)]).reshape(-1)
+    add = lambda t: torch.zeros(32, H, dtype=torch.float64).index_add_(0, b, t.reshape(H, -1).t().contiguous())
+    value, bound = want["dbias"]
+    # no rounding of the terms to bf16 (of P or dS neither: dbias is not behind a second product), out known to 16 bits; two sums rounded to bf16, then theirs
+    limit = add(bound(0.0, 0.0)) + add(value.abs()) * (2.0 ** -16 + L * L * E32) + 3 * 2.0 ** -8 * add(value).abs() + 2.0 ** -16 * add(value.abs())
+    rest = want["out"][1](2.0 ** -8, 2.0 ** -16)      # ... but P was rounded for out, which delta is made of
+    x = torch.matmul(q.double().cpu(), spread(k, H).double().cpu().transpose(2, 3)) * D ** -0.5 + bias.detach().double().cpu()
+    p = torch.softmax(x.masked_fill(~m.cpu()[:, None, None, :], -math.inf), -1)
+    limit = limit + add((p * (g.double().cpu().abs() * rest).sum(-1, keepdim=True)).sum(0))
+    assert ((dtable.double().cpu() - add(value)).abs() <= limit).all()
+    # (and without the second way: the sums of the rounded gradient)
+    changed = torch.autograd.grad(af3.cross_attention(q, k, v, m, bias * 1), table, g)[0]
+    assert ((changed.double().cpu() - add(dbias.double().cpu())).abs() <= 2 * 2.0 ** -8 * add(value).abs() + L * L * E32 * add(value.abs()) + 1e-3).all()
+    error = lambda t: ((t.double().cpu() - add(value)).norm() / add(value).norm()).item()
+    print("table's gradient off by", error(dtable), "and by the plain route", error(changed))
+
+
 def test_the_bias_feeds_the_other_attention_calls(af3, oracle):
     """relative_position_bias into dot_product_attention_cpp, which takes q_len == k_len: the same result as cross_attention's within both bounds."""
     q, k, v, m, _, _ = make(4, 4, 4, 96, 96, 32, F32, 72, "random", "none")
@@ -660,6 +694,21 @@ def test_inputs_changed_between_forward_and_backward_are_noticed(af3):
         t.zero_()
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(out, q, g)
+
+
+def test_a_table_may_change_before_its_gradient_is_taken(af3):
+    table = torch.randn(32, 2, device="cuda", dtype=BF16).requires_grad_(True)
+    q = torch.randn(1, 2, 30, 16, device="cuda", dtype=BF16)
+    bias = af3.relative_position_bias(table, 30, 30)
+    out = af3.cross_attention(q, q, q, None, bias)
+    want = torch.autograd.grad(out.sum(), table, retain_graph=True)[0]
+    with torch.no_grad():
+        table.mul_(2)
+    assert torch.equal(torch.autograd.grad(out.sum(), table)[0], want)
+    # the bias's graph is freed now: another call with it works, its gradient does not
+    again = af3.cross_attention(q, q, q, None, bias)
+    with pytest.raises(RuntimeError, match="second time"):
+        again.sum().backward()
 
 
 @pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
