@@ -42,10 +42,12 @@ struct forward_shape {
 	static constexpr int BUFFERS = 4 * TILE <= 81920 ? 2 : 1;
 	static constexpr int JOIN = KW > 1 ? WAVES * 32 * (DP + 4) * 4 : 0;   // the wavefronts' results on their way to each other
 	static constexpr int LDS = 2 * BUFFERS * TILE > JOIN ? 2 * BUFFERS * TILE : JOIN;
+	// q, the result's sums and the tiles on their way
+	static constexpr int REGISTERS = 4 * tile<T, DP>::STEPS + DP / 2 + 8 * passage<T, DP, KT>::N;
 };
 
 template <typename T, int DP, int KW, bool BIAS>
-__global__ void __launch_bounds__(THREADS) cross_forward_kernel(forward_args a) {
+__global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::REGISTERS)) cross_forward_kernel(forward_args a) {
 	using S  = forward_shape<T, DP, KW>;
 	using TL = tile<T, DP>;
 	constexpr int E = kind<T>::E, KT = S::KT;
@@ -75,15 +77,18 @@ __global__ void __launch_bounds__(THREADS) cross_forward_kernel(forward_args a) 
 	const T* const bias = BIAS ? static_cast<const T*>(p.bias) + h * p.bias_stride[0] + qi * p.bias_stride[1] : nullptr;
 	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b : nullptr;
 
-	float  m = LOWEST, l = 0.f;
+	// p = exp2(t * to_log2 - reference): t = q.k or scale q.k + bias, `reference` = to_log2 * (a maximum of the row's logits so far)
+	const float to_log2 = a.factor;
+	float  m = LOWEST, reference = -INFINITY, l = 0.f;
 	f32x16 o[TL::BLOCKS];
 #pragma unroll
 	for(int db = 0; db < TL::BLOCKS; db++) o[db] = f32x16{};
-	const float slack = 8.f / a.factor;
-	bool        any = false;   // a live key was met
+	bool any = false, fresh = true;   // a live key was met; no block yet
 
 	const int64_t last = (int64_t)(split + 1) * a.part < p.Lk ? (int64_t)(split + 1) * a.part : p.Lk;
 	passage<T, DP, KT> pk, pv;
+	pk.begin(kb, p.k_stride[2], D, a.whole);
+	pv.begin(vb, p.v_stride[2], D, a.whole);
 	int buffer = 0;
 	for(int64_t first = (int64_t)split * a.part; first < last; first += SEGMENT) {
 		const int64_t end = first + SEGMENT < last ? first + SEGMENT : last;
@@ -91,8 +96,8 @@ __global__ void __launch_bounds__(THREADS) cross_forward_kernel(forward_args a) 
 		int t = live.next(0);
 		if(t < 0) continue;
 		any = true;
-		pk.load(kb, p.k_stride[2], first + (int64_t)t * KT, end, D, a.whole);
-		pv.load(vb, p.v_stride[2], first + (int64_t)t * KT, end, D, a.whole);
+		pk.load(first + (int64_t)t * KT, end);
+		pv.load(first + (int64_t)t * KT, end);
 		while(t >= 0) {
 			unsigned char* const ks = smem + buffer * 2 * S::TILE;
 			unsigned char* const vs = ks + S::TILE;
@@ -101,47 +106,76 @@ __global__ void __launch_bounds__(THREADS) cross_forward_kernel(forward_args a) 
 #pragma unroll
 				for(int s = 0; s < S::SUB; s++) load_row16(bs[s], bias, first + (int64_t)t * KT + 32 * (kwave * S::SUB + s) + 16 * half, p.Lk);
 			}
-			if constexpr(S::BUFFERS == 1) __syncthreads();
-			pk.store(ks, D, [&](int row) { return live.keeps(t * KT + row); });
-			pv.store(vs, D, [&](int row) { return live.keeps(t * KT + row); });
-			__syncthreads();
+			const bool full = live.full(t);
+			uint32_t   keep[S::SUB];
+#pragma unroll
+			for(int s = 0; s < S::SUB; s++) keep[s] = live.word(t * (KT / 32) + kwave * S::SUB + s);
 			const int following = live.next(t + 1);
+			if constexpr(S::BUFFERS == 1) __syncthreads();
+			pk.store(ks, full, [&](int row) { return live.keeps(t * KT + row); });
+			pv.store(vs, full, [&](int row) { return live.keeps(t * KT + row); });
+			__syncthreads();
 			if(following >= 0) {
-				pk.load(kb, p.k_stride[2], first + (int64_t)following * KT, end, D, a.whole);
-				pv.load(vb, p.v_stride[2], first + (int64_t)following * KT, end, D, a.whole);
+				pk.load(first + (int64_t)following * KT, end);
+				pv.load(first + (int64_t)following * KT, end);
 			}
 #pragma unroll
 			for(int s = 0; s < S::SUB; s++) {
-				const int      block = kwave * S::SUB + s;
-				const uint32_t keep  = live.word(t * (KT / 32) + block);
-				if(keep == 0u) continue;
-				f32x16 acc{};
-#pragma unroll
-				for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(ks, 32 * block, i, lane), qf[i], acc);
+				const int block = kwave * S::SUB + s;
+				if(keep[s] == 0u) continue;
 				float x[16];
+				auto  logits = [&] {
+					f32x16 acc{};
 #pragma unroll
-				for(int r = 0; r < 16; r++) x[r] = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, bs[s][r]) : acc[r];
-				if(keep != ~0u) {
-					const uint32_t mine = keep >> (16 * half);
+					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(ks, 32 * block, i, lane), qf[i], acc);
 #pragma unroll
-					for(int r = 0; r < 16; r++) x[r] = (mine >> r) & 1u ? x[r] : -INFINITY;
+					for(int r = 0; r < 16; r++) x[r] = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, bs[s][r]) : acc[r];
+					if(keep[s] != ~0u) {
+						const uint32_t mine = keep[s] >> (16 * half);
+#pragma unroll
+						for(int r = 0; r < 16; r++) x[r] = (mine >> r) & 1u ? x[r] : -INFINITY;
+					}
+				};
+				auto probabilities = [&]() -> float {
+					float sum = 0.f;
+#pragma unroll
+					for(int r = 0; r < 16; r++) {
+						x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], to_log2, -reference));
+						sum += x[r];
+					}
+					return sum;
+				};
+				// Optimistic: the probabilities against the reference as it is.  It moves, to the maximum, at a wavefront's first block and where they get large, and
+				// then nothing needs a factor until they get large again.
+				float sum  = 0.f;
+				bool  move = fresh;
+				fresh      = false;
+				logits();
+				if(!move) {
+					sum  = probabilities();
+					move = __any(!(sum < LARGE));
+					if(move) logits();
 				}
-				float top = x[0];
+				if(move) {
+					float top = x[0];
 #pragma unroll
-				for(int r = 1; r < 16; r++) top = maximum(top, x[r]);
-				top = maximum(top, other_half(top));
-				// The reference moves where a logit is more than 2^8 above it: until then no product needs another factor.
-				if(__any(!(top <= m + slack))) {
-					const float to = maximum(m, top), by = __builtin_amdgcn_exp2f((m - to) * a.factor);
-					m = to, l *= by;
+					for(int r = 1; r < 16; r++) top = maximum(top, x[r]);
+					const float to = maximum(m, maximum_of_halves(top)), by = __builtin_amdgcn_exp2f((m - to) * to_log2);
+					m = to, reference = reference_of(m, to_log2), l *= by;
 #pragma unroll
 					for(int db = 0; db < TL::BLOCKS; db++) o[db] *= by;
-				}
+					if(__any(m < FAR_BELOW)) {   // a row of hugely negative biases alone: its logits leave the range in units of log2 e
+						sum = 0.f;
 #pragma unroll
-				for(int r = 0; r < 16; r++) {
-					x[r] = __builtin_amdgcn_exp2f((x[r] - m) * a.factor);
-					l += x[r];
+						for(int r = 0; r < 16; r++) {
+							x[r] = __builtin_amdgcn_exp2f((x[r] - m) * to_log2);
+							sum += x[r];
+						}
+					} else {
+						sum = probabilities();
+					}
 				}
+				l += sum;
 #pragma unroll
 				for(int j = 0; j < TL::JOINTS; j++) {
 					const u32x4 pf = kind<T>::pack(x + E * j);
@@ -153,7 +187,7 @@ __global__ void __launch_bounds__(THREADS) cross_forward_kernel(forward_args a) 
 			if constexpr(S::BUFFERS == 2) buffer ^= 1;
 		}
 	}
-	l += other_half(l);
+	l = sum_of_halves(l);
 
 	const int64_t bh = b * p.Hkv + hk, n_rows = p.B * p.Hkv * rows;
 	if(!any) {

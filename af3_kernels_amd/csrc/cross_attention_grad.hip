@@ -71,7 +71,7 @@ __device__ __forceinline__ float row_delta(const grad_args& a, const u32x4 (&gf)
 		load_operand<T, DP>(of, static_cast<const T*>(p.out_residual) + ((b * p.H + h) * p.Lq + qi) * p.D, ok, (int)p.D, lane);
 		add();
 	}
-	return delta + other_half(delta);
+	return sum_of_halves(delta);
 }
 
 // ---- dQ ----
@@ -82,10 +82,11 @@ struct dq_shape {
 	static constexpr int BUFFERS = 4 * TILE <= 81920 ? 2 : 1;
 	static constexpr int JOIN = KW > 1 ? WAVES * 32 * (DP + 4) * 4 : 0;
 	static constexpr int LDS = 2 * BUFFERS * TILE > JOIN ? 2 * BUFFERS * TILE : JOIN;
+	static constexpr int REGISTERS = 8 * tile<T, DP>::STEPS + DP / 2 + 8 * passage<T, DP, KT>::N - 24;
 };
 
 template <typename T, int DP, int KW, bool BIAS>
-__global__ void __launch_bounds__(THREADS) cross_dq_kernel(grad_args a) {
+__global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGISTERS)) cross_dq_kernel(grad_args a) {
 	using S  = dq_shape<T, DP, KW>;
 	using TL = tile<T, DP>;
 	constexpr int E = kind<T>::E, KT = S::KT;
@@ -124,14 +125,16 @@ __global__ void __launch_bounds__(THREADS) cross_dq_kernel(grad_args a) {
 
 	const int64_t last = (int64_t)(split + 1) * a.part < p.Lk ? (int64_t)(split + 1) * a.part : p.Lk;
 	passage<T, DP, KT> pk, pv;
+	pk.begin(kb, p.k_stride[2], D, a.whole);
+	pv.begin(vb, p.v_stride[2], D, a.whole);
 	int buffer = 0;
 	for(int64_t first = (int64_t)split * a.part; first < last; first += SEGMENT) {
 		const int64_t end = first + SEGMENT < last ? first + SEGMENT : last;
 		live.scan(mask, first, end);
 		int t = live.next(0);
 		if(t < 0) continue;
-		pk.load(kb, p.k_stride[2], first + (int64_t)t * KT, end, D, a.whole);
-		pv.load(vb, p.v_stride[2], first + (int64_t)t * KT, end, D, a.whole);
+		pk.load(first + (int64_t)t * KT, end);
+		pv.load(first + (int64_t)t * KT, end);
 		while(t >= 0) {
 			unsigned char* const ks = smem + buffer * 2 * S::TILE;
 			unsigned char* const vs = ks + S::TILE;
@@ -140,19 +143,23 @@ __global__ void __launch_bounds__(THREADS) cross_dq_kernel(grad_args a) {
 #pragma unroll
 				for(int s = 0; s < S::SUB; s++) load_row16(bs[s], bias, first + (int64_t)t * KT + 32 * (kwave * S::SUB + s) + 16 * half, p.Lk);
 			}
-			if constexpr(S::BUFFERS == 1) __syncthreads();
-			pk.store(ks, D, [&](int r) { return live.keeps(t * KT + r); });
-			pv.store(vs, D, [&](int r) { return live.keeps(t * KT + r); });
-			__syncthreads();
+			const bool full = live.full(t);
+			uint32_t   keeps[S::SUB];
+#pragma unroll
+			for(int s = 0; s < S::SUB; s++) keeps[s] = live.word(t * (KT / 32) + kwave * S::SUB + s);
 			const int following = live.next(t + 1);
+			if constexpr(S::BUFFERS == 1) __syncthreads();
+			pk.store(ks, full, [&](int r) { return live.keeps(t * KT + r); });
+			pv.store(vs, full, [&](int r) { return live.keeps(t * KT + r); });
+			__syncthreads();
 			if(following >= 0) {
-				pk.load(kb, p.k_stride[2], first + (int64_t)following * KT, end, D, a.whole);
-				pv.load(vb, p.v_stride[2], first + (int64_t)following * KT, end, D, a.whole);
+				pk.load(first + (int64_t)following * KT, end);
+				pv.load(first + (int64_t)following * KT, end);
 			}
 #pragma unroll
 			for(int s = 0; s < S::SUB; s++) {
 				const int      block = kwave * S::SUB + s;
-				const uint32_t keep  = live.word(t * (KT / 32) + block);
+				const uint32_t keep  = keeps[s];
 				if(keep == 0u) continue;
 				f32x16 acc{}, dp{};
 #pragma unroll
@@ -220,10 +227,11 @@ struct dkv_shape {
 	static constexpr int BUFFERS = 2 * SET <= 81920 ? 2 : 1;
 	static constexpr int JOIN = RW > 1 ? WAVES * 32 * (DP + 4) * 4 : 0;
 	static constexpr int LDS = BUFFERS * SET > JOIN ? BUFFERS * SET : JOIN;
+	static constexpr int REGISTERS = 8 * tile<T, DP>::STEPS + DP + 8 * passage<T, DP, QT>::N;
 };
 
 template <typename T, int DP, int RW, bool BIAS>
-__global__ void __launch_bounds__(THREADS) cross_dkv_kernel(grad_args a) {
+__global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGISTERS)) cross_dkv_kernel(grad_args a) {
 	using S  = dkv_shape<T, DP, RW>;
 	using TL = tile<T, DP>;
 	constexpr int E = kind<T>::E, QT = S::QT;
@@ -257,11 +265,15 @@ __global__ void __launch_bounds__(THREADS) cross_dkv_kernel(grad_args a) {
 	const int64_t q_tiles = (p.Lq + QT - 1) / QT, n = G * q_tiles;
 	const int64_t last = (int64_t)(split + 1) * a.part < n ? (int64_t)(split + 1) * a.part : n;
 	passage<T, DP, QT> pq, pg;
+	pq.begin(nullptr, p.q_stride[2], D, a.whole);
+	pg.begin(nullptr, a.g.grad_out_stride[2], D, a.whole);
 	float row_stat[3];
 	auto fetch = [&](int64_t it) {
 		const int64_t h = hk * G + it / q_tiles, q0 = it % q_tiles * QT;
-		pq.load(static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1], p.q_stride[2], q0, p.Lq, D, a.whole);
-		pg.load(static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1], a.g.grad_out_stride[2], q0, p.Lq, D, a.whole);
+		pq.base = static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1];
+		pg.base = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1];
+		pq.load(q0, p.Lq);
+		pg.load(q0, p.Lq);
 		row_stat[0] = row_stat[1] = row_stat[2] = 0.f;
 		if((int)threadIdx.x < QT && q0 + threadIdx.x < p.Lq) {
 			const int64_t row = (b * p.H + h) * p.Lq + q0 + threadIdx.x;
@@ -281,8 +293,8 @@ __global__ void __launch_bounds__(THREADS) cross_dkv_kernel(grad_args a) {
 		const int64_t        h = hk * G + it / q_tiles, q0 = it % q_tiles * QT;
 		if constexpr(S::BUFFERS == 1) __syncthreads();
 		const int64_t left = p.Lq - q0;
-		pq.store(qs, D, [&](int r) { return r < left; });
-		pg.store(gs, D, [&](int r) { return r < left; });
+		pq.store(qs, left >= QT, [&](int r) { return r < left; });
+		pg.store(gs, left >= QT, [&](int r) { return r < left; });
 		if((int)threadIdx.x < QT) st[threadIdx.x] = row_stat[0], st[QT + threadIdx.x] = row_stat[1], st[2 * QT + threadIdx.x] = row_stat[2];
 		__syncthreads();
 		if(it + 1 < last) fetch(it + 1);
@@ -396,10 +408,11 @@ struct dbias_shape {
 	static constexpr int QT = sizeof(T) == 2 ? 64 : 32, SUB = QT / 32, KEYS = 128;
 	static constexpr int TILE = QT * tile<T, DP>::STRIDE, STATS = 3 * QT * 4, SET = 2 * TILE + STATS;
 	static constexpr int BUFFERS = 2 * SET <= 81920 ? 2 : 1, LDS = BUFFERS * SET;
+	static constexpr int REGISTERS = 8 * tile<T, DP>::STEPS + 32 * SUB + 8 * passage<T, DP, QT>::N;
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(THREADS) cross_dbias_kernel(grad_args a) {
+__global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGISTERS)) cross_dbias_kernel(grad_args a) {
 	using S  = dbias_shape<T, DP>;
 	using TL = tile<T, DP>;
 	constexpr int QT = S::QT;
@@ -426,10 +439,14 @@ __global__ void __launch_bounds__(THREADS) cross_dbias_kernel(grad_args a) {
 			if(in && q < p.Lq) bs[s][r] = kind<T>::value(static_cast<const T*>(p.bias)[h * p.bias_stride[0] + q * p.bias_stride[1] + key]);
 		}
 	passage<T, DP, QT> pq, pg;
+	pq.begin(nullptr, p.q_stride[2], D, a.whole);
+	pg.begin(nullptr, a.g.grad_out_stride[2], D, a.whole);
 	float row_stat[3];
 	auto fetch = [&](int64_t b) {
-		pq.load(static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1], p.q_stride[2], q0, p.Lq, D, a.whole);
-		pg.load(static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1], a.g.grad_out_stride[2], q0, p.Lq, D, a.whole);
+		pq.base = static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1];
+		pg.base = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1];
+		pq.load(q0, p.Lq);
+		pg.load(q0, p.Lq);
 		row_stat[0] = row_stat[1] = row_stat[2] = 0.f;
 		if((int)threadIdx.x < QT && q0 + threadIdx.x < p.Lq) {
 			const int64_t row = (b * p.H + h) * p.Lq + q0 + threadIdx.x;
@@ -448,8 +465,8 @@ __global__ void __launch_bounds__(THREADS) cross_dbias_kernel(grad_args a) {
 		load_operand<T, DP>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], lives, D, lane);
 		if constexpr(S::BUFFERS == 1) __syncthreads();
 		const int64_t left = p.Lq - q0;
-		pq.store(qs, D, [&](int r) { return r < left; });
-		pg.store(gs, D, [&](int r) { return r < left; });
+		pq.store(qs, left >= QT, [&](int r) { return r < left; });
+		pg.store(gs, left >= QT, [&](int r) { return r < left; });
 		if((int)threadIdx.x < QT) st[threadIdx.x] = row_stat[0], st[QT + threadIdx.x] = row_stat[1], st[2 * QT + threadIdx.x] = row_stat[2];
 		__syncthreads();
 		if(b + 1 < p.B) fetch(b + 1);

@@ -15,6 +15,7 @@ namespace cross {
 
 constexpr int THREADS = 256, WAVES = 4;
 constexpr float LOWEST = -3.402823466e38f;
+constexpr float LARGE  = 65536.f;   // of a lane's sum of 16 probabilities: the reference is left behind
 
 template <typename T>
 struct kind;
@@ -76,78 +77,115 @@ __device__ __forceinline__ u32x4 load_guarded(const T* row, int d, int D) {
 
 __device__ __forceinline__ int   tile_row(int i) { return 16 * ((i >> 2) & 1) + (i & 3) + 4 * (i >> 3); }
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }   // (NaN stays)
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// What is taken off a row's logits in units of log2 e: a row's maximum (or what was its maximum) m times the factor.  -inf, which makes every probability infinite or
+// NaN, sends those who look at them to the exact form, for rows whose maximum is so low that the product could leave fp32's range; a maximum of
+// +inf makes the row NaN, as in the formula.
+constexpr float FAR_BELOW = -1e38f;
+__device__ __forceinline__ float reference_of(float m, float to_log2) {
+	const float r = m * to_log2;
+	return m < FAR_BELOW ? -INFINITY : r - r + r;
+}
+// a value of lane l and that of lane l ^ 32, joined
+__device__ __forceinline__ float sum_of_halves(float x) {
+	const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+	return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float maximum_of_halves(float x) {
+	const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+	return maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
-// A tile in LDS: rows of DP elements and 16 bytes more, which puts consecutive rows on other banks.
+// A tile in LDS: rows of DP elements, whose 16-byte pieces change places by the row so that neither way of reading meets one of the 64 banks twice.  Sixteen lanes
+// of a row_frag read rows 0-7 and 16-23 (or 8 more each) at one column: sixteen rows that differ in their bits 0, 1, 2 and 4.  32 lanes of a col_frag of bf16
+// read 64 bytes of four consecutive rows, which differ in bits 0 and 1.  So bits 0 and 1 move a piece by 64 bytes and more and bits 2 and 4 within 64 bytes, where
+// the rows' own beginnings do not do so already.  (fp32 reads 128 bytes of two rows 16 apart: there bit 4 moves by 128.)  With rows of 16 bytes more instead
+// conflicts were 50 of 101 million clocks of LDS work at 8 x 16 x 1491 x 4096 x 128.
 template <typename T, int DP>
 struct tile {
-	static constexpr int STRIDE = DP * (int)sizeof(T) + 16, STEPS = DP * (int)sizeof(T) / 32, BLOCKS = DP / 32, CHUNKS = DP * (int)sizeof(T) / 16, JOINTS = 32 / (2 * kind<T>::E);
-	// contraction over the columns: A operand, step s, of the 32 rows from `row0` on
+	static constexpr int STRIDE = DP * (int)sizeof(T), STEPS = DP * (int)sizeof(T) / 32, BLOCKS = DP / 32, CHUNKS = DP * (int)sizeof(T) / 16, JOINTS = 32 / (2 * kind<T>::E);
+	// where piece `chunk` of a row lies
+	static __device__ __forceinline__ int place(int row, int chunk) {
+		const int b0 = row & 1, b1 = (row >> 1) & 1, b2 = (row >> 2) & 1, b4 = (row >> 4) & 1;
+		if constexpr(STRIDE % 256 == 0) return 16 * (chunk ^ (sizeof(T) == 2 ? 8 * b0 | 4 * b1 | 2 * b4 | b2 : 8 * b4 | 4 * b0 | 2 * b1 | b2));
+		else if constexpr(STRIDE % 128 == 0) return 16 * (chunk ^ (4 * b1 | 2 * b4 | b2));
+		else return 16 * (chunk ^ (2 * b4 | b2));
+	}
+	// contraction over the columns: A operand, step s, of the 32 rows from `row0` (a multiple of 32) on
 	static __device__ __forceinline__ u32x4 row_frag(const unsigned char* lds, int row0, int s, int lane) {
-		return *reinterpret_cast<const u32x4*>(lds + (row0 + tile_row(lane & 31)) * STRIDE + 32 * s + 16 * (lane >> 5));
+		const int row = tile_row(lane & 31);
+		return *reinterpret_cast<const u32x4*>(lds + row0 * STRIDE + row * STRIDE + place(row, 2 * s + (lane >> 5)));
 	}
 	// contraction over the 32 rows from `row0` on: A operand, step j, of columns 32 db .. 32 db + 31
 	static __device__ __forceinline__ u32x4 col_frag(const unsigned char* lds, int row0, int db, int j, int lane) {
 		if constexpr(sizeof(T) == 2) {
 			// (ds_read_b64_tr_b16: lane i of a group of 16 supplies 4 columns of row i / 4 and receives 4 rows of the group's column i)
-			const int i = lane & 15, G = lane >> 4;
+			const int i = lane & 15, G = lane >> 4, row = 16 * (G >> 1) + (i >> 2);
 			u32x4     f;
 #pragma unroll
 			for(int t = 0; t < 2; t++) {
-				const int   row = row0 + 16 * (G >> 1) + 8 * j + 4 * t + (i >> 2), col = 32 * db + 16 * (i & 1) + 4 * ((i >> 1) & 1) + 8 * (G & 1);
-				const u32x2 r   = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + row * STRIDE + col * 2)));
+				const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + (row0 + 8 * j + row + 4 * t) * STRIDE +
+																	place(row + 4 * t, 4 * db + 2 * (i & 1) + (G & 1)) + 8 * ((i >> 1) & 1))));
 				f[2 * t] = r[0], f[2 * t + 1] = r[1];
 			}
 			return f;
 		} else {
-			u32x4 f;
+			const int col = 32 * db + tile_row(lane & 31), half = 16 * (lane >> 5);
+			u32x4     f;
 #pragma unroll
-			for(int t = 0; t < 4; t++) f[t] = *reinterpret_cast<const uint32_t*>(lds + (row0 + 16 * (lane >> 5) + 4 * j + t) * STRIDE + (32 * db + tile_row(lane & 31)) * 4);
+			for(int t = 0; t < 4; t++) f[t] = *reinterpret_cast<const uint32_t*>(lds + (row0 + half + 4 * j + t) * STRIDE + place(half + 4 * j + t, col >> 2) + 4 * (col & 3));
 			return f;
 		}
 	}
 };
 
-// ROWS rows on their way from memory into a tile, spread over the workgroup's threads.  Where D is a whole number of 16-byte pieces
-// (whole) every piece is one load at a place that exists, and pieces that lie past the rows or past D become zeros on the way into LDS.
+// ROWS rows on their way from memory into a tile, spread over the workgroup's threads in 16-byte pieces.  The plain way (rows all there, D a whole number of pieces,
+// 32-bit offsets within the tile) is one load per piece at a scalar base and an offset that stays the same from tile to tile.
 template <typename T, int DP, int ROWS>
 struct passage {
 	using TL = tile<T, DP>;
-	static constexpr int N = ROWS * TL::CHUNKS / THREADS;
+	static constexpr int N = ROWS * TL::CHUNKS / THREADS, E = kind<T>::E;
 	static_assert(N * THREADS == ROWS * TL::CHUNKS);
-	u32x4 piece[N];
-	// rows row0 .. row0 + ROWS - 1 of a matrix, those below `rows` exist (one at least)
-	__device__ __forceinline__ void load(const T* base, int64_t stride, int64_t row0, int64_t rows, int D, bool whole) {
+	u32x4    piece[N];
+	uint32_t offset[N];   // bytes from the tile's first row
+	const T* base;
+	int64_t  stride;
+	int      D;
+	bool     plain;
+	static __device__ __forceinline__ int row_of(int n) { return (threadIdx.x + THREADS * n) / TL::CHUNKS; }
+	static __device__ __forceinline__ int col_of(int n) { return (threadIdx.x + THREADS * n) % TL::CHUNKS; }
+	__device__ __forceinline__ void begin(const T* base_, int64_t stride_, int D_, bool whole) {
+		base = base_, stride = stride_, D = D_;
+		plain = whole && stride_ <= (int64_t)0x7fffffff / ((int64_t)ROWS * (int)sizeof(T));
+#pragma unroll
+		for(int n = 0; n < N; n++) offset[n] = plain && col_of(n) * E < D ? (uint32_t)((row_of(n) * (int)stride + col_of(n) * E) * (int)sizeof(T)) : 0u;
+	}
+	// rows row0 .. row0 + ROWS - 1, those below `rows` exist (one at least)
+	__device__ __forceinline__ void load(int64_t row0, int64_t rows) {
 		const T*  at   = base + row0 * stride;
 		const int left = rows - row0 < ROWS ? (int)(rows - row0) : ROWS;
-		if(whole) {
+		if(plain) {
 #pragma unroll
-			for(int n = 0; n < N; n++) {
-				const int c = threadIdx.x + THREADS * n, row = c / TL::CHUNKS, d = (c % TL::CHUNKS) * kind<T>::E;
-				piece[n] = load16(at + (int64_t)(row < left ? row : 0) * stride + (d < D ? d : 0));
-			}
+			for(int n = 0; n < N; n++) piece[n] = load16(reinterpret_cast<const T*>(reinterpret_cast<const unsigned char*>(at) + (row_of(n) < left ? offset[n] : 0u)));
 		} else {
 #pragma unroll
-			for(int n = 0; n < N; n++) {
-				const int c = threadIdx.x + THREADS * n, row = c / TL::CHUNKS, d = (c % TL::CHUNKS) * kind<T>::E;
-				piece[n] = load_guarded(at + (int64_t)(row < left ? row : 0) * stride, d, D);
-			}
+			for(int n = 0; n < N; n++) piece[n] = load_guarded(at + (int64_t)(row_of(n) < left ? row_of(n) : 0) * stride, col_of(n) * E, D);
 		}
 	}
-	// keep(row): whether the tile is to hold that row (zeros otherwise)
+	// all: every row of the tile is wanted; otherwise keep(row) says which, the others become zeros
 	template <typename F>
-	__device__ __forceinline__ void store(unsigned char* lds, int D, F keep) const {
+	__device__ __forceinline__ void store(unsigned char* lds, bool all, F keep) const {
 #pragma unroll
 		for(int n = 0; n < N; n++) {
-			const int  c = threadIdx.x + THREADS * n, row = c / TL::CHUNKS, col = c % TL::CHUNKS;
-			const bool in = keep(row) && col * kind<T>::E < D;
-			u32x4      v = piece[n];
+			u32x4 v = piece[n];
+			if(!all || TL::CHUNKS * E != D) {
+				const bool in = (all || keep(row_of(n))) && col_of(n) * E < D;
 #pragma unroll
-			for(int i = 0; i < 4; i++) {
-				const uint32_t x = v[i];
-				v[i] = in ? x : 0u;
+				for(int i = 0; i < 4; i++) {
+					const uint32_t x = v[i];
+					v[i] = in ? x : 0u;
+				}
 			}
-			*reinterpret_cast<u32x4*>(lds + row * TL::STRIDE + 16 * col) = v;
+			*reinterpret_cast<u32x4*>(lds + row_of(n) * TL::STRIDE + TL::place(row_of(n), col_of(n))) = v;
 		}
 	}
 };
@@ -241,8 +279,17 @@ struct live_keys {
 		return -1;
 	}
 	__device__ __forceinline__ uint32_t word(int i) const { return (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[i]); }
+	__device__ __forceinline__ bool full(int t) const {   // every key of tile t is live
+		uint32_t x = ~0u;
+#pragma unroll
+		for(int i = 0; i < KT / 32; i++) x &= bits[t * (KT / 32) + i];
+		return __builtin_amdgcn_readfirstlane((int)x) == -1;
+	}
 	__device__ __forceinline__ bool keeps(int key) const { return (bits[key >> 5] >> (key & 31)) & 1u; }
 };
+
+// Wavefronts per SIMD that a kernel is to leave room for: three where its accumulators and operands (`registers`) are few, two, or one
+constexpr int wavefronts(int registers) { return registers <= 64 ? 3 : registers <= 136 ? 2 : 1; }
 
 // Workgroups that read the same keys and values on the same XCD (workgroup i runs on XCD i % 8): their numbers, side by side
 __device__ __forceinline__ uint32_t xcd_order(uint32_t i, uint32_t n) {

@@ -8,7 +8,6 @@
 #include "cross_tiles.hpp"
 
 #include <math.h>
-#include <vector>
 
 namespace af3 {
 namespace position {
@@ -47,6 +46,14 @@ __device__ __forceinline__ int passed(const int* border, int n, int d) {   // ho
 }
 __device__ __forceinline__ int bucket_of(const args& a, const int* border, int rel) {
 	return rel <= 0 ? a.first_behind + a.step_behind * passed(border, a.borders, -rel) : a.first_ahead + a.step_ahead * passed(border, a.borders, rel);
+}
+// put(offset, bucket) for all offsets -reach .. reach: thread t writes those between border t - 1 and border t
+template <int N, typename F>
+__device__ __forceinline__ void for_all_offsets(const args& a, const int* border, F put) {
+	for(int t = threadIdx.x; t <= a.borders; t += N) {
+		const int from = t == 0 ? 0 : border[t - 1], to = t < a.borders ? border[t] : a.reach + 1, behind = a.first_behind + a.step_behind * t, ahead = a.first_ahead + a.step_ahead * t;
+		put(from, to, behind, ahead);
+	}
 }
 __device__ __forceinline__ int limited(int64_t rel, int reach) { return rel < -reach ? -reach : rel > reach ? reach : (int)rel; }
 // the difference of two positions, limited where it passes 64 bits
@@ -88,7 +95,17 @@ __global__ void __launch_bounds__(THREADS) position_bias_kernel(args a) {
 	for(int i = threadIdx.x; i < a.borders; i += THREADS) border[i] = a.border[i];
 	__syncthreads();
 	const T* const table = static_cast<const T*>(a.table) + h * a.table_stride[1];
-	for(int i = threadIdx.x; i < (LUT ? 2 * a.reach + 1 : a.buckets); i += THREADS) values[i] = table[(LUT ? bucket_of(a, border, i - a.reach) : i) * a.table_stride[0]];
+	if constexpr(LUT) {
+		for_all_offsets<THREADS>(a, border, [&](int from, int to, int behind, int ahead) {
+			const T at_or_behind = table[behind * a.table_stride[0]], in_front = table[ahead * a.table_stride[0]];
+			for(int d = from; d < to; d++) {
+				values[a.reach - d] = at_or_behind;
+				if(d) values[a.reach + d] = in_front;
+			}
+		});
+	} else {
+		for(int i = threadIdx.x; i < a.buckets; i += THREADS) values[i] = table[i * a.table_stride[0]];
+	}
 	__syncthreads();
 
 	const int     columns = 1 << a.columns_log2, tx = threadIdx.x & (columns - 1), ty = threadIdx.x >> a.columns_log2;
@@ -97,9 +114,13 @@ __global__ void __launch_bounds__(THREADS) position_bias_kernel(args a) {
 	const keys_of_chunk<E> keys(a, col);
 	const int64_t row0 = (int64_t)blockIdx.y * a.rows, last = row0 + a.rows < a.Lq ? row0 + a.rows : a.Lq;
 	T* const      out = static_cast<T*>(a.out) + h * a.Lq * a.Lk + col;
-	for(int64_t row = row0 + ty; row < last; row += THREADS >> a.columns_log2) {
-		int rel[E];
-		keys.offsets(a.q_pos ? a.q_pos[row] : row + a.q_offset, a.reach, rel);
+	const int step = THREADS >> a.columns_log2;
+	int64_t   next = a.q_pos && row0 + ty < last ? a.q_pos[row0 + ty] : 0;   // (a row ahead)
+	for(int64_t row = row0 + ty; row < last; row += step) {
+		int           rel[E];
+		const int64_t q = a.q_pos ? next : row + a.q_offset;
+		if(a.q_pos && row + step < last) next = a.q_pos[row + step];
+		keys.offsets(q, a.reach, rel);
 		T v[E];
 #pragma unroll
 		for(int e = 0; e < E; e++) v[e] = values[LUT ? rel[e] + a.reach : bucket_of(a, border, rel[e])];
@@ -134,50 +155,68 @@ __global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
 	for(int i = 0; i < a.buckets; i++) bins[i * COLUMNS + threadIdx.x] = 0.f;
 	__syncthreads();
 	if constexpr(LUT)
-		for(int i = threadIdx.x; i < 2 * a.reach + 1; i += COLUMNS) bucket[i] = (uint16_t)bucket_of(a, border, i - a.reach);
+		for_all_offsets<COLUMNS>(a, border, [&](int from, int to, int behind, int ahead) {
+			for(int d = from; d < to; d++) {
+				bucket[a.reach - d] = (uint16_t)behind;
+				if(d) bucket[a.reach + d] = (uint16_t)ahead;
+			}
+		});
 	__syncthreads();
 
-	const int     columns = 1 << a.columns_log2, tx = threadIdx.x & (columns - 1), ty = threadIdx.x >> a.columns_log2;
+	const int     columns = 1 << a.columns_log2, tx = threadIdx.x & (columns - 1), ty = threadIdx.x >> a.columns_log2, step = COLUMNS >> a.columns_log2;
 	const int64_t col = ((int64_t)blockIdx.x * columns + tx) * E;
 	if(col < a.Lk) {
+		constexpr int AHEAD = 8;   // rows whose loads are in flight together
 		const keys_of_chunk<E> keys(a, col);
 		const int64_t row0 = (int64_t)blockIdx.y * a.rows, last = row0 + a.rows < a.Lq ? row0 + a.rows : a.Lq;
 		const T* const grad = static_cast<const T*>(a.grad) + h * a.grad_stride[0] + col;
 		float* const   mine = bins + threadIdx.x;
+		const bool     full = col + E <= a.Lk;
 		int   current = 0;
 		float run     = 0.f;   // of bucket `current`, not yet in its bin
-		for(int64_t row = row0 + ty; row < last; row += COLUMNS >> a.columns_log2) {
-			float v[E];
-			const T* const at = grad + row * a.grad_stride[1];
-			if(col + E <= a.Lk) {
-				const u32x4 x = load16(at);
+		for(int64_t first = row0 + ty; first < last; first += AHEAD * step) {
+			u32x4   x[AHEAD];
+			int64_t q[AHEAD];
 #pragma unroll
-				for(int e = 0; e < E; e++) v[e] = kind<T>::at(x, e);
-			} else {
-#pragma unroll
-				for(int e = 0; e < E; e++) {
-					v[e] = 0.f;
-					if(col + e < a.Lk) v[e] = kind<T>::value(at[e]);
-				}
+			for(int i = 0; i < AHEAD; i++) {
+				const int64_t row = first + i * step < last ? first + i * step : first;
+				const T* const at = grad + row * a.grad_stride[1];
+				if(full) x[i] = load16(at);
+				else x[i] = cross::load_guarded(at, 0, (int)(a.Lk - col));
+				q[i] = a.q_pos ? a.q_pos[row] : row + a.q_offset;
 			}
-			int rel[E];
-			keys.offsets(a.q_pos ? a.q_pos[row] : row + a.q_offset, a.reach, rel);
 #pragma unroll
-			for(int e = 0; e < E; e++) {
-				const int bk = LUT ? bucket[rel[e] + a.reach] : bucket_of(a, border, rel[e]);
-				if(bk != current) mine[current * COLUMNS] += run, run = 0.f, current = bk;
-				run += v[e];
+			for(int i = 0; i < AHEAD; i++) {
+				if(first + i * step >= last) break;
+				int rel[E], bk[E];
+				keys.offsets(q[i], a.reach, rel);
+#pragma unroll
+				for(int e = 0; e < E; e++) bk[e] = LUT ? bucket[rel[e] + a.reach] : bucket_of(a, border, rel[e]);
+				bool same = true;
+#pragma unroll
+				for(int e = 0; e < E; e++) same = same && bk[e] == current;
+				if(same) {
+#pragma unroll
+					for(int e = 0; e < E; e++) run += kind<T>::at(x[i], e);
+				} else {
+#pragma unroll
+					for(int e = 0; e < E; e++) {
+						if(bk[e] != current) mine[current * COLUMNS] += run, run = 0.f, current = bk[e];
+						run += kind<T>::at(x[i], e);
+					}
+				}
 			}
 		}
 		mine[current * COLUMNS] += run;
 	}
 	__syncthreads();
 	const int64_t part = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, parts = (int64_t)gridDim.x * gridDim.y;
-	for(int i = 0; i < a.buckets; i++) {
-		float sum = bins[i * COLUMNS + threadIdx.x];
-#pragma unroll
-		for(int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
-		if(threadIdx.x == 0) a.partial[(h * parts + part) * a.buckets + i] = sum;
+	// a bucket per thread; the threads begin with different columns, which are different banks
+	for(int i = threadIdx.x; i < a.buckets; i += COLUMNS) {
+		float sum = 0.f;
+#pragma unroll 16
+		for(int c = 0; c < COLUMNS; c++) sum += bins[i * COLUMNS + ((c + threadIdx.x) & (COLUMNS - 1))];
+		a.partial[(h * parts + part) * a.buckets + i] = sum;
 	}
 }
 template <typename T>
@@ -194,22 +233,49 @@ __global__ void __launch_bounds__(THREADS) position_bias_join_kernel(args a, int
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
-// a^n1 * b^n2 as digits of 32 bits, lowest first
-std::vector<uint32_t> product(uint32_t a, int n1, uint32_t b, int n2) {
-	std::vector<uint32_t> d(1, 1u);
-	for(int i = 0; i < n1 + n2; i++) {
-		const uint64_t f = i < n1 ? a : b;
-		uint64_t       carry = 0;
-		for(uint32_t& x : d) carry += x * f, x = (uint32_t)carry, carry >>= 32;
-		if(carry) d.push_back((uint32_t)carry);
+// whole numbers of any length in digits of 32 bits, lowest first: products of at most MAX_BUCKETS factors
+struct whole {
+	int      n = 1;
+	uint32_t digit[MAX_BUCKETS + 1] = {1u};
+	void times(uint32_t f) {
+		uint64_t carry = 0;
+		for(int i = 0; i < n; i++) carry += (uint64_t)digit[i] * f, digit[i] = (uint32_t)carry, carry >>= 32;
+		if(carry) digit[n++] = (uint32_t)carry;
 	}
-	return d;
+	bool not_less(const whole& b) const {
+		if(n != b.n) return n > b.n;
+		for(int i = n - 1; i >= 0; i--)
+			if(digit[i] != b.digit[i]) return digit[i] > b.digit[i];
+		return true;
+	}
+};
+// d^far >= r^i near^(far - i)
+bool reaches(uint32_t d, uint32_t r, uint32_t near, int i, int far) {
+	whole a, b;
+	for(int k = 0; k < far; k++) a.times(d), b.times(k < i ? r : near);
+	return a.not_less(b);
 }
-bool not_less(const std::vector<uint32_t>& a, const std::vector<uint32_t>& b) {
-	if(a.size() != b.size()) return a.size() > b.size();
-	for(size_t i = a.size(); i-- > 0;)
-		if(a[i] != b[i]) return a[i] > b[i];
-	return true;
+
+// The borders of a set of settings take microseconds to work out; a thread keeps those of its last one.
+struct worked_out {
+	int64_t buckets = 0, max_distance = 0;
+	int32_t both = 0, border[MAX_BUCKETS];
+};
+void log_borders(int64_t buckets, int64_t max_distance, bool both, int32_t* border) {
+	static thread_local worked_out last;
+	const int n = (int)(both ? buckets / 2 : buckets), near = n / 2, far = n - near;
+	if(last.buckets != buckets || last.max_distance != max_distance || last.both != both) {
+		for(int i = 0; i < near; i++) last.border[i] = i + 1;
+		for(int i = 1; i < far; i++) {   // the smallest d with (d / near)^far >= (max_distance / near)^i
+			const long double y = near * powl((long double)max_distance / near, (long double)i / far), r = roundl(y);
+			int               d;
+			if(fabsl(y - r) > 1e-6L) d = (int)ceill(y);
+			else d = (int)r + (reaches((uint32_t)r, (uint32_t)max_distance, (uint32_t)near, i, far) ? 0 : 1);
+			last.border[near + i - 1] = d;
+		}
+		last.buckets = buckets, last.max_distance = max_distance, last.both = both;
+	}
+	for(int i = 0; i < n - 1; i++) border[i] = last.border[i];
 }
 
 int prepare(const af3_position_bias_params* p, args& a) {
@@ -227,17 +293,10 @@ int prepare(const af3_position_bias_params* p, args& a) {
 		a.first_behind = both ? a.borders : 0, a.step_behind = 1, a.first_ahead = both ? a.borders : 0, a.step_ahead = both ? -1 : 0;
 	} else if(p->scheme == AF3_POSITION_LOG) {
 		if(both && p->buckets % 2 != 0) return AF3_ERR_BAD_ARGUMENT;
-		const int n = (int)(both ? p->buckets / 2 : p->buckets), near = n / 2, far = n - near;
+		const int n = (int)(both ? p->buckets / 2 : p->buckets), near = n / 2;
 		if(near < 1 || p->max_distance <= near) return AF3_ERR_BAD_ARGUMENT;
 		a.borders = n - 1;
-		for(int i = 0; i < near; i++) a.border[i] = i + 1;
-		for(int i = 1; i < far; i++) {   // the smallest d with (d / near)^far >= (max_distance / near)^i
-			const long double y = near * powl((long double)p->max_distance / near, (long double)i / far), r = roundl(y);
-			int               d;
-			if(fabsl(y - r) > 1e-6L) d = (int)ceill(y);
-			else d = (int)r + (not_less(product((uint32_t)r, far, 1u, 0), product((uint32_t)p->max_distance, i, (uint32_t)near, far - i)) ? 0 : 1);
-			a.border[near + i - 1] = d;
-		}
+		log_borders(p->buckets, p->max_distance, both, a.border);
 		a.first_behind = 0, a.step_behind = 1, a.first_ahead = both ? n : 0, a.step_ahead = both ? 1 : 0;
 	} else {
 		return AF3_ERR_BAD_ARGUMENT;
