@@ -11,6 +11,9 @@
 
 namespace af3 {
 namespace cross {
+#ifndef FWD_WAVES
+#define FWD_WAVES wavefronts(forward_shape<T, DP, KW>::REGISTERS)
+#endif
 
 struct forward_args {
 	af3_cross_attention_params p;
@@ -47,7 +50,7 @@ struct forward_shape {
 };
 
 template <typename T, int DP, int KW, bool BIAS>
-__global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::REGISTERS)) cross_forward_kernel(forward_args a) {
+__global__ void __launch_bounds__(THREADS, FWD_WAVES) cross_forward_kernel(forward_args a) {
 	using S  = forward_shape<T, DP, KW>;
 	using TL = tile<T, DP>;
 	constexpr int E = kind<T>::E, KT = S::KT;
@@ -58,12 +61,9 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int kwave = wave % KW, rwave = wave / KW;
-	uint32_t  id = xcd_order(blockIdx.x, gridDim.x);
-	const uint32_t row_tile = id % a.row_tiles;
-	id /= a.row_tiles;
-	const uint32_t split = id % a.splits;
-	id /= a.splits;
-	const int64_t b = id / (uint32_t)p.Hkv, hk = id % (uint32_t)p.Hkv;
+	const share    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.row_tiles * a.splits);
+	const uint32_t split = own.piece / a.row_tiles, row_tile = own.piece - split * a.row_tiles;
+	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
 	const int64_t G = p.H / p.Hkv, rows = G * p.Lq;
 	const int     D = (int)p.D;
 
@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 	bool any = false, fresh = true;   // a live key was met; no block yet
 
 	const int64_t last = (int64_t)(split + 1) * a.part < p.Lk ? (int64_t)(split + 1) * a.part : p.Lk;
+	const typename TL::reader at(lane);
 	passage<T, DP, KT> pk, pv;
 	pk.begin(kb, p.k_stride[2], D, a.whole);
 	pv.begin(vb, p.v_stride[2], D, a.whole);
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 				auto  logits = [&] {
 					f32x16 acc{};
 #pragma unroll
-					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(ks, 32 * block, i, lane), qf[i], acc);
+					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(ks, 32 * block, i, at), qf[i], acc);
 #pragma unroll
 					for(int r = 0; r < 16; r++) x[r] = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, bs[s][r]) : acc[r];
 					if(keep[s] != ~0u) {
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 				for(int j = 0; j < TL::JOINTS; j++) {
 					const u32x4 pf = kind<T>::pack(x + E * j);
 #pragma unroll
-					for(int db = 0; db < TL::BLOCKS; db++) o[db] = kind<T>::mma(TL::col_frag(vs, 32 * block, db, j, lane), pf, o[db]);
+					for(int db = 0; db < TL::BLOCKS; db++) o[db] = kind<T>::mma(TL::col_frag(vs, 32 * block, db, j, at), pf, o[db]);
 				}
 			}
 			t = following;
@@ -213,8 +214,8 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 		if(part < PARTS) sums[part * DP + d] = sum;
 		__syncthreads();
 		if(!ok || kwave != 0) return;
-		const int64_t at = split * n_rows + bh * rows + R;
-		if(a.splits > 1 && half == 0) a.part_stat[2 * at] = -INFINITY, a.part_stat[2 * at + 1] = (float)(last - first);
+		const int64_t place = split * n_rows + bh * rows + R;
+		if(a.splits > 1 && half == 0) a.part_stat[2 * place] = -INFINITY, a.part_stat[2 * place + 1] = (float)(last - first);
 		T* const out = static_cast<T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2];
 		for(int db = 0; db < TL::BLOCKS; db++) {
 			float v[16];
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 				for(int i = 0; i < PARTS; i++) v[r] += sums[i * DP + 32 * db + 16 * half + r];
 			}
 			if(a.splits > 1) {
-				store_row16(a.part_out + at * D, 32 * db + 16 * half, D, v);
+				store_row16(a.part_out + place * D, 32 * db + 16 * half, D, v);
 				continue;
 			}
 			for(int r = 0; r < 16; r++) v[r] /= (float)p.Lk;
@@ -272,15 +273,15 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 	if(!ok) return;
 	const bool first_of_row = kwave == 0 && half == 0;
 	if(a.splits > 1) {
-		const int64_t at = split * n_rows + bh * rows + R;
-		if(first_of_row) a.part_stat[2 * at] = m, a.part_stat[2 * at + 1] = l;
+		const int64_t place = split * n_rows + bh * rows + R;
+		if(first_of_row) a.part_stat[2 * place] = m, a.part_stat[2 * place + 1] = l;
 #pragma unroll
 		for(int db = 0; db < TL::BLOCKS; db++) {
 			if(db % KW != kwave) continue;
 			float v[16];
 #pragma unroll
 			for(int r = 0; r < 16; r++) v[r] = o[db][r];
-			store_row16(a.part_out + at * D, 32 * db + 16 * half, D, v);
+			store_row16(a.part_out + place * D, 32 * db + 16 * half, D, v);
 		}
 		return;
 	}

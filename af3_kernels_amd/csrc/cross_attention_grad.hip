@@ -96,12 +96,9 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int kwave = wave % KW, rwave = wave / KW;
-	uint32_t  id = xcd_order(blockIdx.x, gridDim.x);
-	const uint32_t row_tile = id % a.tiles;
-	id /= a.tiles;
-	const uint32_t split = id % a.splits;
-	id /= a.splits;
-	const int64_t b = id / (uint32_t)p.Hkv, hk = id % (uint32_t)p.Hkv;
+	const share    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.tiles * a.splits);
+	const uint32_t split = own.piece / a.tiles, row_tile = own.piece - split * a.tiles;
+	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
 	const int64_t G = p.H / p.Hkv, rows = G * p.Lq;
 	const int     D = (int)p.D;
 
@@ -124,6 +121,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 	for(int db = 0; db < TL::BLOCKS; db++) dq[db] = f32x16{};
 
 	const int64_t last = (int64_t)(split + 1) * a.part < p.Lk ? (int64_t)(split + 1) * a.part : p.Lk;
+	const typename TL::reader at(lane);
 	passage<T, DP, KT> pk, pv;
 	pk.begin(kb, p.k_stride[2], D, a.whole);
 	pv.begin(vb, p.v_stride[2], D, a.whole);
@@ -163,9 +161,9 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 				if(keep == 0u) continue;
 				f32x16 acc{}, dp{};
 #pragma unroll
-				for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(ks, 32 * block, i, lane), qf[i], acc);
+				for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(ks, 32 * block, i, at), qf[i], acc);
 #pragma unroll
-				for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(vs, 32 * block, i, lane), gf[i], dp);
+				for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(vs, 32 * block, i, at), gf[i], dp);
 				float x[16];
 #pragma unroll
 				for(int r = 0; r < 16; r++) {
@@ -181,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 				for(int j = 0; j < TL::JOINTS; j++) {
 					const u32x4 f = kind<T>::pack(x + E * j);
 #pragma unroll
-					for(int db = 0; db < TL::BLOCKS; db++) dq[db] = kind<T>::mma(TL::col_frag(ks, 32 * block, db, j, lane), f, dq[db]);
+					for(int db = 0; db < TL::BLOCKS; db++) dq[db] = kind<T>::mma(TL::col_frag(ks, 32 * block, db, j, at), f, dq[db]);
 				}
 			}
 			t = following;
@@ -240,12 +238,9 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int rwave = wave % RW, kwave = wave / RW;
-	uint32_t  id = xcd_order(blockIdx.x, gridDim.x);
-	const uint32_t key_tile = id % a.tiles;
-	id /= a.tiles;
-	const uint32_t split = id % a.splits;
-	id /= a.splits;
-	const int64_t b = id / (uint32_t)p.Hkv, hk = id % (uint32_t)p.Hkv;
+	const share    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.tiles * a.splits);
+	const uint32_t split = own.piece / a.tiles, key_tile = own.piece - split * a.tiles;
+	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
 	const int64_t G = p.H / p.Hkv;
 	const int     D = (int)p.D;
 
@@ -264,6 +259,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 
 	const int64_t q_tiles = (p.Lq + QT - 1) / QT, n = G * q_tiles;
 	const int64_t last = (int64_t)(split + 1) * a.part < n ? (int64_t)(split + 1) * a.part : n;
+	const typename TL::reader at(lane);
 	passage<T, DP, QT> pq, pg;
 	pq.begin(nullptr, p.q_stride[2], D, a.whole);
 	pg.begin(nullptr, a.g.grad_out_stride[2], D, a.whole);
@@ -311,16 +307,16 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 				} else {
 					f32x16 acc{}, dp{};
 #pragma unroll
-					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, row0, i, lane), kf[i], acc);
+					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, row0, i, at), kf[i], acc);
 #pragma unroll
-					for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, row0, i, lane), vf[i], dp);
+					for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, row0, i, at), vf[i], dp);
 					float bs[16];
 					if constexpr(BIAS) {
-						const T* const at = static_cast<const T*>(p.bias) + h * p.bias_stride[0] + (in ? key : 0);
+						const T* const column = static_cast<const T*>(p.bias) + h * p.bias_stride[0] + (in ? key : 0);
 #pragma unroll
 						for(int r = 0; r < 16; r++) {
 							const int64_t q = q0 + row0 + 16 * half + r;
-							const float   v = kind<T>::value(at[(q < p.Lq ? q : 0) * p.bias_stride[1]]);
+							const float   v = kind<T>::value(column[(q < p.Lq ? q : 0) * p.bias_stride[1]]);
 							bs[r] = q < p.Lq ? v : 0.f;
 						}
 					}
@@ -336,8 +332,8 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 					const u32x4 pf = kind<T>::pack(x + E * j), df = kind<T>::pack(y + E * j);
 #pragma unroll
 					for(int db = 0; db < TL::BLOCKS; db++) {
-						dv[db] = kind<T>::mma(TL::col_frag(gs, row0, db, j, lane), pf, dv[db]);
-						dk[db] = kind<T>::mma(TL::col_frag(qs, row0, db, j, lane), df, dk[db]);
+						dv[db] = kind<T>::mma(TL::col_frag(gs, row0, db, j, at), pf, dv[db]);
+						dk[db] = kind<T>::mma(TL::col_frag(qs, row0, db, j, at), df, dk[db]);
 					}
 				}
 			}
@@ -352,7 +348,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 		add_up<DP, RW>(tables, rwave, lane, dk);
 	}
 	if(!in) return;
-	const int64_t at = (b * p.Hkv + hk) * p.Lk + key, n_keys = p.B * p.Hkv * p.Lk;
+	const int64_t place = (b * p.Hkv + hk) * p.Lk + key, n_keys = p.B * p.Hkv * p.Lk;
 	const bool    counts_v = lives || dead, counts_k = lives && !dead;
 #pragma unroll
 	for(int db = 0; db < TL::BLOCKS; db++) {
@@ -361,11 +357,11 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 #pragma unroll
 		for(int r = 0; r < 16; r++) v[r] = counts_v ? dv[db][r] : 0.f, k[r] = counts_k ? dk[db][r] * p.softmax_scale : 0.f;
 		if(a.splits > 1) {
-			store_row16(a.partial + (2 * split * n_keys + at) * D, 32 * db + 16 * half, D, k);
-			store_row16(a.partial + ((2 * split + 1) * n_keys + at) * D, 32 * db + 16 * half, D, v);
+			store_row16(a.partial + (2 * split * n_keys + place) * D, 32 * db + 16 * half, D, k);
+			store_row16(a.partial + ((2 * split + 1) * n_keys + place) * D, 32 * db + 16 * half, D, v);
 		} else {
-			if(a.g.grad_k) store_row16(static_cast<T*>(a.g.grad_k) + at * D, 32 * db + 16 * half, D, k);
-			if(a.g.grad_v) store_row16(static_cast<T*>(a.g.grad_v) + at * D, 32 * db + 16 * half, D, v);
+			if(a.g.grad_k) store_row16(static_cast<T*>(a.g.grad_k) + place * D, 32 * db + 16 * half, D, k);
+			if(a.g.grad_v) store_row16(static_cast<T*>(a.g.grad_v) + place * D, 32 * db + 16 * half, D, v);
 		}
 	}
 }
@@ -421,10 +417,9 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const uint32_t key_tiles = (uint32_t)((p.Lk + S::KEYS - 1) / S::KEYS);
-	uint32_t       id = xcd_order(blockIdx.x, gridDim.x);
-	const uint32_t key_tile = id % key_tiles;
-	id /= key_tiles;
-	const int64_t  q0 = (int64_t)(id % a.tiles) * QT, h = id / a.tiles, hk = h / (p.H / p.Hkv);
+	const share    own((uint32_t)blockIdx.x, (uint32_t)p.H, a.tiles * key_tiles);
+	const uint32_t q_tile = own.piece / key_tiles, key_tile = own.piece - q_tile * key_tiles;
+	const int64_t  q0 = (int64_t)q_tile * QT, h = own.pair, hk = h / (p.H / p.Hkv);
 	const int      D = (int)p.D;
 	const int64_t  key = (int64_t)key_tile * S::KEYS + 32 * wave + (lane & 31);
 	const bool     in = key < p.Lk;
@@ -438,6 +433,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 			sum[s][r] = 0.f, bs[s][r] = 0.f;
 			if(in && q < p.Lq) bs[s][r] = kind<T>::value(static_cast<const T*>(p.bias)[h * p.bias_stride[0] + q * p.bias_stride[1] + key]);
 		}
+	const typename TL::reader at(lane);
 	passage<T, DP, QT> pq, pg;
 	pq.begin(nullptr, p.q_stride[2], D, a.whole);
 	pg.begin(nullptr, a.g.grad_out_stride[2], D, a.whole);
@@ -475,9 +471,9 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 			for(int s = 0; s < S::SUB; s++) {
 				f32x16 acc{}, dp{};
 #pragma unroll
-				for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, 32 * s, i, lane), kf[i], acc);
+				for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, 32 * s, i, at), kf[i], acc);
 #pragma unroll
-				for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, 32 * s, i, lane), vf[i], dp);
+				for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, 32 * s, i, at), vf[i], dp);
 				const float* const sm = st + 32 * s + 16 * half;
 #pragma unroll
 				for(int r = 0; r < 16; r++) {

@@ -103,38 +103,49 @@ __device__ __forceinline__ float maximum_of_halves(float x) {
 template <typename T, int DP>
 struct tile {
 	static constexpr int STRIDE = DP * (int)sizeof(T), STEPS = DP * (int)sizeof(T) / 32, BLOCKS = DP / 32, CHUNKS = DP * (int)sizeof(T) / 16, JOINTS = 32 / (2 * kind<T>::E);
-	// where piece `chunk` of a row lies
-	static __device__ __forceinline__ int place(int row, int chunk) {
+	// where piece `chunk` of a row lies: 16 (chunk ^ turn(row)), in a part of a row that begins at a multiple of SPAN
+	static constexpr int SPAN = STRIDE % 256 == 0 ? 256 : STRIDE % 128 == 0 ? 128 : 64;
+	static constexpr __device__ __forceinline__ int turn(int row) {
 		const int b0 = row & 1, b1 = (row >> 1) & 1, b2 = (row >> 2) & 1, b4 = (row >> 4) & 1;
-		if constexpr(STRIDE % 256 == 0) return 16 * (chunk ^ (sizeof(T) == 2 ? 8 * b0 | 4 * b1 | 2 * b4 | b2 : 8 * b4 | 4 * b0 | 2 * b1 | b2));
-		else if constexpr(STRIDE % 128 == 0) return 16 * (chunk ^ (4 * b1 | 2 * b4 | b2));
-		else return 16 * (chunk ^ (2 * b4 | b2));
+		return SPAN == 256 ? (sizeof(T) == 2 ? 8 * b0 | 4 * b1 | 2 * b4 | b2 : 8 * b4 | 4 * b0 | 2 * b1 | b2) : SPAN == 128 ? 4 * b1 | 2 * b4 | b2 : 2 * b4 | b2;
 	}
+	static __device__ __forceinline__ int place(int row, int chunk) { return 16 * (chunk ^ turn(row)); }
+	// Two numbers per lane that all its reads begin with: a read's own place is an exclusive or and a constant away.
+	struct reader {
+		int row, col;
+		__device__ __forceinline__ explicit reader(int lane) {
+			const int r = tile_row(lane & 31), half = lane >> 5;
+			row = r * STRIDE + place(r, half);
+			if constexpr(sizeof(T) == 2) {
+				// (ds_read_b64_tr_b16: lane i of a group of 16 supplies 4 columns of row i / 4 and receives 4 rows of the group's column i)
+				const int i = lane & 15, G = lane >> 4, c = 16 * (G >> 1) + (i >> 2);
+				col = c * STRIDE + place(c, 2 * (i & 1) + (G & 1)) + 8 * ((i >> 1) & 1);
+			} else {
+				col = 16 * half * STRIDE + place(16 * half, r >> 2) + 4 * (r & 3);
+			}
+		}
+		// what follows is worked out anew, not kept in registers from the last time
+		__device__ __forceinline__ void forget() { asm volatile("" : "+v"(row), "+v"(col)); }
+	};
 	// contraction over the columns: A operand, step s, of the 32 rows from `row0` (a multiple of 32) on
-	static __device__ __forceinline__ u32x4 row_frag(const unsigned char* lds, int row0, int s, int lane) {
-		const int row = tile_row(lane & 31);
-		return *reinterpret_cast<const u32x4*>(lds + row0 * STRIDE + row * STRIDE + place(row, 2 * s + (lane >> 5)));
+	static __device__ __forceinline__ u32x4 row_frag(const unsigned char* lds, int row0, int s, const reader& at) {
+		return *reinterpret_cast<const u32x4*>(lds + row0 * STRIDE + (at.row ^ (32 * s & (SPAN - 1))) + (32 * s & ~(SPAN - 1)));
 	}
 	// contraction over the 32 rows from `row0` on: A operand, step j, of columns 32 db .. 32 db + 31
-	static __device__ __forceinline__ u32x4 col_frag(const unsigned char* lds, int row0, int db, int j, int lane) {
+	static __device__ __forceinline__ u32x4 col_frag(const unsigned char* lds, int row0, int db, int j, const reader& at) {
+		constexpr int W = 32 * (int)sizeof(T);
+		u32x4         f;
 		if constexpr(sizeof(T) == 2) {
-			// (ds_read_b64_tr_b16: lane i of a group of 16 supplies 4 columns of row i / 4 and receives 4 rows of the group's column i)
-			const int i = lane & 15, G = lane >> 4, row = 16 * (G >> 1) + (i >> 2);
-			u32x4     f;
 #pragma unroll
 			for(int t = 0; t < 2; t++) {
-				const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + (row0 + 8 * j + row + 4 * t) * STRIDE +
-																	place(row + 4 * t, 4 * db + 2 * (i & 1) + (G & 1)) + 8 * ((i >> 1) & 1))));
+				const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + row0 * STRIDE + (8 * j + 4 * t) * STRIDE + (at.col ^ ((W * db & (SPAN - 1)) | 16 * turn(4 * t))) + (W * db & ~(SPAN - 1)))));
 				f[2 * t] = r[0], f[2 * t + 1] = r[1];
 			}
-			return f;
 		} else {
-			const int col = 32 * db + tile_row(lane & 31), half = 16 * (lane >> 5);
-			u32x4     f;
 #pragma unroll
-			for(int t = 0; t < 4; t++) f[t] = *reinterpret_cast<const uint32_t*>(lds + (row0 + half + 4 * j + t) * STRIDE + place(half + 4 * j + t, col >> 2) + 4 * (col & 3));
-			return f;
+			for(int t = 0; t < 4; t++) f[t] = *reinterpret_cast<const uint32_t*>(lds + row0 * STRIDE + (4 * j + t) * STRIDE + (at.col ^ ((W * db & (SPAN - 1)) ^ 16 * turn(4 * j + t))) + (W * db & ~(SPAN - 1)));
 		}
+		return f;
 	}
 };
 
@@ -204,6 +215,19 @@ __device__ __forceinline__ void load_operand(u32x4 (&f)[N], const T* row, bool o
 	}
 }
 
+// 16 entries of a row from `first` on, those from L on 0 (`row` is the row's first entry)
+template <typename T, int N>
+__device__ __forceinline__ void load_row16_raw(u32x4 (&out)[N], const T* row, int64_t first, int64_t L) {
+	constexpr int E = kind<T>::E;
+	static_assert(N == 16 / E);
+	if(first + 16 <= L) {
+#pragma unroll
+		for(int i = 0; i < N; i++) out[i] = load16(row + first + E * i);
+	} else {
+#pragma unroll
+		for(int i = 0; i < N; i++) out[i] = first + E * i < L ? load_guarded(row + first + E * i, 0, L - first - E * i < E ? (int)(L - first - E * i) : E) : u32x4{0u, 0u, 0u, 0u};
+	}
+}
 // 16 entries of a row from `first` on as floats, those from L on left at 0 (`row` is the row's first entry)
 template <typename T>
 __device__ __forceinline__ void load_row16(float (&out)[16], const T* row, int64_t first, int64_t L) {
@@ -289,13 +313,23 @@ struct live_keys {
 };
 
 // Wavefronts per SIMD that a kernel is to leave room for: three where its accumulators and operands (`registers`) are few, two, or one
-constexpr int wavefronts(int registers) { return registers <= 64 ? 3 : registers <= 136 ? 2 : 1; }
+constexpr int wavefronts(int registers) { return registers <= 48 ? 3 : registers <= 136 ? 2 : 1; }
 
-// Workgroups that read the same keys and values on the same XCD (workgroup i runs on XCD i % 8): their numbers, side by side
-__device__ __forceinline__ uint32_t xcd_order(uint32_t i, uint32_t n) {
-	const uint32_t whole = n & ~7u;
-	return i < whole ? (i & 7u) * (whole >> 3) + (i >> 3) : i;
-}
+// Which (batch, key head) a workgroup works on, and which of its `each` pieces.  Workgroup i runs on XCD i % 8, whose L2 the pieces of one pair share; a pair goes to an XCD
+// whole where the pairs divide evenly, and consecutive eights of pairs are turned against each other, so that batch rows of few keys and of many are
+// dealt out evenly too (by stretches of consecutive pairs, 8 batch rows of 0.5 to 1 of 1024 keys each had their own XCD: a third of the chip idle).
+struct share {
+	uint32_t pair, piece;
+	__device__ __forceinline__ share(uint32_t i, uint32_t pairs, uint32_t each) {
+		if((pairs & 7u) == 0u) {
+			const uint32_t xcd = i & 7u, turn = (i >> 3) / each;
+			piece = (i >> 3) - turn * each, pair = 8u * turn + ((xcd - turn) & 7u);
+		} else {
+			const uint32_t n = pairs * each, whole = n & ~7u, k = i < whole ? (i & 7u) * (whole >> 3) + (i >> 3) : i;
+			pair = k / each, piece = k - pair * each;
+		}
+	}
+};
 
 }  // namespace cross
 }  // namespace af3
