@@ -11,9 +11,6 @@
 
 namespace af3 {
 namespace cross {
-#ifndef FWD_WAVES
-#define FWD_WAVES wavefronts(forward_shape<T, DP, KW>::REGISTERS)
-#endif
 
 struct forward_args {
 	af3_cross_attention_params p;
@@ -50,7 +47,7 @@ struct forward_shape {
 };
 
 template <typename T, int DP, int KW, bool BIAS>
-__global__ void __launch_bounds__(THREADS, FWD_WAVES) cross_forward_kernel(forward_args a) {
+__global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::REGISTERS)) cross_forward_kernel(forward_args a) {
 	using S  = forward_shape<T, DP, KW>;
 	using TL = tile<T, DP>;
 	constexpr int E = kind<T>::E, KT = S::KT;
@@ -356,6 +353,12 @@ __global__ void __launch_bounds__(THREADS) cross_join_kernel(forward_args a) {
 	if(p.stats && lane == 0) p.stats[2 * row] = dead ? -INFINITY : top, p.stats[2 * row + 1] = inv;
 }
 
+// the most wavefronts that can share rows: four, where the tiles of 128 keys leave registers for the rest
+template <typename T, int DP>
+constexpr int MOST_SHARING = 512 * tile<T, DP>::STRIDE <= 131072 ? 4 : 2;
+int most_sharing(const af3_cross_attention_params& p) { return p.dtype == AF3_F32 && p.D > 64 ? MOST_SHARING<float, 128> : 4; }
+static_assert(MOST_SHARING<uint16_t, 128> == 4 && MOST_SHARING<float, 64> == 4 && MOST_SHARING<float, 96> == 2 && MOST_SHARING<float, 128> == 2);
+
 // ---- host side -------------------------------------------------------------------------------------------------------------
 struct plan {
 	int      kw;
@@ -363,17 +366,20 @@ struct plan {
 	int64_t  part;
 };
 
+// As many wavefronts share rows as leave no more workgroups than fit the chip together, so that a short launch fills it: us of one, two and four sharing, at
+// B x H x Lq x Lk x D of 4 x 16 x 384 x 1491 x 64 33.5, 28.2, 40.6 (192, 384 and 768 workgroups), 1 x 16 x 1491 x 4096 x 128 134, 106, 195 (192, 384, 752), 8 x 12 x 512 x 512 x 64
+// 18.7, 18.2, 31.9 (384, 768, 1536), 1 x 8 x 1024 x 1024 x 64 19.8, 16.7, 13.6 (64, 128, 256), fp32 4 x 8 x 200 x 768 x 32 38.9, 26.1, 18.0.
 plan forward_plan(const af3_cross_attention_params& p) {
 	plan          f;
 	const int64_t rows = p.H / p.Hkv * p.Lq, groups = p.B * p.Hkv;
-	auto          tiles = [&](int64_t per) { return (rows + per - 1) / per; };
-	f.kw        = rows <= 32 || tiles(128) * groups < 256 ? 4 : 1;
-	f.row_tiles = (uint32_t)tiles(f.kw == 4 ? 32 : 128);
-	const int64_t kt = f.kw == 4 ? 128 : 64, key_tiles = (p.Lk + kt - 1) / kt, busy = groups * f.row_tiles;
-	int64_t       splits = busy >= 512 ? 1 : (512 + busy - 1) / busy;
-	if(splits > (key_tiles + 1) / 2) splits = (key_tiles + 1) / 2;   // (at least two tiles to a part)
-	if(splits > MAX_PARTS) splits = MAX_PARTS;
-	if(splits < 1) splits = 1;
+	const bool    fp32 = p.dtype == AF3_F32;
+	auto          busy = [&](int kw) { return (rows + 128 / kw - 1) / (128 / kw) * groups; };
+	f.kw = rows <= 32 || busy(4) <= 512 ? 4 : rows <= 64 || busy(2) <= 512 ? 2 : 1;
+	if(f.kw > most_sharing(p)) f.kw = most_sharing(p);
+	f.row_tiles = (uint32_t)(busy(f.kw) / groups);
+	const int64_t kt = f.kw == 4 ? 128 : 64, key_tiles = (p.Lk + kt - 1) / kt;
+	const double  tile_us = (0.4 + 0.011 * p.D) * (f.kw == 4 ? 1.0 : 0.6) * (fp32 ? 3.0 : 1.0);
+	const int64_t splits = parts_for(busy(f.kw), p.D > 64 || (fp32 && p.D > 32) ? 256 : 512, key_tiles, tile_us, 4.0 * p.B * p.H * p.Lq * p.D, MAX_PARTS);
 	const int64_t per = (key_tiles + splits - 1) / splits;
 	f.part   = per * kt;
 	f.splits = (uint32_t)((key_tiles + per - 1) / per);
@@ -393,7 +399,9 @@ int launch_forward(const forward_args& a, uint32_t grid, hipStream_t s) {
 }
 template <typename T, int DP>
 int launch_forward_form(const forward_args& a, int kw, uint32_t grid, hipStream_t s) {
-	if(kw == 4) return a.p.bias ? launch_forward<T, DP, 4, true>(a, grid, s) : launch_forward<T, DP, 4, false>(a, grid, s);
+	if constexpr(MOST_SHARING<T, DP> == 4)
+		if(kw == 4) return a.p.bias ? launch_forward<T, DP, 4, true>(a, grid, s) : launch_forward<T, DP, 4, false>(a, grid, s);
+	if(kw == 2) return a.p.bias ? launch_forward<T, DP, 2, true>(a, grid, s) : launch_forward<T, DP, 2, false>(a, grid, s);
 	return a.p.bias ? launch_forward<T, DP, 1, true>(a, grid, s) : launch_forward<T, DP, 1, false>(a, grid, s);
 }
 template <typename T>

@@ -508,28 +508,32 @@ struct cut {
 };
 inline int64_t over(int64_t n, int64_t per) { return (n + per - 1) / per; }
 
-// `length` rows that results belong to (128 or 32 of them per workgroup), `steps(shared)` tiles of the other axis
+// `length` rows that results belong to (128 or 32 of them per workgroup), `steps(shared)` tiles of the other axis.  Wavefronts share where the workgroups of 32 fit the chip
+// together: dQ / dK and dV, us, alone and shared, at 2 x 8 x 384 x 1024 x 64 20.6, 14.2 / 17.6, 13.0, 1 x 8 x 1024 x 1024 x 64 25.8, 17.3 / 38.3, 19.6 (256 workgroups of 32),
+// 8 x 12 x 512 x 512 x 64 25.0, 43.0 / 29.5, 43.8 (1536), fp32 2 x 8 x 259 x 384 x 32 25.3, 14.9 / 31.4, 15.8.
 template <typename F>
-cut cut_for(int64_t length, int64_t groups, bool may_share, F steps) {
+cut cut_for(int64_t length, int64_t groups, bool may_share, int64_t slots, double tile_us, double part_bytes, F steps) {
 	cut c;
-	c.shared = may_share && (length <= 32 || over(length, 128) * groups < 256);
+	c.shared = may_share && (length <= 32 || over(length, 32) * groups <= 512);
 	c.tiles  = (uint32_t)over(length, c.shared ? 32 : 128);
-	const int64_t n = steps(c.shared), busy = groups * c.tiles;
-	int64_t       splits = busy >= 512 ? 1 : over(512, busy);
-	if(splits > (n + 1) / 2) splits = (n + 1) / 2;
-	if(splits < 1) splits = 1;
-	c.part   = over(n, splits);
+	const int64_t n = steps(c.shared);
+	const int64_t sp = parts_for(groups * c.tiles, slots, n, tile_us * (c.shared ? 1.0 : 0.6), part_bytes, 64);
+	c.part   = over(n, sp);
 	c.splits = (uint32_t)over(n, c.part);
 	return c;
 }
 cut dq_cut(const af3_cross_attention_params& p) {
-	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, true, [&](bool shared) { return over(p.Lk, shared ? 128 : 64); });
+	const bool fp32 = p.dtype == AF3_F32;
+	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, true, p.D > 64 || (fp32 && p.D > 32) ? 256 : 512, (0.5 + 0.016 * p.D) * (fp32 ? 3.0 : 1.0), 4.0 * p.B * p.H * p.Lq * p.D,
+					[&](bool shared) { return over(p.Lk, shared ? 128 : 64); });
 	c.part *= c.shared ? 128 : 64;
 	return c;
 }
 cut dkv_cut(const af3_cross_attention_params& p) {
 	// (fp32 beyond 64 columns: the tile of 128 rows leaves no registers for the sums)
-	return cut_for(p.Lk, p.B * p.Hkv, p.dtype == AF3_BF16 || p.D <= 64, [&](bool shared) { return p.H / p.Hkv * over(p.Lq, shared ? 128 : p.dtype == AF3_F32 ? 32 : 64); });
+	const bool fp32 = p.dtype == AF3_F32;
+	return cut_for(p.Lk, p.B * p.Hkv, !fp32 || p.D <= 64, p.D > 64 || (fp32 && p.D > 32) ? 256 : 512, (0.6 + 0.022 * p.D) * (fp32 ? 3.0 : 1.0), 8.0 * p.B * p.Hkv * p.Lk * p.D,
+				   [&](bool shared) { return p.H / p.Hkv * over(p.Lq, shared ? 128 : fp32 ? 32 : 64); });
 }
 
 struct grad_space {

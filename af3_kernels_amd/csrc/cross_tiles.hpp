@@ -315,6 +315,19 @@ struct live_keys {
 // Wavefronts per SIMD that a kernel is to leave room for: three where its accumulators and operands (`registers`) are few, two, or one
 constexpr int wavefronts(int registers) { return registers <= 48 ? 3 : registers <= 136 ? 2 : 1; }
 
+// Into how many parts the long axis of a launch goes: `workgroups` of them walk `tiles` tiles each, `tile_us` apiece, and `slots` fit the chip at a time; a part more
+// costs its results' way through memory (`part_bytes`, out and in again) and the kernel that joins them.  The parts of the smallest sum, of two tiles at least.
+inline uint32_t parts_for(int64_t workgroups, int64_t slots, int64_t tiles, double tile_us, double part_bytes, int64_t most) {
+	constexpr double JOIN_US = 6.0, BYTES_PER_US = 2e6;   // (measured: 6 us with its launch; 2 TB/s)
+	double   best = 0.0;
+	uint32_t parts = 1;
+	for(int64_t n = 1; n <= most && (n == 1 || (2 * n <= tiles + 1 && workgroups * n <= slots)); n++) {
+		const double us = (double)((tiles + n - 1) / n) * tile_us + (n > 1 ? JOIN_US + n * 2.0 * part_bytes / BYTES_PER_US : 0.0);
+		if(n == 1 || us < best) best = us, parts = (uint32_t)n;
+	}
+	return parts;
+}
+
 // Which (batch, key head) a workgroup works on, and which of its `each` pieces.  Workgroup i runs on XCD i % 8, whose L2 the pieces of one pair share; a pair goes to an XCD
 // whole where the pairs divide evenly, and consecutive eights of pairs are turned against each other, so that batch rows of few keys and of many are
 // dealt out evenly too (by stretches of consecutive pairs, 8 batch rows of 0.5 to 1 of 1024 keys each had their own XCD: a third of the chip idle).
