@@ -96,14 +96,23 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 		any = true;
 		pk.load(first + (int64_t)t * KT, end);
 		pv.load(first + (int64_t)t * KT, end);
-		while(t >= 0) {
-			unsigned char* const ks = smem + buffer * 2 * S::TILE;
-			unsigned char* const vs = ks + S::TILE;
-			float bs[BIAS ? S::SUB : 1][16];
+		u32x4 bs[S::SUB][16 / E], coming[S::SUB][16 / E];   // biases of this tile and of the one behind it
+		auto  fetch_bias = [&](u32x4(&to)[S::SUB][16 / E], int tile_no) {
 			if constexpr(BIAS) {
 #pragma unroll
-				for(int s = 0; s < S::SUB; s++) load_row16(bs[s], bias, first + (int64_t)t * KT + 32 * (kwave * S::SUB + s) + 16 * half, p.Lk);
+				for(int s = 0; s < S::SUB; s++) load_row16_raw(to[s], bias, first + (int64_t)tile_no * KT + 32 * (kwave * S::SUB + s) + 16 * half, p.Lk);
 			}
+		};
+		fetch_bias(coming, t);
+		while(t >= 0) {
+			if constexpr(BIAS) {
+#pragma unroll
+				for(int s = 0; s < S::SUB; s++)
+#pragma unroll
+					for(int i = 0; i < 16 / E; i++) bs[s][i] = coming[s][i];
+			}
+			unsigned char* const ks = smem + buffer * 2 * S::TILE;
+			unsigned char* const vs = ks + S::TILE;
 			const bool full = live.full(t);
 			uint32_t   keep[S::SUB];
 #pragma unroll
@@ -116,6 +125,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 			if(following >= 0) {
 				pk.load(first + (int64_t)following * KT, end);
 				pv.load(first + (int64_t)following * KT, end);
+				fetch_bias(coming, following);
 			}
 #pragma unroll
 			for(int s = 0; s < S::SUB; s++) {
@@ -127,12 +137,8 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 #pragma unroll
 					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(ks, 32 * block, i, at), qf[i], acc);
 #pragma unroll
-					for(int r = 0; r < 16; r++) x[r] = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, bs[s][r]) : acc[r];
-					if(keep[s] != ~0u) {
-						const uint32_t mine = keep[s] >> (16 * half);
-#pragma unroll
-						for(int r = 0; r < 16; r++) x[r] = (mine >> r) & 1u ? x[r] : -INFINITY;
-					}
+					for(int r = 0; r < 16; r++) x[r] = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, kind<T>::at(bs[s][r / E], r % E)) : acc[r];
+					if(keep[s] != ~0u) drop_keys(x, keep[s], -INFINITY);
 				};
 				auto probabilities = [&]() -> float {
 					float sum = 0.f;

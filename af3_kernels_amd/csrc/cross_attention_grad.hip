@@ -6,7 +6,7 @@
 // of a result is summed by one workgroup, or by one per part of the long axis and a joining kernel, always in the same order.
 //   cross_dq_kernel    32 query rows per wavefront, keys in tiles (writes delta too)
 //   cross_dkv_kernel   32 keys per wavefront, query rows in tiles, over all query heads of the key head
-//   cross_dbias_kernel 64 query rows x 32 keys per wavefront, over the batch
+//   cross_dbias_kernel 32 query rows x 32 keys per wavefront, over the batch
 #include "cross_tiles.hpp"
 
 #include <math.h>
@@ -133,14 +133,23 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 		if(t < 0) continue;
 		pk.load(first + (int64_t)t * KT, end);
 		pv.load(first + (int64_t)t * KT, end);
-		while(t >= 0) {
-			unsigned char* const ks = smem + buffer * 2 * S::TILE;
-			unsigned char* const vs = ks + S::TILE;
-			float bs[BIAS ? S::SUB : 1][16];
+		u32x4 bs[S::SUB][16 / E], coming[S::SUB][16 / E];   // biases of this tile and of the one behind it
+		auto  fetch_bias = [&](u32x4(&to)[S::SUB][16 / E], int tile_no) {
 			if constexpr(BIAS) {
 #pragma unroll
-				for(int s = 0; s < S::SUB; s++) load_row16(bs[s], bias, first + (int64_t)t * KT + 32 * (kwave * S::SUB + s) + 16 * half, p.Lk);
+				for(int s = 0; s < S::SUB; s++) load_row16_raw(to[s], bias, first + (int64_t)tile_no * KT + 32 * (kwave * S::SUB + s) + 16 * half, p.Lk);
 			}
+		};
+		fetch_bias(coming, t);
+		while(t >= 0) {
+			if constexpr(BIAS) {
+#pragma unroll
+				for(int s = 0; s < S::SUB; s++)
+#pragma unroll
+					for(int i = 0; i < 16 / E; i++) bs[s][i] = coming[s][i];
+			}
+			unsigned char* const ks = smem + buffer * 2 * S::TILE;
+			unsigned char* const vs = ks + S::TILE;
 			const bool full = live.full(t);
 			uint32_t   keeps[S::SUB];
 #pragma unroll
@@ -153,6 +162,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 			if(following >= 0) {
 				pk.load(first + (int64_t)following * KT, end);
 				pv.load(first + (int64_t)following * KT, end);
+				fetch_bias(coming, following);
 			}
 #pragma unroll
 			for(int s = 0; s < S::SUB; s++) {
@@ -167,14 +177,10 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 				float x[16];
 #pragma unroll
 				for(int r = 0; r < 16; r++) {
-					const float t0 = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, bs[s][r]) : acc[r];
+					const float t0 = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, kind<T>::at(bs[s][r / E], r % E)) : acc[r];
 					x[r] = __builtin_amdgcn_exp2f((t0 - m) * a.factor) * inv * (dp[r] - delta);
 				}
-				if(keep != ~0u) {
-					const uint32_t mine = keep >> (16 * half);
-#pragma unroll
-					for(int r = 0; r < 16; r++) x[r] = (mine >> r) & 1u ? x[r] : 0.f;
-				}
+				if(keep != ~0u) drop_keys(x, keep, 0.f);
 #pragma unroll
 				for(int j = 0; j < TL::JOINTS; j++) {
 					const u32x4 f = kind<T>::pack(x + E * j);
@@ -218,20 +224,23 @@ __global__ void __launch_bounds__(THREADS) cross_delta_kernel(grad_args a) {
 
 // ---- dK, dV ----
 // RW: wavefronts that share 32 keys and each take 32 rows of a tile of query rows (1: every wavefront has its own keys and takes the whole tile)
-template <typename T, int DP, int RW>
+// A bias comes through LDS as well, read like the columns of dO: a lane's 16 values lie in one column, and taken from memory one by one they were two thirds of the
+// kernel's time (8 x 12 x 512 x 512 x 64: 102 us with a bias, 29 without).
+template <typename T, int DP, int RW, bool BIAS>
 struct dkv_shape {
 	static constexpr int QT = RW == 4 ? 128 : sizeof(T) == 2 ? 64 : 32, SUB = QT / (32 * RW), KEYS = 32 * (WAVES / RW);
-	static constexpr int TILE = QT * tile<T, DP>::STRIDE, STATS = 3 * QT * 4, SET = 2 * TILE + STATS;
+	static constexpr int TILE = QT * tile<T, DP>::STRIDE, STATS = 3 * QT * 4, BIASES = BIAS ? QT * tile<T, KEYS>::STRIDE : 0, SET = 2 * TILE + BIASES + STATS;
 	static constexpr int BUFFERS = 2 * SET <= 81920 ? 2 : 1;
 	static constexpr int JOIN = RW > 1 ? WAVES * 32 * (DP + 4) * 4 : 0;
 	static constexpr int LDS = BUFFERS * SET > JOIN ? BUFFERS * SET : JOIN;
-	static constexpr int REGISTERS = 8 * tile<T, DP>::STEPS + DP + 8 * passage<T, DP, QT>::N;
+	static constexpr int REGISTERS = 8 * tile<T, DP>::STEPS + DP + 8 * passage<T, DP, QT>::N + (BIAS ? 4 * passage<T, KEYS, QT>::N : 0);
 };
 
 template <typename T, int DP, int RW, bool BIAS>
-__global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGISTERS)) cross_dkv_kernel(grad_args a) {
-	using S  = dkv_shape<T, DP, RW>;
+__global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW, BIAS>::REGISTERS)) cross_dkv_kernel(grad_args a) {
+	using S  = dkv_shape<T, DP, RW, BIAS>;
 	using TL = tile<T, DP>;
+	using TB = tile<T, S::KEYS>;
 	constexpr int E = kind<T>::E, QT = S::QT;
 	const af3_cross_attention_params& p = a.p;
 	extern __shared__ __align__(16) unsigned char smem[];
@@ -244,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 	const int64_t G = p.H / p.Hkv;
 	const int     D = (int)p.D;
 
-	const int64_t key = (int64_t)key_tile * S::KEYS + 32 * kwave + (lane & 31);
+	const int64_t key0 = (int64_t)key_tile * S::KEYS, key = key0 + 32 * kwave + tile_row(lane & 31);   // (the order in which the biases' columns come)
 	const bool    in = key < p.Lk;
 	const bool    dead = p.stats[2 * ((b * p.H + hk * G) * p.Lq)] == -INFINITY;   // no live key in the batch row: P is 1 / Lk for all keys, S none of its business
 	const bool    lives = in && (!p.key_mask || p.key_mask[b * p.key_mask_stride_b + key] != 0);
@@ -263,9 +272,19 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 	passage<T, DP, QT> pq, pg;
 	pq.begin(nullptr, p.q_stride[2], D, a.whole);
 	pg.begin(nullptr, a.g.grad_out_stride[2], D, a.whole);
+	const typename TB::reader at_bias(lane);
+	passage<T, S::KEYS, QT>   pb;
+	if constexpr(BIAS) {
+		const int keys = p.Lk - key0 < S::KEYS ? (int)(p.Lk - key0) : S::KEYS;
+		pb.begin(nullptr, p.bias_stride[1], keys, keys % E == 0);
+	}
 	float row_stat[3];
 	auto fetch = [&](int64_t it) {
 		const int64_t h = hk * G + it / q_tiles, q0 = it % q_tiles * QT;
+		if constexpr(BIAS) {
+			pb.base = static_cast<const T*>(p.bias) + h * p.bias_stride[0] + key0;
+			pb.load(q0, p.Lq);
+		}
 		pq.base = static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1];
 		pg.base = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1];
 		pq.load(q0, p.Lq);
@@ -285,12 +304,14 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 	for(; it < last; it++) {
 		unsigned char* const qs = smem + buffer * S::SET;
 		unsigned char* const gs = qs + S::TILE;
-		float* const         st = reinterpret_cast<float*>(gs + S::TILE);
-		const int64_t        h = hk * G + it / q_tiles, q0 = it % q_tiles * QT;
+		unsigned char* const bt = gs + S::TILE;
+		float* const         st = reinterpret_cast<float*>(bt + S::BIASES);
+		const int64_t        q0 = it % q_tiles * QT;
 		if constexpr(S::BUFFERS == 1) __syncthreads();
 		const int64_t left = p.Lq - q0;
 		pq.store(qs, left >= QT, [&](int r) { return r < left; });
 		pg.store(gs, left >= QT, [&](int r) { return r < left; });
+		if constexpr(BIAS) pb.store(bt, left >= QT, [&](int r) { return r < left; });
 		if((int)threadIdx.x < QT) st[threadIdx.x] = row_stat[0], st[QT + threadIdx.x] = row_stat[1], st[2 * QT + threadIdx.x] = row_stat[2];
 		__syncthreads();
 		if(it + 1 < last) fetch(it + 1);
@@ -310,19 +331,14 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW>::REGI
 					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, row0, i, at), kf[i], acc);
 #pragma unroll
 					for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, row0, i, at), vf[i], dp);
-					float bs[16];
+					u32x4 bs[TB::JOINTS];
 					if constexpr(BIAS) {
-						const T* const column = static_cast<const T*>(p.bias) + h * p.bias_stride[0] + (in ? key : 0);
 #pragma unroll
-						for(int r = 0; r < 16; r++) {
-							const int64_t q = q0 + row0 + 16 * half + r;
-							const float   v = kind<T>::value(column[(q < p.Lq ? q : 0) * p.bias_stride[1]]);
-							bs[r] = q < p.Lq ? v : 0.f;
-						}
+						for(int j = 0; j < TB::JOINTS; j++) bs[j] = TB::col_frag(bt, row0, kwave, j, at_bias);
 					}
 #pragma unroll
 					for(int r = 0; r < 16; r++) {
-						const float t0 = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, bs[r]) : acc[r];
+						const float t0 = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, kind<T>::at(bs[r / E], r % E)) : acc[r];
 						x[r] = __builtin_amdgcn_exp2f((t0 - sm[r]) * a.factor) * sm[QT + r];
 						y[r] = x[r] * (dp[r] - sm[2 * QT + r]);
 					}
@@ -399,105 +415,101 @@ __global__ void __launch_bounds__(THREADS) cross_sum_kernel(parts a) {
 }
 
 // ---- dbias ----
+// A workgroup has 64 query rows x 64 keys (a wavefront 32 x 32 of them) and goes through the batch; q, dO, k and v come as tiles.  Few sums to hold leave room for
+// many wavefronts: 128 keys with K and V as operands straight from memory took 57 us at 8 x 12 x 512 x 512 x 64, where the loads of every batch row stood alone.
 template <typename T, int DP>
 struct dbias_shape {
-	static constexpr int QT = sizeof(T) == 2 ? 64 : 32, SUB = QT / 32, KEYS = 128;
-	static constexpr int TILE = QT * tile<T, DP>::STRIDE, STATS = 3 * QT * 4, SET = 2 * TILE + STATS;
-	static constexpr int BUFFERS = 2 * SET <= 81920 ? 2 : 1, LDS = BUFFERS * SET;
-	static constexpr int REGISTERS = 8 * tile<T, DP>::STEPS + 32 * SUB + 8 * passage<T, DP, QT>::N;
+	static constexpr int QT = 64, KT = 64, TILE = 64 * tile<T, DP>::STRIDE, STATS = 3 * QT * 4, LDS = 4 * TILE + STATS;
+	static constexpr int REGISTERS = 32 + 16 * passage<T, DP, 64>::N;
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGISTERS)) cross_dbias_kernel(grad_args a) {
 	using S  = dbias_shape<T, DP>;
 	using TL = tile<T, DP>;
-	constexpr int QT = S::QT;
+	constexpr int QT = S::QT, KT = S::KT;
 	const af3_cross_attention_params& p = a.p;
 	extern __shared__ __align__(16) unsigned char smem[];
+	unsigned char *const qs = smem, *const gs = qs + S::TILE, *const ks = gs + S::TILE, *const vs = ks + S::TILE;
+	float* const st = reinterpret_cast<float*>(vs + S::TILE);
 
-	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-	const uint32_t key_tiles = (uint32_t)((p.Lk + S::KEYS - 1) / S::KEYS);
+	const int      lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+	const uint32_t key_tiles = (uint32_t)((p.Lk + KT - 1) / KT);
 	const share    own((uint32_t)blockIdx.x, (uint32_t)p.H, a.tiles * key_tiles);
 	const uint32_t q_tile = own.piece / key_tiles, key_tile = own.piece - q_tile * key_tiles;
-	const int64_t  q0 = (int64_t)q_tile * QT, h = own.pair, hk = h / (p.H / p.Hkv);
+	const int64_t  q0 = (int64_t)q_tile * QT, k0 = (int64_t)key_tile * KT, h = own.pair, hk = h / (p.H / p.Hkv);
+	const int      row0 = 32 * (wave >> 1), col0 = 32 * (wave & 1);
 	const int      D = (int)p.D;
-	const int64_t  key = (int64_t)key_tile * S::KEYS + 32 * wave + (lane & 31);
+	// (K and V as B operands are read like A operands: lane n holds key tile_row(n) of the block)
+	const int64_t  key = k0 + col0 + tile_row(lane & 31);
 	const bool     in = key < p.Lk;
 
-	float sum[S::SUB][16], bs[S::SUB][16];
+	float sum[16], bs[16];
 #pragma unroll
-	for(int s = 0; s < S::SUB; s++)
-#pragma unroll
-		for(int r = 0; r < 16; r++) {
-			const int64_t q = q0 + 32 * s + 16 * half + r;
-			sum[s][r] = 0.f, bs[s][r] = 0.f;
-			if(in && q < p.Lq) bs[s][r] = kind<T>::value(static_cast<const T*>(p.bias)[h * p.bias_stride[0] + q * p.bias_stride[1] + key]);
-		}
+	for(int r = 0; r < 16; r++) {
+		const int64_t q = q0 + row0 + 16 * half + r;
+		sum[r] = 0.f, bs[r] = 0.f;
+		if(in && q < p.Lq) bs[r] = kind<T>::value(static_cast<const T*>(p.bias)[h * p.bias_stride[0] + q * p.bias_stride[1] + key]);
+	}
 	const typename TL::reader at(lane);
-	passage<T, DP, QT> pq, pg;
+	passage<T, DP, 64> pq, pg, pk, pv;
 	pq.begin(nullptr, p.q_stride[2], D, a.whole);
 	pg.begin(nullptr, a.g.grad_out_stride[2], D, a.whole);
+	pk.begin(nullptr, p.k_stride[2], D, a.whole);
+	pv.begin(nullptr, p.v_stride[2], D, a.whole);
 	float row_stat[3];
 	auto fetch = [&](int64_t b) {
 		pq.base = static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1];
 		pg.base = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1];
+		pk.base = static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[1];
+		pv.base = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
 		pq.load(q0, p.Lq);
 		pg.load(q0, p.Lq);
+		pk.load(k0, p.Lk);
+		pv.load(k0, p.Lk);
 		row_stat[0] = row_stat[1] = row_stat[2] = 0.f;
 		if((int)threadIdx.x < QT && q0 + threadIdx.x < p.Lq) {
 			const int64_t row = (b * p.H + h) * p.Lq + q0 + threadIdx.x;
 			row_stat[0] = p.stats[2 * row], row_stat[1] = p.stats[2 * row + 1], row_stat[2] = a.delta[row];
 		}
 	};
-	int buffer = 0;
 	fetch(0);
+	const int64_t rows_left = p.Lq - q0, keys_left = p.Lk - k0;
 	for(int64_t b = 0; b < p.B; b++) {
-		unsigned char* const qs = smem + buffer * S::SET;
-		unsigned char* const gs = qs + S::TILE;
-		float* const         st = reinterpret_cast<float*>(gs + S::TILE);
-		u32x4 kf[TL::STEPS], vf[TL::STEPS];
 		const bool lives = in && (!p.key_mask || p.key_mask[b * p.key_mask_stride_b + key] != 0);
-		load_operand<T, DP>(kf, static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[1] + (in ? key : 0) * p.k_stride[2], lives, D, lane);
-		load_operand<T, DP>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], lives, D, lane);
-		if constexpr(S::BUFFERS == 1) __syncthreads();
-		const int64_t left = p.Lq - q0;
-		pq.store(qs, left >= QT, [&](int r) { return r < left; });
-		pg.store(gs, left >= QT, [&](int r) { return r < left; });
+		__syncthreads();   // (nobody reads the batch row before any more)
+		pq.store(qs, rows_left >= 64, [&](int r) { return r < rows_left; });
+		pg.store(gs, rows_left >= 64, [&](int r) { return r < rows_left; });
+		pk.store(ks, keys_left >= 64, [&](int r) { return r < keys_left; });
+		pv.store(vs, keys_left >= 64, [&](int r) { return r < keys_left; });
 		if((int)threadIdx.x < QT) st[threadIdx.x] = row_stat[0], st[QT + threadIdx.x] = row_stat[1], st[2 * QT + threadIdx.x] = row_stat[2];
 		__syncthreads();
 		if(b + 1 < p.B) fetch(b + 1);
-		if(st[0] != -INFINITY && __any(lives)) {   // (-inf: a batch row without a live key)
+		if(st[0] == -INFINITY || !__any(lives)) continue;   // (-inf: a batch row without a live key)
+		f32x16 acc{}, dp{};
 #pragma unroll
-			for(int s = 0; s < S::SUB; s++) {
-				f32x16 acc{}, dp{};
+		for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, row0, i, at), TL::row_frag(ks, col0, i, at), acc);
 #pragma unroll
-				for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, 32 * s, i, at), kf[i], acc);
+		for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, row0, i, at), TL::row_frag(vs, col0, i, at), dp);
+		const float* const sm = st + row0 + 16 * half;
 #pragma unroll
-				for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, 32 * s, i, at), vf[i], dp);
-				const float* const sm = st + 32 * s + 16 * half;
-#pragma unroll
-				for(int r = 0; r < 16; r++) {
-					const float pr = __builtin_amdgcn_exp2f((__builtin_fmaf(acc[r], p.softmax_scale, bs[s][r]) - sm[r]) * a.factor) * sm[QT + r];
-					const float ds = pr * (dp[r] - sm[2 * QT + r]);
-					sum[s][r] += lives ? ds : 0.f;
-				}
-			}
+		for(int r = 0; r < 16; r++) {
+			const float pr = __builtin_amdgcn_exp2f((__builtin_fmaf(acc[r], p.softmax_scale, bs[r]) - sm[r]) * a.factor) * sm[QT + r];
+			const float ds = pr * (dp[r] - sm[2 * QT + r]);
+			sum[r] += lives ? ds : 0.f;   // (what k, v and bias hold at a dropped key stays in its own lane)
 		}
-		if constexpr(S::BUFFERS == 2) buffer ^= 1;
 	}
 	if(!in) return;
 	T* const out = static_cast<T*>(a.g.grad_bias) + h * p.Lq * p.Lk + key;
 #pragma unroll
-	for(int s = 0; s < S::SUB; s++)
-#pragma unroll
-		for(int r = 0; r < 16; r++) {
-			const int64_t q = q0 + 32 * s + 16 * half + r;
-			if(q < p.Lq) {
-				const T rounded = kind<T>::bits(sum[s][r]);
-				out[q * p.Lk] = rounded;
-				if(sizeof(T) == 2 && a.g.grad_bias_residual) static_cast<T*>(a.g.grad_bias_residual)[(h * p.Lq + q) * p.Lk + key] = kind<T>::bits(sum[s][r] - kind<T>::value(rounded));
-			}
+	for(int r = 0; r < 16; r++) {
+		const int64_t q = q0 + row0 + 16 * half + r;
+		if(q < p.Lq) {
+			const T rounded = kind<T>::bits(sum[r]);
+			out[q * p.Lk] = rounded;
+			if(sizeof(T) == 2 && a.g.grad_bias_residual) static_cast<T*>(a.g.grad_bias_residual)[(h * p.Lq + q) * p.Lk + key] = kind<T>::bits(sum[r] - kind<T>::value(rounded));
 		}
+	}
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
@@ -591,8 +603,8 @@ int backward(grad_args a, hipStream_t s) {
 		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * c.tiles * c.splits;
 		int rc = AF3_ERR_LAUNCH;
 		if constexpr(sizeof(T) == 2 || DP <= 64)
-			if(c.shared) rc = p.bias ? launch(cross_dkv_kernel<T, DP, 4, true>, dkv_shape<T, DP, 4>::LDS, grid, a, s) : launch(cross_dkv_kernel<T, DP, 4, false>, dkv_shape<T, DP, 4>::LDS, grid, a, s);
-		if(!c.shared) rc = p.bias ? launch(cross_dkv_kernel<T, DP, 1, true>, dkv_shape<T, DP, 1>::LDS, grid, a, s) : launch(cross_dkv_kernel<T, DP, 1, false>, dkv_shape<T, DP, 1>::LDS, grid, a, s);
+			if(c.shared) rc = p.bias ? launch(cross_dkv_kernel<T, DP, 4, true>, dkv_shape<T, DP, 4, true>::LDS, grid, a, s) : launch(cross_dkv_kernel<T, DP, 4, false>, dkv_shape<T, DP, 4, false>::LDS, grid, a, s);
+		if(!c.shared) rc = p.bias ? launch(cross_dkv_kernel<T, DP, 1, true>, dkv_shape<T, DP, 1, true>::LDS, grid, a, s) : launch(cross_dkv_kernel<T, DP, 1, false>, dkv_shape<T, DP, 1, false>::LDS, grid, a, s);
 		if(rc != AF3_OK) return rc;
 		if(c.splits > 1) {
 			add(a.partial, 2 * n_keys * p.D, c.splits, a.g.grad_k, n_keys * p.D);
@@ -606,7 +618,7 @@ int backward(grad_args a, hipStream_t s) {
 	if(a.g.grad_bias) {
 		using S = dbias_shape<T, DP>;
 		a.tiles = (uint32_t)over(p.Lq, S::QT);
-		return launch(cross_dbias_kernel<T, DP>, S::LDS, (uint32_t)(p.H * a.tiles * over(p.Lk, S::KEYS)), a, s);
+		return launch(cross_dbias_kernel<T, DP>, S::LDS, (uint32_t)(p.H * a.tiles * over(p.Lk, S::KT)), a, s);
 	}
 	return AF3_OK;
 }
@@ -625,7 +637,7 @@ int validate_grads(const af3_cross_attention_params* p, const af3_cross_attentio
 	for(int i = 0; i < 3; i++)
 		if(g->grad_out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
 	// (workgroup numbers of the kernels whose results are the keys' and the bias's)
-	if(p->B * p->Hkv * over(p->Lk, 32) > 0x3ffffff || p->H * over(p->Lq, 32) > 0x3ffffff || p->H * over(p->Lq, 32) * over(p->Lk, 128) > 0x3ffffff) return AF3_ERR_BAD_SHAPE;
+	if(p->B * p->Hkv * over(p->Lk, 32) > 0x3ffffff || p->H * over(p->Lq, 32) > 0x3ffffff || p->H * over(p->Lq, 64) * over(p->Lk, 64) > 0x3ffffff) return AF3_ERR_BAD_SHAPE;
 	return AF3_OK;
 }
 

@@ -228,25 +228,6 @@ __device__ __forceinline__ void load_row16_raw(u32x4 (&out)[N], const T* row, in
 		for(int i = 0; i < N; i++) out[i] = first + E * i < L ? load_guarded(row + first + E * i, 0, L - first - E * i < E ? (int)(L - first - E * i) : E) : u32x4{0u, 0u, 0u, 0u};
 	}
 }
-// 16 entries of a row from `first` on as floats, those from L on left at 0 (`row` is the row's first entry)
-template <typename T>
-__device__ __forceinline__ void load_row16(float (&out)[16], const T* row, int64_t first, int64_t L) {
-	constexpr int E = kind<T>::E;
-	if(first + 16 <= L) {
-#pragma unroll
-		for(int i = 0; i < 16 / E; i++) {
-			const u32x4 v = load16(row + first + E * i);
-#pragma unroll
-			for(int e = 0; e < E; e++) out[E * i + e] = kind<T>::at(v, e);
-		}
-	} else {
-#pragma unroll
-		for(int i = 0; i < 16; i++) {
-			out[i] = 0.f;
-			if(first + i < L) out[i] = kind<T>::value(row[first + i]);
-		}
-	}
-}
 // 16 results side by side, from element d on, those below D
 template <typename T>
 __device__ __forceinline__ void store_row16(T* row, int d, int D, const float (&v)[16]) {
@@ -314,6 +295,16 @@ struct live_keys {
 
 // Wavefronts per SIMD that a kernel is to leave room for: three where its accumulators and operands (`registers`) are few, two, or one
 constexpr int wavefronts(int registers) { return registers <= 48 ? 3 : registers <= 136 ? 2 : 1; }
+
+// The registers of a block of keys whose bit in `keep` is 0 become `gone`.  (Register r is key r in the lower half-wave, 16 + r in the upper: the lanes that keep theirs
+// are a scalar, and one vector instruction per register is left.)
+__device__ __forceinline__ void drop_keys(float (&x)[16], uint32_t keep, float gone) {
+#pragma unroll
+	for(int r = 0; r < 16; r++) {
+		const uint64_t lanes = (uint64_t)(uint32_t)((int32_t)(keep << (31 - r)) >> 31) | (uint64_t)(uint32_t)((int32_t)(keep << (15 - r)) >> 31) << 32;
+		x[r] = __builtin_amdgcn_inverse_ballot_w64(lanes) ? x[r] : gone;
+	}
+}
 
 // Into how many parts the long axis of a launch goes: `workgroups` of them walk `tiles` tiles each, `tile_us` apiece, and `slots` fit the chip at a time; a part more
 // costs its results' way through memory (`part_bytes`, out and in again) and the kernel that joins them.  The parts of the smallest sum, of two tiles at least.

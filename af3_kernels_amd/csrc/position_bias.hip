@@ -170,10 +170,9 @@ __global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
 		const keys_of_chunk<E> keys(a, col);
 		const int64_t row0 = (int64_t)blockIdx.y * a.rows, last = row0 + a.rows < a.Lq ? row0 + a.rows : a.Lq;
 		const T* const grad = static_cast<const T*>(a.grad) + h * a.grad_stride[0] + col;
-		float* const   mine = bins + threadIdx.x;
+		// (an addition that LDS does by itself: nothing waits for the sum so far.  The column is this thread's alone, so the order is the program's)
+		auto add = [&](int bk, float v) { __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float*)(bins + bk * COLUMNS + threadIdx.x), v, 0, 0, false); };
 		const bool     full = col + E <= a.Lk;
-		int   current = 0;
-		float run     = 0.f;   // of bucket `current`, not yet in its bin
 		for(int64_t first = row0 + ty; first < last; first += AHEAD * step) {
 			u32x4   x[AHEAD];
 			int64_t q[AHEAD];
@@ -194,20 +193,18 @@ __global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
 				for(int e = 0; e < E; e++) bk[e] = LUT ? bucket[rel[e] + a.reach] : bucket_of(a, border, rel[e]);
 				bool same = true;
 #pragma unroll
-				for(int e = 0; e < E; e++) same = same && bk[e] == current;
+				for(int e = 1; e < E; e++) same = same && bk[e] == bk[0];
 				if(same) {
+					float sum = kind<T>::at(x[i], 0);
 #pragma unroll
-					for(int e = 0; e < E; e++) run += kind<T>::at(x[i], e);
+					for(int e = 1; e < E; e++) sum += kind<T>::at(x[i], e);
+					add(bk[0], sum);
 				} else {
 #pragma unroll
-					for(int e = 0; e < E; e++) {
-						if(bk[e] != current) mine[current * COLUMNS] += run, run = 0.f, current = bk[e];
-						run += kind<T>::at(x[i], e);
-					}
+					for(int e = 0; e < E; e++) add(bk[e], kind<T>::at(x[i], e));
 				}
 			}
 		}
-		mine[current * COLUMNS] += run;
 	}
 	__syncthreads();
 	const int64_t part = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, parts = (int64_t)gridDim.x * gridDim.y;
@@ -326,7 +323,7 @@ dim3 sums_shape(args& a, int E) {
 	// about 2048 workgroups; each adds its bins up, which is worth a few hundred rows of reading
 	const int64_t pieces = a.H * a.Lq * ((a.Lk + E - 1) / E);
 	int64_t       each = pieces / (2048 * COLUMNS);
-	return shape(a, E, COLUMNS, each < 16 ? 16 : each > 4096 ? 4096 : each);
+	return shape(a, E, COLUMNS, each < 8 ? 8 : each > 4096 ? 4096 : each);
 }
 
 template <typename T>
