@@ -47,7 +47,7 @@ struct forward_shape {
 };
 
 template <typename T, int DP, int KW, bool BIAS>
-__global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::REGISTERS)) cross_forward_kernel(forward_args a) {
+__global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::REGISTERS + (BIAS ? 24 : 0))) cross_forward_kernel(forward_args a) {
 	using S  = forward_shape<T, DP, KW>;
 	using TL = tile<T, DP>;
 	constexpr int E = kind<T>::E, KT = S::KT;

@@ -82,11 +82,11 @@ struct dq_shape {
 	static constexpr int BUFFERS = 4 * TILE <= 81920 ? 2 : 1;
 	static constexpr int JOIN = KW > 1 ? WAVES * 32 * (DP + 4) * 4 : 0;
 	static constexpr int LDS = 2 * BUFFERS * TILE > JOIN ? 2 * BUFFERS * TILE : JOIN;
-	static constexpr int REGISTERS = 8 * tile<T, DP>::STEPS + DP / 2 + 8 * passage<T, DP, KT>::N - 24;
+	static constexpr int REGISTERS = 8 * tile<T, DP>::STEPS + DP / 2 + 8 * passage<T, DP, KT>::N - (sizeof(T) == 2 ? 24 : 8);
 };
 
 template <typename T, int DP, int KW, bool BIAS>
-__global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGISTERS)) cross_dq_kernel(grad_args a) {
+__global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGISTERS + (BIAS && DP < 128 ? 32 : 0))) cross_dq_kernel(grad_args a) {
 	using S  = dq_shape<T, DP, KW>;
 	using TL = tile<T, DP>;
 	constexpr int E = kind<T>::E, KT = S::KT;
@@ -111,6 +111,8 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 	const float delta = row_delta<T, DP>(a, gf, b, h, qi, ok, lane);
 	if(ok && half == 0 && kwave == 0 && split == 0) a.delta[row] = delta;
 	const float  m = ok ? p.stats[2 * row] : 0.f, inv = ok ? p.stats[2 * row + 1] : 0.f;
+	const bool   apart = sizeof(T) == 4 || DP > 96 || __any(m < FAR_BELOW);   // (a row whose maximum is far below: exact, in natural units; 128 columns: registers for one form)
+	const float  taken = whole_reference(m, inv, a.factor);
 	const T* const kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[1];
 	const T* const vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
 	const T* const bias = BIAS ? static_cast<const T*>(p.bias) + h * p.bias_stride[0] + qi * p.bias_stride[1] : nullptr;
@@ -175,10 +177,13 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 #pragma unroll
 				for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(vs, 32 * block, i, at), gf[i], dp);
 				float x[16];
+				auto logit = [&](int r) { return BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, kind<T>::at(bs[s][r / E], r % E)) : acc[r]; };
+				if(apart) {
 #pragma unroll
-				for(int r = 0; r < 16; r++) {
-					const float t0 = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, kind<T>::at(bs[s][r / E], r % E)) : acc[r];
-					x[r] = __builtin_amdgcn_exp2f((t0 - m) * a.factor) * inv * (dp[r] - delta);
+					for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f((logit(r) - m) * a.factor) * inv * (dp[r] - delta);
+				} else {
+#pragma unroll
+					for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(logit(r), a.factor, -taken)) * (dp[r] - delta);
 				}
 				if(keep != ~0u) drop_keys(x, keep, 0.f);
 #pragma unroll
@@ -222,6 +227,47 @@ __global__ void __launch_bounds__(THREADS) cross_delta_kernel(grad_args a) {
 	if(ok && lane < 32) a.delta[row] = delta;
 }
 
+// What the kernels with query rows in tiles keep of each row of a tile in LDS: delta with its sign turned (it begins the sum of dP), and, for bf16, the whole reference;
+// maximum and 1 / sum for fp32 and for tiles with a row far below.  Behind them a word that says whether there is one.
+constexpr int ROW_STATS = 4;
+template <typename T, int QT>
+struct row_stats {
+	float taken, less, m, inv;   // of one row, on its way
+	__device__ __forceinline__ void load(const grad_args& a, int64_t bh, int64_t q0) {
+		taken = less = m = inv = 0.f;
+		if((int)threadIdx.x >= QT) return;
+		const bool ok = q0 + threadIdx.x < a.p.Lq;
+		if(ok) {
+			const int64_t row = bh * a.p.Lq + q0 + threadIdx.x;
+			m = a.p.stats[2 * row], inv = a.p.stats[2 * row + 1], less = -a.delta[row];
+		}
+	}
+	__device__ __forceinline__ void store(float* st, float factor) const {
+		if((int)threadIdx.x >= QT) return;
+		st[QT + threadIdx.x] = less, st[2 * QT + threadIdx.x] = m, st[3 * QT + threadIdx.x] = inv;
+		if constexpr(sizeof(T) == 2) {
+			st[threadIdx.x] = whole_reference(m, inv, factor);
+			const bool far = __any(m < FAR_BELOW);   // (of 64 rows: a tile of 128 has two such words)
+			if((threadIdx.x & 63) == 0) reinterpret_cast<int*>(st + ROW_STATS * QT)[threadIdx.x >> 6] = far;
+		}
+	}
+	// whether the rows' maxima and sums are to be taken apart
+	static __device__ __forceinline__ bool apart(const float* st) {
+		if constexpr(sizeof(T) == 4) return true;
+		const int* const far = reinterpret_cast<const int*>(st + ROW_STATS * QT);
+		return __builtin_amdgcn_readfirstlane(QT > 64 ? far[0] | far[1] : far[0]) != 0;
+	}
+	static __device__ __forceinline__ f32x16 sixteen(const float* at) {
+		f32x16 v;
+#pragma unroll
+		for(int i = 0; i < 4; i++) {
+			const f32x4 x = *reinterpret_cast<const f32x4*>(at + 4 * i);
+			v[4 * i] = x[0], v[4 * i + 1] = x[1], v[4 * i + 2] = x[2], v[4 * i + 3] = x[3];
+		}
+		return v;
+	}
+};
+
 // ---- dK, dV ----
 // RW: wavefronts that share 32 keys and each take 32 rows of a tile of query rows (1: every wavefront has its own keys and takes the whole tile)
 // A bias comes through LDS as well, read like the columns of dO: a lane's 16 values lie in one column, and taken from memory one by one they were two thirds of the
@@ -229,7 +275,7 @@ __global__ void __launch_bounds__(THREADS) cross_delta_kernel(grad_args a) {
 template <typename T, int DP, int RW, bool BIAS>
 struct dkv_shape {
 	static constexpr int QT = RW == 4 ? 128 : sizeof(T) == 2 ? 64 : 32, SUB = QT / (32 * RW), KEYS = 32 * (WAVES / RW);
-	static constexpr int TILE = QT * tile<T, DP>::STRIDE, STATS = 3 * QT * 4, BIASES = BIAS ? QT * tile<T, KEYS>::STRIDE : 0, SET = 2 * TILE + BIASES + STATS;
+	static constexpr int TILE = QT * tile<T, DP>::STRIDE, STATS = ROW_STATS * QT * 4 + 16, BIASES = BIAS ? QT * tile<T, KEYS>::STRIDE : 0, SET = 2 * TILE + BIASES + STATS;
 	static constexpr int BUFFERS = 2 * SET <= 81920 ? 2 : 1;
 	static constexpr int JOIN = RW > 1 ? WAVES * 32 * (DP + 4) * 4 : 0;
 	static constexpr int LDS = BUFFERS * SET > JOIN ? BUFFERS * SET : JOIN;
@@ -278,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW, BIAS>
 		const int keys = p.Lk - key0 < S::KEYS ? (int)(p.Lk - key0) : S::KEYS;
 		pb.begin(nullptr, p.bias_stride[1], keys, keys % E == 0);
 	}
-	float row_stat[3];
+	row_stats<T, QT> rs;
 	auto fetch = [&](int64_t it) {
 		const int64_t h = hk * G + it / q_tiles, q0 = it % q_tiles * QT;
 		if constexpr(BIAS) {
@@ -289,11 +335,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW, BIAS>
 		pg.base = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1];
 		pq.load(q0, p.Lq);
 		pg.load(q0, p.Lq);
-		row_stat[0] = row_stat[1] = row_stat[2] = 0.f;
-		if((int)threadIdx.x < QT && q0 + threadIdx.x < p.Lq) {
-			const int64_t row = (b * p.H + h) * p.Lq + q0 + threadIdx.x;
-			row_stat[0] = p.stats[2 * row], row_stat[1] = p.stats[2 * row + 1], row_stat[2] = a.delta[row];
-		}
+		rs.load(a, b * p.H + h, q0);
 	};
 	int     buffer = 0;
 	int64_t it = (int64_t)split * a.part;
@@ -312,8 +354,9 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW, BIAS>
 		pq.store(qs, left >= QT, [&](int r) { return r < left; });
 		pg.store(gs, left >= QT, [&](int r) { return r < left; });
 		if constexpr(BIAS) pb.store(bt, left >= QT, [&](int r) { return r < left; });
-		if((int)threadIdx.x < QT) st[threadIdx.x] = row_stat[0], st[QT + threadIdx.x] = row_stat[1], st[2 * QT + threadIdx.x] = row_stat[2];
+		rs.store(st, a.factor);
 		__syncthreads();
+		const bool apart = rs.apart(st);
 		if(it + 1 < last) fetch(it + 1);
 		if(work) {
 #pragma unroll
@@ -324,9 +367,9 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW, BIAS>
 				const float* const sm = st + row0 + 16 * half;
 				if(dead) {
 #pragma unroll
-					for(int r = 0; r < 16; r++) x[r] = sm[QT + r], y[r] = 0.f;
+					for(int r = 0; r < 16; r++) x[r] = sm[3 * QT + r], y[r] = 0.f;
 				} else {
-					f32x16 acc{}, dp{};
+					f32x16 acc{}, dp = rs.sixteen(sm + QT);
 #pragma unroll
 					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, row0, i, at), kf[i], acc);
 #pragma unroll
@@ -336,12 +379,18 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW, BIAS>
 #pragma unroll
 						for(int j = 0; j < TB::JOINTS; j++) bs[j] = TB::col_frag(bt, row0, kwave, j, at_bias);
 					}
+					auto logit = [&](int r) { return BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, kind<T>::at(bs[r / E], r % E)) : acc[r]; };
+					if(apart) {
+						const f32x16 m = rs.sixteen(sm + 2 * QT), inv = rs.sixteen(sm + 3 * QT);
 #pragma unroll
-					for(int r = 0; r < 16; r++) {
-						const float t0 = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, kind<T>::at(bs[r / E], r % E)) : acc[r];
-						x[r] = __builtin_amdgcn_exp2f((t0 - sm[r]) * a.factor) * sm[QT + r];
-						y[r] = x[r] * (dp[r] - sm[2 * QT + r]);
+						for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f((logit(r) - m[r]) * a.factor) * inv[r];
+					} else {
+						const f32x16 taken = rs.sixteen(sm);
+#pragma unroll
+						for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(logit(r), a.factor, -taken[r]));
 					}
+#pragma unroll
+					for(int r = 0; r < 16; r++) y[r] = x[r] * dp[r];
 				}
 #pragma unroll
 				for(int j = 0; j < TL::JOINTS; j++) {
@@ -419,8 +468,8 @@ __global__ void __launch_bounds__(THREADS) cross_sum_kernel(parts a) {
 // many wavefronts: 128 keys with K and V as operands straight from memory took 57 us at 8 x 12 x 512 x 512 x 64, where the loads of every batch row stood alone.
 template <typename T, int DP>
 struct dbias_shape {
-	static constexpr int QT = 64, KT = 64, TILE = 64 * tile<T, DP>::STRIDE, STATS = 3 * QT * 4, LDS = 4 * TILE + STATS;
-	static constexpr int REGISTERS = 32 + 16 * passage<T, DP, 64>::N;
+	static constexpr int QT = 64, KT = 64, TILE = 64 * tile<T, DP>::STRIDE, STATS = ROW_STATS * QT * 4 + 16, LDS = 4 * TILE + STATS;
+	static constexpr int REGISTERS = 48 + 16 * passage<T, DP, 64>::N;
 };
 
 template <typename T, int DP>
@@ -457,7 +506,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 	pg.begin(nullptr, a.g.grad_out_stride[2], D, a.whole);
 	pk.begin(nullptr, p.k_stride[2], D, a.whole);
 	pv.begin(nullptr, p.v_stride[2], D, a.whole);
-	float row_stat[3];
+	row_stats<T, QT> rs;
 	auto fetch = [&](int64_t b) {
 		pq.base = static_cast<const T*>(p.q) + b * p.q_stride[0] + h * p.q_stride[1];
 		pg.base = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1];
@@ -467,11 +516,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 		pg.load(q0, p.Lq);
 		pk.load(k0, p.Lk);
 		pv.load(k0, p.Lk);
-		row_stat[0] = row_stat[1] = row_stat[2] = 0.f;
-		if((int)threadIdx.x < QT && q0 + threadIdx.x < p.Lq) {
-			const int64_t row = (b * p.H + h) * p.Lq + q0 + threadIdx.x;
-			row_stat[0] = p.stats[2 * row], row_stat[1] = p.stats[2 * row + 1], row_stat[2] = a.delta[row];
-		}
+		rs.load(a, b * p.H + h, q0);
 	};
 	fetch(0);
 	const int64_t rows_left = p.Lq - q0, keys_left = p.Lk - k0;
@@ -482,22 +527,28 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 		pg.store(gs, rows_left >= 64, [&](int r) { return r < rows_left; });
 		pk.store(ks, keys_left >= 64, [&](int r) { return r < keys_left; });
 		pv.store(vs, keys_left >= 64, [&](int r) { return r < keys_left; });
-		if((int)threadIdx.x < QT) st[threadIdx.x] = row_stat[0], st[QT + threadIdx.x] = row_stat[1], st[2 * QT + threadIdx.x] = row_stat[2];
+		rs.store(st, a.factor);
 		__syncthreads();
 		if(b + 1 < p.B) fetch(b + 1);
-		if(st[0] == -INFINITY || !__any(lives)) continue;   // (-inf: a batch row without a live key)
-		f32x16 acc{}, dp{};
+		if(st[2 * QT] == -INFINITY || !__any(lives)) continue;   // (-inf: a batch row without a live key)
+		const float* const sm = st + row0 + 16 * half;
+		f32x16 acc{}, dp = rs.sixteen(sm + QT);
 #pragma unroll
 		for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(qs, row0, i, at), TL::row_frag(ks, col0, i, at), acc);
 #pragma unroll
 		for(int i = 0; i < TL::STEPS; i++) dp = kind<T>::mma(TL::row_frag(gs, row0, i, at), TL::row_frag(vs, col0, i, at), dp);
-		const float* const sm = st + row0 + 16 * half;
+		float x[16];
+		if(rs.apart(st)) {
+			const f32x16 m = rs.sixteen(sm + 2 * QT), inv = rs.sixteen(sm + 3 * QT);
 #pragma unroll
-		for(int r = 0; r < 16; r++) {
-			const float pr = __builtin_amdgcn_exp2f((__builtin_fmaf(acc[r], p.softmax_scale, bs[r]) - sm[r]) * a.factor) * sm[QT + r];
-			const float ds = pr * (dp[r] - sm[2 * QT + r]);
-			sum[r] += lives ? ds : 0.f;   // (what k, v and bias hold at a dropped key stays in its own lane)
+			for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f((__builtin_fmaf(acc[r], p.softmax_scale, bs[r]) - m[r]) * a.factor) * inv[r];
+		} else {
+			const f32x16 taken = rs.sixteen(sm);
+#pragma unroll
+			for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_fmaf(acc[r], p.softmax_scale, bs[r]), a.factor, -taken[r]));
 		}
+#pragma unroll
+		for(int r = 0; r < 16; r++) sum[r] += lives ? x[r] * dp[r] : 0.f;   // (what k, v and bias hold at a dropped key stays in its own lane)
 	}
 	if(!in) return;
 	T* const out = static_cast<T*>(a.g.grad_bias) + h * p.Lq * p.Lk + key;

@@ -85,6 +85,9 @@ __device__ __forceinline__ float reference_of(float m, float to_log2) {
 	const float r = m * to_log2;
 	return m < FAR_BELOW ? -INFINITY : r - r + r;
 }
+// What the gradients take off a row's logits instead (bf16): the reference and the logarithm of the row's sum together, so that P comes out of the exponential as it is.
+// (fp32 keeps the two apart: in one number their rounding, 2^-24 of it, would be the largest error of P.)  1 / sum == 0, a row without a live key, makes P zero.
+__device__ __forceinline__ float whole_reference(float m, float inv, float to_log2) { return m * to_log2 - __builtin_amdgcn_logf(inv); }
 // a value of lane l and that of lane l ^ 32, joined
 __device__ __forceinline__ float sum_of_halves(float x) {
 	const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -294,7 +297,7 @@ struct live_keys {
 };
 
 // Wavefronts per SIMD that a kernel is to leave room for: three where its accumulators and operands (`registers`) are few, two, or one
-constexpr int wavefronts(int registers) { return registers <= 48 ? 3 : registers <= 136 ? 2 : 1; }
+constexpr int wavefronts(int registers) { return registers <= 64 ? 3 : registers <= 136 ? 2 : 1; }
 
 // The registers of a block of keys whose bit in `keep` is 0 become `gone`.  (Register r is key r in the lower half-wave, 16 + r in the upper: the lanes that keep theirs
 // are a scalar, and one vector instruction per register is left.)
