@@ -113,14 +113,13 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 			}
 			unsigned char* const ks = smem + buffer * 2 * S::TILE;
 			unsigned char* const vs = ks + S::TILE;
-			const bool full = live.full(t);
-			uint32_t   keep[S::SUB];
-#pragma unroll
-			for(int s = 0; s < S::SUB; s++) keep[s] = live.word(t * (KT / 32) + kwave * S::SUB + s);
+			const tile_bits<KT> bits(live, t);
+			const bool          full = bits.full();
 			const int following = live.next(t + 1);
 			if constexpr(S::BUFFERS == 1) __syncthreads();
-			pk.store(ks, full, [&](int row) { return live.keeps(t * KT + row); });
-			pv.store(vs, full, [&](int row) { return live.keeps(t * KT + row); });
+			// (what K holds at a dropped key stays in that key's logits, which are not looked at; its row of V meets a weight of zero, and must not be NaN)
+			pk.store(ks, true, [](int) { return true; });
+			pv.store(vs, full, [&](int row) { return bits.keeps(row); });
 			__syncthreads();
 			if(following >= 0) {
 				pk.load(first + (int64_t)following * KT, end);
@@ -129,8 +128,9 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 			}
 #pragma unroll
 			for(int s = 0; s < S::SUB; s++) {
-				const int block = kwave * S::SUB + s;
-				if(keep[s] == 0u) continue;
+				const int      block = kwave * S::SUB + s;
+				const uint32_t keep = bits.of_block(block);
+				if(keep == 0u) continue;
 				float x[16];
 				auto  logits = [&] {
 					f32x16 acc{};
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 					for(int i = 0; i < TL::STEPS; i++) acc = kind<T>::mma(TL::row_frag(ks, 32 * block, i, at), qf[i], acc);
 #pragma unroll
 					for(int r = 0; r < 16; r++) x[r] = BIAS ? __builtin_fmaf(acc[r], p.softmax_scale, kind<T>::at(bs[s][r / E], r % E)) : acc[r];
-					if(keep[s] != ~0u) drop_keys(x, keep[s], -INFINITY);
+					if(keep != ~0u) drop_keys(x, keep, -INFINITY);
 				};
 				auto probabilities = [&]() -> float {
 					float sum = 0.f;

@@ -152,14 +152,12 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 			}
 			unsigned char* const ks = smem + buffer * 2 * S::TILE;
 			unsigned char* const vs = ks + S::TILE;
-			const bool full = live.full(t);
-			uint32_t   keeps[S::SUB];
-#pragma unroll
-			for(int s = 0; s < S::SUB; s++) keeps[s] = live.word(t * (KT / 32) + kwave * S::SUB + s);
+			const tile_bits<KT> bits(live, t);
 			const int following = live.next(t + 1);
 			if constexpr(S::BUFFERS == 1) __syncthreads();
-			pk.store(ks, full, [&](int r) { return live.keeps(t * KT + r); });
-			pv.store(vs, full, [&](int r) { return live.keeps(t * KT + r); });
+			// (V is only multiplied row by row, and dS of a dropped key is not looked at; K's rows are added up under weights of zero)
+			pk.store(ks, bits.full(), [&](int r) { return bits.keeps(r); });
+			pv.store(vs, true, [](int) { return true; });
 			__syncthreads();
 			if(following >= 0) {
 				pk.load(first + (int64_t)following * KT, end);
@@ -169,7 +167,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 #pragma unroll
 			for(int s = 0; s < S::SUB; s++) {
 				const int      block = kwave * S::SUB + s;
-				const uint32_t keep  = keeps[s];
+				const uint32_t keep  = bits.of_block(block);
 				if(keep == 0u) continue;
 				f32x16 acc{}, dp{};
 #pragma unroll

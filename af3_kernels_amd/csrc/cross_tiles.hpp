@@ -287,13 +287,29 @@ struct live_keys {
 		return -1;
 	}
 	__device__ __forceinline__ uint32_t word(int i) const { return (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[i]); }
-	__device__ __forceinline__ bool full(int t) const {   // every key of tile t is live
+};
+// the bits of a tile's keys, the same for all lanes
+template <int KT>
+struct tile_bits {
+	static constexpr int N = KT / 32;
+	uint32_t word[N];
+	__device__ __forceinline__ tile_bits(const live_keys<KT>& live, int t) {
+#pragma unroll
+		for(int i = 0; i < N; i++) word[i] = (uint32_t)__builtin_amdgcn_readfirstlane((int)live.bits[t * N + i]);
+	}
+	__device__ __forceinline__ bool full() const {
 		uint32_t x = ~0u;
 #pragma unroll
-		for(int i = 0; i < KT / 32; i++) x &= bits[t * (KT / 32) + i];
-		return __builtin_amdgcn_readfirstlane((int)x) == -1;
+		for(int i = 0; i < N; i++) x &= word[i];
+		return x == ~0u;
 	}
-	__device__ __forceinline__ bool keeps(int key) const { return (bits[key >> 5] >> (key & 31)) & 1u; }
+	__device__ __forceinline__ uint32_t of_block(int block) const {
+		uint32_t x = word[0];
+#pragma unroll
+		for(int i = 1; i < N; i++) x = block == i ? word[i] : x;
+		return x;
+	}
+	__device__ __forceinline__ bool keeps(int key) const { return (of_block(key >> 5) >> (key & 31)) & 1u; }   // (a key of the tile, any lane's)
 };
 
 // Wavefronts per SIMD that a kernel is to leave room for: three where its accumulators and operands (`registers`) are few, two, or one
