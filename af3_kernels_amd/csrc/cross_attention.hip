@@ -432,7 +432,8 @@ int validate_cross_attention(const af3_cross_attention_params* p) {
 	if(!p->q || !p->k || !p->v || !p->out) return AF3_ERR_NULL_POINTER;
 	for(int i = 0; i < 3; i++)
 		if(p->q_stride[i] < 0 || p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
-	if(p->Lq > 1 && p->out_stride[2] < p->D) return AF3_ERR_BAD_STRIDE;   // (inputs may repeat rows, results may not)
+	// (inputs may repeat rows, results may not)
+	if((p->Lq > 1 && p->out_stride[2] < p->D) || (p->H > 1 && p->out_stride[1] == 0) || (p->B > 1 && p->out_stride[0] == 0)) return AF3_ERR_BAD_STRIDE;
 	if(p->bias && (p->bias_stride[0] < 0 || p->bias_stride[1] < 0)) return AF3_ERR_BAD_STRIDE;
 	if(p->key_mask && p->key_mask_stride_b < 0) return AF3_ERR_BAD_STRIDE;
 	if(!(p->softmax_scale > 0.f) || !(p->softmax_scale < INFINITY)) return AF3_ERR_BAD_ARGUMENT;

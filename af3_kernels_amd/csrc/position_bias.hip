@@ -32,8 +32,11 @@ struct args {
 	int32_t        buckets, borders, reach;
 	int32_t        first_behind, step_behind, first_ahead, step_ahead;   // bucket = first + step * (borders passed), keys behind (and at) the query and ahead of it
 	int32_t        columns_log2, rows;   // threads across the columns of a workgroup, rows of a workgroup
-	int32_t        border[MAX_BUCKETS];
+	int32_t        near;                 // the first `near` borders are 1, 2, 3, ...
+	int32_t        far_border[MAX_BUCKETS / 2];   // the others (arguments lie in host memory, and every workgroup reads what it needs of them from there)
 };
+// border i of a call
+__device__ __forceinline__ int border_of(const args& a, int i) { return i < a.near ? i + 1 : a.far_border[i - a.near]; }
 
 __device__ __forceinline__ int passed(const int* border, int n, int d) {   // how many borders are <= d
 	int low = 0;
@@ -92,7 +95,7 @@ __global__ void __launch_bounds__(THREADS) position_bias_kernel(args a) {
 	__shared__ T   values[LUT ? MAX_OFFSETS : MAX_BUCKETS];   // of the offsets, or of the buckets
 	__shared__ int border[MAX_BUCKETS];
 	const int64_t  h = blockIdx.z;
-	for(int i = threadIdx.x; i < a.borders; i += THREADS) border[i] = a.border[i];
+	for(int i = threadIdx.x; i < a.borders; i += THREADS) border[i] = border_of(a, i);
 	__syncthreads();
 	const T* const table = static_cast<const T*>(a.table) + h * a.table_stride[1];
 	if constexpr(LUT) {
@@ -147,11 +150,12 @@ constexpr int COLUMNS = 64;
 template <typename T, bool LUT>
 __global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
 	constexpr int E = kind<T>::E;
+	// (as much LDS as the call needs: with room for the most of everything five workgroups of 65 buckets stood on a compute unit instead of nine)
 	extern __shared__ float bins[];   // [buckets][COLUMNS]
-	__shared__ uint16_t bucket[LUT ? MAX_OFFSETS : 1];
-	__shared__ int      border[MAX_BUCKETS];
+	int* const      border = reinterpret_cast<int*>(bins + a.buckets * COLUMNS);         // [borders]
+	uint16_t* const bucket = reinterpret_cast<uint16_t*>(border + a.borders);            // [2 reach + 1], where they are tabulated
 	const int64_t  h = blockIdx.z;
-	for(int i = threadIdx.x; i < a.borders; i += COLUMNS) border[i] = a.border[i];
+	for(int i = threadIdx.x; i < a.borders; i += COLUMNS) border[i] = border_of(a, i);
 	for(int i = 0; i < a.buckets; i++) bins[i * COLUMNS + threadIdx.x] = 0.f;
 	__syncthreads();
 	if constexpr(LUT)
@@ -256,23 +260,23 @@ bool reaches(uint32_t d, uint32_t r, uint32_t near, int i, int far) {
 // The borders of a set of settings take microseconds to work out; a thread keeps those of its last one.
 struct worked_out {
 	int64_t buckets = 0, max_distance = 0;
-	int32_t both = 0, border[MAX_BUCKETS];
+	int32_t both = 0, border[MAX_BUCKETS / 2];
 };
+// the borders behind the first near, n - 1 - near of them
 void log_borders(int64_t buckets, int64_t max_distance, bool both, int32_t* border) {
 	static thread_local worked_out last;
 	const int n = (int)(both ? buckets / 2 : buckets), near = n / 2, far = n - near;
 	if(last.buckets != buckets || last.max_distance != max_distance || last.both != both) {
-		for(int i = 0; i < near; i++) last.border[i] = i + 1;
 		for(int i = 1; i < far; i++) {   // the smallest d with (d / near)^far >= (max_distance / near)^i
 			const long double y = near * powl((long double)max_distance / near, (long double)i / far), r = roundl(y);
 			int               d;
 			if(fabsl(y - r) > 1e-6L) d = (int)ceill(y);
 			else d = (int)r + (reaches((uint32_t)r, (uint32_t)max_distance, (uint32_t)near, i, far) ? 0 : 1);
-			last.border[near + i - 1] = d;
+			last.border[i - 1] = d;
 		}
 		last.buckets = buckets, last.max_distance = max_distance, last.both = both;
 	}
-	for(int i = 0; i < n - 1; i++) border[i] = last.border[i];
+	for(int i = 0; i < far - 1; i++) border[i] = last.border[i];
 }
 
 int prepare(const af3_position_bias_params* p, args& a) {
@@ -286,19 +290,20 @@ int prepare(const af3_position_bias_params* p, args& a) {
 	if(p->scheme == AF3_POSITION_CLIP) {
 		if(p->buckets != p->max_distance * (both ? 2 : 1) + 1) return AF3_ERR_BAD_ARGUMENT;
 		a.borders = (int)p->max_distance;
-		for(int i = 0; i < a.borders; i++) a.border[i] = i + 1;
+		a.near = a.borders;
 		a.first_behind = both ? a.borders : 0, a.step_behind = 1, a.first_ahead = both ? a.borders : 0, a.step_ahead = both ? -1 : 0;
 	} else if(p->scheme == AF3_POSITION_LOG) {
 		if(both && p->buckets % 2 != 0) return AF3_ERR_BAD_ARGUMENT;
 		const int n = (int)(both ? p->buckets / 2 : p->buckets), near = n / 2;
 		if(near < 1 || p->max_distance <= near) return AF3_ERR_BAD_ARGUMENT;
 		a.borders = n - 1;
-		log_borders(p->buckets, p->max_distance, both, a.border);
+		a.near = near;
+		log_borders(p->buckets, p->max_distance, both, a.far_border);
 		a.first_behind = 0, a.step_behind = 1, a.first_ahead = both ? n : 0, a.step_ahead = both ? 1 : 0;
 	} else {
 		return AF3_ERR_BAD_ARGUMENT;
 	}
-	a.reach = a.borders > 0 ? a.border[a.borders - 1] : 1;
+	a.reach = a.borders == a.near ? a.near : a.far_border[a.borders - a.near - 1];
 	a.q_pos = p->q_positions, a.k_pos = p->k_positions, a.q_offset = p->q_offset;
 	a.table_stride[0] = p->table_stride[0], a.table_stride[1] = p->table_stride[1];
 	a.grad_stride[0] = p->grad_stride[0], a.grad_stride[1] = p->grad_stride[1];
@@ -325,6 +330,11 @@ dim3 sums_shape(args& a, int E) {
 	int64_t       each = pieces / (2048 * COLUMNS);
 	return shape(a, E, COLUMNS, each < 8 ? 8 : each > 4096 ? 4096 : each);
 }
+dim3 forward_shape(args& a, int E) {
+	// about 1024 workgroups, of one to 16 pieces per thread
+	const int64_t each = a.H * a.Lq * ((a.Lk + E - 1) / E) / (1024 * THREADS);
+	return shape(a, E, THREADS, each < 1 ? 1 : each > 16 ? 16 : each);
+}
 
 template <typename T>
 int forward(const args& a, dim3 grid, hipStream_t s) {
@@ -334,7 +344,7 @@ int forward(const args& a, dim3 grid, hipStream_t s) {
 }
 template <typename T, bool LUT>
 int sums(const args& a, dim3 grid, hipStream_t s) {
-	const int lds = a.buckets * COLUMNS * 4;
+	const int lds = a.buckets * COLUMNS * 4 + a.borders * 4 + (LUT ? (2 * a.reach + 1) * 2 : 0);
 	if(lds > 32768 && hipFuncSetAttribute(reinterpret_cast<const void*>(&position_bias_sums_kernel<T, LUT>), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
 		(void)hipGetLastError();
 		return AF3_ERR_LAUNCH;
@@ -360,7 +370,7 @@ extern "C" int af3_position_bias_forward(const af3_position_bias_params* params,
 	if(!params->table || !params->out) return AF3_ERR_NULL_POINTER;
 	if(const int dc = current_device_status(); dc != AF3_OK) return dc;
 	const hipStream_t s = static_cast<hipStream_t>(hip_stream);
-	const dim3 grid = position::shape(a, params->dtype == AF3_F32 ? 4 : 8, position::THREADS, 16);
+	const dim3 grid = position::forward_shape(a, params->dtype == AF3_F32 ? 4 : 8);
 	return params->dtype == AF3_F32 ? position::forward<float>(a, grid, s) : position::forward<uint16_t>(a, grid, s);
 }
 
@@ -376,6 +386,7 @@ extern "C" int af3_position_bias_backward(const af3_position_bias_params* params
 	if(const int rc = position::prepare(params, a); rc != AF3_OK) return rc;
 	if(!params->grad || !params->out || !params->workspace) return AF3_ERR_NULL_POINTER;
 	if(params->grad_stride[0] < 0 || params->grad_stride[1] < 0) return AF3_ERR_BAD_STRIDE;
+	if((params->buckets > 1 && params->table_stride[0] == 0) || (params->H > 1 && params->table_stride[1] == 0)) return AF3_ERR_BAD_STRIDE;   // (results may not share a place)
 	const dim3 grid = position::sums_shape(a, params->dtype == AF3_F32 ? 4 : 8);
 	if(params->workspace_bytes < (int64_t)grid.x * grid.y * grid.z * a.buckets * 4 || (reinterpret_cast<uintptr_t>(params->workspace) & 15)) return AF3_ERR_BAD_ARGUMENT;
 	if(const int dc = current_device_status(); dc != AF3_OK) return dc;

@@ -76,7 +76,8 @@ def test_cross_attention_validates_on_the_host():
     assert fwd(_cross(D=129)) == -5
     for name in ("q_stride", "k_stride", "v_stride", "out_stride"):
         assert fwd(_cross(**{name: i64x3(-1, 32, 32)})) == -4
-    assert fwd(_cross(out_stride=i64x3(6400, 1600, 31))) == -4
+    for shared in (i64x3(6400, 1600, 31), i64x3(0, 1600, 32), i64x3(6400, 0, 32)):      # results that share a place
+        assert fwd(_cross(out_stride=shared)) == -4
     assert fwd(_cross(bias=BASE, bias_stride=i64x2(-1, 1))) == -4
     assert fwd(_cross(key_mask=BASE, key_mask_stride_b=-1)) == -4
     for scale in (0.0, -1.0, math.inf, math.nan):
@@ -130,6 +131,7 @@ def test_position_bias_validates_on_the_host():
     assert fwd(_position(table=None)) == -1
     assert bwd(_position(grad=None)) == -1 and bwd(_position(workspace=None)) == -1
     assert bwd(_position(grad_stride=i64x2(-1, 1))) == -4
+    assert bwd(_position(table_stride=i64x2(0, 1))) == -4 and bwd(_position(table_stride=i64x2(1, 0))) == -4
     need = lib.af3_position_bias_workspace_bytes(ctypes.byref(_position()))
     assert need > 0 and bwd(_position(workspace_bytes=need - 1)) == -7 and bwd(_position(workspace=BASE + 4)) == -7
 

@@ -542,6 +542,25 @@ def test_position_bias_strides_and_large_sums(af3):
         assert ((got[:, h] - want).abs() <= 5000 * E32 * want).all()
 
 
+def test_a_bias_of_more_than_4_billion_entries(af3):
+    """Places past 32 bits, in the bias and in its gradient."""
+    n = 46400
+    table = torch.randn(32, 2, device="cuda", dtype=BF16).requires_grad_(True)
+    out = af3.relative_position_bias(table, n, n)                       # 8.6 GB
+    assert out.numel() > 2 ** 32
+    rows = torch.tensor([0, 1, 12345, n - 2, n - 1])
+    known = torch.tensor([bucket(x, 32, "log", True, 128) for x in range(-130, 131)])
+    b = known[(torch.arange(n)[None] - rows[:, None]).clamp(-130, 130) + 130].cuda()
+    for h in range(2):
+        assert torch.equal(out[h, rows.cuda()], table.detach()[:, h][b])
+    got = torch.autograd.grad(out, table, torch.ones(1, 1, n, device="cuda", dtype=BF16).expand(2, n, n))[0].double().cpu()
+    offsets = torch.arange(-(n - 1), n)
+    counts = torch.zeros(32, dtype=torch.float64).index_add_(0, known[offsets.clamp(-130, 130) + 130], (n - offsets.abs()).double())
+    assert ((got - counts[:, None]).abs() <= 2.0 ** -8 * counts[:, None]).all()      # ones add up exactly in fp32 as far as a part goes
+    del out
+    torch.cuda.empty_cache()
+
+
 def test_relative_position_bias_refuses(af3):
     t = torch.randn(32, 4, device="cuda")
     for bad, message in [
