@@ -170,42 +170,53 @@ __global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
 	const int     columns = 1 << a.columns_log2, tx = threadIdx.x & (columns - 1), ty = threadIdx.x >> a.columns_log2, step = COLUMNS >> a.columns_log2;
 	const int64_t col = ((int64_t)blockIdx.x * columns + tx) * E;
 	if(col < a.Lk) {
-		constexpr int AHEAD = 8;   // rows whose loads are in flight together
+		// Four rows on their way while four are added up.  (Not more: a row's additions are 3 KB of code, which every compute unit has to fetch for some
+		// microseconds of work.)
+		constexpr int ROWS = 4;
 		const keys_of_chunk<E> keys(a, col);
 		const int64_t row0 = (int64_t)blockIdx.y * a.rows, last = row0 + a.rows < a.Lq ? row0 + a.rows : a.Lq;
 		const T* const grad = static_cast<const T*>(a.grad) + h * a.grad_stride[0] + col;
+		const bool     full = col + E <= a.Lk;
 		// (an addition that LDS does by itself: nothing waits for the sum so far.  The column is this thread's alone, so the order is the program's)
 		auto add = [&](int bk, float v) { __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float*)(bins + bk * COLUMNS + threadIdx.x), v, 0, 0, false); };
-		const bool     full = col + E <= a.Lk;
-		for(int64_t first = row0 + ty; first < last; first += AHEAD * step) {
-			u32x4   x[AHEAD];
-			int64_t q[AHEAD];
+		struct rows_of {
+			u32x4   x[ROWS];
+			int64_t q[ROWS];
+		};
+		auto fetch = [&](rows_of& to, int64_t first) {
 #pragma unroll
-			for(int i = 0; i < AHEAD; i++) {
-				const int64_t row = first + i * step < last ? first + i * step : first;
-				const T* const at = grad + row * a.grad_stride[1];
-				if(full) x[i] = load16(at);
-				else x[i] = cross::load_guarded(at, 0, (int)(a.Lk - col));
-				q[i] = a.q_pos ? a.q_pos[row] : row + a.q_offset;
+			for(int i = 0; i < ROWS; i++) {
+				const int64_t  row = first + i * step < last ? first + i * step : row0;
+				const T* const at  = grad + row * a.grad_stride[1];
+				if(full) to.x[i] = load16(at);
+				else to.x[i] = cross::load_guarded(at, 0, (int)(a.Lk - col));
+				to.q[i] = a.q_pos ? a.q_pos[row] : row + a.q_offset;
 			}
+		};
+		rows_of mine, coming;
+		fetch(coming, row0 + ty);
+#pragma unroll 1
+		for(int64_t first = row0 + ty; first < last; first += ROWS * step) {
+			mine = coming;
+			if(first + ROWS * step < last) fetch(coming, first + ROWS * step);
 #pragma unroll
-			for(int i = 0; i < AHEAD; i++) {
+			for(int i = 0; i < ROWS; i++) {
 				if(first + i * step >= last) break;
 				int rel[E], bk[E];
-				keys.offsets(q[i], a.reach, rel);
+				keys.offsets(mine.q[i], a.reach, rel);
 #pragma unroll
 				for(int e = 0; e < E; e++) bk[e] = LUT ? bucket[rel[e] + a.reach] : bucket_of(a, border, rel[e]);
 				bool same = true;
 #pragma unroll
 				for(int e = 1; e < E; e++) same = same && bk[e] == bk[0];
 				if(same) {
-					float sum = kind<T>::at(x[i], 0);
+					float sum = kind<T>::at(mine.x[i], 0);
 #pragma unroll
-					for(int e = 1; e < E; e++) sum += kind<T>::at(x[i], e);
+					for(int e = 1; e < E; e++) sum += kind<T>::at(mine.x[i], e);
 					add(bk[0], sum);
 				} else {
 #pragma unroll
-					for(int e = 0; e < E; e++) add(bk[e], kind<T>::at(x[i], e));
+					for(int e = 0; e < E; e++) add(bk[e], kind<T>::at(mine.x[i], e));
 				}
 			}
 		}
