@@ -71,7 +71,7 @@ class CrossAttentionGrads(ctypes.Structure):
 class PositionBiasParams(ctypes.Structure):
     """Mirror of struct af3_position_bias_params."""
     _fields_ = [
-        ("table", vp), ("out", vp), ("grad", vp), ("q_positions", vp), ("k_positions", vp), ("q_offset", i64),
+        ("table", vp), ("out", vp), ("grad", vp), ("grad_residual", vp), ("q_positions", vp), ("k_positions", vp), ("q_offset", i64),
         ("table_stride", i64 * 2), ("grad_stride", i64 * 2),
         ("buckets", i64), ("H", i64), ("Lq", i64), ("Lk", i64), ("max_distance", i64),
         ("scheme", i32), ("bidirectional", i32), ("dtype", i32), ("reserved", i32),

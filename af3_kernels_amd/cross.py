@@ -91,7 +91,7 @@ def _backward(grad, q, k, v, keep, bias, out, stats, lost, scale, wants):
 
 class _CrossAttention(torch.autograd.Function):
     """A bfloat16 bias straight out of relative_position_bias hands its table on (`table`, with that call's positions and settings): its gradient reaches the table
-    as bfloat16, and what that rounding lost reaches the table directly."""
+    as bfloat16, and what that rounding and the one of its sums lose reaches the table directly."""
 
     @staticmethod
     def forward(ctx, q, k, v, keep, bias, scale, table, settings, q_positions, k_positions):
@@ -107,13 +107,13 @@ class _CrossAttention(torch.autograd.Function):
         needs = ctx.needs_input_grad
         residual = needs[4] and needs[6] and stats is not None
         dq, dk, dv, dbias, bias_lost = _backward(grad, q, k, v, keep, bias, out, stats, lost, ctx.scale, (needs[0], needs[1], needs[2], needs[4], residual))
-        dtable = _position_sums(bias_lost, ctx.table_shape, ctx.settings, q_positions, k_positions) if residual else None
+        dtable = _position_sums(dbias, bias_lost, ctx.table_shape, ctx.settings, q_positions, k_positions) if residual else None
         return dq, dk, dv, None, dbias, None, dtable, None, None, None
 
 
 def _source(bias):
     """(table, settings, q_positions, k_positions) of a bfloat16 bias that is relative_position_bias's result as it stands."""
-    node = bias.grad_fn if bias is not None and bias.dtype == torch.bfloat16 and bias.requires_grad else None
+    node = bias.grad_fn if bias is not None and bias.dtype == torch.bfloat16 and bias.requires_grad and bias.shape[0] < 1 << 15 else None
     if isinstance(node, _PositionBias._backward_cls):
         try:
             q_positions, k_positions = node.saved_tensors
@@ -208,14 +208,16 @@ def _position_forward(table, q_len, k_len, settings, q_positions, k_positions):
     return out
 
 
-def _position_sums(grad, table_shape, settings, q_positions, k_positions):
-    """The table's gradient of a gradient [H, Lq, Lk] of the bias."""
+def _position_sums(grad, lost, table_shape, settings, q_positions, k_positions):
+    """The table's gradient of a gradient [H, Lq, Lk] of the bias; with what that one's rounding lost (laid out like it): what the first call misses."""
     out = torch.empty(table_shape, dtype=grad.dtype, device=grad.device)
     if grad.numel() == 0:
         return out.zero_()
     grad = _inner_contig(grad)
     p = _position_params(table_shape, out.stride(), grad.dtype, grad.shape[1], grad.shape[2], settings, q_positions, k_positions)
     p.grad, p.grad_stride, p.out = grad.data_ptr(), _i64x2(grad.stride(0), grad.stride(1)), out.data_ptr()
+    if lost is not None:
+        p.grad_residual = lost.data_ptr()
     lib = _lib.load()
     with ops._on_device(grad.device):
         need = lib.af3_position_bias_workspace_bytes(ctypes.byref(p))
@@ -237,7 +239,7 @@ class _PositionBias(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         q_positions, k_positions = ctx.saved_tensors
-        return _position_sums(grad, ctx.table.shape, ctx.settings, q_positions, k_positions), None, None, None, None, None
+        return _position_sums(grad, None, ctx.table.shape, ctx.settings, q_positions, k_positions), None, None, None, None, None
 
 
 def _check_settings(buckets, scheme, bidirectional, max_distance, q_offset):

@@ -702,13 +702,14 @@ struct position_function : torch::autograd::Function<position_function> {
 		ctx->saved_data["settings"] = std::move(s);
 		return out;
 	}
-	// the table's gradient [buckets, H] of a gradient g of the bias
-	static Tensor sums(Tensor g, const Tensor& q_positions, const Tensor& k_positions, const std::vector<int64_t>& s) {
+	// the table's gradient [buckets, H] of a gradient g of the bias; with what g's rounding lost (laid out like g): what that misses
+	static Tensor sums(Tensor g, const Tensor& lost, const Tensor& q_positions, const Tensor& k_positions, const std::vector<int64_t>& s) {
 		const int dev = (int)g.get_device();
 		if(!inner_1(g)) g = g.contiguous();
 		Tensor out = new_tensor({s[6], s[7]}, g.scalar_type(), dev);
 		const position_call call{Tensor(), q_positions, k_positions, s[0], s[1], s[2], s[3], s[4], s[5]};
 		af3_position_bias_params p = call.block(out.sizes(), out.strides(), g.scalar_type());
+		if(lost.defined()) p.grad_residual = lost.const_data_ptr();
 		p.grad = g.const_data_ptr(), p.grad_stride[0] = g.stride(0), p.grad_stride[1] = g.stride(1), p.out = out.data_ptr();
 		const int64_t bytes = af3_position_bias_workspace_bytes(&p);
 		raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_position_bias_workspace_bytes");
@@ -722,7 +723,7 @@ struct position_function : torch::autograd::Function<position_function> {
 		{
 			at::AutoGradMode none(false);
 			const auto saved = ctx->get_saved_variables();
-			grads[0] = sums(grad_out[0], saved[0], saved[1], ctx->saved_data["settings"].toIntVector());
+			grads[0] = sums(grad_out[0], Tensor(), saved[0], saved[1], ctx->saved_data["settings"].toIntVector());
 		}
 		return once(std::move(grads), "relative_position_bias");
 	}
@@ -760,9 +761,9 @@ struct cross_call {
 	}
 };
 // A bfloat16 bias that comes straight out of relative_position_bias hands its table on as an input (`table`, with that call's positions and settings): the
-// bias's gradient takes its usual way to the table, rounded to bfloat16 as a gradient of a bfloat16 tensor has to be, and what that rounding lost goes
-// to the table directly.  The sum of the two is the table's gradient; what a caller does with the bias's gradient on the way is none of the second part's business
-// (2^-8 of the first).
+// bias's gradient takes its usual way to the table, rounded to bfloat16 as a gradient of a bfloat16 tensor has to be, and what that rounding and the one of its
+// sums lose goes to the table directly.  The sum of the two is the table's gradient, rounded once; what a caller does with the bias's gradient on the
+// way is none of the second part's business (2^-8 of the first).
 struct cross_function : torch::autograd::Function<cross_function> {
 	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& given_bias, const std::optional<Tensor>& table,
 					  const std::optional<Tensor>& given_mask, double scale, torch::autograd::variable_list positions, std::vector<int64_t> settings) {
@@ -808,7 +809,7 @@ struct cross_function : torch::autograd::Function<cross_function> {
 			const at::DataPtr ws = new_scratch(bytes);
 			o.workspace = ws.get(), o.workspace_bytes = bytes;
 			raise(af3_cross_attention_backward(&p, &o, current_stream(dev)), "af3_cross_attention_backward");
-			if(bias_lost.defined()) grads[4] = position_function::sums(bias_lost, saved[8], saved[9], ctx->saved_data["settings"].toIntVector());
+			if(bias_lost.defined()) grads[4] = position_function::sums(grads[3], bias_lost, saved[8], saved[9], ctx->saved_data["settings"].toIntVector());
 		}
 		return once(std::move(grads), "cross_attention");
 	}
@@ -824,7 +825,7 @@ Tensor apply_cross(const cross_call& c) {
 	std::optional<Tensor>          table;
 	torch::autograd::variable_list positions;
 	std::vector<int64_t>           settings;
-	if(c.bias.defined() && c.bias.scalar_type() == at::kBFloat16 && c.bias.requires_grad())
+	if(c.bias.defined() && c.bias.scalar_type() == at::kBFloat16 && c.bias.requires_grad() && c.q.size(1) <= 0x7fff)
 		if(auto* node = dynamic_cast<torch::autograd::CppNode<position_function>*>(c.bias.grad_fn().get())) {
 			try {
 				positions = node->ctx_.get_saved_variables(), table = node->ctx_.saved_data["table"].toTensor(), settings = node->ctx_.saved_data["settings"].toIntVector();

@@ -23,8 +23,8 @@ constexpr int THREADS = 256;
 struct args {
 	const void*    table;    // forward: the values; backward: not read
 	void*          out;      // forward: [H, Lq, Lk]; backward: the table's gradient
-	const void*    grad;     // backward: [H, Lq, Lk]
-	float*         partial;  // backward: [H][parts][buckets]
+	const void *   grad, *rest;   // backward: [H, Lq, Lk]; what its rounding lost, or null
+	float*         partial;  // backward: [H][parts][buckets], with rest those of rest behind them
 	const int64_t *q_pos, *k_pos;
 	int64_t        q_offset;
 	int64_t        table_stride[2], grad_stride[2];
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
 	extern __shared__ float bins[];   // [buckets][COLUMNS]
 	int* const      border = reinterpret_cast<int*>(bins + a.buckets * COLUMNS);         // [borders]
 	uint16_t* const bucket = reinterpret_cast<uint16_t*>(border + a.borders);            // [2 reach + 1], where they are tabulated
-	const int64_t  h = blockIdx.z;
+	const int64_t  z = blockIdx.z, h = z < a.H ? z : z - a.H;   // (the second H of them add up `rest`)
 	for(int i = threadIdx.x; i < a.borders; i += COLUMNS) border[i] = border_of(a, i);
 	for(int i = 0; i < a.buckets; i++) bins[i * COLUMNS + threadIdx.x] = 0.f;
 	__syncthreads();
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
 		constexpr int ROWS = 4;
 		const keys_of_chunk<E> keys(a, col);
 		const int64_t row0 = (int64_t)blockIdx.y * a.rows, last = row0 + a.rows < a.Lq ? row0 + a.rows : a.Lq;
-		const T* const grad = static_cast<const T*>(a.grad) + h * a.grad_stride[0] + col;
+		const T* const grad = static_cast<const T*>(z < a.H ? a.grad : a.rest) + h * a.grad_stride[0] + col;
 		const bool     full = col + E <= a.Lk;
 		// (an addition that LDS does by itself: nothing waits for the sum so far.  The column is this thread's alone, so the order is the program's)
 		auto add = [&](int bk, float v) { __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float*)(bins + bk * COLUMNS + threadIdx.x), v, 0, 0, false); };
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
 		float sum = 0.f;
 #pragma unroll 16
 		for(int c = 0; c < COLUMNS; c++) sum += bins[i * COLUMNS + ((c + threadIdx.x) & (COLUMNS - 1))];
-		a.partial[(h * parts + part) * a.buckets + i] = sum;
+		a.partial[(z * parts + part) * a.buckets + i] = sum;
 	}
 }
 template <typename T>
@@ -237,11 +237,21 @@ __global__ void __launch_bounds__(THREADS) position_bias_join_kernel(args a, int
 	const int     lane = threadIdx.x & 63;
 	if(n >= a.H * a.buckets) return;
 	const int64_t h = n / a.buckets, i = n % a.buckets;
-	double        sum = 0.0;
-	for(int64_t part = lane; part < parts; part += 64) sum += (double)a.partial[(h * parts + part) * a.buckets + i];
+	auto total = [&](const float* of) {
+		double sum = 0.0;
+		for(int64_t part = lane; part < parts; part += 64) sum += (double)of[(h * parts + part) * a.buckets + i];
 #pragma unroll
-	for(int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
-	if(lane == 0) static_cast<T*>(a.out)[i * a.table_stride[0] + h * a.table_stride[1]] = kind<T>::bits((float)sum);
+		for(int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
+		return sum;
+	};
+	const double sum   = total(a.partial);
+	T            value = kind<T>::bits((float)sum);
+	if(a.rest) {   // what a call without rest misses: its answer is `value`
+		const double rest = total(a.partial + a.H * parts * a.buckets);
+		const float  own  = kind<T>::value(value);
+		value = kind<T>::bits(__builtin_isfinite(own) ? (float)(sum + rest - (double)own) : 0.f);
+	}
+	if(lane == 0) static_cast<T*>(a.out)[i * a.table_stride[0] + h * a.table_stride[1]] = value;
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
@@ -319,7 +329,7 @@ int prepare(const af3_position_bias_params* p, args& a) {
 	a.table_stride[0] = p->table_stride[0], a.table_stride[1] = p->table_stride[1];
 	a.grad_stride[0] = p->grad_stride[0], a.grad_stride[1] = p->grad_stride[1];
 	a.H = p->H, a.Lq = p->Lq, a.Lk = p->Lk;
-	a.table = p->table, a.out = p->out, a.grad = p->grad, a.partial = nullptr;
+	a.table = p->table, a.out = p->out, a.grad = p->grad, a.rest = p->grad_residual, a.partial = nullptr;
 	return AF3_OK;
 }
 bool tabulated(const args& a) { return 2 * (int64_t)a.reach + 1 <= MAX_OFFSETS; }
@@ -339,7 +349,9 @@ dim3 sums_shape(args& a, int E) {
 	// about 2048 workgroups; each adds its bins up, which is worth a few hundred rows of reading
 	const int64_t pieces = a.H * a.Lq * ((a.Lk + E - 1) / E);
 	int64_t       each = pieces / (2048 * COLUMNS);
-	return shape(a, E, COLUMNS, each < 8 ? 8 : each > 4096 ? 4096 : each);
+	dim3 grid = shape(a, E, COLUMNS, each < 8 ? 8 : each > 4096 ? 4096 : each);
+	if(a.rest) grid.z *= 2;   // (cut like the call without it, whose sums these have to be to the bit)
+	return grid;
 }
 dim3 forward_shape(args& a, int E) {
 	// about 1024 workgroups, of one to 16 pieces per thread
@@ -388,6 +400,7 @@ extern "C" int af3_position_bias_forward(const af3_position_bias_params* params,
 extern "C" int64_t af3_position_bias_workspace_bytes(const af3_position_bias_params* params) {
 	position::args a;
 	if(const int rc = position::prepare(params, a); rc != AF3_OK) return rc;
+	if(a.rest && a.H > 0x7fff) return AF3_ERR_BAD_SHAPE;
 	const dim3 grid = position::sums_shape(a, params->dtype == AF3_F32 ? 4 : 8);
 	return (int64_t)grid.x * grid.y * grid.z * a.buckets * 4;
 }
@@ -396,6 +409,7 @@ extern "C" int af3_position_bias_backward(const af3_position_bias_params* params
 	position::args a;
 	if(const int rc = position::prepare(params, a); rc != AF3_OK) return rc;
 	if(!params->grad || !params->out || !params->workspace) return AF3_ERR_NULL_POINTER;
+	if(a.rest && a.H > 0x7fff) return AF3_ERR_BAD_SHAPE;
 	if(params->grad_stride[0] < 0 || params->grad_stride[1] < 0) return AF3_ERR_BAD_STRIDE;
 	if((params->buckets > 1 && params->table_stride[0] == 0) || (params->H > 1 && params->table_stride[1] == 0)) return AF3_ERR_BAD_STRIDE;   // (results may not share a place)
 	const dim3 grid = position::sums_shape(a, params->dtype == AF3_F32 ? 4 : 8);

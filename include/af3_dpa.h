@@ -408,6 +408,9 @@ int64_t af3_cross_attention_backward_workspace_bytes(const af3_cross_attention_p
  * Positions are q_offset + 0, 1, 2, ... and 0, 1, 2, ..., or, where given, q_positions [Lq] and k_positions [Lk] (device memory, any 64-bit numbers).
  * forward: table [buckets, H] with element strides, out.  backward: grad [H, Lq, Lk] with strides for H and q (key stride 1), out = the table's
  * gradient [buckets, H] with table_stride, workspace of af3_position_bias_workspace_bytes() bytes, 16-byte aligned; sums in a fixed order.
+ * grad_residual (optional, backward only; dtype, layout and strides of grad): what grad lost by its rounding, e.g. an attention call's grad_bias_residual.
+ * out is then what the same call without it misses: the two added are the gradient of grad + grad_residual with its last rounding alone (zeros where the first is
+ * not finite).  With it H <= 32767, and the workspace is asked for with it set.
  * H <= 65535, Lq and Lk < 2^30, buckets <= AF3_POSITION_BIAS_MAX_BUCKETS, |q_offset| <= 2^62.
  */
 #define AF3_POSITION_BIAS_MAX_BUCKETS 576
@@ -416,6 +419,7 @@ typedef struct af3_position_bias_params {
 	const void*    table;
 	void*          out;
 	const void*    grad;
+	const void*    grad_residual;
 	const int64_t* q_positions;
 	const int64_t* k_positions;
 	int64_t        q_offset;

@@ -134,6 +134,11 @@ def test_position_bias_validates_on_the_host():
     assert bwd(_position(table_stride=i64x2(0, 1))) == -4 and bwd(_position(table_stride=i64x2(1, 0))) == -4
     need = lib.af3_position_bias_workspace_bytes(ctypes.byref(_position()))
     assert need > 0 and bwd(_position(workspace_bytes=need - 1)) == -7 and bwd(_position(workspace=BASE + 4)) == -7
+    # with what the gradient's rounding lost: room for both sums, and half the heads at most
+    both = lib.af3_position_bias_workspace_bytes(ctypes.byref(_position(grad_residual=5 * BASE)))
+    assert both == 2 * need and bwd(_position(grad_residual=5 * BASE, workspace_bytes=both - 1)) == -7
+    for call in (bwd, lambda p: lib.af3_position_bias_workspace_bytes(ctypes.byref(p))):
+        assert call(_position(grad_residual=5 * BASE, H=1 << 15)) == -3
 
 
 def test_wrappers_reject_cpu_tensors():
