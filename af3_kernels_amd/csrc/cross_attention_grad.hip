@@ -4,7 +4,7 @@
 // S and P are computed again from q, k and the two numbers per row that the forward pass left (maximum and 1 / sum: kept apart, since
 // a maximum of the lowest float plus the logarithm of a sum is that maximum again).  Three kernels, none with atomics: each element
 // of a result is summed by one workgroup, or by one per part of the long axis and a joining kernel, always in the same order.
-//   cross_dq_kernel    32 query rows per wavefront, keys in tiles (writes delta too)
+//   cross_dq_kernel    32 query rows per wavefront, keys in tiles (writes delta too, and for a bias what it misses)
 //   cross_dkv_kernel   32 keys per wavefront, query rows in tiles, over all query heads of the key head
 //   cross_dbias_kernel 32 query rows x 32 keys per wavefront, over the batch
 #include "cross_tiles.hpp"
@@ -27,6 +27,7 @@ struct grad_args {
 	float*   delta;           // [B, H, Lq]
 	float*   partial;         // dq: [splits][B H Lq][D]; dkv: [splits][2][B Hkv Lk][D]
 	float *  dq_space, *dkv_space;
+	float *  more, *row_sums; // what delta is short of, [B, H, Lq], or null; where cross_dq_kernel writes it: there, or its parts [splits][B, H, Lq]
 };
 
 // the sum of the wavefronts' results of equal shape, wavefront w keeps the blocks of columns that are w modulo N; `mine`: N tables of 32 x (DP + 4)
@@ -118,6 +119,12 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 	const T* const bias = BIAS ? static_cast<const T*>(p.bias) + h * p.bias_stride[0] + qi * p.bias_stride[1] : nullptr;
 	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b : nullptr;
 
+	// The sum of a row of dS, which is zero but for what delta misses: out is made of probabilities rounded to bf16.  The bias's gradient is told (a sum over rows of it,
+	// as a table's gradient is one, is made of what is left of such sums: at 8 x 12 x 512 x 512 x 64 and 32 buckets it was off by 0.0021 without this and is by 0.0014,
+	// its last rounding to bf16 alone; no time lost, 30.2 us before and after).
+	constexpr bool SUMS = BIAS && sizeof(T) == 2;
+	__shared__ float wave_sums[SUMS && KW > 1 ? WAVES : 1][32];
+	float row_sum = 0.f;
 	f32x16 dq[TL::BLOCKS];
 #pragma unroll
 	for(int db = 0; db < TL::BLOCKS; db++) dq[db] = f32x16{};
@@ -184,6 +191,11 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 					for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(logit(r), a.factor, -taken)) * (dp[r] - delta);
 				}
 				if(keep != ~0u) drop_keys(x, keep, 0.f);
+				if constexpr(SUMS)
+					if(a.row_sums) {
+#pragma unroll
+						for(int r = 0; r < 16; r++) row_sum += x[r];
+					}
 #pragma unroll
 				for(int j = 0; j < TL::JOINTS; j++) {
 					const u32x4 f = kind<T>::pack(x + E * j);
@@ -195,11 +207,25 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 			if constexpr(S::BUFFERS == 2) buffer ^= 1;
 		}
 	}
+	if constexpr(SUMS) {
+		row_sum = sum_of_halves(row_sum);
+		if constexpr(KW > 1) wave_sums[wave][lane & 31] = row_sum;
+	}
 	if constexpr(KW > 1) {
 		__syncthreads();
 		add_up<DP, KW>(reinterpret_cast<float*>(smem) + rwave * KW * 32 * (DP + 4), kwave, lane, dq);
 	}
 	if(!ok) return;
+	if constexpr(SUMS)
+		if(a.row_sums && kwave == 0 && half == 0) {
+			if constexpr(KW > 1) {
+				row_sum = 0.f;
+#pragma unroll
+				for(int w = 0; w < KW; w++) row_sum += wave_sums[rwave * KW + w][lane & 31];
+			}
+			a.row_sums[split * (p.B * p.H * p.Lq) + row] = row_sum;
+		}
+	if(!a.g.grad_q) return;
 #pragma unroll
 	for(int db = 0; db < TL::BLOCKS; db++) {
 		if(db % KW != kwave) continue;
@@ -211,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 	}
 }
 
-// delta alone, for calls that want no gradient of q: 32 rows per wavefront, added up as cross_dq_kernel does
+// delta alone, for calls that want no gradient of q or the bias: 32 rows per wavefront, added up as cross_dq_kernel does
 template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS) cross_delta_kernel(grad_args a) {
 	const af3_cross_attention_params& p = a.p;
@@ -231,13 +257,13 @@ constexpr int ROW_STATS = 4;
 template <typename T, int QT>
 struct row_stats {
 	float taken, less, m, inv;   // of one row, on its way
-	__device__ __forceinline__ void load(const grad_args& a, int64_t bh, int64_t q0) {
+	__device__ __forceinline__ void load(const grad_args& a, int64_t bh, int64_t q0, const float* more = nullptr) {
 		taken = less = m = inv = 0.f;
 		if((int)threadIdx.x >= QT) return;
 		const bool ok = q0 + threadIdx.x < a.p.Lq;
 		if(ok) {
 			const int64_t row = bh * a.p.Lq + q0 + threadIdx.x;
-			m = a.p.stats[2 * row], inv = a.p.stats[2 * row + 1], less = -a.delta[row];
+			m = a.p.stats[2 * row], inv = a.p.stats[2 * row + 1], less = -(more ? a.delta[row] + more[row] : a.delta[row]);
 		}
 	}
 	__device__ __forceinline__ void store(float* st, float factor) const {
@@ -429,34 +455,40 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dkv_shape<T, DP, RW, BIAS>
 	}
 }
 
-// The parts' sums added in order, of up to three results at once (a result of one part was written where it belongs).
+// The parts' sums added in order, of up to four results at once (a result of one part was written where it belongs).
+constexpr int RESULTS = 4;
 struct parts {
-	const float* partial[3];
-	int64_t      step[3], n[3];   // elements from one part to the next, elements
-	uint32_t     splits[3], blocks[3];
-	void*        out[3];
+	const float* partial[RESULTS];
+	int64_t      step[RESULTS], n[RESULTS];   // elements from one part to the next, elements
+	uint32_t     splits[RESULTS], blocks[RESULTS];
+	void*        out[RESULTS];
+	bool         wide[RESULTS];   // fp32, whatever T is
 };
 template <typename T>
 __global__ void __launch_bounds__(THREADS) cross_sum_kernel(parts a) {
 	uint32_t block = blockIdx.x;
 	int      which = 0;
-	while(which < 2 && block >= a.blocks[which]) block -= a.blocks[which++];
+	while(which < RESULTS - 1 && block >= a.blocks[which]) block -= a.blocks[which++];
 	const int64_t  i = ((int64_t)block * THREADS + threadIdx.x) * 4, n = a.n[which], step = a.step[which];
 	const uint32_t splits = a.splits[which];
 	const float*   at = a.partial[which] + i;
 	T* const       out = static_cast<T*>(a.out[which]) + i;
+	float* const   wide = a.wide[which] ? static_cast<float*>(a.out[which]) + i : nullptr;
 	if(i >= n) return;
 	if(i + 4 <= n) {
 		f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
 		for(uint32_t s = 0; s < splits; s++, at += step) sum += *reinterpret_cast<const f32x4_any*>(at);
 #pragma unroll
-		for(int e = 0; e < 4; e++) out[e] = kind<T>::bits(sum[e]);
+		for(int e = 0; e < 4; e++)
+			if(wide) wide[e] = sum[e];
+			else out[e] = kind<T>::bits(sum[e]);
 	} else {
 		for(int e = 0; i + e < n; e++) {
 			float x = 0.f;
 			for(uint32_t s = 0; s < splits; s++) x += at[s * step + e];
-			out[e] = kind<T>::bits(x);
+			if(wide) wide[e] = x;
+			else out[e] = kind<T>::bits(x);
 		}
 	}
 }
@@ -514,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 		pg.load(q0, p.Lq);
 		pk.load(k0, p.Lk);
 		pv.load(k0, p.Lk);
-		rs.load(a, b * p.H + h, q0);
+		rs.load(a, b * p.H + h, q0, a.more);
 	};
 	fetch(0);
 	const int64_t rows_left = p.Lq - q0, keys_left = p.Lk - k0;
@@ -598,15 +630,17 @@ cut dkv_cut(const af3_cross_attention_params& p) {
 }
 
 struct grad_space {
-	int64_t delta, dq, dkv, bytes;   // floats
+	int64_t delta, more, row_sums, dq, dkv, bytes;   // floats
 };
 grad_space grad_workspace(const af3_cross_attention_params& p) {
 	const cut  q = dq_cut(p), kv = dkv_cut(p);
 	grad_space w;
 	w.delta = over(p.B * p.H * p.Lq, 4) * 4;
+	w.more  = p.bias && p.dtype == AF3_BF16 ? w.delta : 0;
+	w.row_sums = w.more && q.splits > 1 ? over(q.splits * p.B * p.H * p.Lq, 4) * 4 : 0;
 	w.dq    = q.splits > 1 ? over(q.splits * p.B * p.H * p.Lq * p.D, 4) * 4 : 0;
 	w.dkv   = kv.splits > 1 ? 2 * (int64_t)kv.splits * p.B * p.Hkv * p.Lk * p.D : 0;
-	w.bytes = (w.delta + w.dq + w.dkv) * 4;
+	w.bytes = (w.delta + w.more + w.row_sums + w.dq + w.dkv) * 4;
 	return w;
 }
 
@@ -627,21 +661,27 @@ int backward(grad_args a, hipStream_t s) {
 	parts    sums{};
 	int      n_sums = 0;
 	uint32_t sum_blocks = 0;
-	auto add = [&](const float* partial, int64_t step, uint32_t splits, void* out, int64_t n) {
+	auto add = [&](const float* partial, int64_t step, uint32_t splits, void* out, int64_t n, bool wide = false) {
 		if(!out) return;
+		sums.wide[n_sums] = wide;
 		sums.partial[n_sums] = partial, sums.step[n_sums] = step, sums.n[n_sums] = n, sums.splits[n_sums] = splits, sums.out[n_sums] = out;
 		sum_blocks += sums.blocks[n_sums] = (uint32_t)over(n, 4 * THREADS);
 		n_sums++;
 	};
-	if(a.g.grad_q) {
+	if(!a.g.grad_bias) a.more = nullptr;
+	if(a.g.grad_q || a.more) {
 		const cut c = dq_cut(p);
 		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part, a.partial = a.dq_space;
+		a.row_sums = a.more && c.splits > 1 ? a.row_sums : a.more;
 		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * c.tiles * c.splits;
 		int rc;
 		if(c.shared) rc = p.bias ? launch(cross_dq_kernel<T, DP, 4, true>, dq_shape<T, DP, 4>::LDS, grid, a, s) : launch(cross_dq_kernel<T, DP, 4, false>, dq_shape<T, DP, 4>::LDS, grid, a, s);
 		else rc = p.bias ? launch(cross_dq_kernel<T, DP, 1, true>, dq_shape<T, DP, 1>::LDS, grid, a, s) : launch(cross_dq_kernel<T, DP, 1, false>, dq_shape<T, DP, 1>::LDS, grid, a, s);
 		if(rc != AF3_OK) return rc;
-		if(c.splits > 1) add(a.partial, n_rows * p.D, c.splits, a.g.grad_q, n_rows * p.D);
+		if(c.splits > 1) {
+			add(a.partial, n_rows * p.D, c.splits, a.g.grad_q, n_rows * p.D);
+			add(a.row_sums, n_rows, c.splits, a.more, n_rows, true);
+		}
 	} else {
 		hipLaunchKernelGGL((cross_delta_kernel<T, DP>), dim3((uint32_t)over(n_rows, 32 * WAVES)), dim3(THREADS), 0, s, a);
 		if(const int rc = launch_status(); rc != AF3_OK) return rc;
@@ -710,7 +750,9 @@ extern "C" int af3_cross_attention_backward(const af3_cross_attention_params* pa
 	a.factor  = params->bias ? LOG2E : params->softmax_scale * LOG2E;
 	a.whole   = params->D * (params->dtype == AF3_F32 ? 4 : 2) % 16 == 0;
 	a.delta   = static_cast<float*>(grads->workspace);
-	a.partial = nullptr, a.dq_space = a.delta + w.delta, a.dkv_space = a.dq_space + w.dq;
+	a.more     = w.more ? a.delta + w.delta : nullptr;
+	a.row_sums = a.delta + w.delta + w.more;
+	a.partial  = nullptr, a.dq_space = a.row_sums + w.row_sums, a.dkv_space = a.dq_space + w.dq;
 	const hipStream_t s = static_cast<hipStream_t>(hip_stream);
 	return params->dtype == AF3_F32 ? cross::backward_type<float>(a, s) : cross::backward_type<uint16_t>(a, s);
 }

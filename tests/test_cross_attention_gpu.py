@@ -655,6 +655,30 @@ def test_a_table_behind_bf16_attention_loses_nothing_to_the_biass_gradient(af3, 
     print("table's gradient off by", error(dtable), "and by the plain route", error(changed))
 
 
+@pytest.mark.parametrize("H,Hkv,Lq,Lk,D", [(2, 2, 200, 200, 64), (2, 1, 9, 1500, 32), (96, 48, 300, 130, 64), (1, 1, 1, 1, 16), (3, 1, 40, 777, 100)])
+def test_the_rows_of_the_biass_gradient_sum_to_zero(af3, H, Hkv, Lq, Lk, D):
+    """... although delta comes from a result whose probabilities were rounded to bf16: a table's gradient is made of what is left of these sums.  The same bits whether the
+    gradients of q, k and v are wanted or not."""
+    from af3_kernels_amd import cross
+    q, k, v, m, bias, g = make(1, H, Hkv, Lq, Lk, D, BF16, 83, "random", "given")
+    scale = D ** -0.5
+    out, stats, lost = cross._forward(q, k, v, m, bias, scale, True)
+    alone, whole = (cross._backward(g, q, k, v, m, bias, out, stats, lost, scale, (w, w, w, True, True)) for w in (False, True))
+    assert all(torch.equal(a, b) for a, b in zip(alone[3:], whole[3:]))
+    rows = (alone[3].double() + alone[4].double()).sum(-1).cpu()
+    Q, K, V, X, G = (t.double().cpu() for t in (q[0], spread(k, H)[0], spread(v, H)[0], bias, g[0]))
+    gone = ~m.cpu().expand(1, Lk)
+    x = (torch.matmul(Q, K.transpose(1, 2)) * scale + X).masked_fill(gone, -math.inf)
+    size = (torch.matmul(Q.abs(), K.abs().transpose(1, 2)) * scale + X.abs()).masked_fill(gone, 0.0)
+    p = torch.softmax(x, -1)
+    dp = torch.matmul(G, V.transpose(1, 2))
+    delta = (p * dp).sum(-1, keepdim=True)
+    ep = 2 * (D + 8) * E32 * size.amax(-1, keepdim=True) + (Lk + 16) * E32
+    # P twice (where the row is summed and where dS is made), its sum's distance from one, dP twice, the sum of Lk terms, dbias and its residual rounded to bf16 each
+    limit = (p * ((2 * ep + (Lk + 24) * E32) * (dp.abs() + delta.abs()) + 2 * (D + 2) * E32 * torch.matmul(G.abs(), V.abs().transpose(1, 2)) + 2.0 ** -16 * (dp - delta).abs())).sum(-1)
+    assert (rows.abs() <= limit).all(), (rows.abs() / limit).max()
+
+
 @pytest.mark.parametrize("H,L,buckets,scheme,both,r", [(4, 200, 32, "log", True, 128), (1, 17, 3, "clip", True, 1), (3, 131, 575, "clip", True, 287), (2, 301, 16, "log", False, 5000)])
 def test_the_sums_of_a_rounded_gradient_and_its_residual_round_once(af3, H, L, buckets, scheme, both, r):
     """What goes to the table directly makes up for both roundings: of the terms, and of the sums that go the usual way."""
