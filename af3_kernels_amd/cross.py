@@ -119,7 +119,8 @@ def _source(bias):
             q_positions, k_positions = node.saved_tensors
         except RuntimeError:   # (that graph was freed: a backward pass through the bias will say so)
             return None, None, None, None
-        return node.table, node.settings, q_positions, k_positions
+        if node.table._version == node.version:   # (changed since: what led to the bias is not what its gradient goes to any more)
+            return node.table, node.settings, q_positions, k_positions
     return None, None, None, None
 
 
@@ -232,7 +233,7 @@ class _PositionBias(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, q_len, k_len, settings, q_positions, k_positions):
         ctx.save_for_backward(q_positions, k_positions)
-        ctx.table, ctx.settings = table, settings   # (not a saved tensor: the gradient does not need its values, which may change)
+        ctx.table, ctx.version, ctx.settings = table, table._version, settings   # (not a saved tensor: the gradient does not need its values, which may change)
         return _position_forward(table, q_len, k_len, settings, q_positions, k_positions)
 
     @staticmethod

@@ -427,8 +427,8 @@ int validate_cross_attention(const af3_cross_attention_params* p) {
 	if(p->dtype != AF3_F32 && p->dtype != AF3_BF16) return AF3_ERR_BAD_DTYPE;
 	if(p->B <= 0 || p->H <= 0 || p->Hkv <= 0 || p->Lq <= 0 || p->Lk <= 0 || p->D <= 0 || p->H % p->Hkv != 0) return AF3_ERR_BAD_SHAPE;
 	if(p->D > AF3_DPA_MAX_HEAD_DIM) return AF3_ERR_UNSUPPORTED_D;
-	// (row numbers, workgroup numbers and the parts' sizes stay far inside 32 and 63 bits)
-	if(p->B > 0xffffff || p->H > 0xffff || p->Lq > 0x3fffffff || p->Lk > 0x3fffffff || p->B * p->H > 0xffffff || p->H * p->Lq > 0x7fffffff || p->B * p->H * ((p->Lq + 31) / 32) > 0x3ffffff) return AF3_ERR_BAD_SHAPE;
+	// (row numbers and the parts' sizes stay far inside 63 bits, a launch's workgroups times 256 threads inside 32)
+	if(p->B > 0xffffff || p->H > 0xffff || p->Lq > 0x3fffffff || p->Lk > 0x3fffffff || p->B * p->H > 0xffffff || p->H * p->Lq > 0x7fffffff || p->B * p->H * ((p->Lq + 31) / 32) > 0xffffff) return AF3_ERR_BAD_SHAPE;
 	if(!p->q || !p->k || !p->v || !p->out) return AF3_ERR_NULL_POINTER;
 	for(int i = 0; i < 3; i++)
 		if(p->q_stride[i] < 0 || p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;

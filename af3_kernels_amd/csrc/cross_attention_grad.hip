@@ -726,7 +726,7 @@ int validate_grads(const af3_cross_attention_params* p, const af3_cross_attentio
 	for(int i = 0; i < 3; i++)
 		if(g->grad_out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
 	// (workgroup numbers of the kernels whose results are the keys' and the bias's)
-	if(p->B * p->Hkv * over(p->Lk, 32) > 0x3ffffff || p->H * over(p->Lq, 32) > 0x3ffffff || p->H * over(p->Lq, 64) * over(p->Lk, 64) > 0x3ffffff) return AF3_ERR_BAD_SHAPE;
+	if(p->B * p->Hkv * over(p->Lk, 32) > 0xffffff || (g->grad_bias && p->H * over(p->Lq, 64) * over(p->Lk, 64) > 0xffffff)) return AF3_ERR_BAD_SHAPE;
 	return AF3_OK;
 }
 

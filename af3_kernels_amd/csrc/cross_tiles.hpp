@@ -127,8 +127,6 @@ struct tile {
 				col = 16 * half * STRIDE + place(16 * half, r >> 2) + 4 * (r & 3);
 			}
 		}
-		// what follows is worked out anew, not kept in registers from the last time
-		__device__ __forceinline__ void forget() { asm volatile("" : "+v"(row), "+v"(col)); }
 	};
 	// contraction over the columns: A operand, step s, of the 32 rows from `row0` (a multiple of 32) on
 	static __device__ __forceinline__ u32x4 row_frag(const unsigned char* lds, int row0, int s, const reader& at) {
@@ -286,7 +284,6 @@ struct live_keys {
 		}
 		return -1;
 	}
-	__device__ __forceinline__ uint32_t word(int i) const { return (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[i]); }
 };
 // the bits of a tile's keys, the same for all lanes
 template <int KT>

@@ -698,6 +698,7 @@ struct position_function : torch::autograd::Function<position_function> {
 		raise(position_call{table, q_positions, k_positions, s[0], s[1], s[2], s[3], s[4], s[5]}.forward(out), "af3_position_bias_forward");
 		ctx->save_for_backward({q_positions, k_positions});
 		ctx->saved_data["table"] = table;   // (for apply_cross; not a saved variable: the gradient does not need its values, which may change)
+		ctx->saved_data["version"] = (int64_t)table._version();
 		s.push_back(table.size(0)), s.push_back(table.size(1));
 		ctx->saved_data["settings"] = std::move(s);
 		return out;
@@ -829,6 +830,8 @@ Tensor apply_cross(const cross_call& c) {
 		if(auto* node = dynamic_cast<torch::autograd::CppNode<position_function>*>(c.bias.grad_fn().get())) {
 			try {
 				positions = node->ctx_.get_saved_variables(), table = node->ctx_.saved_data["table"].toTensor(), settings = node->ctx_.saved_data["settings"].toIntVector();
+				// (a table changed since: what led to the bias is not what its gradient goes to any more)
+				if((int64_t)table->_version() != node->ctx_.saved_data["version"].toInt()) table.reset();
 			} catch(const c10::Error&) {   // (that graph was freed: a backward pass through the bias will say so)
 				table.reset();
 			}

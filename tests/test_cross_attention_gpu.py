@@ -781,6 +781,22 @@ def test_a_table_may_change_before_its_gradient_is_taken(af3):
 
 
 @pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_a_table_changed_in_place_behind_its_bias(af3, monkeypatch, native):
+    """The bias's gradient goes to what the table was, not to what it became: the same bits as with a table of its own for each."""
+    from af3_kernels_amd import cross
+    if not native:
+        monkeypatch.setattr(cross, "_host", _NoNativeHost())
+    q, k, v, _, _, g = make(2, 2, 2, 60, 60, 32, BF16, 84)
+    w = torch.randn(32, 2, dtype=BF16).cuda().requires_grad_(True)
+    table = w * 1
+    bias = af3.relative_position_bias(table, 60, 60)
+    table.mul_(1000)
+    got = torch.autograd.grad(af3.cross_attention(q, k, v, None, bias), w, g)[0]
+    want = torch.autograd.grad(af3.cross_attention(q, k, v, None, af3.relative_position_bias(w, 60, 60) * 1), w, g)[0]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
 def test_a_capture_that_would_wait_for_another_stream_is_refused(af3, monkeypatch, native):
     """The leaf's gradient is accumulated on the default stream while an eager result holds the leaf: captured, that would end the process."""
     from af3_kernels_amd import cross
