@@ -7,6 +7,9 @@ Public names, argument order and defaults follow the reference's Python module
 and `self_attention_cpp` (:83-105), with `GridSelfAttentionCpp` (src/af3_kernels/Attention.py:23-82).  Behind them a torch custom op hands raw device pointers to
 libaf3_dpa.so (hand-written HIP for gfx950) through the C ABI of include/af3_dpa.h.
 
+Beside these, without a counterpart in the reference: `cross_attention`, queries to keys of another length with key heads that query heads may share, and
+`relative_position_bias`, the learned bias by buckets of distance that it takes; both with gradients.
+
 Inputs must live on a ROCm device; CPU tensors raise.  The attention core (`dot_product_attention_cpp`, the fp8 variant,
 the casts, pad and repack helpers) runs in the HIP library or not at all: there is no CPU path and no PyTorch fallback, and
 a missing library raises at first use.  The callers around the core compose it with library matrix products where a plain
