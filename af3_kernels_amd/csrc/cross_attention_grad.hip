@@ -495,18 +495,20 @@ __global__ void __launch_bounds__(THREADS) cross_sum_kernel(parts a) {
 
 // ---- dbias ----
 // A workgroup has 64 query rows x 64 keys (a wavefront 32 x 32 of them) and goes through the batch; q, dO, k and v come as tiles.  Few sums to hold leave room for
-// many wavefronts: 128 keys with K and V as operands straight from memory took 57 us at 8 x 12 x 512 x 512 x 64, where the loads of every batch row stood alone.
+// many wavefronts: 128 keys with K and V as operands straight from memory took 57 us at 8 x 12 x 512 x 512 x 64, where the loads of every batch row stood alone.  Nor are
+// tiles fetched ahead of their use: the registers they would wait in cost the third workgroup of a compute unit, which hides more (ahead, two workgroups: 44.5 us there and
+// 76 at 4 x 16 x 768 x 768 x 64; so, three: 29.8 and 49; ahead and three, with spills: 74).  fp32 stays at what it needs without spills.
 template <typename T, int DP>
 struct dbias_shape {
 	static constexpr int QT = 64, KT = 64, TILE = 64 * tile<T, DP>::STRIDE, STATS = ROW_STATS * QT * 4 + 16, LDS = 4 * TILE + STATS;
-	static constexpr int REGISTERS = 48 + 16 * passage<T, DP, 64>::N;
+	static constexpr int REGISTERS = (sizeof(T) == 2 ? 32 : 48) + 16 * passage<T, DP, 64>::N;
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGISTERS)) cross_dbias_kernel(grad_args a) {
 	using S  = dbias_shape<T, DP>;
 	using TL = tile<T, DP>;
-	constexpr int QT = S::QT, KT = S::KT;
+	constexpr int QT = S::QT, KT = S::KT, E = kind<T>::E;
 	const af3_cross_attention_params& p = a.p;
 	extern __shared__ __align__(16) unsigned char smem[];
 	unsigned char *const qs = smem, *const gs = qs + S::TILE, *const ks = gs + S::TILE, *const vs = ks + S::TILE;
@@ -523,13 +525,20 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 	const int64_t  key = k0 + col0 + tile_row(lane & 31);
 	const bool     in = key < p.Lk;
 
-	float sum[16], bs[16];
+	float sum[16];
+	u32x4 bs[16 / E];
+	{
+		T entry[16];
 #pragma unroll
-	for(int r = 0; r < 16; r++) {
-		const int64_t q = q0 + row0 + 16 * half + r;
-		sum[r] = 0.f, bs[r] = 0.f;
-		if(in && q < p.Lq) bs[r] = kind<T>::value(static_cast<const T*>(p.bias)[h * p.bias_stride[0] + q * p.bias_stride[1] + key]);
+		for(int r = 0; r < 16; r++) {
+			const int64_t q = q0 + row0 + 16 * half + r;
+			sum[r] = 0.f, entry[r] = T(0);
+			if(in && q < p.Lq) entry[r] = static_cast<const T*>(p.bias)[h * p.bias_stride[0] + q * p.bias_stride[1] + key];
+		}
+#pragma unroll
+		for(int i = 0; i < 16 / E; i++) __builtin_memcpy(&bs[i], entry + E * i, 16);
 	}
+	auto logit = [&](float qk, int r) { return __builtin_fmaf(qk, p.softmax_scale, kind<T>::at(bs[r / E], r % E)); };
 	const typename TL::reader at(lane);
 	passage<T, DP, 64> pq, pg, pk, pv;
 	pq.begin(nullptr, p.q_stride[2], D, a.whole);
@@ -548,10 +557,13 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 		pv.load(k0, p.Lk);
 		rs.load(a, b * p.H + h, q0, a.more);
 	};
-	fetch(0);
 	const int64_t rows_left = p.Lq - q0, keys_left = p.Lk - k0;
-	for(int64_t b = 0; b < p.B; b++) {
+	// Workgroups begin with different batch rows: beginning alike, all of them waited for each row's way from memory, a row after the other.
+	int64_t b = own.piece % p.B;
+	for(int64_t left = p.B; left > 0; left--) {
+		fetch(b);
 		const bool lives = in && (!p.key_mask || p.key_mask[b * p.key_mask_stride_b + key] != 0);
+		b = b + 1 < p.B ? b + 1 : 0;   // (the next one)
 		__syncthreads();   // (nobody reads the batch row before any more)
 		pq.store(qs, rows_left >= 64, [&](int r) { return r < rows_left; });
 		pg.store(gs, rows_left >= 64, [&](int r) { return r < rows_left; });
@@ -559,7 +571,6 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 		pv.store(vs, keys_left >= 64, [&](int r) { return r < keys_left; });
 		rs.store(st, a.factor);
 		__syncthreads();
-		if(b + 1 < p.B) fetch(b + 1);
 		if(st[2 * QT] == -INFINITY || !__any(lives)) continue;   // (-inf: a batch row without a live key)
 		const float* const sm = st + row0 + 16 * half;
 		f32x16 acc{}, dp = rs.sixteen(sm + QT);
@@ -571,11 +582,11 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dbias_shape<T, DP>::REGIST
 		if(rs.apart(st)) {
 			const f32x16 m = rs.sixteen(sm + 2 * QT), inv = rs.sixteen(sm + 3 * QT);
 #pragma unroll
-			for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f((__builtin_fmaf(acc[r], p.softmax_scale, bs[r]) - m[r]) * a.factor) * inv[r];
+			for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f((logit(acc[r], r) - m[r]) * a.factor) * inv[r];
 		} else {
 			const f32x16 taken = rs.sixteen(sm);
 #pragma unroll
-			for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_fmaf(acc[r], p.softmax_scale, bs[r]), a.factor, -taken[r]));
+			for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(logit(acc[r], r), a.factor, -taken[r]));
 		}
 #pragma unroll
 		for(int r = 0; r < 16; r++) sum[r] += lives ? x[r] * dp[r] : 0.f;   // (what k, v and bias hold at a dropped key stays in its own lane)
