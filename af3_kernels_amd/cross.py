@@ -90,38 +90,21 @@ def _backward(grad, q, k, v, keep, bias, out, stats, lost, scale, wants):
 
 
 class _CrossAttention(torch.autograd.Function):
-    """A bfloat16 bias straight out of relative_position_bias hands its table on (`table`, with that call's positions and settings): its gradient reaches the table
-    as bfloat16, and what that rounding and the one of its sums lose reaches the table directly."""
-
     @staticmethod
-    def forward(ctx, q, k, v, keep, bias, scale, table, settings, q_positions, k_positions):
+    def forward(ctx, q, k, v, keep, bias, scale):
         out, stats, lost = _forward(q, k, v, keep, bias, scale, True)
-        ctx.save_for_backward(q, k, v, keep, bias, out, stats, lost, q_positions, k_positions)
-        ctx.scale, ctx.settings, ctx.table_shape = scale, settings, None if table is None else table.shape
+        ctx.save_for_backward(q, k, v, keep, bias, out, stats, lost)
+        ctx.scale = scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, keep, bias, out, stats, lost, q_positions, k_positions = ctx.saved_tensors
+        q, k, v, keep, bias, out, stats, lost = ctx.saved_tensors
         needs = ctx.needs_input_grad
-        residual = needs[4] and needs[6] and stats is not None
-        dq, dk, dv, dbias, bias_lost = _backward(grad, q, k, v, keep, bias, out, stats, lost, ctx.scale, (needs[0], needs[1], needs[2], needs[4], residual))
-        dtable = _position_sums(dbias, bias_lost, ctx.table_shape, ctx.settings, q_positions, k_positions) if residual else None
-        return dq, dk, dv, None, dbias, None, dtable, None, None, None
-
-
-def _source(bias):
-    """(table, settings, q_positions, k_positions) of a bfloat16 bias that is relative_position_bias's result as it stands."""
-    node = bias.grad_fn if bias is not None and bias.dtype == torch.bfloat16 and bias.requires_grad and bias.shape[0] < 1 << 15 else None
-    if isinstance(node, _PositionBias._backward_cls):
-        try:
-            q_positions, k_positions = node.saved_tensors
-        except RuntimeError:   # (that graph was freed: a backward pass through the bias will say so)
-            return None, None, None, None
-        if node.table._version == node.version:   # (changed since: what led to the bias is not what its gradient goes to any more)
-            return node.table, node.settings, q_positions, k_positions
-    return None, None, None, None
+        # (what the bias's gradient loses by its rounding is not asked for: the native host side knows whether it may be handed on to a table, this side does not)
+        dq, dk, dv, dbias, _ = _backward(grad, q, k, v, keep, bias, out, stats, lost, ctx.scale, (needs[0], needs[1], needs[2], needs[4], False))
+        return dq, dk, dv, None, dbias, None
 
 
 def _check_cross(q, k, v, keep, bias):
@@ -179,7 +162,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
         raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         _host.check_capture(q, k, v, bias)
-        return _CrossAttention.apply(q, k, v, keep, bias, scale, *_source(bias))
+        return _CrossAttention.apply(q, k, v, keep, bias, scale)
     return _forward(q, k, v, keep, bias, scale, False)[0]
 
 
@@ -233,14 +216,14 @@ class _PositionBias(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, q_len, k_len, settings, q_positions, k_positions):
         ctx.save_for_backward(q_positions, k_positions)
-        ctx.table, ctx.version, ctx.settings = table, table._version, settings   # (not a saved tensor: the gradient does not need its values, which may change)
+        ctx.table_shape, ctx.settings = table.shape, settings
         return _position_forward(table, q_len, k_len, settings, q_positions, k_positions)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         q_positions, k_positions = ctx.saved_tensors
-        return _position_sums(grad, None, ctx.table.shape, ctx.settings, q_positions, k_positions), None, None, None, None, None
+        return _position_sums(grad, None, ctx.table_shape, ctx.settings, q_positions, k_positions), None, None, None, None, None
 
 
 def _check_settings(buckets, scheme, bidirectional, max_distance, q_offset):
@@ -286,7 +269,9 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, scheme: 
 
     Positions are 0, 1, 2, ... for keys and q_offset, q_offset + 1, ... for queries (a decoder's token t: q_len=1, q_offset=t), or what q_positions [q_len]
     and k_positions [k_len] hold (int64 or int32, on the table's device; q_offset then does not count for queries).
-    The gradient flows to the table: sums by bucket in a fixed order."""
+    The gradient flows to the table: the sums by bucket, in a fixed order, of the gradient that arrives at the bias.  That of a bfloat16 bias has been rounded to bfloat16 by
+    then, which a sum of such terms feels; a bias that one cross_attention call and nothing else has, with no hook on the way of its gradient, has its table's gradient from
+    what there was before that rounding instead (not in calls prepared in Python, nor if the table was changed in place in between, nor for a gradient with a graph)."""
     out = _host.position_bias(table, q_len, k_len, _lib.POSITION_SCHEMES.get(scheme, -1), bidirectional, max_distance, q_positions, k_positions, q_offset)
     if out is not None:
         return out if out.__class__ is not int else _lib.check(out, "af3_position_bias_forward")

@@ -7,7 +7,9 @@
 #include <Python.h>
 
 #include <array>
+#include <atomic>
 #include <cmath>
+#include <map>
 #include <mutex>
 #include <unordered_map>
 #include <unordered_set>
@@ -25,6 +27,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/af3_dpa.h"
@@ -690,6 +693,34 @@ struct position_call {
 		return af3_position_bias_forward(&p, current_stream(dev));
 	}
 };
+// What a bfloat16 gradient of a bias lost by its rounding, on its way from the one attention call that has the bias to the bias's node: that call leaves it here
+// in a backward pass, and the node takes it if the gradient that arrives is the very tensor the call made (a bias that something else has too, or whose gradient a
+// hook may have changed, has its table's gradient from the gradient that arrives alone).
+struct handed_on : torch::CustomClassHolder {
+	struct share {
+		Tensor  grad, lost;
+		int64_t version;
+	};
+	static constexpr size_t MOST = 8;   // passes through one graph at a time; what a pass that failed left behind goes with newer ones
+	Tensor               table;         // an alias of its values: tells whether they were changed in place
+	int64_t              version;
+	std::atomic<int64_t> calls{0};      // attention calls that have the bias
+	std::mutex           lock;
+	std::map<int, share> passes;        // by the pass they belong to
+	void put(int pass, share s) {
+		const std::lock_guard<std::mutex> hold(lock);
+		passes[pass] = std::move(s);
+		if(passes.size() > MOST) passes.erase(passes.begin());
+	}
+	Tensor take(int pass, const Tensor& grad) {
+		const std::lock_guard<std::mutex> hold(lock);
+		const auto it = passes.find(pass);
+		if(it == passes.end()) return Tensor();
+		const share s = std::move(it->second);
+		passes.erase(it);
+		return s.grad.is_same(grad) && (int64_t)grad._version() == s.version ? s.lost : Tensor();
+	}
+};
 struct position_function : torch::autograd::Function<position_function> {
 	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& table, const std::optional<Tensor>& given_q, const std::optional<Tensor>& given_k,
 					  std::vector<int64_t> s) {
@@ -697,12 +728,17 @@ struct position_function : torch::autograd::Function<position_function> {
 		Tensor       out;
 		raise(position_call{table, q_positions, k_positions, s[0], s[1], s[2], s[3], s[4], s[5]}.forward(out), "af3_position_bias_forward");
 		ctx->save_for_backward({q_positions, k_positions});
-		ctx->saved_data["table"] = table;   // (for apply_cross; not a saved variable: the gradient does not need its values, which may change)
-		ctx->saved_data["version"] = (int64_t)table._version();
+		auto handed     = c10::make_intrusive<handed_on>();
+		handed->table   = table.detach();
+		handed->version = (int64_t)table._version();
+		ctx->saved_data["handed"] = at::IValue::make_capsule(std::move(handed));
 		s.push_back(table.size(0)), s.push_back(table.size(1));
 		ctx->saved_data["settings"] = std::move(s);
 		return out;
 	}
+	static c10::intrusive_ptr<handed_on> handed(torch::autograd::AutogradContext& ctx) { return c10::static_intrusive_pointer_cast<handed_on>(ctx.saved_data["handed"].toCapsule()); }
+	// the node that made a tensor, if it is one of these
+	static torch::autograd::CppNode<position_function>* node(const std::shared_ptr<torch::autograd::Node>& of) { return dynamic_cast<torch::autograd::CppNode<position_function>*>(of.get()); }
 	// the table's gradient [buckets, H] of a gradient g of the bias; with what g's rounding lost (laid out like g): what that misses
 	static Tensor sums(Tensor g, const Tensor& lost, const Tensor& q_positions, const Tensor& k_positions, const std::vector<int64_t>& s) {
 		const int dev = (int)g.get_device();
@@ -723,8 +759,15 @@ struct position_function : torch::autograd::Function<position_function> {
 		torch::autograd::variable_list grads(4);
 		{
 			at::AutoGradMode none(false);
-			const auto saved = ctx->get_saved_variables();
-			grads[0] = sums(grad_out[0], Tensor(), saved[0], saved[1], ctx->saved_data["settings"].toIntVector());
+			const auto   saved = ctx->get_saved_variables();
+			const auto   settings = ctx->saved_data["settings"].toIntVector();
+			const Tensor lost = handed(*ctx)->take(torch::autograd::get_current_graph_task_id(), grad_out[0]);
+			grads[0] = sums(grad_out[0], Tensor(), saved[0], saved[1], settings);
+			if(lost.defined()) {
+				// (lost belongs to the attention call's stream, which need not be this one)
+				c10::hip::HIPCachingAllocator::recordStream(lost.storage().data_ptr(), c10::hip::getCurrentHIPStream((c10::DeviceIndex)lost.get_device()));
+				grads[0].add_(sums(grad_out[0], lost, saved[0], saved[1], settings));
+			}
 		}
 		return once(std::move(grads), "relative_position_bias");
 	}
@@ -761,32 +804,39 @@ struct cross_call {
 		return af3_cross_attention_forward(&p, current_stream(dev));
 	}
 };
-// A bfloat16 bias that comes straight out of relative_position_bias hands its table on as an input (`table`, with that call's positions and settings): the
-// bias's gradient takes its usual way to the table, rounded to bfloat16 as a gradient of a bfloat16 tensor has to be, and what that rounding and the one of its
-// sums lose goes to the table directly.  The sum of the two is the table's gradient, rounded once; what a caller does with the bias's gradient on the
-// way is none of the second part's business (2^-8 of the first).
+// The gradient of a bfloat16 bias is rounded to bfloat16, as that of a bfloat16 tensor has to be.  Where the bias came straight out of relative_position_bias and nothing
+// else has it, what the rounding lost is handed on to its node, and the table's gradient is rounded once.
 struct cross_function : torch::autograd::Function<cross_function> {
-	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& given_bias, const std::optional<Tensor>& table,
-					  const std::optional<Tensor>& given_mask, double scale, torch::autograd::variable_list positions, std::vector<int64_t> settings) {
+	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& given_bias,
+					  const std::optional<Tensor>& given_mask, double scale, bool hands_on) {
 		const Tensor bias = given_bias.value_or(Tensor()), mask = given_mask.value_or(Tensor());
 		Tensor       out, stats, lost;
 		raise(cross_call{q, k, v, mask, bias, scale}.forward(out, &stats, &lost), "af3_cross_attention_forward");
-		torch::autograd::variable_list saved{q, k, v, bias, mask, out, stats, lost};
-		if(table) {
-			saved.insert(saved.end(), positions.begin(), positions.end());
-			ctx->saved_data["settings"] = std::move(settings);
-		}
-		ctx->save_for_backward(std::move(saved));
-		ctx->saved_data["scale"] = scale;
+		ctx->save_for_backward({q, k, v, bias, mask, out, stats, lost});
+		ctx->saved_data["scale"] = scale, ctx->saved_data["hands_on"] = hands_on;
 		return out;
+	}
+	// where what the bias's gradient loses goes in this pass: to the bias's node, if that will run and nobody gets to see the gradient on its way
+	static c10::intrusive_ptr<handed_on> receiver(bool hands_on) {
+		if(!hands_on || at::GradMode::is_enabled()) return {};   // (a graph of the gradient is wanted: it must hold for the gradient as it stands)
+		const auto self = torch::autograd::get_current_node();
+		auto* const to  = self ? position_function::node(self->next_edge(3).function) : nullptr;
+		if(!to || !self->post_hooks().empty() || !to->pre_hooks().empty() || !to->tensor_pre_hooks().empty()) return {};
+		if(const auto* const info = torch::autograd::get_current_graph_task_exec_info(); info && !info->empty()) {
+			const auto it = info->find(to);
+			if(it == info->end() || !it->second.needed_) return {};
+		}
+		const auto handed = position_function::handed(to->ctx_);
+		return handed->calls == 1 ? handed : c10::intrusive_ptr<handed_on>();
 	}
 	static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_out) {
 		const auto saved = ctx->get_saved_variables();
 		const cross_call call{saved[0], saved[1], saved[2], saved[4], saved[3], ctx->saved_data["scale"].toDouble()};
 		const int        dev = (int)call.q.get_device();
 		Tensor           g = grad_out[0];
-		torch::autograd::variable_list grads(9);
+		torch::autograd::variable_list grads(7);
 		Tensor           bias_lost;
+		const auto       handed = receiver(ctx->saved_data["hands_on"].toBool());
 		{
 			at::AutoGradMode none(false);
 			if(!inner_1(g)) g = g.contiguous();
@@ -804,13 +854,13 @@ struct cross_function : torch::autograd::Function<cross_function> {
 			};
 			o.grad_q = want(0, call.q.sizes()), o.grad_k = want(1, call.k.sizes()), o.grad_v = want(2, call.v.sizes());
 			if(call.bias.defined()) o.grad_bias = want(3, call.bias.sizes());
-			if(o.grad_bias && saved.size() > 8 && ctx->needs_input_grad(4)) bias_lost = new_tensor(call.bias.sizes(), call.q.scalar_type(), dev), o.grad_bias_residual = bias_lost.data_ptr();
+			if(o.grad_bias && handed) bias_lost = new_tensor(call.bias.sizes(), call.q.scalar_type(), dev), o.grad_bias_residual = bias_lost.data_ptr();
 			const int64_t     bytes = af3_cross_attention_backward_workspace_bytes(&p);
 			raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_cross_attention_backward_workspace_bytes");
 			const at::DataPtr ws = new_scratch(bytes);
 			o.workspace = ws.get(), o.workspace_bytes = bytes;
 			raise(af3_cross_attention_backward(&p, &o, current_stream(dev)), "af3_cross_attention_backward");
-			if(bias_lost.defined()) grads[4] = position_function::sums(grads[3], bias_lost, saved[8], saved[9], ctx->saved_data["settings"].toIntVector());
+			if(bias_lost.defined()) handed->put(torch::autograd::get_current_graph_task_id(), {grads[3], bias_lost, (int64_t)grads[3]._version()});
 		}
 		return once(std::move(grads), "cross_attention");
 	}
@@ -823,20 +873,14 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
 	return false;
 }
 Tensor apply_cross(const cross_call& c) {
-	std::optional<Tensor>          table;
-	torch::autograd::variable_list positions;
-	std::vector<int64_t>           settings;
-	if(c.bias.defined() && c.bias.scalar_type() == at::kBFloat16 && c.bias.requires_grad() && c.q.size(1) <= 0x7fff)
-		if(auto* node = dynamic_cast<torch::autograd::CppNode<position_function>*>(c.bias.grad_fn().get())) {
-			try {
-				positions = node->ctx_.get_saved_variables(), table = node->ctx_.saved_data["table"].toTensor(), settings = node->ctx_.saved_data["settings"].toIntVector();
-				// (a table changed since: what led to the bias is not what its gradient goes to any more)
-				if((int64_t)table->_version() != node->ctx_.saved_data["version"].toInt()) table.reset();
-			} catch(const c10::Error&) {   // (that graph was freed: a backward pass through the bias will say so)
-				table.reset();
-			}
+	bool hands_on = false;
+	if(c.bias.defined() && c.bias.scalar_type() == at::kBFloat16 && c.bias.requires_grad() && c.q.size(1) <= 0x7fff)   // (heads: as many as the sums take with a residual)
+		if(auto* const node = position_function::node(c.bias.grad_fn())) {
+			const auto handed = position_function::handed(node->ctx_);
+			handed->calls++;
+			hands_on = (int64_t)handed->table._version() == handed->version;   // (a table changed in place since: the bias's gradient alone)
 		}
-	return cross_function::apply(c.q, c.k, c.v, given(c.bias), table, given(c.mask), c.scale, positions, settings);
+	return cross_function::apply(c.q, c.k, c.v, given(c.bias), given(c.mask), c.scale, hands_on);
 }
 // cross_attention(q, k, v, mask, bias, scale or None)
 PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {

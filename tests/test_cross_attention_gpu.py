@@ -825,3 +825,154 @@ def test_a_capture_that_would_wait_for_another_stream_is_refused(af3, monkeypatc
     torch.cuda.synchronize()
     assert torch.equal(plain, eager[0])
     del eager
+
+
+# ---- the table's gradient behind bf16 attention: rounded once where the bias's gradient arrives as the call made it ----------------------
+def _table_case(seed, B=3, H=4, L=90, D=32):
+    q, k, v, m, _, g = make(B, H, H, L, L, D, BF16, seed, "ragged", "none")
+    gen = torch.Generator().manual_seed(seed + 1)
+    return q, k, v, m, g, torch.randn(32, H, generator=gen).to(BF16).cuda().requires_grad_(True)
+
+
+def _plain_sums(af3, table, grad):
+    """The sums by bucket of a bias's gradient as it stands, in bfloat16."""
+    bias = af3.relative_position_bias(table, *grad.shape[1:])
+    return torch.autograd.grad(bias, table, grad)[0]
+
+
+def test_a_tables_gradient_with_one_attention_call_is_rounded_once(af3):
+    """own + missed: the sums of the bias's gradient, and what they and that gradient lost.  In every way of asking for it."""
+    from af3_kernels_amd import cross
+    q, k, v, m, g, table = _table_case(91)
+    bias = af3.relative_position_bias(table, 90, 90)
+    out = af3.cross_attention(q, k, v, m, bias)
+    keep, scale = m.view(torch.uint8), 32 ** -0.5
+    kernel = cross._forward(q, k, v, keep, bias.detach(), scale, True)
+    grads = cross._backward(g, q, k, v, keep, bias.detach(), *kernel, scale, (False, False, False, True, True))
+    settings = ("log", True, 128, 0)
+    own, missed = (cross._position_sums(grads[3], x, table.shape, settings, None, None) for x in (None, grads[4]))
+    want = own + missed
+    assert not torch.equal(own, want)
+    once = torch.autograd.grad(out, table, g, retain_graph=True)[0]
+    assert torch.equal(once, want) and torch.equal(torch.autograd.grad(out, table, g, retain_graph=True)[0], want)
+    both = torch.autograd.grad(out, (bias, table), g, retain_graph=True)
+    assert torch.equal(both[0], grads[3]) and torch.equal(both[1], want)
+    # the bias's gradient alone, and then the table's from it: a gradient like any other
+    dbias = torch.autograd.grad(out, bias, g, retain_graph=True)[0]
+    assert torch.equal(dbias, grads[3]) and torch.equal(torch.autograd.grad(bias, table, dbias, retain_graph=True)[0], own)
+    bias.retain_grad()
+    out.backward(g, retain_graph=True)
+    assert torch.equal(bias.grad, grads[3]) and torch.equal(table.grad, want)
+    # a gradient that has a graph is made of the one that arrives
+    graph = torch.autograd.grad(out, table, g, create_graph=True)[0]
+    assert torch.equal(graph, own)
+
+
+@pytest.mark.parametrize("where", ["tensor", "node", "attention"])
+@pytest.mark.parametrize("change", ["zeros", "in place", "behind torch's back", "one head", "half", "none"])
+def test_a_hook_on_the_biass_gradient_has_the_last_word(af3, where, change):
+    q, k, v, m, g, table = _table_case(92)
+    bias = af3.relative_position_bias(table, 90, 90)
+    out = af3.cross_attention(q, k, v, m, bias)
+    dbias = torch.autograd.grad(out, bias, g, retain_graph=True)[0].clone()
+
+    def changed(t):
+        if change == "zeros":
+            return torch.zeros_like(t)
+        if change == "in place":
+            t.zero_()
+            return None
+        if change == "behind torch's back":      # no version counter sees this
+            t.data.zero_()
+            return None
+        if change == "one head":
+            return torch.cat([torch.zeros_like(t[:1]), t[1:]])
+        return t * 0.5 if change == "half" else None
+
+    arrives = dbias.clone()
+    replaced = changed(arrives)
+    arrives = arrives if replaced is None else replaced
+    if where == "tensor":
+        bias.register_hook(changed)
+    elif where == "node":
+        def before(grads):
+            new = changed(grads[0])
+            return None if new is None else (new,)
+        bias.grad_fn.register_prehook(before)
+    else:
+        def after(grads, _):
+            new = changed(grads[3])
+            return None if new is None else (*grads[:3], new, *grads[4:])
+        out.grad_fn.register_hook(after)
+    got = torch.autograd.grad(out, table, g)[0]
+    assert torch.equal(got, _plain_sums(af3, table, arrives))
+    if change in ("zeros", "in place", "behind torch's back"):
+        assert not got.any()
+    if change == "one head":
+        assert not got[:, 0].any() and got[:, 1:].any()
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+@pytest.mark.parametrize("layers", [2, 3, 12])
+def test_a_bias_that_a_stack_of_layers_shares(af3, monkeypatch, layers, native):
+    """The bias's gradients are added in bf16 before the table sees them: its gradient is the sums of what arrives, to the bit."""
+    from af3_kernels_amd import cross
+    if not native:
+        monkeypatch.setattr(cross, "_host", _NoNativeHost())
+    q, k, v, m, g, table = _table_case(93)
+
+    def stack(bias):
+        x = q
+        for _ in range(layers):
+            x = af3.cross_attention(x, k, v, m, bias)
+        return x
+    bias = af3.relative_position_bias(table, 90, 90)
+    got = torch.autograd.grad(stack(bias), (bias, table), g)
+    plain = af3.relative_position_bias(table, 90, 90)
+    want = torch.autograd.grad(stack(plain * 1), (plain, table), g)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(got[1], _plain_sums(af3, table, got[0]))
+
+
+def test_a_bias_that_something_else_has_too(af3):
+    q, k, v, m, g, table = _table_case(94)
+    w = torch.randn(4, 90, 90, device="cuda", dtype=BF16)
+    for order in (0, 1):
+        bias = af3.relative_position_bias(table, 90, 90)
+        parts = [lambda: (af3.cross_attention(q, k, v, m, bias).float() * g.float()).sum(), lambda: (bias * w).float().sum()]
+        loss = parts[order]() + parts[1 - order]()
+        dbias, got = torch.autograd.grad(loss, (bias, table))
+        assert torch.equal(got, _plain_sums(af3, table, dbias))
+
+
+def test_a_bias_of_another_stream(af3):
+    """The bias is made on one stream, the attention runs on another: the same bits, also where memory is handed round at once."""
+    q, k, v, m, g, table = _table_case(95)
+    want = torch.autograd.grad(af3.cross_attention(q, k, v, m, af3.relative_position_bias(table, 90, 90)), table, g)[0]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        bias = af3.relative_position_bias(table, 90, 90)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out = af3.cross_attention(q, k, v, m, bias)
+            got = torch.autograd.grad(out, table, g)[0]
+            torch.full_like(bias, 1e4), torch.full_like(bias, -1e4)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+
+
+def test_a_table_that_is_changed_by_what_its_bias_led_to_is_freed(af3):
+    """Nothing in the bias's graph holds the table's own: in place, that would be a circle."""
+    import weakref
+    w = torch.randn(32, 2, device="cuda", dtype=BF16).requires_grad_(True)
+    table = w * 1
+    bias = af3.relative_position_bias(table, 40, 40)
+    table.add_(bias.float().mean().to(BF16))
+    gone = weakref.ref(table)
+    node = table.grad_fn
+    seen = []
+    node.metadata["witness"] = type("witness", (), {"__del__": lambda self: seen.append(1)})()
+    del table, bias, node
+    gc.collect()
+    assert gone() is None and seen == [1]
