@@ -160,6 +160,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
     scale = float(q.shape[3]) ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
+    with ops._on_device(q.device):   # (the call as a plain one: what it gives, gradients too, is not a question of how it came)
+        out = _host.cross_attention(q, k, v, None if keep is None else keep.view(torch.bool), bias, scale)
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_cross_attention_forward")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         _host.check_capture(q, k, v, bias)
         return _CrossAttention.apply(q, k, v, keep, bias, scale)
@@ -271,7 +275,7 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, scheme: 
     and k_positions [k_len] hold (int64 or int32, on the table's device; q_offset then does not count for queries).
     The gradient flows to the table: the sums by bucket, in a fixed order, of the gradient that arrives at the bias.  That of a bfloat16 bias has been rounded to bfloat16 by
     then, which a sum of such terms feels; a bias that one cross_attention call and nothing else has, with no hook on the way of its gradient, has its table's gradient from
-    what there was before that rounding instead (not in calls prepared in Python, nor if the table was changed in place in between, nor for a gradient with a graph)."""
+    what there was before that rounding instead (not without the native host module, nor if the table was changed in place in between, nor for a gradient with a graph)."""
     out = _host.position_bias(table, q_len, k_len, _lib.POSITION_SCHEMES.get(scheme, -1), bidirectional, max_distance, q_positions, k_positions, q_offset)
     if out is not None:
         return out if out.__class__ is not int else _lib.check(out, "af3_position_bias_forward")
@@ -286,6 +290,10 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, scheme: 
     _check_settings(table.shape[0], scheme, bidirectional, max_distance, q_offset)
     q_positions, k_positions = _positions_of(q_positions, q_len, "q_positions"), _positions_of(k_positions, k_len, "k_positions")
     settings = (scheme, bool(bidirectional), max_distance, q_offset)
+    with ops._on_device(table.device):   # (as a plain call)
+        out = _host.position_bias(table, q_len, k_len, _lib.POSITION_SCHEMES[scheme], settings[1], max_distance, q_positions, k_positions, q_offset)
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_position_bias_forward")
     if torch.is_grad_enabled() and table.requires_grad:
         _host.check_capture(table)
         return _PositionBias.apply(table, q_len, k_len, settings, q_positions, k_positions)

@@ -976,3 +976,28 @@ def test_a_table_that_is_changed_by_what_its_bias_led_to_is_freed(af3):
     del table, bias, node
     gc.collect()
     assert gone() is None and seen == [1]
+
+
+def test_a_tables_gradient_does_not_depend_on_how_its_calls_come(af3):
+    """int32 positions, lengths of another integer type, masks of numbers, other types of k and v, other strides: each call is prepared in Python first and
+    gives the bits that the plain ones give together, whichever of the two it is."""
+    import numpy
+    q, k, v, m, g, table = _table_case(96)
+    at = torch.arange(90, device="cuda")
+    plain = (lambda: af3.relative_position_bias(table, 90, 90, q_positions=at, k_positions=at), lambda b: af3.cross_attention(q, k, v, m, b))
+
+    def gradient(bias, attend):
+        return torch.autograd.grad(attend(bias()), table, g)[0]
+    want = gradient(*plain)
+    assert not torch.equal(want, gradient(plain[0], lambda b: plain[1](b * 1)))
+    biases = {"int32 positions": lambda: af3.relative_position_bias(table, 90, 90, q_positions=at.int(), k_positions=at.int()),
+              "numpy lengths": lambda: af3.relative_position_bias(table, numpy.int64(90), numpy.int64(90), q_positions=at, k_positions=at)}
+    odd = q.transpose(2, 3).contiguous().transpose(2, 3)
+    attends = {"a mask of numbers": lambda b: af3.cross_attention(q, k, v, m.int(), b), "a mask of rank 4": lambda b: af3.cross_attention(q, k, v, m.float()[:, None, None, :], b),
+               "keys in fp32": lambda b: af3.cross_attention(q, k.float(), v, m, b), "other strides": lambda b: af3.cross_attention(odd, k, v, m, b),
+               "a scale of numpy's": lambda b: af3.cross_attention(q, k, v, m, b, softmax_scale=numpy.float64(32 ** -0.5))}
+    for name, bias in biases.items():
+        assert torch.equal(gradient(bias, plain[1]), want), name
+    for name, attend in attends.items():
+        assert torch.equal(gradient(plain[0], attend), want), name
+    assert torch.equal(gradient(biases["int32 positions"], attends["a mask of numbers"]), want)
