@@ -11,6 +11,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from ._lib import CrossAttentionGrads, CrossAttentionParams, PositionBiasParams
@@ -25,6 +26,13 @@ def _same_device(first, *others):
     for t in others:
         if t is not None and t.device != first.device:
             raise ValueError(f"all tensors must be on one device, got {first.device} and {t.device}")
+
+
+def _no_tangents(what, *tensors):
+    """Forward-mode differentiation is refused: the result would come without a tangent, as if it did not depend on these."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _inner_contig(t):
@@ -100,6 +108,7 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _no_tangents("the gradient of cross_attention", grad)
         q, k, v, keep, bias, out, stats, lost = ctx.saved_tensors
         needs = ctx.needs_input_grad
         # (what the bias's gradient loses by its rounding is not asked for: the native host side knows whether it may be handed on to a table, this side does not)
@@ -139,12 +148,13 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
     that query; a query left without a live key by that gives zeros and no gradient.  The lowest finite bias does as the formula
     says: a row of nothing else weights its live keys alike.  Lk == 0 gives zeros.
 
-    Gradients flow to q, k, v and bias (the same bits every time); not through a second derivative.  In a HIP graph: capture forward and backward
+    Gradients flow to q, k, v and bias (the same bits every time); a second derivative and forward mode raise.  In a HIP graph: capture forward and backward
     together, with leaves that no result of an earlier call on another stream still holds: their gradients would be accumulated on that stream, outside of
     the capture, so such a call raises RuntimeError."""
     out = _host.cross_attention(q, k, v, mask, bias, softmax_scale)
     if out is not None:
         return out if out.__class__ is not int else _lib.check(out, "af3_cross_attention_forward")
+    _no_tangents("cross_attention", q, k, v, bias)
     _same_device(q, k, v, mask, bias)
     if q.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {q.dtype}: float32 or bfloat16")
@@ -226,6 +236,7 @@ class _PositionBias(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _no_tangents("the gradient of relative_position_bias", grad)
         q_positions, k_positions = ctx.saved_tensors
         return _position_sums(grad, None, ctx.table_shape, ctx.settings, q_positions, k_positions), None, None, None, None, None
 
@@ -279,6 +290,7 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, scheme: 
     out = _host.position_bias(table, q_len, k_len, _lib.POSITION_SCHEMES.get(scheme, -1), bidirectional, max_distance, q_positions, k_positions, q_offset)
     if out is not None:
         return out if out.__class__ is not int else _lib.check(out, "af3_position_bias_forward")
+    _no_tangents("relative_position_bias", table)
     _same_device(table, q_positions, k_positions)
     if table.dim() != 2:
         raise ValueError(f"table must be [buckets, H], got {tuple(table.shape)}")

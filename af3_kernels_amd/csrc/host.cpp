@@ -671,6 +671,13 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads, const 
 	auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative", (int64_t)in.size());
 	return error->apply(std::move(in));
 }
+// Forward-mode differentiation would come out without a tangent: inputs that have one go to the Python side, which refuses them, and gradients that have one are refused.
+bool has_tangent(std::initializer_list<const Tensor*> tensors) {
+	for(const Tensor* t : tensors)
+		if(t && t->defined() && t->_fw_grad(0).defined()) return true;
+	return false;
+}
+void no_tangent(const Tensor& grad, const char* what) { TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent({&grad}), what, " has no forward-mode derivative"); }
 void raise(int rc, const char* what) { TORCH_CHECK(rc == AF3_OK, what, ": ", af3_status_string(rc), " (af3_status ", rc, ")"); }
 
 struct position_call {
@@ -757,6 +764,7 @@ struct position_function : torch::autograd::Function<position_function> {
 	}
 	static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_out) {
 		torch::autograd::variable_list grads(4);
+		no_tangent(grad_out[0], "the gradient of relative_position_bias");
 		{
 			at::AutoGradMode none(false);
 			const auto   saved = ctx->get_saved_variables();
@@ -834,6 +842,7 @@ struct cross_function : torch::autograd::Function<cross_function> {
 		const cross_call call{saved[0], saved[1], saved[2], saved[4], saved[3], ctx->saved_data["scale"].toDouble()};
 		const int        dev = (int)call.q.get_device();
 		Tensor           g = grad_out[0];
+		no_tangent(g, "the gradient of cross_attention");
 		torch::autograd::variable_list grads(7);
 		Tensor           bias_lost;
 		const auto       handed = receiver(ctx->saved_data["hands_on"].toBool());
@@ -910,7 +919,7 @@ PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 		PyErr_Clear();
 		return none();
 	}
-	if(!(c.scale > 0.0 && (float)c.scale > 0.f && (float)c.scale < INFINITY)) return none();
+	if(!(c.scale > 0.0 && (float)c.scale > 0.f && (float)c.scale < INFINITY) || has_tangent({q, k, v, &c.bias})) return none();
 	Tensor out;
 	int    rc = AF3_OK;
 	const bool graph = wants_grad({q, k, v, &c.bias});
@@ -936,7 +945,7 @@ PyObject* py_position_bias(PyObject*, PyObject* const* a, Py_ssize_t n) {
 	if(n != 9) return none();
 	const Tensor* table = tensor_of(a[0]);
 	const int     dev   = device_of(table);
-	if(dev < 0 || table->dim() != 2 || dtype_code(*table) < 0 || table->numel() == 0) return none();
+	if(dev < 0 || table->dim() != 2 || dtype_code(*table) < 0 || table->numel() == 0 || has_tangent({table})) return none();
 	int64_t number[5];   // q_len, k_len, scheme, max_distance, q_offset
 	const int at[5] = {1, 2, 3, 5, 8};
 	for(int i = 0; i < 5; i++) {

@@ -162,3 +162,18 @@ def test_a_stale_library_says_so_and_does_not_keep_the_package_from_being_import
     code = "import af3_kernels_amd as a\ntry:\n    a._lib.load()\nexcept ImportError as e:\n    print('said:', 'rebuild' in str(e))"
     r = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True)
     assert r.returncode == 0 and "said: True" in r.stdout, r.stdout + r.stderr
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost without a word: refused before anything else is looked at."""
+    import af3_kernels_amd as af3
+    from torch.autograd import forward_ad
+    plain = {"q": torch.randn(1, 2, 3, 8), "k": torch.randn(1, 2, 4, 8), "v": torch.randn(1, 2, 4, 8), "bias": torch.randn(2, 3, 4)}
+    with forward_ad.dual_level():
+        for name, t in plain.items():
+            args = plain | {name: forward_ad.make_dual(t, torch.ones_like(t))}
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                af3.cross_attention(**args)
+        table = torch.randn(32, 2)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            af3.relative_position_bias(forward_ad.make_dual(table, torch.ones_like(table)), 3, 4)

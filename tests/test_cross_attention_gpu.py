@@ -1001,3 +1001,36 @@ def test_a_tables_gradient_does_not_depend_on_how_its_calls_come(af3):
     for name, attend in attends.items():
         assert torch.equal(gradient(plain[0], attend), want), name
     assert torch.equal(gradient(biases["int32 positions"], attends["a mask of numbers"]), want)
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_no_forward_mode(af3, monkeypatch, native):
+    """A result without a tangent would say that it does not depend on the input; with and without a graph of its own."""
+    from torch.autograd import forward_ad
+    from af3_kernels_amd import cross
+    if not native:
+        monkeypatch.setattr(cross, "_host", _NoNativeHost())
+    q, k, v, m, b, _ = make(1, 2, 2, 10, 20, 16, F32, 97, "random", "given")
+    table = torch.randn(32, 2, device="cuda")
+    want = af3.cross_attention(q, k, v, m, b), af3.relative_position_bias(table, 4, 5)
+    for requires_grad in (False, True):
+        with forward_ad.dual_level():
+            for name, t in {"q": q, "k": k, "v": v, "bias": b}.items():
+                dual = forward_ad.make_dual(t.detach().requires_grad_(requires_grad), torch.ones_like(t))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    af3.cross_attention(**({"q": q, "k": k, "v": v, "mask": m, "bias": b} | {name: dual}))
+            dual = forward_ad.make_dual(table.detach().requires_grad_(requires_grad), torch.ones_like(table))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                af3.relative_position_bias(dual, 4, 5)
+            # (a call without tangents runs inside such a context as ever)
+            assert torch.equal(af3.cross_attention(q, k, v, m, b), want[0]) and torch.equal(af3.relative_position_bias(table, 4, 5), want[1])
+    leaf, leaf_table = q.detach().requires_grad_(True), table.detach().requires_grad_(True)
+    for out, x in ((af3.cross_attention(leaf, k, v, m, b), leaf), (af3.relative_position_bias(leaf_table, 4, 5), leaf_table)):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, x, dual)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: af3.cross_attention(x, k, v, m, b), (q,), (q,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: af3.cross_attention(x, k, v, m, b))(q[None])
