@@ -133,6 +133,16 @@ def _check_cross(q, k, v, keep, bias):
         raise ValueError(f"mask must be [Lk], [B, Lk] or [B, 1, 1, Lk] with B={B}, Lk={Lk}, got {tuple(keep.shape)}")
 
 
+def _check_gradient(q, k, bias):
+    """Sizes whose gradients would be refused (af3_cross_attention_backward), before the forward pass."""
+    B, H, Lq, _ = q.shape
+    Hkv, Lk = k.shape[1], k.shape[2]
+    if B * Hkv * -(-Lk // 32) >= 1 << 24:
+        raise ValueError(f"gradients take B * Hkv * ceil(Lk / 32) below 2^24, got {B} * {Hkv} * ceil({Lk} / 32)")
+    if bias is not None and bias.requires_grad and H * -(-Lq // 64) * -(-Lk // 64) >= 1 << 24:
+        raise ValueError(f"the gradient of a bias takes H * ceil(Lq / 64) * ceil(Lk / 64) below 2^24, got {H} * ceil({Lq} / 64) * ceil({Lk} / 64)")
+
+
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                     softmax_scale: Optional[float] = None) -> torch.Tensor:
     """softmax(q.k^T * softmax_scale + bias, mask) . v for queries and keys of any two lengths, down to a single query token.
@@ -170,11 +180,14 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
     scale = float(q.shape[3]) ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
+    graph = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad))
+    if graph:
+        _check_gradient(q, k, bias)
     with ops._on_device(q.device):   # (the call as a plain one: what it gives, gradients too, is not a question of how it came)
         out = _host.cross_attention(q, k, v, None if keep is None else keep.view(torch.bool), bias, scale)
     if out is not None:
         return out if out.__class__ is not int else _lib.check(out, "af3_cross_attention_forward")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
+    if graph:
         _host.check_capture(q, k, v, bias)
         return _CrossAttention.apply(q, k, v, keep, bias, scale)
     return _forward(q, k, v, keep, bias, scale, False)[0]

@@ -422,6 +422,9 @@ int64_t forward_workspace(const af3_cross_attention_params& p, const plan& f) { 
 
 }  // namespace cross
 
+// whether the gradients of k and v can be launched: workgroups of 32 keys, times 256 threads, inside 32 bits
+bool cross_gradients_fit(const af3_cross_attention_params& p) { return p.B * p.Hkv * ((p.Lk + 31) / 32) <= 0xffffff; }
+
 int validate_cross_attention(const af3_cross_attention_params* p) {
 	if(!p) return AF3_ERR_NULL_POINTER;
 	if(p->dtype != AF3_F32 && p->dtype != AF3_BF16) return AF3_ERR_BAD_DTYPE;
@@ -429,6 +432,7 @@ int validate_cross_attention(const af3_cross_attention_params* p) {
 	if(p->D > AF3_DPA_MAX_HEAD_DIM) return AF3_ERR_UNSUPPORTED_D;
 	// (row numbers and the parts' sizes stay far inside 63 bits, a launch's workgroups times 256 threads inside 32)
 	if(p->B > 0xffffff || p->H > 0xffff || p->Lq > 0x3fffffff || p->Lk > 0x3fffffff || p->B * p->H > 0xffffff || p->H * p->Lq > 0x7fffffff || p->B * p->H * ((p->Lq + 31) / 32) > 0xffffff) return AF3_ERR_BAD_SHAPE;
+	if(p->stats && !cross_gradients_fit(*p)) return AF3_ERR_BAD_SHAPE;   // (they are for a gradient that would be refused)
 	if(!p->q || !p->k || !p->v || !p->out) return AF3_ERR_NULL_POINTER;
 	for(int i = 0; i < 3; i++)
 		if(p->q_stride[i] < 0 || p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;

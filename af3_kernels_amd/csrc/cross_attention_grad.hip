@@ -13,7 +13,8 @@
 
 namespace af3 {
 
-int validate_cross_attention(const af3_cross_attention_params* p);
+int  validate_cross_attention(const af3_cross_attention_params* p);
+bool cross_gradients_fit(const af3_cross_attention_params& p);
 
 namespace cross {
 
@@ -736,8 +737,8 @@ int validate_grads(const af3_cross_attention_params* p, const af3_cross_attentio
 	if((g->grad_bias && !p->bias) || (g->grad_bias_residual && !g->grad_bias)) return AF3_ERR_NULL_POINTER;
 	for(int i = 0; i < 3; i++)
 		if(g->grad_out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
-	// (workgroup numbers of the kernels whose results are the keys' and the bias's)
-	if(p->B * p->Hkv * over(p->Lk, 32) > 0xffffff || (g->grad_bias && p->H * over(p->Lq, 64) * over(p->Lk, 64) > 0xffffff)) return AF3_ERR_BAD_SHAPE;
+	// (the bias's gradient: a workgroup for every 64 x 64 entries.  cross.py and host.cpp refuse such a call before its forward pass)
+	if(!cross_gradients_fit(*p) || (g->grad_bias && p->H * over(p->Lq, 64) * over(p->Lk, 64) > 0xffffff)) return AF3_ERR_BAD_SHAPE;
 	return AF3_OK;
 }
 
@@ -747,8 +748,8 @@ int validate_grads(const af3_cross_attention_params* p, const af3_cross_attentio
 using namespace af3;
 
 extern "C" int64_t af3_cross_attention_backward_workspace_bytes(const af3_cross_attention_params* params) {
-	const int rc = validate_cross_attention(params);
-	return rc != AF3_OK ? rc : cross::grad_workspace(*params).bytes;
+	if(const int rc = validate_cross_attention(params); rc != AF3_OK) return rc;
+	return cross_gradients_fit(*params) ? cross::grad_workspace(*params).bytes : AF3_ERR_BAD_SHAPE;
 }
 
 extern "C" int af3_cross_attention_backward(const af3_cross_attention_params* params, const af3_cross_attention_grads* grads, void* hip_stream) {

@@ -923,6 +923,8 @@ PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 	Tensor out;
 	int    rc = AF3_OK;
 	const bool graph = wants_grad({q, k, v, &c.bias});
+	// (sizes whose gradients would be refused: the Python side says so)
+	if(graph && (B * k->size(1) * ((Lk + 31) / 32) > 0xffffff || (c.bias.defined() && c.bias.requires_grad() && H * ((Lq + 63) / 64) * ((Lk + 63) / 64) > 0xffffff))) return none();
 	{
 		without_gil g;
 		if(graph) check_capture({q, k, v, &c.bias}, dev), out = apply_cross(c);

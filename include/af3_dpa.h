@@ -347,7 +347,8 @@ int af3_linear(const void* x, const void* weight, void* out, int64_t M, int64_t 
  *               too, the row sums of grad_out * out that it takes off every dS are those of out to 16 bits (with out alone they are off by up to
  *               2^-8 in the same direction along a row, which does not average out of a gradient summed along rows, like a position bias's).
  *   workspace : af3_cross_attention_workspace_bytes() bytes, 16-byte aligned; NULL where that is 0.  Overwritten.
- * B, H, Lq, Lk, D >= 1, D <= AF3_DPA_MAX_HEAD_DIM, Lq and Lk < 2^30, H * Lq < 2^31, B * H * ceil(Lq / 32) < 2^26.
+ * B, H, Lq, Lk, D >= 1, D <= AF3_DPA_MAX_HEAD_DIM, Lq and Lk < 2^30, H < 2^16, H * Lq < 2^31, B * H * ceil(Lq / 32) < 2^24; with stats, as for the gradient,
+ * B * Hkv * ceil(Lk / 32) < 2^24 too.  AF3_ERR_BAD_SHAPE otherwise, from the workspace call as well.
  */
 typedef struct af3_cross_attention_params {
 	const void*    q;
@@ -381,6 +382,8 @@ int64_t af3_cross_attention_workspace_bytes(const af3_cross_attention_params* pa
  * grad_bias_residual (optional, beside grad_bias, AF3_BF16 only, same layout): what grad_bias lost by its rounding, as bf16.  Every row of dS sums to zero, so the sums that
  * a learned bias's gradient is made of lose most of their terms against each other, and what is left of grad_bias's own rounding would be several times theirs.
  * workspace: af3_cross_attention_backward_workspace_bytes() bytes, 16-byte aligned, required.
+ * Sizes as for a forward call with stats; with grad_bias H * ceil(Lq / 64) * ceil(Lk / 64) < 2^24 (AF3_ERR_BAD_SHAPE otherwise, from this call alone: whether grad_bias
+ * is wanted the others cannot know).
  */
 typedef struct af3_cross_attention_grads {
 	const void* grad_out;

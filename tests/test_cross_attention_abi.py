@@ -177,3 +177,45 @@ def test_forward_mode_is_refused():
         table = torch.randn(32, 2)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             af3.relative_position_bias(forward_ad.make_dual(table, torch.ones_like(table)), 3, 4)
+
+
+def test_sizes_at_their_limits():
+    """The limits that the header states, from either side; nothing is launched (size queries, and calls that lack their workspace)."""
+    from af3_kernels_amd import _lib
+    lib = _lib.load()
+    ws = lambda **kw: lib.af3_cross_attention_workspace_bytes(ctypes.byref(_cross(**kw)))
+    gws = lambda **kw: lib.af3_cross_attention_backward_workspace_bytes(ctypes.byref(_cross(**kw)))
+    bwd = lambda g, **kw: lib.af3_cross_attention_backward(ctypes.byref(_cross(**kw)), ctypes.byref(_grads(workspace=None, **g)), None)
+    full = 1 << 24
+    for under, over in (({"B": full // 2 - 1, "H": 2, "Hkv": 1, "Lq": 32, "Lk": 1}, {"B": full // 2, "H": 2, "Hkv": 1, "Lq": 32, "Lk": 1}),
+                        ({"B": 1, "H": 255, "Hkv": 1, "Lq": 1 << 21, "Lk": 1}, {"B": 1, "H": 256, "Hkv": 1, "Lq": 1 << 21, "Lk": 1}),
+                        ({"B": 1, "H": 255, "Hkv": 1, "Lq": 1 << 21, "Lk": 1}, {"B": 1, "H": 255, "Hkv": 1, "Lq": (1 << 21) + (1 << 15), "Lk": 1}),
+                        ({"B": 255, "H": 65535, "Hkv": 1, "Lq": 1, "Lk": 1}, {"B": 1, "H": 65536, "Hkv": 1, "Lq": 1, "Lk": 1}),
+                        ({"B": 1, "H": 1, "Hkv": 1, "Lq": 1, "Lk": (1 << 29) - 32}, {"B": 1, "H": 1, "Hkv": 1, "Lq": 1, "Lk": 1 << 30})):
+        assert ws(**under) >= 0 and gws(**under) > 0 and bwd({}, **under) == -7, under
+        assert ws(**over) == -3 and gws(**over) == -3 and bwd({}, **over) == -3, over
+    # keys: a forward pass alone takes more of them than one with its gradient
+    under, over = ({"B": 1 << 10, "H": 4, "Hkv": 4, "Lq": 1, "Lk": n} for n in ((1 << 17) - 32, 1 << 17))
+    assert ws(**under) >= 0 and gws(**under) > 0 and bwd({}, **under) == -7
+    assert ws(**over) == -3 and gws(**over) == -3 and bwd({}, **over) == -3 and lib.af3_cross_attention_forward(ctypes.byref(_cross(**over)), None) == -3
+    assert ws(stats=None, **over) >= 0 and gws(stats=None, **over) == -3
+    # a bias's gradient: tiles of 64 x 64 for every head
+    under, over = ({"B": 1, "H": 1, "Hkv": 1, "Lq": 64 * n, "Lk": 64 * 4096, "bias": BASE} for n in (4095, 4096))
+    for sizes, wanted, rc in ((under, BASE, -7), (over, BASE, -3), (over, None, -7)):
+        assert ws(**sizes) >= 0 and gws(**sizes) > 0 and bwd({"grad_bias": wanted}, **sizes) == rc
+
+
+def test_sizes_without_a_gradient_are_refused_before_the_forward_pass():
+    from af3_kernels_amd import cross
+    thin = lambda *shape: torch.zeros(1).expand(*shape)
+    q, k = thin(1, 2, 64, 8), thin(1, 2, 64, 8)
+    cross._check_gradient(q, k, None)
+    cross._check_gradient(thin(1 << 10, 4, 1, 8), thin(1 << 10, 4, (1 << 17) - 32, 8), None)
+    with pytest.raises(ValueError, match="Hkv"):
+        cross._check_gradient(thin(1 << 10, 4, 1, 8), thin(1 << 10, 4, 1 << 17, 8), None)
+    long, longer = thin(1, 1, 64 * 4095, 8), thin(1, 1, 64 * 4096, 8)
+    leaf = torch.zeros(1, 1, 64 * 4096).requires_grad_(True)
+    cross._check_gradient(long, longer, leaf.expand(1, 64 * 4095, -1))
+    cross._check_gradient(longer, longer, leaf.detach().expand(1, 64 * 4096, -1))
+    with pytest.raises(ValueError, match="gradient of a bias"):
+        cross._check_gradient(longer, longer, leaf.expand(1, 64 * 4096, -1))

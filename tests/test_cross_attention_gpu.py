@@ -1034,3 +1034,21 @@ def test_no_forward_mode(af3, monkeypatch, native):
         torch.func.jvp(lambda x: af3.cross_attention(x, k, v, m, b), (q,), (q,))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda x: af3.cross_attention(x, k, v, m, b))(q[None])
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_sizes_without_a_gradient(af3, monkeypatch, native):
+    """Refused before the forward pass, not behind it; without a graph such calls run."""
+    from af3_kernels_amd import cross
+    if not native:
+        monkeypatch.setattr(cross, "_host", _NoNativeHost())
+    n = 64 * 4096
+    q, k = (torch.zeros(1, 1, 1, 8, device="cuda", dtype=BF16).expand(1, 1, n, 8) for _ in range(2))
+    bias = torch.zeros(1, 1, n, device="cuda", dtype=BF16).requires_grad_(True)
+    with pytest.raises(ValueError, match="gradient of a bias"):
+        af3.cross_attention(q, k, k, None, bias.expand(1, n, n))
+    leaf = torch.zeros(1 << 10, 4, 1, 8, device="cuda", dtype=BF16).requires_grad_(True)
+    many = torch.ones(1, 1, 1, 8, device="cuda", dtype=BF16).expand(1 << 10, 4, 1 << 17, 8)
+    with pytest.raises(ValueError, match="Hkv"):
+        af3.cross_attention(leaf, many, many)
+    assert (af3.cross_attention(leaf.detach(), many, many) == 1).all()
