@@ -737,6 +737,7 @@ int validate_grads(const af3_cross_attention_params* p, const af3_cross_attentio
 	if((g->grad_bias && !p->bias) || (g->grad_bias_residual && !g->grad_bias)) return AF3_ERR_NULL_POINTER;
 	for(int i = 0; i < 3; i++)
 		if(g->grad_out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
+	if(g->grad_bias_residual && p->dtype != AF3_BF16) return AF3_ERR_BAD_DTYPE;   // (nothing would be written there)
 	// (the bias's gradient: a workgroup for every 64 x 64 entries.  cross.py and host.cpp refuse such a call before its forward pass)
 	if(!cross_gradients_fit(*p) || (g->grad_bias && p->H * over(p->Lq, 64) * over(p->Lk, 64) > 0xffffff)) return AF3_ERR_BAD_SHAPE;
 	return AF3_OK;

@@ -379,7 +379,7 @@ int64_t af3_cross_attention_workspace_bytes(const af3_cross_attention_params* pa
  * Gradients of af3_cross_attention_forward.  `params` as in the forward call, with the `out` and `stats` that it wrote (its workspace is not
  * used); grad_out [B, H, Lq, D] with strides, of `dtype`.  grad_q [B, H, Lq, D], grad_k, grad_v [B, Hkv, Lk, D] and grad_bias [H, Lq, Lk] (summed over
  * the batch) are contiguous and written whole, zeros for dropped keys among it; NULL: not wanted.  No atomics: the same bits every time.
- * grad_bias_residual (optional, beside grad_bias, AF3_BF16 only, same layout): what grad_bias lost by its rounding, as bf16.  Every row of dS sums to zero, so the sums that
+ * grad_bias_residual (optional, beside grad_bias, AF3_BF16 only (AF3_ERR_BAD_DTYPE), same layout): what grad_bias lost by its rounding, as bf16.  Every row of dS sums to zero, so the sums that
  * a learned bias's gradient is made of lose most of their terms against each other, and what is left of grad_bias's own rounding would be several times theirs.
  * workspace: af3_cross_attention_backward_workspace_bytes() bytes, 16-byte aligned, required.
  * Sizes as for a forward call with stats; with grad_bias H * ceil(Lq / 64) * ceil(Lk / 64) < 2^24 (AF3_ERR_BAD_SHAPE otherwise, from this call alone: whether grad_bias

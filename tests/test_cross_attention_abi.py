@@ -219,3 +219,12 @@ def test_sizes_without_a_gradient_are_refused_before_the_forward_pass():
     cross._check_gradient(longer, longer, leaf.detach().expand(1, 64 * 4096, -1))
     with pytest.raises(ValueError, match="gradient of a bias"):
         cross._check_gradient(longer, longer, leaf.expand(1, 64 * 4096, -1))
+
+
+def test_what_fp32_does_not_lose_is_not_asked_for():
+    """grad_bias_residual of an fp32 call would be left as it was: refused."""
+    from af3_kernels_amd import _lib
+    lib = _lib.load()
+    bwd = lambda p: lib.af3_cross_attention_backward(ctypes.byref(p), ctypes.byref(_grads(grad_bias=BASE, grad_bias_residual=2 * BASE, workspace=None)), None)
+    assert bwd(_cross(bias=BASE, dtype=_lib.AF3_F32)) == -2
+    assert bwd(_cross(bias=BASE)) == -7      # (as far as its missing workspace)
