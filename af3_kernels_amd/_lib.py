@@ -161,6 +161,13 @@ class _Host:
             warnings.warn(f"{HOST_PATH} is missing: calls are prepared in Python, which takes 10 to 40 us more each; build it with `python -m af3_kernels_amd.build`", RuntimeWarning)
         return lambda *args: None
 
+    def check_capture(self, *tensors):   # (the module's own takes this one's place where there is one)
+        """Raises where a gradient is to be captured: a capture that would wait for another stream ends the process, and on which stream a leaf's gradient is
+        accumulated only the native module can see."""
+        import torch
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"a gradient can be captured into a HIP graph only with the native host side, and {HOST_PATH} is missing: build it with `python -m af3_kernels_amd.build`")
+
 
 def load_host():
     """The native host side where it is built already (its functions are then the module's own), else a stand-in that finds it later."""

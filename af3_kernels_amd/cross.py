@@ -188,7 +188,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
     if out is not None:
         return out if out.__class__ is not int else _lib.check(out, "af3_cross_attention_forward")
     if graph:
-        _host.check_capture(q, k, v, bias)
+        with ops._on_device(q.device):
+            _host.check_capture(q, k, v, bias)
         return _CrossAttention.apply(q, k, v, keep, bias, scale)
     return _forward(q, k, v, keep, bias, scale, False)[0]
 
@@ -320,6 +321,7 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, scheme: 
     if out is not None:
         return out if out.__class__ is not int else _lib.check(out, "af3_position_bias_forward")
     if torch.is_grad_enabled() and table.requires_grad:
-        _host.check_capture(table)
+        with ops._on_device(table.device):
+            _host.check_capture(table)
         return _PositionBias.apply(table, q_len, k_len, settings, q_positions, k_positions)
     return _position_forward(table, q_len, k_len, settings, q_positions, k_positions)

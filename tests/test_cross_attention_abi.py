@@ -228,3 +228,20 @@ def test_what_fp32_does_not_lose_is_not_asked_for():
     bwd = lambda p: lib.af3_cross_attention_backward(ctypes.byref(p), ctypes.byref(_grads(grad_bias=BASE, grad_bias_residual=2 * BASE, workspace=None)), None)
     assert bwd(_cross(bias=BASE, dtype=_lib.AF3_F32)) == -2
     assert bwd(_cross(bias=BASE)) == -7      # (as far as its missing workspace)
+
+
+def test_without_the_native_host_no_gradient_is_captured(monkeypatch, tmp_path):
+    from af3_kernels_amd import _lib
+    host = _lib._Host()
+    monkeypatch.setattr(_lib, "HOST_PATH", str(tmp_path / "_host.so"))
+    monkeypatch.setattr(_lib._Host, "_warned", True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    assert host.cross_attention() is None       # (the Python implementation's turn)
+    with pytest.raises(RuntimeError, match="native host side"):
+        host.check_capture()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert host.check_capture() is None
+    # found later: the module's own
+    monkeypatch.undo()
+    from af3_kernels_amd import _host
+    assert host.cross_attention is _host.cross_attention and host.check_capture is _host.check_capture

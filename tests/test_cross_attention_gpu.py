@@ -1052,3 +1052,28 @@ def test_sizes_without_a_gradient(af3, monkeypatch, native):
     with pytest.raises(ValueError, match="Hkv"):
         af3.cross_attention(leaf, many, many)
     assert (af3.cross_attention(leaf.detach(), many, many) == 1).all()
+
+
+def test_without_the_native_host_no_gradient_is_captured(af3, monkeypatch, tmp_path):
+    from af3_kernels_amd import _lib, cross
+    monkeypatch.setattr(_lib, "HOST_PATH", str(tmp_path / "_host.so"))
+    monkeypatch.setattr(_lib._Host, "_warned", True)
+    monkeypatch.setattr(cross, "_host", _lib._Host())
+    q, table = torch.randn(1, 2, 4, 16, device="cuda"), torch.randn(32, 2, device="cuda")
+    want = af3.cross_attention(q, q, q, None, af3.relative_position_bias(table, 4, 4))
+    leaf, leaf_table = q.clone().requires_grad_(True), table.clone().requires_grad_(True)
+    refused = 0
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: af3.cross_attention(leaf, q, q), lambda: af3.relative_position_bias(leaf_table, 4, 4)):
+            with pytest.raises(RuntimeError, match="native host side"):
+                call()
+            refused += 1
+        plain = af3.cross_attention(q, q, q, None, af3.relative_position_bias(table, 4, 4))
+    assert refused == 2
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(plain, want)
+    # ... and outside of a capture it flows
+    assert torch.autograd.grad(af3.cross_attention(leaf, q, q).sum(), leaf)[0].isfinite().all()
