@@ -159,8 +159,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
     says: a row of nothing else weights its live keys alike.  Lk == 0 gives zeros.
 
     Gradients flow to q, k, v and bias (the same bits every time); a second derivative and forward mode raise.  In a HIP graph: capture forward and backward
-    together, with leaves that no result of an earlier call on another stream still holds: their gradients would be accumulated on that stream, outside of
-    the capture, so such a call raises RuntimeError."""
+    together, and whatever leads to the inputs, with leaves that no result of an earlier call on another stream still holds.  Their gradients would be worked out or
+    accumulated on that stream, outside of the capture, so such a call raises RuntimeError."""
     out = _host.cross_attention(q, k, v, mask, bias, softmax_scale)
     if out is not None:
         return out if out.__class__ is not int else _lib.check(out, "af3_cross_attention_forward")

@@ -633,13 +633,21 @@ PyObject* py_gated_linear_unit(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---- attention to states of another length, relative position bias ------------------------------------------------------------
-// A graph that is captured may not wait for work outside of it.  The gradient of a leaf is accumulated on the stream that was current when the leaf
-// first came into a graph of operations that is still alive; inside a capture that must be the capturing stream, or the engine makes the two wait for each
-// other and ends the process.  Looked at while capturing only.
+// A graph that is captured may not wait for work outside of it, and a backward pass runs each operation on the stream that its forward pass ran on: all that leads to the inputs must
+// have been recorded within the same capture.  The gradient of a leaf is accumulated on the stream that was current when the leaf first came into a graph of operations
+// that is still alive; that must be the capturing stream itself.  Otherwise the engine makes the streams wait for each other and ends the process.  Looked at while capturing only.
 void check_capture(at::ArrayRef<const Tensor*> inputs, int dev) {
 	hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
 	const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev);
 	if(hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+	unsigned long long capture = 0;
+	if(hipStreamGetCaptureInfo(stream.stream(), &status, &capture) != hipSuccess) return;
+	auto within = [&](const c10::Stream& s) {
+		if(s.id() == stream.id() || s.id() == 0) return s.id() == stream.id();   // (0, the default stream, is never captured and must not be asked)
+		hipStreamCaptureStatus of = hipStreamCaptureStatusNone;
+		unsigned long long     id = 0;
+		return hipStreamGetCaptureInfo(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, s).stream(), &of, &id) == hipSuccess && of == hipStreamCaptureStatusActive && id == capture;
+	};
 	std::vector<torch::autograd::Node*>        open;
 	std::unordered_set<torch::autograd::Node*> seen;
 	std::vector<std::shared_ptr<torch::autograd::Node>> leaves;
@@ -654,11 +662,15 @@ void check_capture(at::ArrayRef<const Tensor*> inputs, int dev) {
 	while(!open.empty()) {
 		torch::autograd::Node* node = open.back();
 		open.pop_back();
-		if(dynamic_cast<torch::autograd::AccumulateGrad*>(node)) {
-			const auto own = node->stream();
-			TORCH_CHECK(!own || own->id() == stream.id(),
-						"a gradient is captured into a HIP graph while a graph of operations recorded on another stream still holds one of its leaves (an earlier result that was not "
-						"freed, for instance): the capture would wait for that stream. Free it first, or capture with leaves of their own");
+		if(const auto own = node->stream()) {
+			if(dynamic_cast<torch::autograd::AccumulateGrad*>(node)) {
+				TORCH_CHECK(own->id() == stream.id(),
+							"a gradient is captured into a HIP graph while a graph of operations recorded on another stream still holds one of its leaves (an earlier result that was not "
+							"freed, for instance): the capture would wait for that stream. Free it first, or capture with leaves of their own");
+			} else {
+				TORCH_CHECK(within(*own), "a gradient is captured into a HIP graph of an input that comes from operations outside of the capture (", node->name(),
+							"): the capture would wait for their stream. Detach it, or capture them too");
+			}
 		}
 		for(const auto& e : node->next_edges()) look(e.function);
 	}

@@ -1077,3 +1077,41 @@ def test_without_the_native_host_no_gradient_is_captured(af3, monkeypatch, tmp_p
     assert torch.equal(plain, want)
     # ... and outside of a capture it flows
     assert torch.autograd.grad(af3.cross_attention(leaf, q, q).sum(), leaf)[0].isfinite().all()
+
+
+def test_a_captured_gradient_of_what_was_made_outside_is_refused(af3):
+    """The leaves' gradients belong to the capturing stream here, an operation between them and the call does not: it would run on its own stream, which is not captured."""
+    capturing, aside = torch.cuda.Stream(), torch.cuda.Stream()
+    q, k = torch.randn(1, 2, 4, 16, device="cuda").requires_grad_(True), torch.randn(1, 2, 5, 16, device="cuda")
+    table = torch.randn(32, 2, device="cuda").requires_grad_(True)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(capturing):
+        held = q * 1, table * 1            # the leaves come into a graph here first
+    torch.cuda.synchronize()
+    outside = [q * 2, af3.relative_position_bias(table, 4, 5)]
+    with torch.cuda.stream(aside):
+        outside.append(q * 3)
+    torch.cuda.synchronize()
+    want = af3.cross_attention(outside[0].detach(), k, k, None, outside[1].detach())
+    calls = [lambda: af3.cross_attention(outside[0], k, k), lambda: af3.cross_attention(q.detach(), k, k, None, outside[1]), lambda: af3.cross_attention(outside[2], k, k),
+             lambda: af3.relative_position_bias(table * 1 + held[1].sum() + outside[1].sum(), 4, 5)]
+    refused = 0
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=capturing):
+        for call in calls:
+            with pytest.raises(RuntimeError, match="outside of the capture"):
+                call()
+            refused += 1
+        plain = af3.cross_attention(outside[0].detach(), k, k, None, outside[1].detach())
+        # recorded on another stream of the same capture: taken
+        aside.wait_stream(capturing)
+        with torch.cuda.stream(aside):
+            branch = q * 2
+        capturing.wait_stream(aside)
+        assert af3.cross_attention(branch, k, k).requires_grad
+    assert refused == 4
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(plain, want)
+    del held, outside
