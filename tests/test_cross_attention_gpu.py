@@ -1115,3 +1115,43 @@ def test_a_captured_gradient_of_what_was_made_outside_is_refused(af3):
     torch.cuda.synchronize()
     assert torch.equal(plain, want)
     del held, outside
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,H,Hkv,Lq,Lk,D,live", [
+    # whole rows in one workgroup, which goes through them in two stretches of 16384 keys, in every kernel
+    (64, 8, 8, 1, 20000, 16, [0, 5, 9000, 16383, 16384, 16500, 19999]),
+    (64, 8, 8, 3, 17000, 32, [16383, 16384]),
+    (64, 8, 8, 1, 33000, 8, [40, 16384, 32767, 32768]),      # three of them
+    (16, 16, 16, 200, 17000, 32, [16383, 16384, 16400]),     # 128 rows to a workgroup
+    # a key axis in parts: live keys in a few of them, at their ends among others
+    (1, 2, 2, 1, 40000, 64, [3, 639, 640, 5000, 20011, 39999]),
+    (1, 4, 2, 20, 40000, 128, [0, 12799, 12800, 33333]),
+    (2, 2, 1, 3, 17000, 32, [100, 16384, 16999]),
+])
+def test_few_live_keys_of_a_long_axis(af3, B, H, Hkv, Lq, Lk, D, live, dtype):
+    """Few enough that each of them shows: a result without any one of them is off by more than it may be (of the formula's own results; nothing is planted in the kernels)."""
+    gen = torch.Generator("cuda").manual_seed(98)
+    n = lambda *s: torch.randn(s, generator=gen, device="cuda", dtype=dtype)
+    q, k, v, b, g = n(B, H, Lq, D), n(B, Hkv, Lk, D), n(B, Hkv, Lk, D), n(H, Lq, Lk), n(B, H, Lq, D)
+    mask = torch.zeros(B, Lk, dtype=torch.bool, device="cuda")
+    mask[:, live] = True
+    got = run(af3, q, k, v, mask, b, g)
+    few = lambda keys: formula(q, k[:, :, keys], v[:, :, keys], None, b[:, :, keys], g, D ** -0.5)
+    want = few(live)
+    up, uo = (2.0 ** -8, 2.0 ** -8) if dtype == BF16 else (0.0, E32)
+    for name in ("dk", "dv", "dbias"):
+        rest = got[name].clone()
+        rest.index_fill_(2, torch.tensor(live, device="cuda"), 0.0)
+        assert not rest.any(), name
+        got[name] = got[name][:, :, live]
+    for name, t in got.items():
+        check(name, t, want[name], dtype)
+    for gone in range(len(live)):
+        others = few(live[:gone] + live[gone + 1:])
+        for name in ("out", "dq"):
+            value, bound = want[name]
+            assert ((others[name][0] - value).abs() > bound(up, uo)).any(), (name, live[gone])
+        for name in ("dk", "dv", "dbias"):
+            value, bound = want[name]
+            assert (value.abs() > bound(up, uo))[:, :, gone].any(), (name, live[gone])
