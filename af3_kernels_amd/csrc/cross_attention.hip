@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 	f32x16 o[TL::BLOCKS];
 #pragma unroll
 	for(int db = 0; db < TL::BLOCKS; db++) o[db] = f32x16{};
-	bool any = false, fresh = true;   // a live key was met; no block yet
+	bool any = false, moves = true;   // a live key was met; the reference moves at the next block (the first one, and while a row is far)
 
 	const int64_t last = (int64_t)(split + 1) * a.part < p.Lk ? (int64_t)(split + 1) * a.part : p.Lk;
 	const typename TL::reader at(lane);
@@ -151,24 +151,23 @@ __global__ void __launch_bounds__(THREADS, wavefronts(forward_shape<T, DP, KW>::
 				};
 				// Optimistic: the probabilities against the reference as it is.  It moves, to the maximum, at a wavefront's first block and where they get large, and
 				// then nothing needs a factor until they get large again.
-				float sum  = 0.f;
-				bool  move = fresh;
-				fresh      = false;
+				float sum = 0.f;
 				logits();
-				if(!move) {
-					sum  = probabilities();
-					move = __any(!(sum < LARGE));
-					if(move) logits();
+				if(!moves) {
+					sum   = probabilities();
+					moves = __any(!(sum < LARGE));
+					if(moves) logits();
 				}
-				if(move) {
+				if(moves) {
 					float top = x[0];
 #pragma unroll
 					for(int r = 1; r < 16; r++) top = maximum(top, x[r]);
 					const float to = maximum(m, maximum_of_halves(top)), by = __builtin_amdgcn_exp2f((m - to) * to_log2);
-					m = to, reference = reference_of(m, to_log2), l *= by;
+					m = to, reference = m * to_log2, l *= by;
 #pragma unroll
 					for(int db = 0; db < TL::BLOCKS; db++) o[db] *= by;
-					if(__any(m < FAR_BELOW)) {   // a row of hugely negative biases alone: its logits leave the range in units of log2 e
+					moves = __any(is_far(reference));
+					if(moves) {
 						sum = 0.f;
 #pragma unroll
 						for(int r = 0; r < 16; r++) {

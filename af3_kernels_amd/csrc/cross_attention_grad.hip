@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(THREADS, wavefronts(dq_shape<T, DP, KW>::REGIS
 	const float delta = row_delta<T, DP>(a, gf, b, h, qi, ok, lane);
 	if(ok && half == 0 && kwave == 0 && split == 0) a.delta[row] = delta;
 	const float  m = ok ? p.stats[2 * row] : 0.f, inv = ok ? p.stats[2 * row + 1] : 0.f;
-	const bool   apart = sizeof(T) == 4 || DP > 96 || __any(m < FAR_BELOW);   // (a row whose maximum is far below: exact, in natural units; 128 columns: registers for one form)
+	const bool   apart = sizeof(T) == 4 || DP > 96 || __any(is_far(m * a.factor));   // (a row far from zero: in the logits' own units; 128 columns: registers for one form)
 	const float  taken = whole_reference(m, inv, a.factor);
 	const T* const kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[1];
 	const T* const vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(THREADS) cross_delta_kernel(grad_args a) {
 }
 
 // What the kernels with query rows in tiles keep of each row of a tile in LDS: delta with its sign turned (it begins the sum of dP), and, for bf16, the whole reference;
-// maximum and 1 / sum for fp32 and for tiles with a row far below.  Behind them a word that says whether there is one.
+// maximum and 1 / sum for fp32 and for tiles with a row far from zero.  Behind them a word that says whether there is one.
 constexpr int ROW_STATS = 4;
 template <typename T, int QT>
 struct row_stats {
@@ -272,7 +272,7 @@ struct row_stats {
 		st[QT + threadIdx.x] = less, st[2 * QT + threadIdx.x] = m, st[3 * QT + threadIdx.x] = inv;
 		if constexpr(sizeof(T) == 2) {
 			st[threadIdx.x] = whole_reference(m, inv, factor);
-			const bool far = __any(m < FAR_BELOW);   // (of 64 rows: a tile of 128 has two such words)
+			const bool far = __any(is_far(m * factor));   // (of 64 rows: a tile of 128 has two such words)
 			if((threadIdx.x & 63) == 0) reinterpret_cast<int*>(st + ROW_STATS * QT)[threadIdx.x >> 6] = far;
 		}
 	}

@@ -77,14 +77,11 @@ __device__ __forceinline__ u32x4 load_guarded(const T* row, int d, int D) {
 
 __device__ __forceinline__ int   tile_row(int i) { return 16 * ((i >> 2) & 1) + (i & 3) + 4 * (i >> 3); }
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }   // (NaN stays)
-// What is taken off a row's logits in units of log2 e: a row's maximum (or what was its maximum) m times the factor.  -inf, which makes every probability infinite or
-// NaN, sends those who look at them to the exact form, for rows whose maximum is so low that the product could leave fp32's range; a maximum of
-// +inf makes the row NaN, as in the formula.
-constexpr float FAR_BELOW = -1e38f;
-__device__ __forceinline__ float reference_of(float m, float to_log2) {
-	const float r = m * to_log2;
-	return m < FAR_BELOW ? -INFINITY : r - r + r;
-}
+// What is taken off a row's logits in units of log2 e, its reference, is a row's maximum (or what was its maximum) times the factor, rounded: every probability of the row is off by the
+// same 2^-24 of it.  Far from zero that is felt, and from 2^24 on it alone decides whether they are zero or infinite (rows whose every key has a bias of -1e9, say): such
+// rows have their maximum taken off in the logits' own units, where logits near it lose nothing.  Infinite references and NaN are far as well.
+constexpr float FAR = 4096.f;
+__device__ __forceinline__ bool is_far(float reference) { return !(__builtin_fabsf(reference) < FAR); }
 // What the gradients take off a row's logits instead (bf16): the reference and the logarithm of the row's sum together, so that P comes out of the exponential as it is.
 // (fp32 keeps the two apart: in one number their rounding, 2^-24 of it, would be the largest error of P.)  1 / sum == 0, a row without a live key, makes P zero.
 __device__ __forceinline__ float whole_reference(float m, float inv, float to_log2) { return m * to_log2 - __builtin_amdgcn_logf(inv); }

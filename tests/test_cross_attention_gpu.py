@@ -1155,3 +1155,25 @@ def test_few_live_keys_of_a_long_axis(af3, B, H, Hkv, Lq, Lk, D, live, dtype):
         for name in ("dk", "dv", "dbias"):
             value, bound = want[name]
             assert (value.abs() > bound(up, uo))[:, :, gone].any(), (name, live[gone])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("far", [3000.0, 1e5, 1e7, 1e9, 1e10, 1e20, 1e30, 3.3e38])
+@pytest.mark.parametrize("sign", [1, -1], ids=["high", "low"])
+def test_rows_whose_logits_are_all_far_from_zero(af3, dtype, far, sign):
+    """A bias that is the same for all keys of a query changes nothing, and keys that lie far below the others have no weight: -1e9 as a mask of a padded query, say.
+    The queries are zeros there, so that every logit is the bias, to the bit, and P what it is without it."""
+    c = torch.tensor(sign * far).to(dtype)
+    for B, H, Hkv, Lq, Lk, D in ((2, 2, 2, 40, 150, 32), (1, 2, 1, 1, 1700, 64), (2, 2, 2, 64, 300, 128), (9, 16, 16, 140, 150, 64), (9, 16, 4, 300, 70, 128)):
+        q, k, v, m, b, g = make(B, H, Hkv, Lq, Lk, D, dtype, 99, "ragged", "given")
+        rows = torch.arange(0, Lq, 3, device="cuda")
+        q[:, 0, rows] = 0.0
+        plain = b.clone()
+        for bias, here, there in ((b, c, c / 2 if sign > 0 else c * 2), (plain, 0.0, -math.inf)):
+            bias[0, rows] = here
+            bias[0, rows[:, None], torch.arange(1, Lk, 2, device="cuda")] = there
+        print((B, H, Hkv, Lq, Lk, D), flush=True)
+        got = run(af3, q, k, v, m, b, g)
+        want = formula(q, k, v, m, plain, g, D ** -0.5)
+        for name, t in got.items():
+            check(name, t, want[name], dtype)
