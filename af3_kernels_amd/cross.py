@@ -294,7 +294,8 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, scheme: 
     border fall where the formula puts them.  Bidirectional: keys ahead of the query take the second n buckets; otherwise they count as
     distance 0.  scheme "clip": bucket = position of the query - position of the key limited to -max_distance .. max_distance, plus max_distance
     (2 max_distance + 1 buckets), or limited to 0 .. max_distance (max_distance + 1 buckets) if not bidirectional; with residue numbers
-    as positions that is AlphaFold 3's relative residue encoding.
+    as positions that is what AlphaFold 3's relative residue encoding does within a chain (pairs of different chains, which have a bucket of their own
+    there, fall where their numbers put them here).
 
     Positions are 0, 1, 2, ... for keys and q_offset, q_offset + 1, ... for queries (a decoder's token t: q_len=1, q_offset=t), or what q_positions [q_len]
     and k_positions [k_len] hold (int64 or int32, on the table's device; q_offset then does not count for queries).

@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(THREADS) position_bias_kernel(args a) {
 }
 
 // Sums by bucket.  Every thread has a column of the bins in LDS to itself (64 threads to a workgroup), so that nothing is added in an order that
-// changes; the sums of the threads, then of the workgroups (in 64 bits) follow in a fixed order.
+// changes; the sums of the threads, then of the workgroups (in 64 bits) follow in a fixed order.  A workgroup's own are in 32 bits, which LDS adds by itself: a thread has 4096 pieces
+// at most.
 constexpr int COLUMNS = 64;
 template <typename T, bool LUT>
 __global__ void __launch_bounds__(COLUMNS) position_bias_sums_kernel(args a) {
@@ -346,7 +347,8 @@ dim3 shape(args& a, int E, int n, int64_t each) {
 	return dim3((uint32_t)across, (uint32_t)((a.Lq + a.rows - 1) / a.rows), (uint32_t)a.H);
 }
 dim3 sums_shape(args& a, int E) {
-	// about 2048 workgroups; each adds its bins up, which is worth a few hundred rows of reading
+	// about 2048 workgroups, of 8 pieces per thread at least: each clears its bins and adds them up, whatever it reads (16 x 768 x 768 in fp32 takes 23.5 us with 3 buckets,
+	// 28 with 65, 49 with 129)
 	const int64_t pieces = a.H * a.Lq * ((a.Lk + E - 1) / E);
 	int64_t       each = pieces / (2048 * COLUMNS);
 	dim3 grid = shape(a, E, COLUMNS, each < 8 ? 8 : each > 4096 ? 4096 : each);
