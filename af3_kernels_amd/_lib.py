@@ -79,6 +79,39 @@ class PositionBiasParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    """Mirror of struct af3_rotary_params."""
+    _fields_ = [
+        ("x", vp * 2), ("out", vp * 2), ("frequencies", vp), ("positions", vp), ("position_stride_b", i64), ("offset", i64),
+        ("B", i64), ("L", i64), ("D", i64), ("rotary", i64), ("heads", i64 * 2),
+        ("x_stride", (i64 * 3) * 2), ("out_stride", (i64 * 3) * 2),
+        ("dtype", i32), ("interleaved", i32), ("inverse", i32), ("scale", f32),
+    ]
+
+
+class ResidualNormParams(ctypes.Structure):
+    """Mirror of struct af3_residual_norm_params."""
+    _fields_ = [
+        ("x", vp), ("y", vp), ("gate", vp), ("weight", vp), ("bias", vp), ("post_weight", vp), ("out", vp), ("normed", vp), ("stats", vp),
+        ("rows", i64), ("C", i64), ("group", i64), ("x_stride", i64), ("y_stride", i64),
+        ("gate_share", i32), ("weight_share", i32), ("bias_share", i32), ("norm", i32), ("post_norm", i32), ("gate_sigmoid", i32), ("dtype", i32),
+        ("eps", f32), ("residual_scale", f32), ("reserved", i32),
+    ]
+
+
+class ResidualNormGrads(ctypes.Structure):
+    """Mirror of struct af3_residual_norm_grads."""
+    _fields_ = [
+        ("grad_out", vp), ("grad_normed", vp), ("grad_out_stride", i64), ("grad_normed_stride", i64),
+        ("grad_x", vp), ("grad_y", vp), ("grad_gate", vp), ("grad_weight", vp), ("grad_bias", vp), ("grad_post_weight", vp),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+ROTARY_MAX_HEAD_DIM = 1024                 # AF3_ROTARY_MAX_HEAD_DIM
+RESIDUAL_NORM_MAX_CHANNELS = 16384         # AF3_RESIDUAL_NORM_MAX_CHANNELS
+NORMS = {"none": 0, "rms": 1, "layer": 2}  # af3_norm
+SHARE_NONE, SHARE_CHANNEL, SHARE_GROUP, SHARE_ROW = 0, 1, 2, 3   # af3_share
 POSITION_SCHEMES = {"log": 0, "clip": 1}   # af3_position_scheme
 POSITION_BIAS_MAX_BUCKETS = 576            # AF3_POSITION_BIAS_MAX_BUCKETS
 QKV_SCRATCH_FLOATS = 768   # AF3_QKV_SCRATCH_FLOATS
@@ -103,6 +136,10 @@ SYMBOLS = {
     "af3_position_bias_forward": (ctypes.c_int, [ctypes.POINTER(PositionBiasParams), vp]),
     "af3_position_bias_backward": (ctypes.c_int, [ctypes.POINTER(PositionBiasParams), vp]),
     "af3_position_bias_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(PositionBiasParams)]),
+    "af3_rotary_embedding": (ctypes.c_int, [ctypes.POINTER(RotaryParams), vp]),
+    "af3_residual_norm_forward": (ctypes.c_int, [ctypes.POINTER(ResidualNormParams), vp]),
+    "af3_residual_norm_backward": (ctypes.c_int, [ctypes.POINTER(ResidualNormParams), ctypes.POINTER(ResidualNormGrads), vp]),
+    "af3_residual_norm_backward_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(ResidualNormParams), ctypes.POINTER(ResidualNormGrads)]),
     "af3_convert": (ctypes.c_int, [vp, i32, vp, i32, i64, vp]),
     "af3_amax": (ctypes.c_int, [vp, i32, i64, vp, vp]),
     "af3_quantize_fp8_e4m3": (ctypes.c_int, [vp, i32, vp, i64, i64, i64, i32, i64, i64, f32, vp, vp, vp, vp]),

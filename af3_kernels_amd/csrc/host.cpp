@@ -985,6 +985,275 @@ PyObject* py_position_bias(PyObject*, PyObject* const* a, Py_ssize_t n) {
 	return answer(rc, std::move(out));
 	END_HANDLE_TH_ERRORS
 }
+// ---- rotary positions ------------------------------------------------------------------------------------------------------------
+PyObject* pair(Tensor&& a, Tensor&& b) {   // (an undefined tensor: None)
+	PyObject* const x = a.defined() ? wrap(std::move(a)) : Py_NewRef(Py_None);
+	PyObject* const y = b.defined() ? wrap(std::move(b)) : Py_NewRef(Py_None);
+	PyObject* const t = PyTuple_New(2);
+	PyTuple_SET_ITEM(t, 0, x), PyTuple_SET_ITEM(t, 1, y);
+	return t;
+}
+struct rotary_call {
+	Tensor  frequencies, positions;   // positions [L] or [1|B, L] or undefined
+	int64_t offset;
+	bool    interleaved;
+	double  scale;
+	// x[i] [B, heads, L, D], undefined: none; out[i] likewise
+	int run(const Tensor (&x)[2], Tensor (&out)[2], bool inverse) const {
+		af3_rotary_params p{};
+		int               n = 0, dev = 0;
+		for(int i = 0; i < 2; i++) {
+			if(!x[i].defined()) continue;
+			dev    = (int)x[i].get_device();
+			out[i] = new_tensor(x[i].sizes(), x[i].scalar_type(), dev);
+			p.x[n] = x[i].const_data_ptr(), p.out[n] = out[i].data_ptr(), p.heads[n] = x[i].size(1);
+			put_strides(p.x_stride[n], x[i]), put_strides(p.out_stride[n], out[i]);
+			p.B = x[i].size(0), p.L = x[i].size(2), p.D = x[i].size(3), p.dtype = dtype_code(x[i]);
+			n++;
+		}
+		p.frequencies = frequencies.const_data_ptr<double>(), p.rotary = 2 * frequencies.size(0);
+		if(positions.defined()) p.positions = positions.const_data_ptr<int64_t>(), p.position_stride_b = positions.dim() > 1 && positions.size(0) != 1 ? positions.stride(0) : 0;
+		p.offset = offset, p.interleaved = interleaved, p.inverse = inverse, p.scale = (float)scale;
+		return af3_rotary_embedding(&p, current_stream(dev));
+	}
+};
+struct rotary_function : torch::autograd::Function<rotary_function> {
+	static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k, const Tensor& frequencies,
+												  const std::optional<Tensor>& positions, int64_t offset, bool interleaved, double scale) {
+		const Tensor x[2] = {q, k.value_or(Tensor())};
+		Tensor       out[2];
+		raise(rotary_call{frequencies, positions.value_or(Tensor()), offset, interleaved, scale}.run(x, out, false), "af3_rotary_embedding");
+		ctx->save_for_backward({frequencies, positions.value_or(Tensor())});
+		ctx->saved_data["offset"] = offset, ctx->saved_data["interleaved"] = interleaved, ctx->saved_data["scale"] = scale;
+		ctx->set_materialize_grads(false);
+		if(!out[1].defined()) return {out[0]};
+		return {out[0], out[1]};
+	}
+	static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_out) {
+		torch::autograd::variable_list grads(7);
+		for(const Tensor& g : grad_out) no_tangent(g, "the gradient of rotary_embedding");
+		{
+			at::AutoGradMode none(false);
+			const auto       saved = ctx->get_saved_variables();
+			Tensor           g[2], out[2];
+			for(size_t i = 0; i < grad_out.size(); i++)
+				if(grad_out[i].defined() && ctx->needs_input_grad(i)) g[i] = inner_1(grad_out[i]) ? grad_out[i] : grad_out[i].contiguous();
+			if(g[0].defined() || g[1].defined())
+				raise(rotary_call{saved[0], saved[1], ctx->saved_data["offset"].toInt(), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["scale"].toDouble()}.run(g, out, true), "af3_rotary_embedding");
+			grads[0] = out[0], grads[1] = out[1];
+		}
+		return once(std::move(grads), "rotary_embedding");
+	}
+};
+bool number_of(PyObject* o, int64_t& n) {
+	if(!PyLong_CheckExact(o)) return false;
+	n = PyLong_AsLongLong(o);
+	if(!PyErr_Occurred()) return true;
+	PyErr_Clear();
+	return false;
+}
+bool real_of(PyObject* o, double& x) {
+	if(!PyFloat_CheckExact(o)) return false;
+	x = PyFloat_AS_DOUBLE(o);
+	return true;
+}
+bool truth_of(PyObject* o, bool& x) {
+	x = o == Py_True;
+	return o == Py_True || o == Py_False;
+}
+// rotary(q, k or None, frequencies, positions or None, offset, interleaved, scale): (q, k or None) turned
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+	HANDLE_TH_ERRORS
+	if(n != 7) return none();
+	const Tensor *q = tensor_of(a[0]), *k = a[1] == Py_None ? nullptr : tensor_of(a[1]), *f = tensor_of(a[2]);
+	const int     dev = device_of(q);
+	if(dev < 0 || (!k && a[1] != Py_None) || !f || q->dim() != 4 || q->numel() == 0 || dtype_code(*q) < 0 || !inner_1(*q)) return none();
+	if(k && (!on_device(*k, dev) || k->dim() != 4 || k->scalar_type() != q->scalar_type() || k->size(0) != q->size(0) || k->size(2) != q->size(2) || k->size(3) != q->size(3) || k->numel() == 0 || !inner_1(*k)))
+		return none();
+	if(!on_device(*f, dev) || f->dim() != 1 || f->scalar_type() != at::kDouble || !f->is_contiguous() || f->requires_grad() || f->size(0) < 1 || 2 * f->size(0) > q->size(3) || q->size(3) > AF3_ROTARY_MAX_HEAD_DIM) return none();
+	rotary_call c{*f, Tensor(), 0, false, 1.0};
+	if(a[3] != Py_None) {
+		const Tensor* t = tensor_of(a[3]);
+		if(!t || !on_device(*t, dev) || t->scalar_type() != at::kLong || (t->dim() != 1 && t->dim() != 2) || t->size(-1) != q->size(2) || !inner_1(*t) || (t->dim() == 2 && t->size(0) != 1 && t->size(0) != q->size(0))) return none();
+		c.positions = *t;
+	}
+	if(!number_of(a[4], c.offset) || !truth_of(a[5], c.interleaved) || !real_of(a[6], c.scale) || !std::isfinite((float)c.scale) || c.offset > ((int64_t)1 << 62) || c.offset < -((int64_t)1 << 62) || has_tangent({q, k, f})) return none();
+	const Tensor x[2] = {*q, k ? *k : Tensor()};
+	Tensor       out[2];
+	int          rc = AF3_OK;
+	{
+		without_gil g;
+		if(wants_grad({q, k})) {
+			check_capture({q, k}, dev);
+			auto r = rotary_function::apply(x[0], given(x[1]), c.frequencies, given(c.positions), c.offset, c.interleaved, c.scale);
+			out[0] = r[0];
+			if(r.size() > 1) out[1] = r[1];
+		} else rc = c.run(x, out, false);
+	}
+	return rc == AF3_OK ? pair(std::move(out[0]), std::move(out[1])) : PyLong_FromLong(rc);
+	END_HANDLE_TH_ERRORS
+}
+
+// ---- norms around a block ----------------------------------------------------------------------------------------------------------
+// the distance of a tensor's rows [.., C] where they are equally far apart, -1 otherwise
+int64_t row_stride(const Tensor& t) {
+	int64_t stride = -1, behind = 1;   // of the axes seen so far, from the last; rows behind this axis
+	for(int64_t i = t.dim() - 2; i >= 0; i--) {
+		if(t.size(i) == 1) continue;
+		if(stride < 0) stride = t.stride(i);
+		else if(t.stride(i) != stride * behind) return -1;
+		behind *= t.size(i);
+	}
+	return stride < 0 ? t.size(-1) : stride;
+}
+struct norm_call {
+	Tensor  x, y, gate, weight, bias, post_weight;
+	int64_t norm, post_norm, sigmoid;
+	double  scale, eps;
+	// how a parameter's rows go with those of y; -1: not as the kernels take them
+	static int share(const Tensor& t, const Tensor& y, int64_t& group) {
+		if(!t.defined()) return AF3_SHARE_NONE;
+		const int64_t C = y.size(-1), rows = y.numel() / C;
+		if(!t.is_contiguous() || t.size(-1) != C) return -1;
+		if(t.numel() == C) return t.dim() == 1 || t.dim() == y.dim() ? AF3_SHARE_CHANNEL : -1;
+		if(t.dim() != y.dim()) return -1;
+		int64_t i = 0, each = 1;
+		while(i < y.dim() - 1 && t.size(i) == y.size(i)) i++;
+		for(; i < y.dim() - 1; i++) {
+			if(t.size(i) != 1) return -1;
+			each *= y.size(i);
+		}
+		if(each == 1) return AF3_SHARE_ROW;
+		if(each == rows) return AF3_SHARE_CHANNEL;
+		if(group != 0 && group != each) return -1;
+		group = each;
+		return AF3_SHARE_GROUP;
+	}
+	bool block(af3_residual_norm_params& p) const {
+		p   = af3_residual_norm_params{};
+		p.C = y.size(-1), p.rows = y.numel() / p.C;
+		p.y = y.const_data_ptr(), p.y_stride = row_stride(y);
+		if(x.defined()) p.x = x.const_data_ptr(), p.x_stride = row_stride(x);
+		const Tensor* const of[3] = {&gate, &weight, &bias};
+		const void**        to[3] = {&p.gate, &p.weight, &p.bias};
+		int32_t*            shares[3] = {&p.gate_share, &p.weight_share, &p.bias_share};
+		for(int i = 0; i < 3; i++) {
+			if((*shares[i] = share(*of[i], y, p.group)) < 0) return false;
+			if(of[i]->defined()) *to[i] = of[i]->const_data_ptr();
+		}
+		if(post_weight.defined()) {
+			if(post_weight.dim() != 1 || post_weight.size(0) != p.C || !post_weight.is_contiguous()) return false;
+			p.post_weight = post_weight.const_data_ptr();
+		}
+		p.norm = (int32_t)norm, p.post_norm = (int32_t)post_norm, p.gate_sigmoid = (int32_t)sigmoid, p.dtype = dtype_code(y);
+		p.eps = (float)eps, p.residual_scale = (float)scale;
+		return p.y_stride >= 0 && p.x_stride >= 0;
+	}
+	int forward(Tensor& out, Tensor& normed, Tensor* stats) const {
+		const int                dev = (int)y.get_device();
+		af3_residual_norm_params p;
+		if(!block(p)) return AF3_ERR_BAD_ARGUMENT;
+		out = new_tensor(y.sizes(), y.scalar_type(), dev), p.out = out.data_ptr();
+		if(norm != AF3_NORM_NONE) normed = new_tensor(y.sizes(), y.scalar_type(), dev), p.normed = normed.data_ptr();
+		if(stats) *stats = new_tensor({p.rows, 4}, at::kFloat, dev), p.stats = static_cast<float*>(stats->data_ptr());
+		return af3_residual_norm_forward(&p, current_stream(dev));
+	}
+};
+struct norm_function : torch::autograd::Function<norm_function> {
+	static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const std::optional<Tensor>& x, const Tensor& y, const std::optional<Tensor>& weight,
+												  const std::optional<Tensor>& bias, const std::optional<Tensor>& gate, const std::optional<Tensor>& post_weight, std::vector<int64_t> kinds,
+												  double scale, double eps) {
+		const norm_call c{x.value_or(Tensor()), y, gate.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor()), post_weight.value_or(Tensor()), kinds[0], kinds[1], kinds[2], scale, eps};
+		Tensor          out, normed, stats;
+		raise(c.forward(out, normed, &stats), "af3_residual_norm_forward");
+		ctx->save_for_backward({c.x, y, c.weight, c.bias, c.gate, c.post_weight, stats});
+		ctx->saved_data["kinds"] = std::move(kinds), ctx->saved_data["scale"] = scale, ctx->saved_data["eps"] = eps;
+		ctx->set_materialize_grads(false);
+		if(!normed.defined()) return {out};
+		return {out, normed};
+	}
+	static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_out) {
+		torch::autograd::variable_list grads(9);
+		for(const Tensor& g : grad_out) no_tangent(g, "the gradient of residual_norm");
+		{
+			at::AutoGradMode none(false);
+			const auto       saved = ctx->get_saved_variables();
+			const auto       kinds = ctx->saved_data["kinds"].toIntVector();
+			const norm_call  c{saved[0], saved[1], saved[4], saved[2], saved[3], saved[5], kinds[0], kinds[1], kinds[2], ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble()};
+			const int        dev = (int)c.y.get_device();
+			af3_residual_norm_params p;
+			af3_residual_norm_grads  o{};
+			raise(c.block(p) ? AF3_OK : AF3_ERR_BAD_ARGUMENT, "af3_residual_norm_backward");
+			p.stats = static_cast<float*>(saved[6].data_ptr());
+			Tensor g[2];
+			for(size_t i = 0; i < grad_out.size(); i++)
+				if(grad_out[i].defined()) g[i] = inner_1(grad_out[i]) && row_stride(grad_out[i]) >= 0 ? grad_out[i] : grad_out[i].contiguous();
+			if(g[0].defined()) o.grad_out = g[0].const_data_ptr(), o.grad_out_stride = row_stride(g[0]);
+			if(g[1].defined()) o.grad_normed = g[1].const_data_ptr(), o.grad_normed_stride = row_stride(g[1]);
+			bool   any  = false;
+			size_t edge = 0;   // (tensors that were not given have none)
+			auto want = [&](int i, const Tensor& like, bool reached) -> void* {
+				if(!like.defined() || !ctx->needs_input_grad(edge++)) return nullptr;
+				grads[i] = new_tensor(like.sizes(), like.scalar_type(), dev);
+				if(!reached) {
+					grads[i].zero_();
+					return nullptr;
+				}
+				any = true;
+				return grads[i].data_ptr();
+			};
+			o.grad_x = want(0, c.x, true), o.grad_y = want(1, c.y, true), o.grad_weight = want(2, c.weight, g[1].defined()), o.grad_bias = want(3, c.bias, g[1].defined());
+			o.grad_gate = want(4, c.gate, true), o.grad_post_weight = want(5, c.post_weight, true);
+			if(any && (g[0].defined() || g[1].defined())) {
+				const int64_t bytes = af3_residual_norm_backward_workspace_bytes(&p, &o);
+				raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_residual_norm_backward_workspace_bytes");
+				at::DataPtr ws;
+				if(bytes > 0) ws = new_scratch(bytes), o.workspace = ws.get(), o.workspace_bytes = bytes;
+				raise(af3_residual_norm_backward(&p, &o, current_stream(dev)), "af3_residual_norm_backward");
+			}
+		}
+		return once(std::move(grads), "residual_norm");
+	}
+};
+// residual_norm(x or None, y, weight, bias, gate, post_weight, norm, post_norm, sigmoid, residual_scale, eps): (out, normed or None)
+PyObject* py_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+	HANDLE_TH_ERRORS
+	if(n != 11) return none();
+	const Tensor* y   = tensor_of(a[1]);
+	const int     dev = device_of(y);
+	if(dev < 0 || y->dim() < 1 || y->numel() == 0 || dtype_code(*y) < 0 || !inner_1(*y) || y->size(-1) > AF3_RESIDUAL_NORM_MAX_CHANNELS) return none();
+	norm_call c{Tensor(), *y, Tensor(), Tensor(), Tensor(), Tensor(), 0, 0, 0, 1.0, 0.0};
+	Tensor*   to[5] = {&c.x, &c.weight, &c.bias, &c.gate, &c.post_weight};
+	const int from[5] = {0, 2, 3, 4, 5};
+	for(int i = 0; i < 5; i++) {
+		if(a[from[i]] == Py_None) continue;
+		const Tensor* t = tensor_of(a[from[i]]);
+		if(!t || !on_device(*t, dev) || t->scalar_type() != y->scalar_type() || t->dim() < 1 || t->numel() == 0 || !inner_1(*t)) return none();
+		*to[i] = *t;
+	}
+	bool sigmoid;
+	if(!number_of(a[6], c.norm) || !number_of(a[7], c.post_norm) || !truth_of(a[8], sigmoid) || !real_of(a[9], c.scale) || !real_of(a[10], c.eps)) return none();
+	c.sigmoid = sigmoid;
+	if(c.norm < 0 || c.norm > 2 || c.post_norm < 0 || c.post_norm > 2 || (c.norm == 0 && (c.weight.defined() || c.bias.defined())) || (c.post_norm == 0 && c.post_weight.defined()) || (sigmoid && !c.gate.defined())) return none();
+	if(!(c.eps >= 0.0) || !std::isfinite((float)c.eps) || !std::isfinite((float)c.scale) || (c.x.defined() && c.x.sizes() != y->sizes()) || has_tangent({&c.x, y, &c.weight, &c.bias, &c.gate, &c.post_weight})) return none();
+	af3_residual_norm_params p;
+	if(!c.block(p)) return none();   // (parameters or strides that the Python side lays out anew, or refuses)
+	Tensor out, normed;
+	int    rc = AF3_OK;
+	{
+		without_gil g;
+		const std::initializer_list<const Tensor*> all = {&c.x, &c.y, &c.weight, &c.bias, &c.gate, &c.post_weight};
+		if(wants_grad(all)) {
+			check_capture(all, dev);
+			auto r = norm_function::apply(given(c.x), c.y, given(c.weight), given(c.bias), given(c.gate), given(c.post_weight), std::vector<int64_t>{c.norm, c.post_norm, c.sigmoid}, c.scale, c.eps);
+			out = r[0];
+			if(r.size() > 1) normed = r[1];
+		} else rc = c.forward(out, normed, nullptr);
+	}
+	return rc == AF3_OK ? pair(std::move(out), std::move(normed)) : PyLong_FromLong(rc);
+	END_HANDLE_TH_ERRORS
+}
+
 // check_capture(tensor or None...): raises where a gradient of these cannot be captured
 PyObject* py_check_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
 	HANDLE_TH_ERRORS
@@ -1010,6 +1279,8 @@ PyMethodDef methods[] = {
 	AF3_FN(gated_linear_unit, "gated_linear_unit(x, weight, tag)"),
 	AF3_FN(cross_attention, "cross_attention(q, k, v, mask, bias, scale)"),
 	AF3_FN(position_bias, "position_bias(table, q_len, k_len, scheme, bidirectional, max_distance, q_positions, k_positions, q_offset)"),
+	AF3_FN(rotary, "rotary(q, k, frequencies, positions, offset, interleaved, scale)"),
+	AF3_FN(residual_norm, "residual_norm(x, y, weight, bias, gate, post_weight, norm, post_norm, sigmoid, residual_scale, eps)"),
 	AF3_FN(check_capture, "check_capture(tensor...): raises where their gradients cannot be captured into a graph"),
 	AF3_FN(remember, "remember(tag, value, source...): a matrix derived from weights"),
 	AF3_FN(recalls, "recalls(tag, source...): whether one is remembered for these"),

@@ -1,0 +1,351 @@
+"""What a layer around its attention is made of, beside the attention calls themselves.
+
+    rotary_frequencies, rotary_embedding   positions as turns of the pairs of a head, instead of a bias
+    residual_norm                          the end of one block and the beginning of the next: norm, gate, residual stream, norm
+
+Both work under autograd (first derivatives).  The reference has neither; its LayerNorm is torch's (src/af3_kernels/Attention.py:51).  Every computation on
+the device happens in libaf3_dpa.so (af3_rotary_embedding, af3_residual_norm_*); there is no CPU path.
+"""
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib, ops
+from ._lib import ResidualNormGrads, ResidualNormParams, RotaryParams
+from .cross import _DTYPES, _inner_contig, _no_tangents, _same_device
+
+_host = ops._host
+_i64x3 = ctypes.c_int64 * 3
+_LIMIT = 3.4028234663852886e38   # the largest float32
+
+
+def _finite(x, name):
+    x = float(x)
+    if not abs(x) <= _LIMIT:
+        raise ValueError(f"{name} must be finite in float32, got {x}")
+    return x
+
+
+# ---- rotary positions -----------------------------------------------------------------------------------------------------
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_length: int = 0, beta_fast: float = 32.0,
+                       beta_slow: float = 1.0, device=None) -> Tuple[torch.Tensor, float]:
+    """(frequencies, scale) for rotary_embedding: float64 [rotary_dim // 2], radians per position, and what the turned elements are multiplied with.
+
+    Pair i turns with base^(-2 i / rotary_dim).  For contexts longer than the trained ones:
+    "linear": all frequencies divided by `factor`; "ntk": base * factor^(rotary_dim / (rotary_dim - 2)) in place of base (the slowest pair is slowed by `factor`, the
+    fastest not at all); "yarn": pairs that turn more than beta_fast times within original_length keep their frequency, those that turn less than beta_slow times
+    have it divided by `factor`, a ramp in between, and scale = 0.1 log(factor) + 1.  To be made once and kept (host arithmetic and one copy to the device)."""
+    n = int(rotary_dim)
+    if n < 2 or n % 2 or n > _lib.ROTARY_MAX_HEAD_DIM:
+        raise ValueError(f"rotary_dim must be even, 2 to {_lib.ROTARY_MAX_HEAD_DIM}, got {rotary_dim}")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling must be 'none', 'linear', 'ntk' or 'yarn', got {scaling!r}")
+    base, factor = float(base), float(factor)
+    if not 1.0 < base < math.inf:
+        raise ValueError(f"base must be above 1 and finite, got {base}")
+    if not 1.0 <= factor < math.inf:
+        raise ValueError(f"factor must be at least 1 and finite, got {factor}")
+    if scaling == "none" and factor != 1.0:
+        raise ValueError("a factor belongs to a scaling: 'linear', 'ntk' or 'yarn'")
+    scale = 1.0
+    if scaling == "ntk":
+        if n == 2:
+            raise ValueError("scaling 'ntk' needs a rotary_dim of at least 4")
+        base *= factor ** (n / (n - 2))
+    frequencies = [base ** (-2.0 * i / n) for i in range(n // 2)]
+    if scaling == "linear":
+        frequencies = [f / factor for f in frequencies]
+    elif scaling == "yarn":
+        if int(original_length) < 1:
+            raise ValueError(f"scaling 'yarn' needs the trained length as original_length, got {original_length}")
+        if not 0.0 < beta_slow < beta_fast < math.inf:
+            raise ValueError(f"beta_fast must be above beta_slow and both positive, got {beta_fast} and {beta_slow}")
+
+        def pair_of(turns):   # the pair that turns so often within original_length (a real number)
+            return n * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+        low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), n - 1)
+        for i, f in enumerate(frequencies):
+            slowed = min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0)
+            frequencies[i] = f / factor * slowed + f * (1.0 - slowed)
+        scale = 0.1 * math.log(factor) + 1.0
+    return torch.tensor(frequencies, dtype=torch.float64, device=device), scale
+
+
+def _turn(tensors, frequencies, positions, offset, interleaved, scale, inverse):
+    """The tensors [B, heads, L, D] (None: left out) turned, in one launch."""
+    p, outs, n = RotaryParams(), [], 0
+    for t in tensors:
+        if t is None or t.numel() == 0:
+            outs.append(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device))
+            continue
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        p.x[n], p.out[n], p.heads[n] = t.data_ptr(), out.data_ptr(), t.shape[1]
+        p.x_stride[n], p.out_stride[n] = _i64x3(*t.stride()[:3]), _i64x3(*out.stride()[:3])
+        p.B, p.L, p.D, p.dtype = t.shape[0], t.shape[2], t.shape[3], _DTYPES[t.dtype]
+        outs.append(out)
+        n += 1
+    if n:
+        p.frequencies, p.rotary = frequencies.data_ptr(), 2 * frequencies.shape[0]
+        if positions is not None:
+            p.positions, p.position_stride_b = positions.data_ptr(), 0 if positions.dim() == 1 or positions.shape[0] == 1 else positions.stride(0)
+        p.offset, p.interleaved, p.inverse, p.scale = offset, int(interleaved), int(inverse), scale
+        with ops._on_device(frequencies.device):
+            _lib.check(_lib.load().af3_rotary_embedding(ctypes.byref(p), ops._stream_ptr(frequencies.device)), "af3_rotary_embedding")
+    return outs
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, frequencies, positions, offset, interleaved, scale):
+        ctx.save_for_backward(frequencies, positions)
+        ctx.settings = (offset, interleaved, scale)
+        ctx.set_materialize_grads(False)
+        return tuple(_turn((q, k), frequencies, positions, offset, interleaved, scale, False))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        _no_tangents("the gradient of rotary_embedding", *grads)
+        frequencies, positions = ctx.saved_tensors
+        grads = [_inner_contig(g) if g is not None and need else None for g, need in zip(grads, ctx.needs_input_grad)]
+        return (*_turn(grads, frequencies, positions, *ctx.settings, True), None, None, None, None, None)
+
+
+def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], frequencies: torch.Tensor, positions: Optional[torch.Tensor] = None, offset: int = 0,
+                     interleaved: bool = False, scale: float = 1.0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Queries and keys with their positions: (q, k) with every pair of elements turned by position * frequency.
+
+    q [B, H, L, D] and k [B, Hkv, L, D] (or None), float32 or bfloat16 (k is cast to q's dtype), any strides, D up to 1024.  The first
+    n = 2 * len(frequencies) <= D elements of a head are turned, the others are handed through: pair i is elements (i, i + n / 2), or (2 i, 2 i + 1) if `interleaved`,
+        (x, y) -> scale * (x cos a - y sin a, x sin a + y cos a),  a = position * frequencies[i]
+    with angles in 64 bits, the rest in fp32, one rounding at the end.  frequencies, scale: from rotary_frequencies, or any float64 [n / 2] (float32 is cast).  Positions are
+    offset, offset + 1, ... (a decoder's token t: L = 1, offset = t), or what `positions` holds: [L], or [B, L] for rows at positions of their own
+    (int64 or int32).  New contiguous tensors; (q, None) without k.
+
+    Gradients flow to q and k (turned back), not to frequencies, which must not ask for one; a second derivative and forward mode raise.  In a HIP graph: as
+    cross_attention."""
+    out = _host.rotary(q, k, frequencies, positions, offset, interleaved, scale)
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_rotary_embedding")
+    _no_tangents("rotary_embedding", q, k, frequencies)
+    _same_device(q, k, frequencies, positions)
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
+        raise ValueError(f"q must be [B, H, L, D] and k [B, Hkv, L, D], got {tuple(q.shape)} and {None if k is None else tuple(k.shape)}")
+    if q.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {q.dtype}: float32 or bfloat16")
+    B, _, L, D = q.shape
+    if not 2 <= D <= _lib.ROTARY_MAX_HEAD_DIM:
+        raise ValueError(f"head_dim must be 2 to {_lib.ROTARY_MAX_HEAD_DIM}, got {D}")
+    if frequencies.dim() != 1 or frequencies.dtype not in (torch.float64, torch.float32) or not 2 <= 2 * frequencies.shape[0] <= D:
+        raise ValueError(f"frequencies must be float64 or float32 [n / 2] with n of 2 to head_dim {D}, got {frequencies.dtype} {tuple(frequencies.shape)}")
+    if frequencies.requires_grad:
+        raise ValueError("frequencies have no gradient here: detach them")
+    if positions is not None and (positions.dtype not in (torch.int64, torch.int32) or positions.dim() not in (1, 2) or positions.shape[-1] != L
+                                  or (positions.dim() == 2 and positions.shape[0] not in (1, B))):
+        raise ValueError(f"positions must be int64 or int32 [L] or [B, L] with B={B}, L={L}, got {positions.dtype} {tuple(positions.shape)}")
+    offset, interleaved, scale = int(offset), bool(interleaved), _finite(scale, "scale")
+    if abs(offset) > 1 << 62:
+        raise ValueError(f"offset must lie within 2^62, got {offset}")
+    q, frequencies = _inner_contig(q), frequencies.to(torch.float64).contiguous()
+    k = None if k is None else _inner_contig(k if k.dtype == q.dtype else k.to(q.dtype))
+    positions = None if positions is None else _inner_contig(positions.to(torch.int64))
+    with ops._on_device(q.device):   # (as a plain call)
+        out = _host.rotary(q, k, frequencies, positions, offset, interleaved, scale)
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_rotary_embedding")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        with ops._on_device(q.device):
+            _host.check_capture(q, k)
+        return _Rotary.apply(q, k, frequencies, positions, offset, interleaved, scale)
+    return tuple(_turn((q, k), frequencies, positions, offset, interleaved, scale, False))
+
+
+# ---- norms around a block ---------------------------------------------------------------------------------------------------
+def _row_stride(t):
+    """The distance of a tensor's rows [.., C] where they are equally far apart, None otherwise."""
+    stride, behind = None, 1
+    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if stride is None:
+            stride = step
+        elif step != stride * behind:
+            return None
+        behind *= size
+    return t.shape[-1] if stride is None else stride
+
+
+def _rows(t):
+    return t if t is None or (t.stride(-1) == 1 and _row_stride(t) is not None) else t.contiguous()
+
+
+def _shared_by(t, y):
+    """How many consecutive rows of y a row of the parameter t is for: all of them, some, 1; None: not a parameter for y, or one that is repeated otherwise."""
+    rows, lead = y.numel() // y.shape[-1], t.shape[:-1]
+    if t.dim() == 1 or (t.dim() == y.dim() and t.numel() == t.shape[-1]):
+        return rows
+    if t.dim() != y.dim():
+        return None
+    i = 0
+    while i < len(lead) and lead[i] == y.shape[i]:
+        i += 1
+    return math.prod(y.shape[i:-1]) if all(n == 1 for n in lead[i:]) else None
+
+
+def _norm_block(x, y, weight, bias, gate, post_weight, kinds, scale, eps) -> ResidualNormParams:
+    p = ResidualNormParams()
+    p.C, p.rows = y.shape[-1], y.numel() // y.shape[-1]
+    p.y, p.y_stride = y.data_ptr(), _row_stride(y)
+    if x is not None:
+        p.x, p.x_stride = x.data_ptr(), _row_stride(x)
+    for name, t in (("gate", gate), ("weight", weight), ("bias", bias)):
+        if t is not None:
+            each = _shared_by(t, y)
+            share = _lib.SHARE_CHANNEL if t.dim() == 1 or each == p.rows else _lib.SHARE_ROW if each == 1 else _lib.SHARE_GROUP
+            if share == _lib.SHARE_GROUP:
+                p.group = each
+            setattr(p, name, t.data_ptr())
+            setattr(p, name + "_share", share)
+    if post_weight is not None:
+        p.post_weight = post_weight.data_ptr()
+    p.norm, p.post_norm, p.gate_sigmoid = kinds
+    p.dtype, p.eps, p.residual_scale = _DTYPES[y.dtype], eps, scale
+    return p
+
+
+def _norm_forward(x, y, weight, bias, gate, post_weight, kinds, scale, eps, want_stats):
+    out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    normed = torch.empty_like(out) if kinds[0] else None
+    if y.numel() == 0:
+        return out, normed, None
+    stats = torch.empty(y.numel() // y.shape[-1], 4, dtype=torch.float32, device=y.device) if want_stats else None
+    p = _norm_block(x, y, weight, bias, gate, post_weight, kinds, scale, eps)
+    p.out, p.normed, p.stats = out.data_ptr(), 0 if normed is None else normed.data_ptr(), 0 if stats is None else stats.data_ptr()
+    with ops._on_device(y.device):
+        _lib.check(_lib.load().af3_residual_norm_forward(ctypes.byref(p), ops._stream_ptr(y.device)), "af3_residual_norm_forward")
+    return out, normed, stats
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, weight, bias, gate, post_weight, kinds, scale, eps):
+        out, normed, stats = _norm_forward(x, y, weight, bias, gate, post_weight, kinds, scale, eps, True)
+        ctx.save_for_backward(x, y, weight, bias, gate, post_weight, stats)
+        ctx.settings = (kinds, scale, eps)
+        ctx.set_materialize_grads(False)
+        return out, normed
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out, grad_normed):
+        _no_tangents("the gradient of residual_norm", grad_out, grad_normed)
+        *tensors, stats = ctx.saved_tensors
+        y = tensors[1]
+        # (without a gradient of the normed rows those of weight and bias are zeros)
+        reached = (grad_out is not None or grad_normed is not None, grad_normed is not None)
+        grads = [None if t is None or not need else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t, need in zip(tensors, ctx.needs_input_grad)]
+        for i, g in enumerate(grads):
+            if g is not None and (stats is None or not reached[i in (2, 3)]):
+                g.zero_()
+        wanted = [g if stats is not None and reached[i in (2, 3)] else None for i, g in enumerate(grads)]
+        if any(g is not None for g in wanted):
+            p, o = _norm_block(*tensors, *ctx.settings), ResidualNormGrads()
+            p.stats = stats.data_ptr()
+            grad_out, grad_normed = _rows(grad_out), _rows(grad_normed)
+            if grad_out is not None:
+                o.grad_out, o.grad_out_stride = grad_out.data_ptr(), _row_stride(grad_out)
+            if grad_normed is not None:
+                o.grad_normed, o.grad_normed_stride = grad_normed.data_ptr(), _row_stride(grad_normed)
+            o.grad_x, o.grad_y, o.grad_weight, o.grad_bias, o.grad_gate, o.grad_post_weight = (0 if g is None else g.data_ptr() for g in wanted)
+            lib = _lib.load()
+            with ops._on_device(y.device):
+                need = lib.af3_residual_norm_backward_workspace_bytes(ctypes.byref(p), ctypes.byref(o))
+                _lib.check(min(need, 0), "af3_residual_norm_backward_workspace_bytes")
+                ws = torch.empty(max(need, 16), dtype=torch.uint8, device=y.device)
+                o.workspace, o.workspace_bytes = ws.data_ptr(), need
+                _lib.check(lib.af3_residual_norm_backward(ctypes.byref(p), ctypes.byref(o), ops._stream_ptr(y.device)), "af3_residual_norm_backward")
+        return (*grads, None, None, None)
+
+
+def residual_norm(x: Optional[torch.Tensor], y: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                  post_weight: Optional[torch.Tensor] = None, norm: str = "rms", post_norm: str = "none", gate_activation: str = "none", residual_scale: float = 1.0,
+                  eps: float = 1e-5) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The end of one block and the beginning of the next in one pass: (out, normed) with
+        out    = residual_scale * x + gate * post_norm(y) * post_weight
+        normed = norm(out) * weight + bias
+    x: the residual stream [.., C] (None: no stream); y: the block's result [.., C].  norm, post_norm: "rms", "layer" (biased variance) or "none"; norm="none" gives
+    (out, None).  A norm alone is residual_norm(None, y, post_weight=w, post_norm="rms", norm="none")[0].  gate_activation="sigmoid" takes the logistic function of the gate.
+
+    gate, weight and bias are [C], or have y's number of axes with 1 where they are repeated: [B, 1, C] for all tokens of a sequence, [B, T, C] for
+    every token (a conditioned transformer's), [C] for all.  post_weight [C].  One left out counts as ones (a bias as zeros).  float32 or bfloat16, everything else cast to y's
+    dtype; arithmetic in fp32, out and normed rounded once each (normed is made of out before its rounding).  C up to 16384; x, y: any strides.  New contiguous tensors.
+
+    Gradients flow to all tensors (the same bits every time); a second derivative and forward mode raise.  In a HIP graph: as cross_attention."""
+    kinds = _lib.NORMS.get(norm, -1), _lib.NORMS.get(post_norm, -1), gate_activation == "sigmoid"
+    out = _host.residual_norm(x, y, weight, bias, gate, post_weight, *kinds, residual_scale, eps) if gate_activation in ("none", "sigmoid") else None
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_residual_norm_forward")
+    _no_tangents("residual_norm", x, y, weight, bias, gate, post_weight)
+    _same_device(y, x, weight, bias, gate, post_weight)
+    if y.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {y.dtype}: float32 or bfloat16")
+    for name, kind in (("norm", norm), ("post_norm", post_norm)):
+        if kind not in _lib.NORMS:
+            raise ValueError(f"{name} must be 'none', 'rms' or 'layer', got {kind!r}")
+    if gate_activation not in ("none", "sigmoid"):
+        raise ValueError(f"gate_activation must be 'none' or 'sigmoid', got {gate_activation!r}")
+    if y.dim() < 1 or not 1 <= y.shape[-1] <= _lib.RESIDUAL_NORM_MAX_CHANNELS:
+        raise ValueError(f"y must be [.., C] with C of 1 to {_lib.RESIDUAL_NORM_MAX_CHANNELS}, got {tuple(y.shape)}")
+    if x is not None and x.shape != y.shape:
+        raise ValueError(f"x must have y's shape {tuple(y.shape)}, got {tuple(x.shape)}")
+    if norm == "none" and (weight is not None or bias is not None):
+        raise ValueError("weight and bias belong to a norm, and norm is 'none'")
+    if post_norm == "none" and post_weight is not None:
+        raise ValueError("post_weight belongs to a post_norm, and post_norm is 'none'")
+    if gate_activation != "none" and gate is None:
+        raise ValueError("gate_activation needs a gate")
+    if post_weight is not None and tuple(post_weight.shape) != (y.shape[-1],):
+        raise ValueError(f"post_weight must be [C] with C={y.shape[-1]}, got {tuple(post_weight.shape)}")
+    C, shared = y.shape[-1], {}
+    for name, t in (("gate", gate), ("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.dim() < 1 or t.shape[-1] != C or not (t.dim() == 1 or (t.dim() == y.dim() and all(n in (1, m) for n, m in zip(t.shape, y.shape)))):
+            raise ValueError(f"{name} must be [C] or have y's axes, of y's sizes or 1, and C channels, got {tuple(t.shape)} for y {tuple(y.shape)}")
+        shared[name] = _shared_by(t, y)
+    residual_scale, eps = _finite(residual_scale, "residual_scale"), _finite(eps, "eps")
+    if eps < 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    # Parameters that are repeated along an axis in front of one they are not repeated along have a row for every row of y; of several lengths of repetition the shortest is taken for all.
+    rows = y.numel() // C
+    groups = [n for n in shared.values() if n is not None and 1 < n < rows]
+
+    def laid_out(name, t):
+        if t is None:
+            return None
+        if t.dtype != y.dtype:
+            t = t.to(y.dtype)
+        if name in shared:
+            if shared[name] is None:
+                t = t.expand(y.shape)
+            elif 1 < shared[name] < rows and shared[name] != min(groups):
+                size, each = list(t.shape), 1   # (as many of the last axes stay repeated as the shortest has)
+                for i in range(y.dim() - 2, -1, -1):
+                    if each >= min(groups):
+                        size[i] = y.shape[i]
+                    each *= y.shape[i]
+                t = t.expand(size)
+        return t.contiguous()
+    gate, weight, bias, post_weight = (laid_out(n, t) for n, t in (("gate", gate), ("weight", weight), ("bias", bias), ("post_weight", post_weight)))
+    y, x = _rows(y), None if x is None else _rows(x if x.dtype == y.dtype else x.to(y.dtype))
+    with ops._on_device(y.device):   # (as a plain call)
+        out = _host.residual_norm(x, y, weight, bias, gate, post_weight, *kinds, residual_scale, eps)
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_residual_norm_forward")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, weight, bias, gate, post_weight)):
+        with ops._on_device(y.device):
+            _host.check_capture(x, y, weight, bias, gate, post_weight)
+        return _ResidualNorm.apply(x, y, weight, bias, gate, post_weight, kinds, residual_scale, eps)
+    return _norm_forward(x, y, weight, bias, gate, post_weight, kinds, residual_scale, eps, False)[:2]

@@ -439,6 +439,95 @@ int     af3_position_bias_backward(const af3_position_bias_params* params, void*
 int64_t af3_position_bias_workspace_bytes(const af3_position_bias_params* params);   /* host only */
 
 /*
+ * Rotary positions of queries and keys in one launch: pair i of a head's first `rotary` elements is turned by position * frequencies[i],
+ *     (x, y) -> scale (x cos a - y sin a, x sin a + y cos a);   inverse: by -a, which is the gradient.
+ * The other elements go through as they are.  No reference counterpart.
+ *   x, out      : x[0] [B, heads[0], L, D] and, with heads[1] > 0, x[1] [B, heads[1], L, D], of `dtype` (AF3_BF16 or AF3_F32), element strides for the
+ *                 first three axes, innermost stride 1, any alignment of the element type.  out may be x itself (same strides); otherwise they may not overlap.
+ *   frequencies : rotary / 2 doubles (device memory), radians per position.
+ *   positions   : [L], or [B, L] with batch stride position_stride_b, any 64-bit numbers (device memory; exact below 2^53); NULL: offset + 0, 1, 2, ...
+ *   interleaved : pairs are elements (2 i, 2 i + 1); otherwise (i, i + rotary / 2).
+ * rotary even, 2 to D; D <= AF3_ROTARY_MAX_HEAD_DIM; heads[0] + heads[1] < 2^16, B * L < 2^30 (and B * L * D / 2 < 2^32); scale finite, |offset| <= 2^62.
+ */
+#define AF3_ROTARY_MAX_HEAD_DIM 1024
+typedef struct af3_rotary_params {
+	const void*    x[2];
+	void*          out[2];
+	const double*  frequencies;
+	const int64_t* positions;
+	int64_t        position_stride_b;
+	int64_t        offset;
+	int64_t        B, L, D, rotary;
+	int64_t        heads[2];
+	int64_t        x_stride[2][3];
+	int64_t        out_stride[2][3];
+	int32_t        dtype, interleaved, inverse;
+	float          scale;
+} af3_rotary_params;
+
+int af3_rotary_embedding(const af3_rotary_params* params, void* hip_stream);
+
+/*
+ * The end of one block and the beginning of the next, for every row of C channels:
+ *     z = post_norm(y) * post_weight,   out = residual_scale * x + act(gate) * z,   normed = norm(out) * weight + bias
+ * with norm(v) = v / sqrt(mean(v^2) + eps) (AF3_NORM_RMS), (v - mean(v)) / sqrt(var(v) + eps) (AF3_NORM_LAYER, biased variance) or, for post_norm, v itself
+ * (AF3_NORM_NONE; norm == AF3_NORM_NONE: no `normed`).  Everything between the inputs and the two roundings is fp32: normed is made of out before its rounding.
+ * No reference counterpart (src/af3_kernels/Attention.py:51-52 has its LayerNorm from torch).
+ *   x, y          : [rows, C] with row strides (inputs may repeat rows: 0), innermost stride 1, any alignment; x NULL: no residual stream.
+ *   gate, weight, bias : contiguous rows of C: one (AF3_SHARE_CHANNEL), one for every `group` consecutive rows (AF3_SHARE_GROUP, rows % group == 0), one per row
+ *                   (AF3_SHARE_ROW), or AF3_SHARE_NONE and NULL.  gate_sigmoid: act is the logistic function, otherwise the gate itself.
+ *   post_weight   : [C] or NULL; only with a post_norm.  weight, bias only with a norm.
+ *   out, normed   : [rows, C] contiguous.  out may be x itself where that is contiguous.
+ *   stats         : optional, [rows, 4] floats, 16-byte aligned, written for af3_residual_norm_backward.
+ * All tensors of `dtype`, AF3_BF16 or AF3_F32; C <= AF3_RESIDUAL_NORM_MAX_CHANNELS, rows < 2^30; eps >= 0 and residual_scale finite.
+ */
+#define AF3_RESIDUAL_NORM_MAX_CHANNELS 16384
+typedef enum af3_norm { AF3_NORM_NONE = 0, AF3_NORM_RMS = 1, AF3_NORM_LAYER = 2 } af3_norm;
+typedef enum af3_share { AF3_SHARE_NONE = 0, AF3_SHARE_CHANNEL = 1, AF3_SHARE_GROUP = 2, AF3_SHARE_ROW = 3 } af3_share;
+typedef struct af3_residual_norm_params {
+	const void* x;
+	const void* y;
+	const void* gate;
+	const void* weight;
+	const void* bias;
+	const void* post_weight;
+	void*       out;
+	void*       normed;
+	float*      stats;
+	int64_t     rows, C, group;
+	int64_t     x_stride, y_stride;
+	int32_t     gate_share, weight_share, bias_share;
+	int32_t     norm, post_norm, gate_sigmoid, dtype;
+	float       eps, residual_scale;
+	int32_t     reserved;
+} af3_residual_norm_params;
+
+int af3_residual_norm_forward(const af3_residual_norm_params* params, void* hip_stream);
+
+/*
+ * Gradients of af3_residual_norm_forward.  `params` as there, with the `stats` that it wrote; out and normed are not looked at.  grad_out, grad_normed [rows, C] with
+ * row strides, NULL: zeros (one of them at least; without grad_normed neither grad_weight nor grad_bias).  Results, contiguous, NULL: not wanted: grad_x, grad_y [rows, C]; grad_gate, grad_weight, grad_bias shaped like
+ * what they belong to; grad_post_weight [C].  Sums over rows in a fixed order: the same bits every time.
+ * workspace: af3_residual_norm_backward_workspace_bytes() bytes, 16-byte aligned; 0: none needed.
+ */
+typedef struct af3_residual_norm_grads {
+	const void* grad_out;
+	const void* grad_normed;
+	int64_t     grad_out_stride, grad_normed_stride;
+	void*       grad_x;
+	void*       grad_y;
+	void*       grad_gate;
+	void*       grad_weight;
+	void*       grad_bias;
+	void*       grad_post_weight;
+	void*       workspace;
+	int64_t     workspace_bytes;
+} af3_residual_norm_grads;
+
+int     af3_residual_norm_backward(const af3_residual_norm_params* params, const af3_residual_norm_grads* grads, void* hip_stream);
+int64_t af3_residual_norm_backward_workspace_bytes(const af3_residual_norm_params* params, const af3_residual_norm_grads* grads);   /* host only */
+
+/*
  * N-dimensional pad (ndim <= AF3_PAD_MAX_DIMS): copy src (shape src_shape, element strides
  * src_strides) into the low corner of a contiguous dst of shape dst_shape (>= src_shape in
  * every axis) and fill the rest with the 32-bit pattern `fill_bits` truncated to elem_size
