@@ -108,6 +108,26 @@ class ResidualNormGrads(ctypes.Structure):
     ]
 
 
+class DiffAttentionParams(ctypes.Structure):
+    """Mirror of struct af3_diff_attention_params."""
+    _fields_ = [
+        ("q", vp), ("k", vp), ("v", vp), ("lam", vp), ("key_mask", vp), ("out", vp), ("stats", vp), ("second", vp),
+        ("B", i64), ("H", i64), ("Hkv", i64), ("Lq", i64), ("Lk", i64), ("D", i64), ("Dv", i64),
+        ("q_stride", i64 * 3), ("k_stride", i64 * 3), ("v_stride", i64 * 3), ("out_stride", i64 * 3),
+        ("lam_stride", i64), ("key_mask_stride_b", i64), ("q_offset", i64),
+        ("dtype", i32), ("lam_dtype", i32), ("causal", i32), ("softmax_scale", f32),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class DiffAttentionGrads(ctypes.Structure):
+    """Mirror of struct af3_diff_attention_grads."""
+    _fields_ = [
+        ("grad_out", vp), ("grad_out_stride", i64 * 3), ("grad_q", vp), ("grad_k", vp), ("grad_v", vp), ("grad_lam", vp),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
 ROTARY_MAX_HEAD_DIM = 1024                 # AF3_ROTARY_MAX_HEAD_DIM
 RESIDUAL_NORM_MAX_CHANNELS = 16384         # AF3_RESIDUAL_NORM_MAX_CHANNELS
 NORMS = {"none": 0, "rms": 1, "layer": 2}  # af3_norm
@@ -136,6 +156,10 @@ SYMBOLS = {
     "af3_position_bias_forward": (ctypes.c_int, [ctypes.POINTER(PositionBiasParams), vp]),
     "af3_position_bias_backward": (ctypes.c_int, [ctypes.POINTER(PositionBiasParams), vp]),
     "af3_position_bias_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(PositionBiasParams)]),
+    "af3_diff_attention_forward": (ctypes.c_int, [ctypes.POINTER(DiffAttentionParams), vp]),
+    "af3_diff_attention_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(DiffAttentionParams)]),
+    "af3_diff_attention_backward": (ctypes.c_int, [ctypes.POINTER(DiffAttentionParams), ctypes.POINTER(DiffAttentionGrads), vp]),
+    "af3_diff_attention_backward_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(DiffAttentionParams)]),
     "af3_rotary_embedding": (ctypes.c_int, [ctypes.POINTER(RotaryParams), vp]),
     "af3_residual_norm_forward": (ctypes.c_int, [ctypes.POINTER(ResidualNormParams), vp]),
     "af3_residual_norm_backward": (ctypes.c_int, [ctypes.POINTER(ResidualNormParams), ctypes.POINTER(ResidualNormGrads), vp]),

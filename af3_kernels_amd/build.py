@@ -16,8 +16,8 @@ HOST_SRC = os.path.join(CSRC, "host.cpp")
 HOST = os.path.join(HERE, "_host.so")
 LIB = os.path.join(HERE, "libaf3_dpa.so")
 SOURCES = ["api.hip", "dpa_generic.hip", "dpa_mfma.hip", "dpa_mfma_rows.hip", "dpa_strip.hip", "dpa_mfma_f32.hip", "dpa_mfma_fp8.hip", "elementwise.hip", "pair_bias.hip", "glu.hip", "projection.hip", "grid_project.hip",
-           "cross_attention.hip", "cross_attention_grad.hip", "position_bias.hip", "rotary.hip", "residual_norm.hip"]
-HEADERS = [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "mfma_helpers.hpp"), os.path.join(CSRC, "cross_tiles.hpp"), os.path.join(HERE, "..", "include", "af3_dpa.h")]
+           "cross_attention.hip", "cross_attention_grad.hip", "position_bias.hip", "rotary.hip", "residual_norm.hip", "diff_attention.hip", "diff_attention_grad.hip"]
+HEADERS = [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "mfma_helpers.hpp"), os.path.join(CSRC, "cross_tiles.hpp"), os.path.join(CSRC, "diff_tiles.hpp"), os.path.join(HERE, "..", "include", "af3_dpa.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # packed-fp32 ops are switched off for device code; the host pass warns that it does not know
 # the feature, which is harmless.
@@ -25,7 +25,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", 
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Results of matrix instructions in ordinary vector registers: with the accumulators in the other file the cross-attention kernels copied each of them
 # out and back around every product (64 of 154 instructions of the forward pass's inner part).
-EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("cross_attention.hip", "cross_attention_grad.hip")}
+EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("cross_attention.hip", "cross_attention_grad.hip", "diff_attention.hip", "diff_attention_grad.hip")}
 
 
 def _stale(target, deps):

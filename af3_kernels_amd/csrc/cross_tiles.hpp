@@ -149,19 +149,19 @@ struct tile {
 
 // ROWS rows on their way from memory into a tile, spread over the workgroup's threads in 16-byte pieces.  The plain way (rows all there, D a whole number of pieces,
 // 32-bit offsets within the tile) is one load per piece at a scalar base and an offset that stays the same from tile to tile.
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, int NT = THREADS>   // NT: threads of the workgroup
 struct passage {
 	using TL = tile<T, DP>;
-	static constexpr int N = ROWS * TL::CHUNKS / THREADS, E = kind<T>::E;
-	static_assert(N * THREADS == ROWS * TL::CHUNKS);
+	static constexpr int N = ROWS * TL::CHUNKS / NT, E = kind<T>::E;
+	static_assert(N * NT == ROWS * TL::CHUNKS);
 	u32x4    piece[N];
 	uint32_t offset[N];   // bytes from the tile's first row
 	const T* base;
 	int64_t  stride;
 	int      D;
 	bool     plain;
-	static __device__ __forceinline__ int row_of(int n) { return (threadIdx.x + THREADS * n) / TL::CHUNKS; }
-	static __device__ __forceinline__ int col_of(int n) { return (threadIdx.x + THREADS * n) % TL::CHUNKS; }
+	static __device__ __forceinline__ int row_of(int n) { return (threadIdx.x + NT * n) / TL::CHUNKS; }
+	static __device__ __forceinline__ int col_of(int n) { return (threadIdx.x + NT * n) % TL::CHUNKS; }
 	__device__ __forceinline__ void begin(const T* base_, int64_t stride_, int D_, bool whole) {
 		base = base_, stride = stride_, D = D_;
 		plain = whole && stride_ <= (int64_t)0x7fffffff / ((int64_t)ROWS * (int)sizeof(T));
@@ -248,12 +248,13 @@ struct live_keys {
 	uint32_t bits[SEGMENT / 32];
 	uint32_t tiles[SEGMENT / KT / 32];
 	// keys first .. last - 1 (at most SEGMENT of them); a barrier stands before and behind it
+	template <int NT = THREADS>
 	__device__ __forceinline__ void scan(const uint8_t* mask, int64_t first, int64_t last) {
 		__syncthreads();
-		for(int i = threadIdx.x; i < SEGMENT / KT / 32; i += THREADS) tiles[i] = 0u;
+		for(int i = threadIdx.x; i < SEGMENT / KT / 32; i += NT) tiles[i] = 0u;
 		__syncthreads();
 		const int n = (int)(last - first);
-		for(int k = 32 * threadIdx.x; k < n; k += 32 * THREADS) {
+		for(int k = 32 * threadIdx.x; k < n; k += 32 * NT) {
 			uint32_t w = 0u;
 			if(!mask) {
 				w = n - k >= 32 ? ~0u : (1u << (n - k)) - 1u;
@@ -268,7 +269,7 @@ struct live_keys {
 			if(w) atomicOr(&tiles[(k / KT) >> 5], 1u << ((k / KT) & 31));
 		}
 		// (the words of a tile that begins below n and ends behind it)
-		for(int k = (n + 31) / 32 + threadIdx.x; k < (n + KT - 1) / KT * (KT / 32); k += THREADS) bits[k] = 0u;
+		for(int k = (n + 31) / 32 + threadIdx.x; k < (n + KT - 1) / KT * (KT / 32); k += NT) bits[k] = 0u;
 		__syncthreads();
 	}
 	// the first live tile from t on, -1: none

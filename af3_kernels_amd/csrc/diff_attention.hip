@@ -1,0 +1,458 @@
+// Differential attention: out_h = (softmax(scale q1.k1) - lam_h softmax(scale q2.k2)) . v, two maps over one set of values, bf16 or fp32.
+// af3_diff_attention_forward.
+//
+// Per 32 query rows and 32 keys and map:  S^T[key][row] = K . Q^T,  O^T[column][row] += V^T . P^T,  as in cross_attention.hip: a lane holds one query row, the half-waves 16
+// keys each.  The two maps are different wavefronts' (both maps' sums of twice D columns would leave one wavefront to a SIMD), which share the tiles of V; each keeps its own
+// running maximum and sum, and the difference is taken at the end, since neither sum is known before.
+#include "diff_tiles.hpp"
+
+#include <math.h>
+
+namespace af3 {
+namespace diff {
+
+struct forward_args {
+	af3_diff_attention_params p;
+	uint32_t row_tiles, splits;    // workgroups per (batch, key head); parts of the key axis
+	int64_t  part;                 // keys per part, a multiple of the tile
+	float    factor;               // exp2((t - max) * factor) with t = q.k
+	int32_t  whole_k, whole_v;     // D, Dv are whole numbers of 16-byte pieces
+	float*   part_out;             // [splits][2][B * Hkv * G * Lq][Dv] and ...
+	float*   part_stat;            // ... [splits][2][B * Hkv * G * Lq][2] (maximum, sum); sum 0: no live key in the part, and nothing written
+};
+
+// Eight wavefronts: two maps x KW that share 32 query rows and each take 32 keys of a tile (1: a wavefront takes all keys of one) x 4 / KW blocks of 32 rows
+constexpr int NT = 512;
+constexpr int tile_keys(int bytes, int kw) { return kw == 4 || bytes <= 64 ? 128 : kw == 2 || bytes <= 128 ? 64 : 32; }   // bytes of a row of K
+template <typename T, int DP, int KW>
+struct forward_shape {
+	static constexpr int DV = 2 * DP, KT = tile_keys(DP * (int)sizeof(T), KW), SUB = KT / (32 * KW), GROUPS = 4 / KW, ROWS = 32 * GROUPS;
+	static constexpr int KTILE = KT * tile<T, DP>::STRIDE, VTILE = KT * tile<T, DV>::STRIDE, SET = 2 * KTILE + VTILE;
+	static constexpr int BUFFERS = 2 * SET <= 65536 ? 2 : 1;
+	static constexpr int LINE = DV + 4, TABLE = 32 * LINE * 4;   // results of 32 rows on their way to another wavefront
+	static constexpr int LDS = BUFFERS * SET > 4 * TABLE ? BUFFERS * SET : 4 * TABLE;
+};
+
+template <typename T, int DP, int KW>
+__global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
+	using S  = forward_shape<T, DP, KW>;
+	using TK = tile<T, DP>;
+	using TV = tile<T, S::DV>;
+	constexpr int E = kind<T>::E, KT = S::KT;
+	const af3_diff_attention_params& p = a.p;
+	extern __shared__ __align__(16) unsigned char smem[];
+	__shared__ live_keys<KT> live;
+	__shared__ float         stat[8][32][2];
+
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+	const int map = wave & 1, kwave = (wave >> 1) % KW, group = (wave >> 1) / KW;
+	const share    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.row_tiles * a.splits);
+	const uint32_t split = own.piece / a.row_tiles, row_tile = a.row_tiles - 1 - (own.piece - split * a.row_tiles);   // (causal: those with the most keys first)
+	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
+	const int64_t G = p.H / p.Hkv, rows = G * p.Lq;
+	const int     D = (int)p.D, Dv = (int)p.Dv;
+
+	const int64_t   R = (int64_t)row_tile * S::ROWS + 32 * group + (lane & 31);
+	const row_place at_row(R, rows, G, hk);
+	const bool      ok = at_row.ok;
+	const int64_t   qi = at_row.qi, h = at_row.h;
+	u32x4 qf[TK::STEPS];
+	load_operand<T, DP>(qf, static_cast<const T*>(p.q) + b * p.q_stride[0] + (2 * h + map) * p.q_stride[1] + qi * p.q_stride[2], ok, D, lane);
+	const T* const kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + 2 * hk * p.k_stride[1];
+	const T* const vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
+	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b : nullptr;
+
+	// p = exp2(t * to_log2 - reference), reference = to_log2 * (a maximum of the row's logits so far)
+	const float to_log2 = a.factor;
+	float  m = LOWEST, reference = -INFINITY, l = 0.f;
+	bool   moves = true;   // the reference moves at the next block (the first one, and while a row is far)
+	f32x16 o[TV::BLOCKS];
+#pragma unroll
+	for(int db = 0; db < TV::BLOCKS; db++) o[db] = f32x16{};
+
+	int64_t last = (int64_t)(split + 1) * a.part < p.Lk ? (int64_t)(split + 1) * a.part : p.Lk;
+	if(p.causal) {   // (behind the last key of the workgroup's last query nothing counts)
+		const int64_t end_row = (int64_t)(row_tile + 1) * S::ROWS < rows ? (int64_t)(row_tile + 1) * S::ROWS : rows, end = (end_row - 1) / G + p.q_offset + 1;
+		last = end < last ? end : last;
+	}
+	const int64_t limit = p.causal ? qi + p.q_offset : (int64_t)1 << 41;   // the lane's last key
+	const typename TK::reader at_k(lane);
+	const typename TV::reader at_v(lane);
+	passage<T, DP, KT, NT>    pk[2];
+	passage<T, S::DV, KT, NT> pv;
+	pk[0].begin(kb, p.k_stride[2], D, a.whole_k);
+	pk[1].begin(kb + p.k_stride[1], p.k_stride[2], D, a.whole_k);
+	pv.begin(vb, p.v_stride[2], Dv, a.whole_v);
+	int buffer = 0;
+	for(int64_t first = (int64_t)split * a.part; first < last; first += SEGMENT) {
+		const int64_t end = first + SEGMENT < last ? first + SEGMENT : last;
+		live.template scan<NT>(mask, first, end);
+		int t = live.next(0);
+		if(t < 0) continue;
+		const int within = limit - first > SEGMENT ? SEGMENT : limit - first < -1 ? -1 : (int)(limit - first);
+		auto fetch = [&](int tile_no) {
+			const int64_t from = first + (int64_t)tile_no * KT;
+			pk[0].load(from, end), pk[1].load(from, end), pv.load(from, end);
+		};
+		fetch(t);
+		while(t >= 0) {
+			unsigned char*       ks = smem + buffer * S::SET;
+			unsigned char* const vs = ks + 2 * S::KTILE;
+			const tile_bits<KT> bits(live, t);
+			const bool          full = bits.full();
+			const int following = live.next(t + 1);
+			if constexpr(S::BUFFERS == 1) __syncthreads();
+			// (what K holds at a dropped key stays in that key's logits, which are not looked at; its row of V meets a weight of zero, and must not be NaN)
+			pk[0].store(ks, true, [](int) { return true; });
+			pk[1].store(ks + S::KTILE, true, [](int) { return true; });
+			pv.store(vs, full, [&](int row) { return bits.keeps(row); });
+			__syncthreads();
+			if(following >= 0) fetch(following);
+			ks += map * S::KTILE;
+#pragma unroll
+			for(int s = 0; s < S::SUB; s++) {
+				const int      block = kwave * S::SUB + s;
+				const uint32_t keep = bits.of_block(block);
+				const int      left = within - (t * KT + 32 * block + 16 * half);   // the lane's keys 0 .. left of its 16 count
+				if(keep == 0u || !__any(ok && left >= 0)) continue;
+				const bool diagonal = __any(ok && left < 15);
+				float x[16];
+				auto  logits = [&] {
+					f32x16 acc{};
+#pragma unroll
+					for(int st = 0; st < TK::STEPS; st++) acc = kind<T>::mma(TK::row_frag(ks, 32 * block, st, at_k), qf[st], acc);
+#pragma unroll
+					for(int r = 0; r < 16; r++) x[r] = acc[r];
+					if(keep != ~0u) drop_keys(x, keep, -INFINITY);
+					if(diagonal) drop_later(x, left, -INFINITY);
+				};
+				auto probabilities = [&]() -> float {
+					float sum = 0.f;
+#pragma unroll
+					for(int r = 0; r < 16; r++) {
+						x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], to_log2, -reference));
+						sum += x[r];
+					}
+					return sum;
+				};
+				// (optimistic, as in cross_attention.hip: against the reference as it is, which moves where probabilities get large)
+				float sum = 0.f;
+				logits();
+				if(!moves) {
+					sum   = probabilities();
+					moves = __any(!(sum < LARGE));
+					if(moves) logits();
+				}
+				if(moves) {
+					float top = x[0];
+#pragma unroll
+					for(int r = 1; r < 16; r++) top = maximum(top, x[r]);
+					const float to = maximum(m, maximum_of_halves(top)), by = __builtin_amdgcn_exp2f((m - to) * to_log2);
+					m = to, reference = m * to_log2, l *= by;
+#pragma unroll
+					for(int db = 0; db < TV::BLOCKS; db++) o[db] *= by;
+					moves = __any(is_far(reference));
+					if(moves) {
+						sum = 0.f;
+#pragma unroll
+						for(int r = 0; r < 16; r++) {
+							x[r] = __builtin_amdgcn_exp2f((x[r] - m) * to_log2);
+							sum += x[r];
+						}
+					} else {
+						sum = probabilities();
+					}
+				}
+				l += sum;
+#pragma unroll
+				for(int j = 0; j < TV::JOINTS; j++) {
+					const u32x4 pf = kind<T>::pack(x + E * j);
+#pragma unroll
+					for(int db = 0; db < TV::BLOCKS; db++) o[db] = kind<T>::mma(TV::col_frag(vs, 32 * block, db, j, at_v), pf, o[db]);
+				}
+			}
+			t = following;
+			if constexpr(S::BUFFERS == 2) buffer ^= 1;
+		}
+	}
+	l = sum_of_halves(l);
+
+	float* const tables = reinterpret_cast<float*>(smem);   // four of them, 32 rows each
+	const int    line = (lane & 31) * S::LINE + 16 * half;
+	auto put = [&](float* table, int db, float by) {
+#pragma unroll
+		for(int e = 0; e < 4; e++) *reinterpret_cast<f32x4*>(table + line + 32 * db + 4 * e) = f32x4{o[db][4 * e] * by, o[db][4 * e + 1] * by, o[db][4 * e + 2] * by, o[db][4 * e + 3] * by};
+	};
+	if constexpr(KW > 1) {   // wavefronts that share rows: each weights its own sums by the common maximum, then a part of the columns each; map after map
+		if(half == 0) stat[wave][lane][0] = m, stat[wave][lane][1] = l;
+		__syncthreads();   // (and nobody reads tiles any more)
+		float to = LOWEST, sum = 0.f;
+#pragma unroll
+		for(int w = 0; w < KW; w++) to = maximum(to, stat[2 * (group * KW + w) + map][lane & 31][0]);
+#pragma unroll
+		for(int w = 0; w < KW; w++) sum += stat[2 * (group * KW + w) + map][lane & 31][1] * __builtin_amdgcn_exp2f((stat[2 * (group * KW + w) + map][lane & 31][0] - to) * a.factor);
+		const float by = __builtin_amdgcn_exp2f((m - to) * a.factor);
+		m = to, l = sum;
+#pragma unroll
+		for(int turn = 0; turn < 2; turn++) {
+			if(turn == map) {
+#pragma unroll
+				for(int db = 0; db < TV::BLOCKS; db++) put(tables + (wave >> 1) * (S::TABLE / 4), db, by);
+			}
+			__syncthreads();
+			if(turn == map) {
+#pragma unroll
+				for(int db = 0; db < TV::BLOCKS; db++) {
+					if(db % KW != kwave) continue;
+					o[db] = f32x16{};
+#pragma unroll
+					for(int w = 0; w < KW; w++)
+#pragma unroll
+						for(int e = 0; e < 4; e++) {
+							const f32x4 v = *reinterpret_cast<const f32x4*>(tables + (group * KW + w) * (S::TABLE / 4) + line + 32 * db + 4 * e);
+#pragma unroll
+							for(int c = 0; c < 4; c++) o[db][4 * e + c] += v[c];
+						}
+				}
+			}
+			__syncthreads();
+		}
+	}
+	const bool first_of_row = ok && kwave == 0 && half == 0;
+	if(a.splits > 1) {
+		const int64_t n_rows = p.B * p.Hkv * rows, place = (2 * (int64_t)split + map) * n_rows + (b * p.Hkv + hk) * rows + R;
+		if(first_of_row) a.part_stat[2 * place] = m, a.part_stat[2 * place + 1] = l;
+		if(!ok || l == 0.f) return;
+#pragma unroll
+		for(int db = 0; db < TV::BLOCKS; db++) {
+			if(db % KW != kwave) continue;
+			float v[16];
+#pragma unroll
+			for(int r = 0; r < 16; r++) v[r] = o[db][r];
+			store_row16(a.part_out + place * Dv, 32 * db + 16 * half, Dv, v);
+		}
+		return;
+	}
+	const float   inv = l == 0.f ? 0.f : 1.f / l;   // (0: no live key)
+	const int64_t row = (b * p.H + h) * p.Lq + qi;
+	if(p.stats && first_of_row) {
+		float* const st = p.stats + 2 * ((b * 2 * p.H + 2 * h + map) * p.Lq + qi);
+		st[0] = m, st[1] = inv;
+	}
+	// the second map's result by way of LDS to the wavefront that has the first one
+	if constexpr(KW == 1) __syncthreads();
+	if(map == 1) {
+		const float by = inv * lam_of(p, h);
+#pragma unroll
+		for(int db = 0; db < TV::BLOCKS; db++) {
+			if(db % KW != kwave) continue;
+			put(tables + group * (S::TABLE / 4), db, by);
+			if(p.second && ok) {
+				float v[16];
+#pragma unroll
+				for(int r = 0; r < 16; r++) v[r] = o[db][r] * inv;
+				store_row16(static_cast<T*>(p.second) + row * Dv, 32 * db + 16 * half, Dv, v);
+			}
+		}
+	}
+	__syncthreads();
+	if(map == 1 || !ok) return;
+	T* const out = static_cast<T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2];
+#pragma unroll
+	for(int db = 0; db < TV::BLOCKS; db++) {
+		if(db % KW != kwave) continue;
+		float v[16];
+#pragma unroll
+		for(int e = 0; e < 4; e++) {
+			const f32x4 other = *reinterpret_cast<const f32x4*>(tables + group * (S::TABLE / 4) + line + 32 * db + 4 * e);
+#pragma unroll
+			for(int c = 0; c < 4; c++) v[4 * e + c] = l == 0.f ? 0.f : __builtin_fmaf(o[db][4 * e + c], inv, -other[c]);
+		}
+		store_row16(out, 32 * db + 16 * half, Dv, v);
+	}
+}
+
+// The parts of the key axis joined: one wavefront per query row, columns over its lanes.  The parts' maxima and sums come one to a lane (64 parts at most), so that the
+// parts' results, four of them in flight, wait for nothing but each other.
+constexpr int MAX_PARTS = 64;
+template <typename T, int COLUMNS>   // columns of a lane
+__global__ void __launch_bounds__(THREADS) diff_join_kernel(forward_args a) {
+	const af3_diff_attention_params& p = a.p;
+	const int64_t G = p.H / p.Hkv, rows = G * p.Lq, n_rows = p.B * p.Hkv * rows;
+	const int     lane = threadIdx.x & 63, Dv = (int)p.Dv, splits = (int)a.splits;
+	const int64_t at = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+	if(at >= n_rows) return;
+	const int64_t   bh = at / rows, hk = bh % p.Hkv, b = bh / p.Hkv;
+	const row_place place(at - bh * rows, rows, G, hk);
+	const int64_t   row = (b * p.H + place.h) * p.Lq + place.qi;
+	float o[2][COLUMNS];
+	bool  none = false;   // no live key
+#pragma unroll
+	for(int i = 0; i < 2; i++) {
+		float m = 0.f, l = 0.f;
+		if(lane < splits) m = a.part_stat[2 * ((2 * lane + i) * n_rows + at)], l = a.part_stat[2 * ((2 * lane + i) * n_rows + at) + 1];
+		float top = l == 0.f ? LOWEST : m;
+#pragma unroll
+		for(int d = 32; d; d >>= 1) top = maximum(top, __shfl_xor(top, d));
+		const float weight = l == 0.f ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.factor);
+		float sum = l * weight;
+#pragma unroll
+		for(int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+#pragma unroll
+		for(int k = 0; k < COLUMNS; k++) o[i][k] = 0.f;
+		for(int s0 = 0; s0 < splits; s0 += 4) {
+			float x[4][COLUMNS];
+#pragma unroll
+			for(int s = 0; s < 4; s++) {
+				const bool there = s0 + s < splits && __shfl(l, (s0 + s) & 63) != 0.f;
+#pragma unroll
+				for(int k = 0; k < COLUMNS; k++) {
+					x[s][k] = 0.f;
+					if(there && lane + 64 * k < Dv) x[s][k] = a.part_out[((2 * (s0 + s) + i) * n_rows + at) * Dv + lane + 64 * k];
+				}
+			}
+#pragma unroll
+			for(int s = 0; s < 4; s++) {
+				const float w = __shfl(weight, (s0 + s) & 63);
+#pragma unroll
+				for(int k = 0; k < COLUMNS; k++) o[i][k] = s0 + s < splits ? __builtin_fmaf(x[s][k], w, o[i][k]) : o[i][k];
+			}
+		}
+		const float inv = sum == 0.f ? 0.f : 1.f / sum;
+		none = sum == 0.f;
+#pragma unroll
+		for(int k = 0; k < COLUMNS; k++) o[i][k] *= inv;
+		if(p.stats && lane == 0) {
+			float* const st = p.stats + 2 * ((b * 2 * p.H + 2 * place.h + i) * p.Lq + place.qi);
+			st[0] = top, st[1] = inv;
+		}
+	}
+	const float lam = lam_of(p, place.h);
+	T* const    out = static_cast<T*>(p.out) + b * p.out_stride[0] + place.h * p.out_stride[1] + place.qi * p.out_stride[2];
+#pragma unroll
+	for(int k = 0; k < COLUMNS; k++)
+		if(lane + 64 * k < Dv) {
+			out[lane + 64 * k] = kind<T>::bits(none ? 0.f : __builtin_fmaf(-lam, o[1][k], o[0][k]));
+			if(p.second) static_cast<T*>(p.second)[row * Dv + lane + 64 * k] = kind<T>::bits(o[1][k]);
+		}
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------
+int width(const af3_diff_attention_params& p) {   // columns of a map's queries and keys that a kernel has, half of those of its values
+	const int64_t d = p.D > (p.Dv + 1) / 2 ? p.D : (p.Dv + 1) / 2;
+	return d <= 32 ? 32 : d <= 64 ? 64 : 128;
+}
+// the most wavefronts that can share rows: four where the tiles of 128 keys leave registers and LDS for the rest
+template <typename T, int DP>
+constexpr int MOST_SHARING = DP * (int)sizeof(T) <= 128 ? 4 : 2;
+int most_sharing(const af3_diff_attention_params& p) { return width(p) * (p.dtype == AF3_F32 ? 4 : 2) <= 128 ? 4 : 2; }
+
+struct plan {
+	int      kw;
+	uint32_t row_tiles, splits;
+	int64_t  part;
+};
+plan forward_plan(const af3_diff_attention_params& p) {
+	plan          f;
+	const int64_t rows = p.H / p.Hkv * p.Lq, groups = p.B * p.Hkv;
+	const bool    fp32 = p.dtype == AF3_F32;
+	const int     wide = width(p);
+	const int64_t slots = wide * (fp32 ? 4 : 2) <= 64 ? 512 : 256;
+	auto          busy = [&](int kw) { return (rows + 128 / kw - 1) / (128 / kw) * groups; };
+	f.kw = rows <= 32 || busy(4) <= slots ? 4 : rows <= 64 || busy(2) <= slots ? 2 : 1;
+	if(f.kw > most_sharing(p)) f.kw = most_sharing(p);
+	f.row_tiles = (uint32_t)(busy(f.kw) / groups);
+	const int64_t kt = tile_keys(wide * (fp32 ? 4 : 2), f.kw), key_tiles = (p.Lk + kt - 1) / kt;
+	const double  tile_us = (0.4 + 0.033 * wide) * (f.kw == 4 ? 1.0 : 0.6) * (fp32 ? 3.0 : 1.0);
+	const int64_t splits = parts_for(busy(f.kw), slots, key_tiles, tile_us, 8.0 * p.B * p.H * p.Lq * p.Dv, MAX_PARTS);
+	const int64_t per = (key_tiles + splits - 1) / splits;
+	f.part   = per * kt;
+	f.splits = (uint32_t)((key_tiles + per - 1) / per);
+	return f;
+}
+
+template <typename T, int DP, int KW>
+int launch_forward(const forward_args& a, uint32_t grid, hipStream_t s) {
+	using S = forward_shape<T, DP, KW>;
+	auto kernel = &diff_forward_kernel<T, DP, KW>;
+	if(S::LDS > 65536 - 8192 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess) {
+		(void)hipGetLastError();
+		return AF3_ERR_LAUNCH;
+	}
+	hipLaunchKernelGGL(kernel, dim3(grid), dim3(NT), S::LDS, s, a);
+	return launch_status();
+}
+template <typename T, int DP>
+int launch_forward_form(const forward_args& a, int kw, uint32_t grid, hipStream_t s) {
+	if constexpr(MOST_SHARING<T, DP> == 4)
+		if(kw == 4) return launch_forward<T, DP, 4>(a, grid, s);
+	return kw == 2 ? launch_forward<T, DP, 2>(a, grid, s) : launch_forward<T, DP, 1>(a, grid, s);
+}
+template <typename T>
+int launch_forward_type(const forward_args& a, int kw, uint32_t grid, hipStream_t s) {
+	const int wide = width(a.p);
+	if(wide == 32) return launch_forward_form<T, 32>(a, kw, grid, s);
+	if constexpr(sizeof(T) == 2)
+		if(wide == 128) return launch_forward_form<T, 128>(a, kw, grid, s);
+	return launch_forward_form<T, 64>(a, kw, grid, s);
+}
+
+int64_t forward_workspace(const af3_diff_attention_params& p, const plan& f) { return f.splits > 1 ? (int64_t)f.splits * p.B * p.H * p.Lq * (p.Dv + 2) * 8 : 0; }
+
+}  // namespace diff
+
+// whether the gradients of k and v can be launched: workgroups of 32 keys, times 256 threads, inside 32 bits
+bool diff_gradients_fit(const af3_diff_attention_params& p) { return p.B * p.Hkv * ((p.Lk + 31) / 32) <= 0xffffff; }
+
+int validate_diff_attention(const af3_diff_attention_params* p) {
+	if(!p) return AF3_ERR_NULL_POINTER;
+	if((p->dtype != AF3_F32 && p->dtype != AF3_BF16) || (p->lam_dtype != AF3_F32 && p->lam_dtype != AF3_BF16)) return AF3_ERR_BAD_DTYPE;
+	if(p->B <= 0 || p->H <= 0 || p->Hkv <= 0 || p->Lq <= 0 || p->Lk <= 0 || p->D <= 0 || p->Dv <= 0 || p->H % p->Hkv != 0) return AF3_ERR_BAD_SHAPE;
+	if(p->D > (p->dtype == AF3_F32 ? 64 : 128) || p->Dv > (p->dtype == AF3_F32 ? 128 : 256)) return AF3_ERR_UNSUPPORTED_D;
+	// (row numbers and the parts' sizes stay far inside 63 bits, a launch's workgroups times 256 threads inside 32)
+	if(p->B > 0xffffff || p->H > 0x7fff || p->Lq > 0x3fffffff || p->Lk > 0x3fffffff || p->B * p->H > 0xffffff || p->H * p->Lq > 0x3fffffff || p->B * p->H * ((p->Lq + 31) / 32) > 0xffffff) return AF3_ERR_BAD_SHAPE;
+	if(p->stats && !diff_gradients_fit(*p)) return AF3_ERR_BAD_SHAPE;   // (they are for a gradient that would be refused)
+	if(!p->q || !p->k || !p->v || !p->lam || !p->out || (p->stats != nullptr) != (p->second != nullptr)) return AF3_ERR_NULL_POINTER;
+	for(int i = 0; i < 3; i++)
+		if(p->q_stride[i] < 0 || p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
+	// (inputs may repeat rows, results may not)
+	if((p->Lq > 1 && p->out_stride[2] < p->Dv) || (p->H > 1 && p->out_stride[1] == 0) || (p->B > 1 && p->out_stride[0] == 0) || p->lam_stride < 0) return AF3_ERR_BAD_STRIDE;
+	if(p->key_mask && p->key_mask_stride_b < 0) return AF3_ERR_BAD_STRIDE;
+	if(!(p->softmax_scale > 0.f) || !(p->softmax_scale < INFINITY) || p->q_offset >= (int64_t)1 << 40 || p->q_offset <= -((int64_t)1 << 40)) return AF3_ERR_BAD_ARGUMENT;
+	return AF3_OK;
+}
+
+}  // namespace af3
+
+using namespace af3;
+
+extern "C" int64_t af3_diff_attention_workspace_bytes(const af3_diff_attention_params* params) {
+	const int rc = validate_diff_attention(params);
+	return rc != AF3_OK ? rc : diff::forward_workspace(*params, diff::forward_plan(*params));
+}
+
+extern "C" int af3_diff_attention_forward(const af3_diff_attention_params* params, void* hip_stream) {
+	if(const int rc = validate_diff_attention(params); rc != AF3_OK) return rc;
+	const diff::plan f = diff::forward_plan(*params);
+	if(const int64_t need = diff::forward_workspace(*params, f); need > 0 && (!params->workspace || params->workspace_bytes < need || (reinterpret_cast<uintptr_t>(params->workspace) & 15))) return AF3_ERR_BAD_ARGUMENT;
+	if(const int dc = current_device_status(); dc != AF3_OK) return dc;
+	const hipStream_t  s = static_cast<hipStream_t>(hip_stream);
+	diff::forward_args a;
+	const bool         fp32 = params->dtype == AF3_F32;
+	a.p = *params, a.row_tiles = f.row_tiles, a.splits = f.splits, a.part = f.part;
+	a.factor  = params->softmax_scale * LOG2E;
+	a.whole_k = params->D * (fp32 ? 4 : 2) % 16 == 0, a.whole_v = params->Dv * (fp32 ? 4 : 2) % 16 == 0;
+	const int64_t n_rows = params->B * params->H * params->Lq;
+	a.part_out = static_cast<float*>(params->workspace), a.part_stat = a.part_out + 2 * f.splits * n_rows * params->Dv;
+	const uint32_t grid = (uint32_t)(params->B * params->Hkv) * f.row_tiles * f.splits;
+	const int rc = fp32 ? diff::launch_forward_type<float>(a, f.kw, grid, s) : diff::launch_forward_type<uint16_t>(a, f.kw, grid, s);
+	if(rc != AF3_OK || f.splits == 1) return rc;
+	const dim3 joins((uint32_t)((n_rows + cross::WAVES - 1) / cross::WAVES)), threads(cross::THREADS);
+	if(params->Dv <= 128) {
+		if(fp32) hipLaunchKernelGGL((diff::diff_join_kernel<float, 2>), joins, threads, 0, s, a);
+		else hipLaunchKernelGGL((diff::diff_join_kernel<uint16_t, 2>), joins, threads, 0, s, a);
+	} else {
+		hipLaunchKernelGGL((diff::diff_join_kernel<uint16_t, 4>), joins, threads, 0, s, a);
+	}
+	return launch_status();
+}

@@ -1,0 +1,679 @@
+// The gradients of diff_attention.hip's attention.  With P1, P2 the two maps of a head, O2 = P2 . v, dO = the gradient of out = (P1 - lam P2) . v:
+//     dv = (P1 - lam P2)^T . dO,  dP = dO . v^T (one product for both maps),  d2 = rowsum(dO * O2),  d1 = rowsum(dO * O1) = rowsum(dO * out) + lam d2,
+//     dS1 = P1 * (dP - d1),  dS2 = -lam P2 * (dP - d2),  dq_i = scale dS_i . k_i,  dk_i = scale dS_i^T . q_i,  dlam = -sum of d2 over the head's rows.
+// P1 and P2 are computed again from q, k and the two numbers per row and map that the forward pass left.  Kernels, none with atomics: each element of a result is
+// summed by one workgroup, or by one per part of the long axis and a joining kernel, always in the same order.
+//   diff_dq_kernel    32 query rows per wavefront, both maps, keys in tiles (writes d1 and d2 too)
+//   diff_dkv_kernel   32 keys per wavefront, both maps, query rows in tiles, over all heads of the key head
+//   diff_lam_kernel   the sums of d2
+#include "diff_tiles.hpp"
+
+#include <math.h>
+
+namespace af3 {
+namespace diff {
+
+struct grad_args {
+	af3_diff_attention_params p;
+	af3_diff_attention_grads  g;
+	uint32_t tiles, splits;   // workgroups per (batch, key head), parts of the long axis
+	int64_t  part;            // dq: keys per part; dkv: tiles of query rows per part
+	float    factor;
+	int32_t  whole_k, whole_v;
+	float *  d1, *d2;         // [B, H, Lq] each
+	float*   partial;         // dq: [splits][B 2H Lq][D]; dkv: [splits]([B 2Hkv Lk][D], [B Hkv Lk][Dv])
+	float *  dq_space, *dkv_space;
+};
+
+// the sum of the wavefronts' results of equal shape, wavefront w keeps the blocks of columns that are w modulo N; `tables`: N of 32 x (W + 4)
+template <int W, int N>
+__device__ __forceinline__ void add_up(float* tables, int w, int lane, f32x16 (&o)[W / 32]) {
+	const int at = (lane & 31) * (W + 4) + 16 * (lane >> 5);
+	__syncthreads();
+#pragma unroll
+	for(int db = 0; db < W / 32; db++)
+#pragma unroll
+		for(int i = 0; i < 4; i++) *reinterpret_cast<f32x4*>(tables + w * 32 * (W + 4) + at + 32 * db + 4 * i) = f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+	__syncthreads();
+#pragma unroll
+	for(int db = 0; db < W / 32; db++) {
+		if(db % N != w) continue;
+		o[db] = f32x16{};
+#pragma unroll
+		for(int k = 0; k < N; k++)
+#pragma unroll
+			for(int i = 0; i < 4; i++) {
+				const f32x4 v = *reinterpret_cast<const f32x4*>(tables + k * 32 * (W + 4) + at + 32 * db + 4 * i);
+#pragma unroll
+				for(int e = 0; e < 4; e++) o[db][4 * i + e] += v[e];
+			}
+	}
+}
+
+// a lane's half of a row times its half of the gradient of out, both half-waves added
+template <typename T, int DV, int N>
+__device__ __forceinline__ float row_dot(const u32x4 (&gf)[N], const T* row, bool ok, int Dv, int lane) {
+	u32x4 of[N];
+	load_operand<T, DV>(of, row, ok, Dv, lane);
+	float sum = 0.f;
+#pragma unroll
+	for(int s = 0; s < N; s++)
+#pragma unroll
+		for(int e = 0; e < kind<T>::E; e++) sum = __builtin_fmaf(kind<T>::at(gf[s], e), kind<T>::at(of[s], e), sum);
+	return sum_of_halves(sum);
+}
+// d1 and d2 of a lane's query row
+template <typename T, int DV, int N>
+__device__ __forceinline__ void row_deltas(const grad_args& a, const u32x4 (&gf)[N], int64_t b, int64_t h, int64_t qi, bool ok, int lane, float& d1, float& d2) {
+	const af3_diff_attention_params& p = a.p;
+	d2 = row_dot<T, DV>(gf, static_cast<const T*>(p.second) + ((b * p.H + h) * p.Lq + qi) * p.Dv, ok, (int)p.Dv, lane);
+	d1 = row_dot<T, DV>(gf, static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2], ok, (int)p.Dv, lane);
+	d1 = __builtin_fmaf(lam_of(p, h), d2, d1);
+}
+
+// How many rows a tile has, and how many threads and maps of a wavefront the kernels have, by the bytes of a row of q or k (of 32, 64 or 128 columns).
+constexpr int tile_rows(int bytes, int sharing) { return sharing > 1 ? 32 * sharing : bytes <= 64 ? 128 : bytes <= 128 ? 64 : 32; }
+constexpr int dq_maps(int bytes) { return bytes <= 128 ? 2 : 1; }
+constexpr int dq_threads(int bytes) { return 512; }
+constexpr int dkv_maps(int bytes) { return bytes <= 128 ? 2 : 1; }
+constexpr int dkv_threads(int bytes) { return 256; }
+
+// ---- dQ ----
+// KW: wavefronts that share 32 rows and each take 32 keys of a tile; MAPS: maps of a wavefront, 2, or 1 with the other map beside it in another one
+template <typename T, int DP, int KW>
+struct dq_shape {
+	static constexpr int BYTES = DP * (int)sizeof(T), MAPS = dq_maps(BYTES), NT = dq_threads(BYTES), W = NT / 64, GROUPS = W * MAPS / 2 / KW;
+	static constexpr int DV = 2 * DP, KT = tile_rows(BYTES, KW), SUB = KT / (32 * KW), ROWS = 32 * GROUPS;
+	static constexpr int KTILE = KT * tile<T, DP>::STRIDE, VTILE = KT * tile<T, DV>::STRIDE, SET = 2 * KTILE + VTILE;
+	static constexpr int BUFFERS = 2 * SET <= 65536 ? 2 : 1;
+	static constexpr int JOIN = KW > 1 ? W * 32 * (DP + 4) * 4 : 0;
+	static constexpr int LDS = BUFFERS * SET > JOIN ? BUFFERS * SET : JOIN;
+};
+
+template <typename T, int DP, int KW>
+__global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(grad_args a) {
+	using S  = dq_shape<T, DP, KW>;
+	using TK = tile<T, DP>;
+	using TV = tile<T, S::DV>;
+	constexpr int E = kind<T>::E, KT = S::KT, MAPS = S::MAPS;
+	const af3_diff_attention_params& p = a.p;
+	extern __shared__ __align__(16) unsigned char smem[];
+	__shared__ live_keys<KT> live;
+
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+	const int map0 = MAPS == 2 ? 0 : wave & 1, place = MAPS == 2 ? wave : wave >> 1, kwave = place % KW, group = place / KW;   // (map0: the wavefront's first map)
+	const share    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.tiles * a.splits);
+	const uint32_t split = own.piece / a.tiles, row_tile = a.tiles - 1 - (own.piece - split * a.tiles);
+	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
+	const int64_t G = p.H / p.Hkv, rows = G * p.Lq;
+	const int     D = (int)p.D, Dv = (int)p.Dv;
+
+	const int64_t   R = (int64_t)row_tile * S::ROWS + 32 * group + (lane & 31);
+	const row_place at_row(R, rows, G, hk);
+	const bool      ok = at_row.ok;
+	const int64_t   qi = at_row.qi, h = at_row.h, row = (b * p.H + h) * p.Lq + qi;
+	u32x4 qf[MAPS][TK::STEPS], gf[TV::STEPS];
+#pragma unroll
+	for(int i = 0; i < MAPS; i++) load_operand<T, DP>(qf[i], static_cast<const T*>(p.q) + b * p.q_stride[0] + (2 * h + map0 + i) * p.q_stride[1] + qi * p.q_stride[2], ok, D, lane);
+	load_operand<T, S::DV>(gf, static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1] + qi * a.g.grad_out_stride[2], ok, Dv, lane);
+	float d1, d2, delta[MAPS];
+	row_deltas<T, S::DV>(a, gf, b, h, qi, ok, lane, d1, d2);
+	if(ok && half == 0 && kwave == 0 && map0 == 0 && split == 0) a.d1[row] = d1, a.d2[row] = d2;
+	if(!a.g.grad_q) return;
+	float m[MAPS], inv[MAPS], taken[MAPS];
+	bool  far = false;
+#pragma unroll
+	for(int i = 0; i < MAPS; i++) {
+		delta[i] = map0 + i == 0 ? d1 : d2;
+		const int64_t at = (b * 2 * p.H + 2 * h + map0 + i) * p.Lq + qi;
+		m[i] = ok ? p.stats[2 * at] : 0.f, inv[i] = ok ? p.stats[2 * at + 1] : 0.f;
+		taken[i] = whole_reference(m[i], inv[i], a.factor);
+		far = far || is_far(m[i] * a.factor);
+	}
+	const bool apart = sizeof(T) == 4 || __any(far);   // (a row far from zero: in the logits' own units)
+	const T* const kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + 2 * hk * p.k_stride[1];
+	const T* const vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
+	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b : nullptr;
+
+	f32x16 dq[MAPS][TK::BLOCKS];
+#pragma unroll
+	for(int i = 0; i < MAPS; i++)
+#pragma unroll
+		for(int db = 0; db < TK::BLOCKS; db++) dq[i][db] = f32x16{};
+
+	int64_t last = (int64_t)(split + 1) * a.part < p.Lk ? (int64_t)(split + 1) * a.part : p.Lk;
+	if(p.causal) {
+		const int64_t end_row = (int64_t)(row_tile + 1) * S::ROWS < rows ? (int64_t)(row_tile + 1) * S::ROWS : rows, end = (end_row - 1) / G + p.q_offset + 1;
+		last = end < last ? end : last;
+	}
+	const int64_t limit = p.causal ? qi + p.q_offset : (int64_t)1 << 41;
+	const typename TK::reader at_k(lane);
+	const typename TV::reader at_v(lane);
+	passage<T, DP, KT, S::NT>    pk[2];
+	passage<T, S::DV, KT, S::NT> pv;
+	pk[0].begin(kb, p.k_stride[2], D, a.whole_k);
+	pk[1].begin(kb + p.k_stride[1], p.k_stride[2], D, a.whole_k);
+	pv.begin(vb, p.v_stride[2], Dv, a.whole_v);
+	int buffer = 0;
+	for(int64_t first = (int64_t)split * a.part; first < last; first += SEGMENT) {
+		const int64_t end = first + SEGMENT < last ? first + SEGMENT : last;
+		live.template scan<S::NT>(mask, first, end);
+		int t = live.next(0);
+		if(t < 0) continue;
+		const int within = limit - first > SEGMENT ? SEGMENT : limit - first < -1 ? -1 : (int)(limit - first);
+		auto fetch = [&](int tile_no) {
+			const int64_t from = first + (int64_t)tile_no * KT;
+			pk[0].load(from, end), pk[1].load(from, end), pv.load(from, end);
+		};
+		fetch(t);
+		while(t >= 0) {
+			unsigned char* const ks = smem + buffer * S::SET;
+			unsigned char* const vs = ks + 2 * S::KTILE;
+			const tile_bits<KT> bits(live, t);
+			const bool          full = bits.full();
+			const int following = live.next(t + 1);
+			if constexpr(S::BUFFERS == 1) __syncthreads();
+			// (V is only multiplied row by row, and dS of a dropped key is not looked at; K's rows are added up under weights of zero)
+			pk[0].store(ks, full, [&](int r) { return bits.keeps(r); });
+			pk[1].store(ks + S::KTILE, full, [&](int r) { return bits.keeps(r); });
+			pv.store(vs, true, [](int) { return true; });
+			__syncthreads();
+			if(following >= 0) fetch(following);
+#pragma unroll
+			for(int s = 0; s < S::SUB; s++) {
+				const int      block = kwave * S::SUB + s;
+				const uint32_t keep  = bits.of_block(block);
+				const int      left = within - (t * KT + 32 * block + 16 * half);
+				if(keep == 0u || !__any(ok && left >= 0)) continue;
+				const bool diagonal = __any(ok && left < 15);
+				f32x16 dp{};
+#pragma unroll
+				for(int st = 0; st < TV::STEPS; st++) dp = kind<T>::mma(TV::row_frag(vs, 32 * block, st, at_v), gf[st], dp);
+#pragma unroll
+				for(int i = 0; i < MAPS; i++) {
+					const unsigned char* const km = ks + (map0 + i) * S::KTILE;
+					f32x16 acc{};
+#pragma unroll
+					for(int st = 0; st < TK::STEPS; st++) acc = kind<T>::mma(TK::row_frag(km, 32 * block, st, at_k), qf[i][st], acc);
+					float x[16];
+					if(apart) {
+#pragma unroll
+						for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f((acc[r] - m[i]) * a.factor) * inv[i] * (dp[r] - delta[i]);
+					} else {
+#pragma unroll
+						for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r], a.factor, -taken[i])) * (dp[r] - delta[i]);
+					}
+					if(keep != ~0u) drop_keys(x, keep, 0.f);
+					if(diagonal) drop_later(x, left, 0.f);
+#pragma unroll
+					for(int j = 0; j < TK::JOINTS; j++) {
+						const u32x4 f = kind<T>::pack(x + E * j);
+#pragma unroll
+						for(int db = 0; db < TK::BLOCKS; db++) dq[i][db] = kind<T>::mma(TK::col_frag(km, 32 * block, db, j, at_k), f, dq[i][db]);
+					}
+				}
+			}
+			t = following;
+			if constexpr(S::BUFFERS == 2) buffer ^= 1;
+		}
+	}
+	const float lam = lam_of(p, h);
+#pragma unroll
+	for(int i = 0; i < MAPS; i++) {
+		if constexpr(KW > 1) add_up<DP, KW>(reinterpret_cast<float*>(smem) + (MAPS == 2 ? group : 2 * group + map0) * KW * 32 * (DP + 4), kwave, lane, dq[i]);
+		if(!ok) continue;
+		const float   scale = map0 + i == 0 ? p.softmax_scale : -lam * p.softmax_scale;   // (the second map's dS is -lam times what was summed)
+		const int64_t to = (b * 2 * p.H + 2 * h + map0 + i) * p.Lq + qi;
+#pragma unroll
+		for(int db = 0; db < TK::BLOCKS; db++) {
+			if(db % KW != kwave) continue;
+			float v[16];
+#pragma unroll
+			for(int r = 0; r < 16; r++) v[r] = dq[i][db][r] * scale;
+			if(a.splits > 1) store_row16(a.partial + (split * (p.B * 2 * p.H * p.Lq) + to) * D, 32 * db + 16 * half, D, v);
+			else store_row16(static_cast<T*>(a.g.grad_q) + to * D, 32 * db + 16 * half, D, v);
+		}
+	}
+}
+
+// What the kernel with query rows in tiles keeps of each row of a tile in LDS: d1 and d2, and per map the whole reference (bf16), maximum and 1 / sum (fp32 and tiles with
+// a row far from zero).  Behind them a word per 64 rows that says whether there is one.
+enum { LESS = 0, TAKEN = 2, MOST = 4, INVERSE = 6, ROW_STATS = 8 };
+template <typename T, int QT>
+struct row_stats {
+	float v[ROW_STATS];   // of one row, on its way
+	__device__ __forceinline__ void load(const grad_args& a, int64_t b, int64_t h, int64_t q0) {
+#pragma unroll
+		for(int i = 0; i < ROW_STATS; i++) v[i] = 0.f;
+		const int64_t qi = q0 + threadIdx.x;
+		if((int)threadIdx.x >= QT || qi >= a.p.Lq) return;
+		const int64_t row = (b * a.p.H + h) * a.p.Lq + qi;
+		v[LESS] = a.d1[row], v[LESS + 1] = a.d2[row];
+#pragma unroll
+		for(int i = 0; i < 2; i++) {
+			const int64_t at = (b * 2 * a.p.H + 2 * h + i) * a.p.Lq + qi;
+			v[MOST + i] = a.p.stats[2 * at], v[INVERSE + i] = a.p.stats[2 * at + 1];
+		}
+	}
+	__device__ __forceinline__ void store(float* st, float factor) {
+		if((int)threadIdx.x >= QT) return;
+		bool far = false;
+#pragma unroll
+		for(int i = 0; i < 2; i++) v[TAKEN + i] = whole_reference(v[MOST + i], v[INVERSE + i], factor), far = far || is_far(v[MOST + i] * factor);
+#pragma unroll
+		for(int i = 0; i < ROW_STATS; i++) st[i * QT + threadIdx.x] = v[i];
+		const bool any = __any(far);
+		if((threadIdx.x & 63) == 0) reinterpret_cast<int*>(st + ROW_STATS * QT)[threadIdx.x >> 6] = any;
+	}
+	// whether the rows' maxima and sums are to be taken apart
+	static __device__ __forceinline__ bool apart(const float* st) {
+		if constexpr(sizeof(T) == 4) return true;
+		const int* const far = reinterpret_cast<const int*>(st + ROW_STATS * QT);
+		return __builtin_amdgcn_readfirstlane(QT > 64 ? far[0] | far[1] : far[0]) != 0;
+	}
+	static __device__ __forceinline__ f32x16 sixteen(const float* at) {
+		f32x16 x;
+#pragma unroll
+		for(int i = 0; i < 4; i++) {
+			const f32x4 y = *reinterpret_cast<const f32x4*>(at + 4 * i);
+			x[4 * i] = y[0], x[4 * i + 1] = y[1], x[4 * i + 2] = y[2], x[4 * i + 3] = y[3];
+		}
+		return x;
+	}
+};
+
+// ---- dK, dV ----
+// RW: wavefronts that share 32 keys and each take 32 rows of a tile of query rows (1: every wavefront has its own keys and takes the whole tile)
+template <typename T, int DP, int RW>
+struct dkv_shape {
+	static constexpr int BYTES = DP * (int)sizeof(T), MAPS = dkv_maps(BYTES), NT = dkv_threads(BYTES), W = NT / 64, GROUPS = W * MAPS / 2 / RW;
+	static constexpr int DV = 2 * DP, QT = tile_rows(BYTES, RW), SUB = QT / (32 * RW), KEYS = 32 * GROUPS;
+	static constexpr int VW = RW * (MAPS == 2 ? 1 : 2);   // wavefronts that have a part of the same rows of dV
+	static constexpr int QTILE = QT * tile<T, DP>::STRIDE, GTILE = QT * tile<T, DV>::STRIDE, STATS = ROW_STATS * QT * 4 + 16, SET = 2 * QTILE + GTILE + STATS;
+	static constexpr int BUFFERS = 2 * SET <= 73728 ? 2 : 1;
+	static constexpr int JOIN = VW > 1 ? W * 32 * (DV + 4) * 4 : 0;
+	static constexpr int LDS = BUFFERS * SET > JOIN ? BUFFERS * SET : JOIN;
+	static constexpr int PER_SIMD = NT == 512 || BYTES <= 64 ? 2 : 1;
+};
+
+template <typename T, int DP, int RW>
+__global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, RW>::PER_SIMD)) diff_dkv_kernel(grad_args a) {
+	using S  = dkv_shape<T, DP, RW>;
+	using TK = tile<T, DP>;
+	using TV = tile<T, S::DV>;
+	constexpr int E = kind<T>::E, QT = S::QT, MAPS = S::MAPS;
+	const af3_diff_attention_params& p = a.p;
+	extern __shared__ __align__(16) unsigned char smem[];
+
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+	const int map0 = MAPS == 2 ? 0 : wave & 1, in_group = MAPS == 2 ? wave : wave >> 1, rwave = in_group % RW, group = in_group / RW;   // (map0: the wavefront's first map)
+	const share    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.tiles * a.splits);
+	const uint32_t split = own.piece / a.tiles, key_tile = own.piece - split * a.tiles;   // (causal: the first keys have the most rows)
+	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
+	const int64_t G = p.H / p.Hkv;
+	const int     D = (int)p.D, Dv = (int)p.Dv;
+
+	const int64_t key0 = (int64_t)key_tile * S::KEYS, key = key0 + 32 * group + (lane & 31);
+	const bool    in = key < p.Lk;
+	const bool    lives = in && (!p.key_mask || p.key_mask[b * p.key_mask_stride_b + key] != 0);
+	u32x4 kf[MAPS][TK::STEPS], vf[TV::STEPS];
+#pragma unroll
+	for(int i = 0; i < MAPS; i++) load_operand<T, DP>(kf[i], static_cast<const T*>(p.k) + b * p.k_stride[0] + (2 * hk + map0 + i) * p.k_stride[1] + (in ? key : 0) * p.k_stride[2], in, D, lane);
+	load_operand<T, S::DV>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], in, Dv, lane);
+	const bool work = __any(lives);   // (of this wavefront)
+
+	f32x16 dk[MAPS][TK::BLOCKS], dv[TV::BLOCKS];
+#pragma unroll
+	for(int i = 0; i < MAPS; i++)
+#pragma unroll
+		for(int db = 0; db < TK::BLOCKS; db++) dk[i][db] = f32x16{};
+#pragma unroll
+	for(int db = 0; db < TV::BLOCKS; db++) dv[db] = f32x16{};
+
+	const int64_t q_tiles = (p.Lq + QT - 1) / QT, n = G * q_tiles;
+	// (causal: queries in front of the workgroup's first key have nothing of it)
+	const int64_t from = p.causal && key0 > p.q_offset ? (key0 - p.q_offset) / QT : 0;
+	const int64_t last = (int64_t)(split + 1) * a.part < n ? (int64_t)(split + 1) * a.part : n;
+	const typename TK::reader at_q(lane);
+	const typename TV::reader at_g(lane);
+	passage<T, DP, QT, S::NT>    pq[2];
+	passage<T, S::DV, QT, S::NT> pg;
+	pq[0].begin(nullptr, p.q_stride[2], D, a.whole_k);
+	pq[1].begin(nullptr, p.q_stride[2], D, a.whole_k);
+	pg.begin(nullptr, a.g.grad_out_stride[2], Dv, a.whole_v);
+	row_stats<T, QT> rs;
+	auto fetch = [&](int64_t it) {
+		const int64_t h = hk * G + it / q_tiles, q0 = it % q_tiles * QT;
+		pq[0].base = static_cast<const T*>(p.q) + b * p.q_stride[0] + 2 * h * p.q_stride[1];
+		pq[1].base = pq[0].base + p.q_stride[1];
+		pg.base = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1];
+		pq[0].load(q0, p.Lq), pq[1].load(q0, p.Lq), pg.load(q0, p.Lq);
+		rs.load(a, b, h, q0);
+	};
+	auto next = [&](int64_t it) {   // the first tile from `it` on that counts
+		const int64_t head = it / q_tiles;
+		return it - head * q_tiles < from ? (from < q_tiles ? head * q_tiles + from : (head + 1) * q_tiles + from) : it;
+	};
+	int     buffer = 0;
+	int64_t it = from < q_tiles ? next((int64_t)split * a.part) : last;
+	// (a workgroup none of whose keys counts has nothing to read)
+	const bool any = __syncthreads_or(work);
+	if(!any) it = last;
+	if(it < last) fetch(it);
+	while(it < last) {
+		unsigned char* const qs = smem + buffer * S::SET;
+		unsigned char* const gs = qs + 2 * S::QTILE;
+		float* const         st = reinterpret_cast<float*>(gs + S::GTILE);
+		const int64_t        q0 = it % q_tiles * QT;
+		const float          lam = lam_of(p, hk * G + it / q_tiles);
+		if constexpr(S::BUFFERS == 1) __syncthreads();
+		const int64_t left = p.Lq - q0;
+		pq[0].store(qs, left >= QT, [&](int r) { return r < left; });
+		pq[1].store(qs + S::QTILE, left >= QT, [&](int r) { return r < left; });
+		pg.store(gs, left >= QT, [&](int r) { return r < left; });
+		rs.store(st, a.factor);
+		__syncthreads();
+		const bool    apart = rs.apart(st);
+		const int64_t following = next(it + 1);
+		if(following < last) fetch(following);
+		if(work) {
+#pragma unroll
+			for(int s = 0; s < S::SUB; s++) {
+				const int row0 = 32 * (rwave * S::SUB + s);
+				if(q0 + row0 >= p.Lq) continue;
+				// the lane's rows need .. 15 of its 16 count
+				const int need = p.causal ? clamped(key - p.q_offset - (q0 + row0 + 16 * half)) : -64;
+				if(!__any(in && need <= 15)) continue;
+				const bool diagonal = __any(in && need > 0);
+				const float* const sm = st + row0 + 16 * half;
+				f32x16 dp{};
+#pragma unroll
+				for(int i = 0; i < TV::STEPS; i++) dp = kind<T>::mma(TV::row_frag(gs, row0, i, at_g), vf[i], dp);
+				float both[16];   // P1 - lam P2 (or the wavefront's part of it)
+#pragma unroll
+				for(int i = 0; i < MAPS; i++) {
+					const int                  map = map0 + i;
+					const unsigned char* const qm = qs + map * S::QTILE;
+					f32x16 acc{};
+#pragma unroll
+					for(int k = 0; k < TK::STEPS; k++) acc = kind<T>::mma(TK::row_frag(qm, row0, k, at_q), kf[i][k], acc);
+					float x[16], y[16];
+					if(apart) {
+						const f32x16 m = rs.sixteen(sm + (MOST + map) * QT), inv = rs.sixteen(sm + (INVERSE + map) * QT);
+#pragma unroll
+						for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f((acc[r] - m[r]) * a.factor) * inv[r];
+					} else {
+						const f32x16 taken = rs.sixteen(sm + (TAKEN + map) * QT);
+#pragma unroll
+						for(int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r], a.factor, -taken[r]));
+					}
+					if(diagonal) {
+#pragma unroll
+						for(int r = 0; r < 16; r++) x[r] = r >= need ? x[r] : 0.f;
+					}
+					if(map == 1) {
+#pragma unroll
+						for(int r = 0; r < 16; r++) x[r] *= -lam;
+					}
+					const f32x16 less = rs.sixteen(sm + (LESS + map) * QT);
+#pragma unroll
+					for(int r = 0; r < 16; r++) {
+						y[r]    = x[r] * (dp[r] - less[r]);
+						both[r] = i == 0 ? x[r] : both[r] + x[r];
+					}
+#pragma unroll
+					for(int j = 0; j < TK::JOINTS; j++) {
+						const u32x4 df = kind<T>::pack(y + E * j);
+#pragma unroll
+						for(int db = 0; db < TK::BLOCKS; db++) dk[i][db] = kind<T>::mma(TK::col_frag(qm, row0, db, j, at_q), df, dk[i][db]);
+					}
+				}
+#pragma unroll
+				for(int j = 0; j < TV::JOINTS; j++) {
+					const u32x4 pf = kind<T>::pack(both + E * j);
+#pragma unroll
+					for(int db = 0; db < TV::BLOCKS; db++) dv[db] = kind<T>::mma(TV::col_frag(gs, row0, db, j, at_g), pf, dv[db]);
+				}
+			}
+		}
+		it = following;
+		if constexpr(S::BUFFERS == 2) buffer ^= 1;
+	}
+	float* const tables = reinterpret_cast<float*>(smem);
+	if constexpr(RW > 1) {
+#pragma unroll
+		for(int i = 0; i < MAPS; i++) add_up<DP, RW>(tables + (MAPS == 2 ? group : 2 * group + map0) * RW * 32 * (DP + 4), rwave, lane, dk[i]);
+	}
+	const int vwave = MAPS == 2 ? rwave : 2 * rwave + map0;
+	if constexpr(S::VW > 1) add_up<S::DV, S::VW>(tables + group * S::VW * 32 * (S::DV + 4), vwave, lane, dv);
+	if(!in) return;
+	const int64_t n_keys = p.B * p.Hkv * p.Lk, place = (b * p.Hkv + hk) * p.Lk + key;
+	float* const  partial = a.partial + (int64_t)split * n_keys * (2 * D + Dv);
+#pragma unroll
+	for(int i = 0; i < MAPS; i++) {
+		const int64_t to = (b * 2 * p.Hkv + 2 * hk + map0 + i) * p.Lk + key;
+#pragma unroll
+		for(int db = 0; db < TK::BLOCKS; db++) {
+			if(db % RW != rwave) continue;
+			float k[16];
+#pragma unroll
+			for(int r = 0; r < 16; r++) k[r] = lives ? dk[i][db][r] * p.softmax_scale : 0.f;
+			if(a.splits > 1) store_row16(partial + to * D, 32 * db + 16 * half, D, k);
+			else if(a.g.grad_k) store_row16(static_cast<T*>(a.g.grad_k) + to * D, 32 * db + 16 * half, D, k);
+		}
+	}
+#pragma unroll
+	for(int db = 0; db < TV::BLOCKS; db++) {
+		if(db % S::VW != vwave) continue;
+		float v[16];
+#pragma unroll
+		for(int r = 0; r < 16; r++) v[r] = lives ? dv[db][r] : 0.f;
+		if(a.splits > 1) store_row16(partial + 2 * n_keys * D + place * Dv, 32 * db + 16 * half, Dv, v);
+		else if(a.g.grad_v) store_row16(static_cast<T*>(a.g.grad_v) + place * Dv, 32 * db + 16 * half, Dv, v);
+	}
+}
+
+// dlam: a workgroup per head, over the batch and the queries; each thread's numbers in turn, then the threads' pairwise
+constexpr int LAM_THREADS = 1024;
+__global__ void __launch_bounds__(LAM_THREADS) diff_lam_kernel(grad_args a) {
+	__shared__ double sums[LAM_THREADS];
+	const af3_diff_attention_params& p = a.p;
+	const int64_t h = blockIdx.x, n = p.B * p.Lq;
+	double sum = 0.0;
+#pragma unroll 4
+	for(int64_t i = threadIdx.x; i < n; i += LAM_THREADS) {
+		const int64_t b = i / p.Lq;
+		sum += (double)a.d2[(b * p.H + h) * p.Lq + (i - b * p.Lq)];
+	}
+	sums[threadIdx.x] = sum;
+	for(int k = LAM_THREADS / 2; k; k >>= 1) {
+		__syncthreads();
+		if((int)threadIdx.x < k) sums[threadIdx.x] += sums[threadIdx.x + k];
+	}
+	if(threadIdx.x) return;
+	if(p.lam_dtype == AF3_F32) static_cast<float*>(a.g.grad_lam)[h] = (float)-sums[0];
+	else static_cast<uint16_t*>(a.g.grad_lam)[h] = kind<uint16_t>::bits((float)-sums[0]);
+}
+
+// The parts' sums added in order, of up to three results at once (a result of one part was written where it belongs).
+constexpr int RESULTS = 3;
+struct parts {
+	const float* partial[RESULTS];
+	int64_t      step[RESULTS], n[RESULTS];   // elements from one part to the next, elements
+	uint32_t     splits[RESULTS], blocks[RESULTS];
+	void*        out[RESULTS];
+};
+template <typename T>
+__global__ void __launch_bounds__(THREADS) diff_sum_kernel(parts a) {
+	uint32_t block = blockIdx.x;
+	int      which = 0;
+	while(which < RESULTS - 1 && block >= a.blocks[which]) block -= a.blocks[which++];
+	const int64_t  i = ((int64_t)block * THREADS + threadIdx.x) * 4, n = a.n[which], step = a.step[which];
+	const uint32_t splits = a.splits[which];
+	const float*   at = a.partial[which] + i;
+	T* const       out = static_cast<T*>(a.out[which]) + i;
+	if(i >= n) return;
+	if(i + 4 <= n) {
+		f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+		for(uint32_t s = 0; s < splits; s++, at += step) sum += *reinterpret_cast<const f32x4_any*>(at);
+#pragma unroll
+		for(int e = 0; e < 4; e++) out[e] = kind<T>::bits(sum[e]);
+	} else {
+		for(int e = 0; i + e < n; e++) {
+			float x = 0.f;
+			for(uint32_t s = 0; s < splits; s++) x += at[s * step + e];
+			out[e] = kind<T>::bits(x);
+		}
+	}
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------
+int width(const af3_diff_attention_params& p);   // (diff_attention.hip)
+
+struct cut {
+	bool     shared;   // wavefronts share 32 rows (dq) or keys (dkv)
+	uint32_t tiles, splits;
+	int64_t  part;
+};
+inline int64_t over(int64_t n, int64_t per) { return (n + per - 1) / per; }
+// bytes of a row of K as the kernels have it
+int row_bytes(const af3_diff_attention_params& p) { return width(p) * (p.dtype == AF3_F32 ? 4 : 2); }
+
+// `length` rows that results belong to (`alone` or `together` of them per workgroup), `steps(shared)` tiles of the other axis.  Wavefronts share where their workgroups fit the chip together.
+template <typename F>
+cut cut_for(int64_t length, int64_t groups, int64_t alone, int64_t together, bool may_share, int64_t slots, double tile_us, double part_bytes, F steps) {
+	cut c;
+	c.shared = may_share && (length <= together || over(length, together) * groups <= slots);
+	c.tiles  = (uint32_t)over(length, c.shared ? together : alone);
+	const int64_t n = steps(c.shared);
+	const int64_t sp = parts_for(groups * c.tiles, slots, n, tile_us * (c.shared ? 1.0 : 0.6), part_bytes, 64);
+	c.part   = over(n, sp);
+	c.splits = (uint32_t)over(n, c.part);
+	return c;
+}
+constexpr bool may_share(int bytes) { return bytes <= 128; }   // (wider rows: the tile of 128 leaves neither registers nor LDS)
+cut dq_cut(const af3_diff_attention_params& p) {
+	const int     bytes = row_bytes(p);
+	const int64_t rows = 32 * dq_threads(bytes) / 64 * dq_maps(bytes) / 2, kt = tile_rows(bytes, 1);
+	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, rows, rows / 4, may_share(bytes), 256, (0.5 + 0.025 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0), 8.0 * p.B * p.H * p.Lq * p.D,
+					[&](bool shared) { return over(p.Lk, shared ? 128 : kt); });
+	c.part *= c.shared ? 128 : kt;
+	return c;
+}
+cut dkv_cut(const af3_diff_attention_params& p) {
+	const int     bytes = row_bytes(p);
+	const int64_t keys = 32 * dkv_threads(bytes) / 64 * dkv_maps(bytes) / 2, qt = tile_rows(bytes, 1);
+	return cut_for(p.Lk, p.B * p.Hkv, keys, keys / 4, may_share(bytes), 256, (0.6 + 0.035 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0), 4.0 * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv),
+				   [&](bool shared) { return p.H / p.Hkv * over(p.Lq, shared ? 128 : qt); });
+}
+
+struct grad_space {
+	int64_t delta, dq, dkv, bytes;   // floats
+};
+grad_space grad_workspace(const af3_diff_attention_params& p) {
+	const cut  q = dq_cut(p), kv = dkv_cut(p);
+	grad_space w;
+	w.delta = over(p.B * p.H * p.Lq, 4) * 4;
+	w.dq    = q.splits > 1 ? over(2 * (int64_t)q.splits * p.B * p.H * p.Lq * p.D, 4) * 4 : 0;
+	w.dkv   = kv.splits > 1 ? over((int64_t)kv.splits * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv), 4) * 4 : 0;
+	w.bytes = (2 * w.delta + w.dq + w.dkv) * 4;
+	return w;
+}
+
+template <typename S, typename K>
+int launch(K kernel, uint32_t grid, const grad_args& a, hipStream_t s) {
+	constexpr int lds = S::LDS;
+	if(lds > 65536 - 8192 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+		(void)hipGetLastError();
+		return AF3_ERR_LAUNCH;
+	}
+	hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::NT), lds, s, a);
+	return launch_status();
+}
+
+template <typename T, int DP>
+int backward(grad_args a, hipStream_t s) {
+	const af3_diff_attention_params& p = a.p;
+	const int64_t n_rows = 2 * p.B * p.H * p.Lq, n_keys = p.B * p.Hkv * p.Lk;
+	constexpr bool SHARES = may_share(DP * (int)sizeof(T));
+	parts    sums{};
+	int      n_sums = 0;
+	uint32_t sum_blocks = 0;
+	auto add = [&](const float* partial, int64_t step, uint32_t splits, void* out, int64_t n) {
+		if(!out) return;
+		sums.partial[n_sums] = partial, sums.step[n_sums] = step, sums.n[n_sums] = n, sums.splits[n_sums] = splits, sums.out[n_sums] = out;
+		sum_blocks += sums.blocks[n_sums] = (uint32_t)over(n, 4 * THREADS);
+		n_sums++;
+	};
+	int rc = AF3_ERR_LAUNCH;
+	{   // (without grad_q: d1 and d2 alone)
+		const cut c = dq_cut(p);
+		a.tiles = c.tiles, a.splits = a.g.grad_q ? c.splits : 1, a.part = c.part, a.partial = a.dq_space;
+		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * a.tiles * a.splits;
+		if constexpr(SHARES)
+			if(c.shared) rc = launch<dq_shape<T, DP, 4>>(diff_dq_kernel<T, DP, 4>, grid, a, s);
+		if(!c.shared) rc = launch<dq_shape<T, DP, 1>>(diff_dq_kernel<T, DP, 1>, grid, a, s);
+		if(rc != AF3_OK) return rc;
+		if(a.splits > 1) add(a.partial, n_rows * p.D, c.splits, a.g.grad_q, n_rows * p.D);
+	}
+	if(a.g.grad_k || a.g.grad_v) {
+		const cut c = dkv_cut(p);
+		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part, a.partial = a.dkv_space;
+		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * c.tiles * c.splits;
+		rc = AF3_ERR_LAUNCH;
+		if constexpr(SHARES)
+			if(c.shared) rc = launch<dkv_shape<T, DP, 4>>(diff_dkv_kernel<T, DP, 4>, grid, a, s);
+		if(!c.shared) rc = launch<dkv_shape<T, DP, 1>>(diff_dkv_kernel<T, DP, 1>, grid, a, s);
+		if(rc != AF3_OK) return rc;
+		if(c.splits > 1) {
+			const int64_t step = n_keys * (2 * p.D + p.Dv);
+			add(a.partial, step, c.splits, a.g.grad_k, 2 * n_keys * p.D);
+			add(a.partial + 2 * n_keys * p.D, step, c.splits, a.g.grad_v, n_keys * p.Dv);
+		}
+	}
+	if(n_sums) {
+		hipLaunchKernelGGL(diff_sum_kernel<T>, dim3(sum_blocks), dim3(THREADS), 0, s, sums);
+		if(rc = launch_status(); rc != AF3_OK) return rc;
+	}
+	if(a.g.grad_lam) {
+		hipLaunchKernelGGL(diff_lam_kernel, dim3((uint32_t)p.H), dim3(LAM_THREADS), 0, s, a);
+		return launch_status();
+	}
+	return AF3_OK;
+}
+
+int validate_grads(const af3_diff_attention_params* p, const af3_diff_attention_grads* g) {
+	if(const int rc = validate_diff_attention(p); rc != AF3_OK) return rc;
+	if(!g || !g->grad_out || !p->stats || (!g->grad_q && !g->grad_k && !g->grad_v && !g->grad_lam)) return AF3_ERR_NULL_POINTER;
+	for(int i = 0; i < 3; i++)
+		if(g->grad_out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
+	return AF3_OK;
+}
+
+}  // namespace diff
+}  // namespace af3
+
+using namespace af3;
+
+extern "C" int64_t af3_diff_attention_backward_workspace_bytes(const af3_diff_attention_params* params) {
+	if(const int rc = validate_diff_attention(params); rc != AF3_OK) return rc;
+	return diff_gradients_fit(*params) ? diff::grad_workspace(*params).bytes : AF3_ERR_BAD_SHAPE;
+}
+
+extern "C" int af3_diff_attention_backward(const af3_diff_attention_params* params, const af3_diff_attention_grads* grads, void* hip_stream) {
+	if(const int rc = diff::validate_grads(params, grads); rc != AF3_OK) return rc;
+	const diff::grad_space w = diff::grad_workspace(*params);
+	if(!grads->workspace || grads->workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(grads->workspace) & 15)) return AF3_ERR_BAD_ARGUMENT;
+	if(const int dc = current_device_status(); dc != AF3_OK) return dc;
+	const bool      fp32 = params->dtype == AF3_F32;
+	diff::grad_args a;
+	a.p = *params, a.g = *grads, a.tiles = a.splits = 1, a.part = 0, a.partial = nullptr;
+	a.factor  = params->softmax_scale * LOG2E;
+	a.whole_k = params->D * (fp32 ? 4 : 2) % 16 == 0, a.whole_v = params->Dv * (fp32 ? 4 : 2) % 16 == 0;
+	a.d1 = static_cast<float*>(grads->workspace), a.d2 = a.d1 + w.delta, a.dq_space = a.d2 + w.delta, a.dkv_space = a.dq_space + w.dq;
+	const hipStream_t s = static_cast<hipStream_t>(hip_stream);
+	const int wide = diff::width(*params);
+	if(fp32) return wide == 32 ? diff::backward<float, 32>(a, s) : diff::backward<float, 64>(a, s);
+	return wide == 32 ? diff::backward<uint16_t, 32>(a, s) : wide == 64 ? diff::backward<uint16_t, 64>(a, s) : diff::backward<uint16_t, 128>(a, s);
+}

@@ -1254,6 +1254,117 @@ PyObject* py_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 	END_HANDLE_TH_ERRORS
 }
 
+// ---- differential attention --------------------------------------------------------------------------------------------------------
+struct diff_call {
+	Tensor  q, k, v, lam, mask;   // mask as bytes [1|B, Lk] or undefined
+	double  scale;
+	int64_t causal, offset;
+	af3_diff_attention_params block() const {
+		af3_diff_attention_params p{};
+		p.q = q.const_data_ptr(), p.k = k.const_data_ptr(), p.v = v.const_data_ptr(), p.lam = lam.const_data_ptr();
+		p.B = q.size(0), p.H = q.size(1) / 2, p.Lq = q.size(2), p.D = q.size(3), p.Hkv = v.size(1), p.Lk = k.size(2), p.Dv = v.size(3);
+		put_strides(p.q_stride, q), put_strides(p.k_stride, k), put_strides(p.v_stride, v);
+		if(mask.defined()) p.key_mask = static_cast<const uint8_t*>(mask.const_data_ptr()), p.key_mask_stride_b = mask.dim() > 1 && mask.size(0) != 1 ? mask.stride(0) : 0;
+		p.lam_stride = lam.stride(0), p.lam_dtype = dtype_code(lam), p.dtype = dtype_code(q);
+		p.causal = (int32_t)causal, p.q_offset = offset, p.softmax_scale = (float)scale;
+		return p;
+	}
+	int forward(Tensor& out, Tensor* stats, Tensor* second) const {
+		const int dev = (int)q.get_device();
+		af3_diff_attention_params p = block();
+		out   = new_tensor({p.B, p.H, p.Lq, p.Dv}, q.scalar_type(), dev);
+		p.out = out.data_ptr();
+		put_strides(p.out_stride, out);
+		if(stats) {
+			*stats = new_tensor({p.B, 2 * p.H, p.Lq, 2}, at::kFloat, dev), *second = new_tensor(out.sizes(), q.scalar_type(), dev);
+			p.stats = static_cast<float*>(stats->data_ptr()), p.second = second->data_ptr();
+		}
+		at::DataPtr   ws;
+		const int64_t bytes = af3_diff_attention_workspace_bytes(&p);
+		if(bytes < 0) return (int)bytes;
+		if(bytes > 0) ws = new_scratch(bytes), p.workspace = ws.get(), p.workspace_bytes = bytes;
+		return af3_diff_attention_forward(&p, current_stream(dev));
+	}
+};
+struct diff_function : torch::autograd::Function<diff_function> {
+	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const std::optional<Tensor>& given_mask, double scale,
+						  int64_t causal, int64_t offset) {
+		const Tensor mask = given_mask.value_or(Tensor());
+		Tensor       out, stats, second;
+		raise(diff_call{q, k, v, lam, mask, scale, causal, offset}.forward(out, &stats, &second), "af3_diff_attention_forward");
+		ctx->save_for_backward({q, k, v, lam, mask, out, stats, second});
+		ctx->saved_data["scale"] = scale, ctx->saved_data["causal"] = causal, ctx->saved_data["offset"] = offset;
+		return out;
+	}
+	static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grad_out) {
+		const auto      saved = ctx->get_saved_variables();
+		const diff_call call{saved[0], saved[1], saved[2], saved[3], saved[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toInt(), ctx->saved_data["offset"].toInt()};
+		const int       dev = (int)call.q.get_device();
+		Tensor          g = grad_out[0];
+		no_tangent(g, "the gradient of differential_attention");
+		torch::autograd::variable_list grads(8);
+		{
+			at::AutoGradMode none(false);
+			if(!inner_1(g)) g = g.contiguous();
+			af3_diff_attention_params p = call.block();
+			p.out = saved[5].data_ptr(), p.stats = static_cast<float*>(saved[6].data_ptr()), p.second = saved[7].data_ptr();
+			put_strides(p.out_stride, saved[5]);
+			af3_diff_attention_grads o{};
+			o.grad_out = g.const_data_ptr();
+			put_strides(o.grad_out_stride, g);
+			auto want = [&](int i, const Tensor& like) -> void* {
+				if(!ctx->needs_input_grad((size_t)i)) return nullptr;
+				grads[i] = new_tensor(like.sizes(), like.scalar_type(), dev);
+				return grads[i].data_ptr();
+			};
+			o.grad_q = want(0, call.q), o.grad_k = want(1, call.k), o.grad_v = want(2, call.v), o.grad_lam = want(3, call.lam);
+			const int64_t     bytes = af3_diff_attention_backward_workspace_bytes(&p);
+			raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_diff_attention_backward_workspace_bytes");
+			const at::DataPtr ws = new_scratch(bytes);
+			o.workspace = ws.get(), o.workspace_bytes = bytes;
+			raise(af3_diff_attention_backward(&p, &o, current_stream(dev)), "af3_diff_attention_backward");
+		}
+		return once(std::move(grads), "differential_attention");
+	}
+};
+// differential_attention(q, k, v, lam, mask, causal, q_offset, scale or None)
+PyObject* py_differential_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+	HANDLE_TH_ERRORS
+	if(n != 8) return none();
+	const Tensor *q = tensor_of(a[0]), *k = tensor_of(a[1]), *v = tensor_of(a[2]), *lam = tensor_of(a[3]);
+	if(!q || !k || !v || !lam || q->dim() != 4 || k->dim() != 4 || v->dim() != 4 || lam->dim() != 1 || q->numel() == 0 || k->numel() == 0 || v->numel() == 0) return none();
+	const int  dev  = device_of(q);
+	const auto type = q->scalar_type();
+	if(dev < 0 || dtype_code(*q) < 0 || k->scalar_type() != type || v->scalar_type() != type || (lam->scalar_type() != type && lam->scalar_type() != at::kFloat)) return none();
+	if(!on_device(*k, dev) || !on_device(*v, dev) || !on_device(*lam, dev) || !inner_1(*q) || !inner_1(*k) || !inner_1(*v)) return none();
+	const int64_t B = q->size(0), H = q->size(1) / 2, Hkv = v->size(1), Lk = k->size(2), D = q->size(3), most = type == at::kFloat ? 64 : 128;
+	if(q->size(1) != 2 * H || k->size(1) != 2 * Hkv || H % Hkv != 0 || lam->size(0) != H || k->size(0) != B || v->size(0) != B || k->size(3) != D || v->size(2) != Lk || D > most || v->size(3) > 2 * most) return none();
+	diff_call c{*q, *k, *v, *lam, Tensor(), 0.0, 0, 0};
+	key_mask  m;
+	if(!mask_of(a[4], B, Lk, dev, m)) return none();
+	if(a[4] != Py_None) {
+		const Tensor& t = *tensor_of(a[4]);
+		c.mask = t.dim() == 4 ? t.as_strided({t.size(0), Lk}, {t.stride(0), 1}) : t;
+	}
+	bool causal;
+	if(!truth_of(a[5], causal) || !number_of(a[6], c.offset) || c.offset >= (int64_t)1 << 40 || c.offset <= -((int64_t)1 << 40)) return none();
+	c.causal = causal;
+	c.scale  = std::pow((double)D, -0.5);
+	if(a[7] != Py_None && !real_of(a[7], c.scale)) return none();
+	if(!((float)c.scale > 0.f && (float)c.scale < INFINITY) || has_tangent({q, k, v, lam})) return none();
+	Tensor out;
+	int    rc = AF3_OK;
+	const bool graph = wants_grad({q, k, v, lam});
+	if(graph && B * Hkv * ((Lk + 31) / 32) > 0xffffff) return none();   // (sizes whose gradients would be refused: the Python side says so)
+	{
+		without_gil g;
+		if(graph) check_capture({q, k, v, lam}, dev), out = diff_function::apply(c.q, c.k, c.v, c.lam, given(c.mask), c.scale, c.causal, c.offset);
+		else rc = c.forward(out, nullptr, nullptr);
+	}
+	return answer(rc, std::move(out));
+	END_HANDLE_TH_ERRORS
+}
+
 // check_capture(tensor or None...): raises where a gradient of these cannot be captured
 PyObject* py_check_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
 	HANDLE_TH_ERRORS
@@ -1281,6 +1392,7 @@ PyMethodDef methods[] = {
 	AF3_FN(position_bias, "position_bias(table, q_len, k_len, scheme, bidirectional, max_distance, q_positions, k_positions, q_offset)"),
 	AF3_FN(rotary, "rotary(q, k, frequencies, positions, offset, interleaved, scale)"),
 	AF3_FN(residual_norm, "residual_norm(x, y, weight, bias, gate, post_weight, norm, post_norm, sigmoid, residual_scale, eps)"),
+	AF3_FN(differential_attention, "differential_attention(q, k, v, lam, mask, causal, q_offset, scale)"),
 	AF3_FN(check_capture, "check_capture(tensor...): raises where their gradients cannot be captured into a graph"),
 	AF3_FN(remember, "remember(tag, value, source...): a matrix derived from weights"),
 	AF3_FN(recalls, "recalls(tag, source...): whether one is remembered for these"),

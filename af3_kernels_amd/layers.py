@@ -1,10 +1,11 @@
-"""What a layer around its attention is made of, beside the attention calls themselves.
+"""What a decoder's or a conditioned transformer's layer is made of, beside cross_attention.
 
     rotary_frequencies, rotary_embedding   positions as turns of the pairs of a head, instead of a bias
+    differential_attention                 the difference of two softmax maps over one set of values
     residual_norm                          the end of one block and the beginning of the next: norm, gate, residual stream, norm
 
-Both work under autograd (first derivatives).  The reference has neither; its LayerNorm is torch's (src/af3_kernels/Attention.py:51).  Every computation on
-the device happens in libaf3_dpa.so (af3_rotary_embedding, af3_residual_norm_*); there is no CPU path.
+All work under autograd (first derivatives).  The reference has none of them; its LayerNorm is torch's (src/af3_kernels/Attention.py:51).  Every computation on
+the device happens in libaf3_dpa.so (af3_rotary_embedding, af3_diff_attention_*, af3_residual_norm_*); there is no CPU path.
 """
 import ctypes
 import math
@@ -13,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib, ops
-from ._lib import ResidualNormGrads, ResidualNormParams, RotaryParams
+from ._lib import DiffAttentionGrads, DiffAttentionParams, ResidualNormGrads, ResidualNormParams, RotaryParams
 from .cross import _DTYPES, _inner_contig, _no_tangents, _same_device
 
 _host = ops._host
@@ -160,6 +161,134 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], frequencies: to
             _host.check_capture(q, k)
         return _Rotary.apply(q, k, frequencies, positions, offset, interleaved, scale)
     return tuple(_turn((q, k), frequencies, positions, offset, interleaved, scale, False))
+
+
+# ---- differential attention -------------------------------------------------------------------------------------------------
+def _diff_block(q, k, v, lam, keep, out, stats, second, causal, offset, scale) -> DiffAttentionParams:
+    p = DiffAttentionParams()
+    p.q, p.k, p.v, p.lam, p.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), out.data_ptr()
+    p.B, p.H, p.Lq, p.Dv = out.shape
+    p.D, p.Hkv, p.Lk = q.shape[3], v.shape[1], v.shape[2]
+    p.q_stride, p.k_stride, p.v_stride, p.out_stride = (_i64x3(*t.stride()[:3]) for t in (q, k, v, out))
+    if keep is not None:
+        p.key_mask, p.key_mask_stride_b = keep.data_ptr(), 0 if keep.shape[0] == 1 else keep.stride(0)
+    if stats is not None:
+        p.stats, p.second = stats.data_ptr(), second.data_ptr()
+    p.lam_stride, p.lam_dtype, p.dtype = lam.stride(0), _DTYPES[lam.dtype], _DTYPES[q.dtype]
+    p.causal, p.q_offset, p.softmax_scale = int(causal), offset, scale
+    return p
+
+
+def _diff_forward(q, k, v, lam, keep, causal, offset, scale, want_stats):
+    """(out, stats, second): where the gradient will be asked for, stats [B, 2H, Lq, 2] and the second map's own result."""
+    B, H, Lq = q.shape[0], q.shape[1] // 2, q.shape[2]
+    out = torch.empty(B, H, Lq, v.shape[3], dtype=q.dtype, device=q.device)
+    if out.numel() == 0 or k.shape[2] == 0:
+        return out.zero_(), None, None
+    stats = torch.empty(B, 2 * H, Lq, 2, dtype=torch.float32, device=q.device) if want_stats else None
+    second = torch.empty_like(out) if want_stats else None
+    p = _diff_block(q, k, v, lam, keep, out, stats, second, causal, offset, scale)
+    lib = _lib.load()
+    with ops._on_device(q.device):
+        need = lib.af3_diff_attention_workspace_bytes(ctypes.byref(p))
+        if need > 0:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        _lib.check(lib.af3_diff_attention_forward(ctypes.byref(p), ops._stream_ptr(q.device)), "af3_diff_attention_forward")
+    return out, stats, second
+
+
+class _DifferentialAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, keep, causal, offset, scale):
+        out, stats, second = _diff_forward(q, k, v, lam, keep, causal, offset, scale, True)
+        ctx.save_for_backward(q, k, v, lam, keep, out, stats, second)
+        ctx.settings = (causal, offset, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        _no_tangents("the gradient of differential_attention", grad)
+        q, k, v, lam, keep, out, stats, second = ctx.saved_tensors
+        wants = ctx.needs_input_grad[:4]
+        if stats is None:
+            return (*(torch.zeros(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v, lam), wants)), None, None, None, None)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v, lam), wants)]
+        grad = _inner_contig(grad)
+        p, g = _diff_block(q, k, v, lam, keep, out, stats, second, *ctx.settings), DiffAttentionGrads()
+        g.grad_out, g.grad_out_stride = grad.data_ptr(), _i64x3(*grad.stride()[:3])
+        g.grad_q, g.grad_k, g.grad_v, g.grad_lam = (0 if t is None else t.data_ptr() for t in grads)
+        lib = _lib.load()
+        with ops._on_device(q.device):
+            need = lib.af3_diff_attention_backward_workspace_bytes(ctypes.byref(p))
+            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+            g.workspace, g.workspace_bytes = ws.data_ptr(), need
+            _lib.check(lib.af3_diff_attention_backward(ctypes.byref(p), ctypes.byref(g), ops._stream_ptr(q.device)), "af3_diff_attention_backward")
+        return (*grads, None, None, None, None)
+
+
+def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, mask: Optional[torch.Tensor] = None, causal: bool = False, q_offset: int = 0,
+                           softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """(softmax(q1.k1^T * softmax_scale) - lam * softmax(q2.k2^T * softmax_scale)) . v for every head: what two attention maps have in common cancels.
+
+    q [B, 2 H, Lq, D]: query heads 2 h and 2 h + 1 are the two maps of head h; k [B, 2 Hkv, Lk, D] likewise; v [B, Hkv, Lk, Dv] with H a multiple of Hkv (head h uses key
+    head h // (H // Hkv)); the result is [B, H, Lq, Dv].  lam [H], or one number for all heads (a tensor of one element): float32 or q's dtype, anything else is cast to float32.
+    bfloat16: D up to 128, Dv up to 256; float32: half of that.  mask [Lk], [B, Lk] or [B, 1, 1, Lk], truthy = attend; causal: key j counts for query i if j <= i + q_offset (a
+    decoder's token t: Lq = 1, q_offset = t).  softmax_scale: D^-1/2 unless given.  float32 (fp32 throughout) or bfloat16 (bf16 products, fp32 accumulation and softmax; the
+    probabilities and, in the gradient, dS are rounded to bf16 for the products that follow); k and v are cast to q's dtype.  Any strides; a new contiguous tensor.
+
+    A key that `mask` drops has no part in the result or its gradient, whatever k and v hold there.  A query that is left without a key, by mask and causality, gives zeros and
+    has no gradient (not the mean of its values as in cross_attention: of a difference nothing is left).  Keys behind a causal query have weight zero for it, which NaN and
+    infinities in their k and v do not heed where other queries of the call see those keys.  Lk == 0 gives zeros.
+
+    Gradients flow to q, k, v and lam (the same bits every time); a second derivative and forward mode raise.  In a HIP graph: as cross_attention."""
+    out = _host.differential_attention(q, k, v, lam, mask, causal, q_offset, softmax_scale)
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_diff_attention_forward")
+    _no_tangents("differential_attention", q, k, v, lam)
+    _same_device(q, k, v, lam, mask)
+    if q.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {q.dtype}: float32 or bfloat16")
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"q must be [B, 2 H, Lq, D], k [B, 2 Hkv, Lk, D] and v [B, Hkv, Lk, Dv], got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    B, H, Lq, D = q.shape[0], q.shape[1] // 2, q.shape[2], q.shape[3]
+    Hkv, Lk, Dv = v.shape[1], k.shape[2], v.shape[3]
+    if q.shape[1] % 2 or tuple(k.shape) != (B, 2 * Hkv, Lk, D) or v.shape[0] != B or v.shape[2] != Lk:
+        raise ValueError(f"q must be [B, 2 H, Lq, D], k [B, 2 Hkv, Lk, D] and v [B, Hkv, Lk, Dv], got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    if Hkv == 0 or H % Hkv != 0:
+        raise ValueError(f"the heads must be a multiple of the key heads, got {H} and {Hkv}")
+    most = 64 if q.dtype == torch.float32 else 128
+    if not 1 <= D <= most or not 1 <= Dv <= 2 * most:
+        raise ValueError(f"head_dim must be 1 to {most} and v's 1 to {2 * most} in {q.dtype}, got {D} and {Dv}")
+    if lam.numel() != 1 and tuple(lam.shape) != (H,):
+        raise ValueError(f"lam must be [H] with H={H}, or one number, got {tuple(lam.shape)}")
+    keep = ops._lift_mask(mask, None) if mask is not None else None
+    if keep is not None and (keep.shape[1] != Lk or keep.shape[0] not in (1, B)):
+        raise ValueError(f"mask must be [Lk], [B, Lk] or [B, 1, 1, Lk] with B={B}, Lk={Lk}, got {tuple(mask.shape)}")
+    causal, q_offset = bool(causal), int(q_offset)
+    if abs(q_offset) >= 1 << 40:
+        raise ValueError(f"q_offset must lie within 2^40, got {q_offset}")
+    scale = float(D) ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if not 0.0 < scale <= _LIMIT:
+        raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
+    dtype = q.dtype
+    q, k, v = _inner_contig(q), _inner_contig(k if k.dtype == dtype else k.to(dtype)), _inner_contig(v if v.dtype == dtype else v.to(dtype))
+    if lam.dtype not in (dtype, torch.float32):
+        lam = lam.to(torch.float32)
+    lam = lam.reshape(1).expand(H) if tuple(lam.shape) != (H,) else lam
+    graph = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam))
+    if graph and B * Hkv * -(-Lk // 32) >= 1 << 24:
+        raise ValueError(f"gradients take B * Hkv * ceil(Lk / 32) below 2^24, got {B} * {Hkv} * ceil({Lk} / 32)")
+    with ops._on_device(q.device):   # (as a plain call)
+        out = _host.differential_attention(q, k, v, lam, None if keep is None else keep.view(torch.bool), causal, q_offset, scale)
+    if out is not None:
+        return out if out.__class__ is not int else _lib.check(out, "af3_diff_attention_forward")
+    if graph:
+        with ops._on_device(q.device):
+            _host.check_capture(q, k, v, lam)
+        return _DifferentialAttention.apply(q, k, v, lam, keep, causal, q_offset, scale)
+    return _diff_forward(q, k, v, lam, keep, causal, q_offset, scale, False)[0]
 
 
 # ---- norms around a block ---------------------------------------------------------------------------------------------------

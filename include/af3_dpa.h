@@ -439,6 +439,71 @@ int     af3_position_bias_backward(const af3_position_bias_params* params, void*
 int64_t af3_position_bias_workspace_bytes(const af3_position_bias_params* params);   /* host only */
 
 /*
+ * Differential attention: head h's result is the difference of two softmax maps over one set of values,
+ *     out[b, h] = (softmax(q[b, 2 h] . k[b, 2 hk]^T softmax_scale) - lam[h] softmax(q[b, 2 h + 1] . k[b, 2 hk + 1]^T softmax_scale)) . v[b, hk],   hk = h / (H / Hkv).
+ * No reference counterpart.
+ *   q           : [B, 2 H, Lq, D]; k: [B, 2 Hkv, Lk, D]; v: [B, Hkv, Lk, Dv]; out: [B, H, Lq, Dv]; H a multiple of Hkv.  Element strides for the first three axes,
+ *                 innermost stride 1, any alignment of the element type.  Inputs may have strides of 0.
+ *   lam         : H numbers (device memory) of lam_dtype (AF3_F32, or AF3_BF16), lam_stride elements apart (0: one for all heads).
+ *   key_mask    : bytes, non-zero = attend, [B, Lk] with batch stride key_mask_stride_b (0: one row for the batch); NULL: all.  Nothing that k and v hold for a dropped key
+ *                 reaches a result.
+ *   causal      : key j counts for query i if j <= i + q_offset.  (A key that counts for some queries of the call has weight zero for the others: NaN and infinities
+ *                 of its v reach those too.)
+ *                 A query that is left without a key by mask and causality yields zeros, and has no part in a gradient.
+ *   dtype       : AF3_BF16 (bf16 products, fp32 accumulation and softmax) or AF3_F32 (fp32 throughout), of q, k, v, out.
+ *   stats, second : optional, both or neither, for af3_diff_attention_backward: [B, 2 H, Lq, 2] floats (maximum in the softmax's units and 1 / sum) and
+ *                 [B, H, Lq, Dv] contiguous of `dtype` (the second map's own result).
+ *   workspace   : af3_diff_attention_workspace_bytes() bytes, 16-byte aligned; NULL where that is 0.  Overwritten.
+ * B, H, Lq, Lk, D, Dv >= 1; D <= 128 and Dv <= 256 (AF3_F32: D <= 64 and Dv <= 128; AF3_ERR_UNSUPPORTED_D); Lq and Lk < 2^30, H < 2^15, H * Lq < 2^30,
+ * B * H * ceil(Lq / 32) < 2^24; with stats B * Hkv * ceil(Lk / 32) < 2^24 too; |q_offset| < 2^40.  AF3_ERR_BAD_SHAPE otherwise, from the workspace call as well.
+ */
+typedef struct af3_diff_attention_params {
+	const void*    q;
+	const void*    k;
+	const void*    v;
+	const void*    lam;
+	const uint8_t* key_mask;
+	void*          out;
+	float*         stats;
+	void*          second;
+	int64_t        B, H, Hkv, Lq, Lk, D, Dv;
+	int64_t        q_stride[3];
+	int64_t        k_stride[3];
+	int64_t        v_stride[3];
+	int64_t        out_stride[3];
+	int64_t        lam_stride;
+	int64_t        key_mask_stride_b;
+	int64_t        q_offset;
+	int32_t        dtype, lam_dtype, causal;
+	float          softmax_scale;
+	void*          workspace;
+	int64_t        workspace_bytes;
+} af3_diff_attention_params;
+
+int     af3_diff_attention_forward(const af3_diff_attention_params* params, void* hip_stream);
+int64_t af3_diff_attention_workspace_bytes(const af3_diff_attention_params* params);   /* host only */
+
+/*
+ * Gradients of af3_diff_attention_forward.  `params` as in the forward call, with the out, stats and second that it wrote (its workspace is not used); grad_out
+ * [B, H, Lq, Dv] with strides, of `dtype`.  grad_q [B, 2 H, Lq, D], grad_k [B, 2 Hkv, Lk, D], grad_v [B, Hkv, Lk, Dv] are contiguous and written whole, zeros for
+ * dropped keys among it; grad_lam: H contiguous numbers of lam_dtype (one for each head, also where lam_stride is 0).  NULL: not wanted.  No atomics: the same bits every time.
+ * workspace: af3_diff_attention_backward_workspace_bytes() bytes, 16-byte aligned, required.
+ */
+typedef struct af3_diff_attention_grads {
+	const void* grad_out;
+	int64_t     grad_out_stride[3];
+	void*       grad_q;
+	void*       grad_k;
+	void*       grad_v;
+	void*       grad_lam;
+	void*       workspace;
+	int64_t     workspace_bytes;
+} af3_diff_attention_grads;
+
+int     af3_diff_attention_backward(const af3_diff_attention_params* params, const af3_diff_attention_grads* grads, void* hip_stream);
+int64_t af3_diff_attention_backward_workspace_bytes(const af3_diff_attention_params* params);   /* host only */
+
+/*
  * Rotary positions of queries and keys in one launch: pair i of a head's first `rotary` elements is turned by position * frequencies[i],
  *     (x, y) -> scale (x cos a - y sin a, x sin a + y cos a);   inverse: by -a, which is the gradient.
  * The other elements go through as they are.  No reference counterpart.
