@@ -111,7 +111,7 @@ class ResidualNormGrads(ctypes.Structure):
 class DiffAttentionParams(ctypes.Structure):
     """Mirror of struct af3_diff_attention_params."""
     _fields_ = [
-        ("q", vp), ("k", vp), ("v", vp), ("lam", vp), ("key_mask", vp), ("out", vp), ("stats", vp), ("second", vp),
+        ("q", vp), ("k", vp), ("v", vp), ("lam", vp), ("key_mask", vp), ("out", vp), ("stats", vp), ("second", vp), ("residuals", vp),
         ("B", i64), ("H", i64), ("Hkv", i64), ("Lq", i64), ("Lk", i64), ("D", i64), ("Dv", i64),
         ("q_stride", i64 * 3), ("k_stride", i64 * 3), ("v_stride", i64 * 3), ("out_stride", i64 * 3),
         ("lam_stride", i64), ("key_mask_stride_b", i64), ("q_offset", i64),

@@ -18,11 +18,90 @@ struct forward_args {
 	float    factor;               // exp2((t - max) * factor) with t = q.k
 	int32_t  whole_k, whole_v;     // D, Dv are whole numbers of 16-byte pieces
 	float*   part_out;             // [splits][2][B * Hkv * G * Lq][Dv] and ...
+	void*    values;               // V as fp16, tile after tile, and its tiles' units, or null
+	float*   units;
 	float*   part_stat;            // ... [splits][2][B * Hkv * G * Lq][2] (maximum, sum); sum 0: no live key in the part, and nothing written
 };
 
+// what a result loses by its rounding to bf16, itself as bf16: the gradient's row sums then have the result to 16 bits.  which: 0 of out, 1 of the second map's own
+template <typename T>
+__device__ __forceinline__ void store_residual(const af3_diff_attention_params& p, int which, int64_t row, int d, const float (&v)[16]) {
+	if constexpr(sizeof(T) == 2) {
+		if(!p.residuals) return;
+		float r[16];
+#pragma unroll
+		for(int i = 0; i < 16; i++) r[i] = v[i] - kind<T>::value(kind<T>::bits(v[i]));
+		store_row16(static_cast<T*>(p.residuals) + (which * p.B * p.H * p.Lq + row) * p.Dv, d, (int)p.Dv, r);
+	}
+}
+
+// ---- the values as fp16 ----
+// The rounding of P to bf16 in front of its product with V would be felt more here than in one map: where the maps have much in common their difference loses size and
+// the roundings do not (lam 0.8, logits of variance 1: out off by 1.6 times its own last rounding).  In short launches, whose matrix instructions are few, P goes in two terms, the second
+// what the first one lost.  In long ones it goes as fp16, which has three bits more, and V with it: its bf16 values times a power of two, the tile's unit, are fp16 values as they stand
+// (those of 2^-22 of the tile's largest and less are off by 2^-25 / unit).  Laid out so once, rows of dropped keys as zeros, a tile is then taken as it is by all that read it.  Converted
+// where it is read instead, 2 x 16 (4) x 4096 x 64 took 352 us in place of 278 (between two barriers, with no other workgroup on the compute unit to fill them).
+constexpr int   value_rows(int dp) { return dp == 32 ? 128 : 64; }   // (a whole number of the main kernel's tiles)
+constexpr float UNIT = 256.f, UNIT_BELOW = 32768.f, UNIT_ABOVE = 0x1p-7f;   // the unit of a tile whose largest lies between these of it
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+	const f16x2 p = {(_Float16)lo, (_Float16)hi};
+	return __builtin_bit_cast(uint32_t, p);
+}
+__device__ __forceinline__ u32x4 pack_f16(const float* r) { return u32x4{pack_f16x2(r[0], r[1]), pack_f16x2(r[2], r[3]), pack_f16x2(r[4], r[5]), pack_f16x2(r[6], r[7])}; }
+__device__ __forceinline__ f32x16 mma_f16(const u32x4& a, const u32x4& b, f32x16 c) {
+	return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// a power of two that takes x to 2^8 .. 2^9 (within 2^-112 .. 2^100)
+__device__ __forceinline__ float unit_for(float x) {
+	int e = 8 + 127 - (int)(__float_as_uint(x) >> 23);
+	e     = e > 100 ? 100 : e;
+	return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+// a tile of V per workgroup: [pair][rows up to a whole number of tiles][2 DP], columns from Dv on zeros
+template <int DP>
+__global__ void __launch_bounds__(THREADS) diff_values_kernel(forward_args a) {
+	constexpr int VALUE_ROWS = value_rows(DP);
+	using P = passage<uint16_t, 2 * DP, VALUE_ROWS>;
+	const af3_diff_attention_params& p = a.p;
+	__shared__ uint32_t largest;
+	const uint32_t tiles = (uint32_t)((p.Lk + VALUE_ROWS - 1) / VALUE_ROWS), pair = blockIdx.x / tiles, tile_no = blockIdx.x - pair * tiles;
+	const int64_t  b = pair / (uint32_t)p.Hkv, hk = pair - (uint32_t)b * (uint32_t)p.Hkv, row0 = (int64_t)tile_no * VALUE_ROWS;
+	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b + row0 : nullptr;
+	P v;
+	v.begin(static_cast<const uint16_t*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1], p.v_stride[2], (int)p.Dv, a.whole_v);
+	v.load(row0, p.Lk);
+	if(threadIdx.x == 0) largest = 0u;
+	__syncthreads();
+	float top = 0.f;
+	bool  in[P::N];
+#pragma unroll
+	for(int n = 0; n < P::N; n++) {
+		const int row = P::row_of(n);
+		in[n] = row0 + row < p.Lk && P::col_of(n) * P::E < p.Dv && (!mask || mask[row] != 0);
+#pragma unroll
+		for(int e = 0; e < 8; e++) {
+			const float x = __builtin_fabsf(kind<uint16_t>::at(v.piece[n], e));
+			if(in[n] && x < INFINITY) top = __builtin_fmaxf(x, top);   // (neither infinities nor NaN, which no unit changes)
+		}
+	}
+	atomicMax(&largest, __float_as_uint(top));
+	__syncthreads();
+	top = __uint_as_float(largest);
+	const float unit = top == 0.f || (top * UNIT < UNIT_BELOW && top * UNIT >= UNIT_ABOVE) ? UNIT : unit_for(top);
+	if(threadIdx.x == 0) a.units[blockIdx.x] = unit;
+	u32x4* const out = static_cast<u32x4*>(a.values) + (int64_t)blockIdx.x * VALUE_ROWS * P::TL::CHUNKS;
+#pragma unroll
+	for(int n = 0; n < P::N; n++) {
+		u32x4 h;
+#pragma unroll
+		for(int i = 0; i < 4; i++) h[i] = in[n] ? pack_f16x2(kind<uint16_t>::at(v.piece[n], 2 * i) * unit, kind<uint16_t>::at(v.piece[n], 2 * i + 1) * unit) : 0u;
+		out[threadIdx.x + THREADS * n] = h;
+	}
+}
+
 // Eight wavefronts: two maps x KW that share 32 query rows and each take 32 keys of a tile (1: a wavefront takes all keys of one) x 4 / KW blocks of 32 rows
-constexpr int NT = 512;
+constexpr int   NT   = 512;
+constexpr float MOST = 32768.f;   // of a lane's sum of 16 probabilities, which fp16 has to hold: the reference is left behind
 constexpr int tile_keys(int bytes, int kw) { return kw == 4 || bytes <= 64 ? 128 : kw == 2 || bytes <= 128 ? 64 : 32; }   // bytes of a row of K
 template <typename T, int DP, int KW>
 struct forward_shape {
@@ -33,12 +112,14 @@ struct forward_shape {
 	static constexpr int LDS = BUFFERS * SET > 4 * TABLE ? BUFFERS * SET : 4 * TABLE;
 };
 
-template <typename T, int DP, int KW>
+// HALF: V comes as diff_values_kernel has laid it out
+template <typename T, int DP, int KW, bool HALF>
 __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 	using S  = forward_shape<T, DP, KW>;
 	using TK = tile<T, DP>;
 	using TV = tile<T, S::DV>;
-	constexpr int E = kind<T>::E, KT = S::KT;
+	constexpr int E = kind<T>::E, KT = S::KT, VALUE_ROWS = value_rows(DP);
+	static_assert(!HALF || VALUE_ROWS % KT == 0);
 	const af3_diff_attention_params& p = a.p;
 	extern __shared__ __align__(16) unsigned char smem[];
 	__shared__ live_keys<KT> live;
@@ -59,7 +140,10 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 	u32x4 qf[TK::STEPS];
 	load_operand<T, DP>(qf, static_cast<const T*>(p.q) + b * p.q_stride[0] + (2 * h + map) * p.q_stride[1] + qi * p.q_stride[2], ok, D, lane);
 	const T* const kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + 2 * hk * p.k_stride[1];
-	const T* const vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
+	const int64_t  v_rows = HALF ? (p.Lk + VALUE_ROWS - 1) / VALUE_ROWS * VALUE_ROWS : 0;
+	const T* const vb = HALF ? static_cast<const T*>(a.values) + own.pair * v_rows * S::DV : static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
+	const float* const units = a.units + own.pair * (v_rows / VALUE_ROWS);
+	float unit = HALF ? UNIT : 1.f, coming = unit, p_scale = 1.f, least = 0.f;   // of the sums, of the tile on its way; least: the smallest one so far, 0: none
 	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b : nullptr;
 
 	// p = exp2(t * to_log2 - reference), reference = to_log2 * (a maximum of the row's logits so far)
@@ -82,7 +166,8 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 	passage<T, S::DV, KT, NT> pv;
 	pk[0].begin(kb, p.k_stride[2], D, a.whole_k);
 	pk[1].begin(kb + p.k_stride[1], p.k_stride[2], D, a.whole_k);
-	pv.begin(vb, p.v_stride[2], Dv, a.whole_v);
+	if constexpr(HALF) pv.begin(vb, S::DV, S::DV, true);
+	else pv.begin(vb, p.v_stride[2], Dv, a.whole_v);
 	int buffer = 0;
 	for(int64_t first = (int64_t)split * a.part; first < last; first += SEGMENT) {
 		const int64_t end = first + SEGMENT < last ? first + SEGMENT : last;
@@ -90,9 +175,11 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 		int t = live.next(0);
 		if(t < 0) continue;
 		const int within = limit - first > SEGMENT ? SEGMENT : limit - first < -1 ? -1 : (int)(limit - first);
-		auto fetch = [&](int tile_no) {
+		float coming_next = UNIT;
+		auto  fetch = [&](int tile_no) {
 			const int64_t from = first + (int64_t)tile_no * KT;
-			pk[0].load(from, end), pk[1].load(from, end), pv.load(from, end);
+			pk[0].load(from, end), pk[1].load(from, end), pv.load(from, HALF ? v_rows : end);
+			if constexpr(HALF) coming_next = units[from / VALUE_ROWS];
 		};
 		fetch(t);
 		while(t >= 0) {
@@ -101,12 +188,25 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 			const tile_bits<KT> bits(live, t);
 			const bool          full = bits.full();
 			const int following = live.next(t + 1);
+			coming = coming_next;
 			if constexpr(S::BUFFERS == 1) __syncthreads();
 			// (what K holds at a dropped key stays in that key's logits, which are not looked at; its row of V meets a weight of zero, and must not be NaN)
 			pk[0].store(ks, true, [](int) { return true; });
 			pk[1].store(ks + S::KTILE, true, [](int) { return true; });
-			pv.store(vs, full, [&](int row) { return bits.keeps(row); });
+			if constexpr(HALF) pv.store(vs, true, [](int) { return true; });
+			else pv.store(vs, full, [&](int row) { return bits.keeps(row); });
 			__syncthreads();
+			if constexpr(HALF) {
+				p_scale = 1.f;
+				if(coming != unit) {   // (no more than 2^60 times the smallest one, so that the sums stay finite: what is missing goes to P)
+					const float to = least == 0.f ? coming : __builtin_fminf(coming, least * 0x1p60f), by = least == 0.f ? 1.f : to / unit;
+					unit = to;
+#pragma unroll
+					for(int db = 0; db < TV::BLOCKS; db++) o[db] *= by;
+					p_scale = unit / coming;
+				}
+				least   = least == 0.f ? unit : __builtin_fminf(least, unit);
+			}
 			if(following >= 0) fetch(following);
 			ks += map * S::KTILE;
 #pragma unroll
@@ -140,7 +240,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 				logits();
 				if(!moves) {
 					sum   = probabilities();
-					moves = __any(!(sum < LARGE));
+					moves = __any(!(sum < MOST));
 					if(moves) logits();
 				}
 				if(moves) {
@@ -164,11 +264,28 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 					}
 				}
 				l += sum;
+				if(HALF && p_scale != 1.f) {
+#pragma unroll
+					for(int r = 0; r < 16; r++) x[r] *= p_scale;
+				}
 #pragma unroll
 				for(int j = 0; j < TV::JOINTS; j++) {
-					const u32x4 pf = kind<T>::pack(x + E * j);
+					u32x4 pf, lo;
+					if constexpr(HALF) pf = pack_f16(x + E * j);
+					else pf = kind<T>::pack(x + E * j);
+					if constexpr(sizeof(T) == 2 && !HALF) {   // (what pf lost)
+						float y[E];
 #pragma unroll
-					for(int db = 0; db < TV::BLOCKS; db++) o[db] = kind<T>::mma(TV::col_frag(vs, 32 * block, db, j, at_v), pf, o[db]);
+						for(int e = 0; e < E; e++) y[e] = x[E * j + e] - kind<T>::at(pf, e);
+						lo = kind<T>::pack(y);
+					}
+#pragma unroll
+					for(int db = 0; db < TV::BLOCKS; db++) {
+						const u32x4 vf = TV::col_frag(vs, 32 * block, db, j, at_v);
+						if constexpr(HALF) o[db] = mma_f16(vf, pf, o[db]);
+						else o[db] = kind<T>::mma(vf, pf, o[db]);
+						if constexpr(sizeof(T) == 2 && !HALF) o[db] = kind<T>::mma(vf, lo, o[db]);
+					}
 				}
 			}
 			t = following;
@@ -218,7 +335,8 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 			__syncthreads();
 		}
 	}
-	const bool first_of_row = ok && kwave == 0 && half == 0;
+	const bool  first_of_row = ok && kwave == 0 && half == 0;
+	const float per_unit = 1.f / unit;
 	if(a.splits > 1) {
 		const int64_t n_rows = p.B * p.Hkv * rows, place = (2 * (int64_t)split + map) * n_rows + (b * p.Hkv + hk) * rows + R;
 		if(first_of_row) a.part_stat[2 * place] = m, a.part_stat[2 * place + 1] = l;
@@ -228,12 +346,12 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 			if(db % KW != kwave) continue;
 			float v[16];
 #pragma unroll
-			for(int r = 0; r < 16; r++) v[r] = o[db][r];
+			for(int r = 0; r < 16; r++) v[r] = o[db][r] * per_unit;
 			store_row16(a.part_out + place * Dv, 32 * db + 16 * half, Dv, v);
 		}
 		return;
 	}
-	const float   inv = l == 0.f ? 0.f : 1.f / l;   // (0: no live key)
+	const float   inv = l == 0.f ? 0.f : 1.f / l, inv_units = inv * per_unit;   // (0: no live key)
 	const int64_t row = (b * p.H + h) * p.Lq + qi;
 	if(p.stats && first_of_row) {
 		float* const st = p.stats + 2 * ((b * 2 * p.H + 2 * h + map) * p.Lq + qi);
@@ -242,7 +360,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 	// the second map's result by way of LDS to the wavefront that has the first one
 	if constexpr(KW == 1) __syncthreads();
 	if(map == 1) {
-		const float by = inv * lam_of(p, h);
+		const float by = inv_units * lam_of(p, h);
 #pragma unroll
 		for(int db = 0; db < TV::BLOCKS; db++) {
 			if(db % KW != kwave) continue;
@@ -250,8 +368,9 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 			if(p.second && ok) {
 				float v[16];
 #pragma unroll
-				for(int r = 0; r < 16; r++) v[r] = o[db][r] * inv;
+				for(int r = 0; r < 16; r++) v[r] = o[db][r] * inv_units;
 				store_row16(static_cast<T*>(p.second) + row * Dv, 32 * db + 16 * half, Dv, v);
+				store_residual<T>(p, 1, row, 32 * db + 16 * half, v);
 			}
 		}
 	}
@@ -266,9 +385,10 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 		for(int e = 0; e < 4; e++) {
 			const f32x4 other = *reinterpret_cast<const f32x4*>(tables + group * (S::TABLE / 4) + line + 32 * db + 4 * e);
 #pragma unroll
-			for(int c = 0; c < 4; c++) v[4 * e + c] = l == 0.f ? 0.f : __builtin_fmaf(o[db][4 * e + c], inv, -other[c]);
+			for(int c = 0; c < 4; c++) v[4 * e + c] = l == 0.f ? 0.f : __builtin_fmaf(o[db][4 * e + c], inv_units, -other[c]);
 		}
 		store_row16(out, 32 * db + 16 * half, Dv, v);
+		store_residual<T>(p, 0, row, 32 * db + 16 * half, v);
 	}
 }
 
@@ -332,8 +452,15 @@ __global__ void __launch_bounds__(THREADS) diff_join_kernel(forward_args a) {
 #pragma unroll
 	for(int k = 0; k < COLUMNS; k++)
 		if(lane + 64 * k < Dv) {
-			out[lane + 64 * k] = kind<T>::bits(none ? 0.f : __builtin_fmaf(-lam, o[1][k], o[0][k]));
+			const float v = none ? 0.f : __builtin_fmaf(-lam, o[1][k], o[0][k]);
+			out[lane + 64 * k] = kind<T>::bits(v);
 			if(p.second) static_cast<T*>(p.second)[row * Dv + lane + 64 * k] = kind<T>::bits(o[1][k]);
+			if constexpr(sizeof(T) == 2)
+				if(p.residuals) {
+					T* const lost = static_cast<T*>(p.residuals) + row * Dv + lane + 64 * k;
+					lost[0] = kind<T>::bits(v - kind<T>::value(kind<T>::bits(v)));
+					lost[p.B * p.H * p.Lq * Dv] = kind<T>::bits(o[1][k] - kind<T>::value(kind<T>::bits(o[1][k])));
+				}
 		}
 }
 
@@ -347,10 +474,13 @@ template <typename T, int DP>
 constexpr int MOST_SHARING = DP * (int)sizeof(T) <= 128 ? 4 : 2;
 int most_sharing(const af3_diff_attention_params& p) { return width(p) * (p.dtype == AF3_F32 ? 4 : 2) <= 128 ? 4 : 2; }
 
+int64_t value_tiles(const af3_diff_attention_params& p) { return (p.Lk + value_rows(width(p)) - 1) / value_rows(width(p)); }
+
 struct plan {
 	int      kw;
 	uint32_t row_tiles, splits;
 	int64_t  part;
+	bool     half;   // V as fp16
 };
 plan forward_plan(const af3_diff_attention_params& p) {
 	plan          f;
@@ -362,6 +492,8 @@ plan forward_plan(const af3_diff_attention_params& p) {
 	f.kw = rows <= 32 || busy(4) <= slots ? 4 : rows <= 64 || busy(2) <= slots ? 2 : 1;
 	if(f.kw > most_sharing(p)) f.kw = most_sharing(p);
 	f.row_tiles = (uint32_t)(busy(f.kw) / groups);
+	// (V's way through memory and back is worth it where many rows read it: from four tiles of them on)
+	f.half = !fp32 && f.kw == 1 && f.row_tiles >= 4 && groups * value_tiles(p) <= 0xffffff;
 	const int64_t kt = tile_keys(wide * (fp32 ? 4 : 2), f.kw), key_tiles = (p.Lk + kt - 1) / kt;
 	const double  tile_us = (0.4 + 0.033 * wide) * (f.kw == 4 ? 1.0 : 0.6) * (fp32 ? 3.0 : 1.0);
 	const int64_t splits = parts_for(busy(f.kw), slots, key_tiles, tile_us, 8.0 * p.B * p.H * p.Lq * p.Dv, MAX_PARTS);
@@ -371,10 +503,10 @@ plan forward_plan(const af3_diff_attention_params& p) {
 	return f;
 }
 
-template <typename T, int DP, int KW>
+template <typename T, int DP, int KW, bool HALF = false>
 int launch_forward(const forward_args& a, uint32_t grid, hipStream_t s) {
 	using S = forward_shape<T, DP, KW>;
-	auto kernel = &diff_forward_kernel<T, DP, KW>;
+	auto kernel = &diff_forward_kernel<T, DP, KW, HALF>;
 	if(S::LDS > 65536 - 8192 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess) {
 		(void)hipGetLastError();
 		return AF3_ERR_LAUNCH;
@@ -386,6 +518,12 @@ template <typename T, int DP>
 int launch_forward_form(const forward_args& a, int kw, uint32_t grid, hipStream_t s) {
 	if constexpr(MOST_SHARING<T, DP> == 4)
 		if(kw == 4) return launch_forward<T, DP, 4>(a, grid, s);
+	if constexpr(sizeof(T) == 2)
+		if(a.values) {
+			hipLaunchKernelGGL(diff_values_kernel<DP>, dim3((uint32_t)(a.p.B * a.p.Hkv * value_tiles(a.p))), dim3(THREADS), 0, s, a);
+			const int rc = launch_status();
+			return rc != AF3_OK ? rc : launch_forward<T, DP, 1, true>(a, grid, s);
+		}
 	return kw == 2 ? launch_forward<T, DP, 2>(a, grid, s) : launch_forward<T, DP, 1>(a, grid, s);
 }
 template <typename T>
@@ -397,7 +535,11 @@ int launch_forward_type(const forward_args& a, int kw, uint32_t grid, hipStream_
 	return launch_forward_form<T, 64>(a, kw, grid, s);
 }
 
-int64_t forward_workspace(const af3_diff_attention_params& p, const plan& f) { return f.splits > 1 ? (int64_t)f.splits * p.B * p.H * p.Lq * (p.Dv + 2) * 8 : 0; }
+int64_t values_bytes(const af3_diff_attention_params& p, const plan& f) { return f.half ? p.B * p.Hkv * value_tiles(p) * value_rows(width(p)) * 4 * width(p) : 0; }
+int64_t units_bytes(const af3_diff_attention_params& p, const plan& f) { return f.half ? (p.B * p.Hkv * value_tiles(p) + 3) / 4 * 16 : 0; }
+int64_t forward_workspace(const af3_diff_attention_params& p, const plan& f) {
+	return (f.splits > 1 ? (int64_t)f.splits * p.B * p.H * p.Lq * (p.Dv + 2) * 8 : 0) + values_bytes(p, f) + units_bytes(p, f);
+}
 
 }  // namespace diff
 
@@ -412,7 +554,8 @@ int validate_diff_attention(const af3_diff_attention_params* p) {
 	// (row numbers and the parts' sizes stay far inside 63 bits, a launch's workgroups times 256 threads inside 32)
 	if(p->B > 0xffffff || p->H > 0x7fff || p->Lq > 0x3fffffff || p->Lk > 0x3fffffff || p->B * p->H > 0xffffff || p->H * p->Lq > 0x3fffffff || p->B * p->H * ((p->Lq + 31) / 32) > 0xffffff) return AF3_ERR_BAD_SHAPE;
 	if(p->stats && !diff_gradients_fit(*p)) return AF3_ERR_BAD_SHAPE;   // (they are for a gradient that would be refused)
-	if(!p->q || !p->k || !p->v || !p->lam || !p->out || (p->stats != nullptr) != (p->second != nullptr)) return AF3_ERR_NULL_POINTER;
+	if(!p->q || !p->k || !p->v || !p->lam || !p->out || (p->stats != nullptr) != (p->second != nullptr) || (p->residuals && !p->second)) return AF3_ERR_NULL_POINTER;
+	if(p->residuals && p->dtype != AF3_BF16) return AF3_ERR_BAD_DTYPE;   // (nothing would be written there)
 	for(int i = 0; i < 3; i++)
 		if(p->q_stride[i] < 0 || p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
 	// (inputs may repeat rows, results may not)
@@ -443,7 +586,9 @@ extern "C" int af3_diff_attention_forward(const af3_diff_attention_params* param
 	a.factor  = params->softmax_scale * LOG2E;
 	a.whole_k = params->D * (fp32 ? 4 : 2) % 16 == 0, a.whole_v = params->Dv * (fp32 ? 4 : 2) % 16 == 0;
 	const int64_t n_rows = params->B * params->H * params->Lq;
-	a.part_out = static_cast<float*>(params->workspace), a.part_stat = a.part_out + 2 * f.splits * n_rows * params->Dv;
+	unsigned char* const space = static_cast<unsigned char*>(params->workspace);
+	a.values   = f.half ? space : nullptr, a.units = reinterpret_cast<float*>(space + diff::values_bytes(*params, f));
+	a.part_out = reinterpret_cast<float*>(space + diff::values_bytes(*params, f) + diff::units_bytes(*params, f)), a.part_stat = a.part_out + 2 * f.splits * n_rows * params->Dv;
 	const uint32_t grid = (uint32_t)(params->B * params->Hkv) * f.row_tiles * f.splits;
 	const int rc = fp32 ? diff::launch_forward_type<float>(a, f.kw, grid, s) : diff::launch_forward_type<uint16_t>(a, f.kw, grid, s);
 	if(rc != AF3_OK || f.splits == 1) return rc;

@@ -5,7 +5,8 @@
 // summed by one workgroup, or by one per part of the long axis and a joining kernel, always in the same order.
 //   diff_dq_kernel    32 query rows per wavefront, both maps, keys in tiles (writes d1 and d2 too)
 //   diff_dkv_kernel   32 keys per wavefront, both maps, query rows in tiles, over all heads of the key head
-//   diff_lam_kernel   the sums of d2
+//   diff_lam_kernel   the sums of d2, and of the rows of P2 * (dP - d2): those would be zero, but for what d2 misses by the forward pass's probabilities, rounded to bf16 as they are
+//                     there.  dlam is a sum of many rows' d2 that mostly cancel: without that it was off by up to 0.008 of itself in sums over 300 rows (with: 1e-6 before its last rounding).
 #include "diff_tiles.hpp"
 
 #include <math.h>
@@ -21,6 +22,8 @@ struct grad_args {
 	float    factor;
 	int32_t  whole_k, whole_v;
 	float *  d1, *d2;         // [B, H, Lq] each
+	float*   short_of;        // what d2 is short of, in `shorts` parts [B, H, Lq], or null
+	uint32_t shorts;
 	float*   partial;         // dq: [splits][B 2H Lq][D]; dkv: [splits]([B 2Hkv Lk][D], [B Hkv Lk][Dv])
 	float *  dq_space, *dkv_space;
 };
@@ -66,8 +69,15 @@ __device__ __forceinline__ float row_dot(const u32x4 (&gf)[N], const T* row, boo
 template <typename T, int DV, int N>
 __device__ __forceinline__ void row_deltas(const grad_args& a, const u32x4 (&gf)[N], int64_t b, int64_t h, int64_t qi, bool ok, int lane, float& d1, float& d2) {
 	const af3_diff_attention_params& p = a.p;
-	d2 = row_dot<T, DV>(gf, static_cast<const T*>(p.second) + ((b * p.H + h) * p.Lq + qi) * p.Dv, ok, (int)p.Dv, lane);
-	d1 = row_dot<T, DV>(gf, static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2], ok, (int)p.Dv, lane);
+	const int64_t row = (b * p.H + h) * p.Lq + qi;
+	const int     Dv = (int)p.Dv;
+	d2 = row_dot<T, DV>(gf, static_cast<const T*>(p.second) + row * Dv, ok, Dv, lane);
+	d1 = row_dot<T, DV>(gf, static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2], ok, Dv, lane);
+	if(sizeof(T) == 2 && p.residuals) {
+		const T* const lost = static_cast<const T*>(p.residuals) + row * Dv;
+		d1 += row_dot<T, DV>(gf, lost, ok, Dv, lane);
+		d2 += row_dot<T, DV>(gf, lost + p.B * p.H * p.Lq * Dv, ok, Dv, lane);
+	}
 	d1 = __builtin_fmaf(lam_of(p, h), d2, d1);
 }
 
@@ -119,7 +129,7 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 	float d1, d2, delta[MAPS];
 	row_deltas<T, S::DV>(a, gf, b, h, qi, ok, lane, d1, d2);
 	if(ok && half == 0 && kwave == 0 && map0 == 0 && split == 0) a.d1[row] = d1, a.d2[row] = d2;
-	if(!a.g.grad_q) return;
+	if(!a.g.grad_q && !a.short_of) return;
 	float m[MAPS], inv[MAPS], taken[MAPS];
 	bool  far = false;
 #pragma unroll
@@ -135,6 +145,7 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 	const T* const vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
 	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b : nullptr;
 
+	float  row_sum = 0.f;   // of the second map's dS / -lam
 	f32x16 dq[MAPS][TK::BLOCKS];
 #pragma unroll
 	for(int i = 0; i < MAPS; i++)
@@ -205,6 +216,10 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 					}
 					if(keep != ~0u) drop_keys(x, keep, 0.f);
 					if(diagonal) drop_later(x, left, 0.f);
+					if(map0 + i == 1) {
+#pragma unroll
+						for(int r = 0; r < 16; r++) row_sum += x[r];
+					}
 #pragma unroll
 					for(int j = 0; j < TK::JOINTS; j++) {
 						const u32x4 f = kind<T>::pack(x + E * j);
@@ -217,6 +232,9 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 			if constexpr(S::BUFFERS == 2) buffer ^= 1;
 		}
 	}
+	row_sum = sum_of_halves(row_sum);
+	if(a.short_of && ok && half == 0 && (MAPS == 2 || map0 == 1)) a.short_of[(int64_t)(split * KW + kwave) * (p.B * p.H * p.Lq) + row] = row_sum;
+	if(!a.g.grad_q) return;
 	const float lam = lam_of(p, h);
 #pragma unroll
 	for(int i = 0; i < MAPS; i++) {
@@ -483,7 +501,10 @@ __global__ void __launch_bounds__(LAM_THREADS) diff_lam_kernel(grad_args a) {
 #pragma unroll 4
 	for(int64_t i = threadIdx.x; i < n; i += LAM_THREADS) {
 		const int64_t b = i / p.Lq;
-		sum += (double)a.d2[(b * p.H + h) * p.Lq + (i - b * p.Lq)];
+		const int64_t row = (b * p.H + h) * p.Lq + (i - b * p.Lq);
+		float         d2 = a.d2[row];
+		for(uint32_t k = 0; k < a.shorts; k++) d2 += a.short_of[k * (p.B * p.H * p.Lq) + row];
+		sum += (double)d2;
 	}
 	sums[threadIdx.x] = sum;
 	for(int k = LAM_THREADS / 2; k; k >>= 1) {
@@ -569,15 +590,16 @@ cut dkv_cut(const af3_diff_attention_params& p) {
 }
 
 struct grad_space {
-	int64_t delta, dq, dkv, bytes;   // floats
+	int64_t delta, shorts, dq, dkv, bytes;   // floats
 };
 grad_space grad_workspace(const af3_diff_attention_params& p) {
 	const cut  q = dq_cut(p), kv = dkv_cut(p);
 	grad_space w;
 	w.delta = over(p.B * p.H * p.Lq, 4) * 4;
+	w.shorts = over((int64_t)q.splits * (q.shared ? 4 : 1) * p.B * p.H * p.Lq, 4) * 4;
 	w.dq    = q.splits > 1 ? over(2 * (int64_t)q.splits * p.B * p.H * p.Lq * p.D, 4) * 4 : 0;
 	w.dkv   = kv.splits > 1 ? over((int64_t)kv.splits * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv), 4) * 4 : 0;
-	w.bytes = (2 * w.delta + w.dq + w.dkv) * 4;
+	w.bytes = (2 * w.delta + w.shorts + w.dq + w.dkv) * 4;
 	return w;
 }
 
@@ -607,9 +629,11 @@ int backward(grad_args a, hipStream_t s) {
 		n_sums++;
 	};
 	int rc = AF3_ERR_LAUNCH;
-	{   // (without grad_q: d1 and d2 alone)
+	{   // (without grad_q and grad_lam: d1 and d2 alone)
 		const cut c = dq_cut(p);
-		a.tiles = c.tiles, a.splits = a.g.grad_q ? c.splits : 1, a.part = c.part, a.partial = a.dq_space;
+		a.shorts = c.splits * (c.shared ? 4 : 1);
+		if(!a.g.grad_lam) a.short_of = nullptr;
+		a.tiles = c.tiles, a.splits = a.g.grad_q || a.short_of ? c.splits : 1, a.part = c.part, a.partial = a.dq_space;
 		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * a.tiles * a.splits;
 		if constexpr(SHARES)
 			if(c.shared) rc = launch<dq_shape<T, DP, 4>>(diff_dq_kernel<T, DP, 4>, grid, a, s);
@@ -671,7 +695,7 @@ extern "C" int af3_diff_attention_backward(const af3_diff_attention_params* para
 	a.p = *params, a.g = *grads, a.tiles = a.splits = 1, a.part = 0, a.partial = nullptr;
 	a.factor  = params->softmax_scale * LOG2E;
 	a.whole_k = params->D * (fp32 ? 4 : 2) % 16 == 0, a.whole_v = params->Dv * (fp32 ? 4 : 2) % 16 == 0;
-	a.d1 = static_cast<float*>(grads->workspace), a.d2 = a.d1 + w.delta, a.dq_space = a.d2 + w.delta, a.dkv_space = a.dq_space + w.dq;
+	a.d1 = static_cast<float*>(grads->workspace), a.d2 = a.d1 + w.delta, a.short_of = a.d2 + w.delta, a.shorts = 0, a.dq_space = a.short_of + w.shorts, a.dkv_space = a.dq_space + w.dq;
 	const hipStream_t s = static_cast<hipStream_t>(hip_stream);
 	const int wide = diff::width(*params);
 	if(fp32) return wide == 32 ? diff::backward<float, 32>(a, s) : diff::backward<float, 64>(a, s);

@@ -28,6 +28,7 @@ __device__ __forceinline__ void drop_later(float (&x)[16], int left, float gone)
 #pragma unroll
 	for(int r = 0; r < 16; r++) x[r] = r <= left ? x[r] : gone;
 }
+
 __device__ __forceinline__ int clamped(int64_t x) { return x > 64 ? 64 : x < -64 ? -64 : (int)x; }
 
 }  // namespace diff

@@ -1269,7 +1269,7 @@ struct diff_call {
 		p.causal = (int32_t)causal, p.q_offset = offset, p.softmax_scale = (float)scale;
 		return p;
 	}
-	int forward(Tensor& out, Tensor* stats, Tensor* second) const {
+	int forward(Tensor& out, Tensor* stats, Tensor* second, Tensor* lost) const {
 		const int dev = (int)q.get_device();
 		af3_diff_attention_params p = block();
 		out   = new_tensor({p.B, p.H, p.Lq, p.Dv}, q.scalar_type(), dev);
@@ -1278,6 +1278,7 @@ struct diff_call {
 		if(stats) {
 			*stats = new_tensor({p.B, 2 * p.H, p.Lq, 2}, at::kFloat, dev), *second = new_tensor(out.sizes(), q.scalar_type(), dev);
 			p.stats = static_cast<float*>(stats->data_ptr()), p.second = second->data_ptr();
+			if(p.dtype == AF3_BF16) *lost = new_tensor({2, p.B, p.H, p.Lq, p.Dv}, q.scalar_type(), dev), p.residuals = lost->data_ptr();
 		}
 		at::DataPtr   ws;
 		const int64_t bytes = af3_diff_attention_workspace_bytes(&p);
@@ -1290,9 +1291,9 @@ struct diff_function : torch::autograd::Function<diff_function> {
 	static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const std::optional<Tensor>& given_mask, double scale,
 						  int64_t causal, int64_t offset) {
 		const Tensor mask = given_mask.value_or(Tensor());
-		Tensor       out, stats, second;
-		raise(diff_call{q, k, v, lam, mask, scale, causal, offset}.forward(out, &stats, &second), "af3_diff_attention_forward");
-		ctx->save_for_backward({q, k, v, lam, mask, out, stats, second});
+		Tensor       out, stats, second, lost;
+		raise(diff_call{q, k, v, lam, mask, scale, causal, offset}.forward(out, &stats, &second, &lost), "af3_diff_attention_forward");
+		ctx->save_for_backward({q, k, v, lam, mask, out, stats, second, lost});
 		ctx->saved_data["scale"] = scale, ctx->saved_data["causal"] = causal, ctx->saved_data["offset"] = offset;
 		return out;
 	}
@@ -1308,6 +1309,7 @@ struct diff_function : torch::autograd::Function<diff_function> {
 			if(!inner_1(g)) g = g.contiguous();
 			af3_diff_attention_params p = call.block();
 			p.out = saved[5].data_ptr(), p.stats = static_cast<float*>(saved[6].data_ptr()), p.second = saved[7].data_ptr();
+			if(saved[8].defined()) p.residuals = saved[8].data_ptr();
 			put_strides(p.out_stride, saved[5]);
 			af3_diff_attention_grads o{};
 			o.grad_out = g.const_data_ptr();
@@ -1359,7 +1361,7 @@ PyObject* py_differential_attention(PyObject*, PyObject* const* a, Py_ssize_t n)
 	{
 		without_gil g;
 		if(graph) check_capture({q, k, v, lam}, dev), out = diff_function::apply(c.q, c.k, c.v, c.lam, given(c.mask), c.scale, c.causal, c.offset);
-		else rc = c.forward(out, nullptr, nullptr);
+		else rc = c.forward(out, nullptr, nullptr, nullptr);
 	}
 	return answer(rc, std::move(out));
 	END_HANDLE_TH_ERRORS

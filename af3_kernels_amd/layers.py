@@ -164,7 +164,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], frequencies: to
 
 
 # ---- differential attention -------------------------------------------------------------------------------------------------
-def _diff_block(q, k, v, lam, keep, out, stats, second, causal, offset, scale) -> DiffAttentionParams:
+def _diff_block(q, k, v, lam, keep, out, stats, second, lost, causal, offset, scale) -> DiffAttentionParams:
     p = DiffAttentionParams()
     p.q, p.k, p.v, p.lam, p.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), out.data_ptr()
     p.B, p.H, p.Lq, p.Dv = out.shape
@@ -174,20 +174,23 @@ def _diff_block(q, k, v, lam, keep, out, stats, second, causal, offset, scale) -
         p.key_mask, p.key_mask_stride_b = keep.data_ptr(), 0 if keep.shape[0] == 1 else keep.stride(0)
     if stats is not None:
         p.stats, p.second = stats.data_ptr(), second.data_ptr()
+    if lost is not None:
+        p.residuals = lost.data_ptr()
     p.lam_stride, p.lam_dtype, p.dtype = lam.stride(0), _DTYPES[lam.dtype], _DTYPES[q.dtype]
     p.causal, p.q_offset, p.softmax_scale = int(causal), offset, scale
     return p
 
 
 def _diff_forward(q, k, v, lam, keep, causal, offset, scale, want_stats):
-    """(out, stats, second): where the gradient will be asked for, stats [B, 2H, Lq, 2] and the second map's own result."""
+    """(out, stats, second, lost): where the gradient will be asked for, stats [B, 2H, Lq, 2], the second map's own result, and what the two lost by their rounding to bfloat16."""
     B, H, Lq = q.shape[0], q.shape[1] // 2, q.shape[2]
     out = torch.empty(B, H, Lq, v.shape[3], dtype=q.dtype, device=q.device)
     if out.numel() == 0 or k.shape[2] == 0:
-        return out.zero_(), None, None
+        return out.zero_(), None, None, None
     stats = torch.empty(B, 2 * H, Lq, 2, dtype=torch.float32, device=q.device) if want_stats else None
     second = torch.empty_like(out) if want_stats else None
-    p = _diff_block(q, k, v, lam, keep, out, stats, second, causal, offset, scale)
+    lost = torch.empty(2, *out.shape, dtype=out.dtype, device=out.device) if want_stats and out.dtype == torch.bfloat16 else None
+    p = _diff_block(q, k, v, lam, keep, out, stats, second, lost, causal, offset, scale)
     lib = _lib.load()
     with ops._on_device(q.device):
         need = lib.af3_diff_attention_workspace_bytes(ctypes.byref(p))
@@ -195,14 +198,14 @@ def _diff_forward(q, k, v, lam, keep, causal, offset, scale, want_stats):
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             p.workspace, p.workspace_bytes = ws.data_ptr(), need
         _lib.check(lib.af3_diff_attention_forward(ctypes.byref(p), ops._stream_ptr(q.device)), "af3_diff_attention_forward")
-    return out, stats, second
+    return out, stats, second, lost
 
 
 class _DifferentialAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, keep, causal, offset, scale):
-        out, stats, second = _diff_forward(q, k, v, lam, keep, causal, offset, scale, True)
-        ctx.save_for_backward(q, k, v, lam, keep, out, stats, second)
+        out, stats, second, lost = _diff_forward(q, k, v, lam, keep, causal, offset, scale, True)
+        ctx.save_for_backward(q, k, v, lam, keep, out, stats, second, lost)
         ctx.settings = (causal, offset, scale)
         return out
 
@@ -210,13 +213,13 @@ class _DifferentialAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         _no_tangents("the gradient of differential_attention", grad)
-        q, k, v, lam, keep, out, stats, second = ctx.saved_tensors
+        q, k, v, lam, keep, out, stats, second, lost = ctx.saved_tensors
         wants = ctx.needs_input_grad[:4]
         if stats is None:
             return (*(torch.zeros(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v, lam), wants)), None, None, None, None)
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v, lam), wants)]
         grad = _inner_contig(grad)
-        p, g = _diff_block(q, k, v, lam, keep, out, stats, second, *ctx.settings), DiffAttentionGrads()
+        p, g = _diff_block(q, k, v, lam, keep, out, stats, second, lost, *ctx.settings), DiffAttentionGrads()
         g.grad_out, g.grad_out_stride = grad.data_ptr(), _i64x3(*grad.stride()[:3])
         g.grad_q, g.grad_k, g.grad_v, g.grad_lam = (0 if t is None else t.data_ptr() for t in grads)
         lib = _lib.load()

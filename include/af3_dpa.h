@@ -453,6 +453,8 @@ int64_t af3_position_bias_workspace_bytes(const af3_position_bias_params* params
  *   dtype       : AF3_BF16 (bf16 products, fp32 accumulation and softmax) or AF3_F32 (fp32 throughout), of q, k, v, out.
  *   stats, second : optional, both or neither, for af3_diff_attention_backward: [B, 2 H, Lq, 2] floats (maximum in the softmax's units and 1 / sum) and
  *                 [B, H, Lq, Dv] contiguous of `dtype` (the second map's own result).
+ *   residuals   : with them, AF3_BF16 only: [2, B, H, Lq, Dv] contiguous, what out and second lost by their rounding, as bf16.  Given to af3_diff_attention_backward too, the row
+ *                 sums of grad_out * out that it takes off every dS are those of results to 16 bits.
  *   workspace   : af3_diff_attention_workspace_bytes() bytes, 16-byte aligned; NULL where that is 0.  Overwritten.
  * B, H, Lq, Lk, D, Dv >= 1; D <= 128 and Dv <= 256 (AF3_F32: D <= 64 and Dv <= 128; AF3_ERR_UNSUPPORTED_D); Lq and Lk < 2^30, H < 2^15, H * Lq < 2^30,
  * B * H * ceil(Lq / 32) < 2^24; with stats B * Hkv * ceil(Lk / 32) < 2^24 too; |q_offset| < 2^40.  AF3_ERR_BAD_SHAPE otherwise, from the workspace call as well.
@@ -466,6 +468,7 @@ typedef struct af3_diff_attention_params {
 	void*          out;
 	float*         stats;
 	void*          second;
+	void*          residuals;
 	int64_t        B, H, Hkv, Lq, Lk, D, Dv;
 	int64_t        q_stride[3];
 	int64_t        k_stride[3];
