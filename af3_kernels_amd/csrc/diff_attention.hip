@@ -16,7 +16,7 @@ struct forward_args {
 	uint32_t row_tiles, splits;    // workgroups per (batch, key head); parts of the key axis
 	int64_t  part;                 // keys per part, a multiple of the tile
 	float    factor;               // exp2((t - max) * factor) with t = q.k
-	int32_t  whole_k, whole_v;     // D, Dv are whole numbers of 16-byte pieces
+	int32_t  columns, v_columns;   // of q and k, of v, as they are read: whole pieces
 	float*   part_out;             // [splits][2][B * Hkv * G * Lq][Dv] and ...
 	void*    values;               // V as fp16, tile after tile, and its tiles' units, or null
 	float*   units;
@@ -30,9 +30,36 @@ __device__ __forceinline__ void store_residual(const af3_diff_attention_params& 
 		if(!p.residuals) return;
 		float r[16];
 #pragma unroll
-		for(int i = 0; i < 16; i++) r[i] = v[i] - kind<T>::value(kind<T>::bits(v[i]));
-		store_row16(static_cast<T*>(p.residuals) + (which * p.B * p.H * p.Lq + row) * p.Dv, d, (int)p.Dv, r);
+		for(int i = 0; i < 16; i++) r[i] = v[i] - (float)(__bf16)v[i];
+		store_columns(static_cast<T*>(p.residuals) + (which * p.B * p.H * p.Lq + row) * p.Dv, d, (int)p.Dv, r);
 	}
+}
+
+// ---- rows of whole pieces ----
+__global__ void __launch_bounds__(THREADS) diff_pack_kernel(packing k) {
+	int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+	int     which = 0;
+	while(which < k.count && i >= k.jobs[which].pieces) i -= k.jobs[which++].pieces;
+	if(which == k.count) return;
+	const packing::job& j = k.jobs[which];
+	const int     each = 16 / k.element, per_row = (j.columns + each - 1) / each;
+	const int64_t row = i / per_row, n2 = row % j.n[2], n1 = row / j.n[2] % j.n[1], n0 = row / j.n[2] / j.n[1];
+	const int     c0 = (int)(i - row * per_row) * each;
+	const int64_t from = n0 * j.stride[0] + n1 * j.stride[1] + n2 * j.stride[2];
+	u32x4 v = {0u, 0u, 0u, 0u};
+	for(int c = 0; c < each && c0 + c < j.columns; c++) {
+		if(k.element == 4) v[c] = static_cast<const uint32_t*>(j.from)[from + c0 + c];
+		else v[c >> 1] |= (uint32_t)static_cast<const uint16_t*>(j.from)[from + c0 + c] << (16 * (c & 1));
+	}
+	static_cast<u32x4*>(j.to)[i] = v;
+}
+int packing::launch(hipStream_t s) const {
+	int64_t pieces = 0;
+	for(int i = 0; i < count; i++) pieces += jobs[i].pieces;
+	if(pieces == 0) return AF3_OK;
+	if(pieces > (int64_t)0xffffff * THREADS) return AF3_ERR_BAD_SHAPE;
+	hipLaunchKernelGGL(diff_pack_kernel, dim3((uint32_t)((pieces + THREADS - 1) / THREADS)), dim3(THREADS), 0, s, *this);
+	return launch_status();
 }
 
 // ---- the values as fp16 ----
@@ -61,15 +88,15 @@ __device__ __forceinline__ float unit_for(float x) {
 template <int DP>
 __global__ void __launch_bounds__(THREADS) diff_values_kernel(forward_args a) {
 	constexpr int VALUE_ROWS = value_rows(DP);
-	using P = passage<uint16_t, 2 * DP, VALUE_ROWS>;
+	using P = carrier<uint16_t, 2 * DP, VALUE_ROWS, THREADS>;
 	const af3_diff_attention_params& p = a.p;
 	__shared__ uint32_t largest;
 	const uint32_t tiles = (uint32_t)((p.Lk + VALUE_ROWS - 1) / VALUE_ROWS), pair = blockIdx.x / tiles, tile_no = blockIdx.x - pair * tiles;
 	const int64_t  b = pair / (uint32_t)p.Hkv, hk = pair - (uint32_t)b * (uint32_t)p.Hkv, row0 = (int64_t)tile_no * VALUE_ROWS;
 	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b + row0 : nullptr;
 	P v;
-	v.begin(static_cast<const uint16_t*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1], p.v_stride[2], (int)p.Dv, a.whole_v);
-	v.load(row0, p.Lk);
+	v.begin(p.v_stride[2], a.v_columns);
+	v.load(static_cast<const uint16_t*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1], row0, p.Lk);
 	if(threadIdx.x == 0) largest = 0u;
 	__syncthreads();
 	float top = 0.f;
@@ -77,7 +104,7 @@ __global__ void __launch_bounds__(THREADS) diff_values_kernel(forward_args a) {
 #pragma unroll
 	for(int n = 0; n < P::N; n++) {
 		const int row = P::row_of(n);
-		in[n] = row0 + row < p.Lk && P::col_of(n) * P::E < p.Dv && (!mask || mask[row] != 0);
+		in[n] = row0 + row < p.Lk && P::col_of(n) * P::E < a.v_columns && (!mask || mask[row] != 0);
 #pragma unroll
 		for(int e = 0; e < 8; e++) {
 			const float x = __builtin_fabsf(kind<uint16_t>::at(v.piece[n], e));
@@ -131,14 +158,14 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 	const uint32_t split = own.piece / a.row_tiles, row_tile = a.row_tiles - 1 - (own.piece - split * a.row_tiles);   // (causal: those with the most keys first)
 	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
 	const int64_t G = p.H / p.Hkv, rows = G * p.Lq;
-	const int     D = (int)p.D, Dv = (int)p.Dv;
+	const int     Dv = (int)p.Dv;
 
 	const int64_t   R = (int64_t)row_tile * S::ROWS + 32 * group + (lane & 31);
 	const row_place at_row(R, rows, G, hk);
 	const bool      ok = at_row.ok;
 	const int64_t   qi = at_row.qi, h = at_row.h;
 	u32x4 qf[TK::STEPS];
-	load_operand<T, DP>(qf, static_cast<const T*>(p.q) + b * p.q_stride[0] + (2 * h + map) * p.q_stride[1] + qi * p.q_stride[2], ok, D, lane);
+	load_rows<T, DP>(qf, static_cast<const T*>(p.q) + b * p.q_stride[0] + (2 * h + map) * p.q_stride[1] + qi * p.q_stride[2], ok, a.columns, lane);
 	const T* const kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + 2 * hk * p.k_stride[1];
 	const int64_t  v_rows = HALF ? (p.Lk + VALUE_ROWS - 1) / VALUE_ROWS * VALUE_ROWS : 0;
 	const T* const vb = HALF ? static_cast<const T*>(a.values) + own.pair * v_rows * S::DV : static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
@@ -160,14 +187,13 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 		last = end < last ? end : last;
 	}
 	const int64_t limit = p.causal ? qi + p.q_offset : (int64_t)1 << 41;   // the lane's last key
-	const typename TK::reader at_k(lane);
-	const typename TV::reader at_v(lane);
-	passage<T, DP, KT, NT>    pk[2];
-	passage<T, S::DV, KT, NT> pv;
-	pk[0].begin(kb, p.k_stride[2], D, a.whole_k);
-	pk[1].begin(kb + p.k_stride[1], p.k_stride[2], D, a.whole_k);
-	if constexpr(HALF) pv.begin(vb, S::DV, S::DV, true);
-	else pv.begin(vb, p.v_stride[2], Dv, a.whole_v);
+	const typename TK::reader at_k_(lane);
+	const typename TV::reader at_v_(lane);
+	carrier<T, DP, KT, NT>    pk[2];
+	carrier<T, S::DV, KT, NT> pv;
+	pk[0].begin(p.k_stride[2], a.columns);
+	if constexpr(HALF) pv.begin(S::DV, S::DV);
+	else pv.begin(p.v_stride[2], a.v_columns);
 	int buffer = 0;
 	for(int64_t first = (int64_t)split * a.part; first < last; first += SEGMENT) {
 		const int64_t end = first + SEGMENT < last ? first + SEGMENT : last;
@@ -178,7 +204,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 		float coming_next = UNIT;
 		auto  fetch = [&](int tile_no) {
 			const int64_t from = first + (int64_t)tile_no * KT;
-			pk[0].load(from, end), pk[1].load(from, end), pv.load(from, HALF ? v_rows : end);
+			pk[0].load(kb, from, end), pk[1].load(kb + p.k_stride[1], from, end, pk[0]), pv.load(vb, from, HALF ? v_rows : end);
 			if constexpr(HALF) coming_next = units[from / VALUE_ROWS];
 		};
 		fetch(t);
@@ -192,7 +218,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 			if constexpr(S::BUFFERS == 1) __syncthreads();
 			// (what K holds at a dropped key stays in that key's logits, which are not looked at; its row of V meets a weight of zero, and must not be NaN)
 			pk[0].store(ks, true, [](int) { return true; });
-			pk[1].store(ks + S::KTILE, true, [](int) { return true; });
+			pk[1].store(ks + S::KTILE, true, [](int) { return true; }, a.columns);
 			if constexpr(HALF) pv.store(vs, true, [](int) { return true; });
 			else pv.store(vs, full, [&](int row) { return bits.keeps(row); });
 			__syncthreads();
@@ -209,13 +235,15 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 			}
 			if(following >= 0) fetch(following);
 			ks += map * S::KTILE;
-#pragma unroll
+#pragma unroll 1
 			for(int s = 0; s < S::SUB; s++) {
 				const int      block = kwave * S::SUB + s;
 				const uint32_t keep = bits.of_block(block);
 				const int      left = within - (t * KT + 32 * block + 16 * half);   // the lane's keys 0 .. left of its 16 count
 				if(keep == 0u || !__any(ok && left >= 0)) continue;
 				const bool diagonal = __any(ok && left < 15);
+				const typename TK::reader at_k = DP * sizeof(T) > 128 ? fresh(at_k_) : at_k_;
+				const typename TV::reader at_v = DP * sizeof(T) > 128 ? fresh(at_v_) : at_v_;
 				float x[16];
 				auto  logits = [&] {
 					f32x16 acc{};
@@ -347,7 +375,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 			float v[16];
 #pragma unroll
 			for(int r = 0; r < 16; r++) v[r] = o[db][r] * per_unit;
-			store_row16(a.part_out + place * Dv, 32 * db + 16 * half, Dv, v);
+			store_columns(a.part_out + place * Dv, 32 * db + 16 * half, Dv, v);
 		}
 		return;
 	}
@@ -369,7 +397,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 				float v[16];
 #pragma unroll
 				for(int r = 0; r < 16; r++) v[r] = o[db][r] * inv_units;
-				store_row16(static_cast<T*>(p.second) + row * Dv, 32 * db + 16 * half, Dv, v);
+				store_columns(static_cast<T*>(p.second) + row * Dv, 32 * db + 16 * half, Dv, v);
 				store_residual<T>(p, 1, row, 32 * db + 16 * half, v);
 			}
 		}
@@ -387,7 +415,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 #pragma unroll
 			for(int c = 0; c < 4; c++) v[4 * e + c] = l == 0.f ? 0.f : __builtin_fmaf(o[db][4 * e + c], inv_units, -other[c]);
 		}
-		store_row16(out, 32 * db + 16 * half, Dv, v);
+		store_columns(out, 32 * db + 16 * half, Dv, v);
 		store_residual<T>(p, 0, row, 32 * db + 16 * half, v);
 	}
 }
@@ -537,8 +565,19 @@ int launch_forward_type(const forward_args& a, int kw, uint32_t grid, hipStream_
 
 int64_t values_bytes(const af3_diff_attention_params& p, const plan& f) { return f.half ? p.B * p.Hkv * value_tiles(p) * value_rows(width(p)) * 4 * width(p) : 0; }
 int64_t units_bytes(const af3_diff_attention_params& p, const plan& f) { return f.half ? (p.B * p.Hkv * value_tiles(p) + 3) / 4 * 16 : 0; }
+packing pack_inputs(af3_diff_attention_params& p, int32_t& columns, int32_t& v_columns, void* space) {
+	packing k(p.dtype == AF3_F32 ? 4 : 2);
+	columns = k.add(p.q, p.q_stride, p.B, 2 * p.H, p.Lq, p.D, space);
+	k.add(p.k, p.k_stride, p.B, 2 * p.Hkv, p.Lk, p.D, space);
+	v_columns = k.add(p.v, p.v_stride, p.B, p.Hkv, p.Lk, p.Dv, space);
+	return k;
+}
+int64_t packed_bytes(af3_diff_attention_params p) {
+	int32_t columns;
+	return pack_inputs(p, columns, columns, nullptr).bytes;
+}
 int64_t forward_workspace(const af3_diff_attention_params& p, const plan& f) {
-	return (f.splits > 1 ? (int64_t)f.splits * p.B * p.H * p.Lq * (p.Dv + 2) * 8 : 0) + values_bytes(p, f) + units_bytes(p, f);
+	return packed_bytes(p) + (f.splits > 1 ? (int64_t)f.splits * p.B * p.H * p.Lq * (p.Dv + 2) * 8 : 0) + values_bytes(p, f) + units_bytes(p, f);
 }
 
 }  // namespace diff
@@ -583,14 +622,17 @@ extern "C" int af3_diff_attention_forward(const af3_diff_attention_params* param
 	diff::forward_args a;
 	const bool         fp32 = params->dtype == AF3_F32;
 	a.p = *params, a.row_tiles = f.row_tiles, a.splits = f.splits, a.part = f.part;
-	a.factor  = params->softmax_scale * LOG2E;
-	a.whole_k = params->D * (fp32 ? 4 : 2) % 16 == 0, a.whole_v = params->Dv * (fp32 ? 4 : 2) % 16 == 0;
+	a.factor = params->softmax_scale * LOG2E;
+	unsigned char* space = static_cast<unsigned char*>(params->workspace);
+	const diff::packing pack = diff::pack_inputs(a.p, a.columns, a.v_columns, space);
+	space += pack.bytes;
 	const int64_t n_rows = params->B * params->H * params->Lq;
-	unsigned char* const space = static_cast<unsigned char*>(params->workspace);
 	a.values   = f.half ? space : nullptr, a.units = reinterpret_cast<float*>(space + diff::values_bytes(*params, f));
 	a.part_out = reinterpret_cast<float*>(space + diff::values_bytes(*params, f) + diff::units_bytes(*params, f)), a.part_stat = a.part_out + 2 * f.splits * n_rows * params->Dv;
 	const uint32_t grid = (uint32_t)(params->B * params->Hkv) * f.row_tiles * f.splits;
-	const int rc = fp32 ? diff::launch_forward_type<float>(a, f.kw, grid, s) : diff::launch_forward_type<uint16_t>(a, f.kw, grid, s);
+	int rc = pack.launch(s);
+	if(rc != AF3_OK) return rc;
+	rc = fp32 ? diff::launch_forward_type<float>(a, f.kw, grid, s) : diff::launch_forward_type<uint16_t>(a, f.kw, grid, s);
 	if(rc != AF3_OK || f.splits == 1) return rc;
 	const dim3 joins((uint32_t)((n_rows + cross::WAVES - 1) / cross::WAVES)), threads(cross::THREADS);
 	if(params->Dv <= 128) {

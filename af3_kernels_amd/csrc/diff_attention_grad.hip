@@ -3,8 +3,9 @@
 //     dS1 = P1 * (dP - d1),  dS2 = -lam P2 * (dP - d2),  dq_i = scale dS_i . k_i,  dk_i = scale dS_i^T . q_i,  dlam = -sum of d2 over the head's rows.
 // P1 and P2 are computed again from q, k and the two numbers per row and map that the forward pass left.  Kernels, none with atomics: each element of a result is
 // summed by one workgroup, or by one per part of the long axis and a joining kernel, always in the same order.
-//   diff_dq_kernel    32 query rows per wavefront, both maps, keys in tiles (writes d1 and d2 too)
-//   diff_dkv_kernel   32 keys per wavefront, both maps, query rows in tiles, over all heads of the key head
+//   diff_delta_kernel d1 and d2
+//   diff_dq_kernel    32 query rows per wavefront, both maps, keys in tiles
+//   diff_dkv_kernel   32 keys per wavefront, query rows in tiles, over all heads of the key head
 //   diff_lam_kernel   the sums of d2, and of the rows of P2 * (dP - d2): those would be zero, but for what d2 misses by the forward pass's probabilities, rounded to bf16 as they are
 //                     there.  dlam is a sum of many rows' d2 that mostly cancel: without that it was off by up to 0.008 of itself in sums over 300 rows (with: 1e-6 before its last rounding).
 #include "diff_tiles.hpp"
@@ -18,13 +19,13 @@ struct grad_args {
 	af3_diff_attention_params p;
 	af3_diff_attention_grads  g;
 	uint32_t tiles, splits;   // workgroups per (batch, key head), parts of the long axis
-	int64_t  part;            // dq: keys per part; dkv: tiles of query rows per part
+	int64_t  part;            // dq: keys per part; dK and dV: tiles of query rows per part
 	float    factor;
-	int32_t  whole_k, whole_v;
+	int32_t  columns, v_columns;   // of q and k, of v and grad_out, as they are read: whole pieces
 	float *  d1, *d2;         // [B, H, Lq] each
 	float*   short_of;        // what d2 is short of, in `shorts` parts [B, H, Lq], or null
 	uint32_t shorts;
-	float*   partial;         // dq: [splits][B 2H Lq][D]; dkv: [splits]([B 2Hkv Lk][D], [B Hkv Lk][Dv])
+	float*   partial;         // dq: [splits][B 2H Lq][D]; dK and dV: [splits]([B 2Hkv Lk][D], [B Hkv Lk][Dv])
 	float *  dq_space, *dkv_space;
 };
 
@@ -53,36 +54,54 @@ __device__ __forceinline__ void add_up(float* tables, int w, int lane, f32x16 (&
 	}
 }
 
-// a lane's half of a row times its half of the gradient of out, both half-waves added
-template <typename T, int DV, int N>
-__device__ __forceinline__ float row_dot(const u32x4 (&gf)[N], const T* row, bool ok, int Dv, int lane) {
-	u32x4 of[N];
-	load_operand<T, DV>(of, row, ok, Dv, lane);
-	float sum = 0.f;
-#pragma unroll
-	for(int s = 0; s < N; s++)
-#pragma unroll
-		for(int e = 0; e < kind<T>::E; e++) sum = __builtin_fmaf(kind<T>::at(gf[s], e), kind<T>::at(of[s], e), sum);
-	return sum_of_halves(sum);
-}
-// d1 and d2 of a lane's query row
-template <typename T, int DV, int N>
-__device__ __forceinline__ void row_deltas(const grad_args& a, const u32x4 (&gf)[N], int64_t b, int64_t h, int64_t qi, bool ok, int lane, float& d1, float& d2) {
+// d1 and d2: 32 lanes per row, 8 columns each (those of out and of second are read to 16 bits where the forward pass left what their rounding lost)
+template <typename T>
+__global__ void __launch_bounds__(THREADS) diff_delta_kernel(grad_args a) {
 	const af3_diff_attention_params& p = a.p;
-	const int64_t row = (b * p.H + h) * p.Lq + qi;
-	const int     Dv = (int)p.Dv;
-	d2 = row_dot<T, DV>(gf, static_cast<const T*>(p.second) + row * Dv, ok, Dv, lane);
-	d1 = row_dot<T, DV>(gf, static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2], ok, Dv, lane);
+	const int64_t row = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), n_rows = p.B * p.H * p.Lq;
+	if(row >= n_rows) return;   // (half a wavefront)
+	const int64_t bh = row / p.Lq, qi = row - bh * p.Lq, b = bh / p.H, h = bh - b * p.H;
+	const int     lane = threadIdx.x & 31, Dv = (int)p.Dv;
+	auto eight = [&](const T* from, float (&x)[8]) {
+		if(8 * lane + 8 <= Dv) {
+			if constexpr(sizeof(T) == 2) {
+				const u32x4 v = load16(from + 8 * lane);
+#pragma unroll
+				for(int e = 0; e < 8; e++) x[e] = kind<T>::at(v, e);
+			} else {
+				const u32x4 v = load16(from + 8 * lane), w = load16(from + 8 * lane + 4);
+#pragma unroll
+				for(int e = 0; e < 4; e++) x[e] = kind<T>::at(v, e), x[4 + e] = kind<T>::at(w, e);
+			}
+		} else {
+#pragma unroll
+			for(int e = 0; e < 8; e++) {
+				x[e] = 0.f;
+				if(8 * lane + e < Dv) x[e] = kind<T>::value(from[8 * lane + e]);
+			}
+		}
+	};
+	float g[8], o[8], s[8];
+	eight(static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1] + qi * a.g.grad_out_stride[2], g);
+	eight(static_cast<const T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2], o);
+	eight(static_cast<const T*>(p.second) + row * Dv, s);
 	if(sizeof(T) == 2 && p.residuals) {
-		const T* const lost = static_cast<const T*>(p.residuals) + row * Dv;
-		d1 += row_dot<T, DV>(gf, lost, ok, Dv, lane);
-		d2 += row_dot<T, DV>(gf, lost + p.B * p.H * p.Lq * Dv, ok, Dv, lane);
+		float x[8], y[8];
+		eight(static_cast<const T*>(p.residuals) + row * Dv, x);
+		eight(static_cast<const T*>(p.residuals) + (n_rows + row) * Dv, y);
+#pragma unroll
+		for(int e = 0; e < 8; e++) o[e] += x[e], s[e] += y[e];
 	}
-	d1 = __builtin_fmaf(lam_of(p, h), d2, d1);
+	float d1 = 0.f, d2 = 0.f;
+#pragma unroll
+	for(int e = 0; e < 8; e++) d1 = __builtin_fmaf(g[e], o[e], d1), d2 = __builtin_fmaf(g[e], s[e], d2);
+#pragma unroll
+	for(int i = 16; i; i >>= 1) d1 += __shfl_xor(d1, i), d2 += __shfl_xor(d2, i);
+	if(lane == 0) a.d1[row] = __builtin_fmaf(lam_of(p, h), d2, d1), a.d2[row] = d2;
 }
 
 // How many rows a tile has, and how many threads and maps of a wavefront the kernels have, by the bytes of a row of q or k (of 32, 64 or 128 columns).
-constexpr int tile_rows(int bytes, int sharing) { return sharing > 1 ? 32 * sharing : bytes <= 64 ? 128 : bytes <= 128 ? 64 : 32; }
+constexpr int tile_rows(int bytes, int sharing) { return sharing == 4 || bytes <= 64 ? 128 : bytes <= 128 ? 64 : 32; }
 constexpr int dq_maps(int bytes) { return bytes <= 128 ? 2 : 1; }
 constexpr int dq_threads(int bytes) { return 512; }
 constexpr int dkv_maps(int bytes) { return bytes <= 128 ? 2 : 1; }
@@ -116,7 +135,7 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 	const uint32_t split = own.piece / a.tiles, row_tile = a.tiles - 1 - (own.piece - split * a.tiles);
 	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
 	const int64_t G = p.H / p.Hkv, rows = G * p.Lq;
-	const int     D = (int)p.D, Dv = (int)p.Dv;
+	const int     D = (int)p.D;
 
 	const int64_t   R = (int64_t)row_tile * S::ROWS + 32 * group + (lane & 31);
 	const row_place at_row(R, rows, G, hk);
@@ -124,12 +143,10 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 	const int64_t   qi = at_row.qi, h = at_row.h, row = (b * p.H + h) * p.Lq + qi;
 	u32x4 qf[MAPS][TK::STEPS], gf[TV::STEPS];
 #pragma unroll
-	for(int i = 0; i < MAPS; i++) load_operand<T, DP>(qf[i], static_cast<const T*>(p.q) + b * p.q_stride[0] + (2 * h + map0 + i) * p.q_stride[1] + qi * p.q_stride[2], ok, D, lane);
-	load_operand<T, S::DV>(gf, static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1] + qi * a.g.grad_out_stride[2], ok, Dv, lane);
-	float d1, d2, delta[MAPS];
-	row_deltas<T, S::DV>(a, gf, b, h, qi, ok, lane, d1, d2);
-	if(ok && half == 0 && kwave == 0 && map0 == 0 && split == 0) a.d1[row] = d1, a.d2[row] = d2;
-	if(!a.g.grad_q && !a.short_of) return;
+	for(int i = 0; i < MAPS; i++) load_rows<T, DP>(qf[i], static_cast<const T*>(p.q) + b * p.q_stride[0] + (2 * h + map0 + i) * p.q_stride[1] + qi * p.q_stride[2], ok, a.columns, lane);
+	load_rows<T, S::DV>(gf, static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1] + qi * a.g.grad_out_stride[2], ok, a.v_columns, lane);
+	const float d1 = ok ? a.d1[row] : 0.f, d2 = ok ? a.d2[row] : 0.f;
+	float delta[MAPS];
 	float m[MAPS], inv[MAPS], taken[MAPS];
 	bool  far = false;
 #pragma unroll
@@ -158,13 +175,12 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 		last = end < last ? end : last;
 	}
 	const int64_t limit = p.causal ? qi + p.q_offset : (int64_t)1 << 41;
-	const typename TK::reader at_k(lane);
-	const typename TV::reader at_v(lane);
-	passage<T, DP, KT, S::NT>    pk[2];
-	passage<T, S::DV, KT, S::NT> pv;
-	pk[0].begin(kb, p.k_stride[2], D, a.whole_k);
-	pk[1].begin(kb + p.k_stride[1], p.k_stride[2], D, a.whole_k);
-	pv.begin(vb, p.v_stride[2], Dv, a.whole_v);
+	const typename TK::reader at_k_(lane);
+	const typename TV::reader at_v_(lane);
+	carrier<T, DP, KT, S::NT>    pk[2];
+	carrier<T, S::DV, KT, S::NT> pv;
+	pk[0].begin(p.k_stride[2], a.columns);
+	pv.begin(p.v_stride[2], a.v_columns);
 	int buffer = 0;
 	for(int64_t first = (int64_t)split * a.part; first < last; first += SEGMENT) {
 		const int64_t end = first + SEGMENT < last ? first + SEGMENT : last;
@@ -174,7 +190,7 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 		const int within = limit - first > SEGMENT ? SEGMENT : limit - first < -1 ? -1 : (int)(limit - first);
 		auto fetch = [&](int tile_no) {
 			const int64_t from = first + (int64_t)tile_no * KT;
-			pk[0].load(from, end), pk[1].load(from, end), pv.load(from, end);
+			pk[0].load(kb, from, end), pk[1].load(kb + p.k_stride[1], from, end, pk[0]), pv.load(vb, from, end);
 		};
 		fetch(t);
 		while(t >= 0) {
@@ -186,16 +202,18 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 			if constexpr(S::BUFFERS == 1) __syncthreads();
 			// (V is only multiplied row by row, and dS of a dropped key is not looked at; K's rows are added up under weights of zero)
 			pk[0].store(ks, full, [&](int r) { return bits.keeps(r); });
-			pk[1].store(ks + S::KTILE, full, [&](int r) { return bits.keeps(r); });
+			pk[1].store(ks + S::KTILE, full, [&](int r) { return bits.keeps(r); }, a.columns);
 			pv.store(vs, true, [](int) { return true; });
 			__syncthreads();
 			if(following >= 0) fetch(following);
-#pragma unroll
+#pragma unroll 1
 			for(int s = 0; s < S::SUB; s++) {
 				const int      block = kwave * S::SUB + s;
 				const uint32_t keep  = bits.of_block(block);
 				const int      left = within - (t * KT + 32 * block + 16 * half);
 				if(keep == 0u || !__any(ok && left >= 0)) continue;
+				const typename TK::reader at_k = fresh(at_k_);
+				const typename TV::reader at_v = fresh(at_v_);
 				const bool diagonal = __any(ok && left < 15);
 				f32x16 dp{};
 #pragma unroll
@@ -248,29 +266,31 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 			float v[16];
 #pragma unroll
 			for(int r = 0; r < 16; r++) v[r] = dq[i][db][r] * scale;
-			if(a.splits > 1) store_row16(a.partial + (split * (p.B * 2 * p.H * p.Lq) + to) * D, 32 * db + 16 * half, D, v);
-			else store_row16(static_cast<T*>(a.g.grad_q) + to * D, 32 * db + 16 * half, D, v);
+			if(a.splits > 1) store_columns(a.partial + (split * (p.B * 2 * p.H * p.Lq) + to) * D, 32 * db + 16 * half, D, v);
+			else store_columns(static_cast<T*>(a.g.grad_q) + to * D, 32 * db + 16 * half, D, v);
 		}
 	}
 }
 
 // What the kernel with query rows in tiles keeps of each row of a tile in LDS: d1 and d2, and per map the whole reference (bf16), maximum and 1 / sum (fp32 and tiles with
-// a row far from zero).  Behind them a word per 64 rows that says whether there is one.
+// a row far from zero).  Behind them a word per 64 rows that says whether there is one.  (As a further step of the products instead, three bf16 terms to a number, they were
+// no faster: 236 us for 226 at 4 x 8 (2) x 1491 x 64, 230 for 190 at 4 x 8 x 1024 x 128.)
 enum { LESS = 0, TAKEN = 2, MOST = 4, INVERSE = 6, ROW_STATS = 8 };
 template <typename T, int QT>
 struct row_stats {
+	static constexpr int BYTES = ROW_STATS * QT * 4 + 16;
 	float v[ROW_STATS];   // of one row, on its way
-	__device__ __forceinline__ void load(const grad_args& a, int64_t b, int64_t h, int64_t q0) {
+	__device__ __forceinline__ void load(const grad_args& a, int64_t bh, int q0) {   // bh: b * H + h
 #pragma unroll
 		for(int i = 0; i < ROW_STATS; i++) v[i] = 0.f;
-		const int64_t qi = q0 + threadIdx.x;
-		if((int)threadIdx.x >= QT || qi >= a.p.Lq) return;
-		const int64_t row = (b * a.p.H + h) * a.p.Lq + qi;
-		v[LESS] = a.d1[row], v[LESS + 1] = a.d2[row];
+		const int qi = q0 + (int)threadIdx.x;
+		if((int)threadIdx.x >= QT || qi >= (int)a.p.Lq) return;
+		const int64_t first = bh * a.p.Lq;
+		v[LESS] = a.d1[first + qi], v[LESS + 1] = a.d2[first + qi];
 #pragma unroll
 		for(int i = 0; i < 2; i++) {
-			const int64_t at = (b * 2 * a.p.H + 2 * h + i) * a.p.Lq + qi;
-			v[MOST + i] = a.p.stats[2 * at], v[INVERSE + i] = a.p.stats[2 * at + 1];
+			const float* const st = a.p.stats + 4 * first + 2 * i * a.p.Lq + 2 * qi;
+			v[MOST + i] = st[0], v[INVERSE + i] = st[1];
 		}
 	}
 	__device__ __forceinline__ void store(float* st, float factor) {
@@ -301,17 +321,16 @@ struct row_stats {
 };
 
 // ---- dK, dV ----
-// RW: wavefronts that share 32 keys and each take 32 rows of a tile of query rows (1: every wavefront has its own keys and takes the whole tile)
+// RW: wavefronts that share 32 keys and each take 32 rows of a tile of query rows (1: every wavefront has its own keys and takes the whole tile).  MAPS as in dq_shape.
 template <typename T, int DP, int RW>
 struct dkv_shape {
 	static constexpr int BYTES = DP * (int)sizeof(T), MAPS = dkv_maps(BYTES), NT = dkv_threads(BYTES), W = NT / 64, GROUPS = W * MAPS / 2 / RW;
 	static constexpr int DV = 2 * DP, QT = tile_rows(BYTES, RW), SUB = QT / (32 * RW), KEYS = 32 * GROUPS;
-	static constexpr int VW = RW * (MAPS == 2 ? 1 : 2);   // wavefronts that have a part of the same rows of dV
-	static constexpr int QTILE = QT * tile<T, DP>::STRIDE, GTILE = QT * tile<T, DV>::STRIDE, STATS = ROW_STATS * QT * 4 + 16, SET = 2 * QTILE + GTILE + STATS;
+	static constexpr int QTILE = QT * tile<T, DP>::STRIDE, GTILE = QT * tile<T, DV>::STRIDE, STATS = row_stats<T, QT>::BYTES, SET = 2 * QTILE + GTILE + STATS;
 	static constexpr int BUFFERS = 2 * SET <= 73728 ? 2 : 1;
-	static constexpr int JOIN = VW > 1 ? W * 32 * (DV + 4) * 4 : 0;
+	static constexpr int VW = RW * (MAPS == 2 ? 1 : 2);   // wavefronts that have a part of the same rows of dV
+	static constexpr int JOIN = VW > 1 ? W * 32 * (DV + 4) * 4 : 0, PER_SIMD = BYTES <= 64 ? 2 : 1;   // wavefronts to a SIMD, by the registers of sums and operands
 	static constexpr int LDS = BUFFERS * SET > JOIN ? BUFFERS * SET : JOIN;
-	static constexpr int PER_SIMD = NT == 512 || BYTES <= 64 ? 2 : 1;
 };
 
 template <typename T, int DP, int RW>
@@ -329,15 +348,14 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 	const uint32_t split = own.piece / a.tiles, key_tile = own.piece - split * a.tiles;   // (causal: the first keys have the most rows)
 	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
 	const int64_t G = p.H / p.Hkv;
-	const int     D = (int)p.D, Dv = (int)p.Dv;
 
 	const int64_t key0 = (int64_t)key_tile * S::KEYS, key = key0 + 32 * group + (lane & 31);
 	const bool    in = key < p.Lk;
 	const bool    lives = in && (!p.key_mask || p.key_mask[b * p.key_mask_stride_b + key] != 0);
 	u32x4 kf[MAPS][TK::STEPS], vf[TV::STEPS];
 #pragma unroll
-	for(int i = 0; i < MAPS; i++) load_operand<T, DP>(kf[i], static_cast<const T*>(p.k) + b * p.k_stride[0] + (2 * hk + map0 + i) * p.k_stride[1] + (in ? key : 0) * p.k_stride[2], in, D, lane);
-	load_operand<T, S::DV>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], in, Dv, lane);
+	for(int i = 0; i < MAPS; i++) load_rows<T, DP>(kf[i], static_cast<const T*>(p.k) + b * p.k_stride[0] + (2 * hk + map0 + i) * p.k_stride[1] + (in ? key : 0) * p.k_stride[2], in, a.columns, lane);
+	load_rows<T, S::DV>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], in, a.v_columns, lane);
 	const bool work = __any(lives);   // (of this wavefront)
 
 	f32x16 dk[MAPS][TK::BLOCKS], dv[TV::BLOCKS];
@@ -348,61 +366,60 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 #pragma unroll
 	for(int db = 0; db < TV::BLOCKS; db++) dv[db] = f32x16{};
 
-	const int64_t q_tiles = (p.Lq + QT - 1) / QT, n = G * q_tiles;
+	// Tiles of query rows, head after head: tile `at` of head `head` of the group, counted head * q_tiles + at (below 2^25).
+	const int q_tiles = (int)((p.Lq + QT - 1) / QT), n = (int)G * q_tiles, Lq = (int)p.Lq;
 	// (causal: queries in front of the workgroup's first key have nothing of it)
-	const int64_t from = p.causal && key0 > p.q_offset ? (key0 - p.q_offset) / QT : 0;
-	const int64_t last = (int64_t)(split + 1) * a.part < n ? (int64_t)(split + 1) * a.part : n;
-	const typename TK::reader at_q(lane);
-	const typename TV::reader at_g(lane);
-	passage<T, DP, QT, S::NT>    pq[2];
-	passage<T, S::DV, QT, S::NT> pg;
-	pq[0].begin(nullptr, p.q_stride[2], D, a.whole_k);
-	pq[1].begin(nullptr, p.q_stride[2], D, a.whole_k);
-	pg.begin(nullptr, a.g.grad_out_stride[2], Dv, a.whole_v);
+	const int from = p.causal && key0 > p.q_offset ? (int)((key0 - p.q_offset) / QT < q_tiles ? (key0 - p.q_offset) / QT : q_tiles) : 0;
+	const int last = (int)((int64_t)(split + 1) * a.part < n ? (int64_t)(split + 1) * a.part : n);
+	const typename TK::reader at_q_(lane);
+	const typename TV::reader at_g_(lane);
+	carrier<T, DP, QT, S::NT>    pq[2];
+	carrier<T, S::DV, QT, S::NT> pg;
+	pq[0].begin(p.q_stride[2], a.columns);
+	pg.begin(a.g.grad_out_stride[2], a.v_columns);
 	row_stats<T, QT> rs;
-	auto fetch = [&](int64_t it) {
-		const int64_t h = hk * G + it / q_tiles, q0 = it % q_tiles * QT;
-		pq[0].base = static_cast<const T*>(p.q) + b * p.q_stride[0] + 2 * h * p.q_stride[1];
-		pq[1].base = pq[0].base + p.q_stride[1];
-		pg.base = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + h * a.g.grad_out_stride[1];
-		pq[0].load(q0, p.Lq), pq[1].load(q0, p.Lq), pg.load(q0, p.Lq);
-		rs.load(a, b, h, q0);
+	const T* const qb = static_cast<const T*>(p.q) + b * p.q_stride[0] + 2 * hk * G * p.q_stride[1];
+	const T* const gb = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + hk * G * a.g.grad_out_stride[1];
+	auto fetch = [&](int head, int at) {
+		const T* const q = qb + 2 * head * p.q_stride[1];
+		pq[0].load(q, at * QT, Lq), pq[1].load(q + p.q_stride[1], at * QT, Lq, pq[0]), pg.load(gb + head * a.g.grad_out_stride[1], at * QT, Lq);
+		rs.load(a, b * p.H + hk * G + head, at * QT);
 	};
-	auto next = [&](int64_t it) {   // the first tile from `it` on that counts
-		const int64_t head = it / q_tiles;
-		return it - head * q_tiles < from ? (from < q_tiles ? head * q_tiles + from : (head + 1) * q_tiles + from) : it;
-	};
-	int     buffer = 0;
-	int64_t it = from < q_tiles ? next((int64_t)split * a.part) : last;
+	int head = (int)((int64_t)split * a.part) / q_tiles, at = (int)((int64_t)split * a.part) - head * q_tiles;
+	if(at < from) at = from;
+	if(at >= q_tiles) head++, at = from;
+	int buffer = 0;
 	// (a workgroup none of whose keys counts has nothing to read)
 	const bool any = __syncthreads_or(work);
-	if(!any) it = last;
-	if(it < last) fetch(it);
-	while(it < last) {
+	bool more = any && from < q_tiles && head * q_tiles + at < last;
+	if(more) fetch(head, at);
+	while(more) {
 		unsigned char* const qs = smem + buffer * S::SET;
 		unsigned char* const gs = qs + 2 * S::QTILE;
 		float* const         st = reinterpret_cast<float*>(gs + S::GTILE);
-		const int64_t        q0 = it % q_tiles * QT;
-		const float          lam = lam_of(p, hk * G + it / q_tiles);
+		const int            q0 = at * QT, left = Lq - q0;
+		const float          lam = lam_of(p, hk * G + head);
 		if constexpr(S::BUFFERS == 1) __syncthreads();
-		const int64_t left = p.Lq - q0;
 		pq[0].store(qs, left >= QT, [&](int r) { return r < left; });
-		pq[1].store(qs + S::QTILE, left >= QT, [&](int r) { return r < left; });
+		pq[1].store(qs + S::QTILE, left >= QT, [&](int r) { return r < left; }, a.columns);
 		pg.store(gs, left >= QT, [&](int r) { return r < left; });
 		rs.store(st, a.factor);
 		__syncthreads();
-		const bool    apart = rs.apart(st);
-		const int64_t following = next(it + 1);
-		if(following < last) fetch(following);
+		if(++at == q_tiles) head++, at = from;
+		more = head * q_tiles + at < last;
+		if(more) fetch(head, at);
+		const bool apart = rs.apart(st);
 		if(work) {
-#pragma unroll
+#pragma unroll 1
 			for(int s = 0; s < S::SUB; s++) {
 				const int row0 = 32 * (rwave * S::SUB + s);
-				if(q0 + row0 >= p.Lq) continue;
+				if(row0 >= left) continue;
 				// the lane's rows need .. 15 of its 16 count
 				const int need = p.causal ? clamped(key - p.q_offset - (q0 + row0 + 16 * half)) : -64;
 				if(!__any(in && need <= 15)) continue;
 				const bool diagonal = __any(in && need > 0);
+				const typename TK::reader at_q = S::PER_SIMD == 2 ? fresh(at_q_) : at_q_;
+				const typename TV::reader at_g = S::PER_SIMD == 2 ? fresh(at_g_) : at_g_;
 				const float* const sm = st + row0 + 16 * half;
 				f32x16 dp{};
 #pragma unroll
@@ -415,7 +432,7 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 					f32x16 acc{};
 #pragma unroll
 					for(int k = 0; k < TK::STEPS; k++) acc = kind<T>::mma(TK::row_frag(qm, row0, k, at_q), kf[i][k], acc);
-					float x[16], y[16];
+					float x[16];
 					if(apart) {
 						const f32x16 m = rs.sixteen(sm + (MOST + map) * QT), inv = rs.sixteen(sm + (INVERSE + map) * QT);
 #pragma unroll
@@ -433,15 +450,14 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 #pragma unroll
 						for(int r = 0; r < 16; r++) x[r] *= -lam;
 					}
+#pragma unroll
+					for(int r = 0; r < 16; r++) both[r] = i == 0 ? x[r] : both[r] + x[r];
 					const f32x16 less = rs.sixteen(sm + (LESS + map) * QT);
 #pragma unroll
-					for(int r = 0; r < 16; r++) {
-						y[r]    = x[r] * (dp[r] - less[r]);
-						both[r] = i == 0 ? x[r] : both[r] + x[r];
-					}
+					for(int r = 0; r < 16; r++) x[r] *= dp[r] - less[r];
 #pragma unroll
 					for(int j = 0; j < TK::JOINTS; j++) {
-						const u32x4 df = kind<T>::pack(y + E * j);
+						const u32x4 df = kind<T>::pack(x + E * j);
 #pragma unroll
 						for(int db = 0; db < TK::BLOCKS; db++) dk[i][db] = kind<T>::mma(TK::col_frag(qm, row0, db, j, at_q), df, dk[i][db]);
 					}
@@ -454,7 +470,6 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 				}
 			}
 		}
-		it = following;
 		if constexpr(S::BUFFERS == 2) buffer ^= 1;
 	}
 	float* const tables = reinterpret_cast<float*>(smem);
@@ -465,6 +480,7 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 	const int vwave = MAPS == 2 ? rwave : 2 * rwave + map0;
 	if constexpr(S::VW > 1) add_up<S::DV, S::VW>(tables + group * S::VW * 32 * (S::DV + 4), vwave, lane, dv);
 	if(!in) return;
+	const int     D = (int)p.D, Dv = (int)p.Dv;
 	const int64_t n_keys = p.B * p.Hkv * p.Lk, place = (b * p.Hkv + hk) * p.Lk + key;
 	float* const  partial = a.partial + (int64_t)split * n_keys * (2 * D + Dv);
 #pragma unroll
@@ -476,8 +492,8 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 			float k[16];
 #pragma unroll
 			for(int r = 0; r < 16; r++) k[r] = lives ? dk[i][db][r] * p.softmax_scale : 0.f;
-			if(a.splits > 1) store_row16(partial + to * D, 32 * db + 16 * half, D, k);
-			else if(a.g.grad_k) store_row16(static_cast<T*>(a.g.grad_k) + to * D, 32 * db + 16 * half, D, k);
+			if(a.splits > 1) store_columns(partial + to * D, 32 * db + 16 * half, D, k);
+			else if(a.g.grad_k) store_columns(static_cast<T*>(a.g.grad_k) + to * D, 32 * db + 16 * half, D, k);
 		}
 	}
 #pragma unroll
@@ -486,8 +502,8 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 		float v[16];
 #pragma unroll
 		for(int r = 0; r < 16; r++) v[r] = lives ? dv[db][r] : 0.f;
-		if(a.splits > 1) store_row16(partial + 2 * n_keys * D + place * Dv, 32 * db + 16 * half, Dv, v);
-		else if(a.g.grad_v) store_row16(static_cast<T*>(a.g.grad_v) + place * Dv, 32 * db + 16 * half, Dv, v);
+		if(a.splits > 1) store_columns(partial + 2 * n_keys * D + place * Dv, 32 * db + 16 * half, Dv, v);
+		else if(a.g.grad_v) store_columns(static_cast<T*>(a.g.grad_v) + place * Dv, 32 * db + 16 * half, Dv, v);
 	}
 }
 
@@ -553,53 +569,73 @@ __global__ void __launch_bounds__(THREADS) diff_sum_kernel(parts a) {
 int width(const af3_diff_attention_params& p);   // (diff_attention.hip)
 
 struct cut {
-	bool     shared;   // wavefronts share 32 rows (dq) or keys (dkv)
+	int      sharing;   // wavefronts that share 32 rows (dq) or keys (dK, dV)
 	uint32_t tiles, splits;
 	int64_t  part;
 };
 inline int64_t over(int64_t n, int64_t per) { return (n + per - 1) / per; }
 // bytes of a row of K as the kernels have it
 int row_bytes(const af3_diff_attention_params& p) { return width(p) * (p.dtype == AF3_F32 ? 4 : 2); }
-
-// `length` rows that results belong to (`alone` or `together` of them per workgroup), `steps(shared)` tiles of the other axis.  Wavefronts share where their workgroups fit the chip together.
-template <typename F>
-cut cut_for(int64_t length, int64_t groups, int64_t alone, int64_t together, bool may_share, int64_t slots, double tile_us, double part_bytes, F steps) {
-	cut c;
-	c.shared = may_share && (length <= together || over(length, together) * groups <= slots);
-	c.tiles  = (uint32_t)over(length, c.shared ? together : alone);
-	const int64_t n = steps(c.shared);
-	const int64_t sp = parts_for(groups * c.tiles, slots, n, tile_us * (c.shared ? 1.0 : 0.6), part_bytes, 64);
-	c.part   = over(n, sp);
-	c.splits = (uint32_t)over(n, c.part);
-	return c;
+// the part of all (query, key) pairs that counts
+double counting(const af3_diff_attention_params& p) {
+	if(!p.causal) return 1.0;
+	const double first = (double)p.q_offset + 1.0, last = (double)p.q_offset + (double)p.Lq, Lk = (double)p.Lk;   // keys of the first and the last query
+	const double a = first < 0.0 ? 0.0 : first > Lk ? Lk : first, b = last < 0.0 ? 0.0 : last > Lk ? Lk : last;
+	const double rising = b - a, full = last > Lk ? last - (first > Lk ? first : Lk) : 0.0;
+	const double pairs = rising * (a + b) * 0.5 + full * Lk;
+	return pairs <= 0.0 ? 1e-3 : pairs / ((double)p.Lq * Lk);
 }
-constexpr bool may_share(int bytes) { return bytes <= 128; }   // (wider rows: the tile of 128 leaves neither registers nor LDS)
+// `length` rows that results belong to, `alone` of them per workgroup where every wavefront has its own; `steps(sharing)` tiles of the other axis, of which a launch walks the part
+// `counts`, the workgroups with the most first; `slots` workgroups fit the chip at a time; a tile costs load_us and block_us for each block of 32 x 32 that a wavefront has of it.
+// Sharing makes more and shorter workgroups, so do parts of the long axis, whose results go through memory and are joined: whatever ends first.
+template <typename F>
+cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double counts, int64_t slots, double load_us, double block_us, double part_bytes, F steps) {
+	constexpr double JOIN_US = 6.0, BYTES_PER_US = 2e6;
+	cut    best{};
+	double best_us = 0.0;
+	for(int sharing = 1; sharing <= (bytes > 128 ? 1 : 4); sharing *= 2) {
+		const int64_t tiles = over(length, alone / sharing), n = steps(sharing), workgroups = groups * tiles;
+		const double  tile_us = load_us * tile_rows(bytes, sharing) / 64 + block_us * tile_rows(bytes, sharing) / (32 * sharing);
+		for(int64_t parts = 1; parts <= 64 && (parts == 1 || 2 * parts <= n + 1); parts++) {
+			const double longest = (double)over(n, parts), all = (double)workgroups * n * counts / slots;
+			const double us = (workgroups * parts <= slots ? longest : longest > all + 0.5 * longest ? longest : all + 0.5 * longest) * tile_us + (parts > 1 ? JOIN_US + parts * 2.0 * part_bytes / BYTES_PER_US : 0.0);
+			if(best_us == 0.0 || us < best_us) best_us = us, best.sharing = sharing, best.tiles = (uint32_t)tiles, best.part = over(n, parts), best.splits = (uint32_t)over(n, best.part);
+		}
+	}
+	return best;
+}
 cut dq_cut(const af3_diff_attention_params& p) {
-	const int     bytes = row_bytes(p);
-	const int64_t rows = 32 * dq_threads(bytes) / 64 * dq_maps(bytes) / 2, kt = tile_rows(bytes, 1);
-	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, rows, rows / 4, may_share(bytes), 256, (0.5 + 0.025 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0), 8.0 * p.B * p.H * p.Lq * p.D,
-					[&](bool shared) { return over(p.Lk, shared ? 128 : kt); });
-	c.part *= c.shared ? 128 : kt;
+	const int bytes = row_bytes(p);
+	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, 32 * dq_threads(bytes) / 64 * dq_maps(bytes) / 2, bytes, counting(p), 256, 0.4 + 0.009 * bytes, (0.4 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0),
+					8.0 * p.B * p.H * p.Lq * p.D, [&](int sharing) { return over(p.Lk, tile_rows(bytes, sharing)); });
+	c.part *= tile_rows(bytes, c.sharing);
 	return c;
 }
 cut dkv_cut(const af3_diff_attention_params& p) {
-	const int     bytes = row_bytes(p);
-	const int64_t keys = 32 * dkv_threads(bytes) / 64 * dkv_maps(bytes) / 2, qt = tile_rows(bytes, 1);
-	return cut_for(p.Lk, p.B * p.Hkv, keys, keys / 4, may_share(bytes), 256, (0.6 + 0.035 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0), 4.0 * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv),
-				   [&](bool shared) { return p.H / p.Hkv * over(p.Lq, shared ? 128 : qt); });
+	const int bytes = row_bytes(p);
+	return cut_for(p.Lk, p.B * p.Hkv, 32 * dkv_threads(bytes) / 64 * dkv_maps(bytes) / 2, bytes, counting(p), bytes > 64 ? 256 : 512, 0.3 + 0.006 * bytes, (0.5 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0),
+				   4.0 * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv), [&](int sharing) { return p.H / p.Hkv * over(p.Lq, tile_rows(bytes, sharing)); });
 }
 
+int64_t packed_grad_bytes(const af3_diff_attention_params& p) {
+	packing     k(p.dtype == AF3_F32 ? 4 : 2);
+	const void* grad = nullptr;
+	int64_t     stride[3] = {0, 0, 0};
+	k.add(grad, stride, p.B, p.H, p.Lq, p.Dv, nullptr);
+	return k.bytes;
+}
 struct grad_space {
-	int64_t delta, shorts, dq, dkv, bytes;   // floats
+	int64_t delta, shorts, dq, dkv, packed, bytes;   // floats; bytes of what is laid out anew, of all
 };
 grad_space grad_workspace(const af3_diff_attention_params& p) {
 	const cut  q = dq_cut(p), kv = dkv_cut(p);
 	grad_space w;
 	w.delta = over(p.B * p.H * p.Lq, 4) * 4;
-	w.shorts = over((int64_t)q.splits * (q.shared ? 4 : 1) * p.B * p.H * p.Lq, 4) * 4;
+	w.shorts = over((int64_t)q.splits * q.sharing * p.B * p.H * p.Lq, 4) * 4;
 	w.dq    = q.splits > 1 ? over(2 * (int64_t)q.splits * p.B * p.H * p.Lq * p.D, 4) * 4 : 0;
 	w.dkv   = kv.splits > 1 ? over((int64_t)kv.splits * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv), 4) * 4 : 0;
-	w.bytes = (2 * w.delta + w.shorts + w.dq + w.dkv) * 4;
+	w.packed = packed_bytes(p) + packed_grad_bytes(p);
+	w.bytes = w.packed + (2 * w.delta + w.shorts + w.dq + w.dkv) * 4;
 	return w;
 }
 
@@ -618,7 +654,7 @@ template <typename T, int DP>
 int backward(grad_args a, hipStream_t s) {
 	const af3_diff_attention_params& p = a.p;
 	const int64_t n_rows = 2 * p.B * p.H * p.Lq, n_keys = p.B * p.Hkv * p.Lk;
-	constexpr bool SHARES = may_share(DP * (int)sizeof(T));
+	constexpr bool SHARES = DP * (int)sizeof(T) <= 128;   // (wider rows: tiles that several wavefronts share leave neither registers nor LDS)
 	parts    sums{};
 	int      n_sums = 0;
 	uint32_t sum_blocks = 0;
@@ -628,16 +664,21 @@ int backward(grad_args a, hipStream_t s) {
 		sum_blocks += sums.blocks[n_sums] = (uint32_t)over(n, 4 * THREADS);
 		n_sums++;
 	};
-	int rc = AF3_ERR_LAUNCH;
-	{   // (without grad_q and grad_lam: d1 and d2 alone)
+	hipLaunchKernelGGL(diff_delta_kernel<T>, dim3((uint32_t)over(p.B * p.H * p.Lq, THREADS / 32)), dim3(THREADS), 0, s, a);
+	int rc = launch_status();
+	if(rc != AF3_OK) return rc;
+	if(!a.g.grad_lam) a.short_of = nullptr;
+	if(a.g.grad_q || a.short_of) {
 		const cut c = dq_cut(p);
-		a.shorts = c.splits * (c.shared ? 4 : 1);
-		if(!a.g.grad_lam) a.short_of = nullptr;
-		a.tiles = c.tiles, a.splits = a.g.grad_q || a.short_of ? c.splits : 1, a.part = c.part, a.partial = a.dq_space;
+		a.shorts = c.splits * c.sharing;
+		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part, a.partial = a.dq_space;
 		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * a.tiles * a.splits;
-		if constexpr(SHARES)
-			if(c.shared) rc = launch<dq_shape<T, DP, 4>>(diff_dq_kernel<T, DP, 4>, grid, a, s);
-		if(!c.shared) rc = launch<dq_shape<T, DP, 1>>(diff_dq_kernel<T, DP, 1>, grid, a, s);
+		rc = AF3_ERR_LAUNCH;
+		if constexpr(SHARES) {
+			if(c.sharing == 2) rc = launch<dq_shape<T, DP, 2>>(diff_dq_kernel<T, DP, 2>, grid, a, s);
+			if(c.sharing == 4) rc = launch<dq_shape<T, DP, 4>>(diff_dq_kernel<T, DP, 4>, grid, a, s);
+		}
+		if(c.sharing == 1) rc = launch<dq_shape<T, DP, 1>>(diff_dq_kernel<T, DP, 1>, grid, a, s);
 		if(rc != AF3_OK) return rc;
 		if(a.splits > 1) add(a.partial, n_rows * p.D, c.splits, a.g.grad_q, n_rows * p.D);
 	}
@@ -646,9 +687,11 @@ int backward(grad_args a, hipStream_t s) {
 		a.tiles = c.tiles, a.splits = c.splits, a.part = c.part, a.partial = a.dkv_space;
 		const uint32_t grid = (uint32_t)(p.B * p.Hkv) * c.tiles * c.splits;
 		rc = AF3_ERR_LAUNCH;
-		if constexpr(SHARES)
-			if(c.shared) rc = launch<dkv_shape<T, DP, 4>>(diff_dkv_kernel<T, DP, 4>, grid, a, s);
-		if(!c.shared) rc = launch<dkv_shape<T, DP, 1>>(diff_dkv_kernel<T, DP, 1>, grid, a, s);
+		if constexpr(SHARES) {
+			if(c.sharing == 2) rc = launch<dkv_shape<T, DP, 2>>(diff_dkv_kernel<T, DP, 2>, grid, a, s);
+			if(c.sharing == 4) rc = launch<dkv_shape<T, DP, 4>>(diff_dkv_kernel<T, DP, 4>, grid, a, s);
+		}
+		if(c.sharing == 1) rc = launch<dkv_shape<T, DP, 1>>(diff_dkv_kernel<T, DP, 1>, grid, a, s);
 		if(rc != AF3_OK) return rc;
 		if(c.splits > 1) {
 			const int64_t step = n_keys * (2 * p.D + p.Dv);
@@ -672,6 +715,8 @@ int validate_grads(const af3_diff_attention_params* p, const af3_diff_attention_
 	if(!g || !g->grad_out || !p->stats || (!g->grad_q && !g->grad_k && !g->grad_v && !g->grad_lam)) return AF3_ERR_NULL_POINTER;
 	for(int i = 0; i < 3; i++)
 		if(g->grad_out_stride[i] < 0) return AF3_ERR_BAD_STRIDE;
+	const int bytes = p->dtype == AF3_F32 ? 4 : 2;
+	if(p->Dv * bytes % 16 == 0 && p->Lq > 1 && !takes(p->Dv, g->grad_out_stride[2], bytes)) return AF3_ERR_BAD_STRIDE;   // (the workspace has no place for it)
 	return AF3_OK;
 }
 
@@ -690,14 +735,16 @@ extern "C" int af3_diff_attention_backward(const af3_diff_attention_params* para
 	const diff::grad_space w = diff::grad_workspace(*params);
 	if(!grads->workspace || grads->workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(grads->workspace) & 15)) return AF3_ERR_BAD_ARGUMENT;
 	if(const int dc = current_device_status(); dc != AF3_OK) return dc;
-	const bool      fp32 = params->dtype == AF3_F32;
 	diff::grad_args a;
 	a.p = *params, a.g = *grads, a.tiles = a.splits = 1, a.part = 0, a.partial = nullptr;
-	a.factor  = params->softmax_scale * LOG2E;
-	a.whole_k = params->D * (fp32 ? 4 : 2) % 16 == 0, a.whole_v = params->Dv * (fp32 ? 4 : 2) % 16 == 0;
-	a.d1 = static_cast<float*>(grads->workspace), a.d2 = a.d1 + w.delta, a.short_of = a.d2 + w.delta, a.shorts = 0, a.dq_space = a.short_of + w.shorts, a.dkv_space = a.dq_space + w.dq;
+	a.factor = params->softmax_scale * LOG2E;
+	diff::packing pack = diff::pack_inputs(a.p, a.columns, a.v_columns, grads->workspace);
+	pack.add(a.g.grad_out, a.g.grad_out_stride, params->B, params->H, params->Lq, params->Dv, grads->workspace);
+	a.d1 = reinterpret_cast<float*>(static_cast<unsigned char*>(grads->workspace) + w.packed), a.d2 = a.d1 + w.delta, a.short_of = a.d2 + w.delta, a.shorts = 0;
+	a.dq_space = a.short_of + w.shorts, a.dkv_space = a.dq_space + w.dq;
 	const hipStream_t s = static_cast<hipStream_t>(hip_stream);
+	if(const int rc = pack.launch(s); rc != AF3_OK) return rc;
 	const int wide = diff::width(*params);
-	if(fp32) return wide == 32 ? diff::backward<float, 32>(a, s) : diff::backward<float, 64>(a, s);
+	if(params->dtype == AF3_F32) return wide == 32 ? diff::backward<float, 32>(a, s) : diff::backward<float, 64>(a, s);
 	return wide == 32 ? diff::backward<uint16_t, 32>(a, s) : wide == 64 ? diff::backward<uint16_t, 64>(a, s) : diff::backward<uint16_t, 128>(a, s);
 }

@@ -23,6 +23,87 @@ struct row_place {
 __device__ __forceinline__ float lam_of(const af3_diff_attention_params& p, int64_t h) {
 	return p.lam_dtype == AF3_F32 ? static_cast<const float*>(p.lam)[h * p.lam_stride] : bf16_bits_to_f32(static_cast<const uint16_t*>(p.lam)[h * p.lam_stride]);
 }
+// ---- rows on their way ----
+// The kernels take rows that are whole 16-byte pieces, no further apart than 32 bits reach over a tile; the host lays others out anew (diff_pack_kernel).  With the other way of reading
+// beside it in the same loop, as cross_tiles.hpp's passage has it, dK/dV held 756 branches and twice its scalars in vector registers' lanes, and took four times as long.
+inline bool takes(int64_t columns, int64_t stride, int bytes) { return columns * bytes % 16 == 0 && stride <= (int64_t)0x7fffffff / (128 * bytes); }
+// ROWS rows into a tile in LDS, spread over NT threads in 16-byte pieces: one load per piece, at a scalar base and an offset that stays the same from tile to tile
+template <typename T, int DP, int ROWS, int NT>
+struct carrier {
+	using TL = tile<T, DP>;
+	static constexpr int N = ROWS * TL::CHUNKS / NT, E = kind<T>::E;
+	static_assert(N * NT == ROWS * TL::CHUNKS);
+	u32x4    piece[N];
+	uint32_t offset[N];   // bytes from the tile's first row
+	int64_t  step;        // bytes of a row
+	int      D;
+	static __device__ __forceinline__ int row_of(int n) { return (threadIdx.x + NT * n) / TL::CHUNKS; }
+	static __device__ __forceinline__ int col_of(int n) { return (threadIdx.x + NT * n) % TL::CHUNKS; }
+	__device__ __forceinline__ void begin(int64_t stride, int columns) {
+		step = stride * (int)sizeof(T), D = columns;
+#pragma unroll
+		for(int n = 0; n < N; n++) offset[n] = col_of(n) * E < D ? (uint32_t)(row_of(n) * (int)step + col_of(n) * 16) : 0u;
+	}
+	// rows row0 .. row0 + ROWS - 1 from `base` on, those below `rows` exist (one at least); `like`: one that began with the same strides (this one need not have)
+	__device__ __forceinline__ void load(const T* base, int64_t row0, int64_t rows, const carrier& like) {
+		const unsigned char* const at   = reinterpret_cast<const unsigned char*>(base) + row0 * like.step;
+		const int                  left = rows - row0 < ROWS ? (int)(rows - row0) : ROWS;
+#pragma unroll
+		for(int n = 0; n < N; n++) piece[n] = load16(reinterpret_cast<const T*>(at + (row_of(n) < left ? like.offset[n] : 0u)));
+	}
+	__device__ __forceinline__ void load(const T* base, int64_t row0, int64_t rows) { load(base, row0, rows, *this); }
+	// all: every row of the tile is wanted; otherwise keep(row) says which, the others become zeros
+	template <typename F>
+	__device__ __forceinline__ void store(unsigned char* lds, bool all, F keep) const { store(lds, all, keep, D); }
+	template <typename F>
+	__device__ __forceinline__ void store(unsigned char* lds, bool all, F keep, int columns) const {
+#pragma unroll
+		for(int n = 0; n < N; n++) {
+			u32x4 v = piece[n];
+			if(!all || TL::CHUNKS * E != columns) {
+				const bool in = (all || keep(row_of(n))) && col_of(n) * E < columns;
+#pragma unroll
+				for(int i = 0; i < 4; i++) {
+					const uint32_t x = v[i];
+					v[i] = in ? x : 0u;
+				}
+			}
+			*reinterpret_cast<u32x4*>(lds + row_of(n) * TL::STRIDE + TL::place(row_of(n), col_of(n))) = v;
+		}
+	}
+};
+// a row as a B operand in registers, zeros where `ok` is not
+template <typename T, int DP, int N>
+__device__ __forceinline__ void load_rows(u32x4 (&f)[N], const T* row, bool ok, int columns, int lane) {
+	constexpr int E = kind<T>::E;
+	static_assert(N == tile<T, DP>::STEPS);
+#pragma unroll
+	for(int s = 0; s < N; s++) {
+		const int d = 2 * E * s + E * (lane >> 5);
+		f[s] = u32x4{0u, 0u, 0u, 0u};
+		if(ok && d < columns) f[s] = load16(row + d);
+	}
+}
+
+// 16 results side by side, from column d on, those below D
+template <typename T>
+__device__ __forceinline__ void store_columns(T* row, int d, int D, const float (&v)[16]) {
+	constexpr int E = kind<T>::E;
+	if(D % E == 0) {
+#pragma unroll
+		for(int i = 0; i < 16 / E; i++)
+			if(d + E * i < D) store16(row + d + E * i, kind<T>::pack(v + E * i));
+	} else {
+		store_row16(row, d, D, v);
+	}
+}
+
+// A reader whose places are worked out again where it is used.  (The exclusive ors of them, 30 to 50 registers, otherwise wait in front of the loop, and operands go to memory instead.)
+template <typename R>
+__device__ __forceinline__ R fresh(R at) {
+	asm volatile("" : "+v"(at.row), "+v"(at.col));
+	return at;
+}
 // the registers of a block whose key (16 half + r from the block's first one on) lies behind the lane's last key become `gone`; `left`: last key - block's first key - 16 half
 __device__ __forceinline__ void drop_later(float (&x)[16], int left, float gone) {
 #pragma unroll
@@ -31,6 +112,37 @@ __device__ __forceinline__ void drop_later(float (&x)[16], int left, float gone)
 
 __device__ __forceinline__ int clamped(int64_t x) { return x > 64 ? 64 : x < -64 ? -64 : (int)x; }
 
+}  // namespace diff
+
+namespace diff {
+int width(const af3_diff_attention_params& p);   // columns of a map's queries and keys that a kernel has, half of those of its values
+
+// Up to four tensors [n0, n1, n2, columns] laid out anew where the kernels do not take them as they are: contiguous, rows of whole pieces with zeros at their ends.
+struct packing {
+	struct job {
+		const void* from;
+		void*       to;
+		int64_t     stride[3], n[3], pieces;
+		int32_t     columns;
+	} jobs[4];
+	int32_t count = 0, element;   // bytes of one
+	int64_t bytes = 0;            // of all their places
+	explicit packing(int element_) : element(element_) {}
+	// `t` and `stride`, where it is not taken as it is, become those of its place in `space` (null: only its size counts); the columns that the kernels see
+	int32_t add(const void*& t, int64_t (&stride)[3], int64_t n0, int64_t n1, int64_t n2, int64_t columns, void* space) {
+		if(takes(columns, n2 > 1 ? stride[2] : 0, element)) return (int32_t)columns;
+		const int64_t whole = (columns * element + 15) / 16 * 16 / element;
+		job& j = jobs[count++];
+		j = job{t, static_cast<unsigned char*>(space) + bytes, {stride[0], stride[1], stride[2]}, {n0, n1, n2}, n0 * n1 * n2 * whole * element / 16, (int32_t)columns};
+		bytes += n0 * n1 * n2 * whole * element;
+		t = j.to, stride[0] = n1 * n2 * whole, stride[1] = n2 * whole, stride[2] = whole;
+		return (int32_t)whole;
+	}
+	int launch(hipStream_t s) const;   // (diff_attention.hip)
+};
+// q, k and v as the kernels take them, in `space` (null: only the sizes count), and the columns of their rows
+packing pack_inputs(af3_diff_attention_params& p, int32_t& columns, int32_t& v_columns, void* space);
+int64_t packed_bytes(af3_diff_attention_params p);
 }  // namespace diff
 
 bool diff_gradients_fit(const af3_diff_attention_params& p);
