@@ -35,6 +35,19 @@ __device__ __forceinline__ void store_residual(const af3_diff_attention_params& 
 	}
 }
 
+// one column of a result, and of the second map's own
+template <typename T>
+__device__ __forceinline__ void store_result(const af3_diff_attention_params& p, int64_t b, int64_t h, int64_t qi, int64_t row, int column, float v, float second) {
+	static_cast<T*>(p.out)[b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2] + column] = kind<T>::bits(v);
+	if(p.second) static_cast<T*>(p.second)[row * p.Dv + column] = kind<T>::bits(second);
+	if constexpr(sizeof(T) == 2)
+		if(p.residuals) {
+			T* const lost = static_cast<T*>(p.residuals) + row * p.Dv + column;
+			lost[0] = kind<T>::bits(v - (float)(__bf16)v);
+			lost[p.B * p.H * p.Lq * p.Dv] = kind<T>::bits(second - (float)(__bf16)second);
+		}
+}
+
 // ---- rows of whole pieces ----
 __global__ void __launch_bounds__(THREADS) diff_pack_kernel(packing k) {
 	int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
@@ -420,76 +433,279 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 	}
 }
 
-// The parts of the key axis joined: one wavefront per query row, columns over its lanes.  The parts' maxima and sums come one to a lane (64 parts at most), so that the
-// parts' results, four of them in flight, wait for nothing but each other.
-constexpr int MAX_PARTS = 64;
-template <typename T, int COLUMNS>   // columns of a lane
-__global__ void __launch_bounds__(THREADS) diff_join_kernel(forward_args a) {
+// ---- few query rows ----
+// Up to 16 rows to a pair of key heads, single tokens above all, are bound by the bytes of K and V and by what a launch costs before them.  The 32 rows of a product are then both maps of
+// 16 rows: lanes 0 .. 15 of each half have the first map's, the others the second's; both products of K are taken for all and each lane keeps its own map's logits, so that softmax
+// and the product with V are there once.  K comes straight from memory as the products' operand, V by way of LDS of the wavefront's own, 32 keys at a time: wavefronts wait for nobody
+// until the end, and 16 KB (D = 64) of each are on their way while it works.  P in two terms.  One token of 32 requests over 1491 keys (16 heads on 4, D = 64): 34.5 us with the kernel
+// above, whose 8 wavefronts share tiles, 25.7.
+template <typename T, int DP>
+struct token_shape {
+	static constexpr int DV = 2 * DP, TILE = 32 * tile<T, DV>::STRIDE, LINE = 36, TABLE = 32 * LINE * 4;   // a tile of V, 32 columns of results: of a wavefront
+	static constexpr int LDS = WAVES * (TILE > TABLE ? TILE : TABLE);
+};
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS, (DP * sizeof(T) <= 128 ? 2 : 1)) diff_token_kernel(forward_args a) {
+	using S  = token_shape<T, DP>;
+	using TK = tile<T, DP>;
+	using TV = tile<T, S::DV>;
+	constexpr int E = kind<T>::E, N = TV::CHUNKS * 32 / 64;   // N: pieces of V per lane
 	const af3_diff_attention_params& p = a.p;
-	const int64_t G = p.H / p.Hkv, rows = G * p.Lq, n_rows = p.B * p.Hkv * rows;
-	const int     lane = threadIdx.x & 63, Dv = (int)p.Dv, splits = (int)a.splits;
-	const int64_t at = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
-	if(at >= n_rows) return;
-	const int64_t   bh = at / rows, hk = bh % p.Hkv, b = bh / p.Hkv;
-	const row_place place(at - bh * rows, rows, G, hk);
-	const int64_t   row = (b * p.H + place.h) * p.Lq + place.qi;
-	float o[2][COLUMNS];
-	bool  none = false;   // no live key
+	extern __shared__ __align__(16) unsigned char smem[];
+	__shared__ float stat[WAVES][32][2];
+
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, map = (lane >> 4) & 1;
+	const share    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.splits);
+	const uint32_t split = own.piece;
+	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
+	const int64_t  G = p.H / p.Hkv, rows = G * p.Lq;
+	const int      Dv = (int)p.Dv;
+
+	const row_place at_row(lane & 15, rows, G, hk);
+	u32x4 qf[TK::STEPS];
+	load_rows<T, DP>(qf, static_cast<const T*>(p.q) + b * p.q_stride[0] + (2 * at_row.h + map) * p.q_stride[1] + at_row.qi * p.q_stride[2], at_row.ok, a.columns, lane);
+	const T* const kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + 2 * hk * p.k_stride[1];
+	const T* const vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
+	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b : nullptr;
+	const float to_log2 = a.factor;
+	float  m = LOWEST, reference = -INFINITY, l = 0.f;
+	bool   moves = true;
+	f32x16 o[TV::BLOCKS];
+#pragma unroll
+	for(int db = 0; db < TV::BLOCKS; db++) o[db] = f32x16{};
+
+	int64_t last = (int64_t)(split + 1) * a.part < p.Lk ? (int64_t)(split + 1) * a.part : p.Lk;
+	if(p.causal) last = p.Lq + p.q_offset < last ? p.Lq + p.q_offset : last;   // (behind the last query's last key nothing counts)
+	const int64_t limit = p.causal ? at_row.qi + p.q_offset : (int64_t)1 << 41;   // the lane's last key
+	const typename TV::reader at_v(lane);
+	unsigned char* const vs = smem + wave * S::TILE;
+	const int my_row = tile_row(lane & 31);
+
+	// 32 keys from key0 on: which count at all, and their loads
+	auto keys_of = [&](int64_t key0) -> uint32_t {
+		const int64_t key = key0 + (lane & 31);
+		return (uint32_t)__ballot(key < last && (!mask || mask[key] != 0));
+	};
+	auto next = [&](int64_t& key0, uint32_t& keep) {   // the first 32 from key0 on that have one that counts (the wavefronts' in turn)
+		for(keep = 0u; key0 < last && (keep = keys_of(key0)) == 0u; key0 += 32 * WAVES) {}
+	};
+	u32x4 kf[2][TK::STEPS], vp[N];
+	auto fetch_k = [&](int64_t key0) {
+		const int64_t key = key0 + my_row < last ? key0 + my_row : last - 1;
+		const T* const row = kb + key * p.k_stride[2];
+#pragma unroll
+		for(int i = 0; i < 2; i++)
+#pragma unroll
+			for(int s = 0; s < TK::STEPS; s++) {
+				const int d = 2 * E * s + E * half;
+				kf[i][s] = u32x4{0u, 0u, 0u, 0u};
+				if(d < a.columns) kf[i][s] = load16(row + i * p.k_stride[1] + d);
+			}
+	};
+	auto fetch_v = [&](int64_t key0) {
+#pragma unroll
+		for(int n = 0; n < N; n++) {
+			const int     piece = lane + 64 * n, row = piece / TV::CHUNKS, col = piece % TV::CHUNKS;
+			const int64_t key = key0 + row < last ? key0 + row : last - 1;
+			vp[n] = u32x4{0u, 0u, 0u, 0u};
+			if(col * E < a.v_columns) vp[n] = load16(vb + key * p.v_stride[2] + col * E);
+		}
+	};
+	int64_t  key0 = (int64_t)split * a.part + 32 * wave;
+	uint32_t keep;
+	next(key0, keep);
+	if(keep != 0u) fetch_k(key0), fetch_v(key0);
+	while(keep != 0u) {
+		int64_t  following = key0 + 32 * WAVES;
+		uint32_t keep_following;
+		next(following, keep_following);
+		f32x16 s1{}, s2{};
+#pragma unroll
+		for(int s = 0; s < TK::STEPS; s++) s1 = kind<T>::mma(kf[0][s], qf[s], s1), s2 = kind<T>::mma(kf[1][s], qf[s], s2);
+		float x[16];
+#pragma unroll
+		for(int r = 0; r < 16; r++) x[r] = map == 0 ? s1[r] : s2[r];
+		if(keep_following != 0u) fetch_k(following);
+		if(keep != ~0u) drop_keys(x, keep, -INFINITY);
+		if(p.causal) drop_later(x, clamped(limit - key0 - 16 * half), -INFINITY);
+		// (a block's own maximum each time: the exponentials are few)
+		float top = x[0];
+#pragma unroll
+		for(int r = 1; r < 16; r++) top = maximum(top, x[r]);
+		top = maximum_of_halves(top);
+		if(moves || __any(!((top - m) * to_log2 < 14.f))) {
+			const float to = maximum(m, top), by = __builtin_amdgcn_exp2f((m - to) * to_log2);
+			m = to, reference = m * to_log2, l *= by;
+#pragma unroll
+			for(int db = 0; db < TV::BLOCKS; db++) o[db] *= by;
+			moves = __any(is_far(reference));
+		}
+		float sum = 0.f;
+#pragma unroll
+		for(int r = 0; r < 16; r++) {
+			x[r] = __builtin_amdgcn_exp2f(moves ? (x[r] - m) * to_log2 : __builtin_fmaf(x[r], to_log2, -reference));
+			sum += x[r];
+		}
+		l += sum;
+		// V: what is there by now into LDS (rows that do not count as zeros: theirs are weights of zero, which NaN does not heed), the next one's loads behind it
+#pragma unroll
+		for(int n = 0; n < N; n++) {
+			const int  piece = lane + 64 * n, row = piece / TV::CHUNKS, col = piece % TV::CHUNKS;
+			const bool in = ((keep >> row) & 1u) != 0u;
+			u32x4      v = vp[n];
+#pragma unroll
+			for(int i = 0; i < 4; i++) {
+				const uint32_t w = v[i];
+				v[i] = in ? w : 0u;
+			}
+			*reinterpret_cast<u32x4*>(vs + row * TV::STRIDE + TV::place(row, col)) = v;
+		}
+		if(keep_following != 0u) fetch_v(following);
+		__builtin_amdgcn_wave_barrier();   // (the wavefront's own LDS: in order)
+#pragma unroll
+		for(int j = 0; j < TV::JOINTS; j++) {
+			const u32x4 pf = kind<T>::pack(x + E * j);
+			u32x4       lo;
+			if constexpr(sizeof(T) == 2) {   // (what pf lost)
+				float y[E];
+#pragma unroll
+				for(int e = 0; e < E; e++) y[e] = x[E * j + e] - kind<T>::at(pf, e);
+				lo = kind<T>::pack(y);
+			}
+#pragma unroll
+			for(int db = 0; db < TV::BLOCKS; db++) {
+				const u32x4 vf = TV::col_frag(vs, 0, db, j, at_v);
+				o[db] = kind<T>::mma(vf, pf, o[db]);
+				if constexpr(sizeof(T) == 2) o[db] = kind<T>::mma(vf, lo, o[db]);
+			}
+		}
+		__builtin_amdgcn_wave_barrier();
+		key0 = following, keep = keep_following;
+	}
+	l = sum_of_halves(l);
+	if(half == 0) stat[wave][lane][0] = m, stat[wave][lane][1] = l;
+	__syncthreads();   // (and nobody reads a tile any more)
+	float to = LOWEST;
+#pragma unroll
+	for(int w = 0; w < WAVES; w++) to = maximum(to, stat[w][lane & 31][0]);
+	const float by = __builtin_amdgcn_exp2f((m - to) * to_log2);
+	// Columns 32 at a time through LDS; a thread then has two of them of one of the 16 rows, in both maps.
+	const int       row = threadIdx.x >> 4, column = 2 * (threadIdx.x & 15);
+	const row_place place(row, rows, G, hk);
+	float top[2], total[2], inv[2];
 #pragma unroll
 	for(int i = 0; i < 2; i++) {
-		float m = 0.f, l = 0.f;
-		if(lane < splits) m = a.part_stat[2 * ((2 * lane + i) * n_rows + at)], l = a.part_stat[2 * ((2 * lane + i) * n_rows + at) + 1];
-		float top = l == 0.f ? LOWEST : m;
+		top[i] = LOWEST, total[i] = 0.f;
 #pragma unroll
-		for(int d = 32; d; d >>= 1) top = maximum(top, __shfl_xor(top, d));
-		const float weight = l == 0.f ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.factor);
-		float sum = l * weight;
+		for(int w = 0; w < WAVES; w++) top[i] = maximum(top[i], stat[w][16 * i + row][0]);
 #pragma unroll
-		for(int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+		for(int w = 0; w < WAVES; w++) total[i] += stat[w][16 * i + row][1] * __builtin_amdgcn_exp2f((stat[w][16 * i + row][0] - top[i]) * to_log2);
+		inv[i] = total[i] == 0.f ? 0.f : 1.f / total[i];
+	}
+	const int64_t n_rows = p.B * p.Hkv * rows, part_row = (b * p.Hkv + hk) * rows + row, out_row = (b * p.H + place.h) * p.Lq + place.qi;
+	const float   lam = lam_of(p, place.h);
+	if(place.ok && column == 0) {
 #pragma unroll
-		for(int k = 0; k < COLUMNS; k++) o[i][k] = 0.f;
-		for(int s0 = 0; s0 < splits; s0 += 4) {
-			float x[4][COLUMNS];
-#pragma unroll
-			for(int s = 0; s < 4; s++) {
-				const bool there = s0 + s < splits && __shfl(l, (s0 + s) & 63) != 0.f;
-#pragma unroll
-				for(int k = 0; k < COLUMNS; k++) {
-					x[s][k] = 0.f;
-					if(there && lane + 64 * k < Dv) x[s][k] = a.part_out[((2 * (s0 + s) + i) * n_rows + at) * Dv + lane + 64 * k];
-				}
+		for(int i = 0; i < 2; i++) {
+			if(a.splits > 1) {
+				float* const st = a.part_stat + 2 * ((2 * (int64_t)split + i) * n_rows + part_row);
+				st[0] = top[i], st[1] = total[i];
+			} else if(p.stats) {
+				float* const st = p.stats + 2 * ((b * 2 * p.H + 2 * place.h + i) * p.Lq + place.qi);
+				st[0] = top[i], st[1] = inv[i];
 			}
-#pragma unroll
-			for(int s = 0; s < 4; s++) {
-				const float w = __shfl(weight, (s0 + s) & 63);
-#pragma unroll
-				for(int k = 0; k < COLUMNS; k++) o[i][k] = s0 + s < splits ? __builtin_fmaf(x[s][k], w, o[i][k]) : o[i][k];
-			}
-		}
-		const float inv = sum == 0.f ? 0.f : 1.f / sum;
-		none = sum == 0.f;
-#pragma unroll
-		for(int k = 0; k < COLUMNS; k++) o[i][k] *= inv;
-		if(p.stats && lane == 0) {
-			float* const st = p.stats + 2 * ((b * 2 * p.H + 2 * place.h + i) * p.Lq + place.qi);
-			st[0] = top, st[1] = inv;
 		}
 	}
-	const float lam = lam_of(p, place.h);
-	T* const    out = static_cast<T*>(p.out) + b * p.out_stride[0] + place.h * p.out_stride[1] + place.qi * p.out_stride[2];
+	float* const mine = reinterpret_cast<float*>(smem) + wave * (S::TABLE / 4) + (lane & 31) * S::LINE + 16 * half;
+	const float* const all = reinterpret_cast<const float*>(smem) + row * S::LINE + column;
 #pragma unroll
-	for(int k = 0; k < COLUMNS; k++)
-		if(lane + 64 * k < Dv) {
-			const float v = none ? 0.f : __builtin_fmaf(-lam, o[1][k], o[0][k]);
-			out[lane + 64 * k] = kind<T>::bits(v);
-			if(p.second) static_cast<T*>(p.second)[row * Dv + lane + 64 * k] = kind<T>::bits(o[1][k]);
-			if constexpr(sizeof(T) == 2)
-				if(p.residuals) {
-					T* const lost = static_cast<T*>(p.residuals) + row * Dv + lane + 64 * k;
-					lost[0] = kind<T>::bits(v - kind<T>::value(kind<T>::bits(v)));
-					lost[p.B * p.H * p.Lq * Dv] = kind<T>::bits(o[1][k] - kind<T>::value(kind<T>::bits(o[1][k])));
-				}
+	for(int db = 0; db < TV::BLOCKS; db++) {
+		if(32 * db >= Dv) break;
+		__syncthreads();
+#pragma unroll
+		for(int e = 0; e < 4; e++) *reinterpret_cast<f32x4*>(mine + 4 * e) = f32x4{o[db][4 * e] * by, o[db][4 * e + 1] * by, o[db][4 * e + 2] * by, o[db][4 * e + 3] * by};
+		__syncthreads();
+		if(!place.ok) continue;
+#pragma unroll
+		for(int c = 0; c < 2; c++) {
+			const int at = 32 * db + column + c;
+			if(at >= Dv) continue;
+			float r[2] = {0.f, 0.f};
+#pragma unroll
+			for(int i = 0; i < 2; i++)
+#pragma unroll
+				for(int w = 0; w < WAVES; w++) r[i] += all[w * (S::TABLE / 4) + 16 * i * S::LINE + c];
+			if(a.splits > 1) {
+#pragma unroll
+				for(int i = 0; i < 2; i++) a.part_out[((2 * (int64_t)split + i) * n_rows + part_row) * Dv + at] = r[i];
+			} else {
+				store_result<T>(p, b, place.h, place.qi, out_row, at, total[0] == 0.f ? 0.f : __builtin_fmaf(-lam, r[1] * inv[1], r[0] * inv[0]), r[1] * inv[1]);
+			}
 		}
+	}
+}
+
+// The parts of the key axis joined: a workgroup per query row; two wavefronts to a map, half of the parts each, four columns to a lane.  The parts' maxima and sums come one to a
+// lane (64 parts at most), so that the parts' results, eight of them in flight, wait for nothing but each other.
+constexpr int MAX_PARTS = 64;
+template <typename T>
+__global__ void __launch_bounds__(THREADS) diff_join_kernel(forward_args a) {
+	const af3_diff_attention_params& p = a.p;
+	__shared__ f32x4 joint[2][64];
+	__shared__ f32x4 halves[2][64];
+	const int64_t G = p.H / p.Hkv, rows = G * p.Lq, n_rows = p.B * p.Hkv * rows, at = blockIdx.x;
+	const int     lane = threadIdx.x & 63, wave = threadIdx.x >> 6, map = wave & 1, Dv = (int)p.Dv, splits = (int)a.splits;
+	const int64_t   bh = at / rows, hk = bh % p.Hkv, b = bh / p.Hkv;
+	const row_place place(at - bh * rows, rows, G, hk);
+	float m = 0.f, l = 0.f;
+	if(lane < splits) m = a.part_stat[2 * ((2 * lane + map) * n_rows + at)], l = a.part_stat[2 * ((2 * lane + map) * n_rows + at) + 1];
+	float top = l == 0.f ? LOWEST : m;
+#pragma unroll
+	for(int d = 32; d; d >>= 1) top = maximum(top, __shfl_xor(top, d));
+	const float weight = l == 0.f ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.factor);
+	float sum = l * weight;
+#pragma unroll
+	for(int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+	const float inv = sum == 0.f ? 0.f : 1.f / sum;
+	const int   c = 4 * lane, per = (splits + 1) / 2, first = (wave >> 1) * per, end = first + per < splits ? first + per : splits;
+	f32x4       o = {0.f, 0.f, 0.f, 0.f};
+	for(int s0 = first; s0 < end; s0 += 8) {
+		f32x4 x[8];
+#pragma unroll
+		for(int s = 0; s < 8; s++) {
+			x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+			if(s0 + s < end && __shfl(l, (s0 + s) & 63) != 0.f) {   // (a part without a live key wrote nothing)
+				const float* const from = a.part_out + ((2 * (s0 + s) + map) * n_rows + at) * Dv + c;
+				if(c + 4 <= Dv) x[s] = *reinterpret_cast<const f32x4_any*>(from);
+				else
+					for(int e = 0; e < 4; e++)
+						if(c + e < Dv) x[s][e] = from[e];
+			}
+		}
+#pragma unroll
+		for(int s = 0; s < 8; s++) {
+			const float w = s0 + s < end ? __shfl(weight, (s0 + s) & 63) : 0.f;
+#pragma unroll
+			for(int e = 0; e < 4; e++) o[e] = __builtin_fmaf(x[s][e], w, o[e]);
+		}
+	}
+	if(wave >> 1) halves[map][lane] = o;
+	__syncthreads();
+	if(wave >> 1) return;
+	o += halves[map][lane];
+#pragma unroll
+	for(int e = 0; e < 4; e++) o[e] *= inv;
+	if(p.stats && lane == 0) {
+		float* const st = p.stats + 2 * ((b * 2 * p.H + 2 * place.h + map) * p.Lq + place.qi);
+		st[0] = top, st[1] = inv;
+	}
+	joint[map][lane] = o;
+	__syncthreads();
+	if(map) return;
+	const float lam = lam_of(p, place.h);
+	const f32x4 second = joint[1][lane];
+	for(int e = 0; e < 4; e++)
+		if(c + e < Dv) store_result<T>(p, b, place.h, place.qi, (b * p.H + place.h) * p.Lq + place.qi, c + e, sum == 0.f ? 0.f : __builtin_fmaf(-lam, second[e], o[e]), second[e]);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
@@ -508,14 +724,24 @@ struct plan {
 	int      kw;
 	uint32_t row_tiles, splits;
 	int64_t  part;
-	bool     half;   // V as fp16
+	bool     half;    // V as fp16
+	bool     token;   // diff_token_kernel
 };
+constexpr int TOKEN_ROWS = 16;
 plan forward_plan(const af3_diff_attention_params& p) {
 	plan          f;
 	const int64_t rows = p.H / p.Hkv * p.Lq, groups = p.B * p.Hkv;
 	const bool    fp32 = p.dtype == AF3_F32;
 	const int     wide = width(p);
 	const int64_t slots = wide * (fp32 ? 4 : 2) <= 64 ? 512 : 256;
+	f.token = rows <= TOKEN_ROWS, f.half = false;
+	if(f.token) {
+		// (128 keys to a step of the workgroup; two workgroups to a compute unit)
+		const int64_t steps = (p.Lk + 127) / 128, splits = parts_for(groups, 512, steps, (0.8 + 0.008 * wide) * (fp32 ? 2.0 : 1.0), 8.0 * p.B * p.H * p.Lq * p.Dv, MAX_PARTS);
+		const int64_t each = (steps + splits - 1) / splits;
+		f.kw = 4, f.row_tiles = 1, f.part = 128 * each, f.splits = (uint32_t)((steps + each - 1) / each);
+		return f;
+	}
 	auto          busy = [&](int kw) { return (rows + 128 / kw - 1) / (128 / kw) * groups; };
 	f.kw = rows <= 32 || busy(4) <= slots ? 4 : rows <= 64 || busy(2) <= slots ? 2 : 1;
 	if(f.kw > most_sharing(p)) f.kw = most_sharing(p);
@@ -554,9 +780,26 @@ int launch_forward_form(const forward_args& a, int kw, uint32_t grid, hipStream_
 		}
 	return kw == 2 ? launch_forward<T, DP, 2>(a, grid, s) : launch_forward<T, DP, 1>(a, grid, s);
 }
+template <typename T, int DP>
+int launch_token(const forward_args& a, uint32_t grid, hipStream_t s) {
+	using S = token_shape<T, DP>;
+	auto kernel = &diff_token_kernel<T, DP>;
+	if(S::LDS > 65536 - 8192 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess) {
+		(void)hipGetLastError();
+		return AF3_ERR_LAUNCH;
+	}
+	hipLaunchKernelGGL(kernel, dim3(grid), dim3(THREADS), S::LDS, s, a);
+	return launch_status();
+}
 template <typename T>
-int launch_forward_type(const forward_args& a, int kw, uint32_t grid, hipStream_t s) {
-	const int wide = width(a.p);
+int launch_forward_type(const forward_args& a, const plan& f, uint32_t grid, hipStream_t s) {
+	const int wide = width(a.p), kw = f.kw;
+	if(f.token) {
+		if(wide == 32) return launch_token<T, 32>(a, grid, s);
+		if constexpr(sizeof(T) == 2)
+			if(wide == 128) return launch_token<T, 128>(a, grid, s);
+		return launch_token<T, 64>(a, grid, s);
+	}
 	if(wide == 32) return launch_forward_form<T, 32>(a, kw, grid, s);
 	if constexpr(sizeof(T) == 2)
 		if(wide == 128) return launch_forward_form<T, 128>(a, kw, grid, s);
@@ -632,14 +875,9 @@ extern "C" int af3_diff_attention_forward(const af3_diff_attention_params* param
 	const uint32_t grid = (uint32_t)(params->B * params->Hkv) * f.row_tiles * f.splits;
 	int rc = pack.launch(s);
 	if(rc != AF3_OK) return rc;
-	rc = fp32 ? diff::launch_forward_type<float>(a, f.kw, grid, s) : diff::launch_forward_type<uint16_t>(a, f.kw, grid, s);
+	rc = fp32 ? diff::launch_forward_type<float>(a, f, grid, s) : diff::launch_forward_type<uint16_t>(a, f, grid, s);
 	if(rc != AF3_OK || f.splits == 1) return rc;
-	const dim3 joins((uint32_t)((n_rows + cross::WAVES - 1) / cross::WAVES)), threads(cross::THREADS);
-	if(params->Dv <= 128) {
-		if(fp32) hipLaunchKernelGGL((diff::diff_join_kernel<float, 2>), joins, threads, 0, s, a);
-		else hipLaunchKernelGGL((diff::diff_join_kernel<uint16_t, 2>), joins, threads, 0, s, a);
-	} else {
-		hipLaunchKernelGGL((diff::diff_join_kernel<uint16_t, 4>), joins, threads, 0, s, a);
-	}
+	if(fp32) hipLaunchKernelGGL(diff::diff_join_kernel<float>, dim3((uint32_t)n_rows), dim3(cross::THREADS), 0, s, a);
+	else hipLaunchKernelGGL(diff::diff_join_kernel<uint16_t>, dim3((uint32_t)n_rows), dim3(cross::THREADS), 0, s, a);
 	return launch_status();
 }

@@ -328,9 +328,11 @@ struct dkv_shape {
 	static constexpr int DV = 2 * DP, QT = tile_rows(BYTES, RW), SUB = QT / (32 * RW), KEYS = 32 * GROUPS;
 	static constexpr int QTILE = QT * tile<T, DP>::STRIDE, GTILE = QT * tile<T, DV>::STRIDE, STATS = row_stats<T, QT>::BYTES, SET = 2 * QTILE + GTILE + STATS;
 	static constexpr int BUFFERS = 2 * SET <= 73728 ? 2 : 1;
-	static constexpr int VW = RW * (MAPS == 2 ? 1 : 2);   // wavefronts that have a part of the same rows of dV
-	static constexpr int JOIN = VW > 1 ? W * 32 * (DV + 4) * 4 : 0, PER_SIMD = BYTES <= 64 ? 2 : 1;   // wavefronts to a SIMD, by the registers of sums and operands
-	static constexpr int LDS = BUFFERS * SET > JOIN ? BUFFERS * SET : JOIN;
+	// One map to a wavefront: the two of a pair exchange their probabilities, so that their difference is rounded once, and have half of dV's columns each.
+	static constexpr int VBLOCKS = DV / 32 * MAPS / 2, EXCHANGE = MAPS == 1 ? W * 64 * 64 : 0;
+	static_assert(MAPS == 2 || (RW == 1 && SUB == 1));
+	static constexpr int JOIN = RW > 1 ? W * 32 * (DV + 4) * 4 : 0, PER_SIMD = BYTES <= 64 ? 2 : 1;   // wavefronts to a SIMD, by the registers of sums and operands
+	static constexpr int LDS = BUFFERS * SET + EXCHANGE > JOIN ? BUFFERS * SET + EXCHANGE : JOIN;
 };
 
 template <typename T, int DP, int RW>
@@ -358,13 +360,14 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 	load_rows<T, S::DV>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], in, a.v_columns, lane);
 	const bool work = __any(lives);   // (of this wavefront)
 
-	f32x16 dk[MAPS][TK::BLOCKS], dv[TV::BLOCKS];
+	f32x16 dk[MAPS][TK::BLOCKS], dv[S::VBLOCKS];
+	const int vblock0 = MAPS == 2 ? 0 : map0 * S::VBLOCKS;   // the wavefront's first block of dV's columns
 #pragma unroll
 	for(int i = 0; i < MAPS; i++)
 #pragma unroll
 		for(int db = 0; db < TK::BLOCKS; db++) dk[i][db] = f32x16{};
 #pragma unroll
-	for(int db = 0; db < TV::BLOCKS; db++) dv[db] = f32x16{};
+	for(int db = 0; db < S::VBLOCKS; db++) dv[db] = f32x16{};
 
 	// Tiles of query rows, head after head: tile `at` of head `head` of the group, counted head * q_tiles + at (below 2^25).
 	const int q_tiles = (int)((p.Lq + QT - 1) / QT), n = (int)G * q_tiles, Lq = (int)p.Lq;
@@ -409,6 +412,17 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 		more = head * q_tiles + at < last;
 		if(more) fetch(head, at);
 		const bool apart = rs.apart(st);
+		float both[16];
+		bool  met = false;   // (one map to a wavefront: there is something to exchange)
+		auto  add_values = [&](int row0) {
+			const typename TV::reader at_g = S::PER_SIMD == 2 ? fresh(at_g_) : at_g_;
+#pragma unroll
+			for(int j = 0; j < TV::JOINTS; j++) {
+				const u32x4 pf = kind<T>::pack(both + E * j);
+#pragma unroll
+				for(int db = 0; db < S::VBLOCKS; db++) dv[db] = kind<T>::mma(TV::col_frag(gs, row0, vblock0 + db, j, at_g), pf, dv[db]);
+			}
+		};
 		if(work) {
 #pragma unroll 1
 			for(int s = 0; s < S::SUB; s++) {
@@ -424,7 +438,7 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 				f32x16 dp{};
 #pragma unroll
 				for(int i = 0; i < TV::STEPS; i++) dp = kind<T>::mma(TV::row_frag(gs, row0, i, at_g), vf[i], dp);
-				float both[16];   // P1 - lam P2 (or the wavefront's part of it)
+				// P1 - lam P2 (or the wavefront's part of it)
 #pragma unroll
 				for(int i = 0; i < MAPS; i++) {
 					const int                  map = map0 + i;
@@ -462,12 +476,25 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 						for(int db = 0; db < TK::BLOCKS; db++) dk[i][db] = kind<T>::mma(TK::col_frag(qm, row0, db, j, at_q), df, dk[i][db]);
 					}
 				}
+				if constexpr(MAPS == 2) add_values(row0);
+				met = true;
+			}
+		}
+		if constexpr(MAPS == 1) {
+			f32x4* const exchange = reinterpret_cast<f32x4*>(smem + S::BUFFERS * S::SET) + lane;
+			if(met) {
 #pragma unroll
-				for(int j = 0; j < TV::JOINTS; j++) {
-					const u32x4 pf = kind<T>::pack(both + E * j);
+				for(int i = 0; i < 4; i++) exchange[64 * (4 * wave + i)] = f32x4{both[4 * i], both[4 * i + 1], both[4 * i + 2], both[4 * i + 3]};
+			}
+			__syncthreads();
+			if(met) {   // (and so it is for the other one, which has the same keys)
 #pragma unroll
-					for(int db = 0; db < TV::BLOCKS; db++) dv[db] = kind<T>::mma(TV::col_frag(gs, row0, db, j, at_g), pf, dv[db]);
+				for(int i = 0; i < 4; i++) {
+					const f32x4 other = exchange[64 * (4 * (wave ^ 1) + i)];
+#pragma unroll
+					for(int e = 0; e < 4; e++) both[4 * i + e] += other[e];
 				}
+				add_values(0);
 			}
 		}
 		if constexpr(S::BUFFERS == 2) buffer ^= 1;
@@ -477,8 +504,7 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 #pragma unroll
 		for(int i = 0; i < MAPS; i++) add_up<DP, RW>(tables + (MAPS == 2 ? group : 2 * group + map0) * RW * 32 * (DP + 4), rwave, lane, dk[i]);
 	}
-	const int vwave = MAPS == 2 ? rwave : 2 * rwave + map0;
-	if constexpr(S::VW > 1) add_up<S::DV, S::VW>(tables + group * S::VW * 32 * (S::DV + 4), vwave, lane, dv);
+	if constexpr(RW > 1) add_up<S::DV, RW>(tables + group * RW * 32 * (S::DV + 4), rwave, lane, dv);
 	if(!in) return;
 	const int     D = (int)p.D, Dv = (int)p.Dv;
 	const int64_t n_keys = p.B * p.Hkv * p.Lk, place = (b * p.Hkv + hk) * p.Lk + key;
@@ -497,13 +523,14 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 		}
 	}
 #pragma unroll
-	for(int db = 0; db < TV::BLOCKS; db++) {
-		if(db % S::VW != vwave) continue;
+	for(int db = 0; db < S::VBLOCKS; db++) {
+		if(db % RW != rwave) continue;
 		float v[16];
 #pragma unroll
 		for(int r = 0; r < 16; r++) v[r] = lives ? dv[db][r] : 0.f;
-		if(a.splits > 1) store_columns(partial + 2 * n_keys * D + place * Dv, 32 * db + 16 * half, Dv, v);
-		else if(a.g.grad_v) store_columns(static_cast<T*>(a.g.grad_v) + place * Dv, 32 * db + 16 * half, Dv, v);
+		const int column = 32 * (vblock0 + db) + 16 * half;
+		if(a.splits > 1) store_columns(partial + 2 * n_keys * D + place * Dv, column, Dv, v);
+		else if(a.g.grad_v) store_columns(static_cast<T*>(a.g.grad_v) + place * Dv, column, Dv, v);
 	}
 }
 
@@ -598,7 +625,7 @@ cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double cou
 		const double  tile_us = load_us * tile_rows(bytes, sharing) / 64 + block_us * tile_rows(bytes, sharing) / (32 * sharing);
 		for(int64_t parts = 1; parts <= 64 && (parts == 1 || 2 * parts <= n + 1); parts++) {
 			const double longest = (double)over(n, parts), all = (double)workgroups * n * counts / slots;
-			const double us = (workgroups * parts <= slots ? longest : longest > all + 0.5 * longest ? longest : all + 0.5 * longest) * tile_us + (parts > 1 ? JOIN_US + parts * 2.0 * part_bytes / BYTES_PER_US : 0.0);
+			const double us = (workgroups * parts <= slots ? longest : longest > all + 0.8 * longest ? longest : all + 0.8 * longest) * tile_us + (parts > 1 ? JOIN_US + parts * 2.0 * part_bytes / BYTES_PER_US : 0.0);
 			if(best_us == 0.0 || us < best_us) best_us = us, best.sharing = sharing, best.tiles = (uint32_t)tiles, best.part = over(n, parts), best.splits = (uint32_t)over(n, best.part);
 		}
 	}
