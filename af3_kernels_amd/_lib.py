@@ -129,6 +129,7 @@ class DiffAttentionGrads(ctypes.Structure):
 
 
 ROTARY_MAX_HEAD_DIM = 1024                 # AF3_ROTARY_MAX_HEAD_DIM
+DIFF_ATTENTION_GRAD_ROW_BYTES = 16777216   # AF3_DIFF_ATTENTION_GRAD_ROW_BYTES
 RESIDUAL_NORM_MAX_CHANNELS = 16384         # AF3_RESIDUAL_NORM_MAX_CHANNELS
 NORMS = {"none": 0, "rms": 1, "layer": 2}  # af3_norm
 SHARE_NONE, SHARE_CHANNEL, SHARE_GROUP, SHARE_ROW = 0, 1, 2, 3   # af3_share

@@ -26,7 +26,7 @@ __device__ __forceinline__ float lam_of(const af3_diff_attention_params& p, int6
 // ---- rows on their way ----
 // The kernels take rows that are whole 16-byte pieces, no further apart than 32 bits reach over a tile; the host lays others out anew (diff_pack_kernel).  With the other way of reading
 // beside it in the same loop, as cross_tiles.hpp's passage has it, dK/dV held 756 branches and twice its scalars in vector registers' lanes, and took four times as long.
-inline bool takes(int64_t columns, int64_t stride, int bytes) { return columns * bytes % 16 == 0 && stride <= (int64_t)0x7fffffff / (128 * bytes); }
+inline bool takes(int64_t columns, int64_t stride, int bytes) { return columns * bytes % 16 == 0 && stride * bytes < AF3_DIFF_ATTENTION_GRAD_ROW_BYTES; }   // (tiles of 128 rows at most)
 // ROWS rows into a tile in LDS, spread over NT threads in 16-byte pieces: one load per piece, at a scalar base and an offset that stays the same from tile to tile
 template <typename T, int DP, int ROWS, int NT>
 struct carrier {

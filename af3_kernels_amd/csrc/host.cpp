@@ -1306,7 +1306,7 @@ struct diff_function : torch::autograd::Function<diff_function> {
 		torch::autograd::variable_list grads(8);
 		{
 			at::AutoGradMode none(false);
-			if(!inner_1(g)) g = g.contiguous();
+			if(!inner_1(g) || g.stride(2) * (int64_t)g.element_size() >= AF3_DIFF_ATTENTION_GRAD_ROW_BYTES) g = g.contiguous();
 			af3_diff_attention_params p = call.block();
 			p.out = saved[5].data_ptr(), p.stats = static_cast<float*>(saved[6].data_ptr()), p.second = saved[7].data_ptr();
 			if(saved[8].defined()) p.residuals = saved[8].data_ptr();

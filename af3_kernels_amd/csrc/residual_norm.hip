@@ -162,7 +162,7 @@ __device__ __forceinline__ void standardise(float (&v)[NP][E], const R& row, S& 
 		for(int e = 0; e < E; e++) v[n][e] *= root;
 }
 
-constexpr int threads_for(int tpr) { return tpr < 256 ? 256 : tpr; }
+constexpr int threads_for(int tpr) { return tpr == 64 ? 256 : tpr; }   // (wavefronts that have rows of their own need no barriers, others do)
 
 template <typename T, int TPR, int NP>
 __global__ void __launch_bounds__(threads_for(TPR)) forward_kernel(args a) {
@@ -305,55 +305,63 @@ __global__ void __launch_bounds__(threads_for(TPR)) backward_kernel(args a) {
 	};
 	if constexpr(SUMS) clear(GATE), clear(WEIGHT), clear(BIAS), clear(POST);
 
+	// What a row needs comes in one go, a row ahead of its use where the registers hold two of them; what rows share stays in registers.  4 x 2048 rows of 4096 channels in bf16:
+	// 107 us (5.1 TB/s); with 16 channels a thread, everything loaded where it is used, 210; 4 x 768 conditioned rows of 1024 channels 29 us, that way 54.
+	constexpr bool AHEAD = TPR * NP <= 1024;
+	struct streams {
+		eight<T> y[NP], x[NP], out[NP], normed[NP], gate[NP], weight[NP];
+		f32x4    stats;
+	} coming;
+	const bool through = p.norm != AF3_NORM_NONE && g.grad_normed;   // a gradient comes through the second norm
+	eight<T> post[NP];
+	if(p.post_weight) own.load(post, static_cast<const T*>(p.post_weight));
+	auto shared = [&](int64_t row) {
+		if(p.gate && p.gate_share != AF3_SHARE_ROW) own.load(coming.gate, static_cast<const T*>(p.gate) + share_row(p.gate_share, row, p.group) * C);
+		if(p.weight && p.weight_share != AF3_SHARE_ROW) own.load(coming.weight, static_cast<const T*>(p.weight) + share_row(p.weight_share, row, p.group) * C);
+	};
+	auto fetch = [&](int64_t row) {
+		own.load(coming.y, static_cast<const T*>(p.y) + row * p.y_stride);
+		if(through) {
+			if(p.x) own.load(coming.x, static_cast<const T*>(p.x) + row * p.x_stride);
+			own.load(coming.normed, static_cast<const T*>(g.grad_normed) + row * g.grad_normed_stride);
+			if(p.weight_share == AF3_SHARE_ROW) own.load(coming.weight, static_cast<const T*>(p.weight) + row * C);
+		}
+		if(g.grad_out) own.load(coming.out, static_cast<const T*>(g.grad_out) + row * g.grad_out_stride);
+		if(p.gate_share == AF3_SHARE_ROW) own.load(coming.gate, static_cast<const T*>(p.gate) + row * C);
+		coming.stats = *reinterpret_cast<const f32x4*>(p.stats + 4 * row);
+	};
 	for(int64_t begin = first; begin < last; begin += step) {
 		const int64_t end = begin + step < last ? begin + step : last;
+		if(begin + worker < end) {
+			shared(begin);
+			if(AHEAD) fetch(begin + worker);
+		}
 		for(int64_t row = begin + worker; row < end; row += AT_ONCE) {
-			const f32x4 stats = *reinterpret_cast<const f32x4*>(p.stats + 4 * row);
-			eight<T> m[NP];
-			float    z[NP][E], gate[NP][E], r[NP][E], d[NP][E];   // d: the gradient on its way back
+			if(!AHEAD) fetch(row);
+			const streams s = coming;
+			if(AHEAD && row + AT_ONCE < end) fetch(row + AT_ONCE);
+			const f32x4 stats = s.stats;
+			float       z[NP][E], gate[NP][E], r[NP][E], d[NP][E];   // d: the gradient on its way back
 			// the forward pass again: z = normed y, r = its sum, standardised
-			own.load(m, static_cast<const T*>(p.y) + row * p.y_stride);
 #pragma unroll
 			for(int n = 0; n < NP; n++)
 #pragma unroll
 				for(int e = 0; e < E; e++) {
-					z[n][e] = value(m[n].e[e]), gate[n][e] = 1.f, d[n][e] = 0.f;
+					z[n][e] = value(s.y[n].e[e]), d[n][e] = 0.f;
 					if(p.post_norm != AF3_NORM_NONE) z[n][e] = own.in(n, e) ? (z[n][e] - stats[0]) * stats[1] : 0.f;
+					gate[n][e] = !p.gate ? 1.f : p.gate_sigmoid ? sigmoidf_fast(value(s.gate[n].e[e])) : value(s.gate[n].e[e]);
 				}
-			float post[NP][E];
-			if(p.post_weight) own.load(m, static_cast<const T*>(p.post_weight));
-#pragma unroll
-			for(int n = 0; n < NP; n++)
-#pragma unroll
-				for(int e = 0; e < E; e++) post[n][e] = p.post_weight ? value(m[n].e[e]) : 1.f;
-			if(p.gate) {
-				own.load(m, static_cast<const T*>(p.gate) + share_row(p.gate_share, row, p.group) * C);
+			auto after = [&](int n, int e) { return p.post_weight ? z[n][e] * value(post[n].e[e]) : z[n][e]; };   // what the gate is multiplied with
+			if(through) {
 #pragma unroll
 				for(int n = 0; n < NP; n++)
 #pragma unroll
-					for(int e = 0; e < E; e++) gate[n][e] = p.gate_sigmoid ? sigmoidf_fast(value(m[n].e[e])) : value(m[n].e[e]);
-			}
-			if(p.norm != AF3_NORM_NONE && g.grad_normed) {
-#pragma unroll
-				for(int n = 0; n < NP; n++)
-#pragma unroll
-					for(int e = 0; e < E; e++) r[n][e] = gate[n][e] * (z[n][e] * post[n][e]);
-				if(p.x) {
-					own.load(m, static_cast<const T*>(p.x) + row * p.x_stride);
-#pragma unroll
-					for(int n = 0; n < NP; n++)
-#pragma unroll
-						for(int e = 0; e < E; e++) r[n][e] = __builtin_fmaf(p.residual_scale, value(m[n].e[e]), r[n][e]);
-				}
-#pragma unroll
-				for(int n = 0; n < NP; n++)
-#pragma unroll
-					for(int e = 0; e < E; e++) r[n][e] = own.in(n, e) ? (r[n][e] - stats[2]) * stats[3] : 0.f;
-				own.load(m, static_cast<const T*>(g.grad_normed) + row * g.grad_normed_stride);
-#pragma unroll
-				for(int n = 0; n < NP; n++)
-#pragma unroll
-					for(int e = 0; e < E; e++) d[n][e] = value(m[n].e[e]);
+					for(int e = 0; e < E; e++) {
+						r[n][e] = gate[n][e] * after(n, e);
+						if(p.x) r[n][e] = __builtin_fmaf(p.residual_scale, value(s.x[n].e[e]), r[n][e]);
+						r[n][e] = own.in(n, e) ? (r[n][e] - stats[2]) * stats[3] : 0.f;
+						d[n][e] = value(s.normed[n].e[e]);
+					}
 				if(g.grad_bias) {
 					if(p.bias_share == AF3_SHARE_ROW) own.store(static_cast<T*>(g.grad_bias) + row * C, d);
 					else if constexpr(SUMS) {
@@ -379,20 +387,18 @@ __global__ void __launch_bounds__(threads_for(TPR)) backward_kernel(args a) {
 					}
 				}
 				if(p.weight) {
-					own.load(m, static_cast<const T*>(p.weight) + share_row(p.weight_share, row, p.group) * C);
 #pragma unroll
 					for(int n = 0; n < NP; n++)
 #pragma unroll
-						for(int e = 0; e < E; e++) d[n][e] *= value(m[n].e[e]);
+						for(int e = 0; e < E; e++) d[n][e] *= value(s.weight[n].e[e]);
 				}
 				back(d, r, own, sums, p.norm, a.inv_c, stats[3]);
 			}
 			if(g.grad_out) {
-				own.load(m, static_cast<const T*>(g.grad_out) + row * g.grad_out_stride);
 #pragma unroll
 				for(int n = 0; n < NP; n++)
 #pragma unroll
-					for(int e = 0; e < E; e++) d[n][e] += value(m[n].e[e]);
+					for(int e = 0; e < E; e++) d[n][e] += value(s.out[n].e[e]);
 			}
 			if(g.grad_x) {
 				float dx[NP][E];
@@ -407,7 +413,7 @@ __global__ void __launch_bounds__(threads_for(TPR)) backward_kernel(args a) {
 #pragma unroll
 				for(int n = 0; n < NP; n++)
 #pragma unroll
-					for(int e = 0; e < E; e++) dg[n][e] = d[n][e] * (z[n][e] * post[n][e]) * (p.gate_sigmoid ? gate[n][e] * (1.f - gate[n][e]) : 1.f);
+					for(int e = 0; e < E; e++) dg[n][e] = d[n][e] * after(n, e) * (p.gate_sigmoid ? gate[n][e] * (1.f - gate[n][e]) : 1.f);
 				if(p.gate_share == AF3_SHARE_ROW) own.store(static_cast<T*>(g.grad_gate) + row * C, dg);
 				else if constexpr(SUMS) {
 #pragma unroll
@@ -429,10 +435,12 @@ __global__ void __launch_bounds__(threads_for(TPR)) backward_kernel(args a) {
 				}
 			if(g.grad_y) {
 				if(p.post_norm != AF3_NORM_NONE) {
+					if(p.post_weight) {
 #pragma unroll
-					for(int n = 0; n < NP; n++)
+						for(int n = 0; n < NP; n++)
 #pragma unroll
-						for(int e = 0; e < E; e++) d[n][e] *= post[n][e];
+							for(int e = 0; e < E; e++) d[n][e] *= value(post[n].e[e]);
+					}
 					back(d, z, own, sums, p.post_norm, a.inv_c, stats[1]);
 				}
 				own.store(static_cast<T*>(g.grad_y) + row * C, d);
@@ -496,7 +504,8 @@ __global__ void __launch_bounds__(256) join_kernel(join_args a) {
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
-// f(threads per row, stretches of 8 channels per thread): as few wavefronts to a row as hold it in 16 channels a thread; a workgroup where the rows are few
+// f(threads per row, stretches of 8 channels per thread).  Forward: as few wavefronts to a row as hold it in 16 channels a thread, a workgroup where the rows are few; backward,
+// which holds three times as much of a row and the sums: 8 channels a thread as far as workgroups go.
 template <typename F>
 int with_shape(int64_t C, int64_t rows, F f) {
 	if(C <= 512) return f(ic<64>(), ic<1>());
@@ -504,6 +513,15 @@ int with_shape(int64_t C, int64_t rows, F f) {
 	if(C <= 2048) return f(ic<256>(), ic<1>());
 	if(C <= 4096) return f(ic<256>(), ic<2>());
 	if(C <= 8192) return f(ic<512>(), ic<2>());
+	return f(ic<1024>(), ic<2>());
+}
+template <typename F>
+int with_backward_shape(int64_t C, F f) {
+	if(C <= 512) return f(ic<64>(), ic<1>());
+	if(C <= 1024) return f(ic<128>(), ic<1>());
+	if(C <= 2048) return f(ic<256>(), ic<1>());
+	if(C <= 4096) return f(ic<512>(), ic<1>());
+	if(C <= 8192) return f(ic<1024>(), ic<1>());
 	return f(ic<1024>(), ic<2>());
 }
 inline int64_t over(int64_t n, int64_t per) { return (n + per - 1) / per; }
@@ -534,9 +552,9 @@ plan backward_plan(const af3_residual_norm_params& p, const af3_residual_norm_gr
 	for(int i = 0; i < 4; i++)
 		if(wanted[i] && share[i] != AF3_SHARE_ROW) f.sums = true, grouped = grouped || share[i] == AF3_SHARE_GROUP;
 	f.group = grouped ? p.group : p.rows;
-	// With sums: 512 workgroups, so that their parts' way through memory stays small beside the rows'; without: a few rows to a worker.
-	const int64_t at_once = p.C <= 512 || (p.C <= 1024 && p.rows >= 2048) ? 4 : 1;
-	const int64_t target = f.sums ? over(over(p.rows, 512), at_once) * at_once : 4 * at_once;
+	// With sums: about as many workgroups as fit the chip together, so that their parts' way through memory stays small beside the rows'; without: a few rows to a worker.
+	const int64_t at_once = p.C <= 512 ? 4 : 1, most = p.C <= 512 ? 1024 : p.C <= 1024 ? 2048 : p.C <= 2048 ? 1024 : p.C <= 4096 ? 512 : 256;
+	const int64_t target = f.sums ? over(over(p.rows, most), at_once) * at_once : 4 * at_once;
 	if(f.group >= target) {
 		f.parts = (uint32_t)over(f.group, target), f.per = over(f.group, f.parts);
 		f.workgroups = (uint32_t)(p.rows / f.group) * f.parts;
@@ -559,7 +577,7 @@ plan backward_plan(const af3_residual_norm_params& p, const af3_residual_norm_gr
 
 template <typename T>
 int backward(const args& a, const plan& f, hipStream_t s) {
-	return with_shape(a.p.C, a.p.rows, [&](auto tpr, auto np) {
+	return with_backward_shape(a.p.C, [&](auto tpr, auto np) {
 		constexpr int TPR = decltype(tpr)::value, NP = decltype(np)::value, THREADS = threads_for(TPR);
 		if(f.sums) hipLaunchKernelGGL((backward_kernel<T, TPR, NP, true>), dim3(f.workgroups), dim3(THREADS), 0, s, a);
 		else hipLaunchKernelGGL((backward_kernel<T, TPR, NP, false>), dim3(f.workgroups), dim3(THREADS), 0, s, a);

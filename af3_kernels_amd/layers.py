@@ -219,6 +219,7 @@ class _DifferentialAttention(torch.autograd.Function):
             return (*(torch.zeros(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v, lam), wants)), None, None, None, None)
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v, lam), wants)]
         grad = _inner_contig(grad)
+        grad = grad if grad.stride(2) * grad.element_size() < _lib.DIFF_ATTENTION_GRAD_ROW_BYTES else grad.contiguous()
         p, g = _diff_block(q, k, v, lam, keep, out, stats, second, lost, *ctx.settings), DiffAttentionGrads()
         g.grad_out, g.grad_out_stride = grad.data_ptr(), _i64x3(*grad.stride()[:3])
         g.grad_q, g.grad_k, g.grad_v, g.grad_lam = (0 if t is None else t.data_ptr() for t in grads)

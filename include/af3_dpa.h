@@ -490,9 +490,10 @@ int64_t af3_diff_attention_workspace_bytes(const af3_diff_attention_params* para
  * Gradients of af3_diff_attention_forward.  `params` as in the forward call, with the out, stats and second that it wrote (its workspace is not used); grad_out
  * [B, H, Lq, Dv] with strides, of `dtype`.  grad_q [B, 2 H, Lq, D], grad_k [B, 2 Hkv, Lk, D], grad_v [B, Hkv, Lk, Dv] are contiguous and written whole, zeros for
  * dropped keys among it; grad_lam: H contiguous numbers of lam_dtype (one for each head, also where lam_stride is 0).  NULL: not wanted.  No atomics: the same bits every time.
- * Rows of grad_out no more than 2^23 elements apart (AF3_ERR_BAD_STRIDE).
+ * Rows of grad_out less than AF3_DIFF_ATTENTION_GRAD_ROW_BYTES apart (AF3_ERR_BAD_STRIDE).
  * workspace: af3_diff_attention_backward_workspace_bytes() bytes, 16-byte aligned, required.
  */
+#define AF3_DIFF_ATTENTION_GRAD_ROW_BYTES 16777216
 typedef struct af3_diff_attention_grads {
 	const void* grad_out;
 	int64_t     grad_out_stride[3];
