@@ -8,6 +8,9 @@
 // a fixed order.
 #include "mfma_helpers.hpp"
 
+// (products and sums are fused where fmaf says so: the kernels' instantiations then agree to the last bit, whichever gradients are wanted)
+#pragma clang fp contract(off)
+
 namespace af3 {
 namespace rnorm {
 
@@ -548,7 +551,7 @@ plan backward_plan(const af3_residual_norm_params& p, const af3_residual_norm_gr
 	plan f{};
 	const int32_t share[4] = {p.gate_share, p.weight_share, p.bias_share, AF3_SHARE_CHANNEL};
 	const void*   wanted[4] = {g.grad_gate, g.grad_weight, g.grad_bias, g.grad_post_weight};
-	bool          grouped = false;
+	bool          grouped = p.gate_share == AF3_SHARE_GROUP || p.weight_share == AF3_SHARE_GROUP;   // (rows that are read once for a group, whether their gradient is wanted or not)
 	for(int i = 0; i < 4; i++)
 		if(wanted[i] && share[i] != AF3_SHARE_ROW) f.sums = true, grouped = grouped || share[i] == AF3_SHARE_GROUP;
 	f.group = grouped ? p.group : p.rows;
