@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 // above, whose 8 wavefronts share tiles, 25.7.
 template <typename T, int DP>
 struct token_shape {
-	static constexpr int DV = 2 * DP, TILE = 32 * tile<T, DV>::STRIDE, LINE = 36, TABLE = 32 * LINE * 4;   // a tile of V, 32 columns of results: of a wavefront
+	static constexpr int DV = 2 * DP, TILE = 32 * tile<T, DV>::STRIDE, AT_ONCE = DV * (int)sizeof(T) / 128, LINE = 32 * AT_ONCE + 4, TABLE = 32 * LINE * 4;   // a tile of V; as many columns of results as have its room: of a wavefront
 	static constexpr int LDS = WAVES * (TILE > TABLE ? TILE : TABLE);
 };
 template <typename T, int DP>
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, (DP * sizeof(T) <= 128 ? 2 : 1)) diff
 	constexpr int E = kind<T>::E, N = TV::CHUNKS * 32 / 64;   // N: pieces of V per lane
 	const af3_diff_attention_params& p = a.p;
 	extern __shared__ __align__(16) unsigned char smem[];
-	__shared__ float stat[WAVES][32][2];
+	__shared__ float stat[WAVES][32][2], inverse[32];
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, map = (lane >> 4) & 1;
 	const share    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.splits);
@@ -589,64 +589,66 @@ __global__ void __launch_bounds__(THREADS, (DP * sizeof(T) <= 128 ? 2 : 1)) diff
 #pragma unroll
 	for(int w = 0; w < WAVES; w++) to = maximum(to, stat[w][lane & 31][0]);
 	const float by = __builtin_amdgcn_exp2f((m - to) * to_log2);
-	// Columns 32 at a time through LDS; a thread then has two of them of one of the 16 rows, in both maps.
-	const int       row = threadIdx.x >> 4, column = 2 * (threadIdx.x & 15);
-	const row_place place(row, rows, G, hk);
-	float top[2], total[2], inv[2];
+	const int64_t n_rows = p.B * p.Hkv * rows, first_row = (b * p.Hkv + hk) * rows;
+	if(threadIdx.x < 32) {   // one of the two maps of a row
+		const int       row = threadIdx.x & 15, i = threadIdx.x >> 4;
+		const row_place place(row, rows, G, hk);
+		float           total = 0.f;
 #pragma unroll
-	for(int i = 0; i < 2; i++) {
-		top[i] = LOWEST, total[i] = 0.f;
-#pragma unroll
-		for(int w = 0; w < WAVES; w++) top[i] = maximum(top[i], stat[w][16 * i + row][0]);
-#pragma unroll
-		for(int w = 0; w < WAVES; w++) total[i] += stat[w][16 * i + row][1] * __builtin_amdgcn_exp2f((stat[w][16 * i + row][0] - top[i]) * to_log2);
-		inv[i] = total[i] == 0.f ? 0.f : 1.f / total[i];
-	}
-	const int64_t n_rows = p.B * p.Hkv * rows, part_row = (b * p.Hkv + hk) * rows + row, out_row = (b * p.H + place.h) * p.Lq + place.qi;
-	const float   lam = lam_of(p, place.h);
-	if(place.ok && column == 0) {
-#pragma unroll
-		for(int i = 0; i < 2; i++) {
+		for(int w = 0; w < WAVES; w++) total += stat[w][threadIdx.x][1] * __builtin_amdgcn_exp2f((stat[w][threadIdx.x][0] - to) * to_log2);
+		inverse[threadIdx.x] = total == 0.f ? 0.f : 1.f / total;
+		if(place.ok) {
 			if(a.splits > 1) {
-				float* const st = a.part_stat + 2 * ((2 * (int64_t)split + i) * n_rows + part_row);
-				st[0] = top[i], st[1] = total[i];
+				float* const st = a.part_stat + 2 * ((2 * (int64_t)split + i) * n_rows + first_row + row);
+				st[0] = to, st[1] = total;
 			} else if(p.stats) {
 				float* const st = p.stats + 2 * ((b * 2 * p.H + 2 * place.h + i) * p.Lq + place.qi);
-				st[0] = top[i], st[1] = inv[i];
+				st[0] = to, st[1] = total == 0.f ? 0.f : 1.f / total;
 			}
 		}
 	}
-	float* const mine = reinterpret_cast<float*>(smem) + wave * (S::TABLE / 4) + (lane & 31) * S::LINE + 16 * half;
-	const float* const all = reinterpret_cast<const float*>(smem) + row * S::LINE + column;
+	// As many columns at a time through LDS as a tile of V has room for; a thread then has two of them of one row, in both maps.
+	constexpr int PAIRS = 16 * S::AT_ONCE;
+	float* const  mine = reinterpret_cast<float*>(smem) + wave * (S::TABLE / 4) + (lane & 31) * S::LINE + 16 * half;
 #pragma unroll
-	for(int db = 0; db < TV::BLOCKS; db++) {
+	for(int db = 0; db < TV::BLOCKS; db += S::AT_ONCE) {
 		if(32 * db >= Dv) break;
+		if(db > 0) __syncthreads();
+		if(at_row.ok) {
+#pragma unroll
+			for(int j = 0; j < S::AT_ONCE; j++)
+#pragma unroll
+				for(int e = 0; e < 4; e++)
+					*reinterpret_cast<f32x4*>(mine + 32 * j + 4 * e) = f32x4{o[db + j][4 * e] * by, o[db + j][4 * e + 1] * by, o[db + j][4 * e + 2] * by, o[db + j][4 * e + 3] * by};
+		}
 		__syncthreads();
+		for(int n = threadIdx.x; n < (int)rows * PAIRS; n += THREADS) {
+			const int          row = n / PAIRS, column = 2 * (n - row * PAIRS);
+			const float* const all = reinterpret_cast<const float*>(smem) + row * S::LINE + column;
+			const row_place    place(row, rows, G, hk);
 #pragma unroll
-		for(int e = 0; e < 4; e++) *reinterpret_cast<f32x4*>(mine + 4 * e) = f32x4{o[db][4 * e] * by, o[db][4 * e + 1] * by, o[db][4 * e + 2] * by, o[db][4 * e + 3] * by};
-		__syncthreads();
-		if(!place.ok) continue;
+			for(int c = 0; c < 2; c++) {
+				const int at = 32 * db + column + c;
+				if(at >= Dv) continue;
+				float r[2] = {0.f, 0.f};
 #pragma unroll
-		for(int c = 0; c < 2; c++) {
-			const int at = 32 * db + column + c;
-			if(at >= Dv) continue;
-			float r[2] = {0.f, 0.f};
+				for(int i = 0; i < 2; i++)
 #pragma unroll
-			for(int i = 0; i < 2; i++)
+					for(int w = 0; w < WAVES; w++) r[i] += all[w * (S::TABLE / 4) + 16 * i * S::LINE + c];
+				if(a.splits > 1) {
 #pragma unroll
-				for(int w = 0; w < WAVES; w++) r[i] += all[w * (S::TABLE / 4) + 16 * i * S::LINE + c];
-			if(a.splits > 1) {
-#pragma unroll
-				for(int i = 0; i < 2; i++) a.part_out[((2 * (int64_t)split + i) * n_rows + part_row) * Dv + at] = r[i];
-			} else {
-				store_result<T>(p, b, place.h, place.qi, out_row, at, total[0] == 0.f ? 0.f : __builtin_fmaf(-lam, r[1] * inv[1], r[0] * inv[0]), r[1] * inv[1]);
+					for(int i = 0; i < 2; i++) a.part_out[((2 * (int64_t)split + i) * n_rows + first_row + row) * Dv + at] = r[i];
+				} else {
+					const float second = r[1] * inverse[16 + row];
+					store_result<T>(p, b, place.h, place.qi, (b * p.H + place.h) * p.Lq + place.qi, at, __builtin_fmaf(-lam_of(p, place.h), second, r[0] * inverse[row]), second);
+				}
 			}
 		}
 	}
 }
 
 // The parts of the key axis joined: a workgroup per query row; two wavefronts to a map, half of the parts each, four columns to a lane.  The parts' maxima and sums come one to a
-// lane (64 parts at most), so that the parts' results, eight of them in flight, wait for nothing but each other.
+// lane (64 parts at most), so that the parts' results, 16 of them in flight, wait for nothing but each other.
 constexpr int MAX_PARTS = 64;
 template <typename T>
 __global__ void __launch_bounds__(THREADS) diff_join_kernel(forward_args a) {
@@ -669,24 +671,23 @@ __global__ void __launch_bounds__(THREADS) diff_join_kernel(forward_args a) {
 	const float inv = sum == 0.f ? 0.f : 1.f / sum;
 	const int   c = 4 * lane, per = (splits + 1) / 2, first = (wave >> 1) * per, end = first + per < splits ? first + per : splits;
 	f32x4       o = {0.f, 0.f, 0.f, 0.f};
-	for(int s0 = first; s0 < end; s0 += 8) {
-		f32x4 x[8];
+	const bool    whole = Dv % 4 == 0;   // (lanes behind the last column read what lane 0 does)
+	const float* const from = a.part_out + (map * n_rows + at) * Dv + (whole && c >= Dv ? 0 : c);
+	for(int s0 = first; s0 < end; s0 += 16) {
+		f32x4 x[16];
 #pragma unroll
-		for(int s = 0; s < 8; s++) {
-			x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
-			if(s0 + s < end && __shfl(l, (s0 + s) & 63) != 0.f) {   // (a part without a live key wrote nothing)
-				const float* const from = a.part_out + ((2 * (s0 + s) + map) * n_rows + at) * Dv + c;
-				if(c + 4 <= Dv) x[s] = *reinterpret_cast<const f32x4_any*>(from);
-				else
-					for(int e = 0; e < 4; e++)
-						if(c + e < Dv) x[s][e] = from[e];
-			}
+		for(int s = 0; s < 16; s++) {
+			const float* const part = from + (s0 + s < end ? s0 + s : end - 1) * (2 * n_rows * Dv);
+			if(whole) x[s] = *reinterpret_cast<const f32x4*>(part);
+			else
+#pragma unroll
+				for(int e = 0; e < 4; e++) x[s][e] = c + e < Dv ? part[e] : 0.f;
 		}
 #pragma unroll
-		for(int s = 0; s < 8; s++) {
+		for(int s = 0; s < 16; s++) {
 			const float w = s0 + s < end ? __shfl(weight, (s0 + s) & 63) : 0.f;
 #pragma unroll
-			for(int e = 0; e < 4; e++) o[e] = __builtin_fmaf(x[s][e], w, o[e]);
+			for(int e = 0; e < 4; e++) o[e] = w == 0.f ? o[e] : __builtin_fmaf(x[s][e], w, o[e]);   // (a part without a live key wrote nothing)
 		}
 	}
 	if(wave >> 1) halves[map][lane] = o;
@@ -728,6 +729,17 @@ struct plan {
 	bool     token;   // diff_token_kernel
 };
 constexpr int TOKEN_ROWS = 16;
+// As parts_for, down to parts of a single step: what a step costs is its way from memory.
+int64_t token_parts(const af3_diff_attention_params& p, int64_t groups, int64_t steps, double step_us) {
+	constexpr double JOIN_US = 6.0, BYTES_PER_US = 2e6;
+	double           best = 0.0;
+	int64_t          parts = 1;
+	for(int64_t n = 1; n <= MAX_PARTS && n <= steps && (n == 1 || groups * n <= 512); n++) {
+		const double us = (double)((steps + n - 1) / n) * step_us + (n > 1 ? JOIN_US + n * 16.0 * p.B * p.H * p.Lq * p.Dv / BYTES_PER_US : 0.0);
+		if(n == 1 || us < best) best = us, parts = n;
+	}
+	return parts;
+}
 plan forward_plan(const af3_diff_attention_params& p) {
 	plan          f;
 	const int64_t rows = p.H / p.Hkv * p.Lq, groups = p.B * p.Hkv;
@@ -737,7 +749,7 @@ plan forward_plan(const af3_diff_attention_params& p) {
 	f.token = rows <= TOKEN_ROWS, f.half = false;
 	if(f.token) {
 		// (128 keys to a step of the workgroup; two workgroups to a compute unit)
-		const int64_t steps = (p.Lk + 127) / 128, splits = parts_for(groups, 512, steps, (0.8 + 0.008 * wide) * (fp32 ? 2.0 : 1.0), 8.0 * p.B * p.H * p.Lq * p.Dv, MAX_PARTS);
+		const int64_t steps = (p.Lk + 127) / 128, splits = token_parts(p, groups, steps, (0.9 + 0.018 * wide) * (fp32 ? 2.5 : 1.0));
 		const int64_t each = (steps + splits - 1) / splits;
 		f.kw = 4, f.row_tiles = 1, f.part = 128 * each, f.splits = (uint32_t)((steps + each - 1) / each);
 		return f;

@@ -54,14 +54,16 @@ __device__ __forceinline__ void add_up(float* tables, int w, int lane, f32x16 (&
 	}
 }
 
-// d1 and d2: 32 lanes per row, 8 columns each (those of out and of second are read to 16 bits where the forward pass left what their rounding lost)
+// d1 and d2: 8, 16 or 32 lanes per row, 8 columns each (those of out and of second are read to 16 bits where the forward pass left what their rounding lost)
+__host__ __device__ constexpr int delta_lanes(const af3_diff_attention_params& p) { return p.Dv <= 64 ? 8 : p.Dv <= 128 ? 16 : 32; }
 template <typename T>
 __global__ void __launch_bounds__(THREADS) diff_delta_kernel(grad_args a) {
 	const af3_diff_attention_params& p = a.p;
-	const int64_t row = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), n_rows = p.B * p.H * p.Lq;
-	if(row >= n_rows) return;   // (half a wavefront)
-	const int64_t bh = row / p.Lq, qi = row - bh * p.Lq, b = bh / p.H, h = bh - b * p.H;
-	const int     lane = threadIdx.x & 31, Dv = (int)p.Dv;
+	const int     lanes = delta_lanes(p);
+	const int64_t row = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / lanes, n_rows = p.B * p.H * p.Lq;
+	if(row >= n_rows) return;   // (all lanes of the row)
+	const int64_t bh = (uint32_t)row / (uint32_t)p.Lq, qi = row - bh * p.Lq, b = (uint32_t)bh / (uint32_t)p.H, h = bh - b * p.H;   // (fewer than 2^29 rows)
+	const int     lane = threadIdx.x & (lanes - 1), Dv = (int)p.Dv;
 	auto eight = [&](const T* from, float (&x)[8]) {
 		if(8 * lane + 8 <= Dv) {
 			if constexpr(sizeof(T) == 2) {
@@ -96,7 +98,8 @@ __global__ void __launch_bounds__(THREADS) diff_delta_kernel(grad_args a) {
 #pragma unroll
 	for(int e = 0; e < 8; e++) d1 = __builtin_fmaf(g[e], o[e], d1), d2 = __builtin_fmaf(g[e], s[e], d2);
 #pragma unroll
-	for(int i = 16; i; i >>= 1) d1 += __shfl_xor(d1, i), d2 += __shfl_xor(d2, i);
+	for(int i = 16; i; i >>= 1)
+		if(i < lanes) d1 += __shfl_xor(d1, i), d2 += __shfl_xor(d2, i);
 	if(lane == 0) a.d1[row] = __builtin_fmaf(lam_of(p, h), d2, d1), a.d2[row] = d2;
 }
 
@@ -691,7 +694,7 @@ int backward(grad_args a, hipStream_t s) {
 		sum_blocks += sums.blocks[n_sums] = (uint32_t)over(n, 4 * THREADS);
 		n_sums++;
 	};
-	hipLaunchKernelGGL(diff_delta_kernel<T>, dim3((uint32_t)over(p.B * p.H * p.Lq, THREADS / 32)), dim3(THREADS), 0, s, a);
+	hipLaunchKernelGGL(diff_delta_kernel<T>, dim3((uint32_t)over(p.B * p.H * p.Lq, THREADS / delta_lanes(p))), dim3(THREADS), 0, s, a);
 	int rc = launch_status();
 	if(rc != AF3_OK) return rc;
 	if(!a.g.grad_lam) a.short_of = nullptr;
