@@ -107,8 +107,9 @@ __global__ void __launch_bounds__(THREADS) diff_delta_kernel(grad_args a) {
 constexpr int tile_rows(int bytes, int sharing) { return sharing == 4 || bytes <= 64 ? 128 : bytes <= 128 ? 64 : 32; }
 constexpr int dq_maps(int bytes) { return bytes <= 128 ? 2 : 1; }
 constexpr int dq_threads(int bytes) { return 512; }
-constexpr int dkv_maps(int bytes) { return bytes <= 128 ? 2 : 1; }
-constexpr int dkv_threads(int bytes) { return 256; }
+constexpr int dkv_maps(int bytes, int sharing) { return bytes <= 64 || sharing > 1 ? 2 : 1; }
+constexpr int dkv_threads(int bytes, int sharing) { return bytes == 128 && sharing == 1 ? 512 : 256; }
+constexpr int dkv_rows(int bytes, int sharing) { return tile_rows(bytes, sharing); }
 
 // ---- dQ ----
 // KW: wavefronts that share 32 rows and each take 32 keys of a tile; MAPS: maps of a wavefront, 2, or 1 with the other map beside it in another one
@@ -327,14 +328,14 @@ struct row_stats {
 // RW: wavefronts that share 32 keys and each take 32 rows of a tile of query rows (1: every wavefront has its own keys and takes the whole tile).  MAPS as in dq_shape.
 template <typename T, int DP, int RW>
 struct dkv_shape {
-	static constexpr int BYTES = DP * (int)sizeof(T), MAPS = dkv_maps(BYTES), NT = dkv_threads(BYTES), W = NT / 64, GROUPS = W * MAPS / 2 / RW;
-	static constexpr int DV = 2 * DP, QT = tile_rows(BYTES, RW), SUB = QT / (32 * RW), KEYS = 32 * GROUPS;
+	static constexpr int BYTES = DP * (int)sizeof(T), MAPS = dkv_maps(BYTES, RW), NT = dkv_threads(BYTES, RW), W = NT / 64, GROUPS = W * MAPS / 2 / RW;
+	static constexpr int DV = 2 * DP, QT = dkv_rows(BYTES, RW), SUB = QT / (32 * RW), KEYS = 32 * GROUPS;
 	static constexpr int QTILE = QT * tile<T, DP>::STRIDE, GTILE = QT * tile<T, DV>::STRIDE, STATS = row_stats<T, QT>::BYTES, SET = 2 * QTILE + GTILE + STATS;
 	static constexpr int BUFFERS = 2 * SET <= 73728 ? 2 : 1;
 	// One map to a wavefront: the two of a pair exchange their probabilities, so that their difference is rounded once, and have half of dV's columns each.
-	static constexpr int VBLOCKS = DV / 32 * MAPS / 2, EXCHANGE = MAPS == 1 ? W * 64 * 64 : 0;
-	static_assert(MAPS == 2 || (RW == 1 && SUB == 1));
-	static constexpr int JOIN = RW > 1 ? W * 32 * (DV + 4) * 4 : 0, PER_SIMD = BYTES <= 64 ? 2 : 1;   // wavefronts to a SIMD, by the registers of sums and operands
+	static constexpr int VBLOCKS = DV / 32 * MAPS / 2, EXCHANGE = MAPS == 1 ? SUB * W * 64 * 64 : 0;
+	static_assert(MAPS == 2 || RW == 1);
+	static constexpr int JOIN = RW > 1 ? W * 32 * (DV + 4) * 4 : 0, PER_SIMD = BYTES <= 64 || (BYTES == 128 && MAPS == 1) ? 2 : 1;   // wavefronts to a SIMD, by the registers of sums and operands
 	static constexpr int LDS = BUFFERS * SET + EXCHANGE > JOIN ? BUFFERS * SET + EXCHANGE : JOIN;
 };
 
@@ -416,7 +417,6 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 		if(more) fetch(head, at);
 		const bool apart = rs.apart(st);
 		float both[16];
-		bool  met = false;   // (one map to a wavefront: there is something to exchange)
 		auto  add_values = [&](int row0) {
 			const typename TV::reader at_g = S::PER_SIMD == 2 ? fresh(at_g_) : at_g_;
 #pragma unroll
@@ -426,14 +426,13 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 				for(int db = 0; db < S::VBLOCKS; db++) dv[db] = kind<T>::mma(TV::col_frag(gs, row0, vblock0 + db, j, at_g), pf, dv[db]);
 			}
 		};
-		if(work) {
 #pragma unroll 1
-			for(int s = 0; s < S::SUB; s++) {
-				const int row0 = 32 * (rwave * S::SUB + s);
-				if(row0 >= left) continue;
-				// the lane's rows need .. 15 of its 16 count
-				const int need = p.causal ? clamped(key - p.q_offset - (q0 + row0 + 16 * half)) : -64;
-				if(!__any(in && need <= 15)) continue;
+		for(int s = 0; s < S::SUB; s++) {
+			const int row0 = 32 * (rwave * S::SUB + s);
+			// the lane's rows need .. 15 of its 16 count
+			const int  need = p.causal ? clamped(key - p.q_offset - (q0 + row0 + 16 * half)) : -64;
+			const bool met = work && row0 < left && __any(in && need <= 15);
+			if(met) {
 				const bool diagonal = __any(in && need > 0);
 				const typename TK::reader at_q = S::PER_SIMD == 2 ? fresh(at_q_) : at_q_;
 				const typename TV::reader at_g = S::PER_SIMD == 2 ? fresh(at_g_) : at_g_;
@@ -480,24 +479,23 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 					}
 				}
 				if constexpr(MAPS == 2) add_values(row0);
-				met = true;
 			}
-		}
-		if constexpr(MAPS == 1) {
-			f32x4* const exchange = reinterpret_cast<f32x4*>(smem + S::BUFFERS * S::SET) + lane;
-			if(met) {
+			if constexpr(MAPS == 1) {
+				f32x4* const exchange = reinterpret_cast<f32x4*>(smem + S::BUFFERS * S::SET) + 256 * S::W * s + lane;
+				if(met) {
 #pragma unroll
-				for(int i = 0; i < 4; i++) exchange[64 * (4 * wave + i)] = f32x4{both[4 * i], both[4 * i + 1], both[4 * i + 2], both[4 * i + 3]};
-			}
-			__syncthreads();
-			if(met) {   // (and so it is for the other one, which has the same keys)
-#pragma unroll
-				for(int i = 0; i < 4; i++) {
-					const f32x4 other = exchange[64 * (4 * (wave ^ 1) + i)];
-#pragma unroll
-					for(int e = 0; e < 4; e++) both[4 * i + e] += other[e];
+					for(int i = 0; i < 4; i++) exchange[64 * (4 * wave + i)] = f32x4{both[4 * i], both[4 * i + 1], both[4 * i + 2], both[4 * i + 3]};
 				}
-				add_values(0);
+				__syncthreads();
+				if(met) {   // (and so it is for the other one, which has the same keys)
+#pragma unroll
+					for(int i = 0; i < 4; i++) {
+						const f32x4 other = exchange[64 * (4 * (wave ^ 1) + i)];
+#pragma unroll
+						for(int e = 0; e < 4; e++) both[4 * i + e] += other[e];
+					}
+					add_values(row0);
+				}
 			}
 		}
 		if constexpr(S::BUFFERS == 2) buffer ^= 1;
@@ -618,14 +616,14 @@ double counting(const af3_diff_attention_params& p) {
 // `length` rows that results belong to, `alone` of them per workgroup where every wavefront has its own; `steps(sharing)` tiles of the other axis, of which a launch walks the part
 // `counts`, the workgroups with the most first; `slots` workgroups fit the chip at a time; a tile costs load_us and block_us for each block of 32 x 32 that a wavefront has of it.
 // Sharing makes more and shorter workgroups, so do parts of the long axis, whose results go through memory and are joined: whatever ends first.
-template <typename F>
-cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double counts, int64_t slots, double load_us, double block_us, double part_bytes, F steps) {
+template <typename R, typename F>
+cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double counts, int64_t slots, double load_us, double block_us, double part_bytes, R rows, F steps) {
 	constexpr double JOIN_US = 6.0, BYTES_PER_US = 2e6;
 	cut    best{};
 	double best_us = 0.0;
 	for(int sharing = 1; sharing <= (bytes > 128 ? 1 : 4); sharing *= 2) {
 		const int64_t tiles = over(length, alone / sharing), n = steps(sharing), workgroups = groups * tiles;
-		const double  tile_us = load_us * tile_rows(bytes, sharing) / 64 + block_us * tile_rows(bytes, sharing) / (32 * sharing);
+		const double  tile_us = load_us * rows(sharing) / 64 + block_us * rows(sharing) / (32 * sharing);
 		for(int64_t parts = 1; parts <= 64 && (parts == 1 || 2 * parts <= n + 1); parts++) {
 			const double longest = (double)over(n, parts), all = (double)workgroups * n * counts / slots;
 			const double us = (workgroups * parts <= slots ? longest : longest > all + 0.8 * longest ? longest : all + 0.8 * longest) * tile_us + (parts > 1 ? JOIN_US + parts * 2.0 * part_bytes / BYTES_PER_US : 0.0);
@@ -637,14 +635,14 @@ cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double cou
 cut dq_cut(const af3_diff_attention_params& p) {
 	const int bytes = row_bytes(p);
 	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, 32 * dq_threads(bytes) / 64 * dq_maps(bytes) / 2, bytes, counting(p), 256, 0.4 + 0.009 * bytes, (0.4 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0),
-					8.0 * p.B * p.H * p.Lq * p.D, [&](int sharing) { return over(p.Lk, tile_rows(bytes, sharing)); });
+					8.0 * p.B * p.H * p.Lq * p.D, [&](int sharing) { return tile_rows(bytes, sharing); }, [&](int sharing) { return over(p.Lk, tile_rows(bytes, sharing)); });
 	c.part *= tile_rows(bytes, c.sharing);
 	return c;
 }
 cut dkv_cut(const af3_diff_attention_params& p) {
 	const int bytes = row_bytes(p);
-	return cut_for(p.Lk, p.B * p.Hkv, 32 * dkv_threads(bytes) / 64 * dkv_maps(bytes) / 2, bytes, counting(p), bytes > 64 ? 256 : 512, 0.3 + 0.006 * bytes, (0.5 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0),
-				   4.0 * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv), [&](int sharing) { return p.H / p.Hkv * over(p.Lq, tile_rows(bytes, sharing)); });
+	return cut_for(p.Lk, p.B * p.Hkv, bytes > 128 ? 64 : 128, bytes, counting(p), bytes > 64 ? 256 : 512, 0.3 + 0.006 * bytes, (0.5 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0),
+				   4.0 * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv), [&](int sharing) { return dkv_rows(bytes, sharing); }, [&](int sharing) { return p.H / p.Hkv * over(p.Lq, dkv_rows(bytes, sharing)); });
 }
 
 int64_t packed_grad_bytes(const af3_diff_attention_params& p) {
