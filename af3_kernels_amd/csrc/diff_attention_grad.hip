@@ -107,9 +107,10 @@ __global__ void __launch_bounds__(THREADS) diff_delta_kernel(grad_args a) {
 constexpr int tile_rows(int bytes, int sharing) { return sharing == 4 || bytes <= 64 ? 128 : bytes <= 128 ? 64 : 32; }
 constexpr int dq_maps(int bytes) { return bytes <= 128 ? 2 : 1; }
 constexpr int dq_threads(int bytes) { return 512; }
+// dK and dV of 128-byte rows: both maps in a wavefront need 370 registers, one wavefront to a SIMD; with one map each, and dP computed by both, there are two (2 x 16 (4) x 4096 x 64
+// causal 761 -> 579 us, in workgroups of 256 threads 776).  Where wavefronts share their keys the pairs' exchange would be between twice as many.
 constexpr int dkv_maps(int bytes, int sharing) { return bytes <= 64 || sharing > 1 ? 2 : 1; }
 constexpr int dkv_threads(int bytes, int sharing) { return bytes == 128 && sharing == 1 ? 512 : 256; }
-constexpr int dkv_rows(int bytes, int sharing) { return tile_rows(bytes, sharing); }
 
 // ---- dQ ----
 // KW: wavefronts that share 32 rows and each take 32 keys of a tile; MAPS: maps of a wavefront, 2, or 1 with the other map beside it in another one
@@ -329,7 +330,7 @@ struct row_stats {
 template <typename T, int DP, int RW>
 struct dkv_shape {
 	static constexpr int BYTES = DP * (int)sizeof(T), MAPS = dkv_maps(BYTES, RW), NT = dkv_threads(BYTES, RW), W = NT / 64, GROUPS = W * MAPS / 2 / RW;
-	static constexpr int DV = 2 * DP, QT = dkv_rows(BYTES, RW), SUB = QT / (32 * RW), KEYS = 32 * GROUPS;
+	static constexpr int DV = 2 * DP, QT = tile_rows(BYTES, RW), SUB = QT / (32 * RW), KEYS = 32 * GROUPS;
 	static constexpr int QTILE = QT * tile<T, DP>::STRIDE, GTILE = QT * tile<T, DV>::STRIDE, STATS = row_stats<T, QT>::BYTES, SET = 2 * QTILE + GTILE + STATS;
 	static constexpr int BUFFERS = 2 * SET <= 73728 ? 2 : 1;
 	// One map to a wavefront: the two of a pair exchange their probabilities, so that their difference is rounded once, and have half of dV's columns each.
@@ -616,14 +617,14 @@ double counting(const af3_diff_attention_params& p) {
 // `length` rows that results belong to, `alone` of them per workgroup where every wavefront has its own; `steps(sharing)` tiles of the other axis, of which a launch walks the part
 // `counts`, the workgroups with the most first; `slots` workgroups fit the chip at a time; a tile costs load_us and block_us for each block of 32 x 32 that a wavefront has of it.
 // Sharing makes more and shorter workgroups, so do parts of the long axis, whose results go through memory and are joined: whatever ends first.
-template <typename R, typename F>
-cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double counts, int64_t slots, double load_us, double block_us, double part_bytes, R rows, F steps) {
+template <typename U, typename F>
+cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double counts, int64_t slots, double load_us, U block_us, double part_bytes, F steps) {
 	constexpr double JOIN_US = 6.0, BYTES_PER_US = 2e6;
 	cut    best{};
 	double best_us = 0.0;
 	for(int sharing = 1; sharing <= (bytes > 128 ? 1 : 4); sharing *= 2) {
 		const int64_t tiles = over(length, alone / sharing), n = steps(sharing), workgroups = groups * tiles;
-		const double  tile_us = load_us * rows(sharing) / 64 + block_us * rows(sharing) / (32 * sharing);
+		const double  tile_us = load_us * tile_rows(bytes, sharing) / 64 + block_us(sharing) * tile_rows(bytes, sharing) / (32 * sharing);
 		for(int64_t parts = 1; parts <= 64 && (parts == 1 || 2 * parts <= n + 1); parts++) {
 			const double longest = (double)over(n, parts), all = (double)workgroups * n * counts / slots;
 			const double us = (workgroups * parts <= slots ? longest : longest > all + 0.8 * longest ? longest : all + 0.8 * longest) * tile_us + (parts > 1 ? JOIN_US + parts * 2.0 * part_bytes / BYTES_PER_US : 0.0);
@@ -634,15 +635,15 @@ cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double cou
 }
 cut dq_cut(const af3_diff_attention_params& p) {
 	const int bytes = row_bytes(p);
-	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, 32 * dq_threads(bytes) / 64 * dq_maps(bytes) / 2, bytes, counting(p), 256, 0.4 + 0.009 * bytes, (0.4 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0),
-					8.0 * p.B * p.H * p.Lq * p.D, [&](int sharing) { return tile_rows(bytes, sharing); }, [&](int sharing) { return over(p.Lk, tile_rows(bytes, sharing)); });
+	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, 32 * dq_threads(bytes) / 64 * dq_maps(bytes) / 2, bytes, counting(p), 256, 0.4 + 0.009 * bytes, [&](int) { return (0.4 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0); },
+					8.0 * p.B * p.H * p.Lq * p.D, [&](int sharing) { return over(p.Lk, tile_rows(bytes, sharing)); });
 	c.part *= tile_rows(bytes, c.sharing);
 	return c;
 }
 cut dkv_cut(const af3_diff_attention_params& p) {
 	const int bytes = row_bytes(p);
-	return cut_for(p.Lk, p.B * p.Hkv, bytes > 128 ? 64 : 128, bytes, counting(p), bytes > 64 ? 256 : 512, 0.3 + 0.006 * bytes, (0.5 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0),
-				   4.0 * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv), [&](int sharing) { return dkv_rows(bytes, sharing); }, [&](int sharing) { return p.H / p.Hkv * over(p.Lq, dkv_rows(bytes, sharing)); });
+	return cut_for(p.Lk, p.B * p.Hkv, bytes > 128 ? 64 : 128, bytes, counting(p), bytes > 64 ? 256 : 512, 0.3 + 0.006 * bytes, [&](int sharing) { return (0.5 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : sharing == 1 && bytes == 128 ? 0.7 : 1.0); },
+				   4.0 * p.B * p.Hkv * p.Lk * (2 * p.D + p.Dv), [&](int sharing) { return p.H / p.Hkv * over(p.Lq, tile_rows(bytes, sharing)); });
 }
 
 int64_t packed_grad_bytes(const af3_diff_attention_params& p) {
