@@ -845,8 +845,8 @@ int validate_diff_attention(const af3_diff_attention_params* p) {
 	if((p->dtype != AF3_F32 && p->dtype != AF3_BF16) || (p->lam_dtype != AF3_F32 && p->lam_dtype != AF3_BF16)) return AF3_ERR_BAD_DTYPE;
 	if(p->B <= 0 || p->H <= 0 || p->Hkv <= 0 || p->Lq <= 0 || p->Lk <= 0 || p->D <= 0 || p->Dv <= 0 || p->H % p->Hkv != 0) return AF3_ERR_BAD_SHAPE;
 	if(p->D > (p->dtype == AF3_F32 ? 64 : 128) || p->Dv > (p->dtype == AF3_F32 ? 128 : 256)) return AF3_ERR_UNSUPPORTED_D;
-	// (row numbers and the parts' sizes stay far inside 63 bits, a launch's workgroups times 256 threads inside 32)
-	if(p->B > 0xffffff || p->H > 0x7fff || p->Lq > 0x3fffffff || p->Lk > 0x3fffffff || p->B * p->H > 0xffffff || p->H * p->Lq > 0x3fffffff || p->B * p->H * ((p->Lq + 31) / 32) > 0xffffff) return AF3_ERR_BAD_SHAPE;
+	// (row numbers and the parts' sizes stay far inside 63 bits, a launch's workgroups times their threads inside 32)
+	if(p->B > 0xffffff || p->H > 0x7fff || p->Lq > 0x3fffffff || p->Lk > 0x3fffffff || p->B * p->H > 0xffffff || p->B * p->Hkv > 0x7fffff || p->H * p->Lq > 0x3fffffff || p->B * p->H * ((p->Lq + 31) / 32) > 0xffffff) return AF3_ERR_BAD_SHAPE;
 	if(p->stats && !diff_gradients_fit(*p)) return AF3_ERR_BAD_SHAPE;   // (they are for a gradient that would be refused)
 	if(!p->q || !p->k || !p->v || !p->lam || !p->out || (p->stats != nullptr) != (p->second != nullptr) || (p->residuals && !p->second)) return AF3_ERR_NULL_POINTER;
 	if(p->residuals && p->dtype != AF3_BF16) return AF3_ERR_BAD_DTYPE;   // (nothing would be written there)

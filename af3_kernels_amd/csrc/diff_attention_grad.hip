@@ -60,7 +60,7 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) diff_delta_kernel(grad_args a) {
 	const af3_diff_attention_params& p = a.p;
 	const int     lanes = delta_lanes(p);
-	const int64_t row = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / lanes, n_rows = p.B * p.H * p.Lq;
+	const int64_t n_rows = p.B * p.H * p.Lq, row = (blockIdx.y * (int64_t)gridDim.x + blockIdx.x) * (THREADS / lanes) + threadIdx.x / lanes;
 	if(row >= n_rows) return;   // (all lanes of the row)
 	const int64_t bh = (uint32_t)row / (uint32_t)p.Lq, qi = row - bh * p.Lq, b = (uint32_t)bh / (uint32_t)p.H, h = bh - b * p.H;   // (fewer than 2^29 rows)
 	const int     lane = threadIdx.x & (lanes - 1), Dv = (int)p.Dv;
@@ -627,6 +627,7 @@ cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double cou
 		const double  tile_us = load_us * tile_rows(bytes, sharing) / 64 + block_us(sharing) * tile_rows(bytes, sharing) / (32 * sharing);
 		for(int64_t parts = 1; parts <= 64 && (parts == 1 || 2 * parts <= n + 1); parts++) {
 			const double longest = (double)over(n, parts), all = (double)workgroups * n * counts / slots;
+			if(workgroups * parts > 0x7fffff && (sharing > 1 || parts > 1)) break;   // (times 512 threads inside 32 bits: so are those of the first choice, by what validate_diff_attention takes)
 			const double us = (workgroups * parts <= slots ? longest : longest > all + 0.8 * longest ? longest : all + 0.8 * longest) * tile_us + (parts > 1 ? JOIN_US + parts * 2.0 * part_bytes / BYTES_PER_US : 0.0);
 			if(best_us == 0.0 || us < best_us) best_us = us, best.sharing = sharing, best.tiles = (uint32_t)tiles, best.part = over(n, parts), best.splits = (uint32_t)over(n, best.part);
 		}
@@ -693,7 +694,7 @@ int backward(grad_args a, hipStream_t s) {
 		sum_blocks += sums.blocks[n_sums] = (uint32_t)over(n, 4 * THREADS);
 		n_sums++;
 	};
-	hipLaunchKernelGGL(diff_delta_kernel<T>, dim3((uint32_t)over(p.B * p.H * p.Lq, THREADS / delta_lanes(p))), dim3(THREADS), 0, s, a);
+	hipLaunchKernelGGL(diff_delta_kernel<T>, grid_of(over(p.B * p.H * p.Lq, THREADS / delta_lanes(p))), dim3(THREADS), 0, s, a);
 	int rc = launch_status();
 	if(rc != AF3_OK) return rc;
 	if(!a.g.grad_lam) a.short_of = nullptr;

@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(threads_for(TPR)) forward_kernel(args a) {
 	const af3_residual_norm_params& p = a.p;
 	constexpr int AT_ONCE = threads_for(TPR) / TPR;
 	__shared__ float lds[TPR > 64 ? 4 * (TPR / 64) : 1];
-	const int64_t row = (int64_t)blockIdx.x * AT_ONCE + threadIdx.x / TPR;
+	const int64_t row = (blockIdx.y * (int64_t)gridDim.x + blockIdx.x) * AT_ONCE + threadIdx.x / TPR;
 	if(row >= p.rows) return;   // (a whole wavefront, and with more of them to a row the whole workgroup)
 	const row_of<T, TPR, NP> own(threadIdx.x % TPR, (int)p.C);
 	row_sums<TPR>            sums(lds);
@@ -267,14 +267,16 @@ __global__ void __launch_bounds__(threads_for(TPR)) backward_kernel(args a) {
 	const int64_t C = p.C;
 
 	int64_t first, last, step;   // rows of this workgroup; rows that share a group's row among them
+	const int64_t block = blockIdx.y * (int64_t)gridDim.x + blockIdx.x;
 	if(a.parts) {
-		const int64_t stretch = blockIdx.x / a.parts, part = blockIdx.x - stretch * a.parts;
+		const int64_t stretch = block / a.parts, part = block - stretch * a.parts;
 		first = stretch * a.group + part * a.per, last = first + a.per < (stretch + 1) * a.group ? first + a.per : (stretch + 1) * a.group;
 		step  = a.per;
 	} else {
-		first = blockIdx.x * a.per, last = first + a.per < p.rows ? first + a.per : p.rows;
+		first = block * a.per, last = first + a.per < p.rows ? first + a.per : p.rows;
 		step  = a.group;
 	}
+	if(first >= p.rows) return;   // (the whole workgroup)
 	float total[SUMS ? 4 : 1][NP][E];
 	auto  clear = [&](int which) {
 #pragma unroll
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(threads_for(TPR)) backward_kernel(args a) {
 	if constexpr(SUMS) clear(GATE), clear(WEIGHT), clear(BIAS), clear(POST);
 
 	// What a row needs comes in one go, a row ahead of its use where the registers hold two of them; what rows share stays in registers.  4 x 2048 rows of 4096 channels in bf16:
-	// 107 us (5.1 TB/s); with 16 channels a thread, everything loaded where it is used, 210; 4 x 768 conditioned rows of 1024 channels 29 us, that way 54.
+	// 107 us (5.1 TB/s); with 16 channels a thread, everything loaded where it is used, 210; 8 x 768 conditioned rows of 768 channels 29 us, that way 54.
 	constexpr bool AHEAD = TPR * NP <= 1024;
 	struct streams {
 		eight<T> y[NP], x[NP], out[NP], normed[NP], gate[NP], weight[NP];
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(threads_for(TPR)) backward_kernel(args a) {
 		if constexpr(SUMS) {   // what the rows of a group share
 			auto group_sum = [&](int which, int32_t share, void* result) {
 				if(!result || share != AF3_SHARE_GROUP) return;
-				flush(which, a.partial[which] ? a.partial[which] + blockIdx.x * C : nullptr, static_cast<T*>(result) + begin / p.group * C);
+				flush(which, a.partial[which] ? a.partial[which] + block * C : nullptr, static_cast<T*>(result) + begin / p.group * C);
 				clear(which);
 			};
 			group_sum(GATE, p.gate_share, g.grad_gate), group_sum(WEIGHT, p.weight_share, g.grad_weight), group_sum(BIAS, p.bias_share, g.grad_bias);
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(threads_for(TPR)) backward_kernel(args a) {
 	}
 	if constexpr(SUMS) {
 		auto sum = [&](int which, int32_t share, void* result) {
-			if(result && share == AF3_SHARE_CHANNEL) flush(which, a.partial[which] + blockIdx.x * C, nullptr);
+			if(result && share == AF3_SHARE_CHANNEL) flush(which, a.partial[which] + block * C, nullptr);
 		};
 		sum(GATE, p.gate_share, g.grad_gate), sum(WEIGHT, p.weight_share, g.grad_weight), sum(BIAS, p.bias_share, g.grad_bias), sum(POST, AF3_SHARE_CHANNEL, g.grad_post_weight);
 	}
@@ -533,7 +535,7 @@ template <typename T>
 int forward(const args& a, hipStream_t s) {
 	return with_shape(a.p.C, a.p.rows, [&](auto tpr, auto np) {
 		constexpr int TPR = decltype(tpr)::value, NP = decltype(np)::value, THREADS = threads_for(TPR);
-		hipLaunchKernelGGL((forward_kernel<T, TPR, NP>), dim3((uint32_t)over(a.p.rows, THREADS / TPR)), dim3(THREADS), 0, s, a);
+		hipLaunchKernelGGL((forward_kernel<T, TPR, NP>), grid_of(over(a.p.rows, THREADS / TPR)), dim3(THREADS), 0, s, a);
 		return launch_status();
 	});
 }
@@ -582,8 +584,8 @@ template <typename T>
 int backward(const args& a, const plan& f, hipStream_t s) {
 	return with_backward_shape(a.p.C, [&](auto tpr, auto np) {
 		constexpr int TPR = decltype(tpr)::value, NP = decltype(np)::value, THREADS = threads_for(TPR);
-		if(f.sums) hipLaunchKernelGGL((backward_kernel<T, TPR, NP, true>), dim3(f.workgroups), dim3(THREADS), 0, s, a);
-		else hipLaunchKernelGGL((backward_kernel<T, TPR, NP, false>), dim3(f.workgroups), dim3(THREADS), 0, s, a);
+		if(f.sums) hipLaunchKernelGGL((backward_kernel<T, TPR, NP, true>), grid_of(f.workgroups), dim3(THREADS), 0, s, a);
+		else hipLaunchKernelGGL((backward_kernel<T, TPR, NP, false>), grid_of(f.workgroups), dim3(THREADS), 0, s, a);
 		return launch_status();
 	});
 }

@@ -250,6 +250,8 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     out = _host.differential_attention(q, k, v, lam, mask, causal, q_offset, softmax_scale)
     if out is not None:
         return out if out.__class__ is not int else _lib.check(out, "af3_diff_attention_forward")
+    if not isinstance(lam, torch.Tensor):
+        raise TypeError(f"lam must be a tensor, [H] or of one element, got {type(lam).__name__}")
     _no_tangents("differential_attention", q, k, v, lam)
     _same_device(q, k, v, lam, mask)
     if q.dtype not in _DTYPES:

@@ -457,7 +457,7 @@ int64_t af3_position_bias_workspace_bytes(const af3_position_bias_params* params
  *                 sums of grad_out * out that it takes off every dS are those of results to 16 bits.
  *   workspace   : af3_diff_attention_workspace_bytes() bytes, 16-byte aligned; NULL where that is 0.  Overwritten.
  * B, H, Lq, Lk, D, Dv >= 1; D <= 128 and Dv <= 256 (AF3_F32: D <= 64 and Dv <= 128; AF3_ERR_UNSUPPORTED_D); Lq and Lk < 2^30, H < 2^15, H * Lq < 2^30,
- * B * H * ceil(Lq / 32) < 2^24; with stats B * Hkv * ceil(Lk / 32) < 2^24 too; |q_offset| < 2^40.  AF3_ERR_BAD_SHAPE otherwise, from the workspace call as well.
+ * B * H * ceil(Lq / 32) < 2^24, B * Hkv < 2^23; with stats B * Hkv * ceil(Lk / 32) < 2^24 too; |q_offset| < 2^40.  AF3_ERR_BAD_SHAPE otherwise, from the workspace call as well.
  */
 typedef struct af3_diff_attention_params {
 	const void*    q;

@@ -138,7 +138,8 @@ def test_differential_attention_sizes_at_their_limits(lib):
     size = lambda **kw: lib.af3_diff_attention_workspace_bytes(ctypes.byref(_diff(**kw)))
     back = lambda **kw: lib.af3_diff_attention_backward_workspace_bytes(ctypes.byref(_diff(**kw)))
     full = 1 << 24
-    for under, over in (({"B": full // 2 - 1, "H": 2, "Hkv": 1, "Lq": 32, "Lk": 1}, {"B": full // 2, "H": 2, "Hkv": 1, "Lq": 32, "Lk": 1}),
+    for under, over in (({"B": full // 4 - 1, "H": 4, "Hkv": 1, "Lq": 32, "Lk": 1}, {"B": full // 4, "H": 4, "Hkv": 1, "Lq": 32, "Lk": 1}),
+                        ({"B": (1 << 23) - 1, "H": 1, "Hkv": 1, "Lq": 20, "Lk": 1}, {"B": 1 << 23, "H": 1, "Hkv": 1, "Lq": 20, "Lk": 1}),
                         ({"B": 1, "H": (1 << 15) - 1, "Hkv": 1, "Lq": 1, "Lk": 1}, {"B": 1, "H": 1 << 15, "Hkv": 1, "Lq": 1, "Lk": 1}),
                         ({"B": 1, "H": 511, "Hkv": 1, "Lq": 1 << 20, "Lk": 1}, {"B": 1, "H": 1 << 10, "Hkv": 1, "Lq": 1 << 20, "Lk": 1}),
                         ({"B": 1, "H": 1, "Hkv": 1, "Lq": 1, "Lk": (1 << 29) - 32}, {"B": 1, "H": 1, "Hkv": 1, "Lq": 1, "Lk": 1 << 30})):

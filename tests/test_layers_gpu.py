@@ -585,6 +585,8 @@ def test_differential_attention_refuses(af3, host, native):
             af3.differential_attention(*args, **kw)
     with pytest.raises((RuntimeError, ValueError)):
         af3.differential_attention(q, k.cpu(), v, lam)
+    with pytest.raises(TypeError, match="lam must be a tensor"):
+        af3.differential_attention(q, k, v, 0.8)
 
 
 # ---- norms around a block -----------------------------------------------------------------------------------------------------
@@ -889,6 +891,33 @@ def test_residual_norm_rows_far_apart(af3):
     far.copy_(grads[1])
     assert all(torch.equal(a, b) for a, b in zip(want.values(), norm_run(af3, t, (grads[0], far)).values()))
     del far
+    gc.collect()
+    torch.cuda.empty_cache()
+
+
+def test_residual_norm_of_more_rows_than_a_grid_has_on_one_side(af3):
+    rows, C = (1 << 28) + 5, 8
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free memory")
+    y = torch.empty(rows, C, dtype=BF16, device="cuda")
+    piece = torch.randn(1 << 20, C).to(BF16).cuda()
+    for at in range(0, rows, 1 << 20):
+        n = min(1 << 20, rows - at)
+        y[at:at + n] = piece[:n]
+    want = af3.residual_norm(None, piece)[1]
+    y.requires_grad_(True)
+    out, normed = af3.residual_norm(None, y)
+    for at in (0, 1 << 27, rows - 5):
+        n = min(1 << 20, rows - at)
+        assert torch.equal(out[at:at + n], piece[:n]) and torch.equal(normed[at:at + n], want[:n])
+    d = torch.autograd.grad(normed, y, y.detach())[0]
+    del out, normed
+    leaf = piece.detach().requires_grad_(True)
+    back = torch.autograd.grad(af3.residual_norm(None, leaf)[1], leaf, piece)[0]
+    for at in (0, 1 << 27, rows - 5):
+        n = min(1 << 20, rows - at)
+        assert torch.equal(d[at:at + n], back[:n])
+    del d, y
     gc.collect()
     torch.cuda.empty_cache()
 
