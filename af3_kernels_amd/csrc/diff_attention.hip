@@ -4,6 +4,9 @@
 // Per 32 query rows and 32 keys and map:  S^T[key][row] = K . Q^T,  O^T[column][row] += V^T . P^T,  as in cross_attention.hip: a lane holds one query row, the half-waves 16
 // keys each.  The two maps are different wavefronts' (both maps' sums of twice D columns would leave one wavefront to a SIMD), which share the tiles of V; each keeps its own
 // running maximum and sum, and the difference is taken at the end, since neither sum is known before.
+// Bound by its vector and matrix instructions, which take turns, and by waits of wavefronts that share tiles: 2 x 16 (4) x 4096 x 64 causal 288 us, 716 TFLOP/s (a large product of the
+// library: 1306); 4 x 8 x 1024 x 128 92 us, 560.  Workgroups of 4 wavefronts, two to a compute unit, gain 7 % where a launch is short (68 us for 73 at 4 x 12 x 1024 x 64 causal) and
+// lose up to 40 % (128 columns).
 #include "diff_tiles.hpp"
 
 #include <math.h>
@@ -438,7 +441,8 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 // 16 rows: lanes 0 .. 15 of each half have the first map's, the others the second's; both products of K are taken for all and each lane keeps its own map's logits, so that softmax
 // and the product with V are there once.  K comes straight from memory as the products' operand, V by way of LDS of the wavefront's own, 32 keys at a time: wavefronts wait for nobody
 // until the end, and 16 KB (D = 64) of each are on their way while it works.  P in two terms.  One token of 32 requests over 1491 keys (16 heads on 4, D = 64): 34.5 us with the kernel
-// above, whose 8 wavefronts share tiles, 25.7.
+// above, whose 8 wavefronts share tiles, 25.5 with this one; over 8192 keys 143 and 105 (5.1 TB/s).  A step of 128 keys takes 2 us (D = 64; 3 at D = 128) wherever its bytes come in
+// time, so a long axis of few requests goes over parts of one step: 8192 keys of one request 27 us in 32 parts of a join that branched, 15 now.
 template <typename T, int DP>
 struct token_shape {
 	static constexpr int DV = 2 * DP, TILE = 32 * tile<T, DV>::STRIDE, AT_ONCE = DV * (int)sizeof(T) / 128, LINE = 32 * AT_ONCE + 4, TABLE = 32 * LINE * 4;   // a tile of V; as many columns of results as have its room: of a wavefront

@@ -279,7 +279,7 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 
 // What the kernel with query rows in tiles keeps of each row of a tile in LDS: d1 and d2, and per map the whole reference (bf16), maximum and 1 / sum (fp32 and tiles with
 // a row far from zero).  Behind them a word per 64 rows that says whether there is one.  (As a further step of the products instead, three bf16 terms to a number, they were
-// no faster: 236 us for 226 at 4 x 8 (2) x 1491 x 64, 230 for 190 at 4 x 8 x 1024 x 128.)
+// no faster, both maps to a wavefront: 236 us for 226 at 4 x 8 (2) x 1491 x 64, 230 for 190 at 4 x 8 x 1024 x 128.)
 enum { LESS = 0, TAKEN = 2, MOST = 4, INVERSE = 6, ROW_STATS = 8 };
 template <typename T, int QT>
 struct row_stats {

