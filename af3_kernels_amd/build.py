@@ -17,7 +17,7 @@ HOST = os.path.join(HERE, "_host.so")
 LIB = os.path.join(HERE, "libaf3_dpa.so")
 SOURCES = ["api.hip", "dpa_generic.hip", "dpa_mfma.hip", "dpa_mfma_rows.hip", "dpa_strip.hip", "dpa_mfma_f32.hip", "dpa_mfma_fp8.hip", "elementwise.hip", "pair_bias.hip", "glu.hip", "projection.hip", "grid_project.hip",
            "cross_attention.hip", "cross_attention_grad.hip", "position_bias.hip", "rotary.hip", "residual_norm.hip", "diff_attention.hip", "diff_attention_grad.hip"]
-HEADERS = [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "mfma_helpers.hpp"), os.path.join(CSRC, "cross_tiles.hpp"), os.path.join(CSRC, "diff_tiles.hpp"), os.path.join(HERE, "..", "include", "af3_dpa.h")]
+HEADERS = [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "mfma_helpers.hpp"), os.path.join(CSRC, "cross_tiles.hpp"), os.path.join(CSRC, "diff_tiles.hpp"), os.path.join(CSRC, "launch_grid.hpp"), os.path.join(HERE, "..", "include", "af3_dpa.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # packed-fp32 ops are switched off for device code; the host pass warns that it does not know
 # the feature, which is harmless.

@@ -58,8 +58,6 @@ struct fused_grid_args {
 
 // Status of the launch just enqueued.  A device this library carries no code for (anything but gfx950) shows up
 // here as "no binary for this GPU" / "invalid device function" and is reported as such, not as a generic launch failure.
-// n workgroups as a grid whose sides, times 1024 threads, stay inside the 32 bits that a launch has for each: workgroup y * gridDim.x + x, those from n on have nothing to do
-inline dim3 grid_of(int64_t n) { return n <= (1 << 20) ? dim3((uint32_t)n) : dim3(1u << 20, (uint32_t)((n + (1 << 20) - 1) >> 20)); }
 inline int launch_status() {
 	const hipError_t e = hipGetLastError();
 	if(e == hipSuccess) return AF3_OK;

@@ -9,6 +9,7 @@
 //   diff_lam_kernel   the sums of d2, and of the rows of P2 * (dP - d2): those would be zero, but for what d2 misses by the forward pass's probabilities, rounded to bf16 as they are
 //                     there.  dlam is a sum of many rows' d2 that mostly cancel: without that it was off by up to 0.008 of itself in sums over 300 rows (with: 1e-6 before its last rounding).
 #include "diff_tiles.hpp"
+#include "launch_grid.hpp"
 
 #include <math.h>
 

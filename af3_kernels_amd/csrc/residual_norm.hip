@@ -8,6 +8,7 @@
 // a fixed order.
 // 4 x 2048 rows of 4096 channels in bf16, all of it: 165 us for 108 that a copy of the same bytes takes, each read and written once; the gradient reads x and y again.  Rows of more than
 // 8192 channels spill in the gradient's kernel, whose 1024 threads have 128 registers each.
+#include "launch_grid.hpp"
 #include "mfma_helpers.hpp"
 
 // (products and sums are fused where fmaf says so: the kernels' instantiations then agree to the last bit, whichever gradients are wanted)
