@@ -26,18 +26,22 @@ struct forward_args {
 	float*   part_stat;            // ... [splits][2][B * Hkv * G * Lq][2] (maximum, sum); sum 0: no live key in the part, and nothing written
 };
 
-// what a result loses by its rounding to bf16, itself as bf16: the gradient's row sums then have the result to 16 bits.  which: 0 of out, 1 of the second map's own
+// eight results side by side, from column d on, those below D
 template <typename T>
-__device__ __forceinline__ void store_residual(const af3_diff_attention_params& p, int which, int64_t row, int d, const float (&v)[16]) {
-	if constexpr(sizeof(T) == 2) {
-		if(!p.residuals) return;
-		float r[16];
+__device__ __forceinline__ void store_eight(T* row, int d, int D, const float (&v)[8]) {
+	constexpr int E = kind<T>::E;
+	if(D % E == 0) {
 #pragma unroll
-		for(int i = 0; i < 16; i++) r[i] = v[i] - (float)(__bf16)v[i];
-		store_columns(static_cast<T*>(p.residuals) + (which * p.B * p.H * p.Lq + row) * p.Dv, d, (int)p.Dv, r);
+		for(int i = 0; i < 8 / E; i++)
+			if(d + E * i < D) store16(row + d + E * i, kind<T>::pack(v + E * i));
+	} else {
+#pragma unroll
+		for(int e = 0; e < 8; e++)
+			if(d + e < D) row[d + e] = kind<T>::bits(v[e]);
 	}
 }
 
+// (what a result loses by its rounding to bf16 is left as bf16 itself: the gradient's row sums then have the result to 16 bits)
 // one column of a result, and of the second map's own
 template <typename T>
 __device__ __forceinline__ void store_result(const af3_diff_attention_params& p, int64_t b, int64_t h, int64_t qi, int64_t row, int column, float v, float second) {
@@ -152,7 +156,8 @@ struct forward_shape {
 	static constexpr int KTILE = KT * tile<T, DP>::STRIDE, VTILE = KT * tile<T, DV>::STRIDE, SET = 2 * KTILE + VTILE;
 	static constexpr int BUFFERS = 2 * SET <= 65536 ? 2 : 1;
 	static constexpr int LINE = DV + 4, TABLE = 32 * LINE * 4;   // results of 32 rows on their way to another wavefront
-	static constexpr int LDS = BUFFERS * SET > 4 * TABLE ? BUFFERS * SET : 4 * TABLE;
+	static constexpr int PASS = 2, RESULT_LINE = 32 * PASS + 4, RESULTS = 2 * GROUPS * 32 * RESULT_LINE * 4;   // both maps' results, 64 columns of them
+	static constexpr int JOIN = KW > 1 ? 4 * TABLE : 0, LEAST = JOIN > RESULTS ? JOIN : RESULTS, LDS = BUFFERS * SET > LEAST ? BUFFERS * SET : LEAST;
 };
 
 // HALF: V comes as diff_values_kernel has laid it out
@@ -167,6 +172,8 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 	extern __shared__ __align__(16) unsigned char smem[];
 	__shared__ live_keys<KT> live;
 	__shared__ float         stat[8][32][2];
+	__shared__ int64_t       out_at[S::ROWS], row_at[S::ROWS];   // of the rows: where their results go, -1: no row
+	__shared__ float         lam_at[S::ROWS];
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int map = wave & 1, kwave = (wave >> 1) % KW, group = (wave >> 1) / KW;
@@ -401,38 +408,52 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 		float* const st = p.stats + 2 * ((b * 2 * p.H + 2 * h + map) * p.Lq + qi);
 		st[0] = m, st[1] = inv;
 	}
-	// the second map's result by way of LDS to the wavefront that has the first one
-	if constexpr(KW == 1) __syncthreads();
-	if(map == 1) {
-		const float by = inv_units * lam_of(p, h);
-#pragma unroll
-		for(int db = 0; db < TV::BLOCKS; db++) {
-			if(db % KW != kwave) continue;
-			put(tables + group * (S::TABLE / 4), db, by);
-			if(p.second && ok) {
-				float v[16];
-#pragma unroll
-				for(int r = 0; r < 16; r++) v[r] = o[db][r] * inv_units;
-				store_columns(static_cast<T*>(p.second) + row * Dv, 32 * db + 16 * half, Dv, v);
-				store_residual<T>(p, 1, row, 32 * db + 16 * half, v);
-			}
-		}
+	// Both maps' results by way of LDS, 64 columns at a time, from where eight of a row are stored in one go and the row by lanes side by side (by the lanes that have them, 16 columns
+	// of 32 rows at once, 4 x 12 x 1024 rows over 64 keys with the four results that a gradient needs took 28 us, so 24; 4 x 8 x 1024 x 128 without them 92 and 85).
+	if(map == 0 && kwave == 0 && half == 0) {
+		const int at = 32 * group + lane;
+		out_at[at] = ok ? b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2] : -1;
+		row_at[at] = row, lam_at[at] = l == 0.f ? 0.f : lam_of(p, h);
 	}
-	__syncthreads();
-	if(map == 1 || !ok) return;
-	T* const out = static_cast<T*>(p.out) + b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2];
+	constexpr int PASS = S::PASS, LINE = S::RESULT_LINE, PIECES = 4 * PASS;
+	float* const  mine = tables + (2 * group + map) * (32 * LINE) + (lane & 31) * LINE + 16 * half;
 #pragma unroll
-	for(int db = 0; db < TV::BLOCKS; db++) {
-		if(db % KW != kwave) continue;
-		float v[16];
+	for(int first = 0; first < TV::BLOCKS; first += PASS) {
+		if(32 * first >= Dv) break;
+		__syncthreads();
 #pragma unroll
-		for(int e = 0; e < 4; e++) {
-			const f32x4 other = *reinterpret_cast<const f32x4*>(tables + group * (S::TABLE / 4) + line + 32 * db + 4 * e);
+		for(int j = 0; j < PASS; j++) {
+			const int db = first + j;
+			if(db % KW != kwave) continue;
 #pragma unroll
-			for(int c = 0; c < 4; c++) v[4 * e + c] = l == 0.f ? 0.f : __builtin_fmaf(o[db][4 * e + c], inv_units, -other[c]);
+			for(int e = 0; e < 4; e++)
+				*reinterpret_cast<f32x4*>(mine + 32 * j + 4 * e) = f32x4{o[db][4 * e] * inv_units, o[db][4 * e + 1] * inv_units, o[db][4 * e + 2] * inv_units, o[db][4 * e + 3] * inv_units};
 		}
-		store_columns(out, 32 * db + 16 * half, Dv, v);
-		store_residual<T>(p, 0, row, 32 * db + 16 * half, v);
+		__syncthreads();
+		for(int n = threadIdx.x; n < S::ROWS * PIECES; n += NT) {
+			const int     at = n / PIECES, column = 8 * (n - at * PIECES), d = 32 * first + column;
+			const int64_t to = out_at[at], lost_row = row_at[at];
+			if(to < 0 || d >= Dv) continue;
+			const float* const from = tables + 2 * (at / 32) * (32 * LINE) + (at & 31) * LINE + column;
+			const float        lam = lam_at[at];
+			float              v[8], second[8];
+#pragma unroll
+			for(int i = 0; i < 2; i++) {
+				const f32x4 one = *reinterpret_cast<const f32x4*>(from + 4 * i), two = *reinterpret_cast<const f32x4*>(from + 32 * LINE + 4 * i);
+#pragma unroll
+				for(int e = 0; e < 4; e++) second[4 * i + e] = two[e], v[4 * i + e] = __builtin_fmaf(-lam, two[e], one[e]);
+			}
+			store_eight(static_cast<T*>(p.out) + to, d, Dv, v);
+			if(!p.second) continue;
+			store_eight(static_cast<T*>(p.second) + lost_row * Dv, d, Dv, second);
+			if constexpr(sizeof(T) == 2)
+				if(p.residuals) {
+#pragma unroll
+					for(int e = 0; e < 8; e++) v[e] -= (float)(__bf16)v[e], second[e] -= (float)(__bf16)second[e];
+					T* const lost = static_cast<T*>(p.residuals) + lost_row * Dv;
+					store_eight(lost, d, Dv, v), store_eight(lost + p.B * p.H * p.Lq * Dv, d, Dv, second);
+				}
+		}
 	}
 }
 
