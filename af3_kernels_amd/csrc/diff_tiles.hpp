@@ -23,6 +23,23 @@ struct row_place {
 __device__ __forceinline__ float lam_of(const af3_diff_attention_params& p, int64_t h) {
 	return p.lam_dtype == AF3_F32 ? static_cast<const float*>(p.lam)[h * p.lam_stride] : bf16_bits_to_f32(static_cast<const uint16_t*>(p.lam)[h * p.lam_stride]);
 }
+// Which pair and piece a workgroup works on: as `share` has it, pair after pair, or, where some pieces are longer (causal), piece after piece over all pairs, so that a launch begins with
+// the longest pieces of every pair and not of the first few.  4 x 12 x 1024 x 64: forward 71 us and so 55, dK and dV 107 and 78; 8 x 16 x 2048 x 64, whose pairs' keys are four times
+// an XCD's L2 by then: 405 and 346, 696 and 582.
+struct dealt {
+	uint32_t pair, piece;
+	__device__ __forceinline__ dealt(uint32_t i, uint32_t pairs, uint32_t each, bool by_piece) {
+		if(!by_piece) {
+			const share s(i, pairs, each);
+			pair = s.pair, piece = s.piece;
+		} else if((pairs & 7u) == 0u) {   // (a pair on one XCD, those of a turn not always in the same order)
+			const uint32_t turns = pairs >> 3, j = i >> 3, turn = j % turns;
+			piece = j / turns, pair = 8u * turn + (((i & 7u) - turn) & 7u);
+		} else {
+			piece = i / pairs, pair = i - piece * pairs;
+		}
+	}
+};
 // ---- rows on their way ----
 // The kernels take rows that are whole 16-byte pieces, no further apart than 32 bits reach over a tile; the host lays others out anew (diff_pack_kernel).  With the other way of reading
 // beside it in the same loop, as cross_tiles.hpp's passage has it, dK/dV held 756 branches and twice its scalars in vector registers' lanes, and took four times as long.
