@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int map = wave & 1, kwave = (wave >> 1) % KW, group = (wave >> 1) / KW;
-	const dealt    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.row_tiles * a.splits, p.causal != 0);
-	const uint32_t split = own.piece / a.row_tiles, row_tile = a.row_tiles - 1 - (own.piece - split * a.row_tiles);   // (causal: those with the most keys first)
+	const dealt    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.row_tiles, a.splits, p.causal != 0);
+	const uint32_t split = own.split, row_tile = a.row_tiles - 1 - own.tile;   // (causal: those with the most keys first)
 	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
 	const int64_t G = p.H / p.Hkv, rows = G * p.Lq;
 	const int     Dv = (int)p.Dv;

@@ -137,8 +137,8 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int map0 = MAPS == 2 ? 0 : wave & 1, place = MAPS == 2 ? wave : wave >> 1, kwave = place % KW, group = place / KW;   // (map0: the wavefront's first map)
-	const dealt    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.tiles * a.splits, p.causal != 0);
-	const uint32_t split = own.piece / a.tiles, row_tile = a.tiles - 1 - (own.piece - split * a.tiles);
+	const dealt    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.tiles, a.splits, p.causal != 0);
+	const uint32_t split = own.split, row_tile = a.tiles - 1 - own.tile;
 	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
 	const int64_t G = p.H / p.Hkv, rows = G * p.Lq;
 	const int     D = (int)p.D;
@@ -352,8 +352,8 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int map0 = MAPS == 2 ? 0 : wave & 1, in_group = MAPS == 2 ? wave : wave >> 1, rwave = in_group % RW, group = in_group / RW;   // (map0: the wavefront's first map)
-	const dealt    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.tiles * a.splits, p.causal != 0);
-	const uint32_t split = own.piece / a.tiles, key_tile = own.piece - split * a.tiles;   // (causal: the first keys have the most rows)
+	const dealt    own((uint32_t)blockIdx.x, (uint32_t)(p.B * p.Hkv), a.tiles, a.splits, p.causal != 0);
+	const uint32_t split = own.split, key_tile = own.tile;   // (causal: the first keys have the most rows)
 	const int64_t  b = own.pair / (uint32_t)p.Hkv, hk = own.pair - (uint32_t)b * (uint32_t)p.Hkv;
 	const int64_t G = p.H / p.Hkv;
 
