@@ -4,8 +4,8 @@
 // Per 32 query rows and 32 keys and map:  S^T[key][row] = K . Q^T,  O^T[column][row] += V^T . P^T,  as in cross_attention.hip: a lane holds one query row, the half-waves 16
 // keys each.  The two maps are different wavefronts' (both maps' sums of twice D columns would leave one wavefront to a SIMD), which share the tiles of V; each keeps its own
 // running maximum and sum, and the difference is taken at the end, since neither sum is known before.
-// Bound by its vector and matrix instructions, which take turns, and by waits of wavefronts that share tiles: 2 x 16 (4) x 4096 x 64 causal 288 us, 716 TFLOP/s (a large product of the
-// library: 1306); 4 x 8 x 1024 x 128 92 us, 560.  Workgroups of 4 wavefronts, two to a compute unit, gain 7 % where a launch is short (68 us for 73 at 4 x 12 x 1024 x 64 causal) and
+// Bound by its vector and matrix instructions, which take turns, and by waits of wavefronts that share tiles: 2 x 16 (4) x 4096 x 64 causal 285 us, 725 TFLOP/s (a large product of the
+// library: 1306); 4 x 8 x 1024 x 128 85 us, 610.  Workgroups of 4 wavefronts, two to a compute unit, gain 7 % where a launch is short (68 us for 73 at 4 x 12 x 1024 x 64 causal, dealt out pair by pair) and
 // lose up to 40 % (128 columns).
 #include "diff_tiles.hpp"
 

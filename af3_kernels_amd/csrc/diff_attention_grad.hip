@@ -109,7 +109,7 @@ constexpr int tile_rows(int bytes, int sharing) { return sharing == 4 || bytes <
 constexpr int dq_maps(int bytes) { return bytes <= 128 ? 2 : 1; }
 constexpr int dq_threads(int bytes) { return 512; }
 // dK and dV of 128-byte rows: both maps in a wavefront need 370 registers, one wavefront to a SIMD; with one map each, and dP computed by both, there are two (2 x 16 (4) x 4096 x 64
-// causal 761 -> 579 us, in workgroups of 256 threads 776).  Where wavefronts share their keys the pairs' exchange would be between twice as many.
+// causal 761 -> 579 us, in workgroups of 256 threads 776; 540 with the tiles dealt out longest first).  Where wavefronts share their keys the pairs' exchange would be between twice as many.
 constexpr int dkv_maps(int bytes, int sharing) { return bytes <= 64 || sharing > 1 ? 2 : 1; }
 constexpr int dkv_threads(int bytes, int sharing) { return bytes == 128 && sharing == 1 ? 512 : 256; }
 
@@ -621,6 +621,7 @@ double counting(const af3_diff_attention_params& p) {
 template <typename U, typename F>
 cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double counts, int64_t slots, double load_us, U block_us, double part_bytes, F steps) {
 	constexpr double JOIN_US = 6.0, BYTES_PER_US = 2e6;
+	const double tail = counts < 1.0 && by_tile(groups) ? 0.5 : 0.8;   // of the longest, behind all of them dealt out evenly (8 x 16 x 768 x 64 causal, dQ: 117 us with 0.8 for both, 90)
 	cut    best{};
 	double best_us = 0.0;
 	for(int sharing = 1; sharing <= (bytes > 128 ? 1 : 4); sharing *= 2) {
@@ -629,7 +630,7 @@ cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double cou
 		for(int64_t parts = 1; parts <= 64 && (parts == 1 || 2 * parts <= n + 1); parts++) {
 			const double longest = (double)over(n, parts), all = (double)workgroups * n * counts / slots;
 			if(workgroups * parts > 0x7fffff && (sharing > 1 || parts > 1)) break;   // (times 512 threads inside 32 bits: so are those of the first choice, by what validate_diff_attention takes)
-			const double us = (workgroups * parts <= slots ? longest : longest > all + 0.8 * longest ? longest : all + 0.8 * longest) * tile_us + (parts > 1 ? JOIN_US + parts * 2.0 * part_bytes / BYTES_PER_US : 0.0);
+			const double us = (workgroups * parts <= slots ? longest : longest > all + tail * longest ? longest : all + tail * longest) * tile_us + (parts > 1 ? JOIN_US + parts * 2.0 * part_bytes / BYTES_PER_US : 0.0);
 			if(best_us == 0.0 || us < best_us) best_us = us, best.sharing = sharing, best.tiles = (uint32_t)tiles, best.part = over(n, parts), best.splits = (uint32_t)over(n, best.part);
 		}
 	}

@@ -25,17 +25,18 @@ __device__ __forceinline__ float lam_of(const af3_diff_attention_params& p, int6
 }
 // Which pair, tile (the longest first) and part a workgroup works on.  Where all are alike: as `share` has it, pair after pair.  Where some tiles are longer (causal): tile after tile over all
 // pairs, so that a launch begins with the longest tiles of every pair and not of the first few.  4 x 12 x 1024 x 64: forward 71 us and so 55, dK and dV 107 and 78; 8 x 16 x 2048 x 64, whose
-// pairs' keys are four times an XCD's L2 by then: 405 and 346, 696 and 582.  Pairs that do not come in eights go over the XCDs as they come, and their parts one after the other (2 x 14 x
+// pairs' keys are four times an XCD's L2 by then: 405 and 340, 696 and 576.  Pairs that do not come in eights go over the XCDs as they come, and their parts one after the other (2 x 14 x
 // 1491 x 64: 84 and 65, 129 and 99); fewer than eight gain nothing by it (fp32, 4 pairs of 1024 x 32: 91 and 108).
+__host__ __device__ constexpr bool by_tile(int64_t pairs) { return pairs % 8 == 0 || pairs > 8; }
 struct dealt {
 	uint32_t pair, tile, split;
 	__device__ __forceinline__ dealt(uint32_t i, uint32_t pairs, uint32_t tiles, uint32_t splits, bool causal) {
-		const bool  eights = (pairs & 7u) == 0u, by_tile = causal && (eights || pairs > 8u);
+		const bool  eights = (pairs & 7u) == 0u, row_first = causal && by_tile(pairs);
 		const share whole(i, pairs, tiles * splits);
 		// (eights: a pair on one XCD)
 		const uint32_t across = eights ? pairs >> 3 : pairs, j = eights ? i >> 3 : i, row = j / across, turn = j - row * across;
-		const uint32_t piece = by_tile ? row : whole.piece, in_row = causal && eights ? splits : tiles, outer = piece / in_row, inner = piece - outer * in_row;
-		pair  = __builtin_amdgcn_readfirstlane(by_tile ? (eights ? 8u * turn + (((i & 7u) - turn) & 7u) : turn) : whole.pair);
+		const uint32_t piece = row_first ? row : whole.piece, in_row = causal && eights ? splits : tiles, outer = piece / in_row, inner = piece - outer * in_row;
+		pair  = __builtin_amdgcn_readfirstlane(row_first ? (eights ? 8u * turn + (((i & 7u) - turn) & 7u) : turn) : whole.pair);
 		tile  = __builtin_amdgcn_readfirstlane(causal && eights ? outer : inner);
 		split = __builtin_amdgcn_readfirstlane(causal && eights ? inner : outer);
 	}
