@@ -343,6 +343,13 @@ def test_a_long_axis_of_keys_in_parts(af3, Lq, dtype):
     assert all((x == 0).all() for x in got.values())
 
 
+@pytest.mark.parametrize("B,H,Hkv,L,D,dtype", [(2, 8, 4, 1100, 32, BF16), (3, 3, 3, 900, 64, BF16), (1, 16, 8, 700, 128, BF16), (1, 8, 8, 500, 32, F32), (1, 11, 11, 400, 16, F32), (2, 2, 1, 1300, 64, BF16)])
+def test_causal_tiles_of_every_length(af3, B, H, Hkv, L, D, dtype):
+    """However the tiles of a causal launch are dealt out: pairs in eights, more than eight, fewer; parts of the long axes among them."""
+    t = diff_inputs(B, H, Hkv, L, L, D, 2 * D, dtype, 23, "none")
+    diff_compare(diff_run(af3, *t, causal=True), *t, causal=True)
+
+
 def test_a_long_axis_of_queries_in_parts(af3):
     for dtype in (BF16, F32):
         t = diff_inputs(1, 2, 1, 4000, 33, 32, 64, dtype, 7, "random")
