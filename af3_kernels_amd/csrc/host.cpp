@@ -1190,21 +1190,22 @@ struct norm_function : torch::autograd::Function<norm_function> {
 				if(grad_out[i].defined()) g[i] = inner_1(grad_out[i]) && row_stride(grad_out[i]) >= 0 ? grad_out[i] : grad_out[i].contiguous();
 			if(g[0].defined()) o.grad_out = g[0].const_data_ptr(), o.grad_out_stride = row_stride(g[0]);
 			if(g[1].defined()) o.grad_normed = g[1].const_data_ptr(), o.grad_normed_stride = row_stride(g[1]);
+			const bool reached = g[0].defined() || g[1].defined();   // (a consumer of both results may have no gradient for either)
 			bool   any  = false;
 			size_t edge = 0;   // (tensors that were not given have none)
-			auto want = [&](int i, const Tensor& like, bool reached) -> void* {
+			auto want = [&](int i, const Tensor& like, bool from) -> void* {   // `from`: a gradient comes from where this one is made of
 				if(!like.defined() || !ctx->needs_input_grad(edge++)) return nullptr;
 				grads[i] = new_tensor(like.sizes(), like.scalar_type(), dev);
-				if(!reached) {
+				if(!from) {
 					grads[i].zero_();
 					return nullptr;
 				}
 				any = true;
 				return grads[i].data_ptr();
 			};
-			o.grad_x = want(0, c.x, true), o.grad_y = want(1, c.y, true), o.grad_weight = want(2, c.weight, g[1].defined()), o.grad_bias = want(3, c.bias, g[1].defined());
-			o.grad_gate = want(4, c.gate, true), o.grad_post_weight = want(5, c.post_weight, true);
-			if(any && (g[0].defined() || g[1].defined())) {
+			o.grad_x = want(0, c.x, reached), o.grad_y = want(1, c.y, reached), o.grad_weight = want(2, c.weight, g[1].defined()), o.grad_bias = want(3, c.bias, g[1].defined());
+			o.grad_gate = want(4, c.gate, reached), o.grad_post_weight = want(5, c.post_weight, reached);
+			if(any) {
 				const int64_t bytes = af3_residual_norm_backward_workspace_bytes(&p, &o);
 				raise(bytes < 0 ? (int)bytes : AF3_OK, "af3_residual_norm_backward_workspace_bytes");
 				at::DataPtr ws;
