@@ -86,10 +86,10 @@ int packing::launch(hipStream_t s) const {
 // The rounding of P to bf16 in front of its product with V would be felt more here than in one map: where the maps have much in common their difference loses size and
 // the roundings do not (lam 0.8, logits of variance 1: out off by 1.6 times its own last rounding).  In short launches, whose matrix instructions are few, P goes in two terms, the second
 // what the first one lost.  In long ones it goes as fp16, which has three bits more, and V with it: its bf16 values times a power of two, the tile's unit, are fp16 values as they stand
-// (those of 2^-22 of the tile's largest and less are off by 2^-25 / unit).  Laid out so once, rows of dropped keys as zeros, a tile is then taken as it is by all that read it.  Converted
+// (but for the smallest of a tile).  Laid out so once, rows of dropped keys as zeros, a tile is then taken as it is by all that read it.  Converted
 // where it is read instead, 2 x 16 (4) x 4096 x 64 took 352 us in place of 278 (between two barriers, with no other workgroup on the compute unit to fill them).
 constexpr int   value_rows(int dp) { return dp == 32 ? 128 : 64; }   // (a whole number of the main kernel's tiles)
-constexpr float UNIT = 256.f, UNIT_BELOW = 32768.f, UNIT_ABOVE = 0x1p-7f;   // the unit of a tile whose largest lies between these of it
+constexpr float UNIT = 256.f;   // of the sums in front of the first tile, and of tiles of which nothing else is known
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 	const f16x2 p = {(_Float16)lo, (_Float16)hi};
 	return __builtin_bit_cast(uint32_t, p);
@@ -98,9 +98,13 @@ __device__ __forceinline__ u32x4 pack_f16(const float* r) { return u32x4{pack_f1
 __device__ __forceinline__ f32x16 mma_f16(const u32x4& a, const u32x4& b, f32x16 c) {
 	return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-// a power of two that takes x to 2^8 .. 2^9 (within 2^-112 .. 2^100)
+// A tile's unit takes its largest value to 2^8 .. 2^15: bf16 values of 2^-25 of it and more are then fp16 values without a rounding, smaller ones off by 2^-33 of it at most.  Within that all tiles of
+// a pair have the same one, which suits the largest of some values all along the keys: a tile of another unit than the one before it has the sums multiplied (with the nearest unit for each
+// tile, 2 x 16 (4) x 4096 x 64 of values of 0.25 took 306 us, so 283).
+constexpr float LEAST = 256.f, MOST_UNITS = 32768.f;
+// a power of two that takes x to 2^11 .. 2^12 (x of 2^-89 and more; smaller ones, and zero, by 2^100)
 __device__ __forceinline__ float unit_for(float x) {
-	int e = 8 + 127 - (int)(__float_as_uint(x) >> 23);
+	int e = 11 + 127 - (int)(__float_as_uint(x) >> 23);
 	e     = e > 100 ? 100 : e;
 	return __uint_as_float((uint32_t)(e + 127) << 23);
 }
@@ -110,31 +114,45 @@ __global__ void __launch_bounds__(THREADS) diff_values_kernel(forward_args a) {
 	constexpr int VALUE_ROWS = value_rows(DP);
 	using P = carrier<uint16_t, 2 * DP, VALUE_ROWS, THREADS>;
 	const af3_diff_attention_params& p = a.p;
-	__shared__ uint32_t largest;
+	__shared__ float largest[2][WAVES];   // of the tile, of the pair's values that are looked at
 	const uint32_t tiles = (uint32_t)((p.Lk + VALUE_ROWS - 1) / VALUE_ROWS), pair = blockIdx.x / tiles, tile_no = blockIdx.x - pair * tiles;
 	const int64_t  b = pair / (uint32_t)p.Hkv, hk = pair - (uint32_t)b * (uint32_t)p.Hkv, row0 = (int64_t)tile_no * VALUE_ROWS;
-	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b + row0 : nullptr;
+	const uint8_t* const mask = p.key_mask ? p.key_mask + b * p.key_mask_stride_b : nullptr;
+	const uint16_t* const base = static_cast<const uint16_t*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1];
 	P v;
 	v.begin(p.v_stride[2], a.v_columns);
-	v.load(static_cast<const uint16_t*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1], row0, p.Lk);
-	if(threadIdx.x == 0) largest = 0u;
-	__syncthreads();
+	v.load(base, row0, p.Lk);
+	// (a piece of one of THREADS / CHUNKS rows for each thread)
+	const int64_t key    = P::row_of(0) * p.Lk / (THREADS / P::TL::CHUNKS);
+	const bool    column = P::col_of(0) * P::E < a.v_columns;
+	const u32x4   piece  = load16(base + key * p.v_stride[2] + (column ? P::col_of(0) * P::E : 0));
+	const bool    looked = column && (!mask || mask[key] != 0);
+	auto larger = [](float top, const u32x4& of, bool in) {   // (neither infinities nor NaN, which no unit changes)
+#pragma unroll
+		for(int e = 0; e < 8; e++) {
+			const float x = __builtin_fabsf(kind<uint16_t>::at(of, e));
+			if(in && x < INFINITY) top = __builtin_fmaxf(x, top);
+		}
+		return top;
+	};
 	float top = 0.f;
 	bool  in[P::N];
 #pragma unroll
 	for(int n = 0; n < P::N; n++) {
 		const int row = P::row_of(n);
-		in[n] = row0 + row < p.Lk && P::col_of(n) * P::E < a.v_columns && (!mask || mask[row] != 0);
-#pragma unroll
-		for(int e = 0; e < 8; e++) {
-			const float x = __builtin_fabsf(kind<uint16_t>::at(v.piece[n], e));
-			if(in[n] && x < INFINITY) top = __builtin_fmaxf(x, top);   // (neither infinities nor NaN, which no unit changes)
-		}
+		in[n] = row0 + row < p.Lk && P::col_of(n) * P::E < a.v_columns && (!mask || mask[row0 + row] != 0);
+		top   = larger(top, v.piece[n], in[n]);
 	}
-	atomicMax(&largest, __float_as_uint(top));
+	float looked_at = larger(0.f, piece, looked);
+#pragma unroll
+	for(int d = 32; d; d >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d)), looked_at = __builtin_fmaxf(looked_at, __shfl_xor(looked_at, d));
+	if((threadIdx.x & 63) == 0) largest[0][threadIdx.x >> 6] = top, largest[1][threadIdx.x >> 6] = looked_at;
 	__syncthreads();
-	top = __uint_as_float(largest);
-	const float unit = top == 0.f || (top * UNIT < UNIT_BELOW && top * UNIT >= UNIT_ABOVE) ? UNIT : unit_for(top);
+#pragma unroll
+	for(int w = 0; w < WAVES; w++) top = __builtin_fmaxf(top, largest[0][w]), looked_at = __builtin_fmaxf(looked_at, largest[1][w]);
+	// (zeros have the largest unit where the values that were looked at are zeros too: it takes nothing away from other tiles)
+	const float usual = looked_at == 0.f && top != 0.f ? UNIT : unit_for(looked_at);
+	const float unit = top == 0.f || (top * usual >= LEAST && top * usual < MOST_UNITS) ? usual : unit_for(top);
 	if(threadIdx.x == 0) a.units[blockIdx.x] = unit;
 	u32x4* const out = static_cast<u32x4*>(a.values) + (int64_t)blockIdx.x * VALUE_ROWS * P::TL::CHUNKS;
 #pragma unroll

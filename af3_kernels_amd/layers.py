@@ -240,7 +240,8 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     head h // (H // Hkv)); the result is [B, H, Lq, Dv].  lam [H], or one number for all heads (a tensor of one element): float32 or q's dtype, anything else is cast to float32.
     bfloat16: D up to 128, Dv up to 256; float32: half of that.  mask [Lk], [B, Lk] or [B, 1, 1, Lk], truthy = attend; causal: key j counts for query i if j <= i + q_offset (a
     decoder's token t: Lq = 1, q_offset = t).  softmax_scale: D^-1/2 unless given.  float32 (fp32 throughout) or bfloat16 (bf16 products, fp32 accumulation and softmax; the
-    probabilities and, in the gradient, dS are rounded to bf16 for the products that follow); k and v are cast to q's dtype.  Any strides; a new contiguous tensor.
+    probabilities and, in the gradient, dS are rounded to bf16 for the products that follow; in long calls the probabilities and v go as fp16, v in units of its tile of 64 or 128 keys: values
+    below 2^-25 of the tile's largest are rounded, by 2^-33 of it at most, and results below 2^-70 of the largest v of a call lose bits); k and v are cast to q's dtype.  Any strides; a new contiguous tensor.
 
     A key that `mask` drops has no part in the result or its gradient, whatever k and v hold there.  A query that is left without a key, by mask and causality, gives zeros and
     has no gradient (not the mean of its values as in cross_attention: of a difference nothing is left).  Keys behind a causal query have weight zero for it, which NaN and
