@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(THREADS, (DP * sizeof(T) <= 128 ? 2 : 1)) diff
 					for(int i = 0; i < 2; i++) a.part_out[((2 * (int64_t)split + i) * n_rows + first_row + row) * Dv + at] = r[i];
 				} else {
 					const float second = r[1] * inverse[16 + row];
-					store_result<T>(p, b, place.h, place.qi, (b * p.H + place.h) * p.Lq + place.qi, at, __builtin_fmaf(-lam_of(p, place.h), second, r[0] * inverse[row]), second);
+					store_result<T>(p, b, place.h, place.qi, (b * p.H + place.h) * p.Lq + place.qi, at, inverse[row] == 0.f ? 0.f : __builtin_fmaf(-lam_of(p, place.h), second, r[0] * inverse[row]), second);   // (no live key: zeros, whatever lam is)
 				}
 			}
 		}

@@ -1,4 +1,4 @@
-"""The layer operators where little or nothing is left: results that no gradient reaches, values far below one.
+"""The layer operators where little or nothing is left: results that no gradient reaches, values far below one, queries without a key.
 
 Formulas, bounds and inputs are those of test_layers_gpu.py.
 """
@@ -87,3 +87,17 @@ def test_zeros_beside_the_smallest_values(af3, Lq, B):
             small[:, :, zeros] = 0.0
             t = (q, k, small, lam, m, None)
             diff_compare({"out": af3.differential_attention(*t[:5])}, *t)
+
+
+# ---- queries without a key ----------------------------------------------------------------------------------------------------
+@HOSTS
+@TYPES
+@pytest.mark.parametrize("Lq,Lk,B", [(1, 40, 2), (1, 5000, 2), (16, 40, 3), (40, 70, 2), (40, 5000, 2), (640, 150, 9)])
+def test_queries_without_a_key_whatever_lam_is(af3, host, native, Lq, Lk, B, dtype):
+    host(native)
+    q, k, v, _, _, _ = diff_inputs(B, 4, 4, Lq, Lk, 64, 128, dtype, 43)
+    m = torch.ones(B, Lk, dtype=torch.bool, device="cuda")
+    m[1] = False
+    for worst in (math.inf, -math.inf, math.nan):
+        out = af3.differential_attention(q, k, v, torch.full((4,), worst, device="cuda"), m)
+        assert (out[1] == 0).all(), worst
