@@ -264,7 +264,7 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 	for(int i = 0; i < MAPS; i++) {
 		if constexpr(KW > 1) add_up<DP, KW>(reinterpret_cast<float*>(smem) + (MAPS == 2 ? group : 2 * group + map0) * KW * 32 * (DP + 4), kwave, lane, dq[i]);
 		if(!ok) continue;
-		const float   scale = map0 + i == 0 ? p.softmax_scale : -lam * p.softmax_scale;   // (the second map's dS is -lam times what was summed)
+		const float   scale = map0 + i == 0 ? p.softmax_scale : inv[i] == 0.f ? 0.f : -lam * p.softmax_scale;   // (the second map's dS is -lam times what was summed; no live key: zeros, whatever lam is)
 		const int64_t to = (b * 2 * p.H + 2 * h + map0 + i) * p.Lq + qi;
 #pragma unroll
 		for(int db = 0; db < TK::BLOCKS; db++) {

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_layers_gpu import BF16, HOSTS, NAMES, TYPES, af3, diff_compare, diff_inputs, host, norm_inputs  # noqa: F401
+from test_layers_gpu import BF16, HOSTS, NAMES, TYPES, af3, diff_compare, diff_inputs, diff_run, host, norm_inputs  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,17 @@ def test_queries_without_a_key_whatever_lam_is(af3, host, native, Lq, Lk, B, dty
     for worst in (math.inf, -math.inf, math.nan):
         out = af3.differential_attention(q, k, v, torch.full((4,), worst, device="cuda"), m)
         assert (out[1] == 0).all(), worst
+
+
+@TYPES
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("Lq,Lk,B", [(1, 40, 2), (40, 700, 2), (640, 150, 9)])
+def test_gradients_of_queries_without_a_key_whatever_lam_is(af3, Lq, Lk, B, D, dtype):
+    D = D if dtype == BF16 else min(D, 64)
+    q, k, v, _, _, g = diff_inputs(B, 4, 4, Lq, Lk, D, 2 * D, dtype, 44)
+    m = torch.ones(B, Lk, dtype=torch.bool, device="cuda")
+    m[1] = False
+    for worst in (math.inf, math.nan):
+        got = diff_run(af3, q, k, v, torch.full((4,), worst, device="cuda"), m, g)
+        for name in ("out", "dq", "dk", "dv"):
+            assert (got[name][1] == 0).all(), (name, worst)
