@@ -192,6 +192,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 	__shared__ float         stat[8][32][2];
 	__shared__ int64_t       out_at[S::ROWS], row_at[S::ROWS];   // of the rows: where their results go, -1: no row
 	__shared__ float         lam_at[S::ROWS];
+	__shared__ bool          any_key[2][S::ROWS];   // of the rows: whether a map has a live key
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int map = wave & 1, kwave = (wave >> 1) % KW, group = (wave >> 1) / KW;
@@ -428,6 +429,7 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 	}
 	// Both maps' results by way of LDS, 64 columns at a time, from where eight of a row are stored in one go and the row by lanes side by side (by the lanes that have them, 16 columns
 	// of 32 rows at once, 4 x 12 x 1024 rows over 64 keys with the four results that a gradient needs took 28 us, so 24; 4 x 8 x 1024 x 128 without them 92 and 85).
+	if(kwave == 0 && half == 0) any_key[map][32 * group + lane] = l != 0.f;
 	if(map == 0 && kwave == 0 && half == 0) {
 		const int at = 32 * group + lane;
 		out_at[at] = ok ? b * p.out_stride[0] + h * p.out_stride[1] + qi * p.out_stride[2] : -1;
@@ -454,12 +456,13 @@ __global__ void __launch_bounds__(NT, 2) diff_forward_kernel(forward_args a) {
 			if(to < 0 || d >= Dv) continue;
 			const float* const from = tables + 2 * (at / 32) * (32 * LINE) + (at & 31) * LINE + column;
 			const float        lam = lam_at[at];
+			const bool         live1 = any_key[0][at], live2 = any_key[1][at];   // (without one: zeros, also where other rows' keys reach the sums with weights of zero, which NaN does not heed)
 			float              v[8], second[8];
 #pragma unroll
 			for(int i = 0; i < 2; i++) {
 				const f32x4 one = *reinterpret_cast<const f32x4*>(from + 4 * i), two = *reinterpret_cast<const f32x4*>(from + 32 * LINE + 4 * i);
 #pragma unroll
-				for(int e = 0; e < 4; e++) second[4 * i + e] = two[e], v[4 * i + e] = __builtin_fmaf(-lam, two[e], one[e]);
+				for(int e = 0; e < 4; e++) second[4 * i + e] = live2 ? two[e] : 0.f, v[4 * i + e] = __builtin_fmaf(-lam, second[4 * i + e], live1 ? one[e] : 0.f);
 			}
 			store_eight(static_cast<T*>(p.out) + to, d, Dv, v);
 			if(!p.second) continue;
@@ -669,6 +672,7 @@ __global__ void __launch_bounds__(THREADS, (DP * sizeof(T) <= 128 ? 2 : 1)) diff
 			const int          row = n / PAIRS, column = 2 * (n - row * PAIRS);
 			const float* const all = reinterpret_cast<const float*>(smem) + row * S::LINE + column;
 			const row_place    place(row, rows, G, hk);
+			const float        lam = a.splits > 1 ? 0.f : lam_of(p, place.h);
 #pragma unroll
 			for(int c = 0; c < 2; c++) {
 				const int at = 32 * db + column + c;
@@ -682,8 +686,9 @@ __global__ void __launch_bounds__(THREADS, (DP * sizeof(T) <= 128 ? 2 : 1)) diff
 #pragma unroll
 					for(int i = 0; i < 2; i++) a.part_out[((2 * (int64_t)split + i) * n_rows + first_row + row) * Dv + at] = r[i];
 				} else {
-					const float second = r[1] * inverse[16 + row];
-					store_result<T>(p, b, place.h, place.qi, (b * p.H + place.h) * p.Lq + place.qi, at, inverse[row] == 0.f ? 0.f : __builtin_fmaf(-lam_of(p, place.h), second, r[0] * inverse[row]), second);   // (no live key: zeros, whatever lam is)
+					// (no live key: zeros, whatever lam is and whatever V holds at other rows' keys)
+					const float second = inverse[16 + row] == 0.f ? 0.f : r[1] * inverse[16 + row], out = inverse[row] == 0.f ? 0.f : __builtin_fmaf(-lam, second, r[0] * inverse[row]);
+					store_result<T>(p, b, place.h, place.qi, (b * p.H + place.h) * p.Lq + place.qi, at, out, second);
 				}
 			}
 		}

@@ -115,3 +115,21 @@ def test_gradients_of_queries_without_a_key_whatever_lam_is(af3, Lq, Lk, B, D, d
         got = diff_run(af3, q, k, v, torch.full((4,), worst, device="cuda"), m, g)
         for name in ("out", "dq", "dk", "dv"):
             assert (got[name][1] == 0).all(), (name, worst)
+
+
+@TYPES
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("Lq,Lk,B", [(8, 40, 2), (8, 5000, 2), (40, 70, 2), (40, 5000, 2), (640, 400, 9)])
+def test_queries_without_a_key_beside_values_that_are_not_finite(af3, Lq, Lk, B, D, dtype):
+    D = D if dtype == BF16 else min(D, 64)
+    q, k, v, lam, _, _ = diff_inputs(B, 4, 4, Lq, Lk, D, 2 * D, dtype, 45)
+    for worst in (math.nan, math.inf):
+        v2 = v.clone()
+        v2[:, :, ::3] = worst
+        out = af3.differential_attention(q, k, v2, lam, causal=True, q_offset=-5)
+        assert (out[:, :, :5] == 0).all(), worst
+        # a sequence that is padded in front: its first queries see dropped keys alone
+        m = torch.ones(B, Lk, dtype=torch.bool, device="cuda")
+        m[-1, :5] = False
+        out = af3.differential_attention(q, k, v2, lam, m, causal=True)
+        assert (out[-1, :, :5] == 0).all(), worst
