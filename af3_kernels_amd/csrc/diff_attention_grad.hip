@@ -257,7 +257,10 @@ __global__ void __launch_bounds__((dq_shape<T, DP, KW>::NT), 2) diff_dq_kernel(g
 		}
 	}
 	row_sum = sum_of_halves(row_sum);
-	if(a.short_of && ok && half == 0 && (MAPS == 2 || map0 == 1)) a.short_of[(int64_t)(split * KW + kwave) * (p.B * p.H * p.Lq) + row] = row_sum;
+	if(a.short_of && ok && half == 0 && (MAPS == 2 || map0 == 1)) {
+		a.short_of[(int64_t)(split * KW + kwave) * (p.B * p.H * p.Lq) + row] = row_sum;
+		if(inv[MAPS - 1] == 0.f) a.d2[row] = 0.f;   // (no live key: no part in lam's gradient, whatever its own is; nobody else looks at it)
+	}
 	if(!a.g.grad_q) return;
 	const float lam = lam_of(p, h);
 #pragma unroll
@@ -286,11 +289,11 @@ template <typename T, int QT>
 struct row_stats {
 	static constexpr int BYTES = ROW_STATS * QT * 4 + 16;
 	float v[ROW_STATS];   // of one row, on its way
-	__device__ __forceinline__ void load(const grad_args& a, int64_t bh, int q0) {   // bh: b * H + h
+	__device__ __forceinline__ void load(const grad_args& a, int64_t bh, int q0, int skip) {   // bh: b * H + h; rows in front of `skip` are as those that do not exist
 #pragma unroll
 		for(int i = 0; i < ROW_STATS; i++) v[i] = 0.f;
 		const int qi = q0 + (int)threadIdx.x;
-		if((int)threadIdx.x >= QT || qi >= (int)a.p.Lq) return;
+		if((int)threadIdx.x >= QT || qi >= (int)a.p.Lq || qi < skip) return;
 		const int64_t first = bh * a.p.Lq;
 		v[LESS] = a.d1[first + qi], v[LESS + 1] = a.d2[first + qi];
 #pragma unroll
@@ -348,7 +351,9 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 	using TV = tile<T, S::DV>;
 	constexpr int E = kind<T>::E, QT = S::QT, MAPS = S::MAPS;
 	const af3_diff_attention_params& p = a.p;
+	constexpr int NONE = 1 << 30;
 	extern __shared__ __align__(16) unsigned char smem[];
+	__shared__ int first_live[S::W];   // the wavefronts' first keys that count, from key0 on
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int map0 = MAPS == 2 ? 0 : wave & 1, in_group = MAPS == 2 ? wave : wave >> 1, rwave = in_group % RW, group = in_group / RW;   // (map0: the wavefront's first map)
@@ -364,7 +369,9 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 #pragma unroll
 	for(int i = 0; i < MAPS; i++) load_rows<T, DP>(kf[i], static_cast<const T*>(p.k) + b * p.k_stride[0] + (2 * hk + map0 + i) * p.k_stride[1] + (in ? key : 0) * p.k_stride[2], in, a.columns, lane);
 	load_rows<T, S::DV>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], in, a.v_columns, lane);
-	const bool work = __any(lives);   // (of this wavefront)
+	const uint64_t living = __ballot(lives);
+	const bool     work = living != 0;   // (of this wavefront)
+	if(lane == 0) first_live[wave] = work ? 32 * group + __builtin_ctzll(living) : NONE;
 
 	f32x16 dk[MAPS][TK::BLOCKS], dv[S::VBLOCKS];
 	const int vblock0 = MAPS == 2 ? 0 : map0 * S::VBLOCKS;   // the wavefront's first block of dV's columns
@@ -377,8 +384,15 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 
 	// Tiles of query rows, head after head: tile `at` of head `head` of the group, counted head * q_tiles + at (below 2^25).
 	const int q_tiles = (int)((p.Lq + QT - 1) / QT), n = (int)G * q_tiles, Lq = (int)p.Lq;
-	// (causal: queries in front of the workgroup's first key have nothing of it)
-	const int from = p.causal && key0 > p.q_offset ? (int)((key0 - p.q_offset) / QT < q_tiles ? (key0 - p.q_offset) / QT : q_tiles) : 0;
+	__syncthreads();
+	int first = NONE;
+#pragma unroll
+	for(int w = 0; w < S::W; w++) first = first < first_live[w] ? first : first_live[w];
+	first = __builtin_amdgcn_readfirstlane(first);
+	// Causal: queries in front of the workgroup's first key that counts have nothing of its keys.  Those of them that share a tile with others become zeros: queries without a key are
+	// among them, which have no part in a gradient, and whatever stands there would meet weights of zero, which NaN does not heed.
+	const int64_t skipped = p.causal ? key0 + first - p.q_offset : 0;
+	const int     skip = skipped <= 0 ? 0 : skipped < Lq ? (int)skipped : Lq, from = skip == Lq ? q_tiles : skip / QT;
 	const int last = (int)((int64_t)(split + 1) * a.part < n ? (int64_t)(split + 1) * a.part : n);
 	const typename TK::reader at_q_(lane);
 	const typename TV::reader at_g_(lane);
@@ -392,15 +406,14 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 	auto fetch = [&](int head, int at) {
 		const T* const q = qb + 2 * head * p.q_stride[1];
 		pq[0].load(q, at * QT, Lq), pq[1].load(q + p.q_stride[1], at * QT, Lq, pq[0]), pg.load(gb + head * a.g.grad_out_stride[1], at * QT, Lq);
-		rs.load(a, b * p.H + hk * G + head, at * QT);
+		rs.load(a, b * p.H + hk * G + head, at * QT, skip);
 	};
 	int head = (int)((int64_t)split * a.part) / q_tiles, at = (int)((int64_t)split * a.part) - head * q_tiles;
 	if(at < from) at = from;
 	if(at >= q_tiles) head++, at = from;
 	int buffer = 0;
 	// (a workgroup none of whose keys counts has nothing to read)
-	const bool any = __syncthreads_or(work);
-	bool more = any && from < q_tiles && head * q_tiles + at < last;
+	bool more = first != NONE && from < q_tiles && head * q_tiles + at < last;
 	if(more) fetch(head, at);
 	while(more) {
 		unsigned char* const qs = smem + buffer * S::SET;
@@ -409,9 +422,11 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 		const int            q0 = at * QT, left = Lq - q0;
 		const float          lam = lam_of(p, hk * G + head);
 		if constexpr(S::BUFFERS == 1) __syncthreads();
-		pq[0].store(qs, left >= QT, [&](int r) { return r < left; });
-		pq[1].store(qs + S::QTILE, left >= QT, [&](int r) { return r < left; }, a.columns);
-		pg.store(gs, left >= QT, [&](int r) { return r < left; });
+		const bool all = left >= QT && q0 >= skip;
+		auto       exists = [&](int r) { return r < left && q0 + r >= skip; };
+		pq[0].store(qs, all, exists);
+		pq[1].store(qs + S::QTILE, all, exists, a.columns);
+		pg.store(gs, all, exists);
 		rs.store(st, a.factor);
 		__syncthreads();
 		if(++at == q_tiles) head++, at = from;

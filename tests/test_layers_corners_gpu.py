@@ -133,3 +133,22 @@ def test_queries_without_a_key_beside_values_that_are_not_finite(af3, Lq, Lk, B,
         m[-1, :5] = False
         out = af3.differential_attention(q, k, v2, lam, m, causal=True)
         assert (out[-1, :, :5] == 0).all(), worst
+
+
+@TYPES
+@pytest.mark.parametrize("H,Hkv,Lq,Lk,B,D", [(4, 4, 8, 40, 2, 64), (4, 2, 40, 70, 3, 32), (4, 4, 150, 150, 9, 64), (8, 8, 300, 300, 9, 64), (4, 1, 130, 130, 2, 128), (6, 2, 260, 700, 9, 32), (8, 8, 260, 600, 9, 128)])
+def test_queries_without_a_key_have_no_part_in_a_gradient(af3, H, Hkv, Lq, Lk, B, D, dtype):
+    D = D if dtype == BF16 else min(D, 64)
+    q, k, v, lam, _, g = diff_inputs(B, H, Hkv, Lq, Lk, D, 2 * D, dtype, 46)
+    padded = torch.ones(B, Lk, dtype=torch.bool, device="cuda")
+    padded[0, :6] = False
+    padded[-1, :3] = False
+    for m, kw, dead in ((None, dict(causal=True, q_offset=-5), [5] * B), (padded, dict(causal=True), [6] + [0] * (B - 2) + [3])):
+        gone = (torch.arange(Lq)[None] < torch.tensor(dead)[:, None]).cuda()[:, None, :, None]
+        clean = diff_run(af3, q, k, v, lam, m, g, **kw)
+        diff_compare(clean, q, k, v, lam, m, g, **kw)
+        for worst in (math.nan, math.inf):
+            dirty = diff_run(af3, q.masked_fill(gone, worst), k, v, lam, m, g.masked_fill(gone, worst), **kw)
+            for name in clean:
+                assert torch.equal(clean[name], dirty[name]), (name, worst)
+            assert (dirty["dq"].masked_select(gone) == 0).all() and (dirty["out"].masked_select(gone) == 0).all()
