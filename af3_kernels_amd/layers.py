@@ -281,9 +281,11 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
         raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
     dtype = q.dtype
     q, k, v = _inner_contig(q), _inner_contig(k if k.dtype == dtype else k.to(dtype)), _inner_contig(v if v.dtype == dtype else v.to(dtype))
-    if lam.dtype not in (dtype, torch.float32):
+    shared = tuple(lam.shape) != (H,)
+    # (one number for all heads: its gradient is rounded once, behind their sum)
+    if lam.dtype not in (dtype, torch.float32) or (shared and lam.dtype != torch.float32 and lam.requires_grad and torch.is_grad_enabled()):
         lam = lam.to(torch.float32)
-    lam = lam.reshape(1).expand(H) if tuple(lam.shape) != (H,) else lam
+    lam = lam.reshape(1).expand(H) if shared else lam
     graph = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam))
     if graph and B * Hkv * -(-Lk // 32) >= 1 << 24:
         raise ValueError(f"gradients take B * Hkv * ceil(Lk / 32) below 2^24, got {B} * {Hkv} * ceil({Lk} / 32)")

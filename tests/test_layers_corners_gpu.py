@@ -152,3 +152,19 @@ def test_queries_without_a_key_have_no_part_in_a_gradient(af3, H, Hkv, Lq, Lk, B
             for name in clean:
                 assert torch.equal(clean[name], dirty[name]), (name, worst)
             assert (dirty["dq"].masked_select(gone) == 0).all() and (dirty["out"].masked_select(gone) == 0).all()
+
+
+# ---- one lam for all heads ----------------------------------------------------------------------------------------------------
+@HOSTS
+def test_one_lam_of_few_bits_for_all_heads(af3, host, native):
+    """Its gradient is a sum over heads, and rounded once."""
+    host(native)
+    for seed in range(16):
+        q, k, v, lam, m, g = diff_inputs(2, 8, 4, 30, 40, 32, 64, BF16, 47 + seed, "random")
+        for form in (lam[:1], lam[0]):
+            few = form.detach().to(BF16).requires_grad_(True)
+            more = few.detach().float().requires_grad_(True)
+            a, b = (af3.differential_attention(q, k, v, x, m) for x in (few, more))
+            assert torch.equal(a, b)
+            a, b = torch.autograd.grad(a, few, g)[0], torch.autograd.grad(b, more, g)[0]
+            assert a.dtype == BF16 and torch.equal(a, b.to(BF16))
