@@ -68,7 +68,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
             return n * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
         low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), n - 1)
         for i, f in enumerate(frequencies):
-            slowed = min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0)
+            slowed = min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0) if original_length * f >= beta_slow * 2.0 * math.pi else 1.0   # (within a few tokens not even pair 0 turns so often)
             frequencies[i] = f / factor * slowed + f * (1.0 - slowed)
         scale = 0.1 * math.log(factor) + 1.0
     return torch.tensor(frequencies, dtype=torch.float64, device=device), scale
