@@ -149,19 +149,19 @@ struct tile {
 
 // ROWS rows on their way from memory into a tile, spread over the workgroup's threads in 16-byte pieces.  The plain way (rows all there, D a whole number of pieces,
 // 32-bit offsets within the tile) is one load per piece at a scalar base and an offset that stays the same from tile to tile.
-template <typename T, int DP, int ROWS, int NT = THREADS>   // NT: threads of the workgroup
+template <typename T, int DP, int ROWS>
 struct passage {
 	using TL = tile<T, DP>;
-	static constexpr int N = ROWS * TL::CHUNKS / NT, E = kind<T>::E;
-	static_assert(N * NT == ROWS * TL::CHUNKS);
+	static constexpr int N = ROWS * TL::CHUNKS / THREADS, E = kind<T>::E;
+	static_assert(N * THREADS == ROWS * TL::CHUNKS);
 	u32x4    piece[N];
 	uint32_t offset[N];   // bytes from the tile's first row
 	const T* base;
 	int64_t  stride;
 	int      D;
 	bool     plain;
-	static __device__ __forceinline__ int row_of(int n) { return (threadIdx.x + NT * n) / TL::CHUNKS; }
-	static __device__ __forceinline__ int col_of(int n) { return (threadIdx.x + NT * n) % TL::CHUNKS; }
+	static __device__ __forceinline__ int row_of(int n) { return (threadIdx.x + THREADS * n) / TL::CHUNKS; }
+	static __device__ __forceinline__ int col_of(int n) { return (threadIdx.x + THREADS * n) % TL::CHUNKS; }
 	__device__ __forceinline__ void begin(const T* base_, int64_t stride_, int D_, bool whole) {
 		base = base_, stride = stride_, D = D_;
 		plain = whole && stride_ <= (int64_t)0x7fffffff / ((int64_t)ROWS * (int)sizeof(T));

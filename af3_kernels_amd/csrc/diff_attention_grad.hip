@@ -104,10 +104,10 @@ __global__ void __launch_bounds__(THREADS) diff_delta_kernel(grad_args a) {
 	if(lane == 0) a.d1[row] = __builtin_fmaf(lam_of(p, h), d2, d1), a.d2[row] = d2;
 }
 
-// How many rows a tile has, and how many threads and maps of a wavefront the kernels have, by the bytes of a row of q or k (of 32, 64 or 128 columns).
+// How many rows a tile has, how many maps a wavefront and how many threads the kernels, by the bytes of a row of q or k (of 32, 64 or 128 columns).
 constexpr int tile_rows(int bytes, int sharing) { return sharing == 4 || bytes <= 64 ? 128 : bytes <= 128 ? 64 : 32; }
 constexpr int dq_maps(int bytes) { return bytes <= 128 ? 2 : 1; }
-constexpr int dq_threads(int bytes) { return 512; }
+constexpr int DQ_THREADS = 512;
 // dK and dV of 128-byte rows: both maps in a wavefront need 370 registers, one wavefront to a SIMD; with one map each, and dP computed by both, there are two (2 x 16 (4) x 4096 x 64
 // causal 761 -> 579 us, in workgroups of 256 threads 776; 540 with the tiles dealt out longest first).  Where wavefronts share their keys the pairs' exchange would be between twice as many.
 constexpr int dkv_maps(int bytes, int sharing) { return bytes <= 64 || sharing > 1 ? 2 : 1; }
@@ -117,7 +117,7 @@ constexpr int dkv_threads(int bytes, int sharing) { return bytes == 128 && shari
 // KW: wavefronts that share 32 rows and each take 32 keys of a tile; MAPS: maps of a wavefront, 2, or 1 with the other map beside it in another one
 template <typename T, int DP, int KW>
 struct dq_shape {
-	static constexpr int BYTES = DP * (int)sizeof(T), MAPS = dq_maps(BYTES), NT = dq_threads(BYTES), W = NT / 64, GROUPS = W * MAPS / 2 / KW;
+	static constexpr int BYTES = DP * (int)sizeof(T), MAPS = dq_maps(BYTES), NT = DQ_THREADS, W = NT / 64, GROUPS = W * MAPS / 2 / KW;
 	static constexpr int DV = 2 * DP, KT = tile_rows(BYTES, KW), SUB = KT / (32 * KW), ROWS = 32 * GROUPS;
 	static constexpr int KTILE = KT * tile<T, DP>::STRIDE, VTILE = KT * tile<T, DV>::STRIDE, SET = 2 * KTILE + VTILE;
 	static constexpr int BUFFERS = 2 * SET <= 65536 ? 2 : 1;
@@ -653,7 +653,7 @@ cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double cou
 }
 cut dq_cut(const af3_diff_attention_params& p) {
 	const int bytes = row_bytes(p);
-	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, 32 * dq_threads(bytes) / 64 * dq_maps(bytes) / 2, bytes, counting(p), 256, 0.4 + 0.009 * bytes, [&](int) { return (0.4 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0); },
+	cut c = cut_for(p.H / p.Hkv * p.Lq, p.B * p.Hkv, 32 * DQ_THREADS / 64 * dq_maps(bytes) / 2, bytes, counting(p), 256, 0.4 + 0.009 * bytes, [&](int) { return (0.4 + 0.009 * bytes) * (p.dtype == AF3_F32 ? 2.0 : 1.0); },
 					8.0 * p.B * p.H * p.Lq * p.D, [&](int sharing) { return over(p.Lk, tile_rows(bytes, sharing)); });
 	c.part *= tile_rows(bytes, c.sharing);
 	return c;
