@@ -4,8 +4,8 @@
 // Per 32 query rows and 32 keys and map:  S^T[key][row] = K . Q^T,  O^T[column][row] += V^T . P^T,  as in cross_attention.hip: a lane holds one query row, the half-waves 16
 // keys each.  The two maps are different wavefronts' (both maps' sums of twice D columns would leave one wavefront to a SIMD), which share the tiles of V; each keeps its own
 // running maximum and sum, and the difference is taken at the end, since neither sum is known before.
-// Bound by its vector and matrix instructions, which take turns, and by waits of wavefronts that share tiles: 2 x 16 (4) x 4096 x 64 causal 285 us, 725 TFLOP/s (a large product of the
-// library: 1306); 4 x 8 x 1024 x 128 85 us, 610.  Workgroups of 4 wavefronts, two to a compute unit, gain 7 % where a launch is short (68 us for 73 at 4 x 12 x 1024 x 64 causal, dealt out pair by pair) and
+// Bound by its vector and matrix instructions, which take turns, and by waits of wavefronts that share tiles: 2 x 16 (4) x 4096 x 64 causal 284 us, 727 TFLOP/s (a large product of the
+// library: 1306); 4 x 8 x 1024 x 128 83 us, 620.  Workgroups of 4 wavefronts, two to a compute unit, gain 7 % where a launch is short (68 us for 73 at 4 x 12 x 1024 x 64 causal, dealt out pair by pair) and
 // lose up to 40 % (128 columns).
 #include "diff_tiles.hpp"
 
@@ -806,7 +806,9 @@ plan forward_plan(const af3_diff_attention_params& p) {
 	f.kw = rows <= 32 || busy(4) <= slots ? 4 : rows <= 64 || busy(2) <= slots ? 2 : 1;
 	if(f.kw > most_sharing(p)) f.kw = most_sharing(p);
 	f.row_tiles = (uint32_t)(busy(f.kw) / groups);
-	// (V's way through memory and back is worth it where many rows read it: from four tiles of them on)
+	// (V's way through memory and back is worth it where many rows read it: from four tiles of them on.  Without and with it, 128 pairs (four tiles: 128, two and three: 256) of D = 64, over 256,
+	// 1024 and 4096 keys: two tiles 39 and 44, 104 and 106, 375 and 373 us; three 52 and 55, 143 and 136, 545 and 500; four 35 and 39, 96 and 90, 359 and 313; eight 66 and 64, 186 and 160, 694
+	// and 565.  D = 128, four: 68 and 71, 178 and 171, 659 and 591.)
 	f.half = !fp32 && f.kw == 1 && f.row_tiles >= 4 && groups * value_tiles(p) <= 0xffffff;
 	const int64_t kt = tile_keys(wide * (fp32 ? 4 : 2), f.kw), key_tiles = (p.Lk + kt - 1) / kt;
 	const double  tile_us = (0.4 + 0.033 * wide) * (f.kw == 4 ? 1.0 : 0.6) * (fp32 ? 3.0 : 1.0);

@@ -636,7 +636,9 @@ double counting(const af3_diff_attention_params& p) {
 template <typename U, typename F>
 cut cut_for(int64_t length, int64_t groups, int64_t alone, int bytes, double counts, int64_t slots, double load_us, U block_us, double part_bytes, F steps) {
 	constexpr double JOIN_US = 6.0, BYTES_PER_US = 2e6;
-	const double tail = counts < 1.0 && by_tile(groups) ? 0.5 : 0.8;   // of the longest, behind all of them dealt out evenly (8 x 16 x 768 x 64 causal, dQ: 117 us with 0.8 for both, 90)
+	const double tail = counts < 1.0 && by_tile(groups) ? 0.5 : 0.8;   // of the longest, behind all of them dealt out evenly
+	// (8 x 16 x 768 x 64 causal, dQ: 117 us with 0.8 for both, 90.  Forward and all gradients with 0.8 and with 0.5, n causal pairs x length x 64: 8 x 1491 175 and 147; 16 x 768 126 and 121, x 1491 223 and
+	// 232; 48 x 400 95 and 115, x 1024 195 and 189, x 1491 350 and 327; 128 x 400 136 and 155, x 768 307 and 266, x 1491 760 both.  Not causal: no difference in 20 sizes.)
 	cut    best{};
 	double best_us = 0.0;
 	for(int sharing = 1; sharing <= (bytes > 128 ? 1 : 4); sharing *= 2) {

@@ -26,7 +26,9 @@ __device__ __forceinline__ float lam_of(const af3_diff_attention_params& p, int6
 // Which pair, tile (the longest first) and part a workgroup works on.  Where all are alike: as `share` has it, pair after pair.  Where some tiles are longer (causal): tile after tile over all
 // pairs, so that a launch begins with the longest tiles of every pair and not of the first few.  4 x 12 x 1024 x 64: forward 71 us and so 55, dK and dV 107 and 78; 8 x 16 x 2048 x 64, whose
 // pairs' keys are four times an XCD's L2 by then: 405 and 340, 696 and 576.  Pairs that do not come in eights go over the XCDs as they come, and their parts one after the other (2 x 14 x
-// 1491 x 64: 84 and 65, 129 and 99); fewer than eight gain nothing by it (fp32, 4 pairs of 1024 x 32: 91 and 108).
+// 1491 x 64: 84 and 65, 129 and 99).  Either side of the border, forward and all gradients, n pairs of 1024 x 64 and of 2048 x 64 pair after pair and tile after tile: 4: 97 and 97, 157 and
+// 156 us; 6: 110 and 110, 199 and 180; 9: 142 and 128, 257 and 240; 12: 148 and 140, 285 and 296; 15: 153 and 158, 289 and 297; 24: 167 and 184, 380 and 298; 32: 173 and 174, 466 and 353 (fp32, 4
+// pairs of 1024 x 32: 91 and 108).
 __host__ __device__ constexpr bool by_tile(int64_t pairs) { return pairs % 8 == 0 || pairs > 8; }
 struct dealt {
 	uint32_t pair, tile, split;

@@ -2,11 +2,12 @@
 //     z = post_norm(y) post_weight,   r = residual_scale x + act(gate) z,   h = norm(r) weight + bias.
 // af3_residual_norm_forward / _backward.
 //
-// Both directions are bound by their bytes: a row is read once, held in registers through its reductions (64 to 1024 threads to a row, 8 or 16 channels each) and
-// written once.  The gradient works r out again from x, y and the gate, unrounded as the forward pass had it, with the two norms' statistics from there.  What many
+// A row is read once, held in registers through its reductions (64 to 1024 threads to a row, 8 or 16 channels each) and written once: the forward pass is bound by its bytes, the gradient by its
+// vector instructions and by what its rows wait for at the norms' sums.  The gradient works r out again from x, y and the gate, unrounded as the forward pass had it, with the two norms' statistics from there.  What many
 // rows share (a weight by channel, a gate by sequence) has its gradient summed in registers over the rows of a workgroup; workgroups' sums are joined by a second kernel in
 // a fixed order.
-// 4 x 2048 rows of 4096 channels in bf16, all of it: 165 us for 108 that a copy of the same bytes takes, each read and written once; the gradient reads x and y again.  Rows of more than
+// 4 x 2048 rows of 4096 channels in bf16, all of it: 165 us for 109 that a copy of the same bytes takes, each read and written once (the gradient reads x and y again); the forward pass 49 of them,
+// 268 MB, 5.5 TB/s, the gradient 107, 428 MB, 4.0 TB/s.  Rows of more than
 // 8192 channels spill in the gradient's kernel, whose 1024 threads have 128 registers each.
 #include "launch_grid.hpp"
 #include "mfma_helpers.hpp"
@@ -314,7 +315,8 @@ __global__ void __launch_bounds__(threads_for(TPR)) backward_kernel(args a) {
 	if constexpr(SUMS) clear(GATE), clear(WEIGHT), clear(BIAS), clear(POST);
 
 	// What a row needs comes in one go, a row ahead of its use where the registers hold two of them; what rows share stays in registers.  4 x 2048 rows of 4096 channels in bf16:
-	// 107 us (5.1 TB/s); with 16 channels a thread, everything loaded where it is used, 210; 8 x 768 conditioned rows of 768 channels 29 us, that way 54.
+	// 107 us (six tensors of 67 MB and 25 of workgroups' sums: 4.0 TB/s); with 16 channels a thread, everything loaded where it is used, 210; 8 x 768 conditioned rows of 768 channels 29 us
+	// (104 MB: 3.6 TB/s), that way 54.  Vector instructions take 67 % of the SIMDs' clocks and wavefronts wait 39 % of theirs: two to a SIMD, one row at a time, a barrier for each norm's sums.
 	constexpr bool AHEAD = TPR * NP <= 1024;
 	struct streams {
 		eight<T> y[NP], x[NP], out[NP], normed[NP], gate[NP], weight[NP];

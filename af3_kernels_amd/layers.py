@@ -419,6 +419,7 @@ def residual_norm(x: Optional[torch.Tensor], y: torch.Tensor, weight: Optional[t
     gate, weight and bias are [C], or have y's number of axes with 1 where they are repeated: [B, 1, C] for all tokens of a sequence, [B, T, C] for
     every token (a conditioned transformer's), [C] for all.  post_weight [C].  One left out counts as ones (a bias as zeros).  float32 or bfloat16, everything else cast to y's
     dtype; arithmetic in fp32, out and normed rounded once each (normed is made of out before its rounding).  C up to 16384; x, y: any strides.  New contiguous tensors.
+    (A parameter that is repeated along an axis in front of one that it is not repeated along, [1, T, C], goes as one with a row for every token: torch adds those rows' gradients up, rounded to y's dtype.)
 
     Gradients flow to all tensors (the same bits every time); a second derivative and forward mode raise.  In a HIP graph: as cross_attention."""
     kinds = _lib.NORMS.get(norm, -1), _lib.NORMS.get(post_norm, -1), gate_activation == "sigmoid"

@@ -449,8 +449,9 @@ int64_t af3_position_bias_workspace_bytes(const af3_position_bias_params* params
  *                 reaches a result.
  *   causal      : key j counts for query i if j <= i + q_offset.  (A key that counts for some queries of the call has weight zero for the others: NaN and infinities
  *                 of its v reach those too.)
- *                 A query that is left without a key by mask and causality yields zeros, and has no part in a gradient.
- *   dtype       : AF3_BF16 (bf16 products, fp32 accumulation and softmax) or AF3_F32 (fp32 throughout), of q, k, v, out.
+ *                 A query that is left without a key by mask and causality yields zeros, and has no part in a gradient, whatever lam, its own q and grad_out, or v at other queries' keys hold.
+ *   dtype       : AF3_BF16 (bf16 products, fp32 accumulation and softmax) or AF3_F32 (fp32 throughout), of q, k, v, out.  In long AF3_BF16 calls the probabilities and v go as fp16, v in
+ *                 units of its tile of 64 or 128 keys: values below 2^-25 of the tile's largest are rounded, by 2^-33 of it at most.
  *   stats, second : optional, both or neither, for af3_diff_attention_backward: [B, 2 H, Lq, 2] floats (maximum in the softmax's units and 1 / sum) and
  *                 [B, H, Lq, Dv] contiguous of `dtype` (the second map's own result).
  *   residuals   : with them, AF3_BF16 only: [2, B, H, Lq, Dv] contiguous, what out and second lost by their rounding, as bf16.  Given to af3_diff_attention_backward too, the row

@@ -168,3 +168,16 @@ def test_one_lam_of_few_bits_for_all_heads(af3, host, native):
             assert torch.equal(a, b)
             a, b = torch.autograd.grad(a, few, g)[0], torch.autograd.grad(b, more, g)[0]
             assert a.dtype == BF16 and torch.equal(a, b.to(BF16))
+
+
+# ---- many queries of few keys -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D,Dv", [(64, 128), (32, 1), (24, 64), (128, 7)])
+@pytest.mark.parametrize("Lk", [1, 2, 15, 63, 64, 65, 127, 130])
+def test_many_queries_of_few_keys(af3, Lk, D, Dv):
+    """Long calls whose keys do not fill a tile, with masks that leave a sequence empty or hold back most of its keys."""
+    for seed, mask in ((51, "none"), (52, "empty"), (53, "one")):
+        t = diff_inputs(9, 8, 8, 530, Lk, D, Dv, BF16, seed, mask)
+        for unit in (1.0, 2.0 ** -13):
+            few = (t[0], t[1], (t[2] * unit).to(BF16), *t[3:])
+            diff_compare({"out": af3.differential_attention(*few[:5])}, *few)
+    diff_compare(diff_run(af3, *t, causal=True, q_offset=-3), *t, causal=True, q_offset=-3)
