@@ -289,16 +289,17 @@ template <typename T, int QT>
 struct row_stats {
 	static constexpr int BYTES = ROW_STATS * QT * 4 + 16;
 	float v[ROW_STATS];   // of one row, on its way
-	__device__ __forceinline__ void load(const grad_args& a, int64_t bh, int q0, int skip) {   // bh: b * H + h; rows in front of `skip` are as those that do not exist
+	// bh: b * H + h; rows are counted from `shift` on, `rows` of them
+	__device__ __forceinline__ void load(const grad_args& a, int64_t bh, int q0, int shift, int rows) {
 #pragma unroll
 		for(int i = 0; i < ROW_STATS; i++) v[i] = 0.f;
 		const int qi = q0 + (int)threadIdx.x;
-		if((int)threadIdx.x >= QT || qi >= (int)a.p.Lq || qi < skip) return;
-		const int64_t first = bh * a.p.Lq;
+		if((int)threadIdx.x >= QT || qi >= rows) return;
+		const int64_t first = bh * a.p.Lq + shift;
 		v[LESS] = a.d1[first + qi], v[LESS + 1] = a.d2[first + qi];
 #pragma unroll
 		for(int i = 0; i < 2; i++) {
-			const float* const st = a.p.stats + 4 * first + 2 * i * a.p.Lq + 2 * qi;
+			const float* const st = a.p.stats + 2 * (first + bh * a.p.Lq) + 2 * i * a.p.Lq + 2 * qi;
 			v[MOST + i] = st[0], v[INVERSE + i] = st[1];
 		}
 	}
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 	const af3_diff_attention_params& p = a.p;
 	constexpr int NONE = 1 << 30;
 	extern __shared__ __align__(16) unsigned char smem[];
-	__shared__ int first_live[S::W];   // the wavefronts' first keys that count, from key0 on
+	__shared__ int first_live[S::W];   // of the wavefronts
 
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
 	const int map0 = MAPS == 2 ? 0 : wave & 1, in_group = MAPS == 2 ? wave : wave >> 1, rwave = in_group % RW, group = in_group / RW;   // (map0: the wavefront's first map)
@@ -371,7 +372,6 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 	load_rows<T, S::DV>(vf, static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[1] + (in ? key : 0) * p.v_stride[2], in, a.v_columns, lane);
 	const uint64_t living = __ballot(lives);
 	const bool     work = living != 0;   // (of this wavefront)
-	if(lane == 0) first_live[wave] = work ? 32 * group + __builtin_ctzll(living) : NONE;
 
 	f32x16 dk[MAPS][TK::BLOCKS], dv[S::VBLOCKS];
 	const int vblock0 = MAPS == 2 ? 0 : map0 * S::VBLOCKS;   // the wavefront's first block of dV's columns
@@ -383,16 +383,20 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 	for(int db = 0; db < S::VBLOCKS; db++) dv[db] = f32x16{};
 
 	// Tiles of query rows, head after head: tile `at` of head `head` of the group, counted head * q_tiles + at (below 2^25).
-	const int q_tiles = (int)((p.Lq + QT - 1) / QT), n = (int)G * q_tiles, Lq = (int)p.Lq;
+	const int q_tiles = (int)((p.Lq + QT - 1) / QT), n = (int)G * q_tiles;
+	if(lane == 0) first_live[wave] = work ? 32 * group + __builtin_ctzll(living) : NONE;
 	__syncthreads();
-	int first = NONE;
+	int first = first_live[lane % S::W];   // the workgroup's first key that counts, from key0 on
 #pragma unroll
-	for(int w = 0; w < S::W; w++) first = first < first_live[w] ? first : first_live[w];
+	for(int d = S::W / 2; d; d >>= 1) first = min(first, __shfl_xor(first, d));
 	first = __builtin_amdgcn_readfirstlane(first);
-	// Causal: queries in front of the workgroup's first key that counts have nothing of its keys.  Those of them that share a tile with others become zeros: queries without a key are
-	// among them, which have no part in a gradient, and whatever stands there would meet weights of zero, which NaN does not heed.
+	// Causal: queries in front of the workgroup's first key that counts have nothing of its keys, and the tiles begin behind them: queries without a key are among them, which have no part
+	// in a gradient, and whatever stands there would meet weights of zero, which NaN does not heed.
 	const int64_t skipped = p.causal ? key0 + first - p.q_offset : 0;
-	const int     skip = skipped <= 0 ? 0 : skipped < Lq ? (int)skipped : Lq, from = skip == Lq ? q_tiles : skip / QT;
+	const int     skip = skipped <= 0 ? 0 : skipped < p.Lq ? (int)skipped : (int)p.Lq, from = skip / QT, shift = skip - from * QT;
+	// (rows are counted from `shift` on in what follows, so that tiles begin at whole numbers of them)
+	const int     Lq = (int)p.Lq - shift, tiles_end = skip == (int)p.Lq ? from : (Lq + QT - 1) / QT;
+	const int64_t q_offset = p.q_offset + shift;
 	const int last = (int)((int64_t)(split + 1) * a.part < n ? (int64_t)(split + 1) * a.part : n);
 	const typename TK::reader at_q_(lane);
 	const typename TV::reader at_g_(lane);
@@ -401,19 +405,19 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 	pq[0].begin(p.q_stride[2], a.columns);
 	pg.begin(a.g.grad_out_stride[2], a.v_columns);
 	row_stats<T, QT> rs;
-	const T* const qb = static_cast<const T*>(p.q) + b * p.q_stride[0] + 2 * hk * G * p.q_stride[1];
-	const T* const gb = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + hk * G * a.g.grad_out_stride[1];
+	const T* const qb = static_cast<const T*>(p.q) + b * p.q_stride[0] + 2 * hk * G * p.q_stride[1] + shift * p.q_stride[2];
+	const T* const gb = static_cast<const T*>(a.g.grad_out) + b * a.g.grad_out_stride[0] + hk * G * a.g.grad_out_stride[1] + shift * a.g.grad_out_stride[2];
 	auto fetch = [&](int head, int at) {
 		const T* const q = qb + 2 * head * p.q_stride[1];
 		pq[0].load(q, at * QT, Lq), pq[1].load(q + p.q_stride[1], at * QT, Lq, pq[0]), pg.load(gb + head * a.g.grad_out_stride[1], at * QT, Lq);
-		rs.load(a, b * p.H + hk * G + head, at * QT, skip);
+		rs.load(a, b * p.H + hk * G + head, at * QT, shift, Lq);
 	};
 	int head = (int)((int64_t)split * a.part) / q_tiles, at = (int)((int64_t)split * a.part) - head * q_tiles;
 	if(at < from) at = from;
-	if(at >= q_tiles) head++, at = from;
+	if(at >= tiles_end) head++, at = from;
 	int buffer = 0;
 	// (a workgroup none of whose keys counts has nothing to read)
-	bool more = first != NONE && from < q_tiles && head * q_tiles + at < last;
+	bool more = first != NONE && from < tiles_end && head * q_tiles + at < last;
 	if(more) fetch(head, at);
 	while(more) {
 		unsigned char* const qs = smem + buffer * S::SET;
@@ -422,14 +426,12 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 		const int            q0 = at * QT, left = Lq - q0;
 		const float          lam = lam_of(p, hk * G + head);
 		if constexpr(S::BUFFERS == 1) __syncthreads();
-		const bool all = left >= QT && q0 >= skip;
-		auto       exists = [&](int r) { return r < left && q0 + r >= skip; };
-		pq[0].store(qs, all, exists);
-		pq[1].store(qs + S::QTILE, all, exists, a.columns);
-		pg.store(gs, all, exists);
+		pq[0].store(qs, left >= QT, [&](int r) { return r < left; });
+		pq[1].store(qs + S::QTILE, left >= QT, [&](int r) { return r < left; }, a.columns);
+		pg.store(gs, left >= QT, [&](int r) { return r < left; });
 		rs.store(st, a.factor);
 		__syncthreads();
-		if(++at == q_tiles) head++, at = from;
+		if(++at == tiles_end) head++, at = from;
 		more = head * q_tiles + at < last;
 		if(more) fetch(head, at);
 		const bool apart = rs.apart(st);
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__((dkv_shape<T, DP, RW>::NT), (dkv_shape<T, DP, 
 		for(int s = 0; s < S::SUB; s++) {
 			const int row0 = 32 * (rwave * S::SUB + s);
 			// the lane's rows need .. 15 of its 16 count
-			const int  need = p.causal ? clamped(key - p.q_offset - (q0 + row0 + 16 * half)) : -64;
+			const int  need = p.causal ? clamped(key - q_offset - (q0 + row0 + 16 * half)) : -64;
 			const bool met = work && row0 < left && __any(in && need <= 15);
 			if(met) {
 				const bool diagonal = __any(in && need > 0);
